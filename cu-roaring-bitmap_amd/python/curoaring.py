@@ -39,6 +39,7 @@ EXPORTS = [
     "cr_portable_size_in_bytes", "cr_portable_serialize", "cr_portable_deserialize",
     "cr_upload_batch", "cr_free_batch", "cr_promote_batch", "cr_batch_make_view", "cr_batch_multi_and",
     "cr_batch_decompress", "cr_batch_contains", "cr_batch_view_contains", "cr_debug_fail_device_allocs",
+    "cr_paged_plan", "cr_paged_append", "cr_paged_select", "cr_paged_attention", "cr_beam_select", "cr_beam_reorder",
 ]
 
 
@@ -119,6 +120,25 @@ class Meta(C.Structure):
                 ("universe_size", C.c_uint32), ("total_bytes", C.c_size_t)]
 
 
+class PagedCache(C.Structure):
+    """cr_paged_cache (include/cu_roaring_abi.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [
+        (x, C.c_uint64) for x in ("k_page_stride", "k_slot_stride", "k_head_stride", "v_page_stride", "v_slot_stride",
+                                  "v_head_stride")] + [
+        (x, C.c_uint32) for x in ("n_pages", "page_size", "n_heads", "head_dim", "dtype")]
+
+
+class PagedAttentionArgs(C.Structure):
+    """cr_paged_attention_args (include/cu_roaring_abi.h)."""
+    _fields_ = [("q", C.c_void_p), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+                ("out", C.c_void_p), ("out_token_stride", C.c_uint64), ("out_head_stride", C.c_uint64),
+                ("lse", C.c_void_p), ("n_tokens", C.c_uint32), ("n_heads", C.c_uint32), ("n_requests", C.c_uint32),
+                ("d_starts", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_table", C.c_void_p),
+                ("table_cols", C.c_uint32), ("table_stride", C.c_uint64), ("d_sel", C.c_void_p),
+                ("sel_stride", C.c_uint64), ("d_sel_len", C.c_void_p), ("d_limits", C.c_void_p),
+                ("scale", C.c_float), ("causal", C.c_uint32), ("max_new", C.c_uint32), ("max_kv", C.c_uint32)]
+
+
 assert C.sizeof(GpuRoaring) == 120 and C.sizeof(GpuRoaringView) == 80
 
 _lib = None
@@ -190,6 +210,20 @@ def load(path: Optional[str] = None):
         "cr_batch_contains": [P(RoaringBatch), C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p],
         "cr_batch_view_contains": [P(BatchView), C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p],
         "cr_debug_fail_device_allocs": [C.c_uint32, C.c_uint32],
+        "cr_paged_plan": [P(GpuRoaring), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
+                          C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                          C.c_uint32, C.c_void_p, C.c_void_p],
+        "cr_paged_append": [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32,
+                            C.c_void_p, P(PagedCache), C.c_void_p],
+        "cr_paged_select": [P(GpuRoaring), C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint64, C.c_void_p,
+                            C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                            C.c_void_p],
+        "cr_paged_attention": [P(PagedAttentionArgs), P(PagedCache), C.c_void_p],
+        "cr_beam_select": [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64,
+                           C.c_void_p, C.c_void_p, P(GpuRoaring), C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
+                           C.c_void_p, C.c_void_p, C.c_void_p],
+        "cr_beam_reorder": [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64,
+                            C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p],
     }
     for name, args in sigs.items():
         f = getattr(L, name)
@@ -506,6 +540,183 @@ def download_batch(b: RoaringBatch) -> SimpleNamespace:
         host_container_starts=hcs, host_key_index_starts=hks,
         host_n_bitmap_containers=h(b.host_n_bitmap_containers, n).astype(np.uint32) if n else np.zeros(0, np.uint32),
     )
+
+
+# ---- serving language models (stream-ordered, no synchronisation) ---------------
+F32, F16, BF16 = 0, 1, 2
+_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _typed(t, *types: str) -> int:
+    """The library's code of a tensor's type, one of `types` (all of them if none is named)."""
+    name = str(t.dtype)
+    if name not in _TYPES or (types and name not in types):
+        raise CrError(CR_ERR_INVALID, f"a tensor of {name} where one of {', '.join(types or _TYPES)} is taken")
+    return _TYPES[name]
+
+
+def _array(t, name: str, dtype: str, shape) -> int:
+    """The address of a contiguous CUDA tensor of this type and shape (None: any extent)."""
+    if (str(t.dtype) != "torch." + dtype or not t.is_cuda or not t.is_contiguous() or len(shape) != t.dim()
+            or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+        raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} CUDA tensor of shape "
+                                      f"{tuple('*' if n is None else n for n in shape)} is taken, not "
+                                      f"{t.dtype} {tuple(t.shape)}")
+    return _dptr(t)
+
+
+def _table(t, n_requests: int):
+    """(address, columns, row stride) of a block table, rows of which may lie apart."""
+    if str(t.dtype) != "torch.int32" or not t.is_cuda or t.dim() != 2 or t.shape[0] != n_requests or (
+            t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
+        raise CrError(CR_ERR_INVALID, f"block table: an int32 CUDA tensor of {n_requests} rows is taken")
+    return _dptr(t), t.shape[1], t.stride(0)
+
+
+def _rows(t, name: str, like):
+    """(address, token stride, head stride) of a [tokens, heads, dim] tensor of `like`'s shape and type."""
+    if t.dtype != like.dtype or not t.is_cuda or t.shape != like.shape or t.dim() != 3 or (
+            t.shape[2] > 1 and t.stride(2) != 1):
+        raise CrError(CR_ERR_INVALID, f"{name}: a {like.dtype} CUDA tensor of shape {tuple(like.shape)} with "
+                                      f"contiguous rows is taken, not {t.dtype} {tuple(t.shape)}")
+    return _dptr(t), t.stride(0), t.stride(1)
+
+
+def paged_cache(d_k, d_v) -> PagedCache:
+    """A cache of [pages, page size, heads, dim] keys and values (any strides with contiguous rows)."""
+    if d_k.dim() != 4 or d_k.shape != d_v.shape or d_k.dtype != d_v.dtype or not (d_k.is_cuda and d_v.is_cuda) or (
+            d_k.shape[3] > 1 and (d_k.stride(3) != 1 or d_v.stride(3) != 1)):
+        raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] "
+                                      "with contiguous rows are taken")
+    pages, size, heads, dim = d_k.shape
+    return PagedCache(_dptr(d_k), _dptr(d_v), d_k.stride(0), d_k.stride(1), d_k.stride(2), d_v.stride(0),
+                      d_v.stride(1), d_v.stride(2), pages, size, heads, dim, _typed(d_k))
+
+
+def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d_new, d_table, d_slots, d_starts,
+               d_kv_len, d_taken, d_counts, stream=None):
+    """Block tables and slot maps from the requests' lengths (cr_paged_plan).
+
+    d_cached, d_new: int32 [R], tokens in the cache and new ones.  d_table: int32 [R, cols], completed in place with
+    pages from `free_pages`.  Written: d_slots int64 [at least the new tokens], d_starts int32 [R + 1], d_kv_len
+    int32 [R], d_taken int32 [any], d_counts int32 [3]: new tokens, pages taken, pages missing."""
+    n = d_cached.numel()
+    table, cols, stride = _table(d_table, n)
+    _check(load().cr_paged_plan(C.byref(free_pages), n_pages, page_size, _array(d_cached, "cached", "int32", (n,)),
+                                _array(d_new, "new", "int32", (n,)), n, table, cols, stride,
+                                _array(d_slots, "slots", "int64", (None,)), d_slots.numel(),
+                                _array(d_starts, "starts", "int32", (n + 1,)),
+                                _array(d_kv_len, "kv_len", "int32", (n,)),
+                                _array(d_taken, "taken", "int32", (None,)), d_taken.numel(),
+                                _array(d_counts, "counts", "int32", (3,)), _stream(stream)), "paged_plan")
+
+
+def paged_append(d_k, d_v, d_slots, d_k_cache, d_v_cache, stream=None):
+    """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out."""
+    cache = paged_cache(d_k_cache, d_v_cache)
+    if d_k.dim() != 3 or tuple(d_k.shape[1:]) != (cache.n_heads, cache.head_dim) or d_k.dtype != d_k_cache.dtype:
+        raise CrError(CR_ERR_INVALID, f"paged_append: {d_k_cache.dtype} keys [tokens, {cache.n_heads}, "
+                                      f"{cache.head_dim}] are taken, not {d_k.dtype} {tuple(d_k.shape)}")
+    k, k_token, k_head = _rows(d_k, "k", d_k)
+    v, v_token, v_head = _rows(d_v, "v", d_k)
+    n = d_k.shape[0]
+    _check(load().cr_paged_append(k, v, k_token, k_head, v_token, v_head, n,
+                                  _array(d_slots, "slots", "int64", (n,)), C.byref(cache), _stream(stream)),
+           "paged_append")
+
+
+def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: int, d_sel, d_sel_len, d_limits,
+                 n_pages: Optional[int] = None, stream=None):
+    """The slots of each request that the bitmap `visible` holds, listed once for every layer's attention.
+
+    Written: d_sel int32 [R, at least cols * page_size], d_sel_len int32 [R], d_limits int32 [T].  n_pages: the
+    cache's (default: as many as the bitmap's universe holds)."""
+    n = d_kv_len.numel()
+    table, cols, stride = _table(d_table, n)
+    sel, room, sel_stride = _table(d_sel, n)
+    if room < cols * page_size:
+        raise CrError(CR_ERR_INVALID, f"paged_select: a row of sel holds cols * page_size = {cols * page_size} slots")
+    if n_pages is None:
+        n_pages = visible.universe_size // page_size
+    _check(load().cr_paged_select(C.byref(visible), n_pages, page_size, table, cols, stride,
+                                  _array(d_starts, "starts", "int32", (n + 1,)),
+                                  _array(d_kv_len, "kv_len", "int32", (n,)), n, d_limits.numel(), sel, sel_stride,
+                                  _array(d_sel_len, "sel_len", "int32", (n,)),
+                                  _array(d_limits, "limits", "int32", (None,)), _stream(stream)), "paged_select")
+
+
+def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_out, scale: Optional[float] = None,
+                    causal: bool = True, d_lse=None, selection=None, max_new: int = 0, max_kv: int = 0, stream=None):
+    """Attention of the requests' new tokens q [T, heads, dim] over the paged cache into d_out (cr_paged_attention).
+
+    Request r's tokens are [starts[r], starts[r + 1]), the last of its kv_len[r] positions.  scale: 1 / sqrt(dim) by
+    default.  d_lse: float32 [T, heads] or None.  selection: paged_select's (sel, sel_len, limits) or None.  max_new
+    and max_kv: the most new tokens and keys of a request if known; they choose how the work is split."""
+    cache = paged_cache(d_k_cache, d_v_cache)
+    if d_q.dim() != 3 or d_q.dtype != d_k_cache.dtype or d_q.shape[2] != cache.head_dim:
+        raise CrError(CR_ERR_INVALID, f"paged_attention: {d_k_cache.dtype} queries [tokens, heads, {cache.head_dim}] "
+                                      f"are taken, not {d_q.dtype} {tuple(d_q.shape)}")
+    n, (tokens, heads, dim) = d_kv_len.numel(), d_q.shape
+    a = PagedAttentionArgs()
+    a.q, a.q_token_stride, a.q_head_stride = _rows(d_q, "q", d_q)
+    a.out, a.out_token_stride, a.out_head_stride = _rows(d_out, "out", d_q)
+    a.lse = _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else None
+    a.n_tokens, a.n_heads, a.n_requests = tokens, heads, n
+    a.d_starts = _array(d_starts, "starts", "int32", (n + 1,))
+    a.d_kv_len = _array(d_kv_len, "kv_len", "int32", (n,))
+    a.d_table, a.table_cols, a.table_stride = _table(d_table, n)
+    if selection is not None:
+        sel, sel_len, limits = selection
+        a.d_sel, room, a.sel_stride = _table(sel, n)
+        if room < a.table_cols * cache.page_size:
+            raise CrError(CR_ERR_INVALID, "paged_attention: a row of sel holds cols * page_size slots")
+        a.d_sel_len = _array(sel_len, "sel_len", "int32", (n,))
+        a.d_limits = _array(limits, "limits", "int32", (tokens,))
+    a.scale = dim ** -0.5 if scale is None else scale
+    a.causal, a.max_new, a.max_kv = causal, max_new, max_kv
+    _check(load().cr_paged_attention(C.byref(a), C.byref(cache), _stream(stream)), "paged_attention")
+
+
+def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_lse=None, allowed=None, stream=None):
+    """The k best continuations of each answer's beams (cr_beam_select): k is the outputs' second extent.
+
+    d_scores: [B, W, V] with contiguous rows; d_cum, d_lse: float32 [B, W]; outputs: float32, int32, int32 [B, k].
+    allowed: a bitmap over [0, V), or int32 bitsets [ceil(V / 32)] (one for all) or [B, W, ceil(V / 32)], or None."""
+    b, w, v = d_scores.shape
+    k = d_out_scores.shape[1]
+    if not d_scores.is_cuda or (v > 1 and d_scores.stride(2) != 1):
+        raise CrError(CR_ERR_INVALID, "beam_select: a CUDA tensor of scores with contiguous rows is taken")
+    words, bits, stride = (v + 31) // 32, None, 0
+    if allowed is not None and not isinstance(allowed, GpuRoaring):
+        bits = _array(allowed, "allowed", "int32", (words,) if allowed.dim() == 1 else (b, w, words))
+        stride = 0 if allowed.dim() == 1 else words
+    _check(load().cr_beam_select(_dptr(d_scores), _typed(d_scores), b, w, v, d_scores.stride(0), d_scores.stride(1),
+                                 _array(d_cum, "cum", "float32", (b, w)),
+                                 _array(d_lse, "lse", "float32", (b, w)) if d_lse is not None else None,
+                                 C.byref(allowed) if isinstance(allowed, GpuRoaring) else None, bits, stride, k,
+                                 _array(d_out_scores, "out_scores", "float32", (b, k)),
+                                 _array(d_out_tokens, "out_tokens", "int32", (b, k)),
+                                 _array(d_out_parents, "out_parents", "int32", (b, k)), _stream(stream)),
+           "beam_select")
+
+
+def beam_reorder(d_src, d_parents, d_dst, d_len=None, stream=None):
+    """d_dst[b, i] = d_src[b, parents[b, i]] for states [B, W, ...] of any type (cr_beam_reorder).
+
+    d_len: int32 [B, W]: only the first d_len[b, parent] entries along the third extent move.  Rows without a parent
+    (-1) are left alone."""
+    b, w = d_src.shape[:2]
+    k = d_parents.shape[1]
+    if not (d_src.is_cuda and d_dst.is_cuda and d_src.is_contiguous() and d_dst.is_contiguous()) or (
+            d_src.dtype != d_dst.dtype or tuple(d_dst.shape) != (b, k) + tuple(d_src.shape[2:])):
+        raise CrError(CR_ERR_INVALID, f"beam_reorder: contiguous CUDA states [{b}, {w}, ...] into [{b}, {k}, ...]")
+    if d_len is not None and d_src.dim() < 3:
+        raise CrError(CR_ERR_INVALID, "beam_reorder: lengths count along the states' third extent")
+    row = d_src[0, 0].numel() * d_src.element_size() if b and w else 0
+    unit = row // max(1, d_src.shape[2]) if d_len is not None else 0
+    _check(load().cr_beam_reorder(_dptr(d_src), _array(d_parents, "parents", "int32", (b, k)), b, w, k, row, row, row,
+                                  _array(d_len, "len", "int32", (b, w)) if d_len is not None else None, unit,
+                                  _dptr(d_dst), _stream(stream)), "beam_reorder")
 
 
 def device_free(ptr):

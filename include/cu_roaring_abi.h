@@ -370,6 +370,120 @@ int cr_batch_contains(const cr_roaring_batch* batch, const uint32_t* d_bitmap_id
 int cr_batch_view_contains(const cr_batch_view* view, const uint32_t* d_ids, uint64_t n, uint8_t* d_out,
                            cr_stream_t stream);
 
+/* ---- serving language models (no reference counterpart) ---------------------
+ * A server keeps sets of ids next to its paged key/value cache: free pages,
+ * slots that a request may look at, tokens that an answer may use.  Here those
+ * sets are bitmaps.  These calls are stream-ordered and do NOT synchronise
+ * `stream`; lengths, tables and slots are device arrays, and whatever they hold,
+ * a call stays inside the buffers that its host arguments describe.  Arrays of
+ * one call must not overlap, unless said otherwise.  Strides count elements. */
+#define CR_F32 0
+#define CR_F16 1
+#define CR_BF16 2
+
+/* Keys and values of `n_pages` pages of `page_size` (a power of two) tokens:
+ * dimension d of head h of slot s of page p lies at
+ * k + p * k_page_stride + s * k_slot_stride + h * k_head_stride + d.
+ * A slot's number is p * page_size + s; there are at most 2^31 - 1 of them. */
+typedef struct cr_paged_cache {
+    void* k;
+    void* v;
+    uint64_t k_page_stride, k_slot_stride, k_head_stride;
+    uint64_t v_page_stride, v_slot_stride, v_head_stride;
+    uint32_t n_pages, page_size, n_heads, head_dim;
+    uint32_t dtype; /* CR_F32 (append only), CR_F16 or CR_BF16 */
+} cr_paged_cache;
+
+/* Block tables and slot maps.  Request r holds d_cached[r] tokens in the pages
+ * d_table[r * table_stride + 0 .. ceil(cached / page_size)) and gets d_new[r]
+ * more.  The pages that it lacks come from `free_pages` (a bitmap over
+ * [0, n_pages)), lowest id first, requests in order, and are written behind the
+ * ones it holds.  A request is refused when the free pages end before it has all
+ * of its own (later ones that need none still go through), when its pages would
+ * not fit table_cols, or when a length is negative: its row is left alone.
+ * d_starts[0, n_requests] receives the offsets of the requests' new tokens,
+ * d_slots[0, slots_cap) each new token's slot (-1 for a refused request's),
+ * d_kv_len[r] cached + new (0: refused), d_taken[0, taken_cap) the ids taken,
+ * ascending, and d_counts[0, 3) the new tokens, the pages taken and the pages
+ * that were missing.  `free_pages` stays as it is: take the ids away with
+ * cr_upload_from_device_ids and cr_set_operation(CR_ANDNOT), give them back with CR_OR. */
+int cr_paged_plan(const cr_gpu_roaring* free_pages, uint32_t n_pages, uint32_t page_size, const int32_t* d_cached,
+                  const int32_t* d_new, uint32_t n_requests, int32_t* d_table, uint32_t table_cols,
+                  uint64_t table_stride, int64_t* d_slots, uint32_t slots_cap, int32_t* d_starts, int32_t* d_kv_len,
+                  int32_t* d_taken, uint32_t taken_cap, int32_t* d_counts, cr_stream_t stream);
+/* New keys and values [n_tokens][cache->n_heads][cache->head_dim] into their
+ * slots.  A slot outside the cache (-1) is left out; of two tokens of one slot,
+ * either may stay. */
+int cr_paged_append(const void* d_k, const void* d_v, uint64_t k_token_stride, uint64_t k_head_stride,
+                    uint64_t v_token_stride, uint64_t v_head_stride, uint32_t n_tokens, const int64_t* d_slots,
+                    const cr_paged_cache* cache, cr_stream_t stream);
+/* The slots that a request may look at: d_sel[r * sel_stride + 0 .. d_sel_len[r])
+ * are those slots of its positions [0, d_kv_len[r]), in order, that `visible`
+ * (a bitmap over the slots) holds, and d_limits[t] says how many of them lie at
+ * or before new token t's own position.  A row holds table_cols * page_size
+ * slots.  Positions whose page is outside [0, n_pages) are not visible. */
+int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, uint32_t page_size, const int32_t* d_table,
+                    uint32_t table_cols, uint64_t table_stride, const int32_t* d_starts, const int32_t* d_kv_len,
+                    uint32_t n_requests, uint32_t n_tokens, int32_t* d_sel, uint64_t sel_stride, int32_t* d_sel_len,
+                    int32_t* d_limits, cr_stream_t stream);
+
+/* Attention of new tokens over the cache, which holds their own keys and values
+ * too: out = softmax(scale * q k^T) v, and lse = log(sum(exp(scale * q k^T)))
+ * where it is asked for.  Tokens [d_starts[r], d_starts[r + 1]) are request r's
+ * last ones; with `causal`, the one at position p sees positions [0, p] (none
+ * where d_kv_len[r] says that p is negative), else all of [0, d_kv_len[r]).  With
+ * a selection (cr_paged_select), the request's keys are d_sel's, and with
+ * `causal` a token sees the first d_limits of them.  A token that sees nothing,
+ * or that is in no request, gets zeros and -inf.  Query head h reads key head
+ * h / (n_heads / cache->n_heads).  Queries, cache and outputs are of one type,
+ * with 16-byte aligned rows of a head dimension that is a multiple of 8, up to
+ * 256; sums and softmax are in fp32, and the probabilities are rounded to the
+ * type before they meet the values. */
+typedef struct cr_paged_attention_args {
+    const void* q; /* [n_tokens][n_heads][head_dim] */
+    uint64_t q_token_stride, q_head_stride;
+    void* out;
+    uint64_t out_token_stride, out_head_stride;
+    float* lse; /* [n_tokens][n_heads], or NULL */
+    uint32_t n_tokens, n_heads, n_requests;
+    const int32_t* d_starts; /* [n_requests + 1] */
+    const int32_t* d_kv_len;
+    const int32_t* d_table;
+    uint32_t table_cols;
+    uint64_t table_stride;
+    const int32_t* d_sel; /* a selection, or NULL */
+    uint64_t sel_stride;
+    const int32_t* d_sel_len;
+    const int32_t* d_limits;
+    float scale;
+    uint32_t causal;
+    /* The most new tokens and the most keys of a request, where the caller knows
+     * them (0: not known).  They choose how the work is split, never the answer. */
+    uint32_t max_new, max_kv;
+} cr_paged_attention_args;
+int cr_paged_attention(const cr_paged_attention_args* args, const cr_paged_cache* cache, cr_stream_t stream);
+
+/* Beam search's selection: of the continuations (w, v) of each answer's `beams`
+ * beams by `vocab` tokens, the k (at most 256) with the largest
+ * d_cum[b][w] + (score[b][w][v] - d_lse[b][w]) (d_lse NULL: d_cum + score), in
+ * fp32, descending, ties to the lowest w * vocab + v.  `allowed`, a bitmap over
+ * [0, vocab), or d_allowed_bits, flat bitsets of ceil(vocab / 32) words as
+ * cr_decompress_to_bitset writes them, one for all rows (bits_stride 0) or one for
+ * each (b, w), bits_stride words apart, say which tokens may follow.  A total that
+ * is NaN or -inf is no candidate: a beam that has ended has a d_cum of -inf.
+ * Places without a candidate get -inf, -1 and -1. */
+int cr_beam_select(const void* d_scores, uint32_t dtype, uint32_t batch, uint32_t beams, uint32_t vocab,
+                   uint64_t batch_stride, uint64_t beam_stride, const float* d_cum, const float* d_lse,
+                   const cr_gpu_roaring* allowed, const uint32_t* d_allowed_bits, uint64_t bits_stride, uint32_t k,
+                   float* d_out_scores, int32_t* d_out_tokens, int32_t* d_out_parents, cr_stream_t stream);
+/* States after it: row (b, i) of d_dst, i < beams_out, receives row
+ * (b, d_parents[b][i]) of d_src's beams_in; where d_len is given, only the first
+ * d_len[b][parent] units of unit_bytes of it.  A row whose parent is outside
+ * [0, beams_in) is left alone.  Row strides are in bytes. */
+int cr_beam_reorder(const void* d_src, const int32_t* d_parents, uint32_t batch, uint32_t beams_in,
+                    uint32_t beams_out, uint64_t row_bytes, uint64_t src_stride, uint64_t dst_stride,
+                    const int32_t* d_len, uint64_t unit_bytes, void* d_dst, cr_stream_t stream);
+
 /* ---- utilities (no reference counterpart) -------------------------------- */
 /* L2 size the AUTO rule uses for `device_id` (hipDeviceAttributeL2CacheSize). */
 int cr_device_l2_bytes(int device_id, uint64_t* out_bytes);

@@ -1,0 +1,350 @@
+"""paged_attention against the formula in 64 bits.
+
+The bar of an output element, with u the type's unit roundoff (2^-8 bf16, 2^-11
+f16) and w = sum_j p_j |v_j| over the normalised probabilities p: the result is
+rounded once (u |o|) and each probability is rounded once before it meets its
+value (u w; below f16's normal range by 2^-25 at most, n 2^-25 max|v|).  Scores
+are fp32 sums of exact products: their error moves a probability by at most
+(dim + 8) 2^-23 |scale| sum|q k| relative, counted twice (numerator and sum), as
+do fp32 sums over n keys by n 2^-24.  An lse is off by the same score error and
+by 2^-22 of itself and of log n.
+"""
+import numpy as np
+import pytest
+
+import orc  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+U = {"float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+
+
+def _say(*a):
+    print("CASE", *a, flush=True)
+
+
+class Problem:
+    """Requests over a paged cache, the pages scattered and the unused ones full of NaN."""
+
+    def __init__(self, dtype, new, kv, heads, kv_heads, dim, page, seed=0, spread=2.0, layout="plain", density=None,
+                 causal=True):
+        import torch
+        self.torch, self.dtype, self.page, self.causal = torch, dtype, page, causal
+        self.new, self.kv = list(new), list(kv)
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, dim
+        dt = getattr(torch, dtype)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+        held = [-(-max(0, x) // page) for x in kv]
+        self.cols = max(1, max(held, default=1))
+        pages = sum(held) + 3
+        order = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)
+        self.table = torch.full((len(kv), self.cols), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for r, n in enumerate(held):
+            self.table[r, :n] = order[at:at + n]
+            at += n
+        def cache():
+            if layout == "heads first":
+                return rnd(pages, kv_heads, page, dim).to(dt).transpose(1, 2)
+            if layout == "padded":
+                return rnd(pages, page, kv_heads, dim + 16).to(dt)[..., 8:8 + dim]
+            return rnd(pages, page, kv_heads, dim).to(dt)
+        self.kc, self.vc = cache(), cache()
+        self.kc[order[at:].long()] = float("nan")
+        self.vc[order[at:].long()] = float("nan")
+        for r, n in enumerate(held):  # what lies behind a request's last token is not read into its answer
+            if n and kv[r] % page:
+                self.kc[self.table[r, n - 1].long(), kv[r] % page:] = float("nan")
+                self.vc[self.table[r, n - 1].long(), kv[r] % page:] = float("nan")
+        total = sum(new)
+        if layout == "heads first":
+            self.q = (rnd(heads, total, dim) * spread).to(dt).transpose(0, 1)
+        elif layout == "padded":
+            self.q = (rnd(total, heads + 2, dim + 8) * spread).to(dt)[:, 1:1 + heads, :dim]
+        else:
+            self.q = (rnd(total, heads, dim) * spread).to(dt)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.starts = torch.tensor(np.concatenate([[0], np.cumsum(new)]).astype(np.int32)).cuda()
+        self.kv_len = torch.tensor(kv, **i32)
+        self.visible = None
+        if density is not None:
+            self.visible = (torch.rand(pages * page, device="cuda", generator=g) < density)
+            self.sel = torch.full((len(kv), self.cols * page), -1, **i32)
+            self.sel_len, self.limits = torch.zeros(len(kv), **i32), torch.zeros(total, **i32)
+
+    def run(self, gpu, scale=None, **kw):
+        torch = self.torch
+        selection = None
+        if self.visible is not None:
+            words = self.visible.cpu().numpy()
+            ids = np.nonzero(words)[0].astype(np.uint32)
+            g = gpu.upload_from_ids(ids, len(words))
+            gpu.paged_select(g, self.table, self.starts, self.kv_len, self.page, self.sel, self.sel_len, self.limits,
+                             self.kc.shape[0])
+            selection = (self.sel, self.sel_len, self.limits)
+        out = torch.full((sum(self.new) + 2, self.heads, self.dim), 7.0, device="cuda", dtype=self.q.dtype)
+        lse = torch.full((sum(self.new), self.heads), 7.0, device="cuda")
+        gpu.paged_attention(self.q, self.kc, self.vc, self.table, self.starts, self.kv_len, out[:sum(self.new)],
+                            scale=scale, causal=self.causal, d_lse=lse, selection=selection, **kw)
+        torch.cuda.synchronize()
+        if selection is not None:
+            gpu.free(g)
+        assert torch.all(out[sum(self.new):] == 7.0), "written past the last token"
+        return out[:sum(self.new)].float().cpu().numpy().astype(np.float64), lse.cpu().numpy().astype(np.float64)
+
+    def check(self, gpu, scale=None, **kw):
+        out, lse = self.run(gpu, scale, **kw)
+        scale = self.dim ** -0.5 if scale is None else scale
+        u, group = U[self.dtype], self.heads // self.kv_heads
+        host = lambda t: t.float().cpu().numpy().astype(np.float64)  # noqa: E731
+        q, table = host(self.q), self.table.cpu().numpy()
+        kc, vc = host(self.kc), host(self.vc)
+        visible = None if self.visible is None else self.visible.cpu().numpy()
+        at = 0
+        for n, kv, row in zip(self.new, self.kv, table):
+            pos = np.arange(max(0, kv))
+            page, off = row[pos // self.page], pos % self.page
+            if visible is not None:
+                keep = visible[page * self.page + off]
+                pos, page, off = pos[keep], page[keep], off[keep]
+            for h in range(self.heads if n else 0):
+                k, v = kc[page, off, h // group], vc[page, off, h // group]
+                for i in range(n):
+                    see = pos <= kv - n + i if self.causal else pos >= 0
+                    o, z = out[at + i, h], lse[at + i, h]
+                    if not see.any():
+                        assert np.all(o == 0) and z == -np.inf, (at + i, h)
+                        continue
+                    s = scale * (k[see] @ q[at + i, h])
+                    ds = (self.dim + 8) * 2.0 ** -23 * abs(scale) * (np.abs(k[see]) @ np.abs(q[at + i, h])).max()
+                    m = s.max()
+                    p = np.exp(s - m)
+                    z0 = m + np.log(p.sum())
+                    p /= p.sum()
+                    o0, w = p @ v[see], p @ np.abs(v[see])
+                    c = int(see.sum())
+                    tiny = c * 2.0 ** -25 * np.abs(v[see]).max() if self.dtype == "float16" else 0.0
+                    tol = 1.01 * (u * np.abs(o0) + u * w + tiny + (2 * ds + c * 2.0 ** -24 + 2.0 ** -20) * w)
+                    assert np.all(np.abs(o - o0) <= tol), (at + i, h, np.max(np.abs(o - o0) / tol))
+                    assert abs(z - z0) <= ds + 2.0 ** -22 * (abs(z0) + np.log(c) + 2) + c * 2.0 ** -24, (at + i, h, z, z0)
+            at += n
+
+
+# new, kv, heads, key heads, dim, page
+SHAPES = {
+    "one token, one key": ([1], [1], 1, 1, 64, 16),
+    "short context": ([1], [37], 8, 2, 128, 16),
+    "decode ragged": ([1, 1, 1, 1, 1], [1, 16, 17, 300, 1025], 8, 2, 128, 16),
+    "decode mha": ([1, 1, 1], [63, 64, 65], 5, 5, 64, 32),
+    "decode wide group": ([1, 1], [200, 129], 24, 1, 128, 8),
+    "decode group 33": ([1], [150], 33, 1, 64, 16),
+    "no tokens between": ([1, 0, 2, 0], [40, 33, 70, 0], 4, 4, 64, 16),
+    "a few tokens": ([4, 3, 5], [260, 3, 131], 16, 4, 128, 16),
+    "chunk": ([130, 1, 64], [400, 77, 64], 4, 2, 128, 16),
+    "prompt": ([257], [257], 4, 1, 64, 64),
+    "prompt group 3": ([100, 45], [100, 300], 6, 2, 96, 16),
+    "dims 8": ([3, 40], [50, 40], 4, 2, 8, 16),
+    "dims 80": ([1, 70], [333, 70], 4, 2, 80, 16),
+    "dims 192": ([1, 70], [129, 200], 4, 2, 192, 16),
+    "dims 256": ([2, 90], [97, 150], 4, 2, 256, 16),
+    "pages of one": ([1, 20], [70, 66], 2, 1, 64, 1),
+    "pages longer than the context": ([1, 20], [70, 66], 2, 2, 64, 1024),
+    "more tokens than positions": ([9, 70], [5, 40], 2, 1, 64, 16),
+    "negative length": ([2, 1], [-3, 20], 2, 1, 64, 16),
+}
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("what", SHAPES)
+def test_attention(gpu, dtype, what):
+    _say("attention", dtype, what)
+    Problem(dtype, *SHAPES[what], seed=len(what)).check(gpu)
+
+
+@pytest.mark.parametrize("density", [0.0, 0.02, 0.4, 1.0])
+@pytest.mark.parametrize("what", ["decode ragged", "a few tokens", "chunk", "prompt group 3", "pages of one",
+                                  "more tokens than positions"])
+def test_attention_over_a_selection(gpu, what, density):
+    _say("attention selection", what, density)
+    Problem("float16", *SHAPES[what], seed=3, density=density).check(gpu)
+
+
+@pytest.mark.parametrize("density", [None, 0.3])
+@pytest.mark.parametrize("what", ["decode ragged", "chunk", "more tokens than positions"])
+def test_attention_not_causal(gpu, what, density):
+    _say("attention not causal", what, density)
+    Problem("bfloat16", *SHAPES[what], seed=4, density=density, causal=False).check(gpu)
+
+
+@pytest.mark.parametrize("layout", ["heads first", "padded"])
+@pytest.mark.parametrize("what", ["decode ragged", "chunk", "dims 80"])
+def test_attention_strides(gpu, what, layout):
+    _say("attention strides", what, layout)
+    Problem("bfloat16", *SHAPES[what], seed=5, layout=layout).check(gpu)
+
+
+@pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.2, 1.0), (1.0, 8.0), (1e-3, 1.0)])
+@pytest.mark.parametrize("what", ["decode ragged", "chunk"])
+def test_attention_scales(gpu, what, scale, spread):
+    """Scores that are all alike, turned round, and hundreds apart (one key takes everything)."""
+    _say("attention scale", what, scale)
+    Problem("float16", *SHAPES[what], seed=6, spread=spread).check(gpu, scale=scale)
+
+
+@pytest.mark.parametrize("hints", [dict(max_new=1, max_kv=1), dict(max_new=5000, max_kv=1 << 20), dict(max_kv=200)])
+@pytest.mark.parametrize("what", ["decode ragged", "chunk"])
+def test_hints_do_not_change_the_answer(gpu, what, hints):
+    _say("attention hints", what, hints)
+    Problem("bfloat16", *SHAPES[what], seed=7).check(gpu, **hints)
+
+
+@pytest.mark.parametrize("new,kv", [([1], [20011]), ([1, 1], [5000, 12345]), ([17], [9000]), ([1], [65536])])
+def test_attention_long_contexts(gpu, new, kv):
+    _say("attention long", new, kv)
+    Problem("bfloat16", new, kv, 8, 2, 128, 16, seed=8).check(gpu)
+    Problem("float16", new, kv, 4, 4, 64, 32, seed=9, density=0.2).check(gpu)
+
+
+def test_rising_scores(gpu):
+    """Each key's score beats all before it, by little and by much: the running maximum moves at every key."""
+    import torch
+    for step in (0.02, 1.5):
+        for new, kv in (([1], [700]), ([90], [300])):
+            _say("attention rising", step, kv)
+            p = Problem("float16", new, kv, 2, 1, 64, 16, seed=10)
+            p.q[:] = 0
+            p.q[:, :, 0] = 1.0
+            row = p.table[0].long()
+            pos = torch.arange(kv[0], device="cuda")
+            p.kc[row[pos // 16], pos % 16, :, 0] = (pos * step).half()[:, None]
+            p.check(gpu, scale=1.0)
+
+
+def test_infinite_and_nan_values_where_nothing_looks(gpu):
+    """Keys and values after a token's position hold inf and NaN: earlier tokens do not see them."""
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        _say("attention", bad, "behind the causal limit")
+        p = Problem("bfloat16", [5], [105], 4, 2, 64, 16, seed=11)
+        whole, _ = p.run(__import__("curoaring"))
+        for pos in (103, 104):
+            page = p.table[0, pos // 16].long()
+            p.kc[page, pos % 16] = bad
+            p.vc[page, pos % 16] = bad
+        out, lse = p.run(__import__("curoaring"))
+        assert np.array_equal(out[:3], whole[:3]) and np.all(np.isfinite(lse[:3]))
+
+
+def test_pages_outside_the_cache_are_not_seen(gpu):
+    _say("attention with pages outside the cache")
+    p = Problem("bfloat16", [1, 40], [100, 90], 4, 2, 64, 16, seed=12)
+    p.table[0, 2], p.table[1, 1] = -1, p.kc.shape[0]
+    seen = p.run(gpu)
+    # the same with a selection that leaves these positions out
+    ref = Problem("bfloat16", [1, 40], [100, 90], 4, 2, 64, 16, seed=12, density=1.0)
+    keep = ref.visible.clone()
+    for r, c in ((0, 2), (1, 1)):
+        page = int(ref.table[r, c])
+        keep[page * 16:page * 16 + 16] = False
+    ref.visible = keep
+    want = ref.run(gpu)
+    assert np.allclose(seen[0], want[0], rtol=2.0 ** -6, atol=2.0 ** -6) and np.allclose(seen[1], want[1], rtol=1e-5)
+
+
+def test_tokens_in_no_request_get_zeros(gpu):
+    import torch
+    _say("attention tokens in no request")
+    p = Problem("float16", [3, 2], [50, 40], 2, 1, 64, 16, seed=13)
+    want, want_lse = p.run(gpu)
+    q = torch.cat([p.q, torch.ones_like(p.q)])
+    out, lse = torch.full_like(q, 7.0), torch.full((10, 2), 7.0, device="cuda")
+    gpu.paged_attention(q, p.kc, p.vc, p.table, p.starts, p.kv_len, out, d_lse=lse)
+    torch.cuda.synchronize()
+    assert np.array_equal(out[:5].float().cpu().numpy(), want) and np.array_equal(lse[:5].cpu().numpy(), want_lse)
+    assert torch.all(out[5:] == 0) and torch.all(lse[5:] == float("-inf"))
+
+
+def test_no_requests(gpu):
+    import torch
+    _say("attention without requests")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = torch.ones(3, 2, 64, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    kc = torch.zeros(2, 16, 1, 64, device="cuda").half()
+    gpu.paged_attention(q, kc, kc.clone(), torch.zeros(0, 1, **i32), torch.zeros(1, **i32), torch.zeros(0, **i32), out)
+    torch.cuda.synchronize()
+    assert torch.all(out == 0)
+
+
+def test_two_runs_give_the_same_bits(gpu):
+    _say("attention twice")
+    for what in ("decode ragged", "chunk", "a few tokens"):
+        p = Problem("bfloat16", *SHAPES[what], seed=14)
+        a, b = p.run(gpu), p.run(gpu)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_another_stream(gpu):
+    import torch
+    _say("attention on another stream")
+    p = Problem("bfloat16", *SHAPES["decode ragged"], seed=15)
+    want, _ = p.run(gpu)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    out = torch.zeros_like(p.q)
+    with torch.cuda.stream(s):
+        out.fill_(3.0)
+        gpu.paged_attention(p.q, p.kc, p.vc, p.table, p.starts, p.kv_len, out, stream=s)
+    s.synchronize()
+    assert np.array_equal(out.float().cpu().numpy(), want)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A cache whose last pages lie beyond 2^32 elements."""
+    import torch
+    _say("attention in a cache past 2^32 elements")
+    p = Problem("float16", [1, 33], [200, 150], 8, 8, 128, 16, seed=16)
+    want, want_lse = p.run(gpu)
+    pages = (1 << 32) // (16 * 8 * 128) + 64
+    used = p.kc.shape[0]
+    for name in ("kc", "vc"):
+        small = getattr(p, name)
+        big = torch.empty(pages, 16, 8, 128, device="cuda", dtype=torch.float16)
+        big[pages - used:] = small
+        setattr(p, name, big)
+    p.table[p.table >= 0] += pages - used
+    out, lse = p.run(gpu)
+    assert np.array_equal(out, want) and np.array_equal(lse, want_lse)
+
+
+def test_refusals(gpu):
+    import torch
+    _say("attention refusals")
+    p = Problem("float16", [2], [40], 4, 2, 64, 16)
+    ok = dict(d_q=p.q, d_k_cache=p.kc, d_v_cache=p.vc, d_table=p.table, d_starts=p.starts, d_kv_len=p.kv_len,
+              d_out=torch.empty_like(p.q))
+    gpu.paged_attention(**ok)
+    torch.cuda.synchronize()
+    wide = torch.zeros(2, 4, 264, device="cuda").half()
+    wide_c = torch.zeros(3, 16, 2, 264, device="cuda").half()
+    odd = torch.zeros(2 * 4 * 64 + 1, device="cuda").half()[1:].view(2, 4, 64)
+    for bad, code in ((dict(d_q=p.q.float(), d_out=p.q.float()), gpu.CR_ERR_INVALID),
+                      (dict(d_q=p.q[:, :3], d_out=torch.empty_like(p.q[:, :3])), gpu.CR_ERR_INVALID),
+                      (dict(d_q=p.q[:, :, :32]), gpu.CR_ERR_INVALID),
+                      (dict(d_out=ok["d_out"][:1]), gpu.CR_ERR_INVALID),
+                      (dict(d_v_cache=p.vc[:2]), gpu.CR_ERR_INVALID),
+                      (dict(d_k_cache=p.kc[:, :12], d_v_cache=p.vc[:, :12]), gpu.CR_ERR_INVALID),
+                      (dict(d_table=p.table.long()), gpu.CR_ERR_INVALID),
+                      (dict(d_starts=p.starts[:1]), gpu.CR_ERR_INVALID),
+                      (dict(d_kv_len=p.kv_len.long()), gpu.CR_ERR_INVALID),
+                      (dict(d_lse=torch.zeros(2, 3, device="cuda")), gpu.CR_ERR_INVALID),
+                      (dict(selection=(p.table, p.kv_len, p.kv_len)), gpu.CR_ERR_INVALID),
+                      (dict(d_q=wide, d_out=wide.clone(), d_k_cache=wide_c, d_v_cache=wide_c), gpu.CR_ERR_UNSUPPORTED),
+                      (dict(d_q=wide[..., :60], d_out=wide[..., :60].clone(), d_k_cache=wide_c[..., :60],
+                            d_v_cache=wide_c[..., :60]), gpu.CR_ERR_UNSUPPORTED),
+                      (dict(d_q=odd), gpu.CR_ERR_UNSUPPORTED),
+                      (dict(d_k_cache=p.kc.float(), d_v_cache=p.vc.float(), d_q=p.q.float(), d_out=p.q.float()),
+                       gpu.CR_ERR_UNSUPPORTED)):
+        with pytest.raises(gpu.CrError) as e:
+            gpu.paged_attention(**{**ok, **bad})
+        assert e.value.code == code, bad.keys()
