@@ -13,6 +13,7 @@ namespace crimpl {
 namespace {
 
 constexpr uint32_t AT_DIM_MAX = 256;
+constexpr uint32_t AT_SPLITS = 128;  // ranges of keys at most
 
 struct AttnArgs {
     const uint16_t* q;
@@ -36,85 +37,903 @@ struct AttnArgs {
     const int32_t* limits;
     float scale;
     uint32_t causal;
+    // The launch: tiles of rows by ranges of split_len keys (the last one takes
+    // all that are left), results of several ranges kept in fp32 to be joined.
+    uint32_t n_tiles, splits, split_len;
+    uint64_t rows_total;  // n_tokens * heads
+    float* part_o;        // [splits][rows_total][dim]
+    float* part_lse;      // [splits][rows_total], base 2
 };
 
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The two element types: rounding to nearest even, and the matrix products.
 struct Half {
     static __device__ __forceinline__ float up(uint16_t x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); }
-    static __device__ __forceinline__ uint16_t down(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
+    static __device__ __forceinline__ uint16_t down(float x)
+    {
+        return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
+    }
+    static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+    }
+    static constexpr uint32_t EXP = 0x7C00u;  // the exponent's bits: all set in infinities and NaN
 };
 struct BHalf {
     static __device__ __forceinline__ float up(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
-    static __device__ __forceinline__ uint16_t down(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
+    static __device__ __forceinline__ uint16_t down(float x)
+    {
+        return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+    }
+    static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+    }
+    static constexpr uint32_t EXP = 0x7F80u;
 };
 
-constexpr int AT_NT = 256;
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
+// A row's running maximum may fall this far (in powers of two) behind its
+// scores before the sums are scaled anew: probabilities then stay below 2^8,
+// which f16 holds, and a row is scaled a few times in all instead of at each
+// new maximum.
+constexpr float LAG = 8.0f;
 
-// A workgroup per (token, head), a tile of AT_NT keys at a time.
-template <class E>
-__global__ __launch_bounds__(AT_NT) void at_simple(AttnArgs a)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Four transposed pieces of LDS: of each 16 lanes, lane i names 8 bytes of row
+// i / 4 and receives elements i of the four rows.
+__device__ __forceinline__ v4s lds_tr(const uint16_t* p)
 {
-    __shared__ float s_q[AT_DIM_MAX], s_p[AT_NT], s_red[AT_NT / 64];
-    __shared__ int32_t s_slot[AT_NT];
-    const uint32_t t = threadIdx.x, token = blockIdx.x, h = blockIdx.y, kh = h / (a.heads / a.kv_heads);
-    uint32_t lo = 0, hi = a.n_requests;
-    int64_t limit = 0;
-    if (a.n_requests && a.starts[0] <= static_cast<int32_t>(token) && static_cast<int32_t>(token) < a.starts[a.n_requests]) {
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (a.starts[mid] <= static_cast<int32_t>(token)) lo = mid;
-            else hi = mid;
-        }
-        const int64_t room = static_cast<int64_t>(a.cols) << a.page_lg;
-        const int64_t len = min(room, static_cast<int64_t>(max(a.sel ? a.sel_len[lo] : a.kv_len[lo], 0)));
-        limit = len;
-        if (a.causal) {
-            const int64_t at = a.sel ? a.limits[token] : static_cast<int64_t>(a.kv_len[lo]) - a.starts[lo + 1] + token + 1;
-            limit = max(static_cast<int64_t>(0), min(len, at));
-        }
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p);
+}
+
+__device__ __forceinline__ v8s join(v4s x, v4s y) { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+__device__ __forceinline__ v8s load8(const uint16_t* p) { return *reinterpret_cast<const v8s*>(p); }
+__device__ __forceinline__ v4s load4(const uint16_t* p) { return *reinterpret_cast<const v4s*>(p); }
+
+// Whether any of eight values is infinite or NaN, and the eight with zeros for those.
+__device__ __forceinline__ bool has_special(v8s x, uint32_t exp)
+{
+    const v4u w = __builtin_bit_cast(v4u, x);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & exp) == exp || (w[i] & (exp << 16)) == exp << 16;
+    return bad;
+}
+
+__device__ __forceinline__ v8s without_special(v8s x, uint32_t exp)
+{
+    v4u w = __builtin_bit_cast(v4u, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = (w[i] & exp) == exp ? 0u : 0xFFFFu, hi = (w[i] & (exp << 16)) == exp << 16 ? 0u : 0xFFFF0000u;
+        w[i] &= lo | hi;
     }
-    for (uint32_t d = t; d < a.dim; d += AT_NT) s_q[d] = E::up(a.q[token * a.q_token + h * a.q_head + d]) * a.scale;
-    float m = -__builtin_inff(), l = 0, o = 0;
-    for (int64_t j0 = 0; j0 < limit; j0 += AT_NT) {
-        __syncthreads();
-        const int64_t j = j0 + t;
-        float s = -__builtin_inff();
-        int32_t slot = -1;
-        if (j < limit) {
-            if (a.sel) slot = a.sel[lo * a.sel_stride + j];
-            else {
-                const int32_t page = a.table[lo * a.table_stride + (j >> a.page_lg)];
-                if (static_cast<uint32_t>(page) < a.n_pages) slot = (page << a.page_lg) + static_cast<int32_t>(j & ((1 << a.page_lg) - 1));
+    return __builtin_bit_cast(v8s, w);
+}
+
+__device__ __forceinline__ v8s zero_unless(bool keep, v8s x)
+{
+    const uint32_t mask = keep ? 0xFFFFFFFFu : 0u;
+    return __builtin_bit_cast(v8s, __builtin_bit_cast(v4u, x) & mask);
+}
+
+// Adds the infinite and NaN ones of four values.
+template <class E, class V>
+__device__ __forceinline__ void add_special(V& o, uint32_t i, v4s x)
+{
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+        if ((static_cast<uint16_t>(x[e]) & E::EXP) == E::EXP) o[i + e] += E::up(static_cast<uint16_t>(x[e]));
+}
+
+// Segment i of the tokens: request i - 1's; the first and the last one hold
+// those before and behind all requests, which see nothing.
+__device__ __forceinline__ int32_t segment_start(const AttnArgs& a, uint32_t i)
+{
+    if (i == 0) return 0;
+    return min(max(a.starts[i - 1], 0), static_cast<int32_t>(a.n_tokens));
+}
+
+// A tile of `most` rows of a segment; row m is token m / group, head m % group
+// of those that share a key head.
+struct Tile {
+    uint32_t request;
+    bool real;        // a request's, not the tokens' outside
+    int32_t token0;   // the segment's first token
+    uint32_t tokens;
+    uint32_t row0, rows;  // rows [row0, rows) are this tile's and those behind it
+};
+
+// Tile `id` of the launch: segment i's tiles start at i + (its first token's
+// row) / most, which leaves each of them room for all of its rows.  A wave
+// searches together, 64 segments at a time.
+__device__ __forceinline__ Tile find_tile(const AttnArgs& a, uint32_t id, uint32_t most)
+{
+    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
+    auto base = [&](uint32_t i) {
+        return static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(segment_start(a, i))) * group / most) + i;
+    };
+    uint32_t lo = 0, len = n;  // base(lo) <= id
+    while (len > 1) {
+        const uint32_t step = (len + 63) / 64, i = lo + lane * step;
+        const bool at_most = lane * step < len && base(i) <= id;
+        const uint32_t c = static_cast<uint32_t>(__popcll(__ballot(at_most)));
+        const uint32_t from = c ? (c - 1) * step : 0u;
+        lo += from;
+        len = min(step, len - from);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    Tile t;
+    t.real = lo > 0 && lo <= a.n_requests;
+    t.request = t.real ? lo - 1 : 0;
+    t.token0 = segment_start(a, lo);
+    const int32_t end = lo + 1 < n ? segment_start(a, lo + 1) : static_cast<int32_t>(a.n_tokens);
+    t.tokens = static_cast<uint32_t>(max(end - t.token0, 0));
+    t.rows = t.tokens * group;
+    t.row0 = (id - base(lo)) * most;
+    return t;
+}
+
+// How many of its request's keys a token sees.
+__device__ __forceinline__ uint32_t keys_of(const AttnArgs& a, const Tile& t)
+{
+    if (!t.real) return 0;
+    const int32_t n = a.sel ? a.sel_len[t.request] : a.kv_len[t.request];
+    const uint64_t room = static_cast<uint64_t>(a.cols) << a.page_lg;
+    return n <= 0 ? 0u : static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
+}
+
+__device__ __forceinline__ uint32_t limit_of(const AttnArgs& a, const Tile& t, uint32_t keys, uint32_t token)
+{
+    if (!t.real || !a.causal) return keys;
+    const int64_t at = a.sel ? static_cast<int64_t>(a.limits[t.token0 + token])
+                             : static_cast<int64_t>(a.kv_len[t.request]) - t.tokens + token + 1;
+    return static_cast<uint32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), at)));
+}
+
+// The cache slot of the request's key j < keys, -1 where its page is outside
+// the cache.
+__device__ __forceinline__ int32_t slot_of(const AttnArgs& a, uint32_t request, uint32_t j)
+{
+    int32_t slot;
+    if (a.sel) {
+        slot = a.sel[request * a.sel_stride + j];
+    } else {
+        const int32_t page = a.table[request * a.table_stride + (j >> a.page_lg)];
+        if (static_cast<uint32_t>(page) >= a.n_pages) return -1;
+        slot = (page << a.page_lg) + static_cast<int32_t>(j & ((1u << a.page_lg) - 1u));
+    }
+    return (static_cast<uint32_t>(slot) >> a.page_lg) < a.n_pages ? slot : -1;
+}
+
+__device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, uint64_t page_stride, uint64_t slot_stride)
+{
+    const uint32_t at = static_cast<uint32_t>(max(slot, 0));
+    return (at >> page_lg) * page_stride + (at & ((1u << page_lg) - 1u)) * slot_stride;
+}
+
+// Queries come in with the sign of the scale, so that the largest product is
+// the largest score.
+__device__ __forceinline__ v8s load_query(const AttnArgs& a, const Tile& t, uint32_t row, uint32_t kh, uint32_t d)
+{
+    const uint32_t group = a.heads / a.kv_heads;
+    v8s x = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (row < t.rows && d < a.dim && a.scale != 0.0f) {
+        x = load8(a.q + static_cast<uint64_t>(t.token0 + row / group) * a.q_token + (kh * group + row % group) * a.q_head + d);
+        if (a.scale < 0.0f) x ^= static_cast<short>(0x8000);
+    }
+    return x;
+}
+
+__device__ __forceinline__ float score_scale(const AttnArgs& a)
+{
+    return a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;  // queries are zero where the scale is
+}
+
+// A row's four dimensions from d: rounded into the output, or kept in fp32
+// where another kernel joins the ranges of keys.
+template <class E>
+__device__ __forceinline__ void store_row(const AttnArgs& a, E, uint32_t split, uint64_t row, uint32_t token,
+                                          uint32_t head, uint32_t d, f32x4 x)
+{
+    if (a.splits > 1) {
+        *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows_total + row) * a.dim + d) = x;
+    } else {
+        const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
+                       static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
+        *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
+    }
+}
+
+// lse2: base 2
+__device__ __forceinline__ void store_lse(const AttnArgs& a, uint32_t split, uint64_t row, float lse2)
+{
+    if (a.splits > 1)
+        a.part_lse[split * a.rows_total + row] = lse2;
+    else if (a.lse)
+        a.lse[row] = lse2 * LN2;
+}
+
+// ---- few rows: bound by reading keys and values ------------------------------------
+// A workgroup answers up to 16 NB rows over a range of keys, each of its waves
+// every fourth 32 of them on its own: scores are transposed products (keys x
+// rows) of 16x16x32 matrix instructions, whose result has a row's probabilities
+// in the lanes that the second product wants them in, if keys are taken in the
+// order 4h..4h+3, 16+4h..16+4h+3 for lane group h.  Keys go from memory to
+// registers in operand order; values pass through the wave's LDS, which
+// transposes them.  Both are loaded a tile ahead.
+constexpr int DC_NT = 256;
+constexpr uint32_t DC_WAVES = DC_NT / 64;
+constexpr uint32_t DC_KEYS = 32;
+
+template <uint32_t DIM>
+struct Rows {
+    static constexpr uint32_t CHUNKS = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;  // 16-byte pieces of a row in LDS
+    static constexpr uint32_t STRIDE = CHUNKS * 8;                             // its elements
+};
+
+template <class E, uint32_t DIM, bool FULL, uint32_t NB>
+__global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
+{
+    constexpr uint32_t STEPS = DIM / 32, BLOCKS = DIM / 16, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
+    constexpr uint32_t PER = 64 / CHUNKS, LOADS = DC_KEYS / PER;  // values: rows an instruction covers, instructions
+    constexpr uint32_t RED = DIM + 4;
+    // the values' tiles, and in the end the waves' sums
+    constexpr uint32_t BYTES = DC_WAVES * (DC_KEYS * STRIDE * 2 > 16 * RED * 4 ? DC_KEYS * STRIDE * 2 : 16 * RED * 4);
+    __shared__ alignas(16) char s_mem[BYTES];
+    __shared__ float s_m[DC_WAVES][16 * NB], s_l[DC_WAVES][16 * NB];
+    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c16 = lane & 15u, h = lane >> 4;
+    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
+    const Tile t = find_tile(a, rest / a.splits, 16 * NB);
+    if (t.row0 >= t.rows) return;
+    const uint32_t group = a.heads / a.kv_heads, keys = keys_of(a, t);
+    uint32_t limit[NB], most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        const uint32_t row = t.row0 + b * 16 + c16;
+        limit[b] = row < t.rows ? limit_of(a, t, keys, row / group) : 0u;
+        most = max(most, limit[b]);
+        if (row < t.rows) least = min(least, limit[b]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
+        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+    const uint32_t k0 = split * a.split_len;
+    const uint32_t k1 = split + 1 == a.splits ? most : min(most, k0 + a.split_len);
+    if (split > 0 && k0 >= most) {
+        if (threadIdx.x < 16 * NB && t.row0 + threadIdx.x < t.rows) {
+            const uint32_t row = t.row0 + threadIdx.x;
+            a.part_lse[split * a.rows_total + static_cast<uint64_t>(t.token0 + row / group) * a.heads + kh * group + row % group] = NEG_INF;
+        }
+        return;
+    }
+
+    v8s q[NB][STEPS];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = load_query(a, t, t.row0 + b * 16 + c16, kh, s * 32 + h * 8);
+    f32x4 o[NB][BLOCKS];
+    float m[NB], l[NB];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        m[b] = NEG_INF;
+        l[b] = 0.0f;
+#pragma unroll
+        for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] = f32x4{0, 0, 0, 0};
+    }
+    const float c = score_scale(a);
+    const uint16_t* kp = a.k + kh * a.k_head;
+    const uint16_t* vp = a.v + kh * a.v_head;
+    uint16_t* lds = reinterpret_cast<uint16_t*>(s_mem) + wave * DC_KEYS * STRIDE;
+    const uint32_t vrow = lane / CHUNKS, vchunk = lane % CHUNKS;
+    const uint32_t vcol = vchunk * 8 < a.dim ? vchunk * 8 : 0u;
+
+    v8s k[2][STEPS], v[LOADS];
+    // Lane j < 32 (and j + 32) looks after key j of a tile.
+    auto slots = [&](uint32_t j0) {
+        const uint32_t j = j0 + (lane & 31u);
+        return j < k1 ? slot_of(a, t.request, j) : -1;
+    };
+    auto load_keys = [&](int32_t slot) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const int32_t at = __shfl(slot, static_cast<int>(b * 16 + c16), 64);
+            const uint16_t* p = kp + offset_of(at, a.page_lg, a.k_page, a.k_slot);
+#pragma unroll
+            for (uint32_t s = 0; s < STEPS; ++s) {
+                const uint32_t d = s * 32 + h * 8;
+                k[b][s] = load8(p + (FULL || d < a.dim ? d : 0u));
             }
-            if (static_cast<uint64_t>(static_cast<uint32_t>(slot)) >> a.page_lg >= a.n_pages) slot = -1;
         }
-        s_slot[t] = slot;
-        if (slot >= 0) {
-            const uint16_t* k = a.k + (slot >> a.page_lg) * a.k_page + (slot & ((1 << a.page_lg) - 1)) * a.k_slot + kh * a.k_head;
-            s = 0;
-            for (uint32_t d = 0; d < a.dim; ++d) s += s_q[d] * E::up(k[d]);
+    };
+    auto load_values = [&](int32_t slot) {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            const int32_t at = __shfl(slot, static_cast<int>(i * PER + vrow), 64);
+            v[i] = load8(vp + offset_of(at, a.page_lg, a.v_page, a.v_slot) + vcol);
         }
-        float top = s;
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-        if ((t & 63) == 0) s_red[t >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-        const float now = fmaxf(m, top);
-        if (now == -__builtin_inff()) continue;
-        const float fix = __expf(m - now);
-        m = now;
-        s_p[t] = __expf(s - now);
-        __syncthreads();
-        o *= fix;
-        l *= fix;
-        for (uint32_t i = 0; i < AT_NT; ++i) {
-            if (s_slot[i] < 0) continue;
-            l += s_p[i];
-            if (t < a.dim)
-                o += s_p[i] * E::up(a.v[(s_slot[i] >> a.page_lg) * a.v_page + (s_slot[i] & ((1 << a.page_lg) - 1)) * a.v_slot + kh * a.v_head + t]);
+    };
+
+    uint32_t j0 = k0 + wave * DC_KEYS;
+    int32_t slot = -1, next = -1;
+    if (j0 < k1) {
+        slot = slots(j0);
+        load_keys(slot);
+        load_values(slot);
+        next = slots(j0 + DC_WAVES * DC_KEYS);
+    }
+    for (; j0 < k1; j0 += DC_WAVES * DC_KEYS) {
+        const uint64_t there = __ballot(slot >= 0);
+        const bool more = j0 + DC_WAVES * DC_KEYS < k1;
+        const bool whole = static_cast<uint32_t>(there) == 0xFFFFFFFFu && j0 + DC_KEYS <= least;
+        f32x4 s[NB][2];
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x) s[b][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+            for (uint32_t st = 0; st < STEPS; ++st)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) s[b][x] = E::mfma16(k[x][st], q[b][st], s[b][x]);
+        if (more) load_keys(next);
+
+        v8s p[NB];
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            if (!whole) {
+                const int32_t left = static_cast<int32_t>(limit[b] - j0 - h * 4);
+                const uint32_t on = static_cast<uint32_t>(there) >> (h * 4);
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const bool see = static_cast<int32_t>(x * 16 + i) < left & (on & (1u << (x * 16 + i))) != 0;
+                        s[b][x][i] = see ? s[b][x][i] : NEG_INF;
+                    }
+            }
+            float top = NEG_INF;
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, s[b][x][i]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any((top - m[b]) * c > LAG)) {  // m starts at -inf; NaN where both are
+                const float now = fmaxf(m[b], top);
+                const float fix = now == NEG_INF ? 1.0f : exp2_fast((m[b] - now) * c);
+                m[b] = now;
+                l[b] *= fix;
+#pragma unroll
+                for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] *= fix;
+            }
+            const float mc = m[b] == NEG_INF ? 0.0f : m[b] * c;
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float e = exp2_fast(__builtin_fmaf(s[b][x][i], c, -mc));
+                    l[b] += e;
+                    p[b][x * 4 + i] = static_cast<short>(E::down(e));
+                }
+        }
+
+        // The values of keys that no row sees count as zeros.  (Pieces behind the
+        // head dimension repeat the first one: they meet zero queries, and their
+        // columns are not stored.)
+        uint64_t bad = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            const uint32_t r = i * PER + vrow;
+            v8s x = v[i];
+            if (!whole) {
+                x = zero_unless((there >> r) & 1u, x);
+                bad |= __ballot(has_special(x, E::EXP));
+                x = without_special(x, E::EXP);
+            }
+            const uint32_t turn = CHUNKS == 8 ? ((r >> 1) & 3u) << 1 : (r & 7u) << 1;
+            *reinterpret_cast<v8s*>(lds + r * STRIDE + (vchunk ^ turn) * 8) = x;
+        }
+        const int32_t was = slot;
+        slot = next;
+        if (more) {
+            load_values(next);
+            next = slots(j0 + 2 * DC_WAVES * DC_KEYS);
+        }
+        wave_lds_fence();
+#pragma unroll
+        for (uint32_t d = 0; d < BLOCKS; ++d) {
+            const uint32_t r = h * 4 + c16 / 4, chunk = d * 2 + (c16 & 3u) / 2;
+            const uint32_t turn = CHUNKS == 8 ? ((r >> 1) & 3u) << 1 : (r & 7u) << 1;
+            const uint16_t* at = lds + r * STRIDE + (chunk ^ turn) * 8 + (c16 & 1u) * 4;
+            const v8s x = join(lds_tr(at), lds_tr(at + 16 * STRIDE));
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) o[b][d] = E::mfma16(x, p[b], o[b][d]);
+        }
+        wave_lds_fence();
+        if (bad) {
+            // Infinite and NaN values, left out above so that rows which do not
+            // see their keys are spared, reach the rows that do.
+            for (uint32_t j = 0; j < DC_KEYS; ++j) {
+                const int32_t at = __shfl(was, static_cast<int>(j), 64);
+                if (at < 0) continue;
+                const uint16_t* from = vp + offset_of(at, a.page_lg, a.v_page, a.v_slot);
+                uint32_t h4 = h * 4;
+                asm volatile("" : "+v"(h4));  // the addresses are worked out here, not kept in registers
+#pragma unroll
+                for (uint32_t d = 0; d < BLOCKS; ++d) {
+                    const uint32_t at_d = d * 16 + h4;
+                    const v4s x = load4(from + (at_d < a.dim ? at_d : 0u));
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; ++b)
+                        if (j0 + j < limit[b]) add_special<E>(o[b][d], 0, x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
         }
     }
-    if (t < a.dim) a.out[token * a.out_token + h * a.out_head + t] = E::down(l > 0 ? o / l : 0.0f);
-    if (a.lse && t == 0) a.lse[static_cast<uint64_t>(token) * a.heads + h] = l > 0 ? m + __logf(l) : -__builtin_inff();
+
+    // The waves' sums meet at their common maximum.
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        l[b] += __shfl_xor(l[b], 16, 64);
+        l[b] += __shfl_xor(l[b], 32, 64);
+        if (h == 0) {
+            s_m[wave][b * 16 + c16] = m[b];
+            s_l[wave][b * 16 + c16] = l[b];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        const uint32_t r = b * 16 + c16;
+        float top = NEG_INF;
+#pragma unroll
+        for (uint32_t w = 0; w < DC_WAVES; ++w) top = fmaxf(top, s_m[w][r]);
+        const float fix = m[b] == NEG_INF ? 0.0f : exp2_fast((m[b] - top) * c);
+        float* red = reinterpret_cast<float*>(s_mem) + (wave * 16 + c16) * RED;
+#pragma unroll
+        for (uint32_t d = 0; d < BLOCKS; ++d)
+            *reinterpret_cast<f32x4*>(red + d * 16 + h * 4) = m[b] == NEG_INF ? f32x4{0, 0, 0, 0} : o[b][d] * fix;
+        __syncthreads();
+        // 256 threads: 16 rows, 16 threads of a row, four dimensions at a time
+        const uint32_t mine = threadIdx.x / 16, row = t.row0 + b * 16 + mine;
+        float mt = NEG_INF, lt = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < DC_WAVES; ++w) mt = fmaxf(mt, s_m[w][b * 16 + mine]);
+#pragma unroll
+        for (uint32_t w = 0; w < DC_WAVES; ++w) {
+            const float mw = s_m[w][b * 16 + mine];
+            lt += mw == NEG_INF ? 0.0f : s_l[w][b * 16 + mine] * exp2_fast((mw - mt) * c);
+        }
+        const bool none = mt == NEG_INF;
+        const float part = none ? 0.0f : 1.0f / lt;
+        if (row < t.rows) {
+            const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
+            const uint64_t at = static_cast<uint64_t>(token) * a.heads + head;
+            const float lse2 = none ? NEG_INF : mt * c + __builtin_amdgcn_logf(lt);
+#pragma unroll
+            for (uint32_t d = (threadIdx.x % 16) * 4; d < DIM; d += 64) {
+                f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t w = 0; w < DC_WAVES; ++w)
+                    x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(s_mem) + (w * 16 + mine) * RED + d);
+                if (d < a.dim) store_row(a, E{}, split, at, token, head, d, x * part);
+            }
+            if (threadIdx.x % 16 == 0) store_lse(a, split, at, lse2);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- many rows: bound by the matrix units --------------------------------------------
+// A workgroup answers 128 QB rows, 32 QB of them a wave, over tiles of 64 keys
+// that all its waves read from LDS: the next tile's keys and values are in
+// flight to registers while this one's are used, and go to the other buffer
+// behind it.  Scores are transposed products (keys x rows) of 32x32x16 matrix
+// instructions; a row's probabilities then lie in the lanes that the second
+// product wants them in, if its 16 keys are taken in the order 4h..4h+3,
+// 8+4h..8+4h+3 for lane half h, and values are transposed on their way out of
+// LDS.  Rows of LDS are turned by pieces of 16 bytes so that neither the 32 rows
+// of a key fragment nor the four of a value's share banks.
+constexpr int TL_NT = 256;
+// Keys of a tile: 64, or 32 where longer rows would not leave room for the next tile's in registers.
+constexpr uint32_t tile_keys(uint32_t dim) { return dim <= 128 ? 64 : 32; }
+
+template <class E, uint32_t DIM, bool FULL, uint32_t QB>
+__global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 && DIM <= 128 ? 2 : 1))) void at_tiles(AttnArgs a)
+{
+    constexpr uint32_t STEPS = DIM / 16, BLOCKS = DIM / 32, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
+    constexpr uint32_t KEYS = tile_keys(DIM), HALVES = KEYS / 32;
+    constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << KEYS) - 1ull;
+    constexpr uint32_t PER = TL_NT / CHUNKS, LOADS = KEYS / PER;  // rows that the workgroup loads at once, and how often
+    constexpr uint32_t KTURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
+    __shared__ alignas(16) uint16_t s_k[2][KEYS * STRIDE];
+    __shared__ alignas(16) uint16_t s_v[2][KEYS * STRIDE];
+    __shared__ uint64_t s_koff[3][KEYS], s_voff[3][KEYS], s_there[3];
+    __shared__ uint32_t s_bad[3], s_most[TL_NT / 64], s_least[TL_NT / 64];
+    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
+    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
+    // a request's last rows see the most keys: they go first
+    const Tile t = find_tile(a, a.n_tiles - 1 - rest / a.splits, 128 * QB);
+    if (t.row0 >= t.rows) return;
+    const uint32_t group = a.heads / a.kv_heads, keys = keys_of(a, t);
+    uint32_t limit[QB], most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+    for (uint32_t b = 0; b < QB; ++b) {
+        const uint32_t row = t.row0 + (wave * QB + b) * 32 + c32;
+        limit[b] = row < t.rows ? limit_of(a, t, keys, row / group) : 0u;
+        most = max(most, limit[b]);
+        if (row < t.rows) least = min(least, limit[b]);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
+        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
+    }
+    const uint32_t wave_most = __builtin_amdgcn_readfirstlane(most);
+    const uint32_t wave_least = __builtin_amdgcn_readfirstlane(least);
+    if (lane == 0) {
+        s_most[wave] = wave_most;
+        s_least[wave] = wave_least;
+    }
+    if (threadIdx.x < 3) s_bad[threadIdx.x] = 0;
+    __syncthreads();
+    most = 0;
+    least = 0xFFFFFFFFu;
+#pragma unroll
+    for (uint32_t w = 0; w < TL_NT / 64; ++w) {
+        most = max(most, s_most[w]);
+        least = min(least, s_least[w]);
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+    const uint32_t k0 = split * a.split_len;
+    const uint32_t k1 = split + 1 == a.splits ? most : min(most, k0 + a.split_len);
+    if (split > 0 && k0 >= most) {
+        if (threadIdx.x < 128 * QB && t.row0 + threadIdx.x < t.rows) {
+            const uint32_t row = t.row0 + threadIdx.x;
+            a.part_lse[split * a.rows_total + static_cast<uint64_t>(t.token0 + row / group) * a.heads + kh * group + row % group] = NEG_INF;
+        }
+        return;
+    }
+
+    v8s q[QB][STEPS];
+#pragma unroll
+    for (uint32_t b = 0; b < QB; ++b)
+#pragma unroll
+        for (uint32_t s = 0; s < STEPS; ++s)
+            q[b][s] = load_query(a, t, t.row0 + (wave * QB + b) * 32 + c32, kh, s * 16 + h * 8);
+    f32x16 o[QB][BLOCKS];
+    float m[QB], l[QB];
+#pragma unroll
+    for (uint32_t b = 0; b < QB; ++b) {
+        m[b] = NEG_INF;
+        l[b] = 0.0f;
+#pragma unroll
+        for (uint32_t d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
+    }
+    const float c = score_scale(a);
+    const uint16_t* kp = a.k + kh * a.k_head;
+    const uint16_t* vp = a.v + kh * a.v_head;
+    const uint32_t lrow = threadIdx.x / CHUNKS, lchunk = threadIdx.x % CHUNKS;
+    const uint32_t lcol = lchunk * 8 < a.dim ? lchunk * 8 : 0u;
+
+    v8s rk[LOADS], rv[LOADS];
+    // The first wave looks up where tile i's keys and values are.
+    auto look_up = [&](uint32_t i) {
+        const uint32_t j = k0 + i * KEYS + lane;
+        return lane < KEYS && j < k1 ? slot_of(a, t.request, j) : -1;
+    };
+    auto note = [&](uint32_t i, int32_t slot) {
+        const uint32_t at = i % 3;
+        if (lane < KEYS) {
+            s_koff[at][lane] = offset_of(slot, a.page_lg, a.k_page, a.k_slot);
+            s_voff[at][lane] = offset_of(slot, a.page_lg, a.v_page, a.v_slot);
+        }
+        const uint64_t there = __ballot(slot >= 0);
+        if (lane == 0) {
+            s_there[at] = there;
+            s_bad[at] = 0;
+        }
+    };
+    auto load_tile = [&](uint32_t i) {
+        const uint32_t at = i % 3;
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x) rk[x] = load8(kp + s_koff[at][x * PER + lrow] + lcol);
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x) rv[x] = load8(vp + s_voff[at][x * PER + lrow] + lcol);
+    };
+    auto is_whole = [&](uint32_t i, uint64_t there) { return there == ALL && k0 + (i + 1) * KEYS <= least; };
+    auto store_tile = [&](uint32_t i) {
+        const uint64_t there = s_there[i % 3];
+        const bool whole = is_whole(i, there);
+        uint16_t* sk = s_k[i & 1];
+        uint16_t* sv = s_v[i & 1];
+        uint64_t bad = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t r = x * PER + lrow;
+            *reinterpret_cast<v8s*>(sk + r * STRIDE + (lchunk ^ (r & KTURN)) * 8) = rk[x];
+            v8s y = rv[x];
+            if (!whole) {
+                y = zero_unless((there >> r) & 1u, y);
+                bad |= __ballot(has_special(y, E::EXP));
+                y = without_special(y, E::EXP);
+            }
+            const uint32_t turn = (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2;
+            *reinterpret_cast<v8s*>(sv + r * STRIDE + (lchunk ^ turn) * 8) = y;
+        }
+        if (bad && lane == 0) s_bad[i % 3] = 1;
+    };
+
+    const uint32_t n_tiles = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
+    if (n_tiles) {
+        if (wave == 0) {
+            note(0, look_up(0));
+            note(1, look_up(1));
+        }
+        __syncthreads();
+        load_tile(0);
+        store_tile(0);
+        __syncthreads();
+    }
+    for (uint32_t i = 0; i < n_tiles; ++i) {
+        const bool more = i + 1 < n_tiles;
+        int32_t ahead = -1;
+        if (more) {
+            load_tile(i + 1);
+            if (wave == 0) ahead = look_up(i + 2);
+        }
+        const uint32_t j0 = k0 + i * KEYS;
+        if (j0 < wave_most) {
+            const uint64_t there = s_there[i % 3];
+            const uint16_t* sk = s_k[i & 1];
+            const uint16_t* sv = s_v[i & 1];
+            f32x16 s[QB][HALVES];
+#pragma unroll
+            for (uint32_t b = 0; b < QB; ++b)
+#pragma unroll
+                for (uint32_t x = 0; x < HALVES; ++x)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[b][x][e] = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < HALVES; ++x)
+#pragma unroll
+                for (uint32_t st = 0; st < STEPS; ++st) {
+                    const v8s k = load8(sk + (x * 32 + c32) * STRIDE + ((st * 2 + h) ^ (c32 & KTURN)) * 8);
+#pragma unroll
+                    for (uint32_t b = 0; b < QB; ++b) s[b][x] = E::mfma32(k, q[b][st], s[b][x]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (there != ALL || j0 + KEYS > wave_least) {
+#pragma unroll
+                for (uint32_t b = 0; b < QB; ++b) {
+                    const int32_t left = static_cast<int32_t>(limit[b] - j0 - h * 4);
+#pragma unroll
+                    for (uint32_t x = 0; x < HALVES; ++x) {
+                        const uint32_t on = static_cast<uint32_t>(there >> (x * 32)) >> (h * 4);
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) {
+                            const uint32_t at = (e / 4) * 8 + e % 4;
+                            const bool see = static_cast<int32_t>(x * 32 + at) < left & (on & (1u << at)) != 0;
+                            s[b][x][e] = see ? s[b][x][e] : NEG_INF;
+                        }
+                    }
+                }
+            }
+            v8s p[QB][2 * HALVES];
+#pragma unroll
+            for (uint32_t b = 0; b < QB; ++b) {
+                float top = NEG_INF;
+#pragma unroll
+                for (uint32_t x = 0; x < HALVES; ++x)
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e) top = fmaxf(top, s[b][x][e]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (__any((top - m[b]) * c > LAG)) {  // m starts at -inf; NaN where both are
+                    const float now = fmaxf(m[b], top);
+                    const float fix = now == NEG_INF ? 1.0f : exp2_fast((m[b] - now) * c);
+                    m[b] = now;
+                    l[b] *= fix;
+#pragma unroll
+                    for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] *= fix;
+                }
+                const float mc = m[b] == NEG_INF ? 0.0f : m[b] * c;
+#pragma unroll
+                for (uint32_t x = 0; x < HALVES; ++x)
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e) {
+                        const float y = exp2_fast(__builtin_fmaf(s[b][x][e], c, -mc));
+                        l[b] += y;
+                        p[b][x * 2 + e / 8][e % 8] = static_cast<short>(E::down(y));
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (uint32_t st = 0; st < 2 * HALVES; ++st)
+#pragma unroll
+                for (uint32_t d = 0; d < BLOCKS; ++d) {
+                    const uint32_t i16 = lane & 15u, r = st * 16 + h * 4 + i16 / 4;
+                    const uint32_t chunk = d * 4 + ((lane >> 4) & 1u) * 2 + (i16 & 3u) / 2;
+                    const uint32_t turn = (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2;
+                    const uint16_t* at = sv + r * STRIDE + (chunk ^ turn) * 8 + (i16 & 1u) * 4;
+                    const v8s x = join(lds_tr(at), lds_tr(at + 8 * STRIDE));
+#pragma unroll
+                    for (uint32_t b = 0; b < QB; ++b) o[b][d] = E::mfma32(x, p[b][st], o[b][d]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (s_bad[i % 3]) {
+                // Infinite and NaN values, left out of LDS so that rows which do
+                // not see their keys are spared, reach the rows that do.
+                for (uint32_t j = 0; j < KEYS; ++j) {
+                    if (!((there >> j) & 1ull)) continue;
+                    const uint16_t* from = vp + s_voff[i % 3][j];
+                    uint32_t h4 = h * 4;
+                    asm volatile("" : "+v"(h4));  // the addresses are worked out here, not kept in registers
+#pragma unroll
+                    for (uint32_t d = 0; d < BLOCKS; ++d)
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; e += 4) {
+                            const uint32_t at_d = d * 32 + e * 2 + h4;
+                            const v4s x = load4(from + (at_d < a.dim ? at_d : 0u));
+#pragma unroll
+                            for (uint32_t b = 0; b < QB; ++b)
+                                if (j0 + j < limit[b]) add_special<E>(o[b][d], e, x);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
+            }
+        }
+        if (more) {
+            store_tile(i + 1);
+            if (wave == 0) note(i + 2, ahead);
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (uint32_t b = 0; b < QB; ++b) {
+        const uint32_t row = t.row0 + (wave * QB + b) * 32 + c32;
+        const float lt = l[b] + __shfl_xor(l[b], 32, 64);
+        const bool none = m[b] == NEG_INF;
+        const float part = none ? 0.0f : 1.0f / lt;
+        if (row >= t.rows) continue;
+        const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
+        const uint64_t at = static_cast<uint64_t>(token) * a.heads + head;
+#pragma unroll
+        for (uint32_t d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (uint32_t e = 0; e < 16; e += 4) {
+                const uint32_t at_d = d * 32 + e * 2 + h * 4;
+                const f32x4 x = {o[b][d][e], o[b][d][e + 1], o[b][d][e + 2], o[b][d][e + 3]};
+                if (at_d < a.dim) store_row(a, E{}, split, at, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
+            }
+        if (h == 0) store_lse(a, split, at, none ? NEG_INF : m[b] * c + __builtin_amdgcn_logf(lt));
+    }
+}
+
+// ---- the ranges' results joined: a wave per row ---------------------------------------
+constexpr int JN_NT = 256;
+
+template <class E>
+__global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a)
+{
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (JN_NT / 64) + (threadIdx.x >> 6);
+    if (row >= a.rows_total) return;
+    const uint32_t lane = __lane_id();
+    float top = NEG_INF, own[AT_SPLITS / 64];
+#pragma unroll
+    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
+        const uint32_t s = i * 64 + lane;
+        own[i] = s < a.splits ? a.part_lse[s * a.rows_total + row] : NEG_INF;
+        top = fmaxf(top, own[i]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const bool none = top == NEG_INF;
+    float sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
+        own[i] = none ? 0.0f : exp2_fast(own[i] - top);
+        sum += own[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const float part = none ? 0.0f : 1.0f / sum;
+    const uint32_t d = lane * 4;
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
+        for (uint32_t s = i * 64; s < min(a.splits, i * 64 + 64); ++s) {
+            const float w = __shfl(own[i], static_cast<int>(s & 63u), 64);
+            if (w != 0.0f && d < a.dim)
+                x += w * *reinterpret_cast<const f32x4*>(a.part_o + (s * a.rows_total + row) * a.dim + d);
+        }
+    }
+    const uint32_t token = static_cast<uint32_t>(row / a.heads), head = static_cast<uint32_t>(row % a.heads);
+    x *= part;
+    if (d < a.dim) {
+        const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
+                       static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
+        *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
+    }
+    if (a.lse && lane == 0) a.lse[row] = none ? NEG_INF : (top + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+template <class E, uint32_t DIM, bool FULL>
+int launch_full(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
+{
+    if (per_wave == 0) {
+        CR_TIMED("at_tiles", s);
+        at_tiles<E, DIM, FULL, 1><<<grid, TL_NT, 0, s>>>(a);
+    } else {
+        CR_TIMED("at_rows", s);
+        if constexpr (DIM <= 128) {
+            if (per_wave == 2) {
+                at_rows<E, DIM, FULL, 2><<<grid, DC_NT, 0, s>>>(a);
+                CR_LAUNCH_CHECK();
+                return CR_OK;
+            }
+        }
+        at_rows<E, DIM, FULL, 1><<<grid, DC_NT, 0, s>>>(a);
+    }
+    CR_LAUNCH_CHECK();
+    return CR_OK;
+}
+
+template <class E, uint32_t DIM>
+int launch_dim(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
+{
+    return a.dim == DIM ? launch_full<E, DIM, true>(a, per_wave, grid, s) : launch_full<E, DIM, false>(a, per_wave, grid, s);
+}
+
+template <class E>
+int launch_attention(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
+{
+    if (a.dim <= 64)
+        CR_RET((launch_dim<E, 64>(a, per_wave, grid, s)));
+    else if (a.dim <= 96)
+        CR_RET((launch_dim<E, 96>(a, per_wave, grid, s)));
+    else if (a.dim <= 128)
+        CR_RET((launch_dim<E, 128>(a, per_wave, grid, s)));
+    else if (a.dim <= 192)
+        CR_RET((launch_dim<E, 192>(a, per_wave, grid, s)));
+    else
+        CR_RET((launch_dim<E, 256>(a, per_wave, grid, s)));
+    if (a.splits > 1) {
+        CR_TIMED("at_join", s);
+        at_join<E><<<static_cast<unsigned>((a.rows_total + JN_NT / 64 - 1) / (JN_NT / 64)), JN_NT, 0, s>>>(a);
+        CR_LAUNCH_CHECK();
+    }
+    return CR_OK;
 }
 
 }  // namespace
@@ -184,7 +1003,7 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     a.starts = p.d_starts;
     a.kv_len = p.d_kv_len;
     a.table = p.d_table;
-    a.cols = p.table_cols;
+    a.cols = cache->n_pages ? p.table_cols : 0;  // without a page nothing is there to be seen
     a.table_stride = p.table_stride;
     a.sel = p.d_sel;
     a.sel_stride = p.sel_stride;
@@ -193,11 +1012,39 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     a.scale = p.scale;
     a.causal = p.causal;
     hipStream_t s = as_stream(stream);
-    CR_TIMED("at_simple", s);
-    if (cache->dtype == CR_F16)
-        at_simple<Half><<<dim3(p.n_tokens, p.n_heads), AT_NT, 0, s>>>(a);
-    else
-        at_simple<BHalf><<<dim3(p.n_tokens, p.n_heads), AT_NT, 0, s>>>(a);
-    CR_LAUNCH_CHECK();
-    return CR_OK;
+
+    // Rows of a request that share a key head, as far as the caller says.
+    const uint32_t group = p.n_heads / cache->n_heads, cus = num_cus();
+    const uint64_t typical = p.max_new ? p.max_new : (p.n_tokens + std::max(1u, p.n_requests) - 1) / std::max(1u, p.n_requests);
+    const uint64_t rows = typical * group;
+    // blocks of 16 rows (two of long rows do not fit the registers), or tiles
+    const uint32_t per_wave = rows <= 16 ? 1 : rows <= 32 && a.dim <= 128 ? 2 : 0;
+    const uint32_t most = per_wave ? 16 * per_wave : 128;
+    a.rows_total = static_cast<uint64_t>(p.n_tokens) * p.n_heads;
+    const uint64_t tiles = static_cast<uint64_t>(p.n_tokens) * group / most + p.n_requests + 2;
+    const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
+    // Enough workgroups to fill the card, of at least a few tiles of keys each.
+    const uint64_t busy = std::max<uint64_t>(1, (rows + most - 1) / most * p.n_requests * cache->n_heads);
+    const uint64_t want = per_wave ? 12ull * cus : 2ull * cus;
+    const uint32_t step = per_wave ? DC_KEYS * DC_WAVES : 256;
+    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({AT_SPLITS, want / busy, (max_kv + step - 1) / step}));
+    a.split_len = static_cast<uint32_t>(((max_kv + splits - 1) / splits + step - 1) / step * step);
+    splits = a.split_len ? std::max<uint64_t>(1, (max_kv + a.split_len - 1) / a.split_len) : 1;
+    a.splits = static_cast<uint32_t>(splits);
+    if (a.rows_total >> 32 || (tiles * splits * cache->n_heads) >> 31) {
+        set_error("cr_paged_attention: too many rows for one call");
+        return CR_ERR_UNSUPPORTED;
+    }
+    a.n_tiles = static_cast<uint32_t>(tiles);
+    Scratch sc;
+    if (splits > 1) {
+        Carver cv;
+        const size_t o_part = cv.add(splits * a.rows_total * a.dim * 4), o_lse = cv.add(splits * a.rows_total * 4);
+        CR_RET(sc.alloc(cv.total, s));
+        a.part_o = sc.at<float>(o_part);
+        a.part_lse = sc.at<float>(o_lse);
+    }
+    const uint32_t grid = static_cast<uint32_t>(tiles * splits * cache->n_heads);
+    if (cache->dtype == CR_F16) return launch_attention<Half>(a, per_wave, grid, s);
+    return launch_attention<BHalf>(a, per_wave, grid, s);
 }
