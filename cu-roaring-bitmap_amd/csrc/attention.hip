@@ -13,7 +13,6 @@ namespace crimpl {
 namespace {
 
 constexpr uint32_t AT_DIM_MAX = 256;
-constexpr uint32_t AT_SPLITS = 128;  // ranges of keys at most
 
 struct AttnArgs {
     const uint16_t* q;
@@ -37,12 +36,15 @@ struct AttnArgs {
     const int32_t* limits;
     float scale;
     uint32_t causal;
-    // The launch: tiles of rows by ranges of split_len keys (the last one takes
-    // all that are left), results of several ranges kept in fp32 to be joined.
-    uint32_t n_tiles, splits, split_len;
-    uint64_t rows_total;  // n_tokens * heads
-    float* part_o;        // [splits][rows_total][dim]
-    float* part_lse;      // [splits][rows_total], base 2
+    // The launch.  With `share` 0, a workgroup takes a tile of rows and all of its
+    // keys.  Otherwise the tiles' keys are cut into about `share` ranges of even
+    // length, a workgroup each for every key head; their results, in fp32, are
+    // joined by another kernel.
+    uint32_t n_tiles;
+    uint32_t share, step, least_len;  // ranges are of a multiple of `step` keys, at least least_len
+    uint2* ranges;    // [n_tiles] a tile's first range and how many it has
+    float* part_o;    // [ranges][key heads][rows of a tile][dim]
+    float* part_lse;  // [ranges][key heads][rows of a tile], base 2
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -107,6 +109,11 @@ __device__ __forceinline__ v4s lds_tr(const uint16_t* p)
 __device__ __forceinline__ v8s join(v4s x, v4s y) { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 __device__ __forceinline__ v8s load8(const uint16_t* p) { return *reinterpret_cast<const v8s*>(p); }
+// The same, for data that no other workgroup reads.
+__device__ __forceinline__ v8s load8_once(const uint16_t* p)
+{
+    return __builtin_nontemporal_load(reinterpret_cast<const v8s*>(p));
+}
 __device__ __forceinline__ v4s load4(const uint16_t* p) { return *reinterpret_cast<const v4s*>(p); }
 
 // Whether any of eight values is infinite or NaN, and the eight with zeros for those.
@@ -150,64 +157,139 @@ __device__ __forceinline__ void add_special(V& o, uint32_t i, v4s x)
 __device__ __forceinline__ int32_t segment_start(const AttnArgs& a, uint32_t i)
 {
     if (i == 0) return 0;
+    if (i > a.n_requests + 1) return static_cast<int32_t>(a.n_tokens);
     return min(max(a.starts[i - 1], 0), static_cast<int32_t>(a.n_tokens));
 }
 
-// A tile of `most` rows of a segment; row m is token m / group, head m % group
-// of those that share a key head.
-struct Tile {
-    uint32_t request;
-    bool real;        // a request's, not the tokens' outside
-    int32_t token0;   // the segment's first token
-    uint32_t tokens;
-    uint32_t row0, rows;  // rows [row0, rows) are this tile's and those behind it
-};
-
-// Tile `id` of the launch: segment i's tiles start at i + (its first token's
-// row) / most, which leaves each of them room for all of its rows.  A wave
-// searches together, 64 segments at a time.
-__device__ __forceinline__ Tile find_tile(const AttnArgs& a, uint32_t id, uint32_t most)
+// How many keys a segment's request has.
+__device__ __forceinline__ uint32_t segment_keys(const AttnArgs& a, uint32_t i)
 {
-    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
-    auto base = [&](uint32_t i) {
-        return static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(segment_start(a, i))) * group / most) + i;
-    };
-    uint32_t lo = 0, len = n;  // base(lo) <= id
-    while (len > 1) {
-        const uint32_t step = (len + 63) / 64, i = lo + lane * step;
-        const bool at_most = lane * step < len && base(i) <= id;
-        const uint32_t c = static_cast<uint32_t>(__popcll(__ballot(at_most)));
-        const uint32_t from = c ? (c - 1) * step : 0u;
-        lo += from;
-        len = min(step, len - from);
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    Tile t;
-    t.real = lo > 0 && lo <= a.n_requests;
-    t.request = t.real ? lo - 1 : 0;
-    t.token0 = segment_start(a, lo);
-    const int32_t end = lo + 1 < n ? segment_start(a, lo + 1) : static_cast<int32_t>(a.n_tokens);
-    t.tokens = static_cast<uint32_t>(max(end - t.token0, 0));
-    t.rows = t.tokens * group;
-    t.row0 = (id - base(lo)) * most;
-    return t;
-}
-
-// How many of its request's keys a token sees.
-__device__ __forceinline__ uint32_t keys_of(const AttnArgs& a, const Tile& t)
-{
-    if (!t.real) return 0;
-    const int32_t n = a.sel ? a.sel_len[t.request] : a.kv_len[t.request];
+    if (i == 0 || i > a.n_requests) return 0;
+    const int32_t n = a.sel ? a.sel_len[i - 1] : a.kv_len[i - 1];
     const uint64_t room = static_cast<uint64_t>(a.cols) << a.page_lg;
     return n <= 0 ? 0u : static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
 }
 
-__device__ __forceinline__ uint32_t limit_of(const AttnArgs& a, const Tile& t, uint32_t keys, uint32_t token)
+// Segment i's tiles of `most` rows are numbered from here, which leaves each
+// segment room for all of its rows.
+__device__ __forceinline__ uint32_t tile_base(uint32_t i, int32_t start, uint32_t group, uint32_t most)
 {
-    if (!t.real || !a.causal) return keys;
+    return static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(start)) * group / most) + i;
+}
+
+// A workgroup's work: a tile of rows of a segment (row m is token m / group,
+// head m % group of those that share a key head) and a range of its keys.
+struct Work {
+    uint32_t request;
+    bool real;            // a request's, not the tokens' outside
+    int32_t token0;       // the segment's first token
+    uint32_t tokens;
+    uint32_t row0, rows;  // rows [row0, rows) are this tile's and those behind it
+    uint32_t keys;        // the request's
+    uint32_t k0, k1;      // the range
+    uint32_t range;       // its number
+    bool none;            // nothing to do
+};
+
+__device__ __forceinline__ uint32_t lane_value(uint32_t x, uint32_t lane)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), static_cast<int>(lane)));
+}
+
+// What the workgroup's number `id` stands for.  A wave looks at 64 segments at
+// a time, each lane at one.
+__device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32_t most)
+{
+    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
+    uint32_t lo = 0, start = 0, end = 0, keys = 0, tile = 0, count = 1, part = 0, at = 0;
+    if (a.share == 0) {
+        for (uint32_t len = n; len > 64;) {  // base(lo) <= id < base(lo + len)
+            const uint32_t step = (len + 63) / 64, i = lo + lane * step;
+            const bool below = lane * step < len && tile_base(i, segment_start(a, i), group, most) <= id;
+            const uint32_t from = (max(1u, static_cast<uint32_t>(__popcll(__ballot(below)))) - 1) * step;
+            lo += from;
+            len = min(step, len - from);
+        }
+        const uint32_t i = min(lo + lane, n);
+        start = static_cast<uint32_t>(segment_start(a, i));
+        end = static_cast<uint32_t>(segment_start(a, i + 1));
+        keys = segment_keys(a, i);
+        const uint32_t base = tile_base(i, static_cast<int32_t>(start), group, most);
+        at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lo + lane < n && base <= id)))) - 1;
+        lo += at;
+        tile = id - lane_value(base, at);
+    } else {
+        // ranges of one length for all, so that about `share` of them result
+        uint64_t all = 0;
+#pragma unroll 2
+        for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+            const uint32_t i = min(i0 + lane, n);
+            start = static_cast<uint32_t>(segment_start(a, i));
+            end = static_cast<uint32_t>(segment_start(a, i + 1));
+            keys = segment_keys(a, i);
+            const uint32_t rows = end > start ? (end - start) * group : 0u;
+            all += static_cast<uint64_t>((rows + most - 1) / most) * keys;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
+        const uint64_t even = (all + a.share - 1) / a.share;
+        const uint32_t len = max(a.least_len, static_cast<uint32_t>(min(even, static_cast<uint64_t>(0x7FFFFFFF))));
+        uint32_t before = 0;
+        bool found = false;
+        for (uint32_t i0 = 0; i0 < n && !found; i0 += 64) {
+            const uint32_t i = min(i0 + lane, n);
+            if (n > 64) {
+                start = static_cast<uint32_t>(segment_start(a, i));
+                end = static_cast<uint32_t>(segment_start(a, i + 1));
+                keys = segment_keys(a, i);
+            }
+            const uint32_t rows = end > start ? (end - start) * group : 0u;
+            count = max(1u, (keys + len - 1) / len);
+            const uint32_t mine = i < n ? (rows + most - 1) / most * count : 0u;
+            const uint32_t upto = before + wave_incl_scan(mine);
+            const uint64_t past = __ballot(upto > id);
+            if (past) {
+                at = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(past))) - 1;
+                lo = i0 + at;
+                part = id - lane_value(upto - mine, at);
+                count = lane_value(count, at);
+                tile = part / count;
+                part %= count;
+                found = true;
+            }
+            before = lane_value(upto, 63);
+        }
+        if (!found) {
+            Work w{};
+            w.none = true;
+            return w;
+        }
+    }
+    Work w;
+    w.real = lo > 0 && lo <= a.n_requests;
+    w.request = w.real ? lo - 1 : 0;
+    w.token0 = static_cast<int32_t>(lane_value(start, at));
+    const uint32_t last = lane_value(end, at);
+    w.tokens = last > static_cast<uint32_t>(w.token0) ? last - static_cast<uint32_t>(w.token0) : 0u;
+    w.rows = w.tokens * group;
+    w.row0 = tile * most;
+    w.keys = lane_value(keys, at);
+    w.none = w.row0 >= w.rows;
+    w.range = id;
+    const uint32_t even = ((w.keys + count - 1) / count + a.step - 1) / a.step * a.step;
+    w.k0 = part * even;
+    w.k1 = part + 1 == count ? w.keys : min(w.keys, w.k0 + even);
+    if (a.share && part == 0 && threadIdx.x == 0)
+        a.ranges[tile_base(lo, w.token0, group, most) + tile] = make_uint2(id, count);
+    return w;
+}
+
+__device__ __forceinline__ uint32_t limit_of(const AttnArgs& a, const Work& t, uint32_t token)
+{
+    if (!t.real || !a.causal) return t.keys;
     const int64_t at = a.sel ? static_cast<int64_t>(a.limits[t.token0 + token])
                              : static_cast<int64_t>(a.kv_len[t.request]) - t.tokens + token + 1;
-    return static_cast<uint32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), at)));
+    return static_cast<uint32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(t.keys), at)));
 }
 
 // The cache slot of the request's key j < keys, -1 where its page is outside
@@ -233,7 +315,7 @@ __device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, ui
 
 // Queries come in with the sign of the scale, so that the largest product is
 // the largest score.
-__device__ __forceinline__ v8s load_query(const AttnArgs& a, const Tile& t, uint32_t row, uint32_t kh, uint32_t d)
+__device__ __forceinline__ v8s load_query(const AttnArgs& a, const Work& t, uint32_t row, uint32_t kh, uint32_t d)
 {
     const uint32_t group = a.heads / a.kv_heads;
     v8s x = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -250,13 +332,14 @@ __device__ __forceinline__ float score_scale(const AttnArgs& a)
 }
 
 // A row's four dimensions from d: rounded into the output, or kept in fp32
-// where another kernel joins the ranges of keys.
+// where another kernel joins the ranges of keys.  `place` numbers the rows of
+// the ranges' results.
 template <class E>
-__device__ __forceinline__ void store_row(const AttnArgs& a, E, uint32_t split, uint64_t row, uint32_t token,
-                                          uint32_t head, uint32_t d, f32x4 x)
+__device__ __forceinline__ void store_row(const AttnArgs& a, E, uint64_t place, uint32_t token, uint32_t head,
+                                          uint32_t d, f32x4 x)
 {
-    if (a.splits > 1) {
-        *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows_total + row) * a.dim + d) = x;
+    if (a.share) {
+        *reinterpret_cast<f32x4*>(a.part_o + place * a.dim + d) = x;
     } else {
         const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
                        static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
@@ -265,12 +348,12 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, E, uint32_t split, 
 }
 
 // lse2: base 2
-__device__ __forceinline__ void store_lse(const AttnArgs& a, uint32_t split, uint64_t row, float lse2)
+__device__ __forceinline__ void store_lse(const AttnArgs& a, uint64_t place, uint32_t token, uint32_t head, float lse2)
 {
-    if (a.splits > 1)
-        a.part_lse[split * a.rows_total + row] = lse2;
+    if (a.share)
+        a.part_lse[place] = lse2;
     else if (a.lse)
-        a.lse[row] = lse2 * LN2;
+        a.lse[static_cast<uint64_t>(token) * a.heads + head] = lse2 * LN2;
 }
 
 // ---- few rows: bound by reading keys and values ------------------------------------
@@ -298,19 +381,20 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     constexpr uint32_t PER = 64 / CHUNKS, LOADS = DC_KEYS / PER;  // values: rows an instruction covers, instructions
     constexpr uint32_t RED = DIM + 4;
     // the values' tiles, and in the end the waves' sums
-    constexpr uint32_t BYTES = DC_WAVES * (DC_KEYS * STRIDE * 2 > 16 * RED * 4 ? DC_KEYS * STRIDE * 2 : 16 * RED * 4);
+    constexpr uint32_t KTURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
+    constexpr uint32_t BYTES = DC_WAVES * (DC_KEYS * STRIDE * 4 > 16 * RED * 4 ? DC_KEYS * STRIDE * 4 : 16 * RED * 4);
     __shared__ alignas(16) char s_mem[BYTES];
+    __shared__ uint64_t s_at[DC_WAVES][2][DC_KEYS];  // where a tile's keys and values are
     __shared__ float s_m[DC_WAVES][16 * NB], s_l[DC_WAVES][16 * NB];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c16 = lane & 15u, h = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
-    const Tile t = find_tile(a, rest / a.splits, 16 * NB);
-    if (t.row0 >= t.rows) return;
-    const uint32_t group = a.heads / a.kv_heads, keys = keys_of(a, t);
+    const uint32_t kh = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+    const Work t = find_work(a, blockIdx.x / a.kv_heads, 16 * NB);
+    if (t.none) return;
     uint32_t limit[NB], most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
         const uint32_t row = t.row0 + b * 16 + c16;
-        limit[b] = row < t.rows ? limit_of(a, t, keys, row / group) : 0u;
+        limit[b] = row < t.rows ? limit_of(a, t, row / group) : 0u;
         most = max(most, limit[b]);
         if (row < t.rows) least = min(least, limit[b]);
     }
@@ -321,13 +405,10 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     }
     most = __builtin_amdgcn_readfirstlane(most);
     least = __builtin_amdgcn_readfirstlane(least);
-    const uint32_t k0 = split * a.split_len;
-    const uint32_t k1 = split + 1 == a.splits ? most : min(most, k0 + a.split_len);
-    if (split > 0 && k0 >= most) {
-        if (threadIdx.x < 16 * NB && t.row0 + threadIdx.x < t.rows) {
-            const uint32_t row = t.row0 + threadIdx.x;
-            a.part_lse[split * a.rows_total + static_cast<uint64_t>(t.token0 + row / group) * a.heads + kh * group + row % group] = NEG_INF;
-        }
+    const uint32_t k0 = t.k0, k1 = min(most, t.k1);
+    const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * (16 * NB);  // of the tile's first row
+    if (a.share && k0 >= k1) {
+        if (threadIdx.x < 16 * NB) a.part_lse[place0 + threadIdx.x] = NEG_INF;
         return;
     }
 
@@ -346,44 +427,42 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] = f32x4{0, 0, 0, 0};
     }
     const float c = score_scale(a);
-    const uint16_t* kp = a.k + kh * a.k_head;
-    const uint16_t* vp = a.v + kh * a.v_head;
-    uint16_t* lds = reinterpret_cast<uint16_t*>(s_mem) + wave * DC_KEYS * STRIDE;
+    uint16_t* lds_k = reinterpret_cast<uint16_t*>(s_mem) + wave * 2 * DC_KEYS * STRIDE;
+    uint16_t* lds = lds_k + DC_KEYS * STRIDE;
     const uint32_t vrow = lane / CHUNKS, vchunk = lane % CHUNKS;
     const uint32_t vcol = vchunk * 8 < a.dim ? vchunk * 8 : 0u;
+    const uint16_t* kp = a.k + kh * a.k_head + vcol;
+    const uint16_t* vp = a.v + kh * a.v_head + vcol;
 
-    v8s k[2][STEPS], v[LOADS];
+    v8s k[LOADS], v[LOADS];
     // Lane j < 32 (and j + 32) looks after key j of a tile.
     auto slots = [&](uint32_t j0) {
         const uint32_t j = j0 + (lane & 31u);
         return j < k1 ? slot_of(a, t.request, j) : -1;
     };
-    auto load_keys = [&](int32_t slot) {
-#pragma unroll
-        for (uint32_t b = 0; b < 2; ++b) {
-            const int32_t at = __shfl(slot, static_cast<int>(b * 16 + c16), 64);
-            const uint16_t* p = kp + offset_of(at, a.page_lg, a.k_page, a.k_slot);
-#pragma unroll
-            for (uint32_t s = 0; s < STEPS; ++s) {
-                const uint32_t d = s * 32 + h * 8;
-                k[b][s] = load8(p + (FULL || d < a.dim ? d : 0u));
-            }
+    auto note = [&](int32_t slot) {
+        if (lane < DC_KEYS) {
+            s_at[wave][0][lane] = offset_of(slot, a.page_lg, a.k_page, a.k_slot);
+            s_at[wave][1][lane] = offset_of(slot, a.page_lg, a.v_page, a.v_slot);
         }
+        wave_lds_fence();
     };
-    auto load_values = [&](int32_t slot) {
+    auto load_keys = [&]() {
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) {
-            const int32_t at = __shfl(slot, static_cast<int>(i * PER + vrow), 64);
-            v[i] = load8(vp + offset_of(at, a.page_lg, a.v_page, a.v_slot) + vcol);
-        }
+        for (uint32_t i = 0; i < LOADS; ++i) k[i] = load8_once(kp + s_at[wave][0][i * PER + vrow]);
+    };
+    auto load_values = [&]() {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) v[i] = load8_once(vp + s_at[wave][1][i * PER + vrow]);
     };
 
     uint32_t j0 = k0 + wave * DC_KEYS;
     int32_t slot = -1, next = -1;
     if (j0 < k1) {
         slot = slots(j0);
-        load_keys(slot);
-        load_values(slot);
+        note(slot);
+        load_keys();
+        load_values();
         next = slots(j0 + DC_WAVES * DC_KEYS);
     }
     for (; j0 < k1; j0 += DC_WAVES * DC_KEYS) {
@@ -396,12 +475,23 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 #pragma unroll
             for (uint32_t x = 0; x < 2; ++x) s[b][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            const uint32_t r = i * PER + vrow;
+            *reinterpret_cast<v8s*>(lds_k + r * STRIDE + (vchunk ^ (r & KTURN)) * 8) = k[i];
+        }
+        if (more) {
+            note(next);
+            load_keys();
+        }
+        wave_lds_fence();
+#pragma unroll
         for (uint32_t x = 0; x < 2; ++x)
 #pragma unroll
-            for (uint32_t st = 0; st < STEPS; ++st)
+            for (uint32_t st = 0; st < STEPS; ++st) {
+                const v8s y = load8(lds_k + (x * 16 + c16) * STRIDE + ((st * 4 + h) ^ (c16 & KTURN)) * 8);
 #pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) s[b][x] = E::mfma16(k[x][st], q[b][st], s[b][x]);
-        if (more) load_keys(next);
+                for (uint32_t b = 0; b < NB; ++b) s[b][x] = E::mfma16(y, q[b][st], s[b][x]);
+            }
 
         v8s p[NB];
 #pragma unroll
@@ -462,7 +552,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         const int32_t was = slot;
         slot = next;
         if (more) {
-            load_values(next);
+            load_values();
             next = slots(j0 + 2 * DC_WAVES * DC_KEYS);
         }
         wave_lds_fence();
@@ -482,7 +572,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
             for (uint32_t j = 0; j < DC_KEYS; ++j) {
                 const int32_t at = __shfl(was, static_cast<int>(j), 64);
                 if (at < 0) continue;
-                const uint16_t* from = vp + offset_of(at, a.page_lg, a.v_page, a.v_slot);
+                const uint16_t* from = a.v + kh * a.v_head + offset_of(at, a.page_lg, a.v_page, a.v_slot);
                 uint32_t h4 = h * 4;
                 asm volatile("" : "+v"(h4));  // the addresses are worked out here, not kept in registers
 #pragma unroll
@@ -535,7 +625,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         const float part = none ? 0.0f : 1.0f / lt;
         if (row < t.rows) {
             const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
-            const uint64_t at = static_cast<uint64_t>(token) * a.heads + head;
+            const uint64_t place = place0 + b * 16 + mine;
             const float lse2 = none ? NEG_INF : mt * c + __builtin_amdgcn_logf(lt);
 #pragma unroll
             for (uint32_t d = (threadIdx.x % 16) * 4; d < DIM; d += 64) {
@@ -543,9 +633,9 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 #pragma unroll
                 for (uint32_t w = 0; w < DC_WAVES; ++w)
                     x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(s_mem) + (w * 16 + mine) * RED + d);
-                if (d < a.dim) store_row(a, E{}, split, at, token, head, d, x * part);
+                if (d < a.dim) store_row(a, E{}, place, token, head, d, x * part);
             }
-            if (threadIdx.x % 16 == 0) store_lse(a, split, at, lse2);
+            if (threadIdx.x % 16 == 0) store_lse(a, place, token, head, lse2);
         }
         __syncthreads();
     }
@@ -578,16 +668,15 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     __shared__ uint64_t s_koff[3][KEYS], s_voff[3][KEYS], s_there[3];
     __shared__ uint32_t s_bad[3], s_most[TL_NT / 64], s_least[TL_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
-    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
+    const uint32_t kh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     // a request's last rows see the most keys: they go first
-    const Tile t = find_tile(a, a.n_tiles - 1 - rest / a.splits, 128 * QB);
-    if (t.row0 >= t.rows) return;
-    const uint32_t group = a.heads / a.kv_heads, keys = keys_of(a, t);
+    const Work t = find_work(a, a.share ? id : a.n_tiles - 1 - id, 128 * QB);
+    if (t.none) return;
     uint32_t limit[QB], most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
     for (uint32_t b = 0; b < QB; ++b) {
         const uint32_t row = t.row0 + (wave * QB + b) * 32 + c32;
-        limit[b] = row < t.rows ? limit_of(a, t, keys, row / group) : 0u;
+        limit[b] = row < t.rows ? limit_of(a, t, row / group) : 0u;
         most = max(most, limit[b]);
         if (row < t.rows) least = min(least, limit[b]);
     }
@@ -613,13 +702,10 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     }
     most = __builtin_amdgcn_readfirstlane(most);
     least = __builtin_amdgcn_readfirstlane(least);
-    const uint32_t k0 = split * a.split_len;
-    const uint32_t k1 = split + 1 == a.splits ? most : min(most, k0 + a.split_len);
-    if (split > 0 && k0 >= most) {
-        if (threadIdx.x < 128 * QB && t.row0 + threadIdx.x < t.rows) {
-            const uint32_t row = t.row0 + threadIdx.x;
-            a.part_lse[split * a.rows_total + static_cast<uint64_t>(t.token0 + row / group) * a.heads + kh * group + row % group] = NEG_INF;
-        }
+    const uint32_t k0 = t.k0, k1 = min(most, t.k1);
+    const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * (128 * QB);  // of the tile's first row
+    if (a.share && k0 >= k1) {
+        if (threadIdx.x < 128 * QB) a.part_lse[place0 + threadIdx.x] = NEG_INF;
         return;
     }
 
@@ -827,65 +913,80 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
         const float part = none ? 0.0f : 1.0f / lt;
         if (row >= t.rows) continue;
         const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
-        const uint64_t at = static_cast<uint64_t>(token) * a.heads + head;
+        const uint64_t place = place0 + (wave * QB + b) * 32 + c32;
 #pragma unroll
         for (uint32_t d = 0; d < BLOCKS; ++d)
 #pragma unroll
             for (uint32_t e = 0; e < 16; e += 4) {
                 const uint32_t at_d = d * 32 + e * 2 + h * 4;
                 const f32x4 x = {o[b][d][e], o[b][d][e + 1], o[b][d][e + 2], o[b][d][e + 3]};
-                if (at_d < a.dim) store_row(a, E{}, split, at, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
+                if (at_d < a.dim) store_row(a, E{}, place, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
             }
-        if (h == 0) store_lse(a, split, at, none ? NEG_INF : m[b] * c + __builtin_amdgcn_logf(lt));
+        if (h == 0) store_lse(a, place, token, head, none ? NEG_INF : m[b] * c + __builtin_amdgcn_logf(lt));
     }
 }
 
-// ---- the ranges' results joined: a wave per row ---------------------------------------
+// ---- the ranges' results joined: a workgroup per row -----------------------------------
 constexpr int JN_NT = 256;
 
-template <class E>
-__global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a)
+// TPR threads take four dimensions each of a range's row, JN_NT / TPR ranges at a time.
+template <class E, uint32_t TPR>
+__global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
 {
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (JN_NT / 64) + (threadIdx.x >> 6);
-    if (row >= a.rows_total) return;
-    const uint32_t lane = __lane_id();
-    float top = NEG_INF, own[AT_SPLITS / 64];
-#pragma unroll
-    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
-        const uint32_t s = i * 64 + lane;
-        own[i] = s < a.splits ? a.part_lse[s * a.rows_total + row] : NEG_INF;
-        top = fmaxf(top, own[i]);
+    constexpr uint32_t SLOTS = JN_NT / TPR;
+    __shared__ float s_o[SLOTS][TPR * 4 + 4], s_sum[SLOTS];
+    const uint32_t token = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = __lane_id();
+    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2;
+    // the token's segment: the last that starts at or before it
+    uint32_t lo = 0, len = n, start = 0;
+    while (true) {
+        const uint32_t step = (len + 63) / 64, i = lo + min(lane * step, len);
+        start = static_cast<uint32_t>(segment_start(a, i));
+        const uint32_t at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lane * step < len && start <= token)))) - 1;
+        start = lane_value(start, at);
+        lo += at * step;
+        if (step == 1) break;
+        len = min(step, len - at * step);
     }
+    const uint32_t row = (token - start) * group + head % group;
+    const uint2 range = a.ranges[tile_base(lo, static_cast<int32_t>(start), group, most) + row / most];
+    auto place = [&](uint32_t r) {
+        return (static_cast<uint64_t>(range.x + r) * a.kv_heads + head / group) * most + row % most;
+    };
+    float top = NEG_INF;
+    for (uint32_t r = lane; r < range.y; r += 64) top = fmaxf(top, a.part_lse[place(r)]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const bool none = top == NEG_INF;
+    const uint32_t slot = threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
     float sum = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
-        own[i] = none ? 0.0f : exp2_fast(own[i] - top);
-        sum += own[i];
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float part = none ? 0.0f : 1.0f / sum;
-    const uint32_t d = lane * 4;
     f32x4 x = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t r = slot; r < range.y; r += SLOTS) {
+        const uint64_t at = place(r);
+        const float lse = a.part_lse[at], w = lse == NEG_INF ? 0.0f : exp2_fast(lse - top);
+        sum += w;
+        // a range without a visible key has left nothing to read
+        if (lse != NEG_INF && d < a.dim) x += w * *reinterpret_cast<const f32x4*>(a.part_o + at * a.dim + d);
+    }
+    *reinterpret_cast<f32x4*>(&s_o[slot][d]) = x;
+    if (threadIdx.x % TPR == 0) s_sum[slot] = sum;
+    __syncthreads();
+    if (slot == 0) {
 #pragma unroll
-    for (uint32_t i = 0; i < AT_SPLITS / 64; ++i) {
-        for (uint32_t s = i * 64; s < min(a.splits, i * 64 + 64); ++s) {
-            const float w = __shfl(own[i], static_cast<int>(s & 63u), 64);
-            if (w != 0.0f && d < a.dim)
-                x += w * *reinterpret_cast<const f32x4*>(a.part_o + (s * a.rows_total + row) * a.dim + d);
+        for (uint32_t i = 1; i < SLOTS; ++i) {
+            x += *reinterpret_cast<const f32x4*>(&s_o[i][d]);
+            sum += s_sum[i];
         }
+        x *= none ? 0.0f : 1.0f / sum;
+        if (d < a.dim) {
+            const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
+                           static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
+            *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
+        }
+        if (a.lse && threadIdx.x == 0)
+            a.lse[blockIdx.x] = none ? NEG_INF : (top + __builtin_amdgcn_logf(sum)) * LN2;
     }
-    const uint32_t token = static_cast<uint32_t>(row / a.heads), head = static_cast<uint32_t>(row % a.heads);
-    x *= part;
-    if (d < a.dim) {
-        const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
-                       static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
-        *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
-    }
-    if (a.lse && lane == 0) a.lse[row] = none ? NEG_INF : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 template <class E, uint32_t DIM, bool FULL>
@@ -928,9 +1029,15 @@ int launch_attention(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStr
         CR_RET((launch_dim<E, 192>(a, per_wave, grid, s)));
     else
         CR_RET((launch_dim<E, 256>(a, per_wave, grid, s)));
-    if (a.splits > 1) {
+    if (a.share) {
         CR_TIMED("at_join", s);
-        at_join<E><<<static_cast<unsigned>((a.rows_total + JN_NT / 64 - 1) / (JN_NT / 64)), JN_NT, 0, s>>>(a);
+        const uint32_t rows = a.n_tokens * a.heads, most = per_wave ? 16 * per_wave : 128;
+        if (a.dim <= 64)
+            at_join<E, 16><<<rows, JN_NT, 0, s>>>(a, most);
+        else if (a.dim <= 128)
+            at_join<E, 32><<<rows, JN_NT, 0, s>>>(a, most);
+        else
+            at_join<E, 64><<<rows, JN_NT, 0, s>>>(a, most);
         CR_LAUNCH_CHECK();
     }
     return CR_OK;
@@ -1020,31 +1127,41 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     // blocks of 16 rows (two of long rows do not fit the registers), or tiles
     const uint32_t per_wave = rows <= 16 ? 1 : rows <= 32 && a.dim <= 128 ? 2 : 0;
     const uint32_t most = per_wave ? 16 * per_wave : 128;
-    a.rows_total = static_cast<uint64_t>(p.n_tokens) * p.n_heads;
     const uint64_t tiles = static_cast<uint64_t>(p.n_tokens) * group / most + p.n_requests + 2;
-    const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
-    // Enough workgroups to fill the card, of at least a few tiles of keys each.
-    const uint64_t busy = std::max<uint64_t>(1, (rows + most - 1) / most * p.n_requests * cache->n_heads);
-    const uint64_t want = per_wave ? 12ull * cus : 2ull * cus;
-    const uint32_t step = per_wave ? DC_KEYS * DC_WAVES : 256;
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({AT_SPLITS, want / busy, (max_kv + step - 1) / step}));
-    a.split_len = static_cast<uint32_t>(((max_kv + splits - 1) / splits + step - 1) / step * step);
-    splits = a.split_len ? std::max<uint64_t>(1, (max_kv + a.split_len - 1) / a.split_len) : 1;
-    a.splits = static_cast<uint32_t>(splits);
-    if (a.rows_total >> 32 || (tiles * splits * cache->n_heads) >> 31) {
+    if ((tiles * cache->n_heads) >> 31 || (static_cast<uint64_t>(p.n_tokens) * p.n_heads) >> 31) {
         set_error("cr_paged_attention: too many rows for one call");
         return CR_ERR_UNSUPPORTED;
     }
     a.n_tiles = static_cast<uint32_t>(tiles);
+    // Few tiles are cut into ranges of even length, as many as the card holds
+    // workgroups at once (4 requests of 32768 keys, 128 dimensions: 2 workgroups a
+    // CU 94 us, 3 109, 1 103).  More of them, or requests long enough to lag behind
+    // the others, into about four rounds of workgroups, of no short ranges (64 of
+    // up to 16384 keys: uncut 398 us, two rounds 348, four 338, twelve 370); else
+    // reading the lengths and joining cost more than they even out (256 of up to
+    // 1024 keys: uncut 110 us, cut 160; of up to 4096 372 and 389; 48 of up to 2048
+    // with 16 heads of 64 dimensions 53 and 60).
+    const uint64_t tiles_in_all = (rows + most - 1) / most * std::max(1u, p.n_requests);
+    const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
+    const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= 128 ? 2u : 1u) * cus / cache->n_heads + 1;
+    const bool few = 2 * tiles_in_all <= held;
+    const bool cut = few || (per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held);
+    a.step = per_wave ? DC_KEYS * DC_WAVES : 64;
+    a.least_len = !few ? 1024 : per_wave ? DC_KEYS * DC_WAVES : 256;
+    uint64_t ranges = tiles;
     Scratch sc;
-    if (splits > 1) {
+    if (cut && max_kv > a.least_len) {
+        a.share = static_cast<uint32_t>(few ? held - tiles_in_all : 4 * held);
+        ranges += a.share;
+        const uint64_t part_rows = ranges * cache->n_heads * most;
         Carver cv;
-        const size_t o_part = cv.add(splits * a.rows_total * a.dim * 4), o_lse = cv.add(splits * a.rows_total * 4);
+        const size_t o_part = cv.add(part_rows * a.dim * 4), o_lse = cv.add(part_rows * 4), o_at = cv.add(tiles * 8);
         CR_RET(sc.alloc(cv.total, s));
         a.part_o = sc.at<float>(o_part);
         a.part_lse = sc.at<float>(o_lse);
+        a.ranges = sc.at<uint2>(o_at);
     }
-    const uint32_t grid = static_cast<uint32_t>(tiles * splits * cache->n_heads);
+    const uint32_t grid = static_cast<uint32_t>(ranges * cache->n_heads);
     if (cache->dtype == CR_F16) return launch_attention<Half>(a, per_wave, grid, s);
     return launch_attention<BHalf>(a, per_wave, grid, s);
 }
