@@ -544,53 +544,65 @@ def download_batch(b: RoaringBatch) -> SimpleNamespace:
 
 # ---- serving language models (stream-ordered, no synchronisation) ---------------
 F32, F16, BF16 = 0, 1, 2
-_TYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
+_names = {}
 
 
-def _typed(t, *types: str) -> int:
-    """The library's code of a tensor's type, one of `types` (all of them if none is named)."""
-    name = str(t.dtype)
-    if name not in _TYPES or (types and name not in types):
-        raise CrError(CR_ERR_INVALID, f"a tensor of {name} where one of {', '.join(types or _TYPES)} is taken")
-    return _TYPES[name]
+def _type_name(t) -> str:
+    name = _names.get(t.dtype)
+    if name is None:
+        name = _names[t.dtype] = str(t.dtype).split(".")[-1]
+    return name
+
+
+def _typed(t) -> int:
+    """The library's code of a tensor's type."""
+    code = _TYPES.get(_type_name(t))
+    if code is None:
+        raise CrError(CR_ERR_INVALID, f"a tensor of {t.dtype} where one of {', '.join(_TYPES)} is taken")
+    return code
 
 
 def _array(t, name: str, dtype: str, shape) -> int:
-    """The address of a contiguous CUDA tensor of this type and shape (None: any extent)."""
-    if (str(t.dtype) != "torch." + dtype or not t.is_cuda or not t.is_contiguous() or len(shape) != t.dim()
-            or any(n is not None and n != m for n, m in zip(shape, t.shape))):
-        raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} CUDA tensor of shape "
-                                      f"{tuple('*' if n is None else n for n in shape)} is taken, not "
-                                      f"{t.dtype} {tuple(t.shape)}")
-    return _dptr(t)
+    """The address of a contiguous CUDA tensor of this type and shape (an int: one axis of any extent from there)."""
+    if _type_name(t) == dtype and t.is_cuda and t.is_contiguous() and (
+            t.dim() == 1 if isinstance(shape, int) else t.shape == shape):
+        return t.data_ptr()
+    raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} CUDA tensor of shape "
+                                  f"{'(any,)' if isinstance(shape, int) else tuple(shape)} is taken, not "
+                                  f"{t.dtype} {tuple(t.shape)}")
 
 
 def _table(t, n_requests: int):
     """(address, columns, row stride) of a block table, rows of which may lie apart."""
-    if str(t.dtype) != "torch.int32" or not t.is_cuda or t.dim() != 2 or t.shape[0] != n_requests or (
-            t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
-        raise CrError(CR_ERR_INVALID, f"block table: an int32 CUDA tensor of {n_requests} rows is taken")
-    return _dptr(t), t.shape[1], t.stride(0)
+    if _type_name(t) == "int32" and t.is_cuda and t.dim() == 2:
+        (rows, cols), (stride, one) = t.shape, t.stride()
+        if rows == n_requests and (one == 1 or cols <= 1) and stride >= cols:
+            return t.data_ptr(), cols, stride
+    raise CrError(CR_ERR_INVALID, f"block table: an int32 CUDA tensor of {n_requests} rows is taken, not {t.dtype} "
+                                  f"{tuple(t.shape)}")
 
 
 def _rows(t, name: str, like):
     """(address, token stride, head stride) of a [tokens, heads, dim] tensor of `like`'s shape and type."""
-    if t.dtype != like.dtype or not t.is_cuda or t.shape != like.shape or t.dim() != 3 or (
-            t.shape[2] > 1 and t.stride(2) != 1):
-        raise CrError(CR_ERR_INVALID, f"{name}: a {like.dtype} CUDA tensor of shape {tuple(like.shape)} with "
-                                      f"contiguous rows is taken, not {t.dtype} {tuple(t.shape)}")
-    return _dptr(t), t.stride(0), t.stride(1)
+    if t.dtype == like.dtype and t.is_cuda and t.shape == like.shape and t.dim() == 3:
+        token, head, one = t.stride()
+        if one == 1 or t.shape[2] <= 1:
+            return t.data_ptr(), token, head
+    raise CrError(CR_ERR_INVALID, f"{name}: a {like.dtype} CUDA tensor of shape {tuple(like.shape)} with "
+                                  f"contiguous rows is taken, not {t.dtype} {tuple(t.shape)}")
 
 
 def paged_cache(d_k, d_v) -> PagedCache:
     """A cache of [pages, page size, heads, dim] keys and values (any strides with contiguous rows)."""
-    if d_k.dim() != 4 or d_k.shape != d_v.shape or d_k.dtype != d_v.dtype or not (d_k.is_cuda and d_v.is_cuda) or (
-            d_k.shape[3] > 1 and (d_k.stride(3) != 1 or d_v.stride(3) != 1)):
-        raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] "
-                                      "with contiguous rows are taken")
-    pages, size, heads, dim = d_k.shape
-    return PagedCache(_dptr(d_k), _dptr(d_v), d_k.stride(0), d_k.stride(1), d_k.stride(2), d_v.stride(0),
-                      d_v.stride(1), d_v.stride(2), pages, size, heads, dim, _typed(d_k))
+    if d_k.dim() == 4 and d_k.shape == d_v.shape and d_k.dtype == d_v.dtype and d_k.is_cuda and d_v.is_cuda:
+        (kp, ks, kh, k1), (vp, vs, vh, v1) = d_k.stride(), d_v.stride()
+        pages, size, heads, dim = d_k.shape
+        if (k1 == 1 and v1 == 1) or dim <= 1:
+            return PagedCache(d_k.data_ptr(), d_v.data_ptr(), kp, ks, kh, vp, vs, vh, pages, size, heads, dim,
+                              _typed(d_k))
+    raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] with "
+                                  "contiguous rows are taken")
 
 
 def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d_new, d_table, d_slots, d_starts,
@@ -604,10 +616,10 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
     table, cols, stride = _table(d_table, n)
     _check(load().cr_paged_plan(C.byref(free_pages), n_pages, page_size, _array(d_cached, "cached", "int32", (n,)),
                                 _array(d_new, "new", "int32", (n,)), n, table, cols, stride,
-                                _array(d_slots, "slots", "int64", (None,)), d_slots.numel(),
+                                _array(d_slots, "slots", "int64", 0), d_slots.numel(),
                                 _array(d_starts, "starts", "int32", (n + 1,)),
                                 _array(d_kv_len, "kv_len", "int32", (n,)),
-                                _array(d_taken, "taken", "int32", (None,)), d_taken.numel(),
+                                _array(d_taken, "taken", "int32", 0), d_taken.numel(),
                                 _array(d_counts, "counts", "int32", (3,)), _stream(stream)), "paged_plan")
 
 
@@ -642,7 +654,7 @@ def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: in
                                   _array(d_starts, "starts", "int32", (n + 1,)),
                                   _array(d_kv_len, "kv_len", "int32", (n,)), n, d_limits.numel(), sel, sel_stride,
                                   _array(d_sel_len, "sel_len", "int32", (n,)),
-                                  _array(d_limits, "limits", "int32", (None,)), _stream(stream)), "paged_select")
+                                  _array(d_limits, "limits", "int32", 0), _stream(stream)), "paged_select")
 
 
 def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_out, scale: Optional[float] = None,
@@ -657,23 +669,21 @@ def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_ou
         raise CrError(CR_ERR_INVALID, f"paged_attention: {d_k_cache.dtype} queries [tokens, heads, {cache.head_dim}] "
                                       f"are taken, not {d_q.dtype} {tuple(d_q.shape)}")
     n, (tokens, heads, dim) = d_kv_len.numel(), d_q.shape
-    a = PagedAttentionArgs()
-    a.q, a.q_token_stride, a.q_head_stride = _rows(d_q, "q", d_q)
-    a.out, a.out_token_stride, a.out_head_stride = _rows(d_out, "out", d_q)
-    a.lse = _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else None
-    a.n_tokens, a.n_heads, a.n_requests = tokens, heads, n
-    a.d_starts = _array(d_starts, "starts", "int32", (n + 1,))
-    a.d_kv_len = _array(d_kv_len, "kv_len", "int32", (n,))
-    a.d_table, a.table_cols, a.table_stride = _table(d_table, n)
+    q, q_token, q_head = _rows(d_q, "q", d_q)
+    out, out_token, out_head = _rows(d_out, "out", d_q)
+    table, cols, stride = _table(d_table, n)
+    sel, room, sel_stride, sel_len, limits = None, 0, 0, None, None
     if selection is not None:
-        sel, sel_len, limits = selection
-        a.d_sel, room, a.sel_stride = _table(sel, n)
-        if room < a.table_cols * cache.page_size:
+        sel, room, sel_stride = _table(selection[0], n)
+        if room < cols * cache.page_size:
             raise CrError(CR_ERR_INVALID, "paged_attention: a row of sel holds cols * page_size slots")
-        a.d_sel_len = _array(sel_len, "sel_len", "int32", (n,))
-        a.d_limits = _array(limits, "limits", "int32", (tokens,))
-    a.scale = dim ** -0.5 if scale is None else scale
-    a.causal, a.max_new, a.max_kv = causal, max_new, max_kv
+        sel_len = _array(selection[1], "sel_len", "int32", (n,))
+        limits = _array(selection[2], "limits", "int32", (tokens,))
+    a = PagedAttentionArgs(q, q_token, q_head, out, out_token, out_head,
+                           _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else None,
+                           tokens, heads, n, _array(d_starts, "starts", "int32", (n + 1,)),
+                           _array(d_kv_len, "kv_len", "int32", (n,)), table, cols, stride, sel, sel_stride, sel_len,
+                           limits, dim ** -0.5 if scale is None else scale, causal, max_new, max_kv)
     _check(load().cr_paged_attention(C.byref(a), C.byref(cache), _stream(stream)), "paged_attention")
 
 
@@ -686,14 +696,17 @@ def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_ls
     k = d_out_scores.shape[1]
     if not d_scores.is_cuda or (v > 1 and d_scores.stride(2) != 1):
         raise CrError(CR_ERR_INVALID, "beam_select: a CUDA tensor of scores with contiguous rows is taken")
-    words, bits, stride = (v + 31) // 32, None, 0
-    if allowed is not None and not isinstance(allowed, GpuRoaring):
+    words, bitmap, bits, stride = (v + 31) // 32, None, None, 0
+    if isinstance(allowed, GpuRoaring):
+        bitmap = C.byref(allowed)
+    elif allowed is not None:
         bits = _array(allowed, "allowed", "int32", (words,) if allowed.dim() == 1 else (b, w, words))
         stride = 0 if allowed.dim() == 1 else words
-    _check(load().cr_beam_select(_dptr(d_scores), _typed(d_scores), b, w, v, d_scores.stride(0), d_scores.stride(1),
+    per_batch, per_beam, _ = d_scores.stride()
+    _check(load().cr_beam_select(_dptr(d_scores), _typed(d_scores), b, w, v, per_batch, per_beam,
                                  _array(d_cum, "cum", "float32", (b, w)),
                                  _array(d_lse, "lse", "float32", (b, w)) if d_lse is not None else None,
-                                 C.byref(allowed) if isinstance(allowed, GpuRoaring) else None, bits, stride, k,
+                                 bitmap, bits, stride, k,
                                  _array(d_out_scores, "out_scores", "float32", (b, k)),
                                  _array(d_out_tokens, "out_tokens", "int32", (b, k)),
                                  _array(d_out_parents, "out_parents", "int32", (b, k)), _stream(stream)),
@@ -712,7 +725,7 @@ def beam_reorder(d_src, d_parents, d_dst, d_len=None, stream=None):
         raise CrError(CR_ERR_INVALID, f"beam_reorder: contiguous CUDA states [{b}, {w}, ...] into [{b}, {k}, ...]")
     if d_len is not None and d_src.dim() < 3:
         raise CrError(CR_ERR_INVALID, "beam_reorder: lengths count along the states' third extent")
-    row = d_src[0, 0].numel() * d_src.element_size() if b and w else 0
+    row = d_src.numel() * d_src.element_size() // max(1, b * w)
     unit = row // max(1, d_src.shape[2]) if d_len is not None else 0
     _check(load().cr_beam_reorder(_dptr(d_src), _array(d_parents, "parents", "int32", (b, k)), b, w, k, row, row, row,
                                   _array(d_len, "len", "int32", (b, w)) if d_len is not None else None, unit,
