@@ -152,6 +152,14 @@ __device__ __forceinline__ void add_special(V& o, uint32_t i, v4s x)
         if ((static_cast<uint16_t>(x[e]) & E::EXP) == E::EXP) o[i + e] += E::up(static_cast<uint16_t>(x[e]));
 }
 
+// 16 bytes a lane from memory to LDS, lane after lane from `to`, which is the
+// same for the wave.
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
+{
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
 // Segment i of the tokens: request i - 1's; the first and the last one hold
 // those before and behind all requests, which see nothing.
 __device__ __forceinline__ int32_t segment_start(const AttnArgs& a, uint32_t i)
@@ -294,17 +302,18 @@ __device__ __forceinline__ uint32_t limit_of(const AttnArgs& a, const Work& t, u
 
 // The cache slot of the request's key j < keys, -1 where its page is outside
 // the cache.
-__device__ __forceinline__ int32_t slot_of(const AttnArgs& a, uint32_t request, uint32_t j)
+// In two steps, so that nothing waits for the load before it has to: what the
+// selection or the table holds for it, and what that says.
+__device__ __forceinline__ int32_t look_up(const AttnArgs& a, uint32_t request, uint32_t j)
 {
-    int32_t slot;
-    if (a.sel) {
-        slot = a.sel[request * a.sel_stride + j];
-    } else {
-        const int32_t page = a.table[request * a.table_stride + (j >> a.page_lg)];
-        if (static_cast<uint32_t>(page) >= a.n_pages) return -1;
-        slot = (page << a.page_lg) + static_cast<int32_t>(j & ((1u << a.page_lg) - 1u));
-    }
-    return (static_cast<uint32_t>(slot) >> a.page_lg) < a.n_pages ? slot : -1;
+    return a.sel ? a.sel[request * a.sel_stride + j] : a.table[request * a.table_stride + (j >> a.page_lg)];
+}
+
+__device__ __forceinline__ int32_t slot_of(const AttnArgs& a, int32_t found, uint32_t j)
+{
+    const uint32_t page = a.sel ? static_cast<uint32_t>(found) >> a.page_lg : static_cast<uint32_t>(found);
+    const uint32_t slot = a.sel ? static_cast<uint32_t>(found) : (page << a.page_lg) + (j & ((1u << a.page_lg) - 1u));
+    return page < a.n_pages ? static_cast<int32_t>(slot) : -1;
 }
 
 __device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, uint64_t page_stride, uint64_t slot_stride)
@@ -436,9 +445,10 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 
     v8s k[LOADS], v[LOADS];
     // Lane j < 32 (and j + 32) looks after key j of a tile.
-    auto slots = [&](uint32_t j0) {
+    auto find = [&](uint32_t j0) { return look_up(a, t.request, min(j0 + (lane & 31u), k1 - 1)); };
+    auto slots = [&](uint32_t j0, int32_t found) {
         const uint32_t j = j0 + (lane & 31u);
-        return j < k1 ? slot_of(a, t.request, j) : -1;
+        return j < k1 ? slot_of(a, found, j) : -1;
     };
     auto note = [&](int32_t slot) {
         if (lane < DC_KEYS) {
@@ -457,13 +467,13 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     };
 
     uint32_t j0 = k0 + wave * DC_KEYS;
-    int32_t slot = -1, next = -1;
+    int32_t slot = -1, next = -1, found = -1;
     if (j0 < k1) {
-        slot = slots(j0);
+        slot = slots(j0, find(j0));
         note(slot);
+        found = find(j0 + DC_WAVES * DC_KEYS);
         load_keys();
         load_values();
-        next = slots(j0 + DC_WAVES * DC_KEYS);
     }
     for (; j0 < k1; j0 += DC_WAVES * DC_KEYS) {
         const uint64_t there = __ballot(slot >= 0);
@@ -480,6 +490,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
             *reinterpret_cast<v8s*>(lds_k + r * STRIDE + (vchunk ^ (r & KTURN)) * 8) = k[i];
         }
         if (more) {
+            next = slots(j0 + DC_WAVES * DC_KEYS, found);
             note(next);
             load_keys();
         }
@@ -552,8 +563,8 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         const int32_t was = slot;
         slot = next;
         if (more) {
+            found = find(j0 + 2 * DC_WAVES * DC_KEYS);
             load_values();
-            next = slots(j0 + 2 * DC_WAVES * DC_KEYS);
         }
         wave_lds_fence();
 #pragma unroll
@@ -643,9 +654,8 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 
 // ---- many rows: bound by the matrix units --------------------------------------------
 // A workgroup answers 128 QB rows, 32 QB of them a wave, over tiles of 64 keys
-// that all its waves read from LDS: the next tile's keys and values are in
-// flight to registers while this one's are used, and go to the other buffer
-// behind it.  Scores are transposed products (keys x rows) of 32x32x16 matrix
+// that all its waves read from LDS, where the next tile's keys and values arrive
+// meanwhile without passing through registers.  Scores are transposed products (keys x rows) of 32x32x16 matrix
 // instructions; a row's probabilities then lie in the lanes that the second
 // product wants them in, if its 16 keys are taken in the order 4h..4h+3,
 // 8+4h..8+4h+3 for lane half h, and values are transposed on their way out of
@@ -663,8 +673,9 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << KEYS) - 1ull;
     constexpr uint32_t PER = TL_NT / CHUNKS, LOADS = KEYS / PER;  // rows that the workgroup loads at once, and how often
     constexpr uint32_t KTURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
-    __shared__ alignas(16) uint16_t s_k[2][KEYS * STRIDE];
-    __shared__ alignas(16) uint16_t s_v[2][KEYS * STRIDE];
+    // separate arrays: what is read is not what is being loaded
+    __shared__ alignas(16) uint16_t s_k0[KEYS * STRIDE], s_k1[KEYS * STRIDE];
+    __shared__ alignas(16) uint16_t s_v0[KEYS * STRIDE], s_v1[KEYS * STRIDE];
     __shared__ uint64_t s_koff[3][KEYS], s_voff[3][KEYS], s_there[3];
     __shared__ uint32_t s_bad[3], s_most[TL_NT / 64], s_least[TL_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
@@ -729,17 +740,14 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     const float c = score_scale(a);
     const uint16_t* kp = a.k + kh * a.k_head;
     const uint16_t* vp = a.v + kh * a.v_head;
-    const uint32_t lrow = threadIdx.x / CHUNKS, lchunk = threadIdx.x % CHUNKS;
-    const uint32_t lcol = lchunk * 8 < a.dim ? lchunk * 8 : 0u;
+    const uint32_t lrow = threadIdx.x / CHUNKS, lpos = threadIdx.x % CHUNKS;
+    const uint32_t wave_row = __builtin_amdgcn_readfirstlane(wave) * (64 / CHUNKS);
 
-    v8s rk[LOADS], rv[LOADS];
     // The first wave looks up where tile i's keys and values are.
-    auto look_up = [&](uint32_t i) {
-        const uint32_t j = k0 + i * KEYS + lane;
-        return lane < KEYS && j < k1 ? slot_of(a, t.request, j) : -1;
-    };
-    auto note = [&](uint32_t i, int32_t slot) {
-        const uint32_t at = i % 3;
+    auto find = [&](uint32_t i) { return look_up(a, t.request, min(k0 + i * KEYS + lane % KEYS, k1 - 1)); };
+    auto note = [&](uint32_t i, int32_t found) {
+        const uint32_t at = i % 3, j = k0 + i * KEYS + lane;
+        const int32_t slot = lane < KEYS && j < k1 ? slot_of(a, found, j) : -1;
         if (lane < KEYS) {
             s_koff[at][lane] = offset_of(slot, a.page_lg, a.k_page, a.k_slot);
             s_voff[at][lane] = offset_of(slot, a.page_lg, a.v_page, a.v_slot);
@@ -750,32 +758,34 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
             s_bad[at] = 0;
         }
     };
-    auto load_tile = [&](uint32_t i) {
+    auto v_turn = [](uint32_t r) { return (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2; };
+    // Each lane's 16 bytes go straight to the wave's next 1 KiB of LDS; which of a
+    // row's pieces a lane names turns the row.  Pieces behind the head dimension
+    // repeat the first one: they meet zero queries, and their columns are not stored.
+    auto load_tile = [&](uint32_t i, uint16_t* sk, uint16_t* sv) {
         const uint32_t at = i % 3;
 #pragma unroll
-        for (uint32_t x = 0; x < LOADS; ++x) rk[x] = load8(kp + s_koff[at][x * PER + lrow] + lcol);
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t r = x * PER + lrow, d = (lpos ^ (r & KTURN)) * 8;
+            load_to_lds(kp + s_koff[at][r] + (d < a.dim ? d : 0u), sk + (x * PER + wave_row) * STRIDE);
+        }
 #pragma unroll
-        for (uint32_t x = 0; x < LOADS; ++x) rv[x] = load8(vp + s_voff[at][x * PER + lrow] + lcol);
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t r = x * PER + lrow, d = (lpos ^ v_turn(r)) * 8;
+            load_to_lds(vp + s_voff[at][r] + (d < a.dim ? d : 0u), sv + (x * PER + wave_row) * STRIDE);
+        }
     };
-    auto is_whole = [&](uint32_t i, uint64_t there) { return there == ALL && k0 + (i + 1) * KEYS <= least; };
-    auto store_tile = [&](uint32_t i) {
-        const uint64_t there = s_there[i % 3];
-        const bool whole = is_whole(i, there);
-        uint16_t* sk = s_k[i & 1];
-        uint16_t* sv = s_v[i & 1];
+    // Values of keys that no row sees become zeros, and, in a tile that some rows
+    // see and others do not, infinite and NaN ones too.
+    auto mend_tile = [&](uint32_t i, uint64_t there, uint16_t* sv) {
         uint64_t bad = 0;
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow;
-            *reinterpret_cast<v8s*>(sk + r * STRIDE + (lchunk ^ (r & KTURN)) * 8) = rk[x];
-            v8s y = rv[x];
-            if (!whole) {
-                y = zero_unless((there >> r) & 1u, y);
-                bad |= __ballot(has_special(y, E::EXP));
-                y = without_special(y, E::EXP);
-            }
-            const uint32_t turn = (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2;
-            *reinterpret_cast<v8s*>(sv + r * STRIDE + (lchunk ^ turn) * 8) = y;
+            uint16_t* at = sv + r * STRIDE + lpos * 8;
+            const v8s y = zero_unless((there >> r) & 1u, load8(at));
+            bad |= __ballot(has_special(y, E::EXP));
+            *reinterpret_cast<v8s*>(at) = without_special(y, E::EXP);
         }
         if (bad && lane == 0) s_bad[i % 3] = 1;
     };
@@ -783,26 +793,29 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     const uint32_t n_tiles = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
     if (n_tiles) {
         if (wave == 0) {
-            note(0, look_up(0));
-            note(1, look_up(1));
+            const int32_t first = find(0), second = find(1);
+            note(0, first);
+            note(1, second);
         }
         __syncthreads();
-        load_tile(0);
-        store_tile(0);
-        __syncthreads();
+        load_tile(0, s_k0, s_v0);
     }
-    for (uint32_t i = 0; i < n_tiles; ++i) {
+    // One tile, from `sk` and `sv`, while the next one comes into the other two.
+    auto tile = [&](uint32_t i, uint16_t* sk, uint16_t* sv, uint16_t* next_k, uint16_t* next_v) {
+        __syncthreads();  // this tile is there, and nobody reads the last one any more
         const bool more = i + 1 < n_tiles;
         int32_t ahead = -1;
         if (more) {
-            load_tile(i + 1);
-            if (wave == 0) ahead = look_up(i + 2);
+            if (wave == 0) ahead = find(i + 2);
+            load_tile(i + 1, next_k, next_v);
         }
         const uint32_t j0 = k0 + i * KEYS;
+        const uint64_t there = s_there[i % 3];
+        if (!(there == ALL && j0 + KEYS <= least)) {
+            mend_tile(i, there, sv);
+            __syncthreads();
+        }
         if (j0 < wave_most) {
-            const uint64_t there = s_there[i % 3];
-            const uint16_t* sk = s_k[i & 1];
-            const uint16_t* sv = s_v[i & 1];
             f32x16 s[QB][HALVES];
 #pragma unroll
             for (uint32_t b = 0; b < QB; ++b)
@@ -869,8 +882,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
                 for (uint32_t d = 0; d < BLOCKS; ++d) {
                     const uint32_t i16 = lane & 15u, r = st * 16 + h * 4 + i16 / 4;
                     const uint32_t chunk = d * 4 + ((lane >> 4) & 1u) * 2 + (i16 & 3u) / 2;
-                    const uint32_t turn = (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2;
-                    const uint16_t* at = sv + r * STRIDE + (chunk ^ turn) * 8 + (i16 & 1u) * 4;
+                    const uint16_t* at = sv + r * STRIDE + (chunk ^ v_turn(r)) * 8 + (i16 & 1u) * 4;
                     const v8s x = join(lds_tr(at), lds_tr(at + 8 * STRIDE));
 #pragma unroll
                     for (uint32_t b = 0; b < QB; ++b) o[b][d] = E::mfma32(x, p[b][st], o[b][d]);
@@ -898,11 +910,11 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
                 }
             }
         }
-        if (more) {
-            store_tile(i + 1);
-            if (wave == 0) note(i + 2, ahead);
-        }
-        __syncthreads();
+        if (more && wave == 0) note(i + 2, ahead);
+    };
+    for (uint32_t i = 0; i < n_tiles; i += 2) {
+        tile(i, s_k0, s_v0, s_k1, s_v1);
+        if (i + 1 < n_tiles) tile(i + 1, s_k1, s_v1, s_k0, s_v0);
     }
 
 #pragma unroll
