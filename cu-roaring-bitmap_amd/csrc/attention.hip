@@ -196,6 +196,7 @@ struct Work {
     uint32_t keys;        // the request's
     uint32_t k0, k1;      // the range
     uint32_t range;       // its number
+    bool whole;           // the tile's only range: its results need not be joined
     bool none;            // nothing to do
 };
 
@@ -211,21 +212,43 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
     const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
     uint32_t lo = 0, start = 0, end = 0, keys = 0, tile = 0, count = 1, part = 0, at = 0;
     if (a.share == 0) {
-        for (uint32_t len = n; len > 64;) {  // base(lo) <= id < base(lo + len)
-            const uint32_t step = (len + 63) / 64, i = lo + lane * step;
-            const bool below = lane * step < len && tile_base(i, segment_start(a, i), group, most) <= id;
-            const uint32_t from = (max(1u, static_cast<uint32_t>(__popcll(__ballot(below)))) - 1) * step;
-            lo += from;
-            len = min(step, len - from);
+        if (n <= 64) {
+            // the requests with the most keys go first, and of each its last rows, which see the most
+            const uint32_t i = min(lane, n);
+            start = static_cast<uint32_t>(segment_start(a, i));
+            end = static_cast<uint32_t>(segment_start(a, i + 1));
+            keys = segment_keys(a, i);
+            const uint32_t rows = end > start ? (end - start) * group : 0u, mine = i < n ? (rows + most - 1) / most : 0u;
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t other = lane_value(keys, j), tiles = lane_value(mine, j);
+                before += other > keys || (other == keys && j < lane) ? tiles : 0u;
+            }
+            const uint64_t here = __ballot(before <= id && id - before < mine);
+            if (!here) {
+                Work w{};
+                w.none = true;
+                return w;
+            }
+            at = lo = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(here))) - 1;
+            tile = lane_value(mine, at) - 1 - (id - lane_value(before, at));
+        } else {
+            for (uint32_t len = n; len > 64;) {  // base(lo) <= id < base(lo + len)
+                const uint32_t step = (len + 63) / 64, i = lo + lane * step;
+                const bool below = lane * step < len && tile_base(i, segment_start(a, i), group, most) <= id;
+                const uint32_t from = (max(1u, static_cast<uint32_t>(__popcll(__ballot(below)))) - 1) * step;
+                lo += from;
+                len = min(step, len - from);
+            }
+            const uint32_t i = min(lo + lane, n);
+            start = static_cast<uint32_t>(segment_start(a, i));
+            end = static_cast<uint32_t>(segment_start(a, i + 1));
+            keys = segment_keys(a, i);
+            const uint32_t base = tile_base(i, static_cast<int32_t>(start), group, most);
+            at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lo + lane < n && base <= id)))) - 1;
+            lo += at;
+            tile = id - lane_value(base, at);
         }
-        const uint32_t i = min(lo + lane, n);
-        start = static_cast<uint32_t>(segment_start(a, i));
-        end = static_cast<uint32_t>(segment_start(a, i + 1));
-        keys = segment_keys(a, i);
-        const uint32_t base = tile_base(i, static_cast<int32_t>(start), group, most);
-        at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lo + lane < n && base <= id)))) - 1;
-        lo += at;
-        tile = id - lane_value(base, at);
     } else {
         // ranges of one length for all, so that about `share` of them result
         uint64_t all = 0;
@@ -284,6 +307,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
     w.keys = lane_value(keys, at);
     w.none = w.row0 >= w.rows;
     w.range = id;
+    w.whole = count == 1;
     const uint32_t even = ((w.keys + count - 1) / count + a.step - 1) / a.step * a.step;
     w.k0 = part * even;
     w.k1 = part + 1 == count ? w.keys : min(w.keys, w.k0 + even);
@@ -344,10 +368,10 @@ __device__ __forceinline__ float score_scale(const AttnArgs& a)
 // where another kernel joins the ranges of keys.  `place` numbers the rows of
 // the ranges' results.
 template <class E>
-__device__ __forceinline__ void store_row(const AttnArgs& a, E, uint64_t place, uint32_t token, uint32_t head,
+__device__ __forceinline__ void store_row(const AttnArgs& a, E, const Work& t, uint64_t place, uint32_t token, uint32_t head,
                                           uint32_t d, f32x4 x)
 {
-    if (a.share) {
+    if (!t.whole) {
         *reinterpret_cast<f32x4*>(a.part_o + place * a.dim + d) = x;
     } else {
         const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
@@ -357,9 +381,9 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, E, uint64_t place, 
 }
 
 // lse2: base 2
-__device__ __forceinline__ void store_lse(const AttnArgs& a, uint64_t place, uint32_t token, uint32_t head, float lse2)
+__device__ __forceinline__ void store_lse(const AttnArgs& a, const Work& t, uint64_t place, uint32_t token, uint32_t head, float lse2)
 {
-    if (a.share)
+    if (!t.whole)
         a.part_lse[place] = lse2;
     else if (a.lse)
         a.lse[static_cast<uint64_t>(token) * a.heads + head] = lse2 * LN2;
@@ -383,7 +407,7 @@ struct Rows {
     static constexpr uint32_t STRIDE = CHUNKS * 8;                             // its elements
 };
 
-template <class E, uint32_t DIM, bool FULL, uint32_t NB>
+template <class E, uint32_t DIM, uint32_t NB>
 __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 {
     constexpr uint32_t STEPS = DIM / 32, BLOCKS = DIM / 16, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
@@ -416,7 +440,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     least = __builtin_amdgcn_readfirstlane(least);
     const uint32_t k0 = t.k0, k1 = min(most, t.k1);
     const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * (16 * NB);  // of the tile's first row
-    if (a.share && k0 >= k1) {
+    if (!t.whole && k0 >= k1) {
         if (threadIdx.x < 16 * NB) a.part_lse[place0 + threadIdx.x] = NEG_INF;
         return;
     }
@@ -644,53 +668,73 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 #pragma unroll
                 for (uint32_t w = 0; w < DC_WAVES; ++w)
                     x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(s_mem) + (w * 16 + mine) * RED + d);
-                if (d < a.dim) store_row(a, E{}, place, token, head, d, x * part);
+                if (d < a.dim) store_row(a, E{}, t, place, token, head, d, x * part);
             }
-            if (threadIdx.x % 16 == 0) store_lse(a, place, token, head, lse2);
+            if (threadIdx.x % 16 == 0) store_lse(a, t, place, token, head, lse2);
         }
         __syncthreads();
     }
 }
 
 // ---- many rows: bound by the matrix units --------------------------------------------
-// A workgroup answers 128 QB rows, 32 QB of them a wave, over tiles of 64 keys
-// that all its waves read from LDS, where the next tile's keys and values arrive
-// meanwhile without passing through registers.  Scores are transposed products (keys x rows) of 32x32x16 matrix
-// instructions; a row's probabilities then lie in the lanes that the second
-// product wants them in, if its 16 keys are taken in the order 4h..4h+3,
-// 8+4h..8+4h+3 for lane half h, and values are transposed on their way out of
-// LDS.  Rows of LDS are turned by pieces of 16 bytes so that neither the 32 rows
-// of a key fragment nor the four of a value's share banks.
+// A workgroup answers 128 rows, 32 of them a wave, over tiles of 64 keys that all
+// its waves read from LDS, where the next keys and values arrive meanwhile
+// without passing through registers.  Scores are transposed products (keys x
+// rows) of 32x32x16 matrix instructions; a row's probabilities then lie in the
+// lanes that the second product wants them in, if its 16 keys are taken in the
+// order 4h..4h+3, 8+4h..8+4h+3 for lane half h, and values are transposed on
+// their way out of LDS.  Rows of LDS are turned by pieces of 16 bytes so that
+// neither the 32 rows of a key fragment nor the four of a value's share banks.
+//
+// The products run a tile ahead of the softmax: while the matrix units multiply
+// tile i + 1's keys, the wave turns tile i's scores into probabilities, and while
+// they multiply those with the values, it takes the maximum of the new scores.
+// One workgroup and two waves a SIMD more or less keep the other busy too.
+// 16384 tokens, 32 heads over 8, 128 dimensions, bf16: 2.31 ms, 950 TFLOP/s (a
+// large bf16 library product reaches 1206): the matrix units work 45% of the
+// cycles, at 2.0 GHz, to which their power brings the clock down from 2.35.  On
+// the way: keys and values through registers 2.72 ms; straight to LDS, without
+// running ahead 2.36; 64 rows a wave with one wave a SIMD, which halves what is
+// read from LDS, 3.2.
 constexpr int TL_NT = 256;
 // Keys of a tile: 64, or 32 where longer rows would not leave room for the next tile's in registers.
 constexpr uint32_t tile_keys(uint32_t dim) { return dim <= 128 ? 64 : 32; }
 
-template <class E, uint32_t DIM, bool FULL, uint32_t QB>
-__global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 && DIM <= 128 ? 2 : 1))) void at_tiles(AttnArgs a)
+// Orders the products of the block before: READS fragments of LDS first, then
+// after each product the next one's fragments and a few other
+// instructions, which the matrix units cover.
+template <uint32_t PRODUCTS, uint32_t READS, uint32_t PER_STEP, uint32_t OTHERS>
+__device__ __forceinline__ void between_products()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (uint32_t i = 0; i < PRODUCTS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, PER_STEP, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, OTHERS, 0);
+    }
+}
+
+template <class E, uint32_t DIM>
+__global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 128 ? 2 : 1))) void at_tiles(AttnArgs a)
 {
     constexpr uint32_t STEPS = DIM / 16, BLOCKS = DIM / 32, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
     constexpr uint32_t KEYS = tile_keys(DIM), HALVES = KEYS / 32;
-    constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << KEYS) - 1ull;
+    constexpr uint64_t ALL = ~0ull >> (64 - KEYS);
     constexpr uint32_t PER = TL_NT / CHUNKS, LOADS = KEYS / PER;  // rows that the workgroup loads at once, and how often
     constexpr uint32_t KTURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
     // separate arrays: what is read is not what is being loaded
     __shared__ alignas(16) uint16_t s_k0[KEYS * STRIDE], s_k1[KEYS * STRIDE];
     __shared__ alignas(16) uint16_t s_v0[KEYS * STRIDE], s_v1[KEYS * STRIDE];
-    __shared__ uint64_t s_koff[3][KEYS], s_voff[3][KEYS], s_there[3];
-    __shared__ uint32_t s_bad[3], s_most[TL_NT / 64], s_least[TL_NT / 64];
+    __shared__ uint64_t s_koff[4][KEYS], s_voff[4][KEYS], s_there[4];
+    __shared__ uint32_t s_bad[4], s_most[TL_NT / 64], s_least[TL_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
     const uint32_t kh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
-    // a request's last rows see the most keys: they go first
-    const Work t = find_work(a, a.share ? id : a.n_tiles - 1 - id, 128 * QB);
+    const Work t = find_work(a, id, 128);
     if (t.none) return;
-    uint32_t limit[QB], most = 0, least = 0xFFFFFFFFu;
-#pragma unroll
-    for (uint32_t b = 0; b < QB; ++b) {
-        const uint32_t row = t.row0 + (wave * QB + b) * 32 + c32;
-        limit[b] = row < t.rows ? limit_of(a, t, row / group) : 0u;
-        most = max(most, limit[b]);
-        if (row < t.rows) least = min(least, limit[b]);
-    }
+    const uint32_t row = t.row0 + wave * 32 + c32;  // the lane's
+    const uint32_t limit = row < t.rows ? limit_of(a, t, row / group) : 0u;
+    uint32_t most = limit, least = row < t.rows ? limit : 0xFFFFFFFFu;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
@@ -702,7 +746,6 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
         s_most[wave] = wave_most;
         s_least[wave] = wave_least;
     }
-    if (threadIdx.x < 3) s_bad[threadIdx.x] = 0;
     __syncthreads();
     most = 0;
     least = 0xFFFFFFFFu;
@@ -714,29 +757,21 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     most = __builtin_amdgcn_readfirstlane(most);
     least = __builtin_amdgcn_readfirstlane(least);
     const uint32_t k0 = t.k0, k1 = min(most, t.k1);
-    const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * (128 * QB);  // of the tile's first row
-    if (a.share && k0 >= k1) {
-        if (threadIdx.x < 128 * QB) a.part_lse[place0 + threadIdx.x] = NEG_INF;
+    const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * 128;  // of the tile's first row
+    if (!t.whole && k0 >= k1) {
+        if (threadIdx.x < 128) a.part_lse[place0 + threadIdx.x] = NEG_INF;
         return;
     }
 
-    v8s q[QB][STEPS];
+    v8s q[STEPS];
 #pragma unroll
-    for (uint32_t b = 0; b < QB; ++b)
+    for (uint32_t st = 0; st < STEPS; ++st) q[st] = load_query(a, t, row, kh, st * 16 + h * 8);
+    f32x16 o[BLOCKS];
+    float m = NEG_INF, l = 0.0f;
 #pragma unroll
-        for (uint32_t s = 0; s < STEPS; ++s)
-            q[b][s] = load_query(a, t, t.row0 + (wave * QB + b) * 32 + c32, kh, s * 16 + h * 8);
-    f32x16 o[QB][BLOCKS];
-    float m[QB], l[QB];
+    for (uint32_t d = 0; d < BLOCKS; ++d)
 #pragma unroll
-    for (uint32_t b = 0; b < QB; ++b) {
-        m[b] = NEG_INF;
-        l[b] = 0.0f;
-#pragma unroll
-        for (uint32_t d = 0; d < BLOCKS; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
-    }
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     const float c = score_scale(a);
     const uint16_t* kp = a.k + kh * a.k_head;
     const uint16_t* vp = a.v + kh * a.v_head;
@@ -746,7 +781,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     // The first wave looks up where tile i's keys and values are.
     auto find = [&](uint32_t i) { return look_up(a, t.request, min(k0 + i * KEYS + lane % KEYS, k1 - 1)); };
     auto note = [&](uint32_t i, int32_t found) {
-        const uint32_t at = i % 3, j = k0 + i * KEYS + lane;
+        const uint32_t at = i % 4, j = k0 + i * KEYS + lane;
         const int32_t slot = lane < KEYS && j < k1 ? slot_of(a, found, j) : -1;
         if (lane < KEYS) {
             s_koff[at][lane] = offset_of(slot, a.page_lg, a.k_page, a.k_slot);
@@ -762,17 +797,18 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
     // Each lane's 16 bytes go straight to the wave's next 1 KiB of LDS; which of a
     // row's pieces a lane names turns the row.  Pieces behind the head dimension
     // repeat the first one: they meet zero queries, and their columns are not stored.
-    auto load_tile = [&](uint32_t i, uint16_t* sk, uint16_t* sv) {
-        const uint32_t at = i % 3;
+    auto load_keys = [&](uint32_t i, uint16_t* sk) {
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow, d = (lpos ^ (r & KTURN)) * 8;
-            load_to_lds(kp + s_koff[at][r] + (d < a.dim ? d : 0u), sk + (x * PER + wave_row) * STRIDE);
+            load_to_lds(kp + s_koff[i % 4][r] + (d < a.dim ? d : 0u), sk + (x * PER + wave_row) * STRIDE);
         }
+    };
+    auto load_values = [&](uint32_t i, uint16_t* sv) {
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow, d = (lpos ^ v_turn(r)) * 8;
-            load_to_lds(vp + s_voff[at][r] + (d < a.dim ? d : 0u), sv + (x * PER + wave_row) * STRIDE);
+            load_to_lds(vp + s_voff[i % 4][r] + (d < a.dim ? d : 0u), sv + (x * PER + wave_row) * STRIDE);
         }
     };
     // Values of keys that no row sees become zeros, and, in a tile that some rows
@@ -787,113 +823,153 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
             bad |= __ballot(has_special(y, E::EXP));
             *reinterpret_cast<v8s*>(at) = without_special(y, E::EXP);
         }
-        if (bad && lane == 0) s_bad[i % 3] = 1;
+        if (bad && lane == 0) s_bad[i % 4] = 1;
+    };
+
+    // Where this lane's fragments begin: keys step by step, values by blocks of 32
+    // dimensions (the turn of a row moves a block among four).
+    uint32_t k_at[STEPS], v_at[4];
+#pragma unroll
+    for (uint32_t st = 0; st < STEPS; ++st) k_at[st] = c32 * STRIDE + ((st * 2 + h) ^ (c32 & KTURN)) * 8;
+    {
+        const uint32_t i16 = lane & 15u, r = h * 4 + i16 / 4, turn = v_turn(r) / 4;
+#pragma unroll
+        for (uint32_t d = 0; d < 4; ++d)
+            v_at[d] = r * STRIDE + (d ^ turn) * 32 + ((lane >> 4) & 1u) * 16 + (i16 & 3u) * 4;
+    }
+
+    f32x16 s[HALVES];  // the scores of the tile to come
+    float top;
+    // Its products, as transposed blocks of 32 keys by 32 rows.
+    auto multiply = [&](const uint16_t* sk, f32x16 (&x)[HALVES]) {
+#pragma unroll
+        for (uint32_t y = 0; y < HALVES; ++y)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[y][e] = 0.0f;
+#pragma unroll
+        for (uint32_t y = 0; y < HALVES; ++y)
+#pragma unroll
+            for (uint32_t st = 0; st < STEPS; ++st) {
+                const v8s k = load8(sk + y * 32 * STRIDE + k_at[st]);
+                x[y] = E::mfma32(k, q[st], x[y]);
+            }
+    };
+    auto hide = [&](uint32_t i) {
+        const uint32_t j0 = k0 + i * KEYS;
+        const uint64_t there = s_there[i % 4];
+        if (there == ALL && j0 + KEYS <= wave_least) return;
+        const int32_t left = static_cast<int32_t>(limit - j0 - h * 4);
+#pragma unroll
+        for (uint32_t x = 0; x < HALVES; ++x) {
+            const uint32_t on = static_cast<uint32_t>(there >> (x * 32)) >> (h * 4);
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e) {
+                const uint32_t at = (e / 4) * 8 + e % 4;
+                const bool see = static_cast<int32_t>(x * 32 + at) < left & (on & (1u << at)) != 0;
+                s[x][e] = see ? s[x][e] : NEG_INF;
+            }
+        }
+    };
+    auto highest = [&]() {
+        top = NEG_INF;
+#pragma unroll
+        for (uint32_t x = 0; x < HALVES; ++x)
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
+    };
+    auto follow = [&]() {
+        const float all = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any((all - m) * c > LAG)) {  // m starts at -inf; NaN where both are
+            const float now = fmaxf(m, all);
+            const float fix = now == NEG_INF ? 1.0f : exp2_fast((m - now) * c);
+            m = now;
+            l *= fix;
+#pragma unroll
+            for (uint32_t d = 0; d < BLOCKS; ++d) o[d] *= fix;
+        }
     };
 
     const uint32_t n_tiles = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
+    const uint32_t mine = min(n_tiles, wave_most > k0 ? (wave_most - k0 + KEYS - 1) / KEYS : 0u);  // this wave's
     if (n_tiles) {
         if (wave == 0) {
-            const int32_t first = find(0), second = find(1);
+            const int32_t first = find(0), second = find(1), third = find(2);
             note(0, first);
             note(1, second);
+            note(2, third);
         }
         __syncthreads();
-        load_tile(0, s_k0, s_v0);
-    }
-    // One tile, from `sk` and `sv`, while the next one comes into the other two.
-    auto tile = [&](uint32_t i, uint16_t* sk, uint16_t* sv, uint16_t* next_k, uint16_t* next_v) {
-        __syncthreads();  // this tile is there, and nobody reads the last one any more
-        const bool more = i + 1 < n_tiles;
-        int32_t ahead = -1;
-        if (more) {
-            if (wave == 0) ahead = find(i + 2);
-            load_tile(i + 1, next_k, next_v);
+        load_keys(0, s_k0);
+        load_values(0, s_v0);
+        if (n_tiles > 1) load_keys(1, s_k1);
+        __syncthreads();
+        if (mine) {
+            multiply(s_k0, s);
+            hide(0);
+            highest();
+            follow();
         }
+    }
+    // The queries are waited for here, on every way to the loop, or each of its
+    // turns would wait for all loads before its first product.
+#pragma unroll
+    for (uint32_t st = 0; st < STEPS; ++st) asm volatile("" : "+v"(q[st]));
+    // Tile i's probabilities and values, while the matrix units turn the next
+    // tile's keys into scores; the keys behind those and the next values come in.
+    auto tile = [&](uint32_t i, uint16_t* sk, uint16_t* next_k, uint16_t* sv, uint16_t* next_v) {
+        __syncthreads();  // keys i + 1 and values i are there, and nobody reads those before any more
+        int32_t ahead = -1;
+        if (wave == 0) ahead = find(i + 3);
+        if (i + 1 < n_tiles) load_values(i + 1, next_v);
+        if (i + 2 < n_tiles) load_keys(i + 2, sk);
         const uint32_t j0 = k0 + i * KEYS;
-        const uint64_t there = s_there[i % 3];
+        const uint64_t there = s_there[i % 4];
         if (!(there == ALL && j0 + KEYS <= least)) {
             mend_tile(i, there, sv);
             __syncthreads();
         }
-        if (j0 < wave_most) {
-            f32x16 s[QB][HALVES];
-#pragma unroll
-            for (uint32_t b = 0; b < QB; ++b)
-#pragma unroll
-                for (uint32_t x = 0; x < HALVES; ++x)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[b][x][e] = 0.0f;
+        if (i < mine) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 ahead_s[HALVES];
+            v8s p[2 * HALVES];
+            multiply(next_k, ahead_s);
+            const float mc = m == NEG_INF ? 0.0f : m * c;
 #pragma unroll
             for (uint32_t x = 0; x < HALVES; ++x)
 #pragma unroll
-                for (uint32_t st = 0; st < STEPS; ++st) {
-                    const v8s k = load8(sk + (x * 32 + c32) * STRIDE + ((st * 2 + h) ^ (c32 & KTURN)) * 8);
-#pragma unroll
-                    for (uint32_t b = 0; b < QB; ++b) s[b][x] = E::mfma32(k, q[b][st], s[b][x]);
+                for (uint32_t e = 0; e < 16; ++e) {
+                    const float y = exp2_fast(__builtin_fmaf(s[x][e], c, -mc));
+                    l += y;
+                    p[x * 2 + e / 8][e % 8] = static_cast<short>(E::down(y));
                 }
+            // all of it before the branch, between the products
+            asm volatile("" : "+v"(l));
+#pragma unroll
+            for (uint32_t x = 0; x < 2 * HALVES; ++x) asm volatile("" : "+v"(p[x]));
+            between_products<STEPS * HALVES, 3, 1, 6>();
             __builtin_amdgcn_sched_barrier(0);
-            if (there != ALL || j0 + KEYS > wave_least) {
 #pragma unroll
-                for (uint32_t b = 0; b < QB; ++b) {
-                    const int32_t left = static_cast<int32_t>(limit[b] - j0 - h * 4);
-#pragma unroll
-                    for (uint32_t x = 0; x < HALVES; ++x) {
-                        const uint32_t on = static_cast<uint32_t>(there >> (x * 32)) >> (h * 4);
-#pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e) {
-                            const uint32_t at = (e / 4) * 8 + e % 4;
-                            const bool see = static_cast<int32_t>(x * 32 + at) < left & (on & (1u << at)) != 0;
-                            s[b][x][e] = see ? s[b][x][e] : NEG_INF;
-                        }
-                    }
-                }
-            }
-            v8s p[QB][2 * HALVES];
-#pragma unroll
-            for (uint32_t b = 0; b < QB; ++b) {
-                float top = NEG_INF;
-#pragma unroll
-                for (uint32_t x = 0; x < HALVES; ++x)
-#pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e) top = fmaxf(top, s[b][x][e]);
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                if (__any((top - m[b]) * c > LAG)) {  // m starts at -inf; NaN where both are
-                    const float now = fmaxf(m[b], top);
-                    const float fix = now == NEG_INF ? 1.0f : exp2_fast((m[b] - now) * c);
-                    m[b] = now;
-                    l[b] *= fix;
-#pragma unroll
-                    for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] *= fix;
-                }
-                const float mc = m[b] == NEG_INF ? 0.0f : m[b] * c;
-#pragma unroll
-                for (uint32_t x = 0; x < HALVES; ++x)
-#pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e) {
-                        const float y = exp2_fast(__builtin_fmaf(s[b][x][e], c, -mc));
-                        l[b] += y;
-                        p[b][x * 2 + e / 8][e % 8] = static_cast<short>(E::down(y));
-                    }
-            }
+            for (uint32_t x = 0; x < HALVES; ++x) s[x] = ahead_s[x];
+            if (i + 1 < mine) hide(i + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (uint32_t st = 0; st < 2 * HALVES; ++st)
 #pragma unroll
                 for (uint32_t d = 0; d < BLOCKS; ++d) {
-                    const uint32_t i16 = lane & 15u, r = st * 16 + h * 4 + i16 / 4;
-                    const uint32_t chunk = d * 4 + ((lane >> 4) & 1u) * 2 + (i16 & 3u) / 2;
-                    const uint16_t* at = sv + r * STRIDE + (chunk ^ v_turn(r)) * 8 + (i16 & 1u) * 4;
+                    const uint16_t* at = sv + st * 16 * STRIDE + d / 4 * 128 + v_at[d % 4];
                     const v8s x = join(lds_tr(at), lds_tr(at + 8 * STRIDE));
-#pragma unroll
-                    for (uint32_t b = 0; b < QB; ++b) o[b][d] = E::mfma32(x, p[b][st], o[b][d]);
+                    o[d] = E::mfma32(x, p[st], o[d]);
                 }
+            highest();
+            asm volatile("" : "+v"(top));
+            between_products<2 * HALVES * BLOCKS, 6, 2, 2>();
             __builtin_amdgcn_sched_barrier(0);
-            if (s_bad[i % 3]) {
+            if (s_bad[i % 4]) {
                 // Infinite and NaN values, left out of LDS so that rows which do
                 // not see their keys are spared, reach the rows that do.
                 for (uint32_t j = 0; j < KEYS; ++j) {
                     if (!((there >> j) & 1ull)) continue;
-                    const uint16_t* from = vp + s_voff[i % 3][j];
+                    const uint16_t* from = vp + s_voff[i % 4][j];
                     uint32_t h4 = h * 4;
                     asm volatile("" : "+v"(h4));  // the addresses are worked out here, not kept in registers
 #pragma unroll
@@ -902,40 +978,35 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(QB == 1 &
                         for (uint32_t e = 0; e < 16; e += 4) {
                             const uint32_t at_d = d * 32 + e * 2 + h4;
                             const v4s x = load4(from + (at_d < a.dim ? at_d : 0u));
-#pragma unroll
-                            for (uint32_t b = 0; b < QB; ++b)
-                                if (j0 + j < limit[b]) add_special<E>(o[b][d], e, x);
+                            if (j0 + j < limit) add_special<E>(o[d], e, x);
                             __builtin_amdgcn_sched_barrier(0);
                         }
                 }
             }
+            if (i + 1 < mine) follow();
         }
-        if (more && wave == 0) note(i + 2, ahead);
+        if (wave == 0) note(i + 3, ahead);
     };
     for (uint32_t i = 0; i < n_tiles; i += 2) {
-        tile(i, s_k0, s_v0, s_k1, s_v1);
-        if (i + 1 < n_tiles) tile(i + 1, s_k1, s_v1, s_k0, s_v0);
+        tile(i, s_k0, s_k1, s_v0, s_v1);
+        if (i + 1 < n_tiles) tile(i + 1, s_k1, s_k0, s_v1, s_v0);
     }
 
+    const float lt = l + __shfl_xor(l, 32, 64);
+    const bool none = m == NEG_INF;
+    const float part = none ? 0.0f : 1.0f / lt;
+    if (row >= t.rows) return;
+    const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
+    const uint64_t place = place0 + wave * 32 + c32;
 #pragma unroll
-    for (uint32_t b = 0; b < QB; ++b) {
-        const uint32_t row = t.row0 + (wave * QB + b) * 32 + c32;
-        const float lt = l[b] + __shfl_xor(l[b], 32, 64);
-        const bool none = m[b] == NEG_INF;
-        const float part = none ? 0.0f : 1.0f / lt;
-        if (row >= t.rows) continue;
-        const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
-        const uint64_t place = place0 + (wave * QB + b) * 32 + c32;
+    for (uint32_t d = 0; d < BLOCKS; ++d)
 #pragma unroll
-        for (uint32_t d = 0; d < BLOCKS; ++d)
-#pragma unroll
-            for (uint32_t e = 0; e < 16; e += 4) {
-                const uint32_t at_d = d * 32 + e * 2 + h * 4;
-                const f32x4 x = {o[b][d][e], o[b][d][e + 1], o[b][d][e + 2], o[b][d][e + 3]};
-                if (at_d < a.dim) store_row(a, E{}, place, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
-            }
-        if (h == 0) store_lse(a, place, token, head, none ? NEG_INF : m[b] * c + __builtin_amdgcn_logf(lt));
-    }
+        for (uint32_t e = 0; e < 16; e += 4) {
+            const uint32_t at_d = d * 32 + e * 2 + h * 4;
+            const f32x4 x = {o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            if (at_d < a.dim) store_row(a, E{}, t, place, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
+        }
+    if (h == 0) store_lse(a, t, place, token, head, none ? NEG_INF : m * c + __builtin_amdgcn_logf(lt));
 }
 
 // ---- the ranges' results joined: a workgroup per row -----------------------------------
@@ -962,6 +1033,7 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
     }
     const uint32_t row = (token - start) * group + head % group;
     const uint2 range = a.ranges[tile_base(lo, static_cast<int32_t>(start), group, most) + row / most];
+    if (range.y == 1) return;  // written already
     auto place = [&](uint32_t r) {
         return (static_cast<uint64_t>(range.x + r) * a.kv_heads + head / group) * most + row % most;
     };
@@ -1001,31 +1073,25 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
     }
 }
 
-template <class E, uint32_t DIM, bool FULL>
-int launch_full(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
+template <class E, uint32_t DIM>
+int launch_dim(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
 {
     if (per_wave == 0) {
         CR_TIMED("at_tiles", s);
-        at_tiles<E, DIM, FULL, 1><<<grid, TL_NT, 0, s>>>(a);
+        at_tiles<E, DIM><<<grid, TL_NT, 0, s>>>(a);
     } else {
         CR_TIMED("at_rows", s);
         if constexpr (DIM <= 128) {
             if (per_wave == 2) {
-                at_rows<E, DIM, FULL, 2><<<grid, DC_NT, 0, s>>>(a);
+                at_rows<E, DIM, 2><<<grid, DC_NT, 0, s>>>(a);
                 CR_LAUNCH_CHECK();
                 return CR_OK;
             }
         }
-        at_rows<E, DIM, FULL, 1><<<grid, DC_NT, 0, s>>>(a);
+        at_rows<E, DIM, 1><<<grid, DC_NT, 0, s>>>(a);
     }
     CR_LAUNCH_CHECK();
     return CR_OK;
-}
-
-template <class E, uint32_t DIM>
-int launch_dim(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
-{
-    return a.dim == DIM ? launch_full<E, DIM, true>(a, per_wave, grid, s) : launch_full<E, DIM, false>(a, per_wave, grid, s);
 }
 
 template <class E>

@@ -348,3 +348,22 @@ def test_refusals(gpu):
         with pytest.raises(gpu.CrError) as e:
             gpu.paged_attention(**{**ok, **bad})
         assert e.value.code == code, bad.keys()
+
+
+@pytest.mark.parametrize("hints", [{}, dict(max_kv=20000), dict(max_new=64), dict(max_new=64, max_kv=20000)])
+def test_more_requests_than_a_wave_has_lanes(gpu, hints):
+    """Over 64 requests, some without tokens or keys, by either kernel, with their keys cut into ranges or not."""
+    _say("attention of 150 requests", hints)
+    rng = np.random.default_rng(17)
+    new = rng.integers(0, 4, 150).tolist()
+    kv = [int(rng.integers(0, 300)) for _ in new]
+    kv[77], new[77] = 2500, 3
+    Problem("bfloat16", new, kv, 2, 1, 64, 16, seed=18).check(gpu, **hints)
+
+
+@pytest.mark.parametrize("density", [None, 0.3])
+@pytest.mark.parametrize("hints", [{}, dict(max_kv=5000), dict(max_new=1, max_kv=5000)])
+def test_long_and_short_requests(gpu, hints, density):
+    """One long request among short ones: some tiles are cut into ranges and others are whole."""
+    _say("attention of long and short requests", hints, density)
+    Problem("float16", [40, 3, 1, 0, 70], [4700, 30, 1, 9, 90], 4, 2, 96, 16, seed=19, density=density).check(gpu, **hints)
