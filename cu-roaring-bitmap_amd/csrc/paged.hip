@@ -54,20 +54,34 @@ __device__ __forceinline__ uint64_t block_excl_scan_u64(uint64_t v, uint64_t* ld
     return base + incl - v;
 }
 
-// The free set's bits, 128 pages at a time: flat words, or the containers of a
-// bitmap that holds nothing but bitmap containers.
-struct FreeSet {
-    const uint4* flat;
+// A set's bits: flat words, or the containers of a bitmap that holds nothing but
+// bitmap containers.
+struct SetBits {
+    const uint32_t* flat;
     const uint16_t* key_index;
     const uint32_t* offsets;
     const uint64_t* bitmaps;
     uint32_t max_key;
-    uint32_t flip;     // all bits set where the containers hold the complement
-    uint32_t n_pages;  // pages from here on are not free
+    uint32_t flip;  // all bits set where the containers hold the complement
+    uint32_t end;   // ids from here on are not in the set
+
+    // Word w of the set (ids [32 w, 32 w + 32), w <= (end - 1) / 32).
+    __device__ __forceinline__ uint32_t word(uint32_t w) const
+    {
+        uint32_t x;
+        if (flat) {
+            x = flat[w];
+        } else {
+            const uint32_t key = w / 2048u, c = key <= max_key ? key_index[key] : 0xFFFFu;
+            x = c != 0xFFFFu ? reinterpret_cast<const uint32_t*>(bitmaps)[offsets[c] / 4u + w % 2048u] : 0u;
+            x ^= flip;
+        }
+        return w == end / 32u ? x & ((1u << (end % 32u)) - 1u) : x;
+    }
 };
 
 struct PlanArgs {
-    FreeSet free;
+    SetBits free;
     uint32_t n_quads;   // pieces of 128 pages
     uint32_t n_blocks;
     uint32_t page_lg;
@@ -93,11 +107,11 @@ struct PlanArgs {
 // past the last page.  No load depends on a branch, so that those of all N are
 // in flight together.
 template <uint32_t N>
-__device__ __forceinline__ void free_quads(const FreeSet& f, const uint32_t (&q)[N], uint32_t n_quads, uint4 (&x)[N])
+__device__ __forceinline__ void free_quads(const SetBits& f, const uint32_t (&q)[N], uint32_t n_quads, uint4 (&x)[N])
 {
     if (f.flat) {
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) x[i] = f.flat[min(q[i], n_quads - 1)];
+        for (uint32_t i = 0; i < N; ++i) x[i] = reinterpret_cast<const uint4*>(f.flat)[min(q[i], n_quads - 1)];
     } else {
         uint32_t c[N], at[N];
 #pragma unroll
@@ -118,8 +132,8 @@ __device__ __forceinline__ void free_quads(const FreeSet& f, const uint32_t (&q)
     }
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
-        if (q[i] < f.n_pages / 128u) continue;
-        const uint32_t left = q[i] > f.n_pages / 128u ? 0u : f.n_pages % 128u;  // of these
+        if (q[i] < f.end / 128u) continue;
+        const uint32_t left = q[i] > f.end / 128u ? 0u : f.end % 128u;  // of these
         auto cut = [&](uint32_t w, uint32_t k) {
             return left >= 32u * k + 32u ? w : left <= 32u * k ? 0u : w & ((1u << (left - 32u * k)) - 1u);
         };
@@ -127,7 +141,7 @@ __device__ __forceinline__ void free_quads(const FreeSet& f, const uint32_t (&q)
     }
 }
 
-__device__ __forceinline__ uint4 free_quad(const FreeSet& f, uint32_t q, uint32_t n_quads)
+__device__ __forceinline__ uint4 free_quad(const SetBits& f, uint32_t q, uint32_t n_quads)
 {
     const uint32_t at[1] = {q};
     uint4 x[1];
@@ -468,12 +482,16 @@ __global__ __launch_bounds__(AP_NT) void pg_append(AppendArgs a)
 }
 
 // ---- select --------------------------------------------------------------------
-constexpr int SL_NT = 256;
-constexpr uint32_t SL_POS = 32 * SL_NT;  // positions a workgroup looks at
+// A wave looks at 32 positions a lane: the bits of the pages that hold them are
+// the positions' own, in words (or parts of one, where a page is shorter).
+// Bound by the latency of its look-ups, so that many workgroups of one wave do it
+// (4 requests of 131072 positions: 11.8 us; 17.4 with the bitmap written out as
+// flat words first, 8192 positions a workgroup and a table look-up for each slot).
+constexpr int SL_NT = 64;
+constexpr uint32_t SL_POS = 32 * SL_NT;
 
 struct SelectArgs {
-    const uint32_t* words;  // visible slots, n_words of them
-    uint32_t n_words;
+    SetBits visible;  // slots
     const int32_t* table;
     uint32_t cols;
     uint64_t table_stride;
@@ -498,40 +516,46 @@ __device__ __forceinline__ uint32_t select_len(const SelectArgs& a, uint32_t r)
     return n <= 0 ? 0u : static_cast<uint32_t>(min(most, static_cast<uint64_t>(n)));
 }
 
-// Which of the 32 positions from p0 (a multiple of 32) are visible.
-__device__ __forceinline__ uint32_t visible_word(const SelectArgs& a, uint32_t r, uint32_t p0, uint32_t len)
+// Calls f(first position, first slot, visible bits) for each page, or 32
+// positions of one, among the 32 positions from p0 (a multiple of 32).
+template <class F>
+__device__ __forceinline__ void visible_parts(const SelectArgs& a, uint32_t r, uint32_t p0, uint32_t len, F f)
 {
-    if (p0 >= len) return 0u;
     const int32_t* row = a.table + r * a.table_stride;
     const uint32_t lg = min(a.page_lg, 5u), part = 1u << lg;
-    uint32_t vis = 0;
-    for (uint32_t k = 0; k < 32u && p0 + k < len; k += part) {
-        const uint32_t pos = p0 + k, page = static_cast<uint32_t>(row[pos >> a.page_lg]);
+    for (uint32_t p = p0; p < min(len, p0 + 32u); p += part) {
+        const uint32_t page = static_cast<uint32_t>(row[p >> a.page_lg]);
         if (page >= a.n_pages) continue;
-        const uint64_t slot = (static_cast<uint64_t>(page) << a.page_lg) + (pos & ((1u << a.page_lg) - 1u));
-        uint32_t bits = a.words[slot >> 5] >> (slot & 31u);
-        if (lg < 5u) bits &= (1u << part) - 1u;
-        vis |= bits << k;
+        const uint32_t slot = (page << a.page_lg) + (p & ((1u << a.page_lg) - 1u));
+        if (slot >= a.visible.end) continue;
+        uint32_t bits = a.visible.word(slot >> 5) >> (slot & 31u);
+        const uint32_t n = min(part, len - p);
+        if (n < 32u) bits &= (1u << n) - 1u;
+        f(p, slot, bits);
     }
-    return len - p0 < 32u ? vis & ((1u << (len - p0)) - 1u) : vis;
+}
+
+__device__ __forceinline__ uint32_t wave_total(uint32_t v)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_incl_scan(v)), 63));
 }
 
 __global__ __launch_bounds__(SL_NT) void sl_count(SelectArgs a)
 {
-    __shared__ uint32_t s[SL_NT / 64];
     const uint32_t r = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const uint32_t vis = visible_word(a, r, chunk * SL_POS + threadIdx.x * 32u, select_len(a, r));
-    const uint32_t n = block_sum<SL_NT>(__popc(vis), s);
+    uint32_t n = 0;
+    visible_parts(a, r, chunk * SL_POS + threadIdx.x * 32u, select_len(a, r),
+                  [&](uint32_t, uint32_t, uint32_t bits) { n += __popc(bits); });
+    n = wave_total(n);
     if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
 }
 
 __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
 {
-    __shared__ uint32_t s[SL_NT / 64];
     __shared__ int32_t s_slot[SL_POS];
     const uint32_t r = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, t = threadIdx.x;
     const uint32_t len = select_len(a, r), p0 = chunk * SL_POS + t * 32u;
-    // positions of the new tokens: the last `fresh` of the request's
+    // positions of the new tokens: the last of the request's
     const int32_t t0 = min(max(a.starts[r], 0), static_cast<int32_t>(a.n_tokens));
     const int32_t t1 = min(max(a.starts[r + 1], t0), static_cast<int32_t>(a.n_tokens));
     const int64_t shift = static_cast<int64_t>(t1) - len;  // position p is new token p + shift
@@ -541,24 +565,53 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
     if (chunk * SL_POS >= len && chunk > 0) return;
     uint32_t base = 0;
     for (uint32_t i = t; i < chunk; i += SL_NT) base += a.counts[r * a.chunks + i];
-    if (a.chunks > 1) base = block_sum<SL_NT>(base, s);
-    const uint32_t vis = visible_word(a, r, p0, len);
-    uint32_t total;
-    const uint32_t before = block_excl_scan<SL_NT>(__popc(vis), s, total);
-    const int32_t* row = a.table + r * a.table_stride;
+    uint32_t vis = 0;
+    visible_parts(a, r, p0, len, [&](uint32_t p, uint32_t, uint32_t bits) { vis |= bits << (p - p0); });
+    base = wave_total(base);
+    const uint32_t n = __popc(vis), upto = wave_incl_scan(n), before = upto - n;
+    const uint32_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
     uint32_t at = before;
-    for (uint32_t b = vis; b; b &= b - 1u) {
-        const uint32_t pos = p0 + __ffs(b) - 1;
-        s_slot[at++] = (row[pos >> a.page_lg] << a.page_lg) + static_cast<int32_t>(pos & ((1u << a.page_lg) - 1u));
-    }
-    for (uint32_t k = 0; k < 32u && p0 + k < len; ++k) {
-        const int64_t token = static_cast<int64_t>(p0 + k) + shift;
-        if (token >= t0 && token < t1)
-            a.limits[token] = static_cast<int32_t>(base + before + __popc(vis & (0xFFFFFFFFu >> (31u - k))));
+    visible_parts(a, r, p0, len, [&](uint32_t, uint32_t slot, uint32_t bits) {
+        for (; bits; bits &= bits - 1u) s_slot[at++] = static_cast<int32_t>(slot + __ffs(bits) - 1);
+    });
+    if (p0 < len && p0 + 32 + shift > t0) {
+        for (uint32_t k = 0; k < 32u && p0 + k < len; ++k) {
+            const int64_t token = static_cast<int64_t>(p0 + k) + shift;
+            if (token >= t0 && token < t1)
+                a.limits[token] = static_cast<int32_t>(base + before + __popc(vis & (0xFFFFFFFFu >> (31u - k))));
+        }
     }
     __syncthreads();
     for (uint32_t i = t; i < total; i += SL_NT) a.sel[r * a.sel_stride + base + i] = s_slot[i];
     if (t == 0 && (len <= SL_POS || chunk == (len - 1) / SL_POS)) a.sel_len[r] = static_cast<int32_t>(base + total);
+}
+
+// Bitmap containers are read where they lie; other layouts are written out as
+// flat words first.
+bool is_direct(const cr_gpu_roaring* bm)
+{
+    return bm->key_index && bm->n_containers > 0 && bm->n_bitmap_containers == bm->n_containers &&
+           reinterpret_cast<uintptr_t>(bm->bitmap_data) % 16 == 0;
+}
+
+// The bits of `bm` below `end`; `words` has room for n_words where they are written out.
+int set_bits(const cr_gpu_roaring* bm, bool direct, uint32_t* words, uint32_t n_words, uint32_t end, cr_stream_t stream,
+             SetBits* out)
+{
+    out->end = end;
+    if (!direct) {
+        out->flat = words;
+        return cr_decompress_to_bitset(bm, words, n_words, stream);
+    }
+    out->key_index = bm->key_index;
+    out->offsets = bm->offsets;
+    out->bitmaps = bm->bitmap_data;
+    out->max_key = bm->max_key;
+    if (bm->negated) {
+        out->flip = 0xFFFFFFFFu;
+        out->end = std::min(end, bm->universe_size);
+    }
+    return CR_OK;
 }
 
 bool power_of_two(uint32_t x) { return x && (x & (x - 1)) == 0; }
@@ -587,7 +640,6 @@ extern "C" int cr_paged_plan(const cr_gpu_roaring* free_pages, uint32_t n_pages,
     }
     hipStream_t s = as_stream(stream);
     PlanArgs a{};
-    a.free.n_pages = n_pages;
     a.n_quads = (n_pages + 127u) / 128u;
     a.n_blocks = (n_pages + PG_BLOCK - 1) / PG_BLOCK;
     a.page_lg = static_cast<uint32_t>(__builtin_ctz(page_size));
@@ -604,11 +656,7 @@ extern "C" int cr_paged_plan(const cr_gpu_roaring* free_pages, uint32_t n_pages,
     a.taken = d_taken;
     a.taken_cap = taken_cap;
     a.counts = d_counts;
-    // Bitmap containers are read where they lie; other layouts are written out as
-    // flat words first.
-    const bool direct = free_pages->key_index && free_pages->n_containers > 0 &&
-                        free_pages->n_bitmap_containers == free_pages->n_containers &&
-                        reinterpret_cast<uintptr_t>(free_pages->bitmap_data) % 16 == 0;
+    const bool direct = is_direct(free_pages);
     // One workgroup for a decoding step (64 requests, 8192 pages: 19.4 us in four launches, 9.0 in one).
     const bool small = a.n_quads <= PS_QUADS && n_requests <= PS_REQUESTS && slots_cap <= PS_TOKENS;
     Carver cv;
@@ -620,19 +668,7 @@ extern "C" int cr_paged_plan(const cr_gpu_roaring* free_pages, uint32_t n_pages,
     a.upto = sc.at<uint32_t>(o_upto);
     a.block_pre = sc.at<uint32_t>(o_pre);
     a.n_taken = sc.at<uint32_t>(o_taken);
-    if (direct) {
-        a.free.key_index = free_pages->key_index;
-        a.free.offsets = free_pages->offsets;
-        a.free.bitmaps = free_pages->bitmap_data;
-        a.free.max_key = free_pages->max_key;
-        if (free_pages->negated) {
-            a.free.flip = 0xFFFFFFFFu;
-            a.free.n_pages = std::min(n_pages, free_pages->universe_size);
-        }
-    } else {
-        a.free.flat = sc.at<uint4>(o_words);
-        CR_RET(cr_decompress_to_bitset(free_pages, sc.at<uint32_t>(o_words), a.n_quads * 4u, stream));
-    }
+    CR_RET(set_bits(free_pages, direct, sc.at<uint32_t>(o_words), a.n_quads * 4u, n_pages, stream, &a.free));
     CR_TIMED("pg_plan", s);
     if (small) {
         pg_small<<<1, PG_NT, 0, s>>>(a);
@@ -722,7 +758,8 @@ extern "C" int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, 
         return CR_ERR_UNSUPPORTED;
     }
     hipStream_t s = as_stream(stream);
-    a.n_words = static_cast<uint32_t>((n_slots + 31) / 32);
+    const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
+    const bool direct = is_direct(visible);
     a.table = d_table;
     a.cols = table_cols;
     a.table_stride = table_stride;
@@ -737,13 +774,12 @@ extern "C" int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, 
     a.sel_len = d_sel_len;
     a.limits = d_limits;
     Carver cv;
-    const size_t o_words = cv.add(a.n_words * 4ull);
+    const size_t o_words = cv.add(direct ? 0 : n_words * 4ull);
     const size_t o_counts = cv.add(a.chunks > 1 ? 4ull * a.chunks * n_requests : 0);
     Scratch sc;
-    CR_RET(sc.alloc(cv.total, s));
-    a.words = sc.at<uint32_t>(o_words);
+    if (cv.total) CR_RET(sc.alloc(cv.total, s));
     a.counts = sc.at<uint32_t>(o_counts);
-    CR_RET(cr_decompress_to_bitset(visible, sc.at<uint32_t>(o_words), a.n_words, stream));
+    CR_RET(set_bits(visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream, &a.visible));
     const uint32_t grid = a.chunks * n_requests;
     CR_TIMED("pg_select", s);
     if (a.chunks > 1) sl_count<<<grid, SL_NT, 0, s>>>(a);
