@@ -40,7 +40,7 @@ struct AttnArgs {
     // keys.  Otherwise the tiles' keys are cut into about `share` ranges of even
     // length, a workgroup each for every key head; their results, in fp32, are
     // joined by another kernel.
-    uint32_t n_tiles;
+    uint32_t n_tiles, n_ranges;
     uint32_t share, step, least_len;  // ranges are of a multiple of `step` keys, at least least_len
     uint2* ranges;    // [n_tiles] a tile's first range and how many it has
     float* part_o;    // [ranges][key heads][rows of a tile][dim]
@@ -490,6 +490,15 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         for (uint32_t i = 0; i < LOADS; ++i) v[i] = load8_once(vp + s_at[wave][1][i * PER + vrow]);
     };
 
+    // Pieces behind the head dimension are loaded from the row's beginning.  Those of
+    // keys become zeros, as the queries they meet; those of values reach only columns
+    // that are not stored.
+    const bool inside = vchunk * 8 < a.dim;
+    auto put_key = [&](uint32_t i, v8s x) {
+        const uint32_t r = i * PER + vrow;
+        *reinterpret_cast<v8s*>(lds_k + r * STRIDE + (vchunk ^ (r & KTURN)) * 8) = zero_unless(inside, x);
+    };
+
     uint32_t j0 = k0 + wave * DC_KEYS;
     int32_t slot = -1, next = -1, found = -1;
     if (j0 < k1) {
@@ -509,10 +518,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 #pragma unroll
             for (uint32_t x = 0; x < 2; ++x) s[b][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) {
-            const uint32_t r = i * PER + vrow;
-            *reinterpret_cast<v8s*>(lds_k + r * STRIDE + (vchunk ^ (r & KTURN)) * 8) = k[i];
-        }
+        for (uint32_t i = 0; i < LOADS; ++i) put_key(i, k[i]);
         if (more) {
             next = slots(j0 + DC_WAVES * DC_KEYS, found);
             note(next);
@@ -568,9 +574,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
                 }
         }
 
-        // The values of keys that no row sees count as zeros.  (Pieces behind the
-        // head dimension repeat the first one: they meet zero queries, and their
-        // columns are not stored.)
+        // The values of keys that no row sees count as zeros.
         uint64_t bad = 0;
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
@@ -640,11 +644,11 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         float top = NEG_INF;
 #pragma unroll
         for (uint32_t w = 0; w < DC_WAVES; ++w) top = fmaxf(top, s_m[w][r]);
-        const float fix = m[b] == NEG_INF ? 0.0f : exp2_fast((m[b] - top) * c);
+        const float fix = l[b] == 0.0f ? 0.0f : exp2_fast((m[b] - top) * c);  // NaN scores stay
         float* red = reinterpret_cast<float*>(s_mem) + (wave * 16 + c16) * RED;
 #pragma unroll
         for (uint32_t d = 0; d < BLOCKS; ++d)
-            *reinterpret_cast<f32x4*>(red + d * 16 + h * 4) = m[b] == NEG_INF ? f32x4{0, 0, 0, 0} : o[b][d] * fix;
+            *reinterpret_cast<f32x4*>(red + d * 16 + h * 4) = l[b] == 0.0f ? f32x4{0, 0, 0, 0} : o[b][d] * fix;
         __syncthreads();
         // 256 threads: 16 rows, 16 threads of a row, four dimensions at a time
         const uint32_t mine = threadIdx.x / 16, row = t.row0 + b * 16 + mine;
@@ -653,10 +657,10 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         for (uint32_t w = 0; w < DC_WAVES; ++w) mt = fmaxf(mt, s_m[w][b * 16 + mine]);
 #pragma unroll
         for (uint32_t w = 0; w < DC_WAVES; ++w) {
-            const float mw = s_m[w][b * 16 + mine];
-            lt += mw == NEG_INF ? 0.0f : s_l[w][b * 16 + mine] * exp2_fast((mw - mt) * c);
+            const float lw = s_l[w][b * 16 + mine];
+            lt += lw == 0.0f ? 0.0f : lw * exp2_fast((s_m[w][b * 16 + mine] - mt) * c);
         }
-        const bool none = mt == NEG_INF;
+        const bool none = lt == 0.0f;
         const float part = none ? 0.0f : 1.0f / lt;
         if (row < t.rows) {
             const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
@@ -795,20 +799,21 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     };
     auto v_turn = [](uint32_t r) { return (CHUNKS == 8 ? (r >> 1) & 1u : r & 3u) << 2; };
     // Each lane's 16 bytes go straight to the wave's next 1 KiB of LDS; which of a
-    // row's pieces a lane names turns the row.  Pieces behind the head dimension
-    // repeat the first one: they meet zero queries, and their columns are not stored.
+    // row's pieces a lane names turns the row.  Pieces behind the head dimension are
+    // not loaded: those of keys are zeros, as the queries they meet, and what lies in
+    // those of values reaches only columns that are not stored.
     auto load_keys = [&](uint32_t i, uint16_t* sk) {
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow, d = (lpos ^ (r & KTURN)) * 8;
-            load_to_lds(kp + s_koff[i % 4][r] + (d < a.dim ? d : 0u), sk + (x * PER + wave_row) * STRIDE);
+            if (d < a.dim) load_to_lds(kp + s_koff[i % 4][r] + d, sk + (x * PER + wave_row) * STRIDE);
         }
     };
     auto load_values = [&](uint32_t i, uint16_t* sv) {
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow, d = (lpos ^ v_turn(r)) * 8;
-            load_to_lds(vp + s_voff[i % 4][r] + (d < a.dim ? d : 0u), sv + (x * PER + wave_row) * STRIDE);
+            if (d < a.dim) load_to_lds(vp + s_voff[i % 4][r] + d, sv + (x * PER + wave_row) * STRIDE);
         }
     };
     // Values of keys that no row sees become zeros, and, in a tile that some rows
@@ -820,7 +825,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             const uint32_t r = x * PER + lrow;
             uint16_t* at = sv + r * STRIDE + lpos * 8;
             const v8s y = zero_unless((there >> r) & 1u, load8(at));
-            bad |= __ballot(has_special(y, E::EXP));
+            bad |= __ballot((lpos ^ v_turn(r)) * 8 < a.dim && has_special(y, E::EXP));
             *reinterpret_cast<v8s*>(at) = without_special(y, E::EXP);
         }
         if (bad && lane == 0) s_bad[i % 4] = 1;
@@ -838,6 +843,16 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             v_at[d] = r * STRIDE + (d ^ turn) * 32 + ((lane >> 4) & 1u) * 16 + (i16 & 3u) * 4;
     }
 
+    if (a.dim < DIM) {
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t r = x * PER + lrow, at = r * STRIDE + lpos * 8;
+            if ((lpos ^ (r & KTURN)) * 8 >= a.dim) {
+                *reinterpret_cast<v8s*>(s_k0 + at) = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+                *reinterpret_cast<v8s*>(s_k1 + at) = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+            }
+        }
+    }
     f32x16 s[HALVES];  // the scores of the tile to come
     float top;
     // Its products, as transposed blocks of 32 keys by 32 rows.
@@ -902,6 +917,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         load_keys(0, s_k0);
         load_values(0, s_v0);
         if (n_tiles > 1) load_keys(1, s_k1);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         __syncthreads();
         if (mine) {
             multiply(s_k0, s);
@@ -917,6 +933,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     // Tile i's probabilities and values, while the matrix units turn the next
     // tile's keys into scores; the keys behind those and the next values come in.
     auto tile = [&](uint32_t i, uint16_t* sk, uint16_t* next_k, uint16_t* sv, uint16_t* next_v) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads to LDS have arrived
         __syncthreads();  // keys i + 1 and values i are there, and nobody reads those before any more
         int32_t ahead = -1;
         if (wave == 0) ahead = find(i + 3);
@@ -993,7 +1010,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     }
 
     const float lt = l + __shfl_xor(l, 32, 64);
-    const bool none = m == NEG_INF;
+    const bool none = lt == 0.0f;
     const float part = none ? 0.0f : 1.0f / lt;
     if (row >= t.rows) return;
     const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
@@ -1032,8 +1049,12 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
         len = min(step, len - at * step);
     }
     const uint32_t row = (token - start) * group + head % group;
-    const uint2 range = a.ranges[tile_base(lo, static_cast<int32_t>(start), group, most) + row / most];
+    // (Offsets that do not ascend may lead to no tile's entry, but to none outside.)
+    const uint32_t tile = min(tile_base(lo, static_cast<int32_t>(start), group, most) + row / most, a.n_tiles - 1);
+    uint2 range = a.ranges[tile];
     if (range.y == 1) return;  // written already
+    range.x = min(range.x, a.n_ranges);
+    range.y = min(range.y, a.n_ranges - range.x);
     auto place = [&](uint32_t r) {
         return (static_cast<uint64_t>(range.x + r) * a.kv_heads + head / group) * most + row % most;
     };
@@ -1041,7 +1062,6 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
     for (uint32_t r = lane; r < range.y; r += 64) top = fmaxf(top, a.part_lse[place(r)]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const bool none = top == NEG_INF;
     const uint32_t slot = threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
     float sum = 0.0f;
     f32x4 x = {0, 0, 0, 0};
@@ -1062,6 +1082,7 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
             x += *reinterpret_cast<const f32x4*>(&s_o[i][d]);
             sum += s_sum[i];
         }
+        const bool none = sum == 0.0f;
         x *= none ? 0.0f : 1.0f / sum;
         if (d < a.dim) {
             const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
@@ -1206,7 +1227,9 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     const uint32_t per_wave = rows <= 16 ? 1 : rows <= 32 && a.dim <= 128 ? 2 : 0;
     const uint32_t most = per_wave ? 16 * per_wave : 128;
     const uint64_t tiles = static_cast<uint64_t>(p.n_tokens) * group / most + p.n_requests + 2;
-    if ((tiles * cache->n_heads) >> 31 || (static_cast<uint64_t>(p.n_tokens) * p.n_heads) >> 31) {
+    const uint64_t all_rows = static_cast<uint64_t>(p.n_tokens) * p.n_heads;
+    // a launch holds fewer than 2^32 threads
+    if ((tiles * cache->n_heads) >> 23 || all_rows >> 31) {
         set_error("cr_paged_attention: too many rows for one call");
         return CR_ERR_UNSUPPORTED;
     }
@@ -1223,7 +1246,7 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
     const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= 128 ? 2u : 1u) * cus / cache->n_heads + 1;
     const bool few = 2 * tiles_in_all <= held;
-    const bool cut = few || (per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held);
+    const bool cut = all_rows >> 24 ? false : few || (per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held);
     a.step = per_wave ? DC_KEYS * DC_WAVES : 64;
     a.least_len = !few ? 1024 : per_wave ? DC_KEYS * DC_WAVES : 256;
     uint64_t ranges = tiles;
@@ -1239,6 +1262,7 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
         a.part_lse = sc.at<float>(o_lse);
         a.ranges = sc.at<uint2>(o_at);
     }
+    a.n_ranges = static_cast<uint32_t>(ranges);
     const uint32_t grid = static_cast<uint32_t>(ranges * cache->n_heads);
     if (cache->dtype == CR_F16) return launch_attention<Half>(a, per_wave, grid, s);
     return launch_attention<BHalf>(a, per_wave, grid, s);

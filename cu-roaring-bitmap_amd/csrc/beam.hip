@@ -475,7 +475,7 @@ int launch_reorder(const ReorderArgs& a, uint32_t rows, hipStream_t s)
 {
     const uint64_t chunk = sizeof(U) * BR_PER * BR_NT;
     const uint64_t gx = (a.row_bytes + chunk - 1) / chunk;
-    if (gx >> 31) {
+    if (gx >> 24) {  // a launch holds fewer than 2^32 threads
         set_error("cr_beam_reorder: rows of %llu bytes are too long", static_cast<unsigned long long>(a.row_bytes));
         return CR_ERR_UNSUPPORTED;
     }
@@ -542,7 +542,7 @@ extern "C" int cr_beam_select(const void* d_scores, uint32_t dtype, uint32_t bat
     // 100003 bf16 scores: one 52 us in all, two 48.9, four 49.3, eight 50.2).
     a.per_wave = static_cast<uint32_t>(std::min<uint64_t>(2, std::max<uint64_t>(1, groups / (16ull * num_cus()))));
     a.parts = (a.n_groups + a.per_wave * (BS_NT / 64) - 1) / (a.per_wave * (BS_NT / 64));
-    if (groups >> 32 || (rows * a.parts) >> 31) {
+    if (groups >> 32 || (rows * a.parts) >> 24) {  // a launch holds fewer than 2^32 threads
         set_error("cr_beam_select: too many scores for one call");
         return CR_ERR_UNSUPPORTED;
     }

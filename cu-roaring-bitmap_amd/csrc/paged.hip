@@ -721,7 +721,7 @@ extern "C" int cr_paged_append(const void* d_k, const void* d_v, uint64_t k_toke
     const uint64_t pieces = static_cast<uint64_t>(n_tokens) * a.heads * a.units;
     if (pieces == 0) return CR_OK;
     const uint64_t grid = (pieces + AP_NT - 1) / AP_NT;
-    if (pieces >> 32) {
+    if (grid >> 24) {  // a launch holds fewer than 2^32 threads
         set_error("cr_paged_append: too many elements for one call");
         return CR_ERR_UNSUPPORTED;
     }
@@ -753,7 +753,7 @@ extern "C" int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, 
     const uint64_t n_slots = static_cast<uint64_t>(n_pages) * page_size;
     SelectArgs a{};
     a.chunks = static_cast<uint32_t>(std::max<uint64_t>(1, (room + SL_POS - 1) / SL_POS));
-    if (n_slots >> 31 || room >> 31 || n_tokens >> 31 || (static_cast<uint64_t>(a.chunks) * n_requests) >> 31) {
+    if (n_slots >> 31 || room >> 31 || n_tokens >> 31 || (static_cast<uint64_t>(a.chunks) * n_requests) >> 25) {
         set_error("cr_paged_select: supported up to 2^31 - 1 slots, positions and tokens");
         return CR_ERR_UNSUPPORTED;
     }

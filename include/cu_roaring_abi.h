@@ -433,8 +433,9 @@ int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, uint32_t pa
  * last ones; with `causal`, the one at position p sees positions [0, p] (none
  * where d_kv_len[r] says that p is negative), else all of [0, d_kv_len[r]).  With
  * a selection (cr_paged_select), the request's keys are d_sel's, and with
- * `causal` a token sees the first d_limits of them.  A token that sees nothing,
- * or that is in no request, gets zeros and -inf.  Query head h reads key head
+ * `causal` a token sees the first d_limits of them.  A token that sees nothing
+ * (or scores of -inf alone), or that is in no request, gets zeros and -inf; one
+ * that sees a score of +inf or NaN gets NaN.  Query head h reads key head
  * h / (n_heads / cache->n_heads).  Queries, cache and outputs are of one type,
  * with 16-byte aligned rows of a head dimension that is a multiple of 8, up to
  * 256; sums and softmax are in fp32, and the probabilities are rounded to the

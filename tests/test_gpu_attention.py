@@ -367,3 +367,71 @@ def test_long_and_short_requests(gpu, hints, density):
     """One long request among short ones: some tiles are cut into ranges and others are whole."""
     _say("attention of long and short requests", hints, density)
     Problem("float16", [40, 3, 1, 0, 70], [4700, 30, 1, 9, 90], 4, 2, 96, 16, seed=19, density=density).check(gpu, **hints)
+
+
+@pytest.mark.parametrize("dim", [64, 80, 128, 200])
+@pytest.mark.parametrize("new,kv", [([1], [300]), ([2], [9000]), ([70], [200])])
+def test_scores_that_are_not_finite(gpu, new, kv, dim):
+    """A score of -inf takes no part, one of +inf or NaN makes the answers that see it NaN, and no others."""
+    import torch
+    shape, at = (new, kv, 4, 2, dim, 16), kv[0] - new[0] - 5
+    p = Problem("bfloat16", *shape, seed=16)
+    ref = Problem("bfloat16", *shape, seed=16, density=1.0)
+    slot = int(p.table[0, at // 16]) * 16 + at % 16
+    ref.visible = torch.ones_like(ref.visible)
+    ref.visible[slot] = False
+    for x in (p, ref):
+        x.q[:, 0::2, 0], x.q[:, 1::2, 0] = 1.0, -1.0
+    _say("attention infinite score", new, kv, dim)
+    ref.check(gpu)
+    want, want_lse = ref.run(gpu)
+    p.kc[slot // 16, slot % 16, :, 0] = float("-inf")
+    out, lse = p.run(gpu)
+    assert np.allclose(out[:, 0::2], want[:, 0::2], rtol=2.0 ** -6, atol=2.0 ** -6)
+    assert np.allclose(lse[:, 0::2], want_lse[:, 0::2], rtol=1e-5)
+    assert np.isnan(out[:, 1::2]).all() and np.isnan(lse[:, 1::2]).all()
+    _say("attention NaN score", new, kv, dim)
+    p.kc[slot // 16, slot % 16, 0, 0] = float("nan")  # heads 0 and 1 read key head 0
+    out, lse = p.run(gpu)
+    assert np.isnan(out[:, :2]).all() and np.isnan(lse[:, :2]).all()
+    assert np.allclose(out[:, 2], want[:, 2], rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_no_score_is_finite(gpu, new):
+    _say("attention one key, not finite", new)
+    for bad, want in ((float("nan"), np.nan), (float("-inf"), 0.0)):
+        p = Problem("float16", [new], [new], 2, 1, 64, 16, seed=17)
+        p.q[:, :, 0] = 1.0
+        row = p.table[0].long()
+        for j in range(new):
+            p.kc[row[j // 16], j % 16, 0, 0] = bad
+        out, lse = p.run(gpu)
+        assert np.array_equal(out, np.full_like(out, want), equal_nan=True)
+        assert np.array_equal(lse, np.full_like(lse, np.nan if want else -np.inf), equal_nan=True)
+
+
+@pytest.mark.parametrize("hints", [{}, dict(max_new=1), dict(max_new=200)])
+def test_arrays_that_make_no_sense_stay_inside(gpu, hints):
+    """Offsets that do not ascend, lengths and slots out of range: answers of no meaning, inside the buffers."""
+    import torch
+    _say("attention with senseless arrays", hints)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    rng = np.random.default_rng(18)
+    q = torch.randn(90, 4, 64, device="cuda").half()
+    kc, vc = (torch.randn(600, 16, 2, 64, device="cuda").half() for _ in range(2))
+    room = 512 * 16
+    wild = lambda *s: torch.from_numpy(rng.integers(-2 ** 31, 2 ** 31, s).astype(np.int32)).cuda()  # noqa: E731
+    for n in (5, 100):
+        for starts in (torch.from_numpy(rng.integers(-40, 140, n + 1).astype(np.int32)).cuda(), wild(n + 1),
+                       torch.arange(n, -1, -1, **i32)):
+            for kv_len in (torch.full((n,), room, **i32), wild(n)):
+                for selection in (None, (wild(n, room), kv_len, wild(90))):
+                    table = torch.from_numpy(rng.integers(-5, 605, (n, 512)).astype(np.int32)).cuda()
+                    wide = torch.full((94, 4, 64), 7.0, device="cuda").half()
+                    lse = torch.full((94, 4), 7.0, device="cuda")
+                    gpu.paged_attention(q, kc, vc, table, starts, kv_len, wide[2:92], d_lse=lse[2:92],
+                                        selection=selection, **hints)
+                    torch.cuda.synchronize()
+                    for x in (wide, lse):
+                        assert torch.all(x[:2] == 7.0) and torch.all(x[92:] == 7.0)
