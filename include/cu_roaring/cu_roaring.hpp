@@ -10,4 +10,5 @@
 #include "cu_roaring/detail/to_csr.hpp"
 #include "cu_roaring/detail/serialize.hpp"
 #include "cu_roaring/detail/topk.hpp"
+#include "cu_roaring/detail/serving.hpp"
 #include "cu_roaring/device/make_view.hpp"
