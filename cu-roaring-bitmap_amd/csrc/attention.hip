@@ -57,18 +57,23 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // The two element types: rounding to nearest even, and the matrix products.
 struct Half {
-    static __device__ __forceinline__ float up(uint16_t x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); }
+    static __device__ __forceinline__ float up(uint16_t x)
+    {
+        return static_cast<float>(__builtin_bit_cast(_Float16, x));
+    }
     static __device__ __forceinline__ uint16_t down(float x)
     {
         return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
     }
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
     {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0,
+                                                      0);
     }
     static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
     {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0,
+                                                      0);
     }
     static constexpr uint32_t EXP = 0x7C00u;  // the exponent's bits: all set in infinities and NaN
 };
@@ -80,11 +85,13 @@ struct BHalf {
     }
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
     {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0,
+                                                       0);
     }
     static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
     {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0,
+                                                       0);
     }
     static constexpr uint32_t EXP = 0x7F80u;
 };
@@ -131,7 +138,8 @@ __device__ __forceinline__ v8s without_special(v8s x, uint32_t exp)
     v4u w = __builtin_bit_cast(v4u, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = (w[i] & exp) == exp ? 0u : 0xFFFFu, hi = (w[i] & (exp << 16)) == exp << 16 ? 0u : 0xFFFF0000u;
+        const uint32_t lo = (w[i] & exp) == exp ? 0u : 0xFFFFu;
+        const uint32_t hi = (w[i] & (exp << 16)) == exp << 16 ? 0u : 0xFFFF0000u;
         w[i] &= lo | hi;
     }
     return __builtin_bit_cast(v8s, w);
@@ -218,7 +226,8 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
             start = static_cast<uint32_t>(segment_start(a, i));
             end = static_cast<uint32_t>(segment_start(a, i + 1));
             keys = segment_keys(a, i);
-            const uint32_t rows = end > start ? (end - start) * group : 0u, mine = i < n ? (rows + most - 1) / most : 0u;
+            const uint32_t rows = end > start ? (end - start) * group : 0u;
+            const uint32_t mine = i < n ? (rows + most - 1) / most : 0u;
             uint32_t before = 0;
             for (uint32_t j = 0; j < n; ++j) {
                 const uint32_t other = lane_value(keys, j), tiles = lane_value(mine, j);
@@ -340,7 +349,8 @@ __device__ __forceinline__ int32_t slot_of(const AttnArgs& a, int32_t found, uin
     return page < a.n_pages ? static_cast<int32_t>(slot) : -1;
 }
 
-__device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, uint64_t page_stride, uint64_t slot_stride)
+__device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, uint64_t page_stride,
+                                              uint64_t slot_stride)
 {
     const uint32_t at = static_cast<uint32_t>(max(slot, 0));
     return (at >> page_lg) * page_stride + (at & ((1u << page_lg) - 1u)) * slot_stride;
@@ -353,7 +363,8 @@ __device__ __forceinline__ v8s load_query(const AttnArgs& a, const Work& t, uint
     const uint32_t group = a.heads / a.kv_heads;
     v8s x = {0, 0, 0, 0, 0, 0, 0, 0};
     if (row < t.rows && d < a.dim && a.scale != 0.0f) {
-        x = load8(a.q + static_cast<uint64_t>(t.token0 + row / group) * a.q_token + (kh * group + row % group) * a.q_head + d);
+        const uint64_t token = static_cast<uint64_t>(t.token0) + row / group;
+        x = load8(a.q + token * a.q_token + (kh * group + row % group) * a.q_head + d);
         if (a.scale < 0.0f) x ^= static_cast<short>(0x8000);
     }
     return x;
@@ -368,8 +379,8 @@ __device__ __forceinline__ float score_scale(const AttnArgs& a)
 // where another kernel joins the ranges of keys.  `place` numbers the rows of
 // the ranges' results.
 template <class E>
-__device__ __forceinline__ void store_row(const AttnArgs& a, E, const Work& t, uint64_t place, uint32_t token, uint32_t head,
-                                          uint32_t d, f32x4 x)
+__device__ __forceinline__ void store_row(const AttnArgs& a, E, const Work& t, uint64_t place, uint32_t token,
+                                          uint32_t head, uint32_t d, f32x4 x)
 {
     if (!t.whole) {
         *reinterpret_cast<f32x4*>(a.part_o + place * a.dim + d) = x;
@@ -381,7 +392,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, E, const Work& t, u
 }
 
 // lse2: base 2
-__device__ __forceinline__ void store_lse(const AttnArgs& a, const Work& t, uint64_t place, uint32_t token, uint32_t head, float lse2)
+__device__ __forceinline__ void store_lse(const AttnArgs& a, const Work& t, uint64_t place, uint32_t token,
+                                          uint32_t head, float lse2)
 {
     if (!t.whole)
         a.part_lse[place] = lse2;
@@ -725,7 +737,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     constexpr uint32_t STEPS = DIM / 16, BLOCKS = DIM / 32, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
     constexpr uint32_t KEYS = tile_keys(DIM), HALVES = KEYS / 32;
     constexpr uint64_t ALL = ~0ull >> (64 - KEYS);
-    constexpr uint32_t PER = TL_NT / CHUNKS, LOADS = KEYS / PER;  // rows that the workgroup loads at once, and how often
+    constexpr uint32_t PER = TL_NT / CHUNKS, LOADS = KEYS / PER;  // rows that the workgroup loads at once, how often
     constexpr uint32_t KTURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
     // separate arrays: what is read is not what is being loaded
     __shared__ alignas(16) uint16_t s_k0[KEYS * STRIDE], s_k1[KEYS * STRIDE];
@@ -1221,7 +1233,8 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
 
     // Rows of a request that share a key head, as far as the caller says.
     const uint32_t group = p.n_heads / cache->n_heads, cus = num_cus();
-    const uint64_t typical = p.max_new ? p.max_new : (p.n_tokens + std::max(1u, p.n_requests) - 1) / std::max(1u, p.n_requests);
+    const uint64_t requests = std::max(1u, p.n_requests);
+    const uint64_t typical = p.max_new ? p.max_new : (p.n_tokens + requests - 1) / requests;
     const uint64_t rows = typical * group;
     // blocks of 16 rows (two of long rows do not fit the registers), or tiles
     const uint32_t per_wave = rows <= 16 ? 1 : rows <= 32 && a.dim <= 128 ? 2 : 0;
@@ -1242,11 +1255,12 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     // reading the lengths and joining cost more than they even out (256 of up to
     // 1024 keys: uncut 110 us, cut 160; of up to 4096 372 and 389; 48 of up to 2048
     // with 16 heads of 64 dimensions 53 and 60).
-    const uint64_t tiles_in_all = (rows + most - 1) / most * std::max(1u, p.n_requests);
+    const uint64_t tiles_in_all = (rows + most - 1) / most * requests;
     const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
     const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= 128 ? 2u : 1u) * cus / cache->n_heads + 1;
     const bool few = 2 * tiles_in_all <= held;
-    const bool cut = all_rows >> 24 ? false : few || (per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held);
+    const bool long_ones = per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held;
+    const bool cut = (few || long_ones) && all_rows >> 24 == 0;
     a.step = per_wave ? DC_KEYS * DC_WAVES : 64;
     a.least_len = !few ? 1024 : per_wave ? DC_KEYS * DC_WAVES : 256;
     uint64_t ranges = tiles;

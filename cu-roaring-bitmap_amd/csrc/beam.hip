@@ -82,6 +82,12 @@ __device__ __forceinline__ float total_from(uint32_t order)
     return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
 
+// Lane `lane`'s value.
+__device__ __forceinline__ uint32_t lane_word(uint32_t x, uint32_t lane)
+{
+    return static_cast<uint32_t>(__shfl(static_cast<int>(x), static_cast<int>(lane), 64));
+}
+
 // A beam's row.  Tokens are read 16 bytes at a time from the row's first
 // boundary on; the few before it go with the first group and those behind the
 // last whole piece with the group they lie in, one by one.
@@ -98,7 +104,8 @@ struct Row {
         const uint64_t row = static_cast<uint64_t>(b) * a.beams + w;
         p = static_cast<const T*>(a.x) + b * a.batch_stride + w * a.beam_stride;
         vocab = a.vocab;
-        head = min(vocab, static_cast<uint32_t>((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / static_cast<uint32_t>(sizeof(T)));
+        const uint32_t past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+        head = min(vocab, ((16u - past) & 15u) / static_cast<uint32_t>(sizeof(T)));
         pieces = (vocab - head) / PER;
         words = a.allowed.words ? a.allowed.words + row * a.allowed.stride : nullptr;
         cum = a.cum[row];
@@ -106,7 +113,10 @@ struct Row {
         lse = has_lse ? a.lse[row] : 0.0f;
     }
     __device__ __forceinline__ float total(float x) const { return has_lse ? cum + (x - lse) : cum + x; }
-    __device__ __forceinline__ uint32_t first(uint32_t g, uint32_t u) const { return (g * UNROLL + u) * 64u + __lane_id(); }
+    __device__ __forceinline__ uint32_t first(uint32_t g, uint32_t u) const
+    {
+        return (g * UNROLL + u) * 64u + __lane_id();
+    }
 
     // The lane's pieces of group g; lanes past the last piece read it again.
     __device__ __forceinline__ void load(uint32_t g, cr_v4u (&x)[UNROLL]) const
@@ -121,7 +131,7 @@ struct Row {
     {
         const uint32_t w = min((head + g * SIZE) / 32u + __lane_id(), (vocab - 1u) / 32u);
         if (!s.offsets) return words[w];
-        return words[static_cast<uint32_t>(__shfl(static_cast<int>(at), static_cast<int>(w / 2048u), 64)) + w % 2048u] ^ s.flip;
+        return words[lane_word(at, w / 2048u) + w % 2048u] ^ s.flip;
     }
     // Which tokens of the lane's pieces there are and may follow.
     __device__ __forceinline__ void masks(uint32_t word, uint32_t g, uint32_t (&on)[UNROLL]) const
@@ -131,9 +141,8 @@ struct Row {
             const uint32_t all = first(g, u) < pieces ? (1u << PER) - 1u : 0u;
             if (words) {
                 const uint32_t bit = (head + g * SIZE) % 32u + (u * 64u + __lane_id()) * PER;
-                const uint32_t lo = static_cast<uint32_t>(__shfl(static_cast<int>(word), static_cast<int>(bit / 32u), 64));
-                const uint32_t hi = static_cast<uint32_t>(__shfl(static_cast<int>(word), static_cast<int>(bit / 32u + 1u), 64));
-                on[u] = all & __builtin_amdgcn_alignbit(hi, lo, bit % 32u);
+                on[u] = all & __builtin_amdgcn_alignbit(lane_word(word, bit / 32u + 1u), lane_word(word, bit / 32u),
+                                                        bit % 32u);
             } else {
                 on[u] = all;
             }
@@ -153,7 +162,8 @@ struct Row {
         if (g == pieces * PER / SIZE && lane >= 32u) v = min(vocab, tail + lane - 32u);
         if (v < vocab && words) {
             const uint32_t w = v / 32u;
-            const uint32_t bits = words[s.offsets ? s.offsets[w / 2048u] / 4u + w % 2048u : w] ^ (s.offsets ? s.flip : 0u);
+            const uint32_t at = s.offsets ? s.offsets[w / 2048u] / 4u + w % 2048u : w;
+            const uint32_t bits = words[at] ^ (s.offsets ? s.flip : 0u);
             if (!((bits >> (v % 32u)) & 1u)) v = vocab;
         }
         return v;
@@ -183,9 +193,9 @@ __device__ __forceinline__ float wave_max(float v)
 // Totals rise with the scores (each rounding keeps their order), so that a
 // group's largest total is its largest score's: one comparison a token, and the
 // sum once a group.  Bound by reading the scores: 102 MB of bf16 in 21 us, 4.9
-// TB/s (with a dependent load or a branch between a wave's loads 30 to 41).  SPARSE: scores are read only
-// where a token of theirs is allowed, once the masks are there; else both are
-// on their way together.
+// TB/s (with a dependent load or a branch between a wave's loads 30 to 41).
+// SPARSE: scores are read only where a token of theirs is allowed, once the masks
+// are there; else both are on their way together.
 template <class T, bool SPARSE>
 __global__ __launch_bounds__(BS_NT) void bs_scan(BeamArgs a, uint32_t* __restrict__ gmax)
 {
@@ -306,10 +316,12 @@ __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __rest
         uint32_t in = 0;
 #pragma unroll
         for (uint32_t j = 0; j < OWN; ++j) {
-            const uint32_t gi = g0 + t * OWN + j, most = gi < n_groups ? gm[gi] : 0u, w = gi / a.n_groups, g = gi % a.n_groups;
+            const uint32_t gi = g0 + t * OWN + j, most = gi < n_groups ? gm[gi] : 0u;
+            const uint32_t w = gi / a.n_groups, g = gi % a.n_groups;
             // no token of the group is placed before this one
             const uint32_t place = w * a.vocab + (g ? g * R::SIZE : 0u);
-            if (most != 0 && ((static_cast<uint64_t>(most) << 32) | static_cast<uint32_t>(~place)) >= s_thr) in |= 1u << j;
+            const uint64_t key = (static_cast<uint64_t>(most) << 32) | static_cast<uint32_t>(~place);
+            if (most != 0 && key >= s_thr) in |= 1u << j;
         }
         uint32_t listed;
         uint32_t at = block_excl_scan<NT>(__popc(in), s_scan, listed);
@@ -515,8 +527,8 @@ extern "C" int cr_beam_select(const void* d_scores, uint32_t dtype, uint32_t bat
         return CR_ERR_INVALID;
     }
     if (k > BS_KMAX || (static_cast<uint64_t>(beams) * vocab) >> 31 || batch >> 20) {
-        set_error("cr_beam_select: supported up to k %u, 2^31 - 1 continuations of an answer and 2^20 - 1 answers (k %u)",
-                  BS_KMAX, k);
+        set_error("cr_beam_select: supported up to k %u, 2^31 - 1 continuations of an answer and 2^20 - 1 answers "
+                  "(k %u)", BS_KMAX, k);
         return CR_ERR_UNSUPPORTED;
     }
     hipStream_t s = as_stream(stream);
@@ -549,8 +561,9 @@ extern "C" int cr_beam_select(const void* d_scores, uint32_t dtype, uint32_t bat
     // Bitmap containers for all keys are read where they lie; other layouts are
     // written out as flat words first.
     const uint32_t n_words = (vocab + 31) / 32;
-    const bool direct = allowed && allowed->n_containers == (vocab + 65535) / 65536 && allowed->n_containers <= 64 && allowed->max_key + 1 == allowed->n_containers &&
-                        allowed->n_bitmap_containers == allowed->n_containers &&
+    const uint32_t keys = (vocab + 65535) / 65536;
+    const bool direct = allowed && keys <= 64 && allowed->n_containers == keys && allowed->max_key + 1 == keys &&
+                        allowed->n_bitmap_containers == keys &&
                         (!allowed->negated || allowed->universe_size >= vocab);
     const bool flat = allowed && !direct;
     Carver cv;
@@ -595,7 +608,8 @@ extern "C" int cr_beam_reorder(const void* d_src, const int32_t* d_parents, uint
         set_error("cr_beam_reorder: the states are reordered into another buffer");
         return CR_ERR_INVALID;
     }
-    ReorderArgs a{s0, t0, d_parents, d_len, beams_in, beams_out, row_bytes, d_len ? unit_bytes : 1, src_stride, dst_stride};
+    ReorderArgs a{s0,        t0,        d_parents,              d_len,      beams_in,  beams_out,
+                  row_bytes, d_len ? unit_bytes : 1, src_stride, dst_stride};
     const uint64_t all = reinterpret_cast<uintptr_t>(d_src) | reinterpret_cast<uintptr_t>(d_dst) | row_bytes |
                          src_stride | dst_stride | (d_len ? unit_bytes : 0);
     hipStream_t s = as_stream(stream);

@@ -19,6 +19,7 @@ namespace {
 
 constexpr int PG_NT = 1024;             // the plan's workgroup
 constexpr uint32_t PG_BLOCK = 2048;     // pages a block of the free set holds: 64 words
+constexpr uint32_t PG_GROUP = 64;       // blocks that a workgroup of pg_count counts
 constexpr int PG_TAKE_NT = 256;
 constexpr uint32_t PG_TOKENS = 2048;    // tokens a workgroup of the slot map writes
 constexpr int PG_FILL_NT = 256;
@@ -98,9 +99,11 @@ struct PlanArgs {
     int32_t* taken;
     uint32_t taken_cap;
     int32_t* counts;
-    uint32_t* upto;       // [n_requests + 1] pages that the requests before take, in order
-    uint32_t* block_pre;  // [n_blocks] free pages before each block
-    uint32_t* n_taken;
+    uint32_t* upto;      // [n_requests + 1] pages that the requests before want
+    uint32_t* block_n;   // [n_blocks] free pages of each block
+    uint32_t* group_n;   // [n_groups] and of PG_GROUP blocks
+    uint32_t n_groups;
+    uint64_t* wanted;    // the pages that all requests want; those of requests that can not be
 };
 
 // Pages [128 q, 128 q + 128) of the free set for N values of q, without bits
@@ -149,7 +152,10 @@ __device__ __forceinline__ uint4 free_quad(const SetBits& f, uint32_t q, uint32_
     return x[0];
 }
 
-__device__ __forceinline__ uint32_t count_quad(uint4 x) { return __popc(x.x) + __popc(x.y) + __popc(x.z) + __popc(x.w); }
+__device__ __forceinline__ uint32_t count_quad(uint4 x)
+{
+    return __popc(x.x) + __popc(x.y) + __popc(x.z) + __popc(x.w);
+}
 
 // The place of the n-th set bit of w (it has more than n).
 __device__ __forceinline__ uint32_t nth_bit(uint32_t w, uint32_t n)
@@ -180,17 +186,25 @@ struct Request {
     bool fits;  // lengths are not negative and the row holds the pages
 };
 
+__device__ __forceinline__ uint64_t pages_held(const PlanArgs& a, int32_t cached)
+{
+    return (static_cast<uint64_t>(max(cached, 0)) + ((1ull << a.page_lg) - 1)) >> a.page_lg;
+}
+
 __device__ __forceinline__ Request request_of(const PlanArgs& a, int32_t c, int32_t n)
 {
     const uint64_t page = 1ull << a.page_lg;
     Request q;
     q.tokens = n > 0 ? static_cast<uint64_t>(n) : 0ull;
     const uint64_t before = c > 0 ? static_cast<uint64_t>(c) : 0ull;
-    q.held = (before + page - 1) >> a.page_lg;
+    q.held = pages_held(a, c);
     q.most = (before + q.tokens + page - 1) >> a.page_lg;
     q.fits = c >= 0 && n >= 0 && q.most <= a.cols && before + q.tokens <= 0x7FFFFFFFull;
     return q;
 }
+
+// The pages that a request wants.
+__device__ __forceinline__ uint64_t pages_of(const Request& q) { return q.fits ? q.most - q.held : 0ull; }
 
 // The last entry of a[lo, hi) that is at most v (a[lo] <= v, ascending).
 template <class T>
@@ -226,17 +240,22 @@ __device__ __forceinline__ void wave_range(const T* a, uint32_t n, T v0, T v1, u
     hi = l1 + 1;
 }
 
-// The requests' token offsets, the pages that they take in order and which of
-// them get theirs, of n_free; a workgroup's work.  `upto` may lie in LDS.
-// c, n: the lengths of request threadIdx.x, loaded before.
-__device__ __forceinline__ void plan_requests(const PlanArgs& a, int32_t c, int32_t n, uint64_t n_free, uint32_t* upto,
-                                              uint64_t* s_scan, uint64_t* s_taken, uint64_t* s_missing)
+// The requests' token offsets and the pages wanted before each of them, a
+// workgroup's work; `upto` may lie in LDS.  c, n: the lengths of request
+// threadIdx.x, loaded before.  Returns the pages wanted in all; *s_unfit receives
+// those of requests that can not be, whatever is free.  The offsets go to
+// a.starts, or to s_start if it is there.  ONCE: there are at most PG_NT requests
+// (without a loop around it, a decoding step's plan takes 8.4 instead of 9.9 us).
+template <bool ONCE>
+__device__ __forceinline__ uint64_t scan_requests(const PlanArgs& a, int32_t c, int32_t n, uint32_t* upto,
+                                                  uint64_t* s_scan, uint64_t* s_unfit, int32_t* s_start)
 {
     const uint32_t t = threadIdx.x;
     uint64_t tokens = 0, pages = 0;
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += PG_NT) {
+    if (t == 0) *s_unfit = 0;
+    for (uint32_t r0 = 0; r0 < (ONCE ? 1u : a.n_requests); r0 += PG_NT) {
         const uint32_t r = r0 + t;
-        Request q{0, 0, 0, false};
+        Request q{0, 0, 0, true};
         if (r < a.n_requests) {
             if (r0) {
                 c = a.cached[r];
@@ -244,46 +263,65 @@ __device__ __forceinline__ void plan_requests(const PlanArgs& a, int32_t c, int3
             }
             q = request_of(a, c, n);
         }
-        const uint64_t need = q.fits ? q.most - q.held : 0ull;
         uint64_t all_tokens, all_pages;
         const uint64_t at = tokens + block_excl_scan_u64<PG_NT>(q.tokens, s_scan, all_tokens);
-        const uint64_t before = pages + block_excl_scan_u64<PG_NT>(need, s_scan, all_pages);
-        uint64_t upto_end = 0, lacking = 0;
+        const uint64_t before = pages + block_excl_scan_u64<PG_NT>(pages_of(q), s_scan, all_pages);
         if (r < a.n_requests) {
-            const bool granted = q.fits && (need == 0 || before + need <= n_free);
-            a.starts[r] = static_cast<int32_t>(min(at, static_cast<uint64_t>(0x7FFFFFFF)));
-            a.kv_len[r] = granted ? c + n : 0;
+            const int32_t start = static_cast<int32_t>(min(at, static_cast<uint64_t>(0x7FFFFFFF)));
+            if (s_start)
+                s_start[r] = start;
+            else
+                a.starts[r] = start;
             upto[r] = static_cast<uint32_t>(min(before, static_cast<uint64_t>(0xFFFFFFFF)));
-            upto_end = granted && need ? before + need : 0ull;
-            lacking = granted ? 0ull : q.most - q.held;
         }
-        // the pages taken end where the last of those granted some do; one lane of a wave adds its own
-        for (int o = 32; o > 0; o >>= 1) {
-            upto_end = max(upto_end, static_cast<uint64_t>(__shfl_xor(upto_end, o, 64)));
-            lacking += __shfl_xor(lacking, o, 64);
-        }
-        if (__lane_id() == 0) {
-            if (upto_end) atomicMax(reinterpret_cast<unsigned long long*>(s_taken), static_cast<unsigned long long>(upto_end));
-            if (lacking) atomicAdd(reinterpret_cast<unsigned long long*>(s_missing), static_cast<unsigned long long>(lacking));
-        }
+        if (!q.fits)
+            atomicAdd(reinterpret_cast<unsigned long long*>(s_unfit), static_cast<unsigned long long>(q.most - q.held));
         tokens += all_tokens;
         pages += all_pages;
     }
-    __syncthreads();
     if (t == 0) {
-        const uint64_t most = 0x7FFFFFFF;
-        a.starts[a.n_requests] = static_cast<int32_t>(min(tokens, most));
-        a.counts[0] = static_cast<int32_t>(min(tokens, most));
-        a.counts[1] = static_cast<int32_t>(min(*s_taken, most));
-        a.counts[2] = static_cast<int32_t>(min(*s_missing, most));
+        upto[a.n_requests] = static_cast<uint32_t>(min(pages, static_cast<uint64_t>(0xFFFFFFFF)));
+        const int32_t all = static_cast<int32_t>(min(tokens, static_cast<uint64_t>(0x7FFFFFFF)));
+        if (s_start)
+            s_start[a.n_requests] = all;
+        else
+            a.starts[a.n_requests] = a.counts[0] = all;
     }
+    __syncthreads();
+    return pages;
 }
 
-// Page `id` is the rank-th taken: into the list, and into the table of request r.
-__device__ __forceinline__ void place_page(const PlanArgs& a, uint32_t rank, uint32_t id, uint32_t r, uint32_t before)
+// Of n_free pages, those that are taken: what the requests want up to the first
+// whose pages are not all there.  (Later ones want no fewer before them, so that
+// only those that want none still get theirs.)
+__device__ __forceinline__ uint32_t pages_taken(const uint32_t* upto, uint32_t n_requests, uint32_t n_free)
 {
+    const uint32_t all = upto[n_requests];
+    return all <= n_free ? all : upto[last_at_most(upto, 0u, n_requests + 1, n_free)];
+}
+
+// The length of a request's cache after its new tokens, 0 where it is refused.
+__device__ __forceinline__ int32_t planned_len(const PlanArgs& a, int32_t c, int32_t n, uint32_t before,
+                                               uint32_t n_taken)
+{
+    const Request q = request_of(a, c, n);
+    const uint64_t need = pages_of(q);
+    return q.fits && (need == 0 || before + need <= n_taken) ? c + n : 0;
+}
+
+__device__ __forceinline__ void set_counts(const PlanArgs& a, uint32_t n_taken, uint64_t wanted, uint64_t unfit)
+{
+    a.counts[1] = static_cast<int32_t>(n_taken);
+    a.counts[2] = static_cast<int32_t>(min(wanted - n_taken + unfit, static_cast<uint64_t>(0x7FFFFFFF)));
+}
+
+// Page `id` is the rank-th taken: into the list, and into the table of request
+// r, which holds `cached` tokens and before which `before` pages are taken.
+__device__ __forceinline__ void place_page(const PlanArgs& a, uint32_t rank, uint32_t id, uint32_t r, int32_t cached,
+                                           uint32_t before)
+{
+    const uint64_t col = pages_held(a, cached) + (rank - before);
     if (rank < a.taken_cap) a.taken[rank] = static_cast<int32_t>(id);
-    const uint64_t col = request_of(a, a.cached[r], a.fresh[r]).held + (rank - before);
     if (col < a.cols) a.table[r * a.table_stride + col] = static_cast<int32_t>(id);
 }
 
@@ -295,59 +333,79 @@ __device__ __forceinline__ int64_t slot_at(const PlanArgs& a, uint32_t r, int32_
     return (static_cast<int64_t>(a.table[r * a.table_stride + col]) << a.page_lg) + (pos & ((1u << a.page_lg) - 1u));
 }
 
-// One workgroup: the free pages before each block of them, then the requests.
-__global__ __launch_bounds__(PG_NT) void pg_scan(PlanArgs a)
+// A large plan, in three launches: the first two are bound by the latency of a few
+// dependent loads, the last writes 8 bytes a token (1024 requests, 4.2 million
+// tokens, 2^20 pages: 4.5 + 8.3 + 12 us; the writing alone takes 7.1 at the card's
+// copy rate; one workgroup for all the counting and the scan took 10.6).
+//
+// The first workgroup scans the requests, the others count the free pages of
+// PG_GROUP blocks each, a row of 16 lanes a block.
+__global__ __launch_bounds__(PG_NT) void pg_count(PlanArgs a)
 {
-    constexpr uint32_t QPB = PG_BLOCK / 128u, AHEAD = 8;  // pieces of a block (a row of 16 lanes), loads in flight
-    constexpr uint32_t BLOCKS = AHEAD * PG_NT / QPB;
-    __shared__ uint64_t s_scan[PG_NT / 64];
-    __shared__ uint64_t s_taken, s_missing;
-    __shared__ uint32_t s_count[BLOCKS];
+    constexpr uint32_t QPB = PG_BLOCK / 128u;  // pieces of a block
+    static_assert(QPB == 16 && PG_GROUP * QPB == PG_NT, "a row of 16 lanes per block");
+    __shared__ uint64_t s_scan[PG_NT / 64], s_unfit;
+    __shared__ uint32_t s_sum[PG_NT / 64];
     const uint32_t t = threadIdx.x;
-    if (t == 0) s_taken = s_missing = 0;
-    const int32_t c = t < a.n_requests ? a.cached[t] : 0, n = t < a.n_requests ? a.fresh[t] : 0;
-    static_assert(QPB == 16 && BLOCKS <= PG_NT, "a row of 16 lanes per block, a thread per count");
-    uint64_t n_free = 0;
-    for (uint32_t b0 = 0; b0 < a.n_blocks; b0 += BLOCKS) {
-        uint4 x[AHEAD];
-        uint32_t q[AHEAD];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) q[i] = b0 * QPB + i * PG_NT + t;
-        free_quads(a.free, q, a.n_quads, x);
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) {
-            uint32_t k = count_quad(x[i]);
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) k += static_cast<uint32_t>(__shfl_xor(static_cast<int>(k), o, 64));
-            if (t % QPB == 0) s_count[i * (PG_NT / QPB) + t / QPB] = k;
+    if (blockIdx.x == 0) {
+        const int32_t c = t < a.n_requests ? a.cached[t] : 0, n = t < a.n_requests ? a.fresh[t] : 0;
+        const uint64_t wanted = scan_requests<false>(a, c, n, a.upto, s_scan, &s_unfit, nullptr);
+        if (t == 0) {
+            a.wanted[0] = wanted;
+            a.wanted[1] = s_unfit;
         }
-        __syncthreads();
-        uint64_t all;
-        const uint64_t pre = block_excl_scan_u64<PG_NT>(t < BLOCKS ? s_count[t] : 0u, s_scan, all);
-        if (t < BLOCKS && b0 + t < a.n_blocks) a.block_pre[b0 + t] = static_cast<uint32_t>(n_free + pre);
-        n_free += all;
+        return;
     }
+    const uint32_t group = blockIdx.x - 1, q = group * PG_NT + t, block = q / QPB;
+    uint32_t k = count_quad(free_quad(a.free, q, a.n_quads));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) k += static_cast<uint32_t>(__shfl_xor(static_cast<int>(k), o, 64));
+    if (t % QPB == 0 && block < a.n_blocks) a.block_n[block] = k;
+    k += static_cast<uint32_t>(__shfl_xor(static_cast<int>(k), 16, 64));
+    k += static_cast<uint32_t>(__shfl_xor(static_cast<int>(k), 32, 64));
+    if (__lane_id() == 0) s_sum[t / 64] = k;
     __syncthreads();
-    plan_requests(a, c, n, n_free, a.upto, s_scan, &s_taken, &s_missing);
-    if (t == 0) *a.n_taken = static_cast<uint32_t>(s_taken);
+    if (t == 0) {
+        uint32_t all = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < PG_NT / 64; ++i) all += s_sum[i];
+        a.group_n[group] = all;
+    }
 }
 
 // A workgroup per block of the free set: its pages that are taken, into the
-// list of them and into the tables of the requests that take them.
+// list of them and into the tables of the requests that take them.  The
+// workgroups behind those tell which requests got their pages.
 __global__ __launch_bounds__(PG_TAKE_NT) void pg_take(PlanArgs a)
 {
     constexpr uint32_t PER = PG_BLOCK / PG_TAKE_NT;  // pages a thread looks at
     __shared__ uint32_t s_scan[PG_TAKE_NT / 64];
     __shared__ uint16_t s_id[PG_BLOCK];
-    const uint32_t n_taken = *a.n_taken, base = a.block_pre[blockIdx.x], t = threadIdx.x;
-    if (base >= n_taken) return;
+    const uint32_t t = threadIdx.x, group = blockIdx.x / PG_GROUP;
     const uint32_t first = blockIdx.x * PG_BLOCK + t * PER;
-    uint32_t bits = 0;
+    uint32_t bits = 0, before = 0, in_all = 0;
     if (first / 128u < a.n_quads) {
         const uint4 x = free_quad(a.free, first / 128u, a.n_quads);
         const uint32_t w = first / 32u % 4u;
         bits = ((w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w) >> (first % 32u)) & ((1u << PER) - 1u);
     }
+    for (uint32_t i = t; i < a.n_groups; i += PG_TAKE_NT) {
+        const uint32_t n = a.group_n[i];
+        in_all += n;
+        before += i < group ? n : 0u;
+    }
+    if (t < blockIdx.x % PG_GROUP && blockIdx.x < a.n_blocks) before += a.block_n[group * PG_GROUP + t];
+    uint32_t base, n_free;
+    block_excl_scan<PG_TAKE_NT>(before, s_scan, base);
+    block_excl_scan<PG_TAKE_NT>(in_all, s_scan, n_free);
+    const uint32_t n_taken = pages_taken(a.upto, a.n_requests, n_free);
+    if (blockIdx.x >= a.n_blocks) {
+        const uint32_t r = (blockIdx.x - a.n_blocks) * PG_TAKE_NT + t;
+        if (r < a.n_requests) a.kv_len[r] = planned_len(a, a.cached[r], a.fresh[r], a.upto[r], n_taken);
+        if (r == 0) set_counts(a, n_taken, a.wanted[0], a.wanted[1]);
+        return;
+    }
+    if (base >= n_taken) return;
     uint32_t total;
     uint32_t at = block_excl_scan<PG_TAKE_NT>(__popc(bits), s_scan, total);
     for (; bits; bits &= bits - 1u) s_id[at++] = static_cast<uint16_t>(t * PER + __ffs(bits) - 1);
@@ -358,58 +416,69 @@ __global__ __launch_bounds__(PG_TAKE_NT) void pg_take(PlanArgs a)
     wave_range(a.upto, a.n_requests, base, base + n - 1, lo, hi);
     for (uint32_t i = t; i < n; i += PG_TAKE_NT) {
         const uint32_t rank = base + i, r = last_at_most(a.upto, lo, hi, rank);
-        place_page(a, rank, blockIdx.x * PG_BLOCK + s_id[i], r, a.upto[r]);
+        place_page(a, rank, blockIdx.x * PG_BLOCK + s_id[i], r, a.cached[r], a.upto[r]);
     }
 }
 
-// The slot of each new token, from the tables as pg_take left them.  Two tokens
-// a thread at a time; where the workgroup's tokens are one request's (a prompt),
-// nothing is searched.
+// The slot of each new token, from the tables as pg_take left them, two tokens a
+// thread at a time, past the caches (12 us; through them 13.5).  The requests of
+// the workgroup's tokens are kept in LDS (searched in memory, 15.9 us).
 __global__ __launch_bounds__(PG_FILL_NT) void pg_slots(PlanArgs a, bool pairs)
 {
-    const uint32_t first = blockIdx.x * PG_TOKENS;
+    __shared__ int32_t s_start[PG_FILL_NT], s_kv[PG_FILL_NT], s_cached[PG_FILL_NT];
+    const uint32_t first = blockIdx.x * PG_TOKENS, t = threadIdx.x;
     const uint32_t total = min(a.slots_cap, static_cast<uint32_t>(a.starts[a.n_requests]));
     uint32_t lo, hi;
-    wave_range(a.starts, a.n_requests, static_cast<int32_t>(first), static_cast<int32_t>(min(first + PG_TOKENS, a.slots_cap) - 1), lo, hi);
+    wave_range(a.starts, a.n_requests, static_cast<int32_t>(first),
+               static_cast<int32_t>(min(first + PG_TOKENS, a.slots_cap) - 1), lo, hi);
     if (first >= total) return;
     const uint32_t n = min(PG_TOKENS, total - first);
-    uint32_t r = lo;
-    int32_t start = a.starts[lo], kv = a.kv_len[lo], cached = a.cached[lo];
+    const bool held = hi - lo <= PG_FILL_NT;
+    if (held && t < hi - lo) {
+        s_start[t] = a.starts[lo + t];
+        s_kv[t] = a.kv_len[lo + t];
+        s_cached[t] = a.cached[lo + t];
+    }
+    __syncthreads();
     auto slot_of = [&](uint32_t i) {
         const int32_t token = static_cast<int32_t>(first + i);
-        if (hi - lo > 1) {
-            r = last_at_most(a.starts, lo, hi, token);
-            start = a.starts[r];
-            kv = a.kv_len[r];
-            cached = a.cached[r];
+        if (held) {
+            const uint32_t r = last_at_most(s_start, 0u, hi - lo, token);
+            return slot_at(a, lo + r, s_kv[r], s_cached[r], static_cast<uint32_t>(token - s_start[r]));
         }
-        return slot_at(a, r, kv, cached, static_cast<uint32_t>(token - start));
+        const uint32_t r = last_at_most(a.starts, lo, hi, token);
+        return slot_at(a, r, a.kv_len[r], a.cached[r], static_cast<uint32_t>(token - a.starts[r]));
     };
+    typedef int64_t pair __attribute__((ext_vector_type(2)));
     if (pairs && n == PG_TOKENS) {
 #pragma unroll
         for (uint32_t j = 0; j < PG_TOKENS / (2 * PG_FILL_NT); ++j) {
-            const uint32_t i = 2 * (j * PG_FILL_NT + threadIdx.x);
-            const int64_t x = slot_of(i), y = slot_of(i + 1);
-            *reinterpret_cast<longlong2*>(a.slots + first + i) = make_longlong2(x, y);
+            const uint32_t i = 2 * (j * PG_FILL_NT + t);
+            pair z;
+            z[0] = slot_of(i);
+            z[1] = slot_of(i + 1);
+            __builtin_nontemporal_store(z, reinterpret_cast<pair*>(a.slots + first + i));
         }
     } else {
-        for (uint32_t i = threadIdx.x; i < n; i += PG_FILL_NT) a.slots[first + i] = slot_of(i);
+        for (uint32_t i = t; i < n; i += PG_FILL_NT) a.slots[first + i] = slot_of(i);
     }
 }
 
 // The whole plan in one workgroup, for a decoding step: the free pages before
-// each piece of 128, the offsets and the takers' ranks stay in LDS.
+// each piece of 128, the offsets and the takers' ranks stay in LDS.  Bound by
+// latency: 64 requests of 8192 pages 8.4 us (with the offsets in memory 9.7).
 constexpr uint32_t PS_QUADS = 2048, PS_REQUESTS = 1024, PS_TOKENS = 8192;
 
 __global__ __launch_bounds__(PG_NT) void pg_small(PlanArgs a)
 {
     constexpr uint32_t PER = PS_QUADS / PG_NT;
     __shared__ uint64_t s_scan[PG_NT / 64];
-    __shared__ uint64_t s_taken, s_missing;
+    __shared__ uint64_t s_unfit;
     __shared__ uint32_t s_sum[PG_NT / 64];
-    __shared__ uint32_t s_pre[PS_QUADS], s_upto[PS_REQUESTS];
+    __shared__ uint32_t s_pre[PS_QUADS], s_upto[PS_REQUESTS + 1];
+    __shared__ int32_t s_start[PS_REQUESTS + 1], s_kv[PS_REQUESTS], s_cached[PS_REQUESTS];
+    static_assert(PS_REQUESTS <= PG_NT, "a thread per request");
     const uint32_t t = threadIdx.x;
-    if (t == 0) s_taken = s_missing = 0;
     const int32_t c = t < a.n_requests ? a.cached[t] : 0, fresh = t < a.n_requests ? a.fresh[t] : 0;
     uint4 x[PER];
     uint32_t q[PER], n[PER], mine = 0, n_free;
@@ -427,19 +496,29 @@ __global__ __launch_bounds__(PG_NT) void pg_small(PlanArgs a)
         s_pre[t * PER + i] = before;
         before += n[i];
     }
-    plan_requests(a, c, fresh, n_free, s_upto, s_scan, &s_taken, &s_missing);
-    __syncthreads();
-    const uint32_t n_taken = static_cast<uint32_t>(s_taken);
+    if (t < a.n_requests) s_cached[t] = c;
+    const uint64_t wanted = scan_requests<true>(a, c, fresh, s_upto, s_scan, &s_unfit, s_start);
+    const uint32_t n_taken = pages_taken(s_upto, a.n_requests, n_free);
     for (uint32_t rank = t; rank < n_taken; rank += PG_NT) {
-        const uint32_t q = last_at_most(s_pre, 0u, PS_QUADS, rank);  // pieces without a free page start where the next does
+        // pieces without a free page start where the next one does
+        const uint32_t q = last_at_most(s_pre, 0u, PS_QUADS, rank);
         const uint32_t r = last_at_most(s_upto, 0u, a.n_requests, rank);
-        place_page(a, rank, q * 128u + nth_of_quad(free_quad(a.free, q, a.n_quads), rank - s_pre[q]), r, s_upto[r]);
+        const uint32_t id = q * 128u + nth_of_quad(free_quad(a.free, q, a.n_quads), rank - s_pre[q]);
+        place_page(a, rank, id, r, s_cached[r], s_upto[r]);
     }
+    if (t < a.n_requests) s_kv[t] = planned_len(a, c, fresh, s_upto[t], n_taken);
     __syncthreads();
-    const uint32_t total = min(a.slots_cap, static_cast<uint32_t>(a.starts[a.n_requests]));
+    const uint32_t total = min(a.slots_cap, static_cast<uint32_t>(s_start[a.n_requests]));
     for (uint32_t i = t; i < total; i += PG_NT) {
-        const uint32_t r = last_at_most(a.starts, 0u, a.n_requests, static_cast<int32_t>(i));
-        a.slots[i] = slot_at(a, r, a.kv_len[r], a.cached[r], i - static_cast<uint32_t>(a.starts[r]));
+        const uint32_t r = last_at_most(s_start, 0u, a.n_requests, static_cast<int32_t>(i));
+        a.slots[i] = slot_at(a, r, s_kv[r], s_cached[r], i - static_cast<uint32_t>(s_start[r]));
+    }
+    // (Before a barrier, or a load, these stores would be waited for.)
+    for (uint32_t r = t; r <= a.n_requests; r += PG_NT) a.starts[r] = s_start[r];
+    if (t < a.n_requests) a.kv_len[t] = s_kv[t];
+    if (t == 0) {
+        a.counts[0] = s_start[a.n_requests];
+        set_counts(a, n_taken, wanted, s_unfit);
     }
 }
 
@@ -657,24 +736,27 @@ extern "C" int cr_paged_plan(const cr_gpu_roaring* free_pages, uint32_t n_pages,
     a.taken_cap = taken_cap;
     a.counts = d_counts;
     const bool direct = is_direct(free_pages);
-    // One workgroup for a decoding step (64 requests, 8192 pages: 19.4 us in four launches, 9.0 in one).
+    // One workgroup for a decoding step (64 requests, 8192 pages: 19.4 us in several launches, 8.4 in one).
     const bool small = a.n_quads <= PS_QUADS && n_requests <= PS_REQUESTS && slots_cap <= PS_TOKENS;
     Carver cv;
     const size_t o_words = cv.add(direct ? 0 : a.n_quads * 16ull);
-    const size_t o_upto = cv.add(small ? 0 : (n_requests + 1ull) * 4), o_pre = cv.add(small ? 0 : a.n_blocks * 4ull);
-    const size_t o_taken = cv.add(small ? 0 : 4);
+    a.n_groups = (a.n_blocks + PG_GROUP - 1) / PG_GROUP;
+    const size_t o_upto = cv.add(small ? 0 : (n_requests + 1ull) * 4), o_wanted = cv.add(small ? 0 : 16);
+    const size_t o_block = cv.add(small ? 0 : a.n_blocks * 4ull), o_group = cv.add(small ? 0 : a.n_groups * 4ull);
     Scratch sc;
     if (cv.total) CR_RET(sc.alloc(cv.total, s));
     a.upto = sc.at<uint32_t>(o_upto);
-    a.block_pre = sc.at<uint32_t>(o_pre);
-    a.n_taken = sc.at<uint32_t>(o_taken);
+    a.wanted = sc.at<uint64_t>(o_wanted);
+    a.block_n = sc.at<uint32_t>(o_block);
+    a.group_n = sc.at<uint32_t>(o_group);
     CR_RET(set_bits(free_pages, direct, sc.at<uint32_t>(o_words), a.n_quads * 4u, n_pages, stream, &a.free));
     CR_TIMED("pg_plan", s);
     if (small) {
         pg_small<<<1, PG_NT, 0, s>>>(a);
     } else {
-        pg_scan<<<1, PG_NT, 0, s>>>(a);
-        if (a.n_blocks && n_requests) pg_take<<<a.n_blocks, PG_TAKE_NT, 0, s>>>(a);
+        const uint32_t request_blocks = std::max<uint32_t>(1, (n_requests + PG_TAKE_NT - 1) / PG_TAKE_NT);
+        pg_count<<<1 + a.n_groups, PG_NT, 0, s>>>(a);
+        pg_take<<<a.n_blocks + request_blocks, PG_TAKE_NT, 0, s>>>(a);
         const bool pairs = reinterpret_cast<uintptr_t>(d_slots) % 16 == 0;
         if (slots_cap && n_requests) pg_slots<<<(slots_cap + PG_TOKENS - 1) / PG_TOKENS, PG_FILL_NT, 0, s>>>(a, pairs);
     }
@@ -779,7 +861,8 @@ extern "C" int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, 
     Scratch sc;
     if (cv.total) CR_RET(sc.alloc(cv.total, s));
     a.counts = sc.at<uint32_t>(o_counts);
-    CR_RET(set_bits(visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream, &a.visible));
+    CR_RET(set_bits(visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
+                    &a.visible));
     const uint32_t grid = a.chunks * n_requests;
     CR_TIMED("pg_select", s);
     if (a.chunks > 1) sl_count<<<grid, SL_NT, 0, s>>>(a);
