@@ -406,9 +406,19 @@ __device__ __forceinline__ void store_lse(const AttnArgs& a, const Work& t, uint
 // every fourth 32 of them on its own: scores are transposed products (keys x
 // rows) of 16x16x32 matrix instructions, whose result has a row's probabilities
 // in the lanes that the second product wants them in, if keys are taken in the
-// order 4h..4h+3, 16+4h..16+4h+3 for lane group h.  Keys go from memory to
-// registers in operand order; values pass through the wave's LDS, which
-// transposes them.  Both are loaded a tile ahead.
+// order 4h..4h+3, 16+4h..16+4h+3 for lane group h.  Keys and values are loaded
+// into registers a tile ahead, whole rows by neighbouring lanes and past the
+// caches, and pass through the wave's own LDS, which hands keys out in operand
+// order and transposes values; rows there are turned by pieces of 16 bytes
+// against bank conflicts.  No wave waits for another before the end.
+//
+// 64 requests of up to 16384 keys, 32 heads over 8, 128 dimensions, bf16: 335 us
+// with the join, 5.85 TB/s (the card copies 1 GiB at 4.75 and reads alone at up to
+// 7).  On the way, each alone: keys loaded straight in operand order, which asks
+// for half lines, 400, past the caches even 430; whole rows past them 376; a tile's
+// offsets looked up once, through LDS, 361.  48 requests of 4 rows and up to 2048
+// keys, 16 heads of 64 dimensions: 52 us, 4.2 TB/s; they are one workgroup a slot
+// of the card and wait for the longest (64 keys a tile, with fewer waves, 59).
 constexpr int DC_NT = 256;
 constexpr uint32_t DC_WAVES = DC_NT / 64;
 constexpr uint32_t DC_KEYS = 32;
@@ -1039,6 +1049,9 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 }
 
 // ---- the ranges' results joined: a workgroup per row -----------------------------------
+//   o = sum_r 2^(lse_r - top) o_r / sum_r 2^(lse_r - top),  lse = top + log2(...),
+// in fp32, the ranges in a fixed order.  Bound by latency: 3.5 us for 32 rows of a
+// context of 1003 keys, 4.6 for 128 rows of 31 ranges each.
 constexpr int JN_NT = 256;
 
 // TPR threads take four dimensions each of a range's row, JN_NT / TPR ranges at a time.
