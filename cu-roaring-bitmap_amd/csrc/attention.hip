@@ -1054,20 +1054,21 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 // context of 1003 keys, 4.6 for 128 rows of 31 ranges each.
 constexpr int JN_NT = 256;
 
-// TPR threads take four dimensions each of a range's row, JN_NT / TPR ranges at a time.
-template <class E, uint32_t TPR>
-__global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
+// Which ranges hold a token's row, and where.
+struct Joined {
+    uint32_t first, count, row;  // `row` within the tile
+};
+
+__device__ __forceinline__ Joined find_joined(const AttnArgs& a, uint32_t token, uint32_t head, uint32_t most)
 {
-    constexpr uint32_t SLOTS = JN_NT / TPR;
-    __shared__ float s_o[SLOTS][TPR * 4 + 4], s_sum[SLOTS];
-    const uint32_t token = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = __lane_id();
-    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2;
+    const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
     // the token's segment: the last that starts at or before it
     uint32_t lo = 0, len = n, start = 0;
     while (true) {
         const uint32_t step = (len + 63) / 64, i = lo + min(lane * step, len);
         start = static_cast<uint32_t>(segment_start(a, i));
-        const uint32_t at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lane * step < len && start <= token)))) - 1;
+        const uint32_t at =
+            max(1u, static_cast<uint32_t>(__popcll(__ballot(lane * step < len && start <= token)))) - 1;
         start = lane_value(start, at);
         lo += at * step;
         if (step == 1) break;
@@ -1076,23 +1077,52 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
     const uint32_t row = (token - start) * group + head % group;
     // (Offsets that do not ascend may lead to no tile's entry, but to none outside.)
     const uint32_t tile = min(tile_base(lo, static_cast<int32_t>(start), group, most) + row / most, a.n_tiles - 1);
-    uint2 range = a.ranges[tile];
-    if (range.y == 1) return;  // written already
-    range.x = min(range.x, a.n_ranges);
-    range.y = min(range.y, a.n_ranges - range.x);
-    auto place = [&](uint32_t r) {
-        return (static_cast<uint64_t>(range.x + r) * a.kv_heads + head / group) * most + row % most;
-    };
+    const uint2 range = a.ranges[tile];
+    const uint32_t first = min(range.x, a.n_ranges);
+    return {first, range.y == 1 ? 0u : min(range.y, a.n_ranges - first), row % most};
+}
+
+__device__ __forceinline__ uint64_t part_place(const AttnArgs& a, const Joined& j, uint32_t head, uint32_t most,
+                                               uint32_t r)
+{
+    return (static_cast<uint64_t>(j.first + r) * a.kv_heads + head / (a.heads / a.kv_heads)) * most + j.row;
+}
+
+template <class E>
+__device__ __forceinline__ void store_joined(const AttnArgs& a, E, uint32_t token, uint32_t head, uint32_t d, f32x4 x,
+                                             float sum, float top)
+{
+    const bool none = sum == 0.0f;
+    x *= none ? 0.0f : 1.0f / sum;
+    if (d < a.dim) {
+        const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
+                       static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
+        *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
+    }
+    if (a.lse && d == 0)
+        a.lse[static_cast<uint64_t>(token) * a.heads + head] =
+            none ? NEG_INF : (top + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+// TPR threads take four dimensions each of a range's row, JN_NT / TPR ranges at a time.
+template <class E, uint32_t TPR>
+__global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
+{
+    constexpr uint32_t SLOTS = JN_NT / TPR;
+    __shared__ float s_o[SLOTS][TPR * 4 + 4], s_sum[SLOTS];
+    const uint32_t token = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    const Joined j = find_joined(a, token, head, most);
+    if (j.count == 0) return;  // written already
     float top = NEG_INF;
-    for (uint32_t r = lane; r < range.y; r += 64) top = fmaxf(top, a.part_lse[place(r)]);
+    for (uint32_t r = __lane_id(); r < j.count; r += 64) top = fmaxf(top, a.part_lse[part_place(a, j, head, most, r)]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const uint32_t slot = threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
     float sum = 0.0f;
     f32x4 x = {0, 0, 0, 0};
 #pragma unroll 4
-    for (uint32_t r = slot; r < range.y; r += SLOTS) {
-        const uint64_t at = place(r);
+    for (uint32_t r = slot; r < j.count; r += SLOTS) {
+        const uint64_t at = part_place(a, j, head, most, r);
         const float lse = a.part_lse[at], w = lse == NEG_INF ? 0.0f : exp2_fast(lse - top);
         sum += w;
         // a range without a visible key has left nothing to read
@@ -1107,16 +1137,39 @@ __global__ __launch_bounds__(JN_NT) void at_join(AttnArgs a, uint32_t most)
             x += *reinterpret_cast<const f32x4*>(&s_o[i][d]);
             sum += s_sum[i];
         }
-        const bool none = sum == 0.0f;
-        x *= none ? 0.0f : 1.0f / sum;
-        if (d < a.dim) {
-            const v4s y = {static_cast<short>(E::down(x[0])), static_cast<short>(E::down(x[1])),
-                           static_cast<short>(E::down(x[2])), static_cast<short>(E::down(x[3]))};
-            *reinterpret_cast<v4s*>(a.out + token * a.out_token + head * a.out_head + d) = y;
-        }
-        if (a.lse && threadIdx.x == 0)
-            a.lse[blockIdx.x] = none ? NEG_INF : (top + __builtin_amdgcn_logf(sum)) * LN2;
+        store_joined(a, E{}, token, head, d, x, sum, top);
     }
+}
+
+// The same for many rows: TPR threads a row, one range after another.
+template <class E, uint32_t TPR>
+__global__ __launch_bounds__(JN_NT) void at_join_rows(AttnArgs a, uint32_t most)
+{
+    constexpr uint32_t ROWS = 64 / TPR;  // a wave's
+    const uint32_t lane = __lane_id(), n = a.n_tokens * a.heads;
+    const uint32_t row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * JN_NT + threadIdx.x) / 64 * ROWS);
+    if (row0 >= n) return;
+    const uint32_t mine = min(row0 + lane / TPR, n - 1), token = mine / a.heads, head = mine % a.heads;
+    const uint32_t d = lane % TPR * 4;
+    Joined j = {0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < ROWS; ++i) {
+        const uint32_t row = min(row0 + i, n - 1);
+        const Joined found = find_joined(a, row / a.heads, row % a.heads, most);
+        if (lane / TPR == i) j = found;
+    }
+    if (row0 + lane / TPR >= n || j.count == 0) return;
+    float top = NEG_INF, sum = 0.0f;
+    for (uint32_t r = 0; r < j.count; ++r) top = fmaxf(top, a.part_lse[part_place(a, j, head, most, r)]);
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t r = 0; r < j.count; ++r) {
+        const uint64_t at = part_place(a, j, head, most, r);
+        const float lse = a.part_lse[at], w = lse == NEG_INF ? 0.0f : exp2_fast(lse - top);
+        sum += w;
+        if (lse != NEG_INF && d < a.dim) x += w * *reinterpret_cast<const f32x4*>(a.part_o + at * a.dim + d);
+    }
+    store_joined(a, E{}, token, head, d, x, sum, top);
 }
 
 template <class E, uint32_t DIM>
@@ -1140,6 +1193,20 @@ int launch_dim(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t 
     return CR_OK;
 }
 
+// A workgroup a row where there are few (4 requests of 16 tokens, 2048 rows in
+// about 16 ranges each: 24 us in all, 33 with the other; one of 32 rows 15.8 and
+// 18.6), several rows a wave where there are many (64 of 8 tokens, 16384 rows: 156
+// and 165; 1024 tokens, 32768 rows in two ranges: 48 and 84).
+template <class E, uint32_t TPR>
+void launch_join(const AttnArgs& a, uint32_t rows, uint32_t most, hipStream_t s)
+{
+    constexpr uint32_t PER = JN_NT / TPR;
+    if (rows > 4096)
+        at_join_rows<E, TPR><<<(rows + PER - 1) / PER, JN_NT, 0, s>>>(a, most);
+    else
+        at_join<E, TPR><<<rows, JN_NT, 0, s>>>(a, most);
+}
+
 template <class E>
 int launch_attention(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStream_t s)
 {
@@ -1157,11 +1224,11 @@ int launch_attention(const AttnArgs& a, uint32_t per_wave, uint32_t grid, hipStr
         CR_TIMED("at_join", s);
         const uint32_t rows = a.n_tokens * a.heads, most = per_wave ? 16 * per_wave : 128;
         if (a.dim <= 64)
-            at_join<E, 16><<<rows, JN_NT, 0, s>>>(a, most);
+            launch_join<E, 16>(a, rows, most, s);
         else if (a.dim <= 128)
-            at_join<E, 32><<<rows, JN_NT, 0, s>>>(a, most);
+            launch_join<E, 32>(a, rows, most, s);
         else
-            at_join<E, 64><<<rows, JN_NT, 0, s>>>(a, most);
+            launch_join<E, 64>(a, rows, most, s);
         CR_LAUNCH_CHECK();
     }
     return CR_OK;
@@ -1271,7 +1338,12 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     const uint64_t tiles_in_all = (rows + most - 1) / most * requests;
     const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
     const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= 128 ? 2u : 1u) * cus / cache->n_heads + 1;
-    const bool few = 2 * tiles_in_all <= held;
+    bool few = 2 * tiles_in_all <= held;
+    // Tiles of 128 rows leave as much to join however many keys they see, so that
+    // cutting has to shorten the longest by about 800 keys (one request, 256 tokens
+    // of 1024 uncut 33 us, cut 29; 600 of 2048 60 and 52; 1000 of 4096 111 and 102;
+    // but 512 of 512 23 and 29; 1024 of 1024 38 and 48; 16 of 64 of 1024 36.5 and 37.2).
+    if (!per_wave) few = few && max_kv * (held - tiles_in_all) > 800 * held;
     const bool long_ones = per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held;
     const bool cut = (few || long_ones) && all_rows >> 24 == 0;
     a.step = per_wave ? DC_KEYS * DC_WAVES : 64;

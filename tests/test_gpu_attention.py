@@ -435,3 +435,12 @@ def test_arrays_that_make_no_sense_stay_inside(gpu, hints):
                     torch.cuda.synchronize()
                     for x in (wide, lse):
                         assert torch.all(x[:2] == 7.0) and torch.all(x[92:] == 7.0)
+
+
+@pytest.mark.parametrize("density", [None, 0.4])
+@pytest.mark.parametrize("what", [([256], [1500], 32, 4, 64, 16), ([100, 1, 90], [2100, 1800, 3], 33, 11, 96, 16),
+                                  ([9] * 30, [4100] + [50] * 29, 16, 2, 192, 16)])
+def test_many_rows_of_several_ranges(gpu, what, density):
+    """More rows than are joined by a workgroup each, of requests with several ranges and with one."""
+    _say("attention many rows joined", what, density)
+    Problem("float16", *what, seed=19, density=density).check(gpu, max_new=max(what[0]), max_kv=max(what[1]))
