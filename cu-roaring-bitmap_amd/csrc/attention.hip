@@ -50,6 +50,9 @@ struct AttnArgs {
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint16_t v2u16 __attribute__((ext_vector_type(2)));
+typedef uint16_t v4u16 __attribute__((ext_vector_type(4)));
+typedef uint16_t v8u16 __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -126,11 +129,11 @@ __device__ __forceinline__ v4s load4(const uint16_t* p) { return *reinterpret_ca
 // Whether any of eight values is infinite or NaN, and the eight with zeros for those.
 __device__ __forceinline__ bool has_special(v8s x, uint32_t exp)
 {
-    const v4u w = __builtin_bit_cast(v4u, x);
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & exp) == exp || (w[i] & (exp << 16)) == exp << 16;
-    return bad;
+    const v8u16 y = __builtin_bit_cast(v8u16, x) & static_cast<uint16_t>(0x7FFF);
+    const v4u16 a = __builtin_elementwise_max(__builtin_shufflevector(y, y, 0, 1, 2, 3),
+                                              __builtin_shufflevector(y, y, 4, 5, 6, 7));
+    const v2u16 b = __builtin_elementwise_max(__builtin_shufflevector(a, a, 0, 1), __builtin_shufflevector(a, a, 2, 3));
+    return max(b[0], b[1]) >= exp;
 }
 
 __device__ __forceinline__ v8s without_special(v8s x, uint32_t exp)
@@ -149,6 +152,19 @@ __device__ __forceinline__ v8s zero_unless(bool keep, v8s x)
 {
     const uint32_t mask = keep ? 0xFFFFFFFFu : 0u;
     return __builtin_bit_cast(v8s, __builtin_bit_cast(v4u, x) & mask);
+}
+
+// The lowest n bits, all for n >= 32 and none for n <= 0.
+__device__ __forceinline__ uint32_t low_bits(int32_t n)
+{
+    return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u;
+}
+
+// The score where bit i of `on` is set, else -inf.
+__device__ __forceinline__ float score_if(uint32_t on, uint32_t i, float x)
+{
+    const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(on << (31u - i)) >> 31);
+    return __uint_as_float((__float_as_uint(x) & keep) | (0xFF800000u & ~keep));
 }
 
 // Adds the infinite and NaN ones of four values.
@@ -177,11 +193,12 @@ __device__ __forceinline__ int32_t segment_start(const AttnArgs& a, uint32_t i)
     return min(max(a.starts[i - 1], 0), static_cast<int32_t>(a.n_tokens));
 }
 
-// How many keys a segment's request has.
-__device__ __forceinline__ uint32_t segment_keys(const AttnArgs& a, uint32_t i)
+// How many keys a segment's request has; `n`: what its length says.
+__device__ __forceinline__ uint32_t segment_keys(const AttnArgs& a, uint32_t i, int32_t& n)
 {
+    n = 0;
     if (i == 0 || i > a.n_requests) return 0;
-    const int32_t n = a.sel ? a.sel_len[i - 1] : a.kv_len[i - 1];
+    n = a.sel ? a.sel_len[i - 1] : a.kv_len[i - 1];
     const uint64_t room = static_cast<uint64_t>(a.cols) << a.page_lg;
     return n <= 0 ? 0u : static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
 }
@@ -202,6 +219,7 @@ struct Work {
     uint32_t tokens;
     uint32_t row0, rows;  // rows [row0, rows) are this tile's and those behind it
     uint32_t keys;        // the request's
+    int32_t len;          // what its length says
     uint32_t k0, k1;      // the range
     uint32_t range;       // its number
     bool whole;           // the tile's only range: its results need not be joined
@@ -219,19 +237,23 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
 {
     const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
     uint32_t lo = 0, start = 0, end = 0, keys = 0, tile = 0, count = 1, part = 0, at = 0;
+    int32_t said = 0;
     if (a.share == 0) {
         if (n <= 64) {
             // the requests with the most keys go first, and of each its last rows, which see the most
             const uint32_t i = min(lane, n);
             start = static_cast<uint32_t>(segment_start(a, i));
             end = static_cast<uint32_t>(segment_start(a, i + 1));
-            keys = segment_keys(a, i);
+            keys = segment_keys(a, i, said);
             const uint32_t rows = end > start ? (end - start) * group : 0u;
             const uint32_t mine = i < n ? (rows + most - 1) / most : 0u;
             uint32_t before = 0;
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t other = lane_value(keys, j), tiles = lane_value(mine, j);
-                before += other > keys || (other == keys && j < lane) ? tiles : 0u;
+            for (uint32_t j0 = 0; j0 < n; j0 += 8) {  // (segments from n on have no tiles)
+#pragma unroll
+                for (uint32_t j = j0; j < j0 + 8; ++j) {
+                    const uint32_t other = lane_value(keys, j), tiles = lane_value(mine, j);
+                    before += other > keys || (other == keys && j < lane) ? tiles : 0u;
+                }
             }
             const uint64_t here = __ballot(before <= id && id - before < mine);
             if (!here) {
@@ -252,7 +274,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
             const uint32_t i = min(lo + lane, n);
             start = static_cast<uint32_t>(segment_start(a, i));
             end = static_cast<uint32_t>(segment_start(a, i + 1));
-            keys = segment_keys(a, i);
+            keys = segment_keys(a, i, said);
             const uint32_t base = tile_base(i, static_cast<int32_t>(start), group, most);
             at = max(1u, static_cast<uint32_t>(__popcll(__ballot(lo + lane < n && base <= id)))) - 1;
             lo += at;
@@ -266,7 +288,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
             const uint32_t i = min(i0 + lane, n);
             start = static_cast<uint32_t>(segment_start(a, i));
             end = static_cast<uint32_t>(segment_start(a, i + 1));
-            keys = segment_keys(a, i);
+            keys = segment_keys(a, i, said);
             const uint32_t rows = end > start ? (end - start) * group : 0u;
             all += static_cast<uint64_t>((rows + most - 1) / most) * keys;
         }
@@ -281,7 +303,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
             if (n > 64) {
                 start = static_cast<uint32_t>(segment_start(a, i));
                 end = static_cast<uint32_t>(segment_start(a, i + 1));
-                keys = segment_keys(a, i);
+                keys = segment_keys(a, i, said);
             }
             const uint32_t rows = end > start ? (end - start) * group : 0u;
             count = max(1u, (keys + len - 1) / len);
@@ -314,6 +336,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
     w.rows = w.tokens * group;
     w.row0 = tile * most;
     w.keys = lane_value(keys, at);
+    w.len = static_cast<int32_t>(lane_value(static_cast<uint32_t>(said), at));
     w.none = w.row0 >= w.rows;
     w.range = id;
     w.whole = count == 1;
@@ -329,7 +352,7 @@ __device__ __forceinline__ uint32_t limit_of(const AttnArgs& a, const Work& t, u
 {
     if (!t.real || !a.causal) return t.keys;
     const int64_t at = a.sel ? static_cast<int64_t>(a.limits[t.token0 + token])
-                             : static_cast<int64_t>(a.kv_len[t.request]) - t.tokens + token + 1;
+                             : static_cast<int64_t>(t.len) - t.tokens + token + 1;
     return static_cast<uint32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(t.keys), at)));
 }
 
@@ -356,19 +379,26 @@ __device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, ui
     return (at >> page_lg) * page_stride + (at & ((1u << page_lg) - 1u)) * slot_stride;
 }
 
-// Queries come in with the sign of the scale, so that the largest product is
-// the largest score.
-__device__ __forceinline__ v8s load_query(const AttnArgs& a, const Work& t, uint32_t row, uint32_t kh, uint32_t d)
-{
-    const uint32_t group = a.heads / a.kv_heads;
-    v8s x = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row < t.rows && d < a.dim && a.scale != 0.0f) {
-        const uint64_t token = static_cast<uint64_t>(t.token0) + row / group;
-        x = load8(a.q + token * a.q_token + (kh * group + row % group) * a.q_head + d);
-        if (a.scale < 0.0f) x ^= static_cast<short>(0x8000);
+// A row's queries come in with the sign of the scale, so that the largest product
+// is the largest score.
+struct Query {
+    const uint16_t* p;
+    uint32_t dim;  // 0: zeros
+    uint32_t sign;
+    __device__ __forceinline__ Query(const AttnArgs& a, const Work& t, uint32_t row, uint32_t kh)
+    {
+        const uint32_t group = a.heads / a.kv_heads, at = min(row, t.rows - 1);
+        p = a.q + (static_cast<uint64_t>(t.token0) + at / group) * a.q_token + (kh * group + at % group) * a.q_head;
+        dim = row < t.rows && a.scale != 0.0f ? a.dim : 0u;
+        sign = a.scale < 0.0f ? 0x80008000u : 0u;
     }
-    return x;
-}
+    // Dimensions [d, d + 8).
+    __device__ __forceinline__ v8s load(uint32_t d) const
+    {
+        const v4u x = *reinterpret_cast<const v4u*>(p + (d < dim ? d : 0u));
+        return __builtin_bit_cast(v8s, (x & (d < dim ? 0xFFFFFFFFu : 0u)) ^ sign);
+    }
+};
 
 __device__ __forceinline__ float score_scale(const AttnArgs& a)
 {
@@ -469,9 +499,11 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 
     v8s q[NB][STEPS];
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b)
+    for (uint32_t b = 0; b < NB; ++b) {
+        const Query from(a, t, t.row0 + b * 16 + c16, kh);
 #pragma unroll
-        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = load_query(a, t, t.row0 + b * 16 + c16, kh, s * 32 + h * 8);
+        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = from.load(s * 32 + h * 8);
+    }
     f32x4 o[NB][BLOCKS];
     float m[NB], l[NB];
 #pragma unroll
@@ -561,14 +593,11 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         for (uint32_t b = 0; b < NB; ++b) {
             if (!whole) {
                 const int32_t left = static_cast<int32_t>(limit[b] - j0 - h * 4);
-                const uint32_t on = static_cast<uint32_t>(there) >> (h * 4);
+                const uint32_t on = (static_cast<uint32_t>(there) >> (h * 4)) & low_bits(left);
 #pragma unroll
                 for (uint32_t x = 0; x < 2; ++x)
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const bool see = static_cast<int32_t>(x * 16 + i) < left & (on & (1u << (x * 16 + i))) != 0;
-                        s[b][x][i] = see ? s[b][x][i] : NEG_INF;
-                    }
+                    for (uint32_t i = 0; i < 4; ++i) s[b][x][i] = score_if(on, x * 16 + i, s[b][x][i]);
             }
             float top = NEG_INF;
 #pragma unroll
@@ -758,6 +787,16 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     const uint32_t kh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     const Work t = find_work(a, id, 128);
     if (t.none) return;
+    // The first wave looks up where tiles are: first of all, since what is loaded
+    // later is waited for later.
+    auto find = [&](uint32_t i, uint32_t end) {
+        return look_up(a, t.request, min(t.k0 + i * KEYS + lane % KEYS, end - 1));
+    };
+    int32_t found[3] = {-1, -1, -1};
+    if (wave == 0 && t.k0 < t.k1) {
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) found[i] = find(i, t.k1);
+    }
     const uint32_t row = t.row0 + wave * 32 + c32;  // the lane's
     const uint32_t limit = row < t.rows ? limit_of(a, t, row / group) : 0u;
     uint32_t most = limit, least = row < t.rows ? limit : 0xFFFFFFFFu;
@@ -789,9 +828,10 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         return;
     }
 
+    const Query from(a, t, row, kh);
     v8s q[STEPS];
 #pragma unroll
-    for (uint32_t st = 0; st < STEPS; ++st) q[st] = load_query(a, t, row, kh, st * 16 + h * 8);
+    for (uint32_t st = 0; st < STEPS; ++st) q[st] = from.load(st * 16 + h * 8);
     f32x16 o[BLOCKS];
     float m = NEG_INF, l = 0.0f;
 #pragma unroll
@@ -804,8 +844,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     const uint32_t lrow = threadIdx.x / CHUNKS, lpos = threadIdx.x % CHUNKS;
     const uint32_t wave_row = __builtin_amdgcn_readfirstlane(wave) * (64 / CHUNKS);
 
-    // The first wave looks up where tile i's keys and values are.
-    auto find = [&](uint32_t i) { return look_up(a, t.request, min(k0 + i * KEYS + lane % KEYS, k1 - 1)); };
+    // The first wave notes where tile i's keys and values are.
     auto note = [&](uint32_t i, int32_t found) {
         const uint32_t at = i % 4, j = k0 + i * KEYS + lane;
         const int32_t slot = lane < KEYS && j < k1 ? slot_of(a, found, j) : -1;
@@ -842,14 +881,17 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     // see and others do not, infinite and NaN ones too.
     auto mend_tile = [&](uint32_t i, uint64_t there, uint16_t* sv) {
         uint64_t bad = 0;
+        v8s y[LOADS];
 #pragma unroll
         for (uint32_t x = 0; x < LOADS; ++x) {
             const uint32_t r = x * PER + lrow;
-            uint16_t* at = sv + r * STRIDE + lpos * 8;
-            const v8s y = zero_unless((there >> r) & 1u, load8(at));
-            bad |= __ballot((lpos ^ v_turn(r)) * 8 < a.dim && has_special(y, E::EXP));
-            *reinterpret_cast<v8s*>(at) = without_special(y, E::EXP);
+            y[x] = zero_unless((there >> r) & 1u, load8(sv + r * STRIDE + lpos * 8));
+            bad |= __ballot((lpos ^ v_turn(r)) * 8 < a.dim && has_special(y[x], E::EXP));
         }
+        if (there == ALL && !bad) return;
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x)
+            *reinterpret_cast<v8s*>(sv + (x * PER + lrow) * STRIDE + lpos * 8) = without_special(y[x], E::EXP);
         if (bad && lane == 0) s_bad[i % 4] = 1;
     };
 
@@ -897,14 +939,10 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         if (there == ALL && j0 + KEYS <= wave_least) return;
         const int32_t left = static_cast<int32_t>(limit - j0 - h * 4);
 #pragma unroll
-        for (uint32_t x = 0; x < HALVES; ++x) {
-            const uint32_t on = static_cast<uint32_t>(there >> (x * 32)) >> (h * 4);
+        for (int32_t x = 0; x < static_cast<int32_t>(HALVES); ++x) {
+            const uint32_t on = (static_cast<uint32_t>(there >> (x * 32)) >> (h * 4)) & low_bits(left - x * 32);
 #pragma unroll
-            for (uint32_t e = 0; e < 16; ++e) {
-                const uint32_t at = (e / 4) * 8 + e % 4;
-                const bool see = static_cast<int32_t>(x * 32 + at) < left & (on & (1u << at)) != 0;
-                s[x][e] = see ? s[x][e] : NEG_INF;
-            }
+            for (uint32_t e = 0; e < 16; ++e) s[x][e] = score_if(on, (e / 4) * 8 + e % 4, s[x][e]);
         }
     };
     auto highest = [&]() {
@@ -930,10 +968,8 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     const uint32_t mine = min(n_tiles, wave_most > k0 ? (wave_most - k0 + KEYS - 1) / KEYS : 0u);  // this wave's
     if (n_tiles) {
         if (wave == 0) {
-            const int32_t first = find(0), second = find(1), third = find(2);
-            note(0, first);
-            note(1, second);
-            note(2, third);
+#pragma unroll
+            for (uint32_t i = 0; i < 3; ++i) note(i, found[i]);
         }
         __syncthreads();
         load_keys(0, s_k0);
@@ -945,7 +981,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             multiply(s_k0, s);
             hide(0);
             highest();
-            follow();
+            m = fmaxf(top, __shfl_xor(top, 32, 64));
         }
     }
     // The queries are waited for here, on every way to the loop, or each of its
@@ -958,7 +994,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads to LDS have arrived
         __syncthreads();  // keys i + 1 and values i are there, and nobody reads those before any more
         int32_t ahead = -1;
-        if (wave == 0) ahead = find(i + 3);
+        if (wave == 0) ahead = find(i + 3, k1);
         if (i + 1 < n_tiles) load_values(i + 1, next_v);
         if (i + 2 < n_tiles) load_keys(i + 2, sk);
         const uint32_t j0 = k0 + i * KEYS;
