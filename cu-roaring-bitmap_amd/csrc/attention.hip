@@ -252,7 +252,9 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
 #pragma unroll
                 for (uint32_t j = j0; j < j0 + 8; ++j) {
                     const uint32_t other = lane_value(keys, j), tiles = lane_value(mine, j);
-                    before += other > keys || (other == keys && j < lane) ? tiles : 0u;
+                    // more keys, or as many and an earlier segment
+                    const int32_t below = static_cast<int32_t>(keys) - (j < lane ? 1 : 0);
+                    before += static_cast<int32_t>(other) > below ? tiles : 0u;
                 }
             }
             const uint64_t here = __ballot(before <= id && id - before < mine);
@@ -392,10 +394,13 @@ struct Query {
         dim = row < t.rows && a.scale != 0.0f ? a.dim : 0u;
         sign = a.scale < 0.0f ? 0x80008000u : 0u;
     }
-    // Dimensions [d, d + 8).
-    __device__ __forceinline__ v8s load(uint32_t d) const
+    // Dimensions [d, d + 8), in two steps: nothing waits for the load but the second.
+    __device__ __forceinline__ v4u load(uint32_t d) const
     {
-        const v4u x = *reinterpret_cast<const v4u*>(p + (d < dim ? d : 0u));
+        return *reinterpret_cast<const v4u*>(p + (d < dim ? d : 0u));
+    }
+    __device__ __forceinline__ v8s finish(uint32_t d, v4u x) const
+    {
         return __builtin_bit_cast(v8s, (x & (d < dim ? 0xFFFFFFFFu : 0u)) ^ sign);
     }
 };
@@ -502,7 +507,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     for (uint32_t b = 0; b < NB; ++b) {
         const Query from(a, t, t.row0 + b * 16 + c16, kh);
 #pragma unroll
-        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = from.load(s * 32 + h * 8);
+        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = from.finish(s * 32 + h * 8, from.load(s * 32 + h * 8));
     }
     f32x4 o[NB][BLOCKS];
     float m[NB], l[NB];
@@ -799,28 +804,40 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     }
     const uint32_t row = t.row0 + wave * 32 + c32;  // the lane's
     const uint32_t limit = row < t.rows ? limit_of(a, t, row / group) : 0u;
-    uint32_t most = limit, least = row < t.rows ? limit : 0xFFFFFFFFu;
+    uint32_t most, least, wave_most, wave_least;
+    if (a.sel) {
+        most = limit;
+        least = row < t.rows ? limit : 0xFFFFFFFFu;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
-        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
-    }
-    const uint32_t wave_most = __builtin_amdgcn_readfirstlane(most);
-    const uint32_t wave_least = __builtin_amdgcn_readfirstlane(least);
-    if (lane == 0) {
-        s_most[wave] = wave_most;
-        s_least[wave] = wave_least;
-    }
-    __syncthreads();
-    most = 0;
-    least = 0xFFFFFFFFu;
+        for (int o = 1; o < 32; o <<= 1) {
+            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
+            least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
+        }
+        wave_most = __builtin_amdgcn_readfirstlane(most);
+        wave_least = __builtin_amdgcn_readfirstlane(least);
+        if (lane == 0) {
+            s_most[wave] = wave_most;
+            s_least[wave] = wave_least;
+        }
+        __syncthreads();
+        most = 0;
+        least = 0xFFFFFFFFu;
 #pragma unroll
-    for (uint32_t w = 0; w < TL_NT / 64; ++w) {
-        most = max(most, s_most[w]);
-        least = min(least, s_least[w]);
+        for (uint32_t w = 0; w < TL_NT / 64; ++w) {
+            most = max(most, s_most[w]);
+            least = min(least, s_least[w]);
+        }
+        most = __builtin_amdgcn_readfirstlane(most);
+        least = __builtin_amdgcn_readfirstlane(least);
+    } else {
+        // without a selection they rise with the rows
+        const uint32_t w0 = __builtin_amdgcn_readfirstlane(t.row0 + wave * 32), last = t.rows - 1;
+        auto at_row = [&](uint32_t r) { return limit_of(a, t, min(r, last) / group); };
+        least = at_row(t.row0);
+        most = at_row(t.row0 + 127);
+        wave_least = w0 < t.rows ? at_row(w0) : 0xFFFFFFFFu;
+        wave_most = w0 < t.rows ? at_row(w0 + 31) : 0u;
     }
-    most = __builtin_amdgcn_readfirstlane(most);
-    least = __builtin_amdgcn_readfirstlane(least);
     const uint32_t k0 = t.k0, k1 = min(most, t.k1);
     const uint64_t place0 = (static_cast<uint64_t>(t.range) * a.kv_heads + kh) * 128;  // of the tile's first row
     if (!t.whole && k0 >= k1) {
@@ -829,9 +846,9 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     }
 
     const Query from(a, t, row, kh);
-    v8s q[STEPS];
+    v4u q_raw[STEPS];
 #pragma unroll
-    for (uint32_t st = 0; st < STEPS; ++st) q[st] = from.load(st * 16 + h * 8);
+    for (uint32_t st = 0; st < STEPS; ++st) q_raw[st] = from.load(st * 16 + h * 8);
     f32x16 o[BLOCKS];
     float m = NEG_INF, l = 0.0f;
 #pragma unroll
@@ -917,6 +934,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             }
         }
     }
+    v8s q[STEPS];
     f32x16 s[HALVES];  // the scores of the tile to come
     float top;
     // Its products, as transposed blocks of 32 keys by 32 rows.
@@ -975,6 +993,8 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         load_keys(0, s_k0);
         load_values(0, s_v0);
         if (n_tiles > 1) load_keys(1, s_k1);
+#pragma unroll
+        for (uint32_t st = 0; st < STEPS; ++st) q[st] = from.finish(st * 16 + h * 8, q_raw[st]);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         __syncthreads();
         if (mine) {
