@@ -271,8 +271,41 @@ __device__ __forceinline__ uint32_t rank_of(const uint64_t* key, uint32_t n, uin
     return r;
 }
 
-// NT threads: 512 for few winners (k = 8 of 64 x 8 x 100003: 10.1 us, with 256
-// 12.5, with 1024 10.6), 1024 for many, whose groups then take fewer rounds.
+// The largest score of the lane's allowed tokens of group g.
+template <class T>
+__device__ __forceinline__ float lane_best(const Row<T>& row, const Allowed& allowed, uint32_t at, uint32_t g)
+{
+    using R = Row<T>;
+    float best = -__builtin_inff();
+    if (row.pieces) {
+        uint32_t on[R::UNROLL], word = 0;
+        cr_v4u x[R::UNROLL];
+        row.load(g, x);
+        if (row.words) word = row.load_words(allowed, at, g);
+        row.masks(word, g, on);
+#pragma unroll
+        for (uint32_t u = 0; u < R::UNROLL; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < R::PER; ++i) {
+                const float y = to_f32(R::value(x[u], i));
+                best = ((on[u] >> i) & 1u) && y > best ? y : best;
+            }
+    }
+    if (row.has_singles(g)) {
+        const uint32_t v = row.single(allowed, g);
+        if (v < row.vocab) {
+            const float y = to_f32(row.p[v]);
+            best = y > best ? y : best;
+        }
+    }
+    return best;
+}
+
+// A workgroup per answer, bound by the latency of its few dependent reads.  NT
+// threads: 512 for few winners (k = 8 of 64 x 8 x 100003: 10.1 us, with 256 12.5,
+// with 1024 10.6), 1024 for many, whose groups then take fewer rounds.  With the
+// lanes' maxima where groups are few, 10 x 8 x 1507, k = 8, takes 19 us in all
+// instead of 50, 4 x 4 x 30000, k = 64, 40 instead of 134.
 template <class T, uint32_t NT>
 __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __restrict__ gmax)
 {
@@ -282,6 +315,7 @@ __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __rest
     __shared__ uint64_t s_key[BP_CAP];
     __shared__ uint64_t s_set[SETS];
     __shared__ uint32_t s_list[BP_GROUPS];
+    __shared__ uint32_t s_best[NT];
     __shared__ uint32_t s_scan[WAVES];
     __shared__ uint32_t s_n;
     __shared__ uint64_t s_thr;
@@ -295,21 +329,34 @@ __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __rest
         s_n = 0;
         s_thr = 1;  // any candidate
     }
-    uint32_t best = 0;
-    for (uint32_t i = t; i < n_groups; i += NT) best = max(best, gm[i]);
-    // one set is four threads' groups; the set's place makes the keys distinct
-    best = max(best, static_cast<uint32_t>(__shfl_xor(static_cast<int>(best), 1, 64)));
-    best = max(best, static_cast<uint32_t>(__shfl_xor(static_cast<int>(best), 2, 64)));
-    if ((t & 3u) == 0) s_set[t >> 2] = (static_cast<uint64_t>(best) << 32) | (SETS - (t >> 2));
-    __syncthreads();
-    {  // four threads count what lies above a set, a quarter of the sets each
+    // `best`: the thread's, of totals that are no other thread's.  Returns how many
+    // of the sets, four threads' totals each, have a candidate.
+    auto bound = [&](uint32_t best) {
+        s_best[t] = best;
+        __syncthreads();
+        if (t < SETS) {  // the set's place makes the keys distinct
+            uint32_t most = s_best[t];
+#pragma unroll
+            for (uint32_t i = 1; i < 4; ++i) most = max(most, s_best[t + i * SETS]);
+            s_set[t] = (static_cast<uint64_t>(most) << 32) | (SETS - t);
+        }
+        __syncthreads();
+        // four threads count what lies above a set, a quarter of the sets each
         const uint64_t mine = s_set[t >> 2];
         uint32_t above = rank_of(s_set + (t & 3u) * (SETS / 4), SETS / 4, mine);
         above += static_cast<uint32_t>(__shfl_xor(static_cast<int>(above), 1, 64));
         above += static_cast<uint32_t>(__shfl_xor(static_cast<int>(above), 2, 64));
-        if ((t & 3u) == 0 && above + 1 == a.k && (mine >> 32)) s_thr = (mine >> 32) << 32;
-    }
-    __syncthreads();
+        const bool filled = (t & 3u) == 0 && (mine >> 32) != 0;
+        if (filled && above + 1 == a.k) s_thr = max(s_thr, (mine >> 32) << 32);
+        uint32_t all;
+        block_excl_scan<NT>(filled ? 1u : 0u, s_scan, all);
+        return all;
+    };
+    uint32_t best = 0;
+    for (uint32_t i = t; i < n_groups; i += NT) best = max(best, gm[i]);
+    // Few groups bound the answer badly (8 beams of 1507 tokens, k = 8: 16 maxima):
+    // their lanes' own maxima are taken instead, below.
+    const bool weak = bound(best) < min(2 * a.k, SETS);
 
     for (uint32_t g0 = 0; g0 < n_groups; g0 += BP_GROUPS) {
         // the groups that can hold one of the k: in order, so that of equal totals the first are met first
@@ -329,6 +376,15 @@ __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __rest
         for (uint32_t j = 0; j < OWN; ++j)
             if ((in >> j) & 1u) s_list[at++] = g0 + t * OWN + j;
         __syncthreads();
+        if (weak && g0 == 0 && listed > 1) {
+            uint32_t most = 0;
+            for (uint32_t l = wave; l < listed; l += WAVES) {
+                const uint32_t id = s_list[l], g = id % a.n_groups;
+                const R row(a, b, id / a.n_groups);
+                most = max(most, order_of(row.total(lane_best(row, a.allowed, starts, g))));
+            }
+            bound(most);
+        }
         for (uint32_t l0 = 0; l0 < listed; l0 += WAVES) {
             const uint64_t thr = s_thr;
             uint64_t key[MINE + 1];
@@ -427,6 +483,9 @@ __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __rest
 }
 
 // ---- reorder ---------------------------------------------------------------------
+// Bound by memory: a thread moves four pieces, past the caches (64 x 8 rows of 64
+// KiB, half of them in use: 9.5 us, 3.5 TB/s read and written with the launch;
+// through the caches 20).
 constexpr int BR_NT = 256;
 constexpr uint32_t BR_PER = 4;
 

@@ -190,6 +190,26 @@ def test_select_many_over_the_bound(gpu):
 
 
 # ---- reorder ---------------------------------------------------------------------
+@pytest.mark.parametrize("b,w,v,k", [(3, 8, 1507, 8), (2, 5, 5614, 10), (2, 2, 1025, 2), (4, 4, 16468, 8),
+                                     (1, 3, 30000, 64), (2, 1, 70000, 256), (1, 6, 2047, 200)])
+def test_select_from_few_groups(gpu, b, w, v, k):
+    """Few pieces of the vocabulary to bound the answer by: as they come, equal, one lane's, and few allowed."""
+    import torch
+    _say("beam few groups", b, w, v, k)
+    x, cum = _inputs(b, w, v, "bfloat16", 31)
+    check(gpu, x, cum, k)
+    mask = np.zeros(v, bool)
+    mask[v // 3:v // 3 + 90] = True
+    bits = torch.from_numpy(_bits(mask)).cuda()
+    check(gpu, x, cum, k, mask=mask, allowed=bits)
+    x[:, :, 8:16] += 50.0  # the best are neighbours: a lane has several of them
+    check(gpu, x, cum, k)
+    x[:, :, ::3] = float("nan")
+    x[:, :, 1::5] = float("-inf")
+    check(gpu, x, cum, k)
+    check(gpu, torch.zeros_like(x), torch.zeros_like(cum), k)
+
+
 @pytest.mark.parametrize("dtype,shape", [("bfloat16", (40, 8, 64)), ("int32", (17,)), ("uint8", (5, 3)), ("float32", (1,)),
                                          ("float16", (3, 70000)), ("int64", (33, 2))])
 @pytest.mark.parametrize("lengths", [False, True])
