@@ -750,6 +750,9 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 // tile i + 1's keys, the wave turns tile i's scores into probabilities, and while
 // they multiply those with the values, it takes the maximum of the new scores.
 // One workgroup and two waves a SIMD more or less keep the other busy too.
+// Up to 192 dimensions (8 requests of 1000 tokens of up to 8192, 24 heads over 8:
+// 588 us, 657 TFLOP/s, with one wave a SIMD 950); 256 leave registers for one
+// (1540 us, 413).
 // 16384 tokens, 32 heads over 8, 128 dimensions, bf16: 2.31 ms, 950 TFLOP/s (a
 // large bf16 library product reaches 1206): the matrix units work 45% of the
 // cycles, at 2.0 GHz, to which their power brings the clock down from 2.35.  On
@@ -776,7 +779,7 @@ __device__ __forceinline__ void between_products()
 }
 
 template <class E, uint32_t DIM>
-__global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 128 ? 2 : 1))) void at_tiles(AttnArgs a)
+__global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 192 ? 2 : 1))) void at_tiles(AttnArgs a)
 {
     constexpr uint32_t STEPS = DIM / 16, BLOCKS = DIM / 32, CHUNKS = Rows<DIM>::CHUNKS, STRIDE = Rows<DIM>::STRIDE;
     constexpr uint32_t KEYS = tile_keys(DIM), HALVES = KEYS / 32;
@@ -914,9 +917,8 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 
     // Where this lane's fragments begin: keys step by step, values by blocks of 32
     // dimensions (the turn of a row moves a block among four).
-    uint32_t k_at[STEPS], v_at[4];
-#pragma unroll
-    for (uint32_t st = 0; st < STEPS; ++st) k_at[st] = c32 * STRIDE + ((st * 2 + h) ^ (c32 & KTURN)) * 8;
+    uint32_t v_at[4];
+    const uint32_t k_at = c32 * STRIDE + (h ^ (c32 & KTURN)) * 8;  // of step st: k_at ^ st * 16
     {
         const uint32_t i16 = lane & 15u, r = h * 4 + i16 / 4, turn = v_turn(r) / 4;
 #pragma unroll
@@ -943,11 +945,14 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         for (uint32_t y = 0; y < HALVES; ++y)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[y][e] = 0.0f;
+        uint32_t at = k_at;
+        // Two waves a SIMD leave 192 dimensions no registers to keep all addresses in.
+        if constexpr (DIM == 192) asm volatile("" : "+v"(at));
 #pragma unroll
         for (uint32_t y = 0; y < HALVES; ++y)
 #pragma unroll
             for (uint32_t st = 0; st < STEPS; ++st) {
-                const v8s k = load8(sk + y * 32 * STRIDE + k_at[st]);
+                const v8s k = load8(sk + y * 32 * STRIDE + (at ^ (st * 16)));
                 x[y] = E::mfma32(k, q[st], x[y]);
             }
     };
@@ -1393,7 +1398,7 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     // with 16 heads of 64 dimensions 53 and 60).
     const uint64_t tiles_in_all = (rows + most - 1) / most * requests;
     const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
-    const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= 128 ? 2u : 1u) * cus / cache->n_heads + 1;
+    const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= (per_wave ? 128 : 192) ? 2u : 1u) * cus / cache->n_heads + 1;
     bool few = 2 * tiles_in_all <= held;
     // Tiles of 128 rows leave as much to join however many keys they see, so that
     // cutting has to shorten the longest by about 800 keys (one request, 256 tokens
