@@ -42,6 +42,7 @@ struct AttnArgs {
     // joined by another kernel.
     uint32_t n_tiles, n_ranges;
     uint32_t share, step, least_len;  // ranges are of a multiple of `step` keys, at least least_len
+    uint32_t if_uneven;               // cut only if the longest tile has 2.5 times the keys of such a range
     uint2* ranges;    // [n_tiles] a tile's first range and how many it has
     float* part_o;    // [ranges][key heads][rows of a tile][dim]
     float* part_lse;  // [ranges][key heads][rows of a tile], base 2
@@ -233,12 +234,37 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t x, uint32_t lane)
 
 // What the workgroup's number `id` stands for.  A wave looks at 64 segments at
 // a time, each lane at one.
+// IF_UNEVEN: it may be left to the lengths whether tiles are cut.
+template <bool IF_UNEVEN>
 __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32_t most)
 {
     const uint32_t group = a.heads / a.kv_heads, n = a.n_requests + 2, lane = __lane_id();
     uint32_t lo = 0, start = 0, end = 0, keys = 0, tile = 0, count = 1, part = 0, at = 0;
     int32_t said = 0;
-    if (a.share == 0) {
+    bool cut = a.share != 0;
+    uint64_t all = 0;
+    if (cut) {
+        uint32_t longest = 0;
+#pragma unroll 2
+        for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+            const uint32_t i = min(i0 + lane, n);
+            start = static_cast<uint32_t>(segment_start(a, i));
+            end = static_cast<uint32_t>(segment_start(a, i + 1));
+            keys = segment_keys(a, i, said);
+            const uint32_t rows = end > start ? (end - start) * group : 0u;
+            all += static_cast<uint64_t>((rows + most - 1) / most) * keys;
+            if (IF_UNEVEN) longest = max(longest, rows ? keys : 0u);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
+        if (IF_UNEVEN && a.if_uneven) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1)
+                longest = max(longest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(longest), o, 64)));
+            cut = static_cast<uint64_t>(longest) * a.share * 2 > all * 5;
+        }
+    }
+    if (!cut) {
         if (n <= 64) {
             // the requests with the most keys go first, and of each its last rows, which see the most
             const uint32_t i = min(lane, n);
@@ -284,18 +310,6 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
         }
     } else {
         // ranges of one length for all, so that about `share` of them result
-        uint64_t all = 0;
-#pragma unroll 2
-        for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-            const uint32_t i = min(i0 + lane, n);
-            start = static_cast<uint32_t>(segment_start(a, i));
-            end = static_cast<uint32_t>(segment_start(a, i + 1));
-            keys = segment_keys(a, i, said);
-            const uint32_t rows = end > start ? (end - start) * group : 0u;
-            all += static_cast<uint64_t>((rows + most - 1) / most) * keys;
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
         const uint64_t even = (all + a.share - 1) / a.share;
         const uint32_t len = max(a.least_len, static_cast<uint32_t>(min(even, static_cast<uint64_t>(0x7FFFFFFF))));
         uint32_t before = 0;
@@ -478,7 +492,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     __shared__ float s_m[DC_WAVES][16 * NB], s_l[DC_WAVES][16 * NB];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c16 = lane & 15u, h = lane >> 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
-    const Work t = find_work(a, blockIdx.x / a.kv_heads, 16 * NB);
+    const Work t = find_work<false>(a, blockIdx.x / a.kv_heads, 16 * NB);
     if (t.none) return;
     uint32_t limit[NB], most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
@@ -793,7 +807,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 19
     __shared__ uint32_t s_bad[4], s_most[TL_NT / 64], s_least[TL_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
     const uint32_t kh = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
-    const Work t = find_work(a, id, 128);
+    const Work t = find_work<(DIM <= 128)>(a, id, 128);
     if (t.none) return;
     // The first wave looks up where tiles are: first of all, since what is loaded
     // later is waited for later.
@@ -1406,13 +1420,21 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     // but 512 of 512 23 and 29; 1024 of 1024 38 and 48; 16 of 64 of 1024 36.5 and 37.2).
     if (!per_wave) few = few && max_kv * (held - tiles_in_all) > 800 * held;
     const bool long_ones = per_wave && max_kv >= 4096 && tiles_in_all <= (max_kv >= 16384 ? 16 : 2) * held;
-    const bool cut = (few || long_ones) && all_rows >> 24 == 0;
+    // Tiles for more than half of the card, but perhaps of requests so uneven that the
+    // longest would be waited for: the device looks at the lengths (5 of 1924 tokens
+    // of up to 42670, 4 heads: uncut 955 us, cut 410; 16 of 100 of 4096 104 and 83).
+    // With more tiles the rows to be joined cost more than it gains (8 of 1000 of
+    // 8192, 192 tiles for 65 places: 179 and 201).
+    const bool uneven =
+        !per_wave && !few && p.n_requests > 1 && a.dim <= 128 && max_kv >= 4096 && tiles_in_all <= held;
+    const bool cut = (few || long_ones || uneven) && all_rows >> 24 == 0;
+    a.if_uneven = uneven;
     a.step = per_wave ? DC_KEYS * DC_WAVES : 64;
     a.least_len = !few ? 1024 : per_wave ? DC_KEYS * DC_WAVES : 256;
     uint64_t ranges = tiles;
     Scratch sc;
     if (cut && max_kv > a.least_len) {
-        a.share = static_cast<uint32_t>(few ? held - tiles_in_all : 4 * held);
+        a.share = static_cast<uint32_t>(few ? held - tiles_in_all : uneven ? held : 4 * held);
         ranges += a.share;
         const uint64_t part_rows = ranges * cache->n_heads * most;
         Carver cv;
