@@ -1412,7 +1412,8 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
     // with 16 heads of 64 dimensions 53 and 60).
     const uint64_t tiles_in_all = (rows + most - 1) / most * requests;
     const uint64_t max_kv = std::min<uint64_t>(room, p.max_kv ? p.max_kv : room);
-    const uint64_t held = (a.dim <= 64 && per_wave ? 3u : a.dim <= (per_wave ? 128 : 192) ? 2u : 1u) * cus / cache->n_heads + 1;
+    const uint32_t on_a_cu = per_wave && a.dim <= 64 ? 3 : a.dim <= (per_wave ? 128 : 192) ? 2 : 1;
+    const uint64_t held = on_a_cu * cus / cache->n_heads + 1;
     bool few = 2 * tiles_in_all <= held;
     // Tiles of 128 rows leave as much to join however many keys they see, so that
     // cutting has to shorten the longest by about 800 keys (one request, 256 tokens
