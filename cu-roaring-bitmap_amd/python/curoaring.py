@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from types import SimpleNamespace
 from typing import Optional, Sequence
 
@@ -214,11 +215,11 @@ def load(path: Optional[str] = None):
                           C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
                           C.c_uint32, C.c_void_p, C.c_void_p],
         "cr_paged_append": [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32,
-                            C.c_void_p, P(PagedCache), C.c_void_p],
+                            C.c_void_p, C.c_void_p, C.c_void_p],
         "cr_paged_select": [P(GpuRoaring), C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint64, C.c_void_p,
                             C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
                             C.c_void_p],
-        "cr_paged_attention": [P(PagedAttentionArgs), P(PagedCache), C.c_void_p],
+        "cr_paged_attention": [C.c_void_p, C.c_void_p, C.c_void_p],
         "cr_beam_select": [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64,
                            C.c_void_p, C.c_void_p, P(GpuRoaring), C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
                            C.c_void_p, C.c_void_p, C.c_void_p],
@@ -545,7 +546,11 @@ def download_batch(b: RoaringBatch) -> SimpleNamespace:
 # ---- serving language models (stream-ordered, no synchronisation) ---------------
 F32, F16, BF16 = 0, 1, 2
 _TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
-_names = {}
+_names, _codes = {}, {}
+# The structs as the calls pass them: packed bytes cost a third of a filled ctypes structure.
+_CACHE = struct.Struct("@PPQQQQQQIIIII4x")
+_ATTENTION = struct.Struct("@PQQPQQPIIIPPPIQPQPPfIII")
+assert _CACHE.size == C.sizeof(PagedCache) and _ATTENTION.size == C.sizeof(PagedAttentionArgs)
 
 
 def _type_name(t) -> str:
@@ -557,9 +562,12 @@ def _type_name(t) -> str:
 
 def _typed(t) -> int:
     """The library's code of a tensor's type."""
-    code = _TYPES.get(_type_name(t))
+    code = _codes.get(t.dtype)
     if code is None:
-        raise CrError(CR_ERR_INVALID, f"a tensor of {t.dtype} where one of {', '.join(_TYPES)} is taken")
+        code = _TYPES.get(_type_name(t))
+        if code is None:
+            raise CrError(CR_ERR_INVALID, f"a tensor of {t.dtype} where one of {', '.join(_TYPES)} is taken")
+        _codes[t.dtype] = code
     return code
 
 
@@ -583,26 +591,32 @@ def _table(t, n_requests: int):
                                   f"{tuple(t.shape)}")
 
 
-def _rows(t, name: str, like):
-    """(address, token stride, head stride) of a [tokens, heads, dim] tensor of `like`'s shape and type."""
-    if t.dtype == like.dtype and t.is_cuda and t.shape == like.shape and t.dim() == 3:
+def _rows(t, name: str, dtype, shape):
+    """(address, token stride, head stride) of a [tokens, heads, dim] tensor of this type and shape."""
+    if t.dtype == dtype and t.is_cuda and t.shape == shape and len(shape) == 3:
         token, head, one = t.stride()
-        if one == 1 or t.shape[2] <= 1:
+        if one == 1 or shape[2] <= 1:
             return t.data_ptr(), token, head
-    raise CrError(CR_ERR_INVALID, f"{name}: a {like.dtype} CUDA tensor of shape {tuple(like.shape)} with "
-                                  f"contiguous rows is taken, not {t.dtype} {tuple(t.shape)}")
+    raise CrError(CR_ERR_INVALID, f"{name}: a {dtype} CUDA tensor of shape {tuple(shape)} with contiguous rows is "
+                                  f"taken, not {t.dtype} {tuple(t.shape)}")
+
+
+def _cache(d_k, d_v):
+    """(cr_paged_cache, page size, heads, dim) of a cache's tensors."""
+    shape = d_k.shape
+    if len(shape) == 4 and d_v.shape == shape and d_k.dtype == d_v.dtype and d_k.is_cuda and d_v.is_cuda:
+        (kp, ks, kh, k1), (vp, vs, vh, v1) = d_k.stride(), d_v.stride()
+        pages, size, heads, dim = shape
+        if (k1 == 1 and v1 == 1) or dim <= 1:
+            return _CACHE.pack(d_k.data_ptr(), d_v.data_ptr(), kp, ks, kh, vp, vs, vh, pages, size, heads, dim,
+                               _typed(d_k)), size, heads, dim
+    raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] with "
+                                  "contiguous rows are taken")
 
 
 def paged_cache(d_k, d_v) -> PagedCache:
     """A cache of [pages, page size, heads, dim] keys and values (any strides with contiguous rows)."""
-    if d_k.dim() == 4 and d_k.shape == d_v.shape and d_k.dtype == d_v.dtype and d_k.is_cuda and d_v.is_cuda:
-        (kp, ks, kh, k1), (vp, vs, vh, v1) = d_k.stride(), d_v.stride()
-        pages, size, heads, dim = d_k.shape
-        if (k1 == 1 and v1 == 1) or dim <= 1:
-            return PagedCache(d_k.data_ptr(), d_v.data_ptr(), kp, ks, kh, vp, vs, vh, pages, size, heads, dim,
-                              _typed(d_k))
-    raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] with "
-                                  "contiguous rows are taken")
+    return PagedCache.from_buffer_copy(_cache(d_k, d_v)[0])
 
 
 def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d_new, d_table, d_slots, d_starts,
@@ -625,16 +639,16 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
 
 def paged_append(d_k, d_v, d_slots, d_k_cache, d_v_cache, stream=None):
     """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out."""
-    cache = paged_cache(d_k_cache, d_v_cache)
-    if d_k.dim() != 3 or tuple(d_k.shape[1:]) != (cache.n_heads, cache.head_dim) or d_k.dtype != d_k_cache.dtype:
-        raise CrError(CR_ERR_INVALID, f"paged_append: {d_k_cache.dtype} keys [tokens, {cache.n_heads}, "
-                                      f"{cache.head_dim}] are taken, not {d_k.dtype} {tuple(d_k.shape)}")
-    k, k_token, k_head = _rows(d_k, "k", d_k)
-    v, v_token, v_head = _rows(d_v, "v", d_k)
-    n = d_k.shape[0]
+    cache, _, heads, dim = _cache(d_k_cache, d_v_cache)
+    dtype, shape = d_k_cache.dtype, d_k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or d_k.dtype != dtype:
+        raise CrError(CR_ERR_INVALID, f"paged_append: {dtype} keys [tokens, {heads}, {dim}] are taken, not "
+                                      f"{d_k.dtype} {tuple(shape)}")
+    k, k_token, k_head = _rows(d_k, "k", dtype, shape)
+    v, v_token, v_head = _rows(d_v, "v", dtype, shape)
+    n = shape[0]
     _check(load().cr_paged_append(k, v, k_token, k_head, v_token, v_head, n,
-                                  _array(d_slots, "slots", "int64", (n,)), C.byref(cache), _stream(stream)),
-           "paged_append")
+                                  _array(d_slots, "slots", "int64", (n,)), cache, _stream(stream)), "paged_append")
 
 
 def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: int, d_sel, d_sel_len, d_limits,
@@ -664,27 +678,30 @@ def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_ou
     Request r's tokens are [starts[r], starts[r + 1]), the last of its kv_len[r] positions.  scale: 1 / sqrt(dim) by
     default.  d_lse: float32 [T, heads] or None.  selection: paged_select's (sel, sel_len, limits) or None.  max_new
     and max_kv: the most new tokens and keys of a request if known; they choose how the work is split."""
-    cache = paged_cache(d_k_cache, d_v_cache)
-    if d_q.dim() != 3 or d_q.dtype != d_k_cache.dtype or d_q.shape[2] != cache.head_dim:
-        raise CrError(CR_ERR_INVALID, f"paged_attention: {d_k_cache.dtype} queries [tokens, heads, {cache.head_dim}] "
-                                      f"are taken, not {d_q.dtype} {tuple(d_q.shape)}")
-    n, (tokens, heads, dim) = d_kv_len.numel(), d_q.shape
-    q, q_token, q_head = _rows(d_q, "q", d_q)
-    out, out_token, out_head = _rows(d_out, "out", d_q)
+    cache, page_size, _, dim = _cache(d_k_cache, d_v_cache)
+    dtype, shape = d_k_cache.dtype, d_q.shape
+    if len(shape) != 3 or d_q.dtype != dtype or shape[2] != dim:
+        raise CrError(CR_ERR_INVALID, f"paged_attention: {dtype} queries [tokens, heads, {dim}] are taken, not "
+                                      f"{d_q.dtype} {tuple(shape)}")
+    n, (tokens, heads, _) = d_kv_len.numel(), shape
+    q, q_token, q_head = _rows(d_q, "q", dtype, shape)
+    out, out_token, out_head = _rows(d_out, "out", dtype, shape)
     table, cols, stride = _table(d_table, n)
-    sel, room, sel_stride, sel_len, limits = None, 0, 0, None, None
+    sel, room, sel_stride, sel_len, limits = 0, 0, 0, 0, 0
     if selection is not None:
         sel, room, sel_stride = _table(selection[0], n)
-        if room < cols * cache.page_size:
+        if room < cols * page_size:
             raise CrError(CR_ERR_INVALID, "paged_attention: a row of sel holds cols * page_size slots")
         sel_len = _array(selection[1], "sel_len", "int32", (n,))
         limits = _array(selection[2], "limits", "int32", (tokens,))
-    a = PagedAttentionArgs(q, q_token, q_head, out, out_token, out_head,
-                           _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else None,
-                           tokens, heads, n, _array(d_starts, "starts", "int32", (n + 1,)),
-                           _array(d_kv_len, "kv_len", "int32", (n,)), table, cols, stride, sel, sel_stride, sel_len,
-                           limits, dim ** -0.5 if scale is None else scale, causal, max_new, max_kv)
-    _check(load().cr_paged_attention(C.byref(a), C.byref(cache), _stream(stream)), "paged_attention")
+    if not (0 <= max_new < 1 << 32 and 0 <= max_kv < 1 << 32):
+        raise CrError(CR_ERR_INVALID, f"paged_attention: max_new {max_new}, max_kv {max_kv}")
+    a = _ATTENTION.pack(q, q_token, q_head, out, out_token, out_head,
+                        _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else 0,
+                        tokens, heads, n, _array(d_starts, "starts", "int32", (n + 1,)),
+                        _array(d_kv_len, "kv_len", "int32", (n,)), table, cols, stride, sel, sel_stride, sel_len,
+                        limits, dim ** -0.5 if scale is None else scale, causal, max_new, max_kv)
+    _check(load().cr_paged_attention(a, cache, _stream(stream)), "paged_attention")
 
 
 def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_lse=None, allowed=None, stream=None):
