@@ -400,24 +400,23 @@ __device__ __forceinline__ uint64_t offset_of(int32_t slot, uint32_t page_lg, ui
 struct Query {
     const uint16_t* p;
     uint32_t dim;  // 0: zeros
-    uint32_t sign;
     __device__ __forceinline__ Query(const AttnArgs& a, const Work& t, uint32_t row, uint32_t kh)
     {
         const uint32_t group = a.heads / a.kv_heads, at = min(row, t.rows - 1);
         p = a.q + (static_cast<uint64_t>(t.token0) + at / group) * a.q_token + (kh * group + at % group) * a.q_head;
         dim = row < t.rows && a.scale != 0.0f ? a.dim : 0u;
-        sign = a.scale < 0.0f ? 0x80008000u : 0u;
     }
     // Dimensions [d, d + 8), in two steps: nothing waits for the load but the second.
     __device__ __forceinline__ v4u load(uint32_t d) const
     {
         return *reinterpret_cast<const v4u*>(p + (d < dim ? d : 0u));
     }
-    __device__ __forceinline__ v8s finish(uint32_t d, v4u x) const
-    {
-        return __builtin_bit_cast(v8s, (x & (d < dim ? 0xFFFFFFFFu : 0u)) ^ sign);
-    }
 };
+
+__device__ __forceinline__ v8s finish_query(const AttnArgs& a, uint32_t dim, uint32_t d, v4u x)
+{
+    return __builtin_bit_cast(v8s, (x & (d < dim ? 0xFFFFFFFFu : 0u)) ^ (a.scale < 0.0f ? 0x80008000u : 0u));
+}
 
 __device__ __forceinline__ float score_scale(const AttnArgs& a)
 {
@@ -494,6 +493,11 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     const uint32_t kh = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
     const Work t = find_work<false>(a, blockIdx.x / a.kv_heads, 16 * NB);
     if (t.none) return;
+    // Lane j < 32 (and j + 32) looks after key j of a tile.  The first look-up comes
+    // before all that is not needed for it: what is loaded later is waited for later.
+    auto find = [&](uint32_t j0, uint32_t end) { return look_up(a, t.request, min(j0 + (lane & 31u), end - 1)); };
+    uint32_t j0 = t.k0 + wave * DC_KEYS;
+    int32_t found = j0 < t.k1 ? find(j0, t.k1) : -1;
     uint32_t limit[NB], most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
@@ -516,12 +520,14 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         return;
     }
 
-    v8s q[NB][STEPS];
+    v4u q_raw[NB][STEPS];
+    uint32_t q_dim[NB];
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
         const Query from(a, t, t.row0 + b * 16 + c16, kh);
+        q_dim[b] = from.dim;
 #pragma unroll
-        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = from.finish(s * 32 + h * 8, from.load(s * 32 + h * 8));
+        for (uint32_t s = 0; s < STEPS; ++s) q_raw[b][s] = from.load(s * 32 + h * 8);
     }
     f32x4 o[NB][BLOCKS];
     float m[NB], l[NB];
@@ -541,8 +547,6 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
     const uint16_t* vp = a.v + kh * a.v_head + vcol;
 
     v8s k[LOADS], v[LOADS];
-    // Lane j < 32 (and j + 32) looks after key j of a tile.
-    auto find = [&](uint32_t j0) { return look_up(a, t.request, min(j0 + (lane & 31u), k1 - 1)); };
     auto slots = [&](uint32_t j0, int32_t found) {
         const uint32_t j = j0 + (lane & 31u);
         return j < k1 ? slot_of(a, found, j) : -1;
@@ -572,15 +576,19 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         *reinterpret_cast<v8s*>(lds_k + r * STRIDE + (vchunk ^ (r & KTURN)) * 8) = zero_unless(inside, x);
     };
 
-    uint32_t j0 = k0 + wave * DC_KEYS;
-    int32_t slot = -1, next = -1, found = -1;
+    int32_t slot = -1, next = -1;
     if (j0 < k1) {
-        slot = slots(j0, find(j0));
+        slot = slots(j0, found);
         note(slot);
-        found = find(j0 + DC_WAVES * DC_KEYS);
+        found = find(j0 + DC_WAVES * DC_KEYS, k1);
         load_keys();
         load_values();
     }
+    v8s q[NB][STEPS];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+        for (uint32_t s = 0; s < STEPS; ++s) q[b][s] = finish_query(a, q_dim[b], s * 32 + h * 8, q_raw[b][s]);
     for (; j0 < k1; j0 += DC_WAVES * DC_KEYS) {
         const uint64_t there = __ballot(slot >= 0);
         const bool more = j0 + DC_WAVES * DC_KEYS < k1;
@@ -661,7 +669,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         const int32_t was = slot;
         slot = next;
         if (more) {
-            found = find(j0 + 2 * DC_WAVES * DC_KEYS);
+            found = find(j0 + 2 * DC_WAVES * DC_KEYS, k1);
             load_values();
         }
         wave_lds_fence();
@@ -1013,7 +1021,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 19
         load_values(0, s_v0);
         if (n_tiles > 1) load_keys(1, s_k1);
 #pragma unroll
-        for (uint32_t st = 0; st < STEPS; ++st) q[st] = from.finish(st * 16 + h * 8, q_raw[st]);
+        for (uint32_t st = 0; st < STEPS; ++st) q[st] = finish_query(a, from.dim, st * 16 + h * 8, q_raw[st]);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         __syncthreads();
         if (mine) {
