@@ -453,3 +453,16 @@ def test_tiles_of_uneven_requests(gpu, kv, density):
     _say("attention uneven tiles", kv, density)
     p = Problem("bfloat16", [33] * 5, kv, 64, 64, 64, 16, seed=20, density=density)
     p.check(gpu, max_new=33)
+
+
+@pytest.mark.parametrize("density", [None, 0.4])
+@pytest.mark.parametrize("n", [63, 70, 128, 140])
+def test_many_requests_of_single_tokens(gpu, n, density):
+    """Requests without tokens or keys, of one key and of many, in any order of lengths."""
+    _say("attention many requests", n, density)
+    rng = np.random.default_rng(21)
+    kv = (2 ** rng.uniform(0, 9, n)).astype(int)
+    kv[::9], kv[5], kv[n - 1] = 0, 700, 511
+    new = np.ones(n, int)
+    new[3::11] = 0
+    Problem("float16", new.tolist(), kv.tolist(), 4, 2, 64, 16, seed=22, density=density).check(gpu, max_new=1)
