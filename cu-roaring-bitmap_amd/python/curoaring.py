@@ -572,12 +572,12 @@ def _typed(t) -> int:
 
 
 def _array(t, name: str, dtype: str, shape) -> int:
-    """The address of a contiguous CUDA tensor of this type and shape (an int: one axis of any extent from there)."""
-    if _type_name(t) == dtype and t.is_cuda and t.is_contiguous() and (
-            t.dim() == 1 if isinstance(shape, int) else t.shape == shape):
+    """The address of a contiguous CUDA tensor of this type and shape (0: one axis of any extent)."""
+    if (_names.get(t.dtype) or _type_name(t)) == dtype and t.is_cuda and t.is_contiguous() and (
+            t.dim() == 1 if shape == 0 else t.shape == shape):
         return t.data_ptr()
     raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} CUDA tensor of shape "
-                                  f"{'(any,)' if isinstance(shape, int) else tuple(shape)} is taken, not "
+                                  f"{'(any,)' if shape == 0 else tuple(shape)} is taken, not "
                                   f"{t.dtype} {tuple(t.shape)}")
 
 
@@ -593,7 +593,7 @@ def _table(t, n_requests: int):
 
 def _rows(t, name: str, dtype, shape):
     """(address, token stride, head stride) of a [tokens, heads, dim] tensor of this type and shape."""
-    if t.dtype == dtype and t.is_cuda and t.shape == shape and len(shape) == 3:
+    if t.dtype == dtype and t.is_cuda and t.shape == shape:
         token, head, one = t.stride()
         if one == 1 or shape[2] <= 1:
             return t.data_ptr(), token, head
@@ -640,13 +640,10 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
 def paged_append(d_k, d_v, d_slots, d_k_cache, d_v_cache, stream=None):
     """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out."""
     cache, _, heads, dim = _cache(d_k_cache, d_v_cache)
-    dtype, shape = d_k_cache.dtype, d_k.shape
-    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or d_k.dtype != dtype:
-        raise CrError(CR_ERR_INVALID, f"paged_append: {dtype} keys [tokens, {heads}, {dim}] are taken, not "
-                                      f"{d_k.dtype} {tuple(shape)}")
+    n, dtype = d_slots.numel(), d_k_cache.dtype
+    shape = (n, heads, dim)
     k, k_token, k_head = _rows(d_k, "k", dtype, shape)
     v, v_token, v_head = _rows(d_v, "v", dtype, shape)
-    n = shape[0]
     _check(load().cr_paged_append(k, v, k_token, k_head, v_token, v_head, n,
                                   _array(d_slots, "slots", "int64", (n,)), cache, _stream(stream)), "paged_append")
 
@@ -735,15 +732,15 @@ def beam_reorder(d_src, d_parents, d_dst, d_len=None, stream=None):
 
     d_len: int32 [B, W]: only the first d_len[b, parent] entries along the third extent move.  Rows without a parent
     (-1) are left alone."""
-    b, w = d_src.shape[:2]
+    b, w, *of_state = d_src.shape
     k = d_parents.shape[1]
     if not (d_src.is_cuda and d_dst.is_cuda and d_src.is_contiguous() and d_dst.is_contiguous()) or (
-            d_src.dtype != d_dst.dtype or tuple(d_dst.shape) != (b, k) + tuple(d_src.shape[2:])):
+            d_src.dtype != d_dst.dtype or d_dst.shape != (b, k, *of_state)):
         raise CrError(CR_ERR_INVALID, f"beam_reorder: contiguous CUDA states [{b}, {w}, ...] into [{b}, {k}, ...]")
-    if d_len is not None and d_src.dim() < 3:
+    if d_len is not None and not of_state:
         raise CrError(CR_ERR_INVALID, "beam_reorder: lengths count along the states' third extent")
-    row = d_src.numel() * d_src.element_size() // max(1, b * w)
-    unit = row // max(1, d_src.shape[2]) if d_len is not None else 0
+    row = d_src.nbytes // (b * w or 1)
+    unit = row // (of_state[0] or 1) if d_len is not None else 0
     _check(load().cr_beam_reorder(_dptr(d_src), _array(d_parents, "parents", "int32", (b, k)), b, w, k, row, row, row,
                                   _array(d_len, "len", "int32", (b, w)) if d_len is not None else None, unit,
                                   _dptr(d_dst), _stream(stream)), "beam_reorder")
