@@ -79,6 +79,32 @@ struct SetBits {
         }
         return w == end / 32u ? x & ((1u << (end % 32u)) - 1u) : x;
     }
+
+    // N words of a set with end > 0, their look-ups side by side.
+    template <uint32_t N>
+    __device__ __forceinline__ void words(const uint32_t (&w)[N], uint32_t (&x)[N]) const
+    {
+        if (flat) {
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) x[j] = flat[w[j]];
+        } else {
+            uint32_t c[N], at[N];
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) c[j] = key_index[min(w[j] / 2048u, max_key)];
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) {
+                if (w[j] / 2048u > max_key) c[j] = 0xFFFFu;
+                at[j] = offsets[c[j] != 0xFFFFu ? c[j] : 0u];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) x[j] = reinterpret_cast<const uint32_t*>(bitmaps)[at[j] / 4u + w[j] % 2048u];
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) x[j] = (c[j] != 0xFFFFu ? x[j] : 0u) ^ flip;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j)
+            if (w[j] == end / 32u) x[j] &= (1u << (end % 32u)) - 1u;
+    }
 };
 
 struct PlanArgs {
@@ -564,10 +590,15 @@ __global__ __launch_bounds__(AP_NT) void pg_append(AppendArgs a)
 // A wave looks at 32 positions a lane: the bits of the pages that hold them are
 // the positions' own, in words (or parts of one, where a page is shorter).
 // Bound by the latency of its look-ups, so that many workgroups of one wave do it
-// (4 requests of 131072 positions: 11.8 us; 17.4 with the bitmap written out as
+// (4 requests of 131072 positions: 10 us; 17.4 with the bitmap written out as
 // flat words first, 8192 positions a workgroup and a table look-up for each slot).
 constexpr int SL_NT = 64;
 constexpr uint32_t SL_POS = 32 * SL_NT;
+// Up to this many look-ups a lane, a workgroup counts what lies before its chunk by
+// itself; above, a launch of its own counts every chunk.  (8 requests, us counted and
+// alone: 16 look-ups 8.9 and 8.2 in pages of 64, 8.9 and 8.6 in pages of 16; 32 of
+// them 8.9 and 12.3, 8.9 and 12.4; 4 of them, 8192 positions in pages of 64, 8.8 and 6.4.)
+constexpr uint32_t SL_ALONE = 16;
 
 struct SelectArgs {
     SetBits visible;  // slots
@@ -585,7 +616,7 @@ struct SelectArgs {
     int32_t* sel_len;
     int32_t* limits;
     uint32_t chunks;
-    uint32_t* counts;  // [n_requests][chunks] visible positions, where there is more than one chunk
+    uint32_t* counts;  // [n_requests][chunks] visible positions, or nullptr: each workgroup counts those before it
 };
 
 __device__ __forceinline__ uint32_t select_len(const SelectArgs& a, uint32_t r)
@@ -629,9 +660,39 @@ __global__ __launch_bounds__(SL_NT) void sl_count(SelectArgs a)
     if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
 }
 
+// The visible ones among this lane's positions of the chunks before `chunk`, all of
+// which are the request's.
+__device__ __forceinline__ uint32_t visible_before(const SelectArgs& a, uint32_t r, uint32_t chunk)
+{
+    constexpr uint32_t N = 8;  // look-ups side by side
+    if (a.visible.end == 0) return 0;
+    const int32_t* row = a.table + r * a.table_stride;
+    const uint32_t lg = min(a.page_lg, 5u), parts_lg = 5u - lg, items = chunk << parts_lg;
+    const uint32_t keep = 0xFFFFFFFFu >> (32u - (1u << lg));
+    uint32_t n = 0;
+    for (uint32_t i = 0; i < items; i += N) {
+        uint32_t slot[N], w[N], x[N];
+        bool in[N];
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            const uint32_t u = min(i + j, items - 1u);
+            const uint32_t p = (u >> parts_lg) * SL_POS + threadIdx.x * 32u + ((u & ((1u << parts_lg) - 1u)) << lg);
+            const uint32_t page = static_cast<uint32_t>(row[p >> a.page_lg]);
+            slot[j] = (page << a.page_lg) + (p & ((1u << a.page_lg) - 1u));
+            in[j] = i + j < items && page < a.n_pages && slot[j] < a.visible.end;
+            w[j] = in[j] ? slot[j] >> 5 : 0u;
+        }
+        a.visible.words(w, x);
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) n += in[j] ? __popc((x[j] >> (slot[j] & 31u)) & keep) : 0u;
+    }
+    return n;
+}
+
 __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
 {
     __shared__ int32_t s_slot[SL_POS];
+    __shared__ uint32_t s_vis[SL_NT], s_before[SL_NT];
     const uint32_t r = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, t = threadIdx.x;
     const uint32_t len = select_len(a, r), p0 = chunk * SL_POS + t * 32u;
     // positions of the new tokens: the last of the request's
@@ -643,7 +704,11 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
     }
     if (chunk * SL_POS >= len && chunk > 0) return;
     uint32_t base = 0;
-    for (uint32_t i = t; i < chunk; i += SL_NT) base += a.counts[r * a.chunks + i];
+    if (a.counts) {
+        for (uint32_t i = t; i < chunk; i += SL_NT) base += a.counts[r * a.chunks + i];
+    } else {
+        base = visible_before(a, r, chunk);
+    }
     uint32_t vis = 0;
     visible_parts(a, r, p0, len, [&](uint32_t p, uint32_t, uint32_t bits) { vis |= bits << (p - p0); });
     base = wave_total(base);
@@ -653,14 +718,17 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
     visible_parts(a, r, p0, len, [&](uint32_t, uint32_t slot, uint32_t bits) {
         for (; bits; bits &= bits - 1u) s_slot[at++] = static_cast<int32_t>(slot + __ffs(bits) - 1);
     });
-    if (p0 < len && p0 + 32 + shift > t0) {
-        for (uint32_t k = 0; k < 32u && p0 + k < len; ++k) {
-            const int64_t token = static_cast<int64_t>(p0 + k) + shift;
-            if (token >= t0 && token < t1)
-                a.limits[token] = static_cast<int32_t>(base + before + __popc(vis & (0xFFFFFFFFu >> (31u - k))));
-        }
-    }
+    s_vis[t] = vis;
+    s_before[t] = base + before;
     __syncthreads();
+    // the new tokens' positions in this chunk
+    const uint32_t c0 = chunk * SL_POS;
+    const uint32_t from = static_cast<uint32_t>(max(static_cast<int64_t>(t0) - shift, static_cast<int64_t>(c0)));
+    for (uint32_t p = from + t; p < min(len, c0 + SL_POS); p += SL_NT) {
+        const uint32_t k = p - c0;
+        a.limits[p + shift] =
+            static_cast<int32_t>(s_before[k / 32u] + __popc(s_vis[k / 32u] & (0xFFFFFFFFu >> (31u - k % 32u))));
+    }
     for (uint32_t i = t; i < total; i += SL_NT) a.sel[r * a.sel_stride + base + i] = s_slot[i];
     if (t == 0 && (len <= SL_POS || chunk == (len - 1) / SL_POS)) a.sel_len[r] = static_cast<int32_t>(base + total);
 }
@@ -857,15 +925,16 @@ extern "C" int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, 
     a.limits = d_limits;
     Carver cv;
     const size_t o_words = cv.add(direct ? 0 : n_words * 4ull);
-    const size_t o_counts = cv.add(a.chunks > 1 ? 4ull * a.chunks * n_requests : 0);
+    const bool counted = a.chunks * std::max(1u, 32u / page_size) > SL_ALONE;
+    const size_t o_counts = cv.add(counted ? 4ull * a.chunks * n_requests : 0);
     Scratch sc;
     if (cv.total) CR_RET(sc.alloc(cv.total, s));
-    a.counts = sc.at<uint32_t>(o_counts);
+    if (counted) a.counts = sc.at<uint32_t>(o_counts);
     CR_RET(set_bits(visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                     &a.visible));
     const uint32_t grid = a.chunks * n_requests;
     CR_TIMED("pg_select", s);
-    if (a.chunks > 1) sl_count<<<grid, SL_NT, 0, s>>>(a);
+    if (counted) sl_count<<<grid, SL_NT, 0, s>>>(a);
     sl_write<<<grid, SL_NT, 0, s>>>(a);
     CR_LAUNCH_CHECK();
     return CR_OK;

@@ -268,6 +268,37 @@ def test_select(gpu, density, page, pages, kv, new):
         assert np.array_equal(limits.cpu().numpy(), want_limits)
 
 
+@pytest.mark.parametrize("kind", ["bitmap", "stored"])
+@pytest.mark.parametrize("page,pages,kv,new", [(64, 1100, [32768, 2049, 32767, 0], [2050, 1, 64, 0]),
+                                               (64, 600, [32769, 32705], [1, 4097]),
+                                               (16, 2100, [16384, 4097, 2048, 4096], [3, 4097, 2048, 1]),
+                                               (8, 1200, [8192, 6145, 1], [40, 2047, 1]),
+                                               (2, 3000, [2050, 2048, 2047], [2050, 2, 1]),
+                                               (128, 300, [30001, 16385], [33, 2])])
+def test_select_counts_chunks(gpu, page, pages, kv, new, kind):
+    """Requests of several chunks, up to and above the look-ups that a workgroup makes by itself; some pages outside."""
+    import torch
+    _say("select chunks", page, pages, kv, kind)
+    rng = np.random.default_rng(page)
+    cols = max(-(-x // page) for x in kv)
+    table = rng.integers(-3, pages + 3, (len(kv), cols)).astype(np.int32)
+    visible = rng.random(pages * page) < 0.4
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    g = _bitmap(gpu, visible, kind)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    sel, length = torch.full((len(kv), cols * page + 2), -5, **i32), torch.full((len(kv),), -5, **i32)
+    limits = torch.full((int(starts[-1]),), -5, **i32)
+    gpu.paged_select(g, _cuda(table), _cuda(starts), _cuda(np.array(kv, np.int32)), page, sel, length, limits, pages)
+    torch.cuda.synchronize()
+    gpu.free(g)
+    want, want_limits = select_oracle(visible, table, starts, np.array(kv), page, pages)
+    assert np.array_equal(length.cpu().numpy(), [len(x) for x in want])
+    for r, x in enumerate(want):
+        row = sel[r].cpu().numpy()
+        assert np.array_equal(row[:len(x)], x) and np.all(row[len(x):] == -5)
+    assert np.array_equal(limits.cpu().numpy(), want_limits)
+
+
 # ---- refusals --------------------------------------------------------------------
 def test_refusals(gpu):
     import torch
