@@ -689,6 +689,32 @@ __device__ __forceinline__ uint32_t visible_before(const SelectArgs& a, uint32_t
     return n;
 }
 
+// visible_parts for pages of 8 or more, looked up once and side by side: slot[j] and
+// bits[j] of the lane's part j, of at most SL_PARTS.
+constexpr uint32_t SL_PARTS = 4;
+__device__ __forceinline__ void visible_own(const SelectArgs& a, uint32_t r, uint32_t p0, uint32_t len,
+                                            uint32_t (&slot)[SL_PARTS], uint32_t (&bits)[SL_PARTS])
+{
+    const int32_t* row = a.table + r * a.table_stride;
+    const uint32_t lg = min(a.page_lg, 5u), part = 1u << lg;
+    uint32_t w[SL_PARTS];
+    bool in[SL_PARTS];
+#pragma unroll
+    for (uint32_t j = 0; j < SL_PARTS; ++j) {
+        const uint32_t p = min(p0 + (j << lg), len - 1u);
+        const uint32_t page = static_cast<uint32_t>(row[p >> a.page_lg]);
+        slot[j] = (page << a.page_lg) + (p & ((1u << a.page_lg) - 1u));
+        in[j] = j << lg < 32u && p0 + (j << lg) < len && page < a.n_pages && slot[j] < a.visible.end;
+        w[j] = in[j] ? slot[j] >> 5 : 0u;
+    }
+    a.visible.words(w, bits);
+#pragma unroll
+    for (uint32_t j = 0; j < SL_PARTS; ++j) {
+        const uint32_t n = in[j] ? min(part, len - p0 - (j << lg)) : 0u;  // positions there are
+        bits[j] = n ? (bits[j] >> (slot[j] & 31u)) & (0xFFFFFFFFu >> (32u - n)) : 0u;
+    }
+}
+
 __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
 {
     __shared__ int32_t s_slot[SL_POS];
@@ -709,15 +735,27 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
     } else {
         base = visible_before(a, r, chunk);
     }
-    uint32_t vis = 0;
-    visible_parts(a, r, p0, len, [&](uint32_t p, uint32_t, uint32_t bits) { vis |= bits << (p - p0); });
+    uint32_t vis = 0, own_slot[SL_PARTS] = {}, own[SL_PARTS] = {};
+    if (a.page_lg >= 3) {
+        if (len && a.visible.end) visible_own(a, r, p0, len, own_slot, own);
+#pragma unroll
+        for (uint32_t j = 0; j < SL_PARTS; ++j) vis |= own[j] << ((j << a.page_lg) & 31u);  // (0 from the last part on)
+    } else {
+        visible_parts(a, r, p0, len, [&](uint32_t p, uint32_t, uint32_t bits) { vis |= bits << (p - p0); });
+    }
     base = wave_total(base);
     const uint32_t n = __popc(vis), upto = wave_incl_scan(n), before = upto - n;
     const uint32_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
     uint32_t at = before;
-    visible_parts(a, r, p0, len, [&](uint32_t, uint32_t slot, uint32_t bits) {
+    auto list = [&](uint32_t, uint32_t slot, uint32_t bits) {
         for (; bits; bits &= bits - 1u) s_slot[at++] = static_cast<int32_t>(slot + __ffs(bits) - 1);
-    });
+    };
+    if (a.page_lg >= 3) {
+#pragma unroll
+        for (uint32_t j = 0; j < SL_PARTS; ++j) list(0, own_slot[j], own[j]);
+    } else {
+        visible_parts(a, r, p0, len, list);
+    }
     s_vis[t] = vis;
     s_before[t] = base + before;
     __syncthreads();
