@@ -596,8 +596,8 @@ constexpr int SL_NT = 64;
 constexpr uint32_t SL_POS = 32 * SL_NT;
 // Up to this many look-ups a lane, a workgroup counts what lies before its chunk by
 // itself; above, a launch of its own counts every chunk.  (8 requests, us counted and
-// alone: 16 look-ups 8.9 and 8.2 in pages of 64, 8.9 and 8.6 in pages of 16; 32 of
-// them 8.9 and 12.3, 8.9 and 12.4; 4 of them, 8192 positions in pages of 64, 8.8 and 6.4.)
+// alone: 16 look-ups 9.5 and 8.1 in pages of 64, 9.5 and 7.9 in pages of 16; 32 of
+// them 8.9 and 12.3, 8.9 and 12.4; 4 of them, 8192 positions in pages of 64, 8.8 and 6.5.)
 constexpr uint32_t SL_ALONE = 16;
 
 struct SelectArgs {
