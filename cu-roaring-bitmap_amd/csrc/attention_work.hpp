@@ -339,7 +339,8 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, uint32_t id, uint32
     const uint32_t even = ((w.keys + count - 1) / count + a.step - 1) / a.step * a.step;
     w.k0 = part * even;
     w.k1 = part + 1 == count ? w.keys : min(w.keys, w.k0 + even);
-    if (a.share && part == 0 && threadIdx.x == 0)
+    // (A number behind the last segment's tiles has no entry: there are more numbers than entries.)
+    if (a.share && part == 0 && !w.none && threadIdx.x == 0)
         a.ranges[tile_base(lo, w.token0, group, most) + tile] = make_uint2(id, count);
     return w;
 }

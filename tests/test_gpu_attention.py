@@ -466,3 +466,15 @@ def test_many_requests_of_single_tokens(gpu, n, density):
     new = np.ones(n, int)
     new[3::11] = 0
     Problem("float16", new.tolist(), kv.tolist(), 4, 2, 64, 16, seed=22, density=density).check(gpu, max_new=1)
+
+
+@pytest.mark.parametrize("density", [None, 0.5])
+@pytest.mark.parametrize("new_of_the_longest", [0, 40])
+@pytest.mark.parametrize("requests,heads", [(63, 8), (200, 2), (260, 1)])
+def test_tiles_of_many_requests(gpu, requests, heads, new_of_the_longest, density):
+    """More requests than a wave has lanes, in tiles for more than half of the card's places: the device cuts them where
+    one stands out, and leaves them whole where the longest has no new tokens."""
+    _say("attention tiles of many requests", requests, heads, new_of_the_longest, density)
+    new, kv = [33 + i % 3 for i in range(requests)], [70 + i % 23 for i in range(requests)]
+    p = Problem("bfloat16", new + [new_of_the_longest], kv + [4100], heads, heads, 64, 16, seed=23, density=density)
+    p.check(gpu, max_new=40)
