@@ -47,6 +47,7 @@ struct Half {
                                                       0);
     }
     static constexpr uint32_t EXP = 0x7C00u;  // the exponent's bits: all set in infinities and NaN
+    static constexpr float LIFT = 7.0f;
 };
 struct BHalf {
     static __device__ __forceinline__ float up(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
@@ -65,15 +66,28 @@ struct BHalf {
                                                        0);
     }
     static constexpr uint32_t EXP = 0x7F80u;
+    static constexpr float LIFT = 0.0f;
 };
 
 constexpr float NEG_INF = -__builtin_inff();
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 // A row's running maximum may fall this far (in powers of two) behind its
-// scores before the sums are scaled anew: probabilities then stay below 2^8,
-// which f16 holds, and a row is scaled a few times in all instead of at each
-// new maximum.
+// scores before the sums are scaled anew: a row is then scaled a few times in all
+// instead of at each new maximum.
 constexpr float LAG = 8.0f;
+
+// What a row's scores, in powers of two, are lowered by before their exponentials.
+// Those are summed in fp32, and rounded to the keys' type for the second product:
+// the matrix units take that type, and products of an upper and a lower part would
+// be twice as many.  bf16 has fp32's range.  f16 begins at 2^-24, so that its
+// exponentials are lifted by 2^LIFT: with the lag they reach 2^15, which it holds,
+// and a key counts down to 2^-32 of the row's largest (unlifted, 131072 keys at 2^-25
+// of it were lost).  Sums are lifted alike; the log-sum is lowered again.
+template <class E>
+__device__ __forceinline__ float base_of(float m, float c)
+{
+    return __builtin_fmaf(m, c, -E::LIFT);
+}
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -426,7 +440,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 #pragma unroll
                 for (uint32_t d = 0; d < BLOCKS; ++d) o[b][d] *= fix;
             }
-            const float mc = m[b] == NEG_INF ? 0.0f : m[b] * c;
+            const float mc = m[b] == NEG_INF ? 0.0f : base_of<E>(m[b], c);
 #pragma unroll
             for (uint32_t x = 0; x < 2; ++x)
 #pragma unroll
@@ -528,7 +542,7 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
         if (row < t.rows) {
             const uint32_t token = t.token0 + row / group, head = kh * group + row % group;
             const uint64_t place = place0 + b * 16 + mine;
-            const float lse2 = none ? NEG_INF : mt * c + __builtin_amdgcn_logf(lt);
+            const float lse2 = none ? NEG_INF : base_of<E>(mt, c) + __builtin_amdgcn_logf(lt);
 #pragma unroll
             for (uint32_t d = (threadIdx.x % 16) * 4; d < DIM; d += 64) {
                 f32x4 x = {0, 0, 0, 0};
@@ -840,7 +854,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 19
             f32x16 ahead_s[HALVES];
             v8s p[2 * HALVES];
             multiply(next_k, ahead_s);
-            const float mc = m == NEG_INF ? 0.0f : m * c;
+            const float mc = m == NEG_INF ? 0.0f : base_of<E>(m, c);
 #pragma unroll
             for (uint32_t x = 0; x < HALVES; ++x)
 #pragma unroll
@@ -913,7 +927,7 @@ __global__ __launch_bounds__(TL_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 19
             const f32x4 x = {o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
             if (at_d < a.dim) store_row(a, E{}, t, place, token, head, at_d, none ? f32x4{0, 0, 0, 0} : x * part);
         }
-    if (h == 0) store_lse(a, t, place, token, head, none ? NEG_INF : m * c + __builtin_amdgcn_logf(lt));
+    if (h == 0) store_lse(a, t, place, token, head, none ? NEG_INF : base_of<E>(m, c) + __builtin_amdgcn_logf(lt));
 }
 
 // ---- the ranges' results joined: a workgroup per row -----------------------------------

@@ -439,7 +439,8 @@ int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, uint32_t pa
  * h / (n_heads / cache->n_heads).  Queries, cache and outputs are of one type,
  * with 16-byte aligned rows of a head dimension that is a multiple of 8, up to
  * 256; sums and softmax are in fp32, and the probabilities are rounded to the
- * type before they meet the values. */
+ * type before they meet the values (f16: those below 2^-32 of a row's largest
+ * become zeros). */
 typedef struct cr_paged_attention_args {
     const void* q; /* [n_tokens][n_heads][head_dim] */
     uint64_t q_token_stride, q_head_stride;

@@ -478,3 +478,28 @@ def test_tiles_of_many_requests(gpu, requests, heads, new_of_the_longest, densit
     new, kv = [33 + i % 3 for i in range(requests)], [70 + i % 23 for i in range(requests)]
     p = Problem("bfloat16", new + [new_of_the_longest], kv + [4100], heads, heads, 64, 16, seed=23, density=density)
     p.check(gpu, max_new=40)
+
+
+@pytest.mark.parametrize("below", [17.5, 19.0, 21.0])
+@pytest.mark.parametrize("new,hints,sinks", [(1, dict(max_kv=100), [0, 32, 64, 96]), (40, dict(max_kv=200), [0])])
+def test_many_small_probabilities_count_in_f16(gpu, new, hints, sinks, below):
+    """A few keys that outdo 131072 others by e^17 and more, which together still weigh: each rounded probability is off by
+    2^-11 of itself, or, below f16's normal range, by 2^-32 of the largest at most."""
+    import torch
+    _say("attention small probabilities", new, below)
+    n = 131072
+    p = Problem("float16", [new], [n], 1, 1, 64, 16, seed=24, causal=False)
+    p.q[:], p.kc[:], p.vc[:] = 0, 0, 1
+    p.q[:, :, 0] = 1.0
+    for j in sinks:  # one for each wave that takes its own keys
+        page = p.table[0, j // 16].long()
+        p.kc[page, j % 16, 0, 0], p.vc[page, j % 16] = below, 0
+    out, lse = p.run(gpu, scale=1.0, **hints)
+    rest = (n - len(sinks)) * np.exp(-below)
+    o0, z0 = rest / (len(sinks) + rest), below + np.log(len(sinks) + rest)
+    ds = (64 + 8) * 2.0 ** -23 * below
+    u = U["float16"]
+    tol = 1.01 * (2 * u * o0 + n * 2.0 ** -32 + (2 * ds + n * 2.0 ** -24 + 2.0 ** -20) * o0)
+    assert np.all(np.abs(out - o0) <= tol), (out.min(), out.max(), o0, tol)
+    assert np.all(np.abs(lse - z0) <= ds + 2.0 ** -22 * (z0 + np.log(n) + 2) + n * 2.0 ** -24)
+    assert torch.isfinite(p.vc).all()
