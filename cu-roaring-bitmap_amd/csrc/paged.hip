@@ -621,9 +621,9 @@ struct SelectArgs {
 
 __device__ __forceinline__ uint32_t select_len(const SelectArgs& a, uint32_t r)
 {
-    const int32_t n = a.kv_len[r];
-    const uint64_t most = static_cast<uint64_t>(a.cols) << a.page_lg;
-    return n <= 0 ? 0u : static_cast<uint32_t>(min(most, static_cast<uint64_t>(n)));
+    // (Not `n <= 0 ? 0 : min(most, n)`: the compiler moves the min before the test and then takes n for positive.)
+    const uint64_t n = static_cast<uint64_t>(max(a.kv_len[r], 0));
+    return static_cast<uint32_t>(min(static_cast<uint64_t>(a.cols) << a.page_lg, n));
 }
 
 // Calls f(first position, first slot, visible bits) for each page, or 32
@@ -724,7 +724,8 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
     // positions of the new tokens: the last of the request's
     const int32_t t0 = min(max(a.starts[r], 0), static_cast<int32_t>(a.n_tokens));
     const int32_t t1 = min(max(a.starts[r + 1], t0), static_cast<int32_t>(a.n_tokens));
-    const int64_t shift = static_cast<int64_t>(t1) - len;  // position p is new token p + shift
+    // position p is new token p + shift: by the request's own length, of which the table may not hold all
+    const int64_t shift = static_cast<int64_t>(t1) - a.kv_len[r];
     if (chunk == 0) {  // tokens before the first position see nothing
         for (int64_t i = t0 + t; i < min(static_cast<int64_t>(t1), shift); i += SL_NT) a.limits[i] = 0;
     }
@@ -768,7 +769,12 @@ __global__ __launch_bounds__(SL_NT) void sl_write(SelectArgs a)
             static_cast<int32_t>(s_before[k / 32u] + __popc(s_vis[k / 32u] & (0xFFFFFFFFu >> (31u - k % 32u))));
     }
     for (uint32_t i = t; i < total; i += SL_NT) a.sel[r * a.sel_stride + base + i] = s_slot[i];
-    if (t == 0 && (len <= SL_POS || chunk == (len - 1) / SL_POS)) a.sel_len[r] = static_cast<int32_t>(base + total);
+    if (len <= SL_POS || chunk == (len - 1) / SL_POS) {
+        if (t == 0) a.sel_len[r] = static_cast<int32_t>(base + total);
+        // tokens behind the table's last position see all that it holds
+        for (int64_t i = max(static_cast<int64_t>(t0), len + shift) + t; i < t1; i += SL_NT)
+            a.limits[i] = static_cast<int32_t>(base + total);
+    }
 }
 
 // Bitmap containers are read where they lie; other layouts are written out as

@@ -420,8 +420,9 @@ int cr_paged_append(const void* d_k, const void* d_v, uint64_t k_token_stride, u
 /* The slots that a request may look at: d_sel[r * sel_stride + 0 .. d_sel_len[r])
  * are those slots of its positions [0, d_kv_len[r]), in order, that `visible`
  * (a bitmap over the slots) holds, and d_limits[t] says how many of them lie at
- * or before new token t's own position.  A row holds table_cols * page_size
- * slots.  Positions whose page is outside [0, n_pages) are not visible. */
+ * or before new token t's own position, which d_kv_len gives.  A row holds
+ * table_cols * page_size slots.  Positions behind the table's row, or whose page is
+ * outside [0, n_pages), are not visible. */
 int cr_paged_select(const cr_gpu_roaring* visible, uint32_t n_pages, uint32_t page_size, const int32_t* d_table,
                     uint32_t table_cols, uint64_t table_stride, const int32_t* d_starts, const int32_t* d_kv_len,
                     uint32_t n_requests, uint32_t n_tokens, int32_t* d_sel, uint64_t sel_stride, int32_t* d_sel_len,

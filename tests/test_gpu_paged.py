@@ -299,6 +299,44 @@ def test_select_counts_chunks(gpu, page, pages, kv, new, kind):
     assert np.array_equal(limits.cpu().numpy(), want_limits)
 
 
+@pytest.mark.parametrize("page,cols,kv,new", [(16, 3, [55, 48, 200, 30, 49, -4, 0], [10, 4, 70, 3, 1, 2, 2]),
+                                              (64, 70, [4490, 9000], [30, 4600]), (2, 1100, [2205, 2201], [2205, 1])])
+@pytest.mark.parametrize("density", [0.4, 1.0])
+def test_select_of_requests_longer_than_the_table(gpu, page, cols, kv, new, density):
+    """A token's place is by its request's length, also where the table does not hold all of it, as attention has it."""
+    import torch
+    _say("select past the table", page, cols, kv)
+    rng = np.random.default_rng(cols)
+    n, pages, room = len(kv), 2 * cols, cols * page
+    table = np.stack([rng.permutation(pages)[:cols] for _ in range(n)]).astype(np.int32)
+    visible = rng.random(pages * page) < density
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    want, want_len = [], []
+    for r in range(n):
+        pos = np.arange(min(room, max(0, kv[r])))
+        upto = np.concatenate([[0], np.cumsum(visible[table[r, pos // page].astype(np.int64) * page + pos % page])])
+        want_len.append(upto[-1])
+        want += [upto[min(len(pos), max(0, kv[r] - new[r] + i + 1))] for i in range(new[r])]
+    g = _bitmap(gpu, visible)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    sel, length, limits = torch.zeros(n, room, **i32), torch.full((n,), -5, **i32), torch.full((len(want) + 2,), -5, **i32)
+    lens = _cuda(np.array(kv, np.int32))
+    gpu.paged_select(g, _cuda(table), _cuda(starts), lens, page, sel, length, limits[:-2], pages)
+    torch.cuda.synchronize()
+    gpu.free(g)
+    assert np.array_equal(length.cpu().numpy(), want_len)
+    assert np.array_equal(limits.cpu().numpy(), want + [-5, -5])
+    if density == 1.0:  # all is visible: the answers of attention without a selection, to the order of its sums
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        q, kc, vc = (torch.randn(*s, device="cuda", generator=gen).half() for s in ((len(want), 2, 64), (pages, page, 1, 64),
+                                                                                  (pages, page, 1, 64)))
+        out = [torch.full_like(q, 7.0) for _ in range(2)]
+        for o, chosen in zip(out, (None, (sel, length, limits[:-2].contiguous()))):
+            gpu.paged_attention(q, kc, vc, _cuda(table), _cuda(starts), lens, o, selection=chosen)
+        torch.cuda.synchronize()
+        assert torch.allclose(out[0].float(), out[1].float(), rtol=2.0 ** -9, atol=2.0 ** -9)
+
+
 # ---- refusals --------------------------------------------------------------------
 def test_refusals(gpu):
     import torch
