@@ -124,8 +124,8 @@ __device__ __forceinline__ uint32_t segment_keys(const AttnArgs& a, uint32_t i, 
     n = 0;
     if (i == 0 || i > a.n_requests) return 0;
     n = a.sel ? a.sel_len[i - 1] : a.kv_len[i - 1];
-    const uint64_t room = static_cast<uint64_t>(a.cols) << a.page_lg;
-    return n <= 0 ? 0u : static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
+    // (Not `n <= 0 ? 0 : min(room, n)`: the compiler moves the min before the test and then takes n for positive.)
+    return static_cast<uint32_t>(min(static_cast<uint64_t>(a.cols) << a.page_lg, static_cast<uint64_t>(max(n, 0))));
 }
 
 // Segment i's tiles of `most` rows are numbered from here, which leaves each
