@@ -1106,9 +1106,13 @@ extern "C" int cr_paged_attention(const cr_paged_attention_args* args, const cr_
                   cache->n_heads, cache->page_size);
         return CR_ERR_INVALID;
     }
-    const uint64_t strides = p.q_token_stride | p.q_head_stride | p.out_token_stride | p.out_head_stride |
-                             cache->k_page_stride | cache->k_slot_stride | cache->k_head_stride |
-                             cache->v_page_stride | cache->v_slot_stride | cache->v_head_stride | cache->head_dim;
+    // The strides that lead anywhere: that of an axis of one entry may be any number.
+    auto over = [](uint32_t extent, uint64_t x, uint64_t y) { return extent > 1 ? x | y : 0; };
+    const uint64_t strides = over(p.n_tokens, p.q_token_stride, p.out_token_stride) |
+                             over(p.n_heads, p.q_head_stride, p.out_head_stride) |
+                             over(cache->n_pages, cache->k_page_stride, cache->v_page_stride) |
+                             over(cache->page_size, cache->k_slot_stride, cache->v_slot_stride) |
+                             over(cache->n_heads, cache->k_head_stride, cache->v_head_stride) | cache->head_dim;
     const uintptr_t at = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) |
                          reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v);
     if ((cache->dtype != CR_F16 && cache->dtype != CR_BF16) || cache->head_dim > AT_DIM_MAX || strides % 8 || at % 16) {

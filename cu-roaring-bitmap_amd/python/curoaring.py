@@ -585,6 +585,8 @@ def _table(t, n_requests: int):
     """(address, columns, row stride) of a block table, rows of which may lie apart."""
     if _type_name(t) == "int32" and t.is_cuda and t.dim() == 2:
         (rows, cols), (stride, one) = t.shape, t.stride()
+        if rows <= 1:  # whose stride may be any number
+            stride = cols
         if rows == n_requests and (one == 1 or cols <= 1) and stride >= cols:
             return t.data_ptr(), cols, stride
     raise CrError(CR_ERR_INVALID, f"block table: an int32 CUDA tensor of {n_requests} rows is taken, not {t.dtype} "

@@ -503,3 +503,26 @@ def test_many_small_probabilities_count_in_f16(gpu, new, hints, sinks, below):
     assert np.all(np.abs(out - o0) <= tol), (out.min(), out.max(), o0, tol)
     assert np.all(np.abs(lse - z0) <= ds + 2.0 ** -22 * (z0 + np.log(n) + 2) + n * 2.0 ** -24)
     assert torch.isfinite(p.vc).all()
+
+
+def test_strides_of_axes_of_one_entry(gpu):
+    """One token, one key head, one page, a table of one row: their strides lead nowhere, and may be odd numbers."""
+    import torch
+    _say("attention odd strides of single entries")
+    p = Problem("float16", [1], [11], 3, 1, 64, 16, seed=25)
+    row, one = p.table[0, :1].clone(), dict(scale=0.125, max_new=1)
+    kc, vc = (x[row.long()].clone() for x in (p.kc, p.vc))
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    want, got = torch.zeros_like(p.q), torch.zeros(1, 3, 64, device="cuda").half()
+    gpu.paged_attention(p.q, kc, vc, table, p.starts, p.kv_len, want, **one)
+    odd = lambda x, *stride: torch.as_strided(x, x.shape, stride)  # noqa: E731
+    gpu.paged_attention(odd(p.q, 1, 64, 1), odd(kc, 3, 64, 1, 1), odd(vc, 5, 64, 7, 1), odd(table, 0, 1), p.starts,
+                        p.kv_len, odd(got, 1, 64, 1), **one)
+    torch.cuda.synchronize()
+    assert torch.equal(want, got) and torch.isfinite(got).all() and got.abs().sum() > 0
+    # with one slot a page, its stride leads nowhere either
+    kc, vc = (x[:, :1].clone() for x in (kc, vc))
+    gpu.paged_attention(p.q, kc, vc, table, p.starts, torch.ones_like(p.kv_len), want, **one)
+    gpu.paged_attention(p.q, odd(kc, 3, 9, 1, 1), odd(vc, 1, 1, 1, 1), table, p.starts, torch.ones_like(p.kv_len), got, **one)
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
