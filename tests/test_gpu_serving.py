@@ -81,3 +81,44 @@ def test_constrained_beam_search(gpu, lengths, beams):
     assert ex.cr.cardinality(server.free) == 1024
     ex.cr.free(allowed)
     server.close()
+
+
+def test_allocation_failures_are_reported(gpu):
+    """Select, attention and beam selection without memory for their workspace: an error, nothing written, and the same
+    call goes through afterwards."""
+    import torch
+    i32 = dict(dtype=torch.int32, device="cuda")
+    half = lambda *s: torch.randn(*s, device="cuda").half()  # noqa: E731
+    kv, page = 20000, 16  # long enough to be counted by a launch of its own
+    pages = -(-kv // page)
+    table, starts, kv_len = torch.arange(pages, **i32)[None], torch.tensor([0, 1], **i32), torch.tensor([kv], **i32)
+    visible = gpu.upload_from_ids(np.arange(0, pages * page, 2, dtype=np.uint32), pages * page)
+    sparse = gpu.upload_from_ids(np.arange(0, 300, 7, dtype=np.uint32), 1000, gpu.PROMOTE_KEEP_DEFAULT)
+    sel, sel_len, limits = torch.full((1, pages * page), -5, **i32), torch.full((1,), -5, **i32), torch.full((1,), -5, **i32)
+    q, kc, vc = half(1, 4, 64), half(pages, page, 1, 64), half(pages, page, 1, 64)
+    out, lse = torch.full_like(q, 7.0), torch.full((1, 4), 7.0, device="cuda")
+    scores, tokens, parents = torch.full((1, 3), 7.0, device="cuda"), torch.full((1, 3), -5, **i32), torch.full((1, 3), -5, **i32)
+    x, cum = torch.randn(1, 2, 1000, device="cuda"), torch.zeros(1, 2, device="cuda")
+    lib = gpu.load()
+    for what, call, outputs in (
+            ("select", lambda: gpu.paged_select(visible, table, starts, kv_len, page, sel, sel_len, limits, pages),
+             (sel, sel_len, limits)),
+            ("attention", lambda: gpu.paged_attention(q, kc, vc, table, starts, kv_len, out, d_lse=lse), (out, lse)),
+            ("beam select", lambda: gpu.beam_select(x, cum, scores, tokens, parents, allowed=sparse),
+             (scores, tokens, parents))):
+        print("CASE allocation failure", what, flush=True)
+        before = [t.clone() for t in outputs]
+        lib.cr_debug_fail_device_allocs(0, 1)
+        try:
+            with pytest.raises(gpu.CrError) as e:
+                call()
+            assert e.value.code == gpu.CR_ERR_ALLOC
+        finally:
+            lib.cr_debug_fail_device_allocs(0, 0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(before, outputs)), what
+        call()
+        torch.cuda.synchronize()
+        assert not any(torch.equal(a, b) for a, b in zip(before, outputs)), what
+    for g in (visible, sparse):
+        gpu.free(g)
