@@ -553,6 +553,20 @@ _ATTENTION = struct.Struct("@PQQPQQPIIIPPPIQPQPPfIII")
 assert _CACHE.size == C.sizeof(PagedCache) and _ATTENTION.size == C.sizeof(PagedAttentionArgs)
 
 
+_devices = None
+
+
+def _device() -> int:
+    """The number of the current device, on which the calls below run, and their tensors have to be: -2 without one."""
+    global _devices
+    if _devices is None or _devices > 1:
+        import torch
+        _devices = torch.cuda.device_count()
+        if _devices > 1:
+            return torch.cuda.current_device()
+    return 0 if _devices else -2
+
+
 def _type_name(t) -> str:
     name = _names.get(t.dtype)
     if name is None:
@@ -571,54 +585,54 @@ def _typed(t) -> int:
     return code
 
 
-def _array(t, name: str, dtype: str, shape) -> int:
-    """The address of a contiguous CUDA tensor of this type and shape (0: one axis of any extent)."""
-    if (_names.get(t.dtype) or _type_name(t)) == dtype and t.is_cuda and t.is_contiguous() and (
+def _array(t, name: str, dtype: str, shape, device: int) -> int:
+    """The address of a contiguous tensor of this type and shape (0: one axis of any extent) on this device."""
+    if (_names.get(t.dtype) or _type_name(t)) == dtype and t.get_device() == device and t.is_contiguous() and (
             t.dim() == 1 if shape == 0 else t.shape == shape):
         return t.data_ptr()
-    raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} CUDA tensor of shape "
-                                  f"{'(any,)' if shape == 0 else tuple(shape)} is taken, not "
-                                  f"{t.dtype} {tuple(t.shape)}")
+    raise CrError(CR_ERR_INVALID, f"{name}: a contiguous {dtype} tensor of shape "
+                                  f"{'(any,)' if shape == 0 else tuple(shape)} on the current CUDA device is taken, not "
+                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _table(t, n_requests: int):
+def _table(t, n_requests: int, device: int):
     """(address, columns, row stride) of a block table, rows of which may lie apart."""
-    if _type_name(t) == "int32" and t.is_cuda and t.dim() == 2:
+    if _type_name(t) == "int32" and t.get_device() == device and t.dim() == 2:
         (rows, cols), (stride, one) = t.shape, t.stride()
         if rows <= 1:  # whose stride may be any number
             stride = cols
         if rows == n_requests and (one == 1 or cols <= 1) and stride >= cols:
             return t.data_ptr(), cols, stride
-    raise CrError(CR_ERR_INVALID, f"block table: an int32 CUDA tensor of {n_requests} rows is taken, not {t.dtype} "
-                                  f"{tuple(t.shape)}")
+    raise CrError(CR_ERR_INVALID, f"block table: an int32 tensor of {n_requests} rows on the current CUDA device is "
+                                  f"taken, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _rows(t, name: str, dtype, shape):
+def _rows(t, name: str, dtype, shape, device: int):
     """(address, token stride, head stride) of a [tokens, heads, dim] tensor of this type and shape."""
-    if t.dtype == dtype and t.is_cuda and t.shape == shape:
+    if t.dtype == dtype and t.get_device() == device and t.shape == shape:
         token, head, one = t.stride()
         if one == 1 or shape[2] <= 1:
             return t.data_ptr(), token, head
-    raise CrError(CR_ERR_INVALID, f"{name}: a {dtype} CUDA tensor of shape {tuple(shape)} with contiguous rows is "
-                                  f"taken, not {t.dtype} {tuple(t.shape)}")
+    raise CrError(CR_ERR_INVALID, f"{name}: a {dtype} tensor of shape {tuple(shape)} with contiguous rows on the "
+                                  f"current CUDA device is taken, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _cache(d_k, d_v):
+def _cache(d_k, d_v, device: int):
     """(cr_paged_cache, page size, heads, dim) of a cache's tensors."""
     shape = d_k.shape
-    if len(shape) == 4 and d_v.shape == shape and d_k.dtype == d_v.dtype and d_k.is_cuda and d_v.is_cuda:
+    if len(shape) == 4 and d_v.shape == shape and d_k.dtype == d_v.dtype and d_k.get_device() == device == d_v.get_device():
         (kp, ks, kh, k1), (vp, vs, vh, v1) = d_k.stride(), d_v.stride()
         pages, size, heads, dim = shape
         if (k1 == 1 and v1 == 1) or dim <= 1:
             return _CACHE.pack(d_k.data_ptr(), d_v.data_ptr(), kp, ks, kh, vp, vs, vh, pages, size, heads, dim,
                                _typed(d_k)), size, heads, dim
     raise CrError(CR_ERR_INVALID, "cache: keys and values of one type and shape [pages, page size, heads, dim] with "
-                                  "contiguous rows are taken")
+                                  "contiguous rows on the current CUDA device are taken")
 
 
 def paged_cache(d_k, d_v) -> PagedCache:
     """A cache of [pages, page size, heads, dim] keys and values (any strides with contiguous rows)."""
-    return PagedCache.from_buffer_copy(_cache(d_k, d_v)[0])
+    return PagedCache.from_buffer_copy(_cache(d_k, d_v, _device())[0])
 
 
 def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d_new, d_table, d_slots, d_starts,
@@ -628,26 +642,27 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
     d_cached, d_new: int32 [R], tokens in the cache and new ones.  d_table: int32 [R, cols], completed in place with
     pages from `free_pages`.  Written: d_slots int64 [at least the new tokens], d_starts int32 [R + 1], d_kv_len
     int32 [R], d_taken int32 [any], d_counts int32 [3]: new tokens, pages taken, pages missing."""
-    n = d_cached.numel()
-    table, cols, stride = _table(d_table, n)
-    _check(load().cr_paged_plan(C.byref(free_pages), n_pages, page_size, _array(d_cached, "cached", "int32", (n,)),
-                                _array(d_new, "new", "int32", (n,)), n, table, cols, stride,
-                                _array(d_slots, "slots", "int64", 0), d_slots.numel(),
-                                _array(d_starts, "starts", "int32", (n + 1,)),
-                                _array(d_kv_len, "kv_len", "int32", (n,)),
-                                _array(d_taken, "taken", "int32", 0), d_taken.numel(),
-                                _array(d_counts, "counts", "int32", (3,)), _stream(stream)), "paged_plan")
+    n, on = d_cached.numel(), _device()
+    table, cols, stride = _table(d_table, n, on)
+    _check(load().cr_paged_plan(C.byref(free_pages), n_pages, page_size, _array(d_cached, "cached", "int32", (n,), on),
+                                _array(d_new, "new", "int32", (n,), on), n, table, cols, stride,
+                                _array(d_slots, "slots", "int64", 0, on), d_slots.numel(),
+                                _array(d_starts, "starts", "int32", (n + 1,), on),
+                                _array(d_kv_len, "kv_len", "int32", (n,), on),
+                                _array(d_taken, "taken", "int32", 0, on), d_taken.numel(),
+                                _array(d_counts, "counts", "int32", (3,), on), _stream(stream)), "paged_plan")
 
 
 def paged_append(d_k, d_v, d_slots, d_k_cache, d_v_cache, stream=None):
     """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out."""
-    cache, _, heads, dim = _cache(d_k_cache, d_v_cache)
+    on = _device()
+    cache, _, heads, dim = _cache(d_k_cache, d_v_cache, on)
     n, dtype = d_slots.numel(), d_k_cache.dtype
     shape = (n, heads, dim)
-    k, k_token, k_head = _rows(d_k, "k", dtype, shape)
-    v, v_token, v_head = _rows(d_v, "v", dtype, shape)
+    k, k_token, k_head = _rows(d_k, "k", dtype, shape, on)
+    v, v_token, v_head = _rows(d_v, "v", dtype, shape, on)
     _check(load().cr_paged_append(k, v, k_token, k_head, v_token, v_head, n,
-                                  _array(d_slots, "slots", "int64", (n,)), cache, _stream(stream)), "paged_append")
+                                  _array(d_slots, "slots", "int64", (n,), on), cache, _stream(stream)), "paged_append")
 
 
 def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: int, d_sel, d_sel_len, d_limits,
@@ -656,18 +671,18 @@ def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: in
 
     Written: d_sel int32 [R, at least cols * page_size], d_sel_len int32 [R], d_limits int32 [T].  n_pages: the
     cache's (default: as many as the bitmap's universe holds)."""
-    n = d_kv_len.numel()
-    table, cols, stride = _table(d_table, n)
-    sel, room, sel_stride = _table(d_sel, n)
+    n, on = d_kv_len.numel(), _device()
+    table, cols, stride = _table(d_table, n, on)
+    sel, room, sel_stride = _table(d_sel, n, on)
     if room < cols * page_size:
         raise CrError(CR_ERR_INVALID, f"paged_select: a row of sel holds cols * page_size = {cols * page_size} slots")
     if n_pages is None:
         n_pages = visible.universe_size // page_size
     _check(load().cr_paged_select(C.byref(visible), n_pages, page_size, table, cols, stride,
-                                  _array(d_starts, "starts", "int32", (n + 1,)),
-                                  _array(d_kv_len, "kv_len", "int32", (n,)), n, d_limits.numel(), sel, sel_stride,
-                                  _array(d_sel_len, "sel_len", "int32", (n,)),
-                                  _array(d_limits, "limits", "int32", 0), _stream(stream)), "paged_select")
+                                  _array(d_starts, "starts", "int32", (n + 1,), on),
+                                  _array(d_kv_len, "kv_len", "int32", (n,), on), n, d_limits.numel(), sel, sel_stride,
+                                  _array(d_sel_len, "sel_len", "int32", (n,), on),
+                                  _array(d_limits, "limits", "int32", 0, on), _stream(stream)), "paged_select")
 
 
 def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_out, scale: Optional[float] = None,
@@ -677,28 +692,29 @@ def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_ou
     Request r's tokens are [starts[r], starts[r + 1]), the last of its kv_len[r] positions.  scale: 1 / sqrt(dim) by
     default.  d_lse: float32 [T, heads] or None.  selection: paged_select's (sel, sel_len, limits) or None.  max_new
     and max_kv: the most new tokens and keys of a request if known; they choose how the work is split."""
-    cache, page_size, _, dim = _cache(d_k_cache, d_v_cache)
+    on = _device()
+    cache, page_size, _, dim = _cache(d_k_cache, d_v_cache, on)
     dtype, shape = d_k_cache.dtype, d_q.shape
     if len(shape) != 3 or d_q.dtype != dtype or shape[2] != dim:
         raise CrError(CR_ERR_INVALID, f"paged_attention: {dtype} queries [tokens, heads, {dim}] are taken, not "
                                       f"{d_q.dtype} {tuple(shape)}")
     n, (tokens, heads, _) = d_kv_len.numel(), shape
-    q, q_token, q_head = _rows(d_q, "q", dtype, shape)
-    out, out_token, out_head = _rows(d_out, "out", dtype, shape)
-    table, cols, stride = _table(d_table, n)
+    q, q_token, q_head = _rows(d_q, "q", dtype, shape, on)
+    out, out_token, out_head = _rows(d_out, "out", dtype, shape, on)
+    table, cols, stride = _table(d_table, n, on)
     sel, room, sel_stride, sel_len, limits = 0, 0, 0, 0, 0
     if selection is not None:
-        sel, room, sel_stride = _table(selection[0], n)
+        sel, room, sel_stride = _table(selection[0], n, on)
         if room < cols * page_size:
             raise CrError(CR_ERR_INVALID, "paged_attention: a row of sel holds cols * page_size slots")
-        sel_len = _array(selection[1], "sel_len", "int32", (n,))
-        limits = _array(selection[2], "limits", "int32", (tokens,))
+        sel_len = _array(selection[1], "sel_len", "int32", (n,), on)
+        limits = _array(selection[2], "limits", "int32", (tokens,), on)
     if not (0 <= max_new < 1 << 32 and 0 <= max_kv < 1 << 32):
         raise CrError(CR_ERR_INVALID, f"paged_attention: max_new {max_new}, max_kv {max_kv}")
     a = _ATTENTION.pack(q, q_token, q_head, out, out_token, out_head,
-                        _array(d_lse, "lse", "float32", (tokens, heads)) if d_lse is not None else 0,
-                        tokens, heads, n, _array(d_starts, "starts", "int32", (n + 1,)),
-                        _array(d_kv_len, "kv_len", "int32", (n,)), table, cols, stride, sel, sel_stride, sel_len,
+                        _array(d_lse, "lse", "float32", (tokens, heads), on) if d_lse is not None else 0,
+                        tokens, heads, n, _array(d_starts, "starts", "int32", (n + 1,), on),
+                        _array(d_kv_len, "kv_len", "int32", (n,), on), table, cols, stride, sel, sel_stride, sel_len,
                         limits, dim ** -0.5 if scale is None else scale, causal, max_new, max_kv)
     _check(load().cr_paged_attention(a, cache, _stream(stream)), "paged_attention")
 
@@ -710,22 +726,24 @@ def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_ls
     allowed: a bitmap over [0, V), or int32 bitsets [ceil(V / 32)] (one for all) or [B, W, ceil(V / 32)], or None."""
     b, w, v = d_scores.shape
     k = d_out_scores.shape[1]
-    if not d_scores.is_cuda or (v > 1 and d_scores.stride(2) != 1):
-        raise CrError(CR_ERR_INVALID, "beam_select: a CUDA tensor of scores with contiguous rows is taken")
+    on = _device()
+    if d_scores.get_device() != on or (v > 1 and d_scores.stride(2) != 1):
+        raise CrError(CR_ERR_INVALID, "beam_select: scores with contiguous rows on the current CUDA device are taken, not "
+                                      f"on {d_scores.device}")
     words, bitmap, bits, stride = (v + 31) // 32, None, None, 0
     if isinstance(allowed, GpuRoaring):
         bitmap = C.byref(allowed)
     elif allowed is not None:
-        bits = _array(allowed, "allowed", "int32", (words,) if allowed.dim() == 1 else (b, w, words))
+        bits = _array(allowed, "allowed", "int32", (words,) if allowed.dim() == 1 else (b, w, words), on)
         stride = 0 if allowed.dim() == 1 else words
     per_batch, per_beam, _ = d_scores.stride()
     _check(load().cr_beam_select(_dptr(d_scores), _typed(d_scores), b, w, v, per_batch, per_beam,
-                                 _array(d_cum, "cum", "float32", (b, w)),
-                                 _array(d_lse, "lse", "float32", (b, w)) if d_lse is not None else None,
+                                 _array(d_cum, "cum", "float32", (b, w), on),
+                                 _array(d_lse, "lse", "float32", (b, w), on) if d_lse is not None else None,
                                  bitmap, bits, stride, k,
-                                 _array(d_out_scores, "out_scores", "float32", (b, k)),
-                                 _array(d_out_tokens, "out_tokens", "int32", (b, k)),
-                                 _array(d_out_parents, "out_parents", "int32", (b, k)), _stream(stream)),
+                                 _array(d_out_scores, "out_scores", "float32", (b, k), on),
+                                 _array(d_out_tokens, "out_tokens", "int32", (b, k), on),
+                                 _array(d_out_parents, "out_parents", "int32", (b, k), on), _stream(stream)),
            "beam_select")
 
 
@@ -736,15 +754,17 @@ def beam_reorder(d_src, d_parents, d_dst, d_len=None, stream=None):
     (-1) are left alone."""
     b, w, *of_state = d_src.shape
     k = d_parents.shape[1]
-    if not (d_src.is_cuda and d_dst.is_cuda and d_src.is_contiguous() and d_dst.is_contiguous()) or (
+    on = _device()
+    if not (d_src.get_device() == on == d_dst.get_device() and d_src.is_contiguous() and d_dst.is_contiguous()) or (
             d_src.dtype != d_dst.dtype or d_dst.shape != (b, k, *of_state)):
-        raise CrError(CR_ERR_INVALID, f"beam_reorder: contiguous CUDA states [{b}, {w}, ...] into [{b}, {k}, ...]")
+        raise CrError(CR_ERR_INVALID, f"beam_reorder: contiguous states [{b}, {w}, ...] into [{b}, {k}, ...] on the current CUDA "
+                                      "device")
     if d_len is not None and not of_state:
         raise CrError(CR_ERR_INVALID, "beam_reorder: lengths count along the states' third extent")
     row = d_src.nbytes // (b * w or 1)
     unit = row // (of_state[0] or 1) if d_len is not None else 0
-    _check(load().cr_beam_reorder(_dptr(d_src), _array(d_parents, "parents", "int32", (b, k)), b, w, k, row, row, row,
-                                  _array(d_len, "len", "int32", (b, w)) if d_len is not None else None, unit,
+    _check(load().cr_beam_reorder(_dptr(d_src), _array(d_parents, "parents", "int32", (b, k), on), b, w, k, row, row, row,
+                                  _array(d_len, "len", "int32", (b, w), on) if d_len is not None else None, unit,
                                   _dptr(d_dst), _stream(stream)), "beam_reorder")
 
 

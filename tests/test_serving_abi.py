@@ -130,3 +130,58 @@ def test_tensors_on_the_host_are_refused():
         with pytest.raises(cr.CrError) as e:
             call()
         assert e.value.code == INVALID
+
+
+class _On:
+    """A host tensor that says it is on a device; the library is not called with it."""
+
+    def __init__(self, t, device):
+        self.t, self.number = t, device
+
+    is_cuda = True
+
+    def get_device(self):
+        return self.number
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    import torch
+    i32, half = dict(dtype=torch.int32), dict(dtype=torch.float16)
+    k, cache = torch.zeros(2, 2, 64, **half), torch.zeros(4, 16, 2, 64, **half)
+    n, starts, table = torch.ones(2, **i32), torch.zeros(3, **i32), torch.zeros(2, 4, **i32)
+    calls = {
+        "paged_plan": (dict(d_cached=n, d_new=n, d_table=table, d_slots=torch.zeros(8, dtype=torch.int64), d_starts=starts,
+                            d_kv_len=n, d_taken=n, d_counts=starts), dict(free_pages=cr.GpuRoaring(), n_pages=8, page_size=16)),
+        "paged_append": (dict(d_k=k, d_v=k, d_slots=torch.zeros(2, dtype=torch.int64), d_k_cache=cache, d_v_cache=cache), {}),
+        "paged_select": (dict(d_table=table, d_starts=starts, d_kv_len=n, d_sel=torch.zeros(2, 64, **i32), d_sel_len=n,
+                              d_limits=n), dict(visible=cr.GpuRoaring(), page_size=16)),
+        "paged_attention": (dict(d_q=k, d_k_cache=cache, d_v_cache=cache, d_table=table, d_starts=starts, d_kv_len=n, d_out=k,
+                                 d_lse=torch.zeros(2, 2)), {}),
+        "beam_select": (dict(d_scores=torch.zeros(1, 2, 10), d_cum=torch.zeros(1, 2), d_out_scores=torch.zeros(1, 3),
+                             d_out_tokens=torch.zeros(1, 3, **i32), d_out_parents=torch.zeros(1, 3, **i32),
+                             d_lse=torch.zeros(1, 2), allowed=torch.zeros(1, **i32)), {}),
+        "beam_reorder": (dict(d_src=k, d_parents=torch.zeros(2, 2, **i32), d_dst=k.clone(), d_len=torch.ones(2, 2, **i32)), {})}
+    called = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: called.append(name) or OK
+
+    monkeypatch.setattr(cr, "load", Library)
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 2)
+    for here in (0, 1):
+        monkeypatch.setattr(cr, "_devices", None)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: here)
+        for name, (tensors, rest) in calls.items():
+            on = {x: _On(t, here) for x, t in tensors.items()}
+            called.clear()
+            getattr(cr, name)(**on, **rest)
+            assert called == ["cr_" + name]
+            for x, t in tensors.items():
+                with pytest.raises(cr.CrError) as e:
+                    getattr(cr, name)(**{**on, x: _On(t, 1 - here)}, **rest)
+                assert e.value.code == INVALID and "current CUDA device" in str(e.value), (name, x)
+            assert len(called) == 1
