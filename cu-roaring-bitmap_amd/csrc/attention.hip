@@ -267,7 +267,7 @@ __device__ __forceinline__ void store_lse(const AttnArgs& a, const Work& t, uint
 // 7).  On the way, each alone: keys loaded straight in operand order, which asks
 // for half lines, 400, past the caches even 430; whole rows past them 376; a tile's
 // offsets looked up once, through LDS, 361.  48 requests of 4 rows and up to 2048
-// keys, 16 heads of 64 dimensions: 52 us, 4.2 TB/s; they are one workgroup a slot
+// keys, 16 heads of 64 dimensions: 49 us, 4.5 TB/s; they are one workgroup a slot
 // of the card and wait for the longest (64 keys a tile, with fewer waves, 59).
 
 template <uint32_t DIM>
@@ -573,7 +573,9 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 // One workgroup and two waves a SIMD more or less keep the other busy too.
 // Up to 192 dimensions (8 requests of 1000 tokens of up to 8192, 24 heads over 8:
 // 588 us, 657 TFLOP/s, with one wave a SIMD 950); 256 leave registers for one
-// (1540 us, 413).
+// (1540 us, 413).  Of ragged chunks the longest is waited for (8 of up to 1000 tokens
+// of up to 8192 keys, of which 0.6 are visible, 96 dimensions: 872 workgroups on 512
+// places, which the longest first keep busy 0.8 of the time: 140 us, 640 TFLOP/s).
 // 16384 tokens, 32 heads over 8, 128 dimensions, bf16: 2.31 ms, 950 TFLOP/s (a
 // large bf16 library product reaches 1206): the matrix units work 45% of the
 // cycles, at 2.0 GHz, to which their power brings the clock down from 2.35.  On
@@ -581,7 +583,9 @@ __global__ __launch_bounds__(DC_NT) void at_rows(AttnArgs a)
 // running ahead 2.36; 64 rows a wave with one wave a SIMD, which halves what is
 // read from LDS, 3.2.
 constexpr int TL_NT = 256;
-// Keys of a tile: 64, or 32 where longer rows would not leave room for the next tile's in registers.
+// Keys of a tile: 64, or 32 of longer rows: the tile's keys and values and the next
+// one's take 64 KB of LDS then, as 64 of up to 128 dimensions do (of up to 64, 32
+// KB), and 128 KB would leave no room for a second workgroup.
 constexpr uint32_t tile_keys(uint32_t dim) { return dim <= 128 ? 64 : 32; }
 
 // Orders the products of the block before: READS fragments of LDS first, then

@@ -77,6 +77,11 @@ inline bool size_launch(AttnArgs& a, uint64_t room, uint32_t max_new, uint32_t m
     // reading the lengths and joining cost more than they even out (256 of up to
     // 1024 keys: uncut 110 us, cut 160; of up to 4096 372 and 389; 48 of up to 2048
     // with 16 heads of 64 dimensions 53 and 60).
+    // `held`, the workgroups that the card holds at once, is that of one block of rows a
+    // wave.  Of two, a CU holds one less (two up to 64 dimensions, one above), so that
+    // theirs run in about two rounds.  Counted as they are, 8 tokens of 8192 keys would
+    // take 20 us instead of 32 and 64 requests of 8 of 4096 239 instead of 262, but 20
+    // of 6 of 30000 456 instead of 397 (32 heads over 8, 128 dimensions).
     const uint64_t tiles_in_all = (rows + most - 1) / most * requests;
     const uint64_t longest = std::min<uint64_t>(room, max_kv ? max_kv : room);
     const uint32_t on_a_cu = per_wave && a.dim <= 64 ? 3 : a.dim <= (per_wave ? 128 : 192) ? 2 : 1;
@@ -91,8 +96,9 @@ inline bool size_launch(AttnArgs& a, uint64_t room, uint32_t max_new, uint32_t m
     // Tiles for more than half of the card, but perhaps of requests so uneven that the
     // longest would be waited for: the device looks at the lengths (5 of 1924 tokens
     // of up to 42670, 4 heads: uncut 955 us, cut 410; 16 of 100 of 4096 104 and 83).
-    // With more tiles the rows to be joined cost more than it gains (8 of 1000 of
-    // 8192, 192 tiles for 65 places: 179 and 201).
+    // With more tiles it costs more than it gains: rows to be joined, and ranges in
+    // the requests' order where uncut tiles go longest first (8 of 1000 of 8192, 192
+    // tiles for 65 places: 179 and 201).
     const bool uneven =
         !per_wave && !few && a.n_requests > 1 && a.dim <= 128 && longest >= 4096 && tiles_in_all <= held;
     const bool cut = (few || long_ones || uneven) && all_rows >> 24 == 0;

@@ -305,7 +305,7 @@ __device__ __forceinline__ float lane_best(const Row<T>& row, const Allowed& all
 // threads: 512 for few winners (k = 8 of 64 x 8 x 100003: 10.1 us, with 256 12.5,
 // with 1024 10.6), 1024 for many, whose groups then take fewer rounds.  With the
 // lanes' maxima where groups are few, 10 x 8 x 1507, k = 8, takes 19 us in all
-// instead of 50, 4 x 4 x 30000, k = 64, 40 instead of 134.
+// instead of 50, 4 x 4 x 30000, k = 64, 37 instead of 134.
 template <class T, uint32_t NT>
 __global__ __launch_bounds__(NT) void bs_pick(BeamArgs a, const uint32_t* __restrict__ gmax)
 {

@@ -448,7 +448,8 @@ __global__ __launch_bounds__(PG_TAKE_NT) void pg_take(PlanArgs a)
 
 // The slot of each new token, from the tables as pg_take left them, two tokens a
 // thread at a time, past the caches (12 us; through them 13.5).  The requests of
-// the workgroup's tokens are kept in LDS (searched in memory, 15.9 us).
+// the workgroup's tokens are kept in LDS (searched in memory, 15.9 us).  Each token
+// still looks for its request and reads its page's entry by itself.
 __global__ __launch_bounds__(PG_FILL_NT) void pg_slots(PlanArgs a, bool pairs)
 {
     __shared__ int32_t s_start[PG_FILL_NT], s_kv[PG_FILL_NT], s_cached[PG_FILL_NT];

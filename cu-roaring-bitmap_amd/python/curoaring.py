@@ -544,6 +544,8 @@ def download_batch(b: RoaringBatch) -> SimpleNamespace:
 
 
 # ---- serving language models (stream-ordered, no synchronisation) ---------------
+# As in all calls here, stream=None is the null stream, also inside torch.cuda.stream(s), where the tensors' own
+# producers run on s: pass stream=torch.cuda.current_stream() there.  Tensors lie on the current device.
 F32, F16, BF16 = 0, 1, 2
 _TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
 _names, _codes = {}, {}
@@ -641,7 +643,8 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
 
     d_cached, d_new: int32 [R], tokens in the cache and new ones.  d_table: int32 [R, cols], completed in place with
     pages from `free_pages`.  Written: d_slots int64 [at least the new tokens], d_starts int32 [R + 1], d_kv_len
-    int32 [R], d_taken int32 [any], d_counts int32 [3]: new tokens, pages taken, pages missing."""
+    int32 [R], d_taken int32 [any], d_counts int32 [3]: new tokens, pages taken, pages missing.  stream: None is the
+    null stream."""
     n, on = d_cached.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
     _check(load().cr_paged_plan(C.byref(free_pages), n_pages, page_size, _array(d_cached, "cached", "int32", (n,), on),
@@ -654,7 +657,9 @@ def paged_plan(free_pages: GpuRoaring, n_pages: int, page_size: int, d_cached, d
 
 
 def paged_append(d_k, d_v, d_slots, d_k_cache, d_v_cache, stream=None):
-    """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out."""
+    """New keys and values [T, heads, dim] into slots int64 [T] of the cache; slots outside it (-1) are left out.
+
+    stream: None is the null stream."""
     on = _device()
     cache, _, heads, dim = _cache(d_k_cache, d_v_cache, on)
     n, dtype = d_slots.numel(), d_k_cache.dtype
@@ -670,7 +675,7 @@ def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: in
     """The slots of each request that the bitmap `visible` holds, listed once for every layer's attention.
 
     Written: d_sel int32 [R, at least cols * page_size], d_sel_len int32 [R], d_limits int32 [T].  n_pages: the
-    cache's (default: as many as the bitmap's universe holds)."""
+    cache's (default: as many as the bitmap's universe holds).  stream: None is the null stream."""
     n, on = d_kv_len.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
     sel, room, sel_stride = _table(d_sel, n, on)
@@ -691,7 +696,8 @@ def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_ou
 
     Request r's tokens are [starts[r], starts[r + 1]), the last of its kv_len[r] positions.  scale: 1 / sqrt(dim) by
     default.  d_lse: float32 [T, heads] or None.  selection: paged_select's (sel, sel_len, limits) or None.  max_new
-    and max_kv: the most new tokens and keys of a request if known; they choose how the work is split."""
+    and max_kv: the most new tokens and keys of a request if known; they choose how the work is split.  stream: None is
+    the null stream."""
     on = _device()
     cache, page_size, _, dim = _cache(d_k_cache, d_v_cache, on)
     dtype, shape = d_k_cache.dtype, d_q.shape
@@ -723,7 +729,8 @@ def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_ls
     """The k best continuations of each answer's beams (cr_beam_select): k is the outputs' second extent.
 
     d_scores: [B, W, V] with contiguous rows; d_cum, d_lse: float32 [B, W]; outputs: float32, int32, int32 [B, k].
-    allowed: a bitmap over [0, V), or int32 bitsets [ceil(V / 32)] (one for all) or [B, W, ceil(V / 32)], or None."""
+    allowed: a bitmap over [0, V), or int32 bitsets [ceil(V / 32)] (one for all) or [B, W, ceil(V / 32)], or None.
+    stream: None is the null stream."""
     b, w, v = d_scores.shape
     k = d_out_scores.shape[1]
     on = _device()
@@ -751,7 +758,7 @@ def beam_reorder(d_src, d_parents, d_dst, d_len=None, stream=None):
     """d_dst[b, i] = d_src[b, parents[b, i]] for states [B, W, ...] of any type (cr_beam_reorder).
 
     d_len: int32 [B, W]: only the first d_len[b, parent] entries along the third extent move.  Rows without a parent
-    (-1) are left alone."""
+    (-1) are left alone.  stream: None is the null stream."""
     b, w, *of_state = d_src.shape
     k = d_parents.shape[1]
     on = _device()
