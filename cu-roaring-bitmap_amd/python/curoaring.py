@@ -675,14 +675,14 @@ def paged_select(visible: GpuRoaring, d_table, d_starts, d_kv_len, page_size: in
     """The slots of each request that the bitmap `visible` holds, listed once for every layer's attention.
 
     Written: d_sel int32 [R, at least cols * page_size], d_sel_len int32 [R], d_limits int32 [T].  n_pages: the
-    cache's (default: as many as the bitmap's universe holds).  stream: None is the null stream."""
+    cache's (default: those that the bitmap's universe reaches into).  stream: None is the null stream."""
     n, on = d_kv_len.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
     sel, room, sel_stride = _table(d_sel, n, on)
     if room < cols * page_size:
         raise CrError(CR_ERR_INVALID, f"paged_select: a row of sel holds cols * page_size = {cols * page_size} slots")
     if n_pages is None:
-        n_pages = visible.universe_size // page_size
+        n_pages = -(-visible.universe_size // page_size)
     _check(load().cr_paged_select(C.byref(visible), n_pages, page_size, table, cols, stride,
                                   _array(d_starts, "starts", "int32", (n + 1,), on),
                                   _array(d_kv_len, "kv_len", "int32", (n,), on), n, d_limits.numel(), sel, sel_stride,

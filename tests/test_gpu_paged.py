@@ -391,3 +391,21 @@ def test_allocation_failure_is_reported(gpu):
     finally:
         lib.cr_debug_fail_device_allocs(0, 0)
     gpu.free(g)
+
+
+def test_select_with_a_universe_inside_a_page(gpu):
+    """Without n_pages, the page that the bitmap's universe ends in is one of them: what the set holds of it is listed."""
+    import torch
+    _say("select, universe inside a page")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for kind in ("bitmap", "stored"):
+        visible = np.ones(37, bool)
+        visible[[0, 33]] = False
+        g = _bitmap(gpu, visible, kind)
+        sel, length, limits = torch.full((1, 64), -5, **i32), torch.zeros(1, **i32), torch.zeros(1, **i32)
+        table = torch.tensor([[2, 0, 3, 1]], **i32)
+        gpu.paged_select(g, table, torch.tensor([0, 1], **i32), torch.tensor([64], **i32), 16, sel, length, limits)
+        torch.cuda.synchronize()
+        gpu.free(g)
+        want = [32, 34, 35, 36] + list(range(1, 32))
+        assert int(length) == int(limits) == len(want) and sel[0, :len(want)].tolist() == want
