@@ -309,6 +309,34 @@ static void release_block(const CachedBlock& b)
 // through, then the ones to fail.  Read under g_cache_mu.
 static uint32_t g_fail_skip = 0, g_fail_count = 0;
 
+// A call that is captured into a graph keeps its workspace for good: the graph names
+// its address and may be replayed at any time, beside whatever runs then.  Such
+// blocks are allocated past the pool, which a capture would record, never handed out
+// again, and marked by this in place of a device.
+constexpr int CAPTURED = -1;
+
+static bool is_capturing(hipStream_t s)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return s && hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusActive;
+}
+
+static int captured_alloc(void** p, size_t bytes)
+{
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    CR_HIP_RET(hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipMalloc(p, bytes);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) {
+        set_error("hipMalloc(%zu bytes) for a captured call failed: %s", bytes, hipGetErrorString(e));
+        *p = nullptr;
+        return e == hipErrorOutOfMemory ? CR_ERR_ALLOC : CR_ERR_HIP;
+    }
+    std::lock_guard<std::mutex> lock(g_cache_mu);
+    g_live[*p] = {bytes, CAPTURED};
+    return CR_OK;
+}
+
 int dev_alloc(void** p, size_t bytes, hipStream_t s)
 {
     CR_HOST_PHASE("alloc");
@@ -316,6 +344,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
     if (bytes == 0) bytes = 256;
     int dev = 0;
     CR_HIP_RET(hipGetDevice(&dev));
+    const bool capturing = is_capturing(s);
     {
         std::lock_guard<std::mutex> lock(g_cache_mu);
         if (g_fail_count) {
@@ -328,7 +357,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
             }
         }
         size_t best = g_cache.size();
-        for (size_t i = 0; i < g_cache.size(); ++i) {
+        for (size_t i = 0; !capturing && i < g_cache.size(); ++i) {
             const CachedBlock& b = g_cache[i];
             if (b.dev == dev && b.stream == s && b.bytes >= bytes && b.bytes <= 2 * bytes &&
                 (best == g_cache.size() || b.bytes < g_cache[best].bytes))
@@ -343,6 +372,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
             return CR_OK;
         }
     }
+    if (capturing) return captured_alloc(p, bytes);
     hipMemPool_t pool = library_pool();
     hipError_t e = pool ? hipMallocFromPoolAsync(p, bytes, pool, s) : hipMallocAsync(p, bytes, s);
     if (e != hipSuccess) {
@@ -365,6 +395,10 @@ int dev_free(void* p, hipStream_t s)
         auto it = g_live.find(p);
         if (it == g_live.end()) {  // not a library block
             CR_HIP_RET(hipFreeAsync(p, s));
+            return CR_OK;
+        }
+        if (it->second.second == CAPTURED) {
+            g_live.erase(it);
             return CR_OK;
         }
         g_cache.push_back({p, it->second.first, it->second.second, s});
