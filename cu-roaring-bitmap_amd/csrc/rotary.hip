@@ -1,0 +1,307 @@
+// Rotary positions, for serving language models (no reference implementation):
+// queries and keys turned by the angles of their positions, and keys and values
+// into their slots of the paged cache.
+//
+//   a = position * freq_i,  (x, y) -> m (x cos a - y sin a, y cos a + x sin a)
+//
+// for the pairs (x, y) of a row's first `rotated` dimensions: dimensions i and
+// i + rotated / 2, or 2 i and 2 i + 1.  The rest of a row stays as it is.
+#include <algorithm>
+
+#include "internal.hpp"
+#include "elements.hpp"
+#include "set_bits.hpp"
+
+namespace crimpl {
+
+namespace {
+
+constexpr int RO_NT = 256;
+constexpr uint32_t RO_PAIRS = 2048;  // cosines and sines that a workgroup keeps
+constexpr uint32_t RO_AHEAD = 2;     // pieces that a thread asks for at a time
+
+struct Plane {  // rows of one of the tensors; strides in elements
+    const void* src;
+    uint64_t src_token, src_head;
+    void* dst;
+    uint64_t dst_token, dst_head;  // queries
+};
+
+struct RotaryArgs {
+    Plane q, k, v;
+    uint64_t k_page, k_slot, k_head, v_page, v_slot, v_head;  // of the cache
+    uint32_t n_tokens, heads, kv_heads, dim, half, magnitude_bits;
+    const int32_t* positions;
+    const double* freqs;
+    const int64_t* slots;
+    uint64_t n_slots;
+    uint32_t page_lg;
+    uint32_t tokens;     // of a workgroup
+    uint32_t splits;     // workgroups that share them
+    uint32_t per_row, per_token;  // pieces' pairs
+};
+
+// Cosine and sine of position * freq, in 64 bits until whole turns are taken
+// away: a position of 2^20 at one radian each has 17 bits before the point, which
+// would leave 32 bits 2^-8 of a radian.  Within an eighth of a turn the first five terms
+// of either series are off by less than 2^-29.
+__device__ __forceinline__ float2 cos_sin(int32_t position, double freq, float m)
+{
+    const double turns = static_cast<double>(position) * (freq * 0.15915494309189533577);
+    const double part = turns - rint(turns), quarter = rint(part * 4.0);  // [-1/2, 1/2], [-2, 2]
+    const float x = static_cast<float>((part - quarter * 0.25) * 6.28318530717958647692), z = x * x;
+    float s = __builtin_fmaf(z, 2.7557319224e-6f, -1.9841269841e-4f);
+    s = __builtin_fmaf(z, s, 8.3333333333e-3f);
+    s = __builtin_fmaf(z, s, -1.6666666667e-1f);
+    s = __builtin_fmaf(z * x, s, x);
+    float c = __builtin_fmaf(z, -2.7557319224e-7f, 2.4801587302e-5f);
+    c = __builtin_fmaf(z, c, -1.3888888889e-3f);
+    c = __builtin_fmaf(z, c, 4.1666666667e-2f);
+    c = __builtin_fmaf(z, c, -0.5f);
+    c = __builtin_fmaf(z, c, 1.0f);
+    const int n = static_cast<int>(quarter) & 3;
+    const float cn = n & 1 ? s : c, sn = n & 1 ? c : s;
+    return make_float2((n == 1 || n == 2 ? -cn : cn) * m, (n >= 2 ? -sn : sn) * m);
+}
+
+// Bound by memory: a thread asks for the two pieces that turn together (or two
+// neighbours), and the next two, before the workgroup's cosines are there.
+template <class E, uint32_t N, bool NEXT>
+__global__ __launch_bounds__(RO_NT) void ro_turn(RotaryArgs a)
+{
+    typedef typename E::Bits Bits;
+    typedef Piece<E, N> P;
+    __shared__ float2 s_turn[RO_PAIRS];
+    const uint32_t t = threadIdx.x, token0 = blockIdx.x / a.splits * a.tokens, part = blockIdx.x % a.splits;
+    const uint32_t tokens = min(a.tokens, a.n_tokens - token0), items = tokens * a.per_token;
+    const uint32_t turned = NEXT ? a.half * 2 : a.half;  // dimensions whose pieces come in turned pairs
+    struct Item {
+        P x, y;
+        Bits* to;         // nullptr: nowhere
+        uint32_t at, two;  // the pieces' first dimensions
+        uint32_t token;
+        bool both, turn;
+    };
+    auto load = [&](uint32_t i) {
+        Item it;
+        const uint32_t local = i / a.per_token, in = i % a.per_token, row = in / a.per_row, c = in % a.per_row * N;
+        const uint32_t token = token0 + local;
+        it.token = local;
+        it.at = c;
+        it.two = c + a.half;
+        if (NEXT) {
+            it.at = 2 * c;
+            it.two = 2 * c + N;
+        } else if (c >= turned) {
+            it.at = 2 * a.half + 2 * (c - a.half);
+            it.two = it.at + N;
+        }
+        it.both = it.two < a.dim;
+        const bool query = row < a.heads, key = !query && row < a.heads + a.kv_heads;
+        const uint32_t head = query ? row : key ? row - a.heads : row - a.heads - a.kv_heads;
+        const Plane& p = query ? a.q : key ? a.k : a.v;
+        it.turn = query || key;
+        const Bits* from = static_cast<const Bits*>(p.src) + token * p.src_token + head * p.src_head;
+        Bits* to;
+        if (query) {
+            to = static_cast<Bits*>(p.dst) + token * p.dst_token + head * p.dst_head;
+        } else {
+            const int64_t slot = a.slots[token];
+            const uint64_t page = static_cast<uint64_t>(slot) >> a.page_lg, off = slot & ((1u << a.page_lg) - 1u);
+            to = static_cast<Bits*>(p.dst) + (key ? page * a.k_page + off * a.k_slot + head * a.k_head
+                                                  : page * a.v_page + off * a.v_slot + head * a.v_head);
+            if (slot < 0 || static_cast<uint64_t>(slot) >= a.n_slots) to = nullptr;
+        }
+        it.to = to;
+        it.x = P::load(from + it.at);
+        it.y = P::load(from + (it.both ? it.two : it.at));
+        return it;
+    };
+    auto finish = [&](Item it) {
+        const float2* turn = s_turn + it.token * a.half;
+        if (it.turn) {
+            if (NEXT) {
+                if constexpr (N == 1) {
+                    if (it.at < turned) {
+                        const float2 w = turn[it.at / 2];
+                        const float x = it.x.get(0), y = it.y.get(0);
+                        it.x.set(0, __builtin_fmaf(x, w.x, -(y * w.y)));
+                        it.y.set(0, __builtin_fmaf(y, w.x, x * w.y));
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e += 2) {
+                        if (it.at + e < turned) {
+                            const float2 w = turn[(it.at + e) / 2];
+                            const float x = it.x.get(e), y = it.x.get(e + 1);
+                            it.x.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
+                            it.x.set(e + 1, __builtin_fmaf(y, w.x, x * w.y));
+                        }
+                        if (it.two + e < turned) {
+                            const float2 w = turn[(it.two + e) / 2];
+                            const float x = it.y.get(e), y = it.y.get(e + 1);
+                            it.y.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
+                            it.y.set(e + 1, __builtin_fmaf(y, w.x, x * w.y));
+                        }
+                    }
+                }
+            } else if (it.at < turned) {
+#pragma unroll
+                for (uint32_t e = 0; e < N; ++e) {
+                    const float2 w = turn[it.at + e];
+                    const float x = it.x.get(e), y = it.y.get(e);
+                    it.x.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
+                    it.y.set(e, __builtin_fmaf(y, w.x, x * w.y));
+                }
+            }
+        }
+        if (it.to) {
+            it.x.store(it.to + it.at);
+            if (it.both) it.y.store(it.to + it.two);
+        }
+    };
+    const uint32_t step = RO_NT * a.splits;
+    uint32_t i = part * RO_NT + t;
+    Item it[RO_AHEAD];
+#pragma unroll
+    for (uint32_t j = 0; j < RO_AHEAD; ++j)
+        if (i + j * step < items) it[j] = load(i + j * step);
+    const float m = __uint_as_float(a.magnitude_bits);
+    for (uint32_t k = t; k < tokens * a.half; k += RO_NT)
+        s_turn[k] = cos_sin(a.positions[token0 + k / a.half], a.freqs[k % a.half], m);
+    __syncthreads();
+    while (i < items) {
+#pragma unroll
+        for (uint32_t j = 0; j < RO_AHEAD; ++j)
+            if (i + j * step < items) finish(it[j]);
+        i += RO_AHEAD * step;
+#pragma unroll
+        for (uint32_t j = 0; j < RO_AHEAD; ++j)
+            if (i + j * step < items) it[j] = load(i + j * step);
+    }
+}
+
+template <class E, uint32_t N>
+void launch_rotary(const RotaryArgs& a, bool next, uint32_t grid, hipStream_t s)
+{
+    if (next)
+        ro_turn<E, N, true><<<grid, RO_NT, 0, s>>>(a);
+    else
+        ro_turn<E, N, false><<<grid, RO_NT, 0, s>>>(a);
+}
+
+}  // namespace
+
+}  // namespace crimpl
+
+using namespace crimpl;
+
+extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_cache* cache, cr_stream_t stream)
+{
+    if (!args || !cache) {
+        set_error("cr_paged_rotary: invalid argument");
+        return CR_ERR_INVALID;
+    }
+    const cr_paged_rotary_args& p = *args;
+    if (p.n_tokens == 0) return CR_OK;
+    const uint32_t dim = cache->head_dim;
+    if (!p.k || !p.v || !p.d_slots || !cache->k || !cache->v || !power_of_two(cache->page_size) ||
+        cache->dtype > CR_BF16 || (p.n_heads && (!p.q || !p.q_out)) || dim == 0 || p.rotated % 2 || p.rotated > dim ||
+        (p.rotated && (!p.d_positions || !p.d_freqs))) {
+        set_error("cr_paged_rotary: invalid argument (%u of %u dimensions, page size %u)", p.rotated, dim,
+                  cache->page_size);
+        return CR_ERR_INVALID;
+    }
+    if (p.rotated / 2 > RO_PAIRS) {
+        set_error("cr_paged_rotary: up to %u dimensions are turned (%u)", 2 * RO_PAIRS, p.rotated);
+        return CR_ERR_UNSUPPORTED;
+    }
+    const uint32_t es = cache->dtype == CR_F32 ? 4 : 2;
+    RotaryArgs a{};
+    a.q = {p.q, p.q_token_stride, p.q_head_stride, p.q_out, p.out_token_stride, p.out_head_stride};
+    a.k = {p.k, p.k_token_stride, p.k_head_stride, cache->k, 0, 0};
+    a.v = {p.v, p.v_token_stride, p.v_head_stride, cache->v, 0, 0};
+    a.k_page = cache->k_page_stride;
+    a.k_slot = cache->k_slot_stride;
+    a.k_head = cache->k_head_stride;
+    a.v_page = cache->v_page_stride;
+    a.v_slot = cache->v_slot_stride;
+    a.v_head = cache->v_head_stride;
+    a.n_tokens = p.n_tokens;
+    a.heads = p.n_heads;
+    a.kv_heads = cache->n_heads;
+    a.dim = dim;
+    a.half = p.rotated / 2;
+    a.magnitude_bits = __builtin_bit_cast(uint32_t, p.magnitude);
+    a.positions = p.d_positions;
+    a.freqs = p.d_freqs;
+    a.slots = p.d_slots;
+    a.n_slots = static_cast<uint64_t>(cache->n_pages) * cache->page_size;
+    a.page_lg = static_cast<uint32_t>(__builtin_ctz(cache->page_size));
+    // Pieces of 16 bytes, of 8, or single values: what every row's pieces are aligned
+    // to, and what does not reach over the end of the turned dimensions.
+    auto over = [](uint32_t extent, uint64_t x, uint64_t y) { return extent > 1 ? x | y : 0; };
+    uint64_t all = over(p.n_tokens, p.k_token_stride, p.v_token_stride) |
+                   over(cache->n_heads, p.k_head_stride, p.v_head_stride) |
+                   over(cache->n_pages, a.k_page, a.v_page) | over(cache->page_size, a.k_slot, a.v_slot) |
+                   over(cache->n_heads, a.k_head, a.v_head) | dim;
+    uintptr_t at = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                   reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v);
+    if (p.n_heads) {
+        all |= over(p.n_tokens, p.q_token_stride, p.out_token_stride) | over(p.n_heads, p.q_head_stride, p.out_head_stride);
+        at |= reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.q_out);
+    }
+    if (!p.interleaved) all |= a.half;
+    const uint64_t bytes = all * es | at;
+    const uint32_t n = bytes % 16 == 0 ? 16 / es : bytes % 8 == 0 ? 8 / es : 1;
+    a.per_row = (dim + 2 * n - 1) / (2 * n);
+    const uint64_t per_token = (static_cast<uint64_t>(p.n_heads) + 2ull * cache->n_heads) * a.per_row;
+    if (per_token >> 24 || p.n_tokens >> 31) {
+        set_error("cr_paged_rotary: too many elements for one call");
+        return CR_ERR_UNSUPPORTED;
+    }
+    if (per_token == 0) return CR_OK;
+    a.per_token = static_cast<uint32_t>(per_token);
+    // A workgroup's cosines serve all heads of its tokens.  Enough tokens for two
+    // rounds of pieces where there are many; where there are few, several workgroups
+    // share a token.
+    const uint32_t fit = a.half ? RO_PAIRS / a.half : 64;
+    const uint32_t want = std::max<uint32_t>(1, (RO_AHEAD * RO_NT + a.per_token - 1) / a.per_token);
+    a.tokens = std::min({want, fit, std::max<uint32_t>(1, p.n_tokens / num_cus())});
+    const uint32_t groups = (p.n_tokens + a.tokens - 1) / a.tokens;
+    const uint32_t rounds = (a.tokens * a.per_token + RO_NT - 1) / RO_NT;
+    a.splits = std::max<uint32_t>(1, std::min(rounds, num_cus() / groups));
+    const uint64_t grid = static_cast<uint64_t>(groups) * a.splits;
+    if (grid >> 23) {  // a launch holds fewer than 2^32 threads
+        set_error("cr_paged_rotary: too many tokens for one call");
+        return CR_ERR_UNSUPPORTED;
+    }
+    hipStream_t s = as_stream(stream);
+    CR_TIMED("ro_turn", s);
+    const uint32_t g = static_cast<uint32_t>(grid);
+    const bool next = p.interleaved != 0;
+    if (cache->dtype == CR_F32) {
+        if (n == 4)
+            launch_rotary<F32, 4>(a, next, g, s);
+        else if (n == 2)
+            launch_rotary<F32, 2>(a, next, g, s);
+        else
+            launch_rotary<F32, 1>(a, next, g, s);
+    } else if (cache->dtype == CR_F16) {
+        if (n == 8)
+            launch_rotary<F16, 8>(a, next, g, s);
+        else if (n == 4)
+            launch_rotary<F16, 4>(a, next, g, s);
+        else
+            launch_rotary<F16, 1>(a, next, g, s);
+    } else {
+        if (n == 8)
+            launch_rotary<BF16, 8>(a, next, g, s);
+        else if (n == 4)
+            launch_rotary<BF16, 4>(a, next, g, s);
+        else
+            launch_rotary<BF16, 1>(a, next, g, s);
+    }
+    CR_LAUNCH_CHECK();
+    return CR_OK;
+}

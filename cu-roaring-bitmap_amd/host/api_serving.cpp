@@ -42,6 +42,33 @@ void paged_attention(const PagedAttentionArgs& args, const PagedCache& cache, hi
     throw_on_error(cr_paged_attention(&args, &cache, S(stream)), "paged_attention");
 }
 
+void paged_rotary(const PagedRotaryArgs& args, const PagedCache& cache, hipStream_t stream)
+{
+    throw_on_error(cr_paged_rotary(&args, &cache, S(stream)), "paged_rotary");
+}
+
+void paged_weights(const PagedWeightsArgs& args, const PagedCache& cache, hipStream_t stream)
+{
+    throw_on_error(cr_paged_weights(&args, &cache, S(stream)), "paged_weights");
+}
+
+void paged_evict(const PagedEvictArgs& args, hipStream_t stream)
+{
+    throw_on_error(cr_paged_evict(&args, S(stream)), "paged_evict");
+}
+
+void paged_move(const int32_t* d_moves, uint32_t moves_cap, uint64_t moves_stride, const int32_t* d_n_moves,
+                uint32_t n_requests, const PagedCache& cache, hipStream_t stream)
+{
+    throw_on_error(cr_paged_move(d_moves, moves_cap, moves_stride, d_n_moves, n_requests, &cache, S(stream)),
+                   "paged_move");
+}
+
+void draft_verify(const DraftVerifyArgs& args, hipStream_t stream)
+{
+    throw_on_error(cr_draft_verify(&args, S(stream)), "draft_verify");
+}
+
 void beam_select(const void* d_scores, uint32_t dtype, uint32_t batch, uint32_t beams, uint32_t vocab,
                  uint64_t batch_stride, uint64_t beam_stride, const float* d_cum, const float* d_lse,
                  const GpuRoaring* allowed, const uint32_t* d_allowed_bits, uint64_t bits_stride, uint32_t k,

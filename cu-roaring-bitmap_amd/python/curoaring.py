@@ -40,7 +40,8 @@ EXPORTS = [
     "cr_portable_size_in_bytes", "cr_portable_serialize", "cr_portable_deserialize",
     "cr_upload_batch", "cr_free_batch", "cr_promote_batch", "cr_batch_make_view", "cr_batch_multi_and",
     "cr_batch_decompress", "cr_batch_contains", "cr_batch_view_contains", "cr_debug_fail_device_allocs",
-    "cr_paged_plan", "cr_paged_append", "cr_paged_select", "cr_paged_attention", "cr_beam_select", "cr_beam_reorder",
+    "cr_paged_plan", "cr_paged_append", "cr_paged_select", "cr_paged_attention", "cr_paged_rotary", "cr_paged_weights", "cr_paged_evict", "cr_paged_move",
+    "cr_draft_verify", "cr_beam_select", "cr_beam_reorder",
 ]
 
 
@@ -140,6 +141,51 @@ class PagedAttentionArgs(C.Structure):
                 ("scale", C.c_float), ("causal", C.c_uint32), ("max_new", C.c_uint32), ("max_kv", C.c_uint32)]
 
 
+class PagedRotaryArgs(C.Structure):
+    """cr_paged_rotary_args (include/cu_roaring_abi.h)."""
+    _fields_ = [("q", C.c_void_p), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+                ("q_out", C.c_void_p), ("out_token_stride", C.c_uint64), ("out_head_stride", C.c_uint64),
+                ("k", C.c_void_p), ("k_token_stride", C.c_uint64), ("k_head_stride", C.c_uint64),
+                ("v", C.c_void_p), ("v_token_stride", C.c_uint64), ("v_head_stride", C.c_uint64),
+                ("d_positions", C.c_void_p), ("d_freqs", C.c_void_p), ("d_slots", C.c_void_p),
+                ("n_tokens", C.c_uint32), ("n_heads", C.c_uint32), ("rotated", C.c_uint32),
+                ("interleaved", C.c_uint32), ("magnitude", C.c_float)]
+
+
+class PagedWeightsArgs(C.Structure):
+    """cr_paged_weights_args (include/cu_roaring_abi.h)."""
+    _fields_ = [("q", C.c_void_p), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("lse", C.c_void_p),
+                ("n_tokens", C.c_uint32), ("n_heads", C.c_uint32), ("n_requests", C.c_uint32),
+                ("d_starts", C.c_void_p), ("d_new", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_table", C.c_void_p),
+                ("table_cols", C.c_uint32), ("table_stride", C.c_uint64), ("visible", C.c_void_p),
+                ("d_past", C.c_void_p), ("past_stride", C.c_uint64), ("d_out", C.c_void_p), ("out_stride", C.c_uint64),
+                ("scale", C.c_float), ("decay", C.c_float), ("causal", C.c_uint32), ("continued", C.c_uint32),
+                ("max_new", C.c_uint32), ("max_kv", C.c_uint32)]
+
+
+class PagedEvictArgs(C.Structure):
+    """cr_paged_evict_args (include/cu_roaring_abi.h)."""
+    _fields_ = [("d_weights", C.c_void_p), ("weights_stride", C.c_uint64), ("d_positions", C.c_void_p),
+                ("positions_stride", C.c_uint64), ("d_kept", C.c_void_p), ("d_seen", C.c_void_p),
+                ("d_kv_len", C.c_void_p), ("d_keep", C.c_void_p), ("d_table", C.c_void_p), ("table_cols", C.c_uint32),
+                ("table_stride", C.c_uint64), ("page_size", C.c_uint32), ("n_pages", C.c_uint32),
+                ("n_requests", C.c_uint32), ("sinks", C.c_uint32), ("recent", C.c_uint32), ("pinned", C.c_void_p),
+                ("d_weights_out", C.c_void_p), ("weights_out_stride", C.c_uint64), ("d_positions_out", C.c_void_p),
+                ("positions_out_stride", C.c_uint64), ("d_len", C.c_void_p), ("d_moves", C.c_void_p),
+                ("moves_cap", C.c_uint32), ("moves_stride", C.c_uint64), ("d_n_moves", C.c_void_p),
+                ("d_freed", C.c_void_p), ("freed_cap", C.c_uint32), ("d_counts", C.c_void_p)]
+
+
+class DraftVerifyArgs(C.Structure):
+    """cr_draft_verify_args (include/cu_roaring_abi.h)."""
+    _fields_ = [("d_scores", C.c_void_p), ("row_stride", C.c_uint64), ("d_draft", C.c_void_p),
+                ("draft_row_stride", C.c_uint64), ("dtype", C.c_uint32), ("n_rows", C.c_uint32),
+                ("n_requests", C.c_uint32), ("vocab", C.c_uint32), ("d_tokens", C.c_void_p), ("d_starts", C.c_void_p),
+                ("d_uniform", C.c_void_p), ("allowed", C.c_void_p), ("d_allowed_bits", C.c_void_p),
+                ("bits_stride", C.c_uint64), ("temperature", C.c_float), ("d_accepted", C.c_void_p),
+                ("d_out", C.c_void_p), ("out_cols", C.c_uint32), ("out_stride", C.c_uint64)]
+
+
 assert C.sizeof(GpuRoaring) == 120 and C.sizeof(GpuRoaringView) == 80
 
 _lib = None
@@ -220,6 +266,11 @@ def load(path: Optional[str] = None):
                             C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
                             C.c_void_p],
         "cr_paged_attention": [C.c_void_p, C.c_void_p, C.c_void_p],
+        "cr_paged_rotary": [C.c_void_p, C.c_void_p, C.c_void_p],
+        "cr_paged_weights": [C.c_void_p, C.c_void_p, C.c_void_p],
+        "cr_paged_evict": [C.c_void_p, C.c_void_p],
+        "cr_paged_move": [C.c_void_p, C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p],
+        "cr_draft_verify": [C.c_void_p, C.c_void_p],
         "cr_beam_select": [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64,
                            C.c_void_p, C.c_void_p, P(GpuRoaring), C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
                            C.c_void_p, C.c_void_p, C.c_void_p],
@@ -552,7 +603,13 @@ _names, _codes = {}, {}
 # The structs as the calls pass them: packed bytes cost a third of a filled ctypes structure.
 _CACHE = struct.Struct("@PPQQQQQQIIIII4x")
 _ATTENTION = struct.Struct("@PQQPQQPIIIPPPIQPQPPfIII")
+_ROTARY = struct.Struct("@PQQPQQPQQPQQPPPIIIIf4x")
+_WEIGHTS = struct.Struct("@PQQPIIIPPPPIQPPQPQffIIII")
+_EVICT = struct.Struct("@PQPQPPPPPIQIIIIIPPQPQPPIQPPIP")
+_VERIFY = struct.Struct("@PQPQIIIIPPPPPQfPPIQ")
 assert _CACHE.size == C.sizeof(PagedCache) and _ATTENTION.size == C.sizeof(PagedAttentionArgs)
+assert _ROTARY.size == C.sizeof(PagedRotaryArgs) and _WEIGHTS.size == C.sizeof(PagedWeightsArgs)
+assert _EVICT.size == C.sizeof(PagedEvictArgs) and _VERIFY.size == C.sizeof(DraftVerifyArgs)
 
 
 _devices = None
@@ -607,6 +664,18 @@ def _table(t, n_requests: int, device: int):
             return t.data_ptr(), cols, stride
     raise CrError(CR_ERR_INVALID, f"block table: an int32 tensor of {n_requests} rows on the current CUDA device is "
                                   f"taken, not {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _matrix(t, name: str, dtype: str, n_rows: int, cols: int, device: int):
+    """(address, row stride) of a tensor of n_rows rows of at least `cols` values, which may lie apart."""
+    if (_names.get(t.dtype) or _type_name(t)) == dtype and t.get_device() == device and t.dim() == 2:
+        (rows, held), (stride, one) = t.shape, t.stride()
+        if rows <= 1:  # whose stride may be any number
+            stride = held
+        if rows == n_rows and held >= cols and (one == 1 or held <= 1) and stride >= held:
+            return t.data_ptr(), stride
+    raise CrError(CR_ERR_INVALID, f"{name}: a {dtype} tensor of {n_rows} rows of at least {cols} values on the current "
+                                  f"CUDA device is taken, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _rows(t, name: str, dtype, shape, device: int):
@@ -723,6 +792,186 @@ def paged_attention(d_q, d_k_cache, d_v_cache, d_table, d_starts, d_kv_len, d_ou
                         _array(d_kv_len, "kv_len", "int32", (n,), on), table, cols, stride, sel, sel_stride, sel_len,
                         limits, dim ** -0.5 if scale is None else scale, causal, max_new, max_kv)
     _check(load().cr_paged_attention(a, cache, _stream(stream)), "paged_attention")
+
+
+def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original: int = 4096, fast: float = 32.0, slow: float = 1.0, device="cuda"):
+    """(freqs, magnitude) of paged_rotary for `rotated` dimensions: base^(-2 i / rotated) radians a position.
+
+    scaling, for contexts `factor` times as long: "linear" divides every frequency by it; "base" raises the base, so
+    that the slowest pair is divided by it and the fastest stays; "parts" leaves the pairs that turn more than `fast`
+    times over the `original` positions, divides those that turn fewer than `slow` times, passes over evenly between
+    them, and lengthens the rows by a tenth of the factor's logarithm.  Worked out in 64 bits."""
+    import torch
+    if rotated < 0 or rotated % 2 or base <= 0 or factor <= 0 or scaling not in (None, "linear", "base", "parts"):
+        raise CrError(CR_ERR_INVALID, f"rotary_frequencies: {rotated} dimensions, base {base}, scaling {scaling!r} by "
+                                      f"{factor}")
+    if scaling == "base" and rotated > 2:
+        base = base * factor ** (rotated / (rotated - 2))
+    freqs = base ** (-torch.arange(0, rotated, 2, dtype=torch.float64) / max(1, rotated))
+    magnitude = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "parts":
+        turns = original * freqs / (2 * np.pi)
+        stays = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        freqs = freqs * (stays + (1 - stays) / factor)
+        magnitude = max(1.0, 1.0 + 0.1 * float(np.log(factor)))
+    return freqs.to(device), magnitude
+
+
+def paged_rotary(d_k, d_v, d_positions, d_freqs, d_slots, d_k_cache, d_v_cache, d_q=None, d_q_out=None,
+                 interleaved: bool = False, magnitude: float = 1.0, stream=None):
+    """paged_append with keys, and queries d_q [T, heads, dim] into d_q_out, turned by their positions
+    (cr_paged_rotary).
+
+    d_positions: int32 [T].  d_freqs: float64 [rotated / 2], radians a position (rotary_frequencies makes them); the
+    rows' first `rotated` dimensions are turned, in halves or, interleaved, in neighbouring pairs.  d_q_out: d_q itself
+    by default.  stream: None is the null stream."""
+    on = _device()
+    cache, _, heads, dim = _cache(d_k_cache, d_v_cache, on)
+    n, dtype = d_slots.numel(), d_k_cache.dtype
+    q = q_token = q_head = out = out_token = out_head = n_heads = 0
+    if d_q is not None:
+        n_heads = d_q.shape[1] if d_q.dim() == 3 else 0
+        q, q_token, q_head = _rows(d_q, "q", dtype, (n, n_heads, dim), on)
+        out, out_token, out_head = (q, q_token, q_head) if d_q_out is None else _rows(d_q_out, "q_out", dtype,
+                                                                                      (n, n_heads, dim), on)
+    elif d_q_out is not None:
+        raise CrError(CR_ERR_INVALID, "paged_rotary: q_out without q")
+    shape = (n, heads, dim)
+    k, k_token, k_head = _rows(d_k, "k", dtype, shape, on)
+    v, v_token, v_head = _rows(d_v, "v", dtype, shape, on)
+    a = _ROTARY.pack(q, q_token, q_head, out, out_token, out_head, k, k_token, k_head, v, v_token, v_head,
+                     _array(d_positions, "positions", "int32", (n,), on), _array(d_freqs, "freqs", "float64", 0, on),
+                     _array(d_slots, "slots", "int64", (n,), on), n, n_heads, 2 * d_freqs.numel(), interleaved, magnitude)
+    _check(load().cr_paged_rotary(a, cache, _stream(stream)), "paged_rotary")
+
+
+def paged_weights(d_q, d_k_cache, d_table, d_starts, d_kv_len, d_lse, d_out, d_past=None, decay: float = 1.0, d_new=None,
+                  scale: Optional[float] = None, causal: bool = True, visible: Optional[GpuRoaring] = None,
+                  continued: bool = False, max_new: int = 0, max_kv: int = 0, stream=None):
+    """The attention weight that each cached token got from the rows q [T, heads, dim] (cr_paged_weights), summed over
+    heads into d_out float32 [R, at least cols * page_size].
+
+    d_lse: float32 [T, heads], what paged_attention left for the same rows and scale.  d_past (d_out itself, if need
+    be): what the tokens older than these rows had, times decay; continued: what all had, as between the layers of a
+    step whose weights are summed.  Rows of request r: [starts[r], starts[r + 1]), or
+    new[r] of them from starts[r] where d_new int32 [R] is given (d_starts then has R or R + 1 entries): the last of its
+    kv_len[r] positions.  visible: a bitmap of slots.  max_new and max_kv: the most rows and positions of a request if
+    known; they choose how the work is split.  stream: None is the null stream."""
+    on = _device()
+    shape, (pages, page_size, kv_heads, dim) = d_q.shape, d_k_cache.shape
+    if len(shape) != 3 or shape[2] != dim or d_q.dtype != d_k_cache.dtype:
+        raise CrError(CR_ERR_INVALID, f"paged_weights: {d_k_cache.dtype} queries [tokens, heads, {dim}] are taken, not "
+                                      f"{d_q.dtype} {tuple(shape)}")
+    kp, ks, kh, one = d_k_cache.stride()
+    if d_k_cache.get_device() != on or (one != 1 and dim > 1):
+        raise CrError(CR_ERR_INVALID, "paged_weights: keys [pages, page size, heads, dim] with contiguous rows on the "
+                                      "current CUDA device are taken")
+    cache = _CACHE.pack(d_k_cache.data_ptr(), 0, kp, ks, kh, 0, 0, 0, pages, page_size, kv_heads, dim, _typed(d_k_cache))
+    n, (tokens, heads, _) = d_kv_len.numel(), shape
+    q, q_token, q_head = _rows(d_q, "q", d_q.dtype, shape, on)
+    table, cols, stride = _table(d_table, n, on)
+    out, out_stride = _matrix(d_out, "out", "float32", n, cols * page_size, on)
+    past, past_stride = (0, 0) if d_past is None else _matrix(d_past, "past", "float32", n, cols * page_size, on)
+    new = 0 if d_new is None else _array(d_new, "new", "int32", (n,), on)
+    entries = n if d_new is not None and d_starts.numel() == n else n + 1
+    if not (0 <= max_new < 1 << 32 and 0 <= max_kv < 1 << 32):
+        raise CrError(CR_ERR_INVALID, f"paged_weights: max_new {max_new}, max_kv {max_kv}")
+    a = _WEIGHTS.pack(q, q_token, q_head, _array(d_lse, "lse", "float32", (tokens, heads), on), tokens, heads, n,
+                      _array(d_starts, "starts", "int32", (entries,), on), new,
+                      _array(d_kv_len, "kv_len", "int32", (n,), on), table, cols, stride,
+                      C.addressof(visible) if visible is not None else 0, past, past_stride, out, out_stride,
+                      dim ** -0.5 if scale is None else scale, decay, causal, continued, max_new, max_kv)
+    _check(load().cr_paged_weights(a, cache, _stream(stream)), "paged_weights")
+
+
+def paged_evict(d_weights, d_kv_len, d_keep, d_table, page_size: int, d_weights_out, d_len, d_moves, d_n_moves, d_freed,
+                d_counts, d_positions=None, d_kept=None, d_seen=None, d_positions_out=None, sinks: int = 0,
+                recent: int = 0, pinned: Optional[GpuRoaring] = None, n_pages: Optional[int] = None, stream=None):
+    """Which tokens of each request stay in the cache, by their weights (cr_paged_evict); paged_move then moves them.
+
+    d_weights float32 [R, at least cols * page_size]; d_kv_len, d_keep int32 [R]: how many there are, and how many may
+    stay.  Always safe are the first `sinks` and last `recent` of the d_seen int32 [R] tokens that a request has had
+    (kv_len if not given), and slots in the bitmap `pinned`.  d_positions int32 [R, ...]: the positions of the first
+    d_kept[r] entries, as the last call left them; the others are the newest in order.  Written: d_weights_out and
+    d_positions_out (the inputs themselves, if need be), d_len int32 [R], d_moves int32 [R, at least half of
+    cols * page_size, 2], d_n_moves int32 [R], d_freed int32 [any], d_counts int32 [2]: pages freed and moves in all.
+    n_pages: the cache's (default: those that pinned's universe reaches into, or any).  stream: None is the null
+    stream."""
+    n, on = d_kv_len.numel(), _device()
+    table, cols, stride = _table(d_table, n, on)
+    room = cols * page_size
+    weights, weights_stride = _matrix(d_weights, "weights", "float32", n, room, on)
+    w_out, w_out_stride = _matrix(d_weights_out, "weights_out", "float32", n, room, on)
+    positions, positions_stride = (0, 0) if d_positions is None else _matrix(d_positions, "positions", "int32", n, room, on)
+    p_out, p_out_stride = (0, 0) if d_positions_out is None else _matrix(d_positions_out, "positions_out", "int32", n,
+                                                                         room, on)
+    if d_moves.dim() != 3:
+        raise CrError(CR_ERR_INVALID, f"paged_evict: moves [{n}, at least {room // 2}, 2] are taken")
+    cap = d_moves.shape[1]
+    if n_pages is None:
+        n_pages = ((1 << 31) - 1) // page_size if pinned is None else -(-pinned.universe_size // page_size)
+    if not (0 <= sinks < 1 << 32 and 0 <= recent < 1 << 32):
+        raise CrError(CR_ERR_INVALID, f"paged_evict: sinks {sinks}, recent {recent}")
+    a = _EVICT.pack(weights, weights_stride, positions, positions_stride,
+                    0 if d_kept is None else _array(d_kept, "kept", "int32", (n,), on),
+                    0 if d_seen is None else _array(d_seen, "seen", "int32", (n,), on),
+                    _array(d_kv_len, "kv_len", "int32", (n,), on), _array(d_keep, "keep", "int32", (n,), on), table, cols,
+                    stride, page_size, n_pages, n, sinks, recent, C.addressof(pinned) if pinned is not None else 0, w_out,
+                    w_out_stride, p_out, p_out_stride, _array(d_len, "len", "int32", (n,), on),
+                    _array(d_moves, "moves", "int32", (n, cap, 2), on), cap, cap,
+                    _array(d_n_moves, "n_moves", "int32", (n,), on), _array(d_freed, "freed", "int32", 0, on),
+                    d_freed.numel(), _array(d_counts, "counts", "int32", (2,), on))
+    _check(load().cr_paged_evict(a, _stream(stream)), "paged_evict")
+
+
+def paged_move(d_moves, d_n_moves, d_k_cache, d_v_cache, stream=None):
+    """Keys and values from slot to slot (cr_paged_move): paged_evict's moves int32 [R, any, 2] and n_moves int32 [R],
+    once for each layer's cache.  stream: None is the null stream."""
+    on = _device()
+    cache = _cache(d_k_cache, d_v_cache, on)[0]
+    n = d_n_moves.numel()
+    cap = d_moves.shape[1] if d_moves.dim() == 3 else 0
+    _check(load().cr_paged_move(_array(d_moves, "moves", "int32", (n, cap, 2), on), cap, cap,
+                                _array(d_n_moves, "n_moves", "int32", (n,), on), n, cache, _stream(stream)), "paged_move")
+
+
+def draft_verify(d_scores, d_tokens, d_starts, d_uniform, d_accepted, d_out, d_draft=None, temperature: float = 1.0,
+                 allowed=None, stream=None):
+    """Drafted tokens against the model's own probabilities, and the token behind the accepted ones (cr_draft_verify).
+
+    d_scores [T, V] and d_draft (or None: looked-up drafts, without probabilities) of one type with contiguous rows: what
+    the two models say after each of the step's tokens d_tokens int32 [T], of which request r's are [starts[r],
+    starts[r + 1]) and those behind the first are its drafts.  d_uniform: float32 [T] in [0, 1).  Written: d_accepted
+    int32 [R], d_out int32 [R, any]: the accepted drafts, one token more, then -1.  allowed: a bitmap over [0, V), or
+    int32 bitsets [ceil(V / 32)] (one for all) or [T, ceil(V / 32)], or None.  stream: None is the null stream."""
+    on = _device()
+    if d_scores.dim() != 2 or d_scores.get_device() != on or (
+            d_scores.numel() and d_scores.shape[1] > 1 and d_scores.stride(1) != 1):
+        raise CrError(CR_ERR_INVALID, "draft_verify: scores [tokens, vocab] with contiguous rows on the current CUDA "
+                                      f"device are taken, not {tuple(d_scores.shape)} on {d_scores.device}")
+    rows, vocab = d_scores.shape
+    draft = draft_stride = 0
+    if d_draft is not None:
+        if d_draft.dtype != d_scores.dtype or d_draft.shape != d_scores.shape or d_draft.get_device() != on or (
+                rows and vocab > 1 and d_draft.stride(1) != 1):
+            raise CrError(CR_ERR_INVALID, f"draft_verify: {d_scores.dtype} draft scores of shape {tuple(d_scores.shape)} "
+                                          "with contiguous rows on the current CUDA device are taken")
+        draft, draft_stride = d_draft.data_ptr(), d_draft.stride(0)
+    n, words, bitmap, bits, bits_stride = d_accepted.numel(), (vocab + 31) // 32, 0, 0, 0
+    if isinstance(allowed, GpuRoaring):
+        bitmap = C.addressof(allowed)
+    elif allowed is not None:
+        bits = _array(allowed, "allowed", "int32", (words,) if allowed.dim() == 1 else (rows, words), on)
+        bits_stride = 0 if allowed.dim() == 1 else words
+    out, out_stride = _matrix(d_out, "out", "int32", n, 0, on)
+    a = _VERIFY.pack(d_scores.data_ptr(), d_scores.stride(0), draft, draft_stride, _typed(d_scores), rows, n, vocab,
+                     _array(d_tokens, "tokens", "int32", (rows,), on), _array(d_starts, "starts", "int32", (n + 1,), on),
+                     _array(d_uniform, "uniform", "float32", (rows,), on), bitmap, bits, bits_stride, temperature,
+                     _array(d_accepted, "accepted", "int32", (n,), on), out, d_out.shape[1], out_stride)
+    _check(load().cr_draft_verify(a, _stream(stream)), "draft_verify")
 
 
 def beam_select(d_scores, d_cum, d_out_scores, d_out_tokens, d_out_parents, d_lse=None, allowed=None, stream=None):

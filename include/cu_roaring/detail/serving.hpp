@@ -12,6 +12,11 @@ namespace cu_roaring {
 // Keys and values of a paged cache, and the arguments of its attention.
 using PagedCache = ::cr_paged_cache;
 using PagedAttentionArgs = ::cr_paged_attention_args;
+// The arguments of the calls for long and speculative answers.
+using PagedRotaryArgs = ::cr_paged_rotary_args;
+using PagedWeightsArgs = ::cr_paged_weights_args;
+using PagedEvictArgs = ::cr_paged_evict_args;
+using DraftVerifyArgs = ::cr_draft_verify_args;
 
 // Block tables and slot maps from the requests' lengths; the pages come from the
 // bitmap of free ones.
@@ -33,6 +38,23 @@ void paged_select(const GpuRoaring& visible, uint32_t n_pages, uint32_t page_siz
 
 // Attention of the requests' new tokens over the cache.
 void paged_attention(const PagedAttentionArgs& args, const PagedCache& cache, hipStream_t stream = 0);
+
+// New keys and values into their slots, keys and queries turned by their positions.
+void paged_rotary(const PagedRotaryArgs& args, const PagedCache& cache, hipStream_t stream = 0);
+
+// The attention weights that the cached tokens got from the new ones.
+void paged_weights(const PagedWeightsArgs& args, const PagedCache& cache, hipStream_t stream = 0);
+
+// Which tokens of each request stay, and the moves that close the holes.
+void paged_evict(const PagedEvictArgs& args, hipStream_t stream = 0);
+
+// Keys and values from slot to slot.
+void paged_move(const int32_t* d_moves, uint32_t moves_cap, uint64_t moves_stride, const int32_t* d_n_moves,
+                uint32_t n_requests, const PagedCache& cache, hipStream_t stream = 0);
+
+// Drafted tokens against the model's probabilities, and the token behind the
+// accepted ones.
+void draft_verify(const DraftVerifyArgs& args, hipStream_t stream = 0);
 
 // The k best continuations of each answer's beams; `allowed` (nullptr: every
 // token) or d_allowed_bits say which tokens may follow.

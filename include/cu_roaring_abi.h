@@ -466,6 +466,124 @@ typedef struct cr_paged_attention_args {
 } cr_paged_attention_args;
 int cr_paged_attention(const cr_paged_attention_args* args, const cr_paged_cache* cache, cr_stream_t stream);
 
+/* New keys and values into their slots as cr_paged_append, keys and queries turned
+ * by the angles of their positions on the way: of a row's first `rotated`
+ * dimensions (an even number), pair i (dimensions i and i + rotated / 2, or 2 i and
+ * 2 i + 1 where `interleaved`) is turned by d_positions[token] * d_freqs[i] and
+ * multiplied by `magnitude`; the rest of the row, and the values, stay as they are.
+ * Angles are worked out in 64 bits, products in fp32 and rounded once.  q_out may be
+ * q.  n_heads 0: keys and values alone.  A token whose slot is outside the cache (-1)
+ * gets its queries turned. */
+typedef struct cr_paged_rotary_args {
+    const void* q; /* [n_tokens][n_heads][cache->head_dim] */
+    uint64_t q_token_stride, q_head_stride;
+    void* q_out;
+    uint64_t out_token_stride, out_head_stride;
+    const void* k; /* [n_tokens][cache->n_heads][cache->head_dim] */
+    uint64_t k_token_stride, k_head_stride;
+    const void* v;
+    uint64_t v_token_stride, v_head_stride;
+    const int32_t* d_positions;
+    const double* d_freqs; /* [rotated / 2], radians a position */
+    const int64_t* d_slots;
+    uint32_t n_tokens, n_heads, rotated, interleaved;
+    float magnitude;
+} cr_paged_rotary_args;
+int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_cache* cache, cr_stream_t stream);
+
+/* Attention weights that tokens of the cache got, summed over rows and heads:
+ * d_out[r][i] = (i < older ? decay * d_past[r][i] : 0)
+ *               + sum of exp(scale * q k_i - lse) over the request's rows that see i,
+ * for the request's entries i < d_kv_len[r].  Its rows are tokens [d_starts[r],
+ * d_starts[r] + d_new[r]), or up to d_starts[r + 1] where d_new is NULL: the last of
+ * its positions, so that `older` is d_kv_len[r] less their number, and with `causal`
+ * row t sees entries [0, older + t].  (A prompt's last tokens are counted alone with
+ * d_starts moved up to them; after a verification, the accepted ones with d_new and
+ * a shorter d_kv_len.)  lse [n_tokens][n_heads] is what the attention of these rows
+ * left, with the same scale; a row whose lse is -inf counts for nothing.  `visible`, a
+ * bitmap over the slots, or NULL: others got nothing, nor did entries whose page is
+ * outside the cache.  d_past may be d_out, or NULL: nothing before.  Sums are in
+ * fp32, in an order that depends on the arguments alone.  Entries behind d_kv_len[r]
+ * are left as they were.  Types and alignment are those of cr_paged_attention;
+ * cache->v is not looked at. */
+typedef struct cr_paged_weights_args {
+    const void* q; /* [n_tokens][n_heads][head_dim] */
+    uint64_t q_token_stride, q_head_stride;
+    const float* lse;
+    uint32_t n_tokens, n_heads, n_requests;
+    const int32_t* d_starts; /* [n_requests + 1], or [n_requests] with d_new */
+    const int32_t* d_new;
+    const int32_t* d_kv_len;
+    const int32_t* d_table;
+    uint32_t table_cols;
+    uint64_t table_stride;
+    const cr_gpu_roaring* visible;
+    const float* d_past; /* rows of table_cols * page_size */
+    uint64_t past_stride;
+    float* d_out;
+    uint64_t out_stride;
+    float scale, decay;
+    uint32_t causal;
+    uint32_t continued; /* d_past counts for all entries: a step's layers behind the first */
+    /* The most rows and positions of a request, where the caller knows them (0: not
+     * known).  They choose how the work is split, never the answer. */
+    uint32_t max_new, max_kv;
+} cr_paged_weights_args;
+int cr_paged_weights(const cr_paged_weights_args* args, const cr_paged_cache* cache, cr_stream_t stream);
+
+/* Which tokens of each request stay in the cache.  Entry i < L = d_kv_len[r] has the
+ * position d_positions[r][i] for i < d_kept[r], and d_seen[r] - L + i behind them:
+ * d_seen[r] is how many tokens the request has had in all (d_positions NULL: all are
+ * counted that way; d_seen NULL: L).  It is safe if its slot is in `pinned` (a bitmap
+ * over the slots, or NULL), or if its position is one of the first `sinks` or among
+ * the last `recent` of d_seen[r].  Of the others those with the largest weights stay,
+ * ties to the lowest i, until m = max(min(L, d_keep[r]), the safe ones) stay in all
+ * (NaN weighs least).  d_len[r] receives m.  The ones that stay in [m, L) move, in
+ * order, into the places in [0, m) that get free: d_moves[r][0, d_n_moves[r]) are
+ * pairs (from slot, to slot) for cr_paged_move, never the same slot twice, and
+ * d_weights_out[r][0, m) and d_positions_out[r][0, m) (NULL: not wanted) what then
+ * lies there; those two may be the inputs themselves.  A row of d_moves holds half as
+ * many pairs as a row of the table has positions.  d_freed[0, freed_cap) receives the
+ * pages that no entry of their request is in any more, requests in order, and
+ * d_counts[0, 2) their number and that of all moves.  The table stays as it is:
+ * cr_paged_plan, with d_len for d_cached, writes over what is behind.  Pages that
+ * several requests share have to be pinned, first in their rows and no more than
+ * m slots, so that nothing moves into them; they are then no page that gets free. */
+typedef struct cr_paged_evict_args {
+    const float* d_weights;
+    uint64_t weights_stride;
+    const int32_t* d_positions;
+    uint64_t positions_stride;
+    const int32_t* d_kept;
+    const int32_t* d_seen;
+    const int32_t* d_kv_len;
+    const int32_t* d_keep;
+    const int32_t* d_table;
+    uint32_t table_cols;
+    uint64_t table_stride;
+    uint32_t page_size, n_pages, n_requests;
+    uint32_t sinks, recent;
+    const cr_gpu_roaring* pinned;
+    float* d_weights_out;
+    uint64_t weights_out_stride;
+    int32_t* d_positions_out;
+    uint64_t positions_out_stride;
+    int32_t* d_len;
+    int32_t* d_moves; /* [n_requests][moves_stride][2] */
+    uint32_t moves_cap;
+    uint64_t moves_stride;
+    int32_t* d_n_moves;
+    int32_t* d_freed;
+    uint32_t freed_cap;
+    int32_t* d_counts;
+} cr_paged_evict_args;
+int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t stream);
+/* Keys and values from slot to slot, for each layer of the cache: the first
+ * d_n_moves[r] pairs (from, to) of each request.  A pair with a slot outside the cache
+ * is left out.  No slot may be both a source and a destination. */
+int cr_paged_move(const int32_t* d_moves, uint32_t moves_cap, uint64_t moves_stride, const int32_t* d_n_moves,
+                  uint32_t n_requests, const cr_paged_cache* cache, cr_stream_t stream);
+
 /* Beam search's selection: of the continuations (w, v) of each answer's `beams`
  * beams by `vocab` tokens, the k (at most 256) with the largest
  * d_cum[b][w] + (score[b][w][v] - d_lse[b][w]) (d_lse NULL: d_cum + score), in
@@ -486,6 +604,41 @@ int cr_beam_select(const void* d_scores, uint32_t dtype, uint32_t batch, uint32_
 int cr_beam_reorder(const void* d_src, const int32_t* d_parents, uint32_t batch, uint32_t beams_in,
                     uint32_t beams_out, uint64_t row_bytes, uint64_t src_stride, uint64_t dst_stride,
                     const int32_t* d_len, uint64_t unit_bytes, void* d_dst, cr_stream_t stream);
+
+/* Drafted tokens against the model's own probabilities.  Request r's rows are
+ * [d_starts[r], d_starts[r + 1]): row i of d_scores holds the model's scores after
+ * token d_tokens[i], and row i of d_draft the drafting model's; the tokens behind a
+ * request's first are its drafts, d_tokens[i + 1] drawn after row i.  (d_draft's last
+ * row of each request is not looked at.)  p = softmax(scores / temperature) over the
+ * allowed tokens, q likewise; without d_draft, q is 1 for the draft itself.  A draft d
+ * is accepted while u q(d) < p(d), u = d_uniform of its row i.  d_out[r] receives the
+ * accepted drafts, then one token drawn from max(p - q, 0) of the row of the first
+ * that was not, or from p of the last row (from p, where nothing else is left): the
+ * lowest token at which the running sum exceeds d_uniform[last row] times the whole;
+ * then -1 up to out_cols.  d_accepted[r] counts the accepted ones.  A score that is
+ * NaN or -inf has probability 0, scores of +inf share it evenly; after a row without a
+ * candidate no draft is accepted and the token is -1, as for a request without rows.
+ * `allowed` and d_allowed_bits are those of cr_beam_select, a set of bits for each
+ * row of d_scores.  Probabilities and their sums are in fp64. */
+typedef struct cr_draft_verify_args {
+    const void* d_scores; /* [n_rows][vocab] */
+    uint64_t row_stride;
+    const void* d_draft; /* [n_rows][vocab], or NULL */
+    uint64_t draft_row_stride;
+    uint32_t dtype, n_rows, n_requests, vocab;
+    const int32_t* d_tokens;  /* [n_rows] */
+    const int32_t* d_starts;  /* [n_requests + 1] */
+    const float* d_uniform;   /* [n_rows], in [0, 1) */
+    const cr_gpu_roaring* allowed;
+    const uint32_t* d_allowed_bits;
+    uint64_t bits_stride;
+    float temperature; /* > 0 */
+    int32_t* d_accepted; /* [n_requests] */
+    int32_t* d_out;      /* [n_requests][out_cols] */
+    uint32_t out_cols;
+    uint64_t out_stride;
+} cr_draft_verify_args;
+int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t stream);
 
 /* ---- utilities (no reference counterpart) -------------------------------- */
 /* L2 size the AUTO rule uses for `device_id` (hipDeviceAttributeL2CacheSize). */
