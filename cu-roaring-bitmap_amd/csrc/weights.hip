@@ -21,6 +21,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct Half {
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
@@ -28,11 +29,21 @@ struct Half {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0,
                                                       0);
     }
+    static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0,
+                                                      0);
+    }
 };
 struct BHalf {
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0,
+                                                       0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(v8s x, v8s y, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0,
                                                        0);
     }
 };
@@ -62,7 +73,13 @@ struct WeightArgs {
     uint64_t out_stride;
     float scale2;  // scale * log2(e)
     bool causal, continued;
-    uint32_t head_waves, spans;  // waves that share the heads; workgroups of a request
+    uint32_t head_waves, spans;  // few rows: waves that share the heads; workgroups of a request
+    // Many rows: parts of the requests' rows, the i-th request's from base[i] on, of
+    // base[n_requests + 1] rows each; tiles of positions that the launch has for each; and
+    // their sums [parts][key heads][room].
+    uint32_t* base;
+    uint32_t most_parts, part_rows, tiles, room;
+    float* sums;
 };
 
 struct Counted {  // a request's rows and positions
@@ -80,6 +97,9 @@ __device__ __forceinline__ Counted counted_of(const WeightArgs& a, uint32_t r)
     return {static_cast<uint32_t>(t0), static_cast<uint32_t>(t1 - t0),
             static_cast<uint32_t>(min(room, static_cast<uint64_t>(len))), static_cast<int64_t>(a.kv_len[r]) - (t1 - t0)};
 }
+
+// Up to this many rows that share a key head in a request, wt_rows.
+constexpr uint32_t WT_FEW = 32;
 
 constexpr int WR_NT = 256;
 constexpr uint32_t WR_WAVES = WR_NT / 64;
@@ -195,19 +215,306 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
     }
 }
 
+// ---- many rows ------------------------------------------------------------------------
+// A workgroup takes a part of a request's rows, one key head and a tile of 256
+// positions, 64 a wave, whose keys stay in registers as the columns of 32x32x16
+// products; the queries pass by through LDS, 64 rows at a time, where the next ones
+// arrive meanwhile without passing through registers.  A lane sums what its two
+// columns get; the parts' sums are joined by another kernel, heads and parts in order.
+// Rows of LDS are turned by pieces of 16 bytes so that the 32 rows of a fragment
+// share no banks.
+constexpr int WT_NT = 256;
+constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
+constexpr int WP_NT = 1024;
+
+template <uint32_t DIM>
+struct Stage {
+    static constexpr uint32_t CHUNKS = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;  // 16-byte pieces of a row in LDS
+    static constexpr uint32_t STRIDE = CHUNKS * 8;                             // its elements
+    static constexpr uint32_t TURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
+    static constexpr uint32_t PER = WT_NT / CHUNKS, LOADS = WT_ROWS / PER;  // rows that the workgroup loads at once
+};
+
+// Blocks of 32 positions whose keys a wave holds; positions of a workgroup's tile.
+constexpr uint32_t tile_blocks(uint32_t dim) { return dim <= 192 ? 2 : 1; }
+constexpr uint32_t tile_cols(uint32_t dim) { return tile_blocks(dim) * 32 * (WT_NT / 64); }
+
+__device__ __forceinline__ uint32_t parts_of(uint32_t rows, uint32_t part_rows)
+{
+    return max(1u, (rows + part_rows - 1) / part_rows);
+}
+
+// Numbers the parts.  Rows may be counted for several requests, so that there may be more
+// of them than tokens: the parts then get longer.
+__global__ __launch_bounds__(WP_NT) void wt_parts(WeightArgs a)
+{
+    __shared__ uint32_t s_scan[WP_NT / 64];
+    const uint32_t t = threadIdx.x, group = a.heads / a.kv_heads;
+    uint32_t size = a.part_rows, total = 0;
+    for (;; size *= 2) {
+        total = 0;
+        for (uint32_t r0 = 0; r0 < a.n_requests && total <= a.most_parts; r0 += WP_NT) {
+            const uint32_t r = r0 + t, n = r < a.n_requests ? parts_of(counted_of(a, r).tokens * group, size) : 0u;
+            uint32_t all;
+            const uint32_t before = total + block_excl_scan<WP_NT>(min(n, a.most_parts + 1), s_scan, all);
+            if (r < a.n_requests) a.base[r] = before;
+            total += all;
+        }
+        if (total <= a.most_parts || size >> 31) break;
+    }
+    if (t == 0) {
+        a.base[a.n_requests] = total;
+        a.base[a.n_requests + 1] = size;
+    }
+}
+
+// The first row that sees a position, at or behind all that its tokens are.
+__device__ __forceinline__ int64_t first_row(const WeightArgs& a, const Counted& t, uint32_t p, uint32_t group)
+{
+    return a.causal ? max(static_cast<int64_t>(0), static_cast<int64_t>(p) - t.older) * group : 0;
+}
+
+// The rows [first, end) of part i that a tile whose first position is p counts.
+__device__ __forceinline__ void rows_of_part(const WeightArgs& a, const Counted& t, uint32_t p, uint32_t group, uint32_t i,
+                                             uint32_t size, uint32_t& first, uint32_t& end)
+{
+    const uint64_t rows = static_cast<uint64_t>(t.tokens) * group, from = static_cast<uint64_t>(i) * size;
+    const uint64_t sees = static_cast<uint64_t>(first_row(a, t, p, group)) / 32 * 32;
+    end = static_cast<uint32_t>(min(rows, from + size));
+    first = static_cast<uint32_t>(min(static_cast<uint64_t>(end), max(from, sees)));
+}
+
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
+{
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <class E, uint32_t DIM>
+__global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void wt_tiles(WeightArgs a)
+{
+    using S = Stage<DIM>;
+    constexpr uint32_t STEPS = DIM / 16, NB = tile_blocks(DIM), COLS = tile_cols(DIM);
+    // separate arrays: what is read is not what is being loaded
+    __shared__ alignas(16) uint16_t s_q0[WT_ROWS * S::STRIDE], s_q1[WT_ROWS * S::STRIDE];
+    __shared__ uint64_t s_at[4][WT_ROWS];
+    __shared__ alignas(16) float s_lse[4][WT_ROWS];
+    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
+    const uint32_t kh = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads / a.tiles;
+    const uint32_t group = a.heads / a.kv_heads;
+    if (part >= a.base[a.n_requests]) return;
+    uint32_t r = 0;  // the last request whose parts begin at or before this one
+    for (uint32_t end = a.n_requests; end - r > 1;) {
+        const uint32_t mid = (r + end) / 2;
+        if (a.base[mid] <= part)
+            r = mid;
+        else
+            end = mid;
+    }
+    const Counted t = counted_of(a, r);
+    const uint32_t size = a.base[a.n_requests + 1], nth = part - a.base[r];
+    const uint32_t rows = t.tokens * group;
+    const uint32_t lrow = threadIdx.x / S::CHUNKS, lpos = threadIdx.x % S::CHUNKS;
+    const uint32_t wave_row = __builtin_amdgcn_readfirstlane(wave) * (64 / S::CHUNKS);
+    if (a.dim < DIM) {  // pieces behind the head dimension: zeros, as the keys that they meet
+#pragma unroll
+        for (uint32_t x = 0; x < S::LOADS; ++x) {
+            const uint32_t lr = x * S::PER + lrow, at = lr * S::STRIDE + lpos * 8;
+            if ((lpos ^ (lr & S::TURN)) * 8 >= a.dim) {
+                *reinterpret_cast<v8s*>(s_q0 + at) = v8s{};
+                *reinterpret_cast<v8s*>(s_q1 + at) = v8s{};
+            }
+        }
+    }
+    // (more than once where the caller's most positions are fewer than there are)
+    for (uint32_t first = blockIdx.x / a.kv_heads % a.tiles * COLS; first < t.keys; first += a.tiles * COLS) {
+        uint32_t row0, row1;
+        rows_of_part(a, t, first, group, nth, size, row0, row1);
+        if (row0 >= row1) continue;
+        v8s key[NB][STEPS];
+        uint32_t from[NB], latest = 0;
+        bool see[NB];
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            const uint32_t p = first + (wave * NB + b) * 32 + c32;
+            uint64_t at = 0;
+            see[b] = false;
+            from[b] = 0;
+            if (p < t.keys) {
+                const uint32_t page = static_cast<uint32_t>(a.table[r * a.table_stride + (p >> a.page_lg)]);
+                const uint32_t off = p & ((1u << a.page_lg) - 1u), slot = (page << a.page_lg) + off;
+                see[b] = page < a.n_pages;
+                if (see[b] && a.gated)
+                    see[b] = slot < a.visible.end && ((a.visible.word(slot >> 5) >> (slot & 31u)) & 1u);
+                const int64_t sees = first_row(a, t, p, group);
+                see[b] = see[b] && sees < row1;
+                if (see[b]) {
+                    at = page * a.k_page + off * a.k_slot;
+                    from[b] = static_cast<uint32_t>(sees);
+                }
+            }
+            latest = max(latest, from[b]);
+#pragma unroll
+            for (uint32_t st = 0; st < STEPS; ++st) {
+                const uint32_t d = st * 16 + h * 8;
+                key[b][st] = see[b] && d < a.dim ? *reinterpret_cast<const v8s*>(a.k + at + kh * a.k_head + d) : v8s{};
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) latest = max(latest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(latest), o, 64)));
+        latest = __builtin_amdgcn_readfirstlane(latest);
+        bool any = false;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) any = any || __ballot(see[b]) != 0;
+        float sum[NB] = {};
+
+        // Where a stage's rows are, and their log-sums: lane l looks after row l.
+        const uint32_t n_stages = (row1 - row0 + WT_ROWS - 1) / WT_ROWS;
+        auto note = [&](uint32_t i) {
+            const uint32_t row = min(row0 + i * WT_ROWS + lane, rows - 1);
+            const uint64_t token = t.token0 + row / group;
+            const uint32_t head = kh * group + row % group;
+            const float z = a.lse[token * a.heads + head];
+            s_at[i % 4][lane] = token * a.q_token + head * a.q_head;
+            s_lse[i % 4][lane] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
+        };
+        auto load = [&](uint32_t i, uint16_t* sq) {
+#pragma unroll
+            for (uint32_t x = 0; x < S::LOADS; ++x) {
+                const uint32_t lr = x * S::PER + lrow, d = (lpos ^ (lr & S::TURN)) * 8;
+                if (d < a.dim) load_to_lds(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
+            }
+        };
+        auto multiply = [&](uint32_t i, const uint16_t* sq) {
+            if (!any) return;
+#pragma unroll
+            for (uint32_t y = 0; y < WT_ROWS / 32; ++y) {
+                const uint32_t base = row0 + i * WT_ROWS + y * 32;
+                if (base >= row1) break;
+                f32x16 x[NB];
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e) x[b][e] = 0.0f;
+#pragma unroll
+                for (uint32_t st = 0; st < STEPS; ++st) {
+                    const v8s q = *reinterpret_cast<const v8s*>(sq + (y * 32 + c32) * S::STRIDE +
+                                                                ((st * 2 + h) ^ (c32 & S::TURN)) * 8);
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; ++b) x[b] = E::mfma32(q, key[b][st], x[b]);
+                }
+                f32x4 z[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    z[e] = *reinterpret_cast<const f32x4*>(&s_lse[i % 4][y * 32 + e * 8 + h * 4]);
+                const bool whole = base >= latest && base + 32 <= row1;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    float w[16];
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e)
+                        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], a.scale2, -z[e / 4][e % 4]));
+                    if (!whole) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) {
+                            const uint32_t row = base + e / 4 * 8 + h * 4 + e % 4;
+                            w[e] = row >= from[b] && row < row1 ? w[e] : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t o = 8; o > 0; o >>= 1)
+#pragma unroll
+                        for (uint32_t e = 0; e < o; ++e) w[e] += w[e + o];
+                    sum[b] += w[0];
+                }
+            }
+        };
+        __syncthreads();  // the tile before is done with LDS
+        if (wave < 2) note(wave);
+        __syncthreads();
+        load(0, s_q0);
+        for (uint32_t i = 0; i < n_stages; i += 2) {
+            __syncthreads();
+            if (i + 1 < n_stages) load(i + 1, s_q1);
+            if (wave == 2 && i + 2 < n_stages) note(i + 2);
+            multiply(i, s_q0);
+            if (i + 1 >= n_stages) break;
+            __syncthreads();
+            if (i + 2 < n_stages) load(i + 2, s_q0);
+            if (wave == 3 && i + 3 < n_stages) note(i + 3);
+            multiply(i + 1, s_q1);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            sum[b] += __shfl_xor(sum[b], 32, 64);
+            const uint32_t p = first + (wave * NB + b) * 32 + c32;
+            if (h == 0 && p < t.keys)
+                a.sums[(static_cast<uint64_t>(part) * a.kv_heads + kh) * a.room + p] = see[b] ? sum[b] : 0.0f;
+        }
+    }
+}
+
+// The parts' sums joined: 64 positions a workgroup, whose waves share the heads and
+// parts.
+constexpr int WJ_NT = 1024;
+
+__global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t cols)
+{
+    constexpr uint32_t WAVES = WJ_NT / 64;
+    __shared__ float s_sum[WAVES][64];
+    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, group = a.heads / a.kv_heads;
+    const uint32_t r = blockIdx.x / per_request;
+    const Counted t = counted_of(a, r);
+    const uint32_t base = a.base[r], parts = a.base[r + 1] - base, size = a.base[a.n_requests + 1];
+    for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
+        const uint32_t p = p0 + lane, n = parts * a.kv_heads;
+        float sum = 0.0f;
+        uint32_t skip = 0;  // parts that see nothing of the position's tile: the first ones
+        for (; skip < parts; ++skip) {
+            uint32_t first, end;
+            rows_of_part(a, t, p0 / cols * cols, group, skip, size, first, end);
+            if (first < end) break;
+        }
+        if (p < t.keys)
+#pragma unroll 4
+            for (uint32_t i = skip * a.kv_heads + wave; i < n; i += WAVES)
+                sum += a.sums[(static_cast<uint64_t>(base) * a.kv_heads + i) * a.room + p];
+        s_sum[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && p < t.keys) {
+            float all = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < WAVES; ++w) all += s_sum[w][lane];
+            const float past =
+                a.past && (a.continued || static_cast<int64_t>(p) < t.older) ? a.past[r * a.past_stride + p] * a.decay : 0.0f;
+            a.out[r * a.out_stride + p] = past + all;
+        }
+        __syncthreads();
+    }
+}
+
+template <class E, uint32_t DIM>
+void launch_dim(const WeightArgs& a, uint32_t grid, hipStream_t s)
+{
+    if (a.sums)
+        wt_tiles<E, DIM><<<grid, WT_NT, 0, s>>>(a);
+    else
+        wt_rows<E, DIM><<<grid, WR_NT, 0, s>>>(a);
+}
+
 template <class E>
 void launch_weights(const WeightArgs& a, uint32_t grid, hipStream_t s)
 {
     if (a.dim <= 64)
-        wt_rows<E, 64><<<grid, WR_NT, 0, s>>>(a);
+        launch_dim<E, 64>(a, grid, s);
     else if (a.dim <= 96)
-        wt_rows<E, 96><<<grid, WR_NT, 0, s>>>(a);
+        launch_dim<E, 96>(a, grid, s);
     else if (a.dim <= 128)
-        wt_rows<E, 128><<<grid, WR_NT, 0, s>>>(a);
+        launch_dim<E, 128>(a, grid, s);
     else if (a.dim <= 192)
-        wt_rows<E, 192><<<grid, WR_NT, 0, s>>>(a);
+        launch_dim<E, 192>(a, grid, s);
     else
-        wt_rows<E, 256><<<grid, WR_NT, 0, s>>>(a);
+        launch_dim<E, 256>(a, grid, s);
 }
 
 }  // namespace
@@ -287,28 +594,69 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     a.causal = p.causal != 0;
     a.continued = p.continued != 0;
     const uint64_t most = p.max_kv ? std::min<uint64_t>(room, p.max_kv) : room;
-    a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
-    const uint32_t span = WR_WAVES / a.head_waves * WR_TILES * 16;
-    a.spans = static_cast<uint32_t>((most + span - 1) / span);
-    if (a.spans == 0) return CR_OK;
-    const uint64_t grid = static_cast<uint64_t>(a.spans) * a.n_requests;
-    if (grid >> 23) {  // a launch holds fewer than 2^32 threads
-        set_error("cr_paged_weights: too many positions for one call");
-        return CR_ERR_UNSUPPORTED;
+    if (most == 0) return CR_OK;
+    // Rows of a request that share a key head, as far as the caller says.
+    const uint32_t group = a.heads / a.kv_heads;
+    const uint64_t typical = p.max_new ? p.max_new : (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests;
+    const bool many = typical * group > WT_FEW;
+    const uint32_t cols = tile_cols(a.dim);
+    a.room = static_cast<uint32_t>(room);
+    uint64_t grid;
+    Carver cv;
+    size_t o_base = 0, o_sums = 0;
+    if (many) {
+        a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
+        // Parts of the rows: as many workgroups as fill the card a few times, and no longer
+        // sums than 2048 rows.
+        const uint64_t rows = static_cast<uint64_t>(p.n_tokens) * group;
+        const uint64_t even = rows * a.tiles * a.kv_heads / (8ull * num_cus());
+        a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
+        const uint64_t parts = rows / a.part_rows + p.n_requests;
+        grid = parts * a.tiles * a.kv_heads;
+        if (parts >> 21 || grid >> 23) {  // a launch holds fewer than 2^32 threads
+            set_error("cr_paged_weights: too many rows and positions for one call");
+            return CR_ERR_UNSUPPORTED;
+        }
+        a.most_parts = static_cast<uint32_t>(parts);
+        o_base = cv.add((p.n_requests + 2ull) * 4);
+        o_sums = cv.add(parts * a.kv_heads * room * 4);
+    } else {
+        a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
+        const uint32_t span = WR_WAVES / a.head_waves * WR_TILES * 16;
+        a.spans = static_cast<uint32_t>((most + span - 1) / span);
+        grid = static_cast<uint64_t>(a.spans) * a.n_requests;
+        if (grid >> 23) {
+            set_error("cr_paged_weights: too many positions for one call");
+            return CR_ERR_UNSUPPORTED;
+        }
     }
     hipStream_t s = as_stream(stream);
     const bool direct = p.visible && is_direct(p.visible);
     const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
+    const size_t o_words = cv.add(p.visible && !direct ? std::max<size_t>(4, n_words * 4ull) : 0);
     Scratch sc;
-    if (p.visible && !direct) CR_RET(sc.alloc(std::max<size_t>(256, n_words * 4ull), s));
+    if (cv.total) CR_RET(sc.alloc(cv.total, s));
     if (p.visible)
-        CR_RET(set_bits(p.visible, direct, sc.at<uint32_t>(0), n_words, static_cast<uint32_t>(n_slots), stream,
+        CR_RET(set_bits(p.visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                         &a.visible));
-    CR_TIMED("wt_rows", s);
-    if (cache->dtype == CR_F16)
-        launch_weights<Half>(a, static_cast<uint32_t>(grid), s);
-    else
-        launch_weights<BHalf>(a, static_cast<uint32_t>(grid), s);
+    if (many) {
+        a.base = sc.at<uint32_t>(o_base);
+        a.sums = sc.at<float>(o_sums);
+        CR_TIMED("wt_parts", s);
+        wt_parts<<<1, WP_NT, 0, s>>>(a);
+    }
+    {
+        CR_TIMED(many ? "wt_tiles" : "wt_rows", s);
+        if (cache->dtype == CR_F16)
+            launch_weights<Half>(a, static_cast<uint32_t>(grid), s);
+        else
+            launch_weights<BHalf>(a, static_cast<uint32_t>(grid), s);
+    }
+    if (many) {
+        CR_TIMED("wt_join", s);
+        const uint32_t per_request = static_cast<uint32_t>(std::min<uint64_t>((most + 63) / 64, std::max<uint64_t>(1, (1u << 22) / p.n_requests)));
+        wt_join<<<per_request * p.n_requests, WJ_NT, 0, s>>>(a, per_request, cols);
+    }
     CR_LAUNCH_CHECK();
     return CR_OK;
 }

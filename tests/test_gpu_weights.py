@@ -109,8 +109,8 @@ class Problem:
             gpu.free(g)
         return out.cpu().numpy().astype(np.float64)
 
-    def check(self, gpu, past=True, decay=0.75, **kw):
-        out = self.run(gpu, past, decay, **kw)
+    def check(self, gpu, past=True, decay=0.75, out=None, **kw):
+        out = self.run(gpu, past, decay, **kw) if out is None else out
         before = self.past.cpu().numpy().astype(np.float64)
         want, tol = np.zeros(out.shape), np.zeros(out.shape)
         terms = np.zeros(len(self.kv))
@@ -257,15 +257,29 @@ def test_some_rows_of_a_request(gpu):
     got = p.run(gpu, starts=starts, d_new=torch.tensor(take, **i32))
     p.new, p.q, p.lse = take, torch.cat([p.q[32:40], p.q[40:47], p.q[47:52]]), torch.cat([p.lse[32:40], p.lse[40:]])
     p.starts = torch.tensor([0, 8, 15, 20], **i32)
-    assert np.array_equal(got, p.run(gpu))
+    p.check(gpu, out=got)
     p.check(gpu)
     # the first 3, 0 and 5 tokens, the requests cut off behind them
     p, take, kv = whole, [3, 0, 5], [53, 53, 5]
     got = p.run(gpu, starts=p.starts, kv_len=torch.tensor(kv, **i32), d_new=torch.tensor(take, **i32))
     p.q, p.lse = torch.cat([p.q[:3], p.q[47:52]]), torch.cat([p.lse[:3], p.lse[47:52]])
     p.new, p.kv, p.kv_len, p.starts = take, kv, torch.tensor(kv, **i32), torch.tensor([0, 3, 3, 8], **i32)
-    assert np.array_equal(got, p.run(gpu))
+    p.check(gpu, out=got)
     p.check(gpu)
+
+
+def test_rows_of_several_requests(gpu):
+    """Requests that count the same rows, more of them in all than there are, and in any order."""
+    import torch
+    _say("weights of shared rows")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n, take = 40, 70
+    p = Problem("bfloat16", [take + 30] + [0] * (n - 1), [500] * n, 4, 1, 64, 16, seed=19)
+    starts = [(7 * i) % 31 for i in range(n)]
+    got = p.run(gpu, starts=torch.tensor(starts, **i32), d_new=torch.full((n,), take, **i32))
+    p.new, p.q = [take] * n, torch.cat([p.q[s:s + take] for s in starts])
+    p.lse = torch.cat([p.lse[s:s + take] for s in starts])
+    p.check(gpu, out=got)
 
 
 def test_pages_outside_the_cache_get_nothing(gpu):
