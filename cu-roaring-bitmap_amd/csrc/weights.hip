@@ -385,6 +385,22 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                 if (d < a.dim) load_to_lds(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
             }
         };
+        auto add = [&](const f32x16 (&x)[NB], const f32x4 (&z)[4], auto counts) {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                float w[16];
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], a.scale2, -z[e / 4][e % 4]));
+                    if (!counts(b, e)) w[e] = 0.0f;
+                }
+#pragma unroll
+                for (uint32_t o = 8; o > 0; o >>= 1)
+#pragma unroll
+                    for (uint32_t e = 0; e < o; ++e) w[e] += w[e + o];
+                sum[b] += w[0];
+            }
+        };
         auto multiply = [&](uint32_t i, const uint16_t* sq) {
             if (!any) return;
 #pragma unroll
@@ -407,26 +423,14 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e)
                     z[e] = *reinterpret_cast<const f32x4*>(&s_lse[i % 4][y * 32 + e * 8 + h * 4]);
-                const bool whole = base >= latest && base + 32 <= row1;
-#pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) {
-                    float w[16];
-#pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e)
-                        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], a.scale2, -z[e / 4][e % 4]));
-                    if (!whole) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e) {
-                            const uint32_t row = base + e / 4 * 8 + h * 4 + e % 4;
-                            w[e] = row >= from[b] && row < row1 ? w[e] : 0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (uint32_t o = 8; o > 0; o >>= 1)
-#pragma unroll
-                        for (uint32_t e = 0; e < o; ++e) w[e] += w[e + o];
-                    sum[b] += w[0];
-                }
+                // Apart, so that rows which all see all are not tested one by one.
+                if (base >= latest && base + 32 <= row1)
+                    add(x, z, [](uint32_t, uint32_t) { return true; });
+                else
+                    add(x, z, [&](uint32_t b, uint32_t e) {
+                        const uint32_t row = base + e / 4 * 8 + h * 4 + e % 4;
+                        return row >= from[b] && row < row1;
+                    });
             }
         };
         __syncthreads();  // the tile before is done with LDS
