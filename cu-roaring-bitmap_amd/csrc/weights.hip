@@ -74,11 +74,9 @@ struct WeightArgs {
     float scale2;  // scale * log2(e)
     bool causal, continued;
     uint32_t head_waves, spans;  // few rows: waves that share the heads; workgroups of a request
-    // Many rows: parts of the requests' rows, the i-th request's from base[i] on, of
-    // base[n_requests + 1] rows each; tiles of positions that the launch has for each; and
-    // their sums [parts][key heads][room].
-    uint32_t* base;
-    uint32_t most_parts, part_rows, tiles, room;
+    // Many rows: parts of a request's rows, of part_rows or more each; tiles of positions
+    // that the launch has for a request; and their sums [n_requests][parts][key heads][room].
+    uint32_t parts, part_rows, tiles, room;
     float* sums;
 };
 
@@ -225,7 +223,6 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 // share no banks.
 constexpr int WT_NT = 256;
 constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
-constexpr int WP_NT = 1024;
 
 template <uint32_t DIM>
 struct Stage {
@@ -239,48 +236,26 @@ struct Stage {
 constexpr uint32_t tile_blocks(uint32_t dim) { return dim <= 192 ? 2 : 1; }
 constexpr uint32_t tile_cols(uint32_t dim) { return tile_blocks(dim) * 32 * (WT_NT / 64); }
 
-__device__ __forceinline__ uint32_t parts_of(uint32_t rows, uint32_t part_rows)
-{
-    return max(1u, (rows + part_rows - 1) / part_rows);
-}
-
-// Numbers the parts.  Rows may be counted for several requests, so that there may be more
-// of them than tokens: the parts then get longer.
-__global__ __launch_bounds__(WP_NT) void wt_parts(WeightArgs a)
-{
-    __shared__ uint32_t s_scan[WP_NT / 64];
-    const uint32_t t = threadIdx.x, group = a.heads / a.kv_heads;
-    uint32_t size = a.part_rows, total = 0;
-    for (;; size *= 2) {
-        total = 0;
-        for (uint32_t r0 = 0; r0 < a.n_requests && total <= a.most_parts; r0 += WP_NT) {
-            const uint32_t r = r0 + t, n = r < a.n_requests ? parts_of(counted_of(a, r).tokens * group, size) : 0u;
-            uint32_t all;
-            const uint32_t before = total + block_excl_scan<WP_NT>(min(n, a.most_parts + 1), s_scan, all);
-            if (r < a.n_requests) a.base[r] = before;
-            total += all;
-        }
-        if (total <= a.most_parts || size >> 31) break;
-    }
-    if (t == 0) {
-        a.base[a.n_requests] = total;
-        a.base[a.n_requests + 1] = size;
-    }
-}
-
 // The first row that sees a position, at or behind all that its tokens are.
 __device__ __forceinline__ int64_t first_row(const WeightArgs& a, const Counted& t, uint32_t p, uint32_t group)
 {
     return a.causal ? max(static_cast<int64_t>(0), static_cast<int64_t>(p) - t.older) * group : 0;
 }
 
+// The rows of each of a request's parts.
+__device__ __forceinline__ uint32_t part_size(const WeightArgs& a, uint32_t rows)
+{
+    return max(a.part_rows, ((rows + a.parts - 1) / a.parts + 63u) / 64u * 64u);
+}
+
 // The rows [first, end) of part i that a tile whose first position is p counts.
 __device__ __forceinline__ void rows_of_part(const WeightArgs& a, const Counted& t, uint32_t p, uint32_t group, uint32_t i,
-                                             uint32_t size, uint32_t& first, uint32_t& end)
+                                             uint32_t& first, uint32_t& end)
 {
-    const uint64_t rows = static_cast<uint64_t>(t.tokens) * group, from = static_cast<uint64_t>(i) * size;
+    const uint32_t rows = t.tokens * group, size = part_size(a, rows);
+    const uint64_t from = static_cast<uint64_t>(i) * size;
     const uint64_t sees = static_cast<uint64_t>(first_row(a, t, p, group)) / 32 * 32;
-    end = static_cast<uint32_t>(min(rows, from + size));
+    end = static_cast<uint32_t>(min(static_cast<uint64_t>(rows), from + size));
     first = static_cast<uint32_t>(min(static_cast<uint64_t>(end), max(from, sees)));
 }
 
@@ -291,7 +266,7 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
 }
 
 template <class E, uint32_t DIM>
-__global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void wt_tiles(WeightArgs a)
+__global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 128 ? 3 : 2))) void wt_tiles(WeightArgs a)
 {
     using S = Stage<DIM>;
     constexpr uint32_t STEPS = DIM / 16, NB = tile_blocks(DIM), COLS = tile_cols(DIM);
@@ -301,18 +276,8 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
     __shared__ alignas(16) float s_lse[4][WT_ROWS];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
     const uint32_t kh = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads / a.tiles;
-    const uint32_t group = a.heads / a.kv_heads;
-    if (part >= a.base[a.n_requests]) return;
-    uint32_t r = 0;  // the last request whose parts begin at or before this one
-    for (uint32_t end = a.n_requests; end - r > 1;) {
-        const uint32_t mid = (r + end) / 2;
-        if (a.base[mid] <= part)
-            r = mid;
-        else
-            end = mid;
-    }
+    const uint32_t r = part / a.parts, group = a.heads / a.kv_heads;
     const Counted t = counted_of(a, r);
-    const uint32_t size = a.base[a.n_requests + 1], nth = part - a.base[r];
     const uint32_t rows = t.tokens * group;
     const uint32_t lrow = threadIdx.x / S::CHUNKS, lpos = threadIdx.x % S::CHUNKS;
     const uint32_t wave_row = __builtin_amdgcn_readfirstlane(wave) * (64 / S::CHUNKS);
@@ -329,44 +294,14 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
     // (more than once where the caller's most positions are fewer than there are)
     for (uint32_t first = blockIdx.x / a.kv_heads % a.tiles * COLS; first < t.keys; first += a.tiles * COLS) {
         uint32_t row0, row1;
-        rows_of_part(a, t, first, group, nth, size, row0, row1);
+        rows_of_part(a, t, first, group, part % a.parts, row0, row1);
         if (row0 >= row1) continue;
-        v8s key[NB][STEPS];
-        uint32_t from[NB], latest = 0;
-        bool see[NB];
+        uint32_t page[NB];
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            const uint32_t p = first + (wave * NB + b) * 32 + c32;
-            uint64_t at = 0;
-            see[b] = false;
-            from[b] = 0;
-            if (p < t.keys) {
-                const uint32_t page = static_cast<uint32_t>(a.table[r * a.table_stride + (p >> a.page_lg)]);
-                const uint32_t off = p & ((1u << a.page_lg) - 1u), slot = (page << a.page_lg) + off;
-                see[b] = page < a.n_pages;
-                if (see[b] && a.gated)
-                    see[b] = slot < a.visible.end && ((a.visible.word(slot >> 5) >> (slot & 31u)) & 1u);
-                const int64_t sees = first_row(a, t, p, group);
-                see[b] = see[b] && sees < row1;
-                if (see[b]) {
-                    at = page * a.k_page + off * a.k_slot;
-                    from[b] = static_cast<uint32_t>(sees);
-                }
-            }
-            latest = max(latest, from[b]);
-#pragma unroll
-            for (uint32_t st = 0; st < STEPS; ++st) {
-                const uint32_t d = st * 16 + h * 8;
-                key[b][st] = see[b] && d < a.dim ? *reinterpret_cast<const v8s*>(a.k + at + kh * a.k_head + d) : v8s{};
-            }
+            const uint32_t p = min(first + (wave * NB + b) * 32 + c32, t.keys - 1);
+            page[b] = static_cast<uint32_t>(a.table[r * a.table_stride + (p >> a.page_lg)]);
         }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) latest = max(latest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(latest), o, 64)));
-        latest = __builtin_amdgcn_readfirstlane(latest);
-        bool any = false;
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) any = any || __ballot(see[b]) != 0;
-        float sum[NB] = {};
 
         // Where a stage's rows are, and their log-sums: lane l looks after row l.
         const uint32_t n_stages = (row1 - row0 + WT_ROWS - 1) / WT_ROWS;
@@ -385,6 +320,34 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                 if (d < a.dim) load_to_lds(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
             }
         };
+        __syncthreads();  // the tile before is done with LDS
+        if (wave < 2) note(wave);
+        v8s key[NB][STEPS];
+        uint32_t from[NB], latest = 0;  // the first row that sees the lane's positions, if any
+        bool any = false;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            const uint32_t p = first + (wave * NB + b) * 32 + c32;
+            const uint32_t off = p & ((1u << a.page_lg) - 1u), slot = (page[b] << a.page_lg) + off;
+            bool see = p < t.keys && page[b] < a.n_pages;
+            if (see && a.gated) see = slot < a.visible.end && ((a.visible.word(slot >> 5) >> (slot & 31u)) & 1u);
+            const int64_t sees = first_row(a, t, p, group);
+            see = see && sees < row1;
+            from[b] = see ? static_cast<uint32_t>(sees) : 0xFFFFFFFFu;
+            latest = max(latest, see ? from[b] : 0u);
+            any = any || __ballot(see) != 0;
+            const uint16_t* at = a.k + (see ? page[b] * a.k_page + off * a.k_slot : 0) + kh * a.k_head;
+#pragma unroll
+            for (uint32_t st = 0; st < STEPS; ++st) {
+                const uint32_t d = st * 16 + h * 8;
+                key[b][st] = see && d < a.dim ? *reinterpret_cast<const v8s*>(at + d) : v8s{};
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) latest = max(latest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(latest), o, 64)));
+        latest = __builtin_amdgcn_readfirstlane(latest);
+        float sum[NB] = {};
+        const uint32_t q_at = c32 * S::STRIDE + (h ^ (c32 & S::TURN)) * 8;  // of step st: q_at ^ st * 16
         auto add = [&](const f32x16 (&x)[NB], const f32x4 (&z)[4], auto counts) {
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
@@ -412,10 +375,15 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                 for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
                     for (uint32_t e = 0; e < 16; ++e) x[b][e] = 0.0f;
+                // Three waves a SIMD leave 128 dimensions no registers to keep all addresses in: the
+                // second half's are worked out from the first's.
+                uint32_t half = DIM == 128 ? 64u : 0u;
+                if constexpr (DIM == 128) asm volatile("" : "+v"(half));
 #pragma unroll
                 for (uint32_t st = 0; st < STEPS; ++st) {
-                    const v8s q = *reinterpret_cast<const v8s*>(sq + (y * 32 + c32) * S::STRIDE +
-                                                                ((st * 2 + h) ^ (c32 & S::TURN)) * 8);
+                    const v8s q = *reinterpret_cast<const v8s*>(
+                        sq + y * 32 * S::STRIDE +
+                        (DIM == 128 && st >= 4 ? (q_at ^ (st * 16 - 64)) ^ half : q_at ^ (st * 16)));
 #pragma unroll
                     for (uint32_t b = 0; b < NB; ++b) x[b] = E::mfma32(q, key[b][st], x[b]);
                 }
@@ -433,8 +401,6 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                     });
             }
         };
-        __syncthreads();  // the tile before is done with LDS
-        if (wave < 2) note(wave);
         __syncthreads();
         load(0, s_q0);
         for (uint32_t i = 0; i < n_stages; i += 2) {
@@ -453,7 +419,8 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(2))) void
             sum[b] += __shfl_xor(sum[b], 32, 64);
             const uint32_t p = first + (wave * NB + b) * 32 + c32;
             if (h == 0 && p < t.keys)
-                a.sums[(static_cast<uint64_t>(part) * a.kv_heads + kh) * a.room + p] = see[b] ? sum[b] : 0.0f;
+                a.sums[(static_cast<uint64_t>(part) * a.kv_heads + kh) * a.room + p] =
+                    from[b] != 0xFFFFFFFFu ? sum[b] : 0.0f;
         }
     }
 }
@@ -469,20 +436,18 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, group = a.heads / a.kv_heads;
     const uint32_t r = blockIdx.x / per_request;
     const Counted t = counted_of(a, r);
-    const uint32_t base = a.base[r], parts = a.base[r + 1] - base, size = a.base[a.n_requests + 1];
     for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
-        const uint32_t p = p0 + lane, n = parts * a.kv_heads;
+        const uint32_t p = p0 + lane, n = a.parts * a.kv_heads;
         float sum = 0.0f;
         uint32_t skip = 0;  // parts that see nothing of the position's tile: the first ones
-        for (; skip < parts; ++skip) {
-            uint32_t first, end;
-            rows_of_part(a, t, p0 / cols * cols, group, skip, size, first, end);
+        for (uint32_t first, end; skip < a.parts; ++skip) {
+            rows_of_part(a, t, p0 / cols * cols, group, skip, first, end);
             if (first < end) break;
         }
         if (p < t.keys)
 #pragma unroll 4
             for (uint32_t i = skip * a.kv_heads + wave; i < n; i += WAVES)
-                sum += a.sums[(static_cast<uint64_t>(base) * a.kv_heads + i) * a.room + p];
+                sum += a.sums[(static_cast<uint64_t>(r) * n + i) * a.room + p];
         s_sum[wave][lane] = sum;
         __syncthreads();
         if (wave == 0 && p < t.keys) {
@@ -607,23 +572,22 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     a.room = static_cast<uint32_t>(room);
     uint64_t grid;
     Carver cv;
-    size_t o_base = 0, o_sums = 0;
+    size_t o_sums = 0;
     if (many) {
         a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
         // Parts of the rows: as many workgroups as fill the card a few times, and no longer
         // sums than 2048 rows.
-        const uint64_t rows = static_cast<uint64_t>(p.n_tokens) * group;
-        const uint64_t even = rows * a.tiles * a.kv_heads / (8ull * num_cus());
+        const uint64_t rows = (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests * group;
+        const uint64_t even = rows * p.n_requests * a.tiles * a.kv_heads / (8ull * num_cus());
         a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
-        const uint64_t parts = rows / a.part_rows + p.n_requests;
-        grid = parts * a.tiles * a.kv_heads;
-        if (parts >> 21 || grid >> 23) {  // a launch holds fewer than 2^32 threads
+        const uint64_t parts = std::max<uint64_t>(1, (rows + a.part_rows - 1) / a.part_rows);
+        grid = parts * p.n_requests * a.tiles * a.kv_heads;
+        if (grid >> 23) {  // a launch holds fewer than 2^32 threads
             set_error("cr_paged_weights: too many rows and positions for one call");
             return CR_ERR_UNSUPPORTED;
         }
-        a.most_parts = static_cast<uint32_t>(parts);
-        o_base = cv.add((p.n_requests + 2ull) * 4);
-        o_sums = cv.add(parts * a.kv_heads * room * 4);
+        a.parts = static_cast<uint32_t>(parts);
+        o_sums = cv.add(parts * p.n_requests * a.kv_heads * room * 4);
     } else {
         a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
         const uint32_t span = WR_WAVES / a.head_waves * WR_TILES * 16;
@@ -643,12 +607,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     if (p.visible)
         CR_RET(set_bits(p.visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                         &a.visible));
-    if (many) {
-        a.base = sc.at<uint32_t>(o_base);
-        a.sums = sc.at<float>(o_sums);
-        CR_TIMED("wt_parts", s);
-        wt_parts<<<1, WP_NT, 0, s>>>(a);
-    }
+    if (many) a.sums = sc.at<float>(o_sums);
     {
         CR_TIMED(many ? "wt_tiles" : "wt_rows", s);
         if (cache->dtype == CR_F16)
