@@ -17,11 +17,10 @@ namespace crimpl {
 namespace {
 
 constexpr int EV_NT = 1024;
-constexpr uint32_t EV_WAVES = EV_NT / 64;
-constexpr uint32_t EV_ROW = 256;       // entries that a wave takes at a time, four a lane
 constexpr uint32_t EV_SAFE = 0xFFFFFFFFu;  // above the order of every weight
-constexpr uint32_t EV_BINS = 2048;     // of a digit of 11 bits
-constexpr uint32_t EV_COPIES = 4;      // of the first digit's counts
+constexpr uint32_t EV_BINS = 2048;         // of a digit of 11 bits
+constexpr uint32_t EV_COPIES = 4;          // of the first digit's counts
+constexpr uint32_t EV_NO_DIGIT = 2046;     // a first digit above those of all weights and below that of EV_SAFE
 
 struct EvictArgs {
     const float* weights;
@@ -51,8 +50,16 @@ struct EvictArgs {
     int32_t* freed;
     uint32_t freed_cap;
     int32_t* counts;
-    uint32_t* keys;       // [n_requests][room rounded up to EV_ROW]
-    uint32_t keys_stride;
+    bool wide;            // rows can be read four entries at a time
+    // Long rows, in segments: the entries' places in the order, and what the launches leave
+    // for one another.
+    uint32_t segments;
+    uint32_t* keys;       // [n_requests][segments][SG_SIZE]
+    uint2* undecided;     // the same: (key, entry)
+    uint32_t* bins;       // [n_requests][segments][EV_BINS / 2], two counts a word
+    uint4* counts_of;     // [n_requests][segments]
+    uint4* from;          // [n_requests][segments]
+    uint4* picked;        // [n_requests][2]
 };
 
 __device__ __forceinline__ uint32_t request_len(const EvictArgs& a, uint32_t r)
@@ -91,29 +98,22 @@ struct Ages {  // of a request's entries
     __device__ __forceinline__ bool safe(int64_t p) const { return p < sinks || p >= recent; }
 };
 
-__device__ __forceinline__ uint32_t lanes_below(unsigned long long m)
-{
-    const uint32_t lane = __lane_id();
-    return static_cast<uint32_t>(__popcll(m & ((1ull << lane) - 1ull)));
-}
-
 // Finds the digit in which the n-th largest of the counted values lies (n >= 1, at
-// most their number): counts are EV_BINS, the highest digit first taken.  Every
-// thread gets the digit and how many values have a higher one.
-__device__ __forceinline__ void find_digit(const uint32_t* s_bins, uint32_t copies, uint32_t n, uint32_t* s_scan,
-                                           uint32_t* s_found, uint32_t& digit, uint32_t& above)
+// most their number).  count(bin): how many have it.  Every thread gets the digit and
+// how many values have a higher one.
+template <int NT, class F>
+__device__ __forceinline__ void find_digit(F count, uint32_t n, uint32_t* s_scan, uint32_t* s_found, uint32_t& digit,
+                                           uint32_t& above)
 {
-    constexpr uint32_t PER = EV_BINS / EV_NT;
+    constexpr uint32_t PER = EV_BINS / NT;
     const uint32_t t = threadIdx.x;
     uint32_t c[PER], mine = 0, total;
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
-        const uint32_t bin = EV_BINS - 1 - (t * PER + j);
-        c[j] = 0;
-        for (uint32_t k = 0; k < copies; ++k) c[j] += s_bins[k * EV_BINS + bin];
+        c[j] = count(EV_BINS - 1 - (t * PER + j));
         mine += c[j];
     }
-    uint32_t before = block_excl_scan<EV_NT>(mine, s_scan, total);
+    uint32_t before = block_excl_scan<NT>(mine, s_scan, total);
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         if (before < n && n <= before + c[j]) {
@@ -128,168 +128,553 @@ __device__ __forceinline__ void find_digit(const uint32_t* s_bins, uint32_t copi
     __syncthreads();
 }
 
-// A workgroup a request.
+// Four neighbouring values of a row from entry i, of which those behind `n` are not
+// looked at.
+template <class T>
+__device__ __forceinline__ void load4(const T* row, uint32_t i, uint32_t n, uint32_t room, bool wide, T (&x)[4])
+{
+    if (wide && i + 4 <= room) {
+        typedef T V __attribute__((ext_vector_type(4)));
+        const V v = *reinterpret_cast<const V*>(row + i);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) x[e] = i + e < n ? row[i + e] : T(0);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* row, uint32_t i, uint32_t on, bool wide, const T (&x)[4])
+{
+    if (wide && on == 15u) {
+        typedef T V __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<V*>(row + i) = V{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if ((on >> e) & 1u) row[i + e] = x[e];
+    }
+}
+
+// The places in the order of entries i .. i + 3 of request r (0 behind its last).
+__device__ __forceinline__ void keys4(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t i, uint32_t len,
+                                      uint32_t (&key)[4])
+{
+    if (i >= len) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) key[e] = 0u;
+        return;
+    }
+    float w[4];
+    load4(a.weights + r * a.weights_stride, i, len, a.room, a.wide, w);
+    int32_t p[4] = {0, 0, 0, 0};
+    if (i < ages.kept) load4(ages.row, i, ages.kept, a.room, a.wide, p);
+    uint32_t pinned = 0;
+    if (a.pins) {
+        if (a.page_lg >= 2) {  // four neighbours lie in one page and one word
+            const int32_t slot = slot_at(a, r, i);
+            if (slot >= 0 && static_cast<uint32_t>(slot) < a.pinned.end)
+                pinned = a.pinned.word(static_cast<uint32_t>(slot) >> 5) >> (slot & 31);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const int32_t slot = i + e < len ? slot_at(a, r, i + e) : -1;
+                if (slot >= 0 && static_cast<uint32_t>(slot) < a.pinned.end)
+                    pinned |= ((a.pinned.word(static_cast<uint32_t>(slot) >> 5) >> (slot & 31)) & 1u) << e;
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        const int64_t at = i + e < ages.kept ? static_cast<int64_t>(p[e]) : ages.first + i + e;
+        key[e] = i + e >= len ? 0u : ages.safe(at) || ((pinned >> e) & 1u) ? EV_SAFE : weight_order(w[e]);
+    }
+}
+
+// Bits e of the entries i + e < m of four.
+__device__ __forceinline__ uint32_t below4(uint32_t i, uint32_t m)
+{
+    return i >= m ? 0u : m - i >= 4 ? 15u : (1u << (m - i)) - 1u;
+}
+
+// Which of four stay: those above `last`, the safe ones, and of those that equal it the
+// ones before whom fewer than `ties` do; tie: how many do before the first.
+__device__ __forceinline__ uint32_t stays4(const uint32_t (&key)[4], uint32_t in, uint32_t last, uint32_t ties, uint32_t tie)
+{
+    uint32_t stay = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        const bool eq = key[e] == last && ((in >> e) & 1u) && last != EV_SAFE;
+        stay |= (key[e] > last || key[e] == EV_SAFE || (eq && tie < ties) ? 1u : 0u) << e;
+        tie += eq ? 1u : 0u;
+    }
+    return stay & in;
+}
+
+__device__ __forceinline__ uint32_t ties4(const uint32_t (&key)[4], uint32_t in, uint32_t last)
+{
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) n += key[e] == last && ((in >> e) & 1u) && last != EV_SAFE ? 1u : 0u;
+    return n;
+}
+
+// What lies in the entries `on` of four from i afterwards, where they stay.
+__device__ __forceinline__ void keep4(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t i, uint32_t len, uint32_t on)
+{
+    if (!on) return;
+    float w[4];
+    load4(a.weights + r * a.weights_stride, i, len, a.room, a.wide, w);
+    store4(a.weights_out + r * a.weights_out_stride, i, on, a.wide, w);
+    if (a.positions_out) {
+        int32_t p[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) p[e] = static_cast<int32_t>(ages.first + i + e);
+        if (i < ages.kept) {
+            int32_t x[4];
+            load4(ages.row, i, ages.kept, a.room, a.wide, x);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) p[e] = i + e < ages.kept ? x[e] : p[e];
+        }
+        store4(a.positions_out + r * a.positions_out_stride, i, on, a.wide, p);
+    }
+}
+
+// Entry `from` goes to place `to`.
+__device__ __forceinline__ int2 move_entry(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t from, uint32_t to)
+{
+    a.weights_out[r * a.weights_out_stride + to] = a.weights[r * a.weights_stride + from];
+    if (a.positions_out)
+        a.positions_out[r * a.positions_out_stride + to] = static_cast<int32_t>(ages.position(from));
+    return make_int2(slot_at(a, r, from), slot_at(a, r, to));
+}
+
+// How many of the entries are safe, and how many stay in all.
+__device__ __forceinline__ uint32_t staying(uint32_t len, uint32_t keep, uint32_t n_safe)
+{
+    return keep >= len ? len : max(keep, n_safe);
+}
+
+constexpr uint64_t EV_WHOLE = 16 * EV_NT;  // entries of a request that one workgroup takes
+
+// A workgroup a request of at most E * EV_NT entries, whose places in the order stay in
+// registers: four neighbours a lane, 256 a wave at a time.
+template <uint32_t E>
 __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
 {
-    __shared__ uint32_t s_bins[EV_COPIES * EV_BINS];
-    __shared__ uint32_t s_scan[EV_WAVES], s_found[2], s_safe;
+    constexpr uint32_t ROWS = E / 4, WAVES = EV_NT / 64, HOLES = E * EV_NT / 2;
+    __shared__ uint32_t s_mem[EV_COPIES * EV_BINS > HOLES ? EV_COPIES * EV_BINS : HOLES];  // counts, then holes
+    __shared__ uint32_t s_scan[WAVES], s_found[2], s_of[2][WAVES];
     const uint32_t r = blockIdx.x, t = threadIdx.x, lane = __lane_id(), wave = t >> 6;
     const uint32_t len = request_len(a, r);
-    const uint32_t rows = (len + EV_ROW - 1) / EV_ROW, per_wave = (rows + EV_WAVES - 1) / EV_WAVES;
-    const uint32_t row0 = min(wave * per_wave, rows), row1 = min(row0 + per_wave, rows);
-    uint32_t* keys = a.keys + static_cast<uint64_t>(r) * a.keys_stride;
-    const float* weights = a.weights + r * a.weights_stride;
     const Ages ages(a, r, len);
     const uint32_t keep = static_cast<uint32_t>(max(a.keep[r], 0));
-    const bool all = keep >= len;
-    for (uint32_t i = t; i < EV_COPIES * EV_BINS; i += EV_NT) s_bins[i] = 0;
-    if (t == 0) s_safe = 0;
-    __syncthreads();
-
-    // Every entry's place in the order, and how many have each first digit.
-    if (!all) {
-        uint32_t n_safe = 0;
-        for (uint32_t row = row0; row < row1; ++row) {
+    const uint32_t i0 = wave * 64 * E + lane * 4;  // row j: from i0 + j * 256
+    uint32_t key[ROWS][4], n_safe = 0;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t i = row * EV_ROW + j * 64 + lane;
-                if (i >= len) continue;
-                bool safe = ages.safe(ages.position(i));
-                if (a.pins) {
-                    const int32_t slot = slot_at(a, r, i);
-                    if (slot >= 0 && static_cast<uint32_t>(slot) < a.pinned.end)
-                        safe |= (a.pinned.word(static_cast<uint32_t>(slot) >> 5) >> (slot & 31)) & 1u;
-                }
-                const uint32_t key = safe ? EV_SAFE : weight_order(weights[i]);
-                keys[i] = key;
-                n_safe += safe ? 1u : 0u;
-                if (!safe) atomicAdd(&s_bins[(wave % EV_COPIES) * EV_BINS + (key >> 21)], 1u);
-            }
-        }
-        n_safe = wave_sum(n_safe);
-        if (lane == 0) atomicAdd(&s_safe, n_safe);
-    }
+    for (uint32_t j = 0; j < ROWS; ++j) keys4(a, ages, r, i0 + j * 256, len, key[j]);
+    for (uint32_t i = t; i < EV_COPIES * EV_BINS; i += EV_NT) s_mem[i] = 0;
     __syncthreads();
-    const uint32_t n_safe = s_safe;
-    const uint32_t m = all ? len : max(keep, n_safe);
-    // Of the others, the m - n_safe largest stay: those above `last`, and the first `ties` that equal it.
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if (i0 + j * 256 + e >= len) continue;
+            n_safe += key[j][e] == EV_SAFE ? 1u : 0u;
+            if (key[j][e] != EV_SAFE) atomicAdd(&s_mem[wave % EV_COPIES * EV_BINS + (key[j][e] >> 21)], 1u);
+        }
+    n_safe = block_sum<EV_NT>(n_safe, s_scan);
+    const uint32_t m = staying(len, keep, n_safe);
+    // Of the others, the m - n_safe largest stay.
     uint32_t last = EV_SAFE, ties = 0;
-    if (!all && m > n_safe) {
-        uint32_t n = m - n_safe, digit, above, prefix;
-        find_digit(s_bins, EV_COPIES, n, s_scan, s_found, digit, above);
+    if (m == len) {
+        last = 0;
+        ties = len;
+    } else if (m > n_safe) {
+        uint32_t n = m - n_safe, digit, above;
+        find_digit<EV_NT>(
+            [&](uint32_t bin) {
+                uint32_t c = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < EV_COPIES; ++k) c += s_mem[k * EV_BINS + bin];
+                return c;
+            },
+            n, s_scan, s_found, digit, above);
         n -= above;
-        prefix = digit << 21;
+        last = digit << 21;
+#pragma unroll
         for (int shift = 10; shift >= 0; shift -= 10) {
             const uint32_t bits = shift == 10 ? 11 : 10, mask = (1u << bits) - 1u;
-            for (uint32_t i = t; i < EV_BINS; i += EV_NT) s_bins[i] = 0;
+            for (uint32_t i = t; i < EV_BINS; i += EV_NT) s_mem[i] = 0;
             __syncthreads();
-            for (uint32_t row = row0; row < row1; ++row) {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t i = row * EV_ROW + j * 64 + lane;
-                    if (i >= len) continue;
-                    const uint32_t key = keys[i];
-                    if (key != EV_SAFE && (key >> (shift + bits)) == (prefix >> (shift + bits)))
-                        atomicAdd(&s_bins[(key >> shift) & mask], 1u);
-                }
-            }
+            for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (i0 + j * 256 + e < len && key[j][e] >> (shift + bits) == last >> (shift + bits))
+                        atomicAdd(&s_mem[(key[j][e] >> shift) & mask], 1u);
             __syncthreads();
-            find_digit(s_bins, 1, n, s_scan, s_found, digit, above);
+            find_digit<EV_NT>([&](uint32_t bin) { return s_mem[bin]; }, n, s_scan, s_found, digit, above);
             n -= above;
-            prefix |= digit << shift;
+            last |= digit << shift;
         }
-        last = prefix;
         ties = n;
     }
-
-    // Which stay, wave by wave over even parts of the row: ties first, then holes and movers.
-    uint32_t tie0 = 0, hole0, move0, total;
-    auto each = [&](auto f) {
-        for (uint32_t row = row0; row < row1; ++row) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t i = row * EV_ROW + j * 64 + lane;
-                f(i, i < len ? (all ? EV_SAFE : keys[i]) : 0u, i < len);
-            }
-        }
-    };
-    const bool tied = ties != 0;
-    if (tied) {
+    // Which stay, and how many holes and movers lie before each lane's four: both counts and
+    // the ties' fit one word for a wave's 256.
+    uint32_t tie0 = 0;
+    if (ties && m < len) {
         uint32_t n = 0;
-        each([&](uint32_t, uint32_t key, bool in) { n += in && key == last ? 1u : 0u; });
+#pragma unroll
+        for (uint32_t j = 0; j < ROWS; ++j) n += ties4(key[j], below4(i0 + j * 256, len), last);
         n = wave_sum(n);
         if (lane == 0) s_scan[wave] = n;
         __syncthreads();
         for (uint32_t w = 0; w < wave; ++w) tie0 += s_scan[w];
-        __syncthreads();
     }
-    auto stays = [&](uint32_t key, bool in, uint32_t& tie) {
-        bool stay = in && (key > last || key == EV_SAFE);
-        if (tied) {
-            const bool eq = in && key == last;
-            const unsigned long long same = __ballot(eq);
-            stay |= eq && tie + lanes_below(same) < ties;
-            tie += static_cast<uint32_t>(__popcll(same));
+    uint32_t stay[ROWS], rank[ROWS], holes = 0, movers = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j) {
+        const uint32_t i = i0 + j * 256, in = below4(i, len), mine = below4(i, m);
+        uint32_t tie = tie0;
+        if (ties && m < len) {
+            const uint32_t n = ties4(key[j], in, last), upto = wave_incl_scan(n);
+            tie = tie0 + upto - n;
+            tie0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
         }
-        return stay;
-    };
-    {
-        uint32_t holes = 0, movers = 0, tie = tie0;
-        each([&](uint32_t i, uint32_t key, bool in) {
-            const bool stay = stays(key, in, tie);
-            holes += static_cast<uint32_t>(__popcll(__ballot(i < m && !stay)));
-            movers += static_cast<uint32_t>(__popcll(__ballot(i >= m && stay)));
-        });
-        hole0 = move0 = total = 0;
-        if (lane == 0) s_scan[wave] = holes | 0u;
-        __syncthreads();
-        for (uint32_t w = 0; w < EV_WAVES; ++w) {
-            if (w < wave) hole0 += s_scan[w];
-            total += s_scan[w];
-        }
-        __syncthreads();
-        if (lane == 0) s_scan[wave] = movers;
-        __syncthreads();
-        for (uint32_t w = 0; w < wave; ++w) move0 += s_scan[w];
+        stay[j] = stays4(key[j], in, last, ties, tie);
+        const uint32_t n = __popc(mine & ~stay[j]) | static_cast<uint32_t>(__popc(stay[j] & ~mine)) << 16;
+        const uint32_t upto = wave_incl_scan(n);
+        rank[j] = (holes | movers << 16) + upto - n;  // (of a wave: at most 64 E of either)
+        const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+        holes += all & 0xFFFFu;
+        movers += all >> 16;
     }
-    int2* moves = a.moves + r * a.moves_stride;
-    float* w_out = a.weights_out + r * a.weights_out_stride;
-    int32_t* p_out = a.positions_out ? a.positions_out + r * a.positions_out_stride : nullptr;
-    {
-        uint32_t hole = hole0, tie = tie0;
-        each([&](uint32_t i, uint32_t key, bool in) {
-            const bool stay = stays(key, in, tie);
-            const bool open = i < m && !stay;
-            const unsigned long long opens = __ballot(open);
-            if (open) moves[hole + lanes_below(opens)].y = static_cast<int32_t>(i);
-            hole += static_cast<uint32_t>(__popcll(opens));
-            if (i < m && stay) {
-                w_out[i] = weights[i];
-                if (p_out) p_out[i] = static_cast<int32_t>(ages.position(i));
-            }
-        });
-    }
-    __threadfence_block();
     __syncthreads();
-    {
-        uint32_t mover = move0, tie = tie0;
-        each([&](uint32_t i, uint32_t key, bool in) {
-            const bool stay = stays(key, in, tie);
-            const bool go = i >= m && stay;
-            const unsigned long long goes = __ballot(go);
-            if (go) {
-                const uint32_t j = mover + lanes_below(goes);
-                const uint32_t to = static_cast<uint32_t>(moves[j].y);
-                w_out[to] = weights[i];
-                if (p_out) p_out[to] = static_cast<int32_t>(ages.position(i));
-                moves[j] = make_int2(slot_at(a, r, i), slot_at(a, r, to));
-            }
-            mover += static_cast<uint32_t>(__popcll(goes));
-        });
+    if (lane == 0) {
+        s_of[0][wave] = holes;
+        s_of[1][wave] = movers;
+    }
+    __syncthreads();
+    uint32_t hole0 = 0, move0 = 0, total = 0;
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        hole0 += w < wave ? s_of[0][w] : 0u;
+        move0 += w < wave ? s_of[1][w] : 0u;
+        total += s_of[0][w];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j) {
+        const uint32_t i = i0 + j * 256, mine = below4(i, m);
+        uint32_t at = hole0 + (rank[j] & 0xFFFFu);
+        for (uint32_t open = mine & ~stay[j]; open; open &= open - 1u) s_mem[at++] = i + __ffs(open) - 1;
+        keep4(a, ages, r, i, len, mine & stay[j]);
+    }
+    __syncthreads();
+    int2* moves = a.moves + r * a.moves_stride;
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j) {
+        const uint32_t i = i0 + j * 256;
+        uint32_t at = move0 + (rank[j] >> 16);
+        for (uint32_t go = stay[j] & ~below4(i, m); go; go &= go - 1u, ++at)
+            moves[at] = move_entry(a, ages, r, i + __ffs(go) - 1, s_mem[at]);
     }
     if (t == 0) {
         a.len[r] = static_cast<int32_t>(m);
         a.n_moves[r] = static_cast<int32_t>(total);
+    }
+}
+
+// ---- long rows: a workgroup per segment ----------------------------------------------
+// The same in launches that leave one another their counts: keys and first digits
+// (sg_keys), the digit in which the last that stays lies (sg_digit), those that have it
+// (sg_split), which of them stay and where each segment's holes and movers begin
+// (sg_decide), and what lies where (sg_place); ev_finish then moves the weights.
+constexpr int SG_NT = 256;
+constexpr uint32_t SG_WAVES = SG_NT / 64;
+constexpr uint32_t SG_ROWS = 4;                             // of 256 entries, a wave's
+constexpr uint32_t SG_SIZE = SG_WAVES * SG_ROWS * 256;
+
+__global__ __launch_bounds__(SG_NT) void sg_keys(EvictArgs a)
+{
+    __shared__ uint32_t s_bins[2][EV_BINS];
+    __shared__ uint32_t s_scan[SG_WAVES];
+    const uint32_t r = blockIdx.x / a.segments, seg = blockIdx.x % a.segments, t = threadIdx.x;
+    const uint32_t lane = __lane_id(), wave = t >> 6, len = request_len(a, r);
+    if (seg * SG_SIZE >= len) return;
+    const Ages ages(a, r, len);
+    uint32_t key[SG_ROWS][4], n_safe = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j)
+        keys4(a, ages, r, seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, len, key[j]);
+    for (uint32_t i = t; i < EV_BINS; i += SG_NT) s_bins[0][i] = s_bins[1][i] = 0;
+    __syncthreads();
+    uint32_t* keys = a.keys + static_cast<uint64_t>(blockIdx.x) * SG_SIZE;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint32_t in = (wave * SG_ROWS + j) * 256 + lane * 4;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if (seg * SG_SIZE + in + e >= len) continue;
+            n_safe += key[j][e] == EV_SAFE ? 1u : 0u;
+            if (key[j][e] != EV_SAFE) atomicAdd(&s_bins[wave % 2][key[j][e] >> 21], 1u);
+        }
+        *reinterpret_cast<uint4*>(keys + in) = make_uint4(key[j][0], key[j][1], key[j][2], key[j][3]);
+    }
+    n_safe = block_sum<SG_NT>(n_safe, s_scan);
+    uint32_t* bins = a.bins + static_cast<uint64_t>(blockIdx.x) * (EV_BINS / 2);
+    for (uint32_t i = t; i < EV_BINS / 2; i += SG_NT)  // (a segment's counts are at most SG_SIZE)
+        bins[i] = (s_bins[0][2 * i] + s_bins[1][2 * i]) | (s_bins[0][2 * i + 1] + s_bins[1][2 * i + 1]) << 16;
+    if (t == 0) a.counts_of[blockIdx.x].w = n_safe;
+}
+
+// picked[2 r]: m, the digit, how many stay of those that have it, the request's segments.
+__global__ __launch_bounds__(EV_NT) void sg_digit(EvictArgs a)
+{
+    __shared__ uint32_t s_scan[EV_NT / 64], s_found[2];
+    const uint32_t r = blockIdx.x, t = threadIdx.x, len = request_len(a, r);
+    const uint32_t keep = static_cast<uint32_t>(max(a.keep[r], 0)), segments = (len + SG_SIZE - 1) / SG_SIZE;
+    const uint64_t seg0 = static_cast<uint64_t>(r) * a.segments;
+    uint32_t n_safe = 0;
+    for (uint32_t i = t; i < segments; i += EV_NT) n_safe += a.counts_of[seg0 + i].w;
+    n_safe = block_sum<EV_NT>(n_safe, s_scan);
+    const uint32_t m = staying(len, keep, n_safe);
+    uint32_t digit = EV_NO_DIGIT, above = 0;
+    if (m > n_safe) {
+        static_assert(EV_BINS == 2 * EV_NT, "a word of two counts per thread");
+        const uint32_t word = (EV_BINS - 1 - t * 2) / 2;
+        uint32_t lo = 0, hi = 0;
+        for (uint32_t i = 0; i < segments; ++i) {
+            const uint32_t x = a.bins[(seg0 + i) * (EV_BINS / 2) + word];
+            lo += x & 0xFFFFu;
+            hi += x >> 16;
+        }
+        find_digit<EV_NT>([&](uint32_t bin) { return bin & 1u ? hi : lo; }, m - n_safe, s_scan, s_found, digit, above);
+    }
+    if (t == 0) a.picked[2 * r] = make_uint4(m, digit, m > n_safe ? m - n_safe - above : 0u, segments);
+}
+
+// Rank of a lane's count among the workgroup's, wave by wave in order; s_wave: a slot a wave.
+__device__ __forceinline__ uint32_t wave_base(uint32_t mine, uint32_t* s_wave)
+{
+    __syncthreads();
+    if (__lane_id() == 0) s_wave[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    uint32_t base = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < SG_WAVES; ++w) base += w < threadIdx.x >> 6 ? s_wave[w] : 0u;
+    return base;
+}
+
+__device__ __forceinline__ void load_keys(const EvictArgs& a, uint32_t (&key)[SG_ROWS][4])
+{
+    const uint32_t* keys = a.keys + static_cast<uint64_t>(blockIdx.x) * SG_SIZE;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(keys + ((threadIdx.x >> 6) * SG_ROWS + j) * 256 + __lane_id() * 4);
+        key[j][0] = x.x;
+        key[j][1] = x.y;
+        key[j][2] = x.z;
+        key[j][3] = x.w;
+    }
+}
+
+// counts_of: the undecided, and of the others the holes and the movers.
+__global__ __launch_bounds__(SG_NT) void sg_split(EvictArgs a)
+{
+    __shared__ uint32_t s_wave[SG_WAVES], s_scan[SG_WAVES];
+    const uint32_t r = blockIdx.x / a.segments, seg = blockIdx.x % a.segments, lane = __lane_id(), wave = threadIdx.x >> 6;
+    const uint32_t len = request_len(a, r);
+    if (seg * SG_SIZE >= len) return;
+    uint32_t key[SG_ROWS][4], open[SG_ROWS], rank[SG_ROWS], n_open = 0, holes = 0, movers = 0;
+    load_keys(a, key);
+    const uint4 picked = a.picked[2 * r];
+    const uint32_t m = picked.x, digit = picked.y;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, in = below4(i, len), mine = below4(i, m);
+        uint32_t stay = 0;
+        open[j] = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            stay |= (key[j][e] >> 21 > digit ? 1u : 0u) << e;
+            open[j] |= (key[j][e] >> 21 == digit ? 1u : 0u) << e;
+        }
+        open[j] &= in;
+        stay &= in;
+        holes += __popc(mine & ~stay & ~open[j]);
+        movers += __popc(stay & ~mine);
+        const uint32_t n = __popc(open[j]), upto = wave_incl_scan(n);
+        rank[j] = n_open + upto - n;
+        n_open += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+    }
+    const uint32_t base = wave_base(n_open, s_wave);
+    uint2* to = a.undecided + static_cast<uint64_t>(blockIdx.x) * SG_SIZE;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4;
+        uint32_t at = base + rank[j];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if ((open[j] >> e) & 1u) to[at++] = make_uint2(key[j][e], i + e);
+    }
+    holes = block_sum<SG_NT>(holes, s_scan);
+    movers = block_sum<SG_NT>(movers, s_scan);
+    const uint32_t all = block_sum<SG_NT>(lane == 0 ? n_open : 0u, s_scan);
+    if (threadIdx.x == 0) a.counts_of[blockIdx.x] = make_uint4(all, holes, movers, 0);
+}
+
+// picked[2 r + 1]: the last key that stays and how many that equal it do, the moves.
+// from: the ties, holes and movers before each segment.
+__global__ __launch_bounds__(EV_NT) void sg_decide(EvictArgs a)
+{
+    constexpr uint32_t WAVES = EV_NT / 64;
+    __shared__ uint32_t s_bins[EV_BINS], s_scan[WAVES], s_found[2];
+    const uint32_t r = blockIdx.x, t = threadIdx.x, lane = __lane_id(), wave = t >> 6;
+    const uint4 picked = a.picked[2 * r];
+    const uint32_t m = picked.x, segments = picked.w;
+    const uint64_t seg0 = static_cast<uint64_t>(r) * a.segments;
+    uint32_t n = picked.z, last = EV_SAFE, ties = 0;
+    // a wave a segment, its undecided in order
+    auto each = [&](uint32_t seg, auto f) {
+        const uint2* from = a.undecided + (seg0 + seg) * SG_SIZE;
+        const uint32_t all = a.counts_of[seg0 + seg].x;
+        for (uint32_t i0 = 0; i0 < all; i0 += 64) {
+            const uint2 x = from[min(i0 + lane, all - 1)];
+            f(i0 + lane < all, x.x, x.y);
+        }
+    };
+    if (n) {
+        last = picked.y << 21;
+#pragma unroll
+        for (int shift = 10; shift >= 0; shift -= 10) {
+            const uint32_t bits = shift == 10 ? 11 : 10, mask = (1u << bits) - 1u;
+            uint32_t digit, above;
+            for (uint32_t i = t; i < EV_BINS; i += EV_NT) s_bins[i] = 0;
+            __syncthreads();
+            for (uint32_t seg = wave; seg < segments; seg += WAVES)
+                each(seg, [&](bool in, uint32_t key, uint32_t) {
+                    if (in && key >> (shift + bits) == last >> (shift + bits)) atomicAdd(&s_bins[(key >> shift) & mask], 1u);
+                });
+            __syncthreads();
+            find_digit<EV_NT>([&](uint32_t bin) { return s_bins[bin]; }, n, s_scan, s_found, digit, above);
+            n -= above;
+            last |= digit << shift;
+        }
+        ties = n;
+    }
+    // ties of each segment, then those before it
+    uint32_t base = 0, holes0 = 0, movers0 = 0;
+    for (uint32_t s0 = 0; s0 < segments; s0 += WAVES) {
+        const uint32_t seg = s0 + wave;
+        uint32_t mine = 0;
+        if (seg < segments)
+            each(seg, [&](bool in, uint32_t key, uint32_t) {
+                mine += static_cast<uint32_t>(__popcll(__ballot(in && key == last && ties)));
+            });
+        __syncthreads();
+        if (lane == 0) s_scan[wave] = mine;
+        __syncthreads();
+        uint32_t tie = base;
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            tie += w < wave ? s_scan[w] : 0u;
+            base += s_scan[w];
+        }
+        uint32_t holes = 0, movers = 0, run = tie;
+        if (seg < segments) {
+            const uint4 c = a.counts_of[seg0 + seg];
+            holes = c.y;
+            movers = c.z;
+            each(seg, [&](bool in, uint32_t key, uint32_t i) {
+                const unsigned long long same = __ballot(in && key == last && ties);
+                const uint32_t rank = run + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
+                const bool stay = key > last || (key == last && ties && rank < ties);
+                run += static_cast<uint32_t>(__popcll(same));
+                holes += static_cast<uint32_t>(__popcll(__ballot(in && !stay && i < m)));
+                movers += static_cast<uint32_t>(__popcll(__ballot(in && stay && i >= m)));
+            });
+        }
+        __syncthreads();
+        if (lane == 0) {
+            s_bins[wave] = holes;
+            s_bins[WAVES + wave] = movers;
+        }
+        __syncthreads();
+        uint32_t hole = holes0, move = movers0;
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            hole += w < wave ? s_bins[w] : 0u;
+            move += w < wave ? s_bins[WAVES + w] : 0u;
+            holes0 += s_bins[w];
+            movers0 += s_bins[WAVES + w];
+        }
+        if (lane == 0 && seg < segments) a.from[seg0 + seg] = make_uint4(tie, hole, move, 0);
+    }
+    if (t == 0) {
+        a.picked[2 * r + 1] = make_uint4(last, ties, holes0, 0);
+        a.len[r] = static_cast<int32_t>(m);
+        a.n_moves[r] = static_cast<int32_t>(holes0);
+    }
+}
+
+// What stays in its place; the moves as pairs of entries.
+__global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
+{
+    __shared__ uint32_t s_wave[SG_WAVES];
+    const uint32_t r = blockIdx.x / a.segments, seg = blockIdx.x % a.segments, lane = __lane_id(), wave = threadIdx.x >> 6;
+    const uint32_t len = request_len(a, r);
+    if (seg * SG_SIZE >= len) return;
+    const Ages ages(a, r, len);
+    uint32_t key[SG_ROWS][4];
+    load_keys(a, key);
+    const uint32_t m = a.picked[2 * r].x;
+    const uint4 picked = a.picked[2 * r + 1], from = a.from[blockIdx.x];
+    const uint32_t last = picked.x, ties = picked.y;
+    uint32_t tie0 = from.x;
+    if (ties) {
+        uint32_t n = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < SG_ROWS; ++j)
+            n += ties4(key[j], below4(seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, len), last);
+        tie0 += wave_base(wave_sum(n), s_wave);
+    }
+    uint32_t stay[SG_ROWS], rank[SG_ROWS], counts = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, in = below4(i, len), mine = below4(i, m);
+        uint32_t tie = tie0;
+        if (ties) {
+            const uint32_t n = ties4(key[j], in, last), upto = wave_incl_scan(n);
+            tie += upto - n;
+            tie0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+        }
+        stay[j] = stays4(key[j], in, last, ties, tie);
+        const uint32_t n = __popc(mine & ~stay[j]) | static_cast<uint32_t>(__popc(stay[j] & ~mine)) << 16;
+        const uint32_t upto = wave_incl_scan(n);
+        rank[j] = counts + upto - n;
+        counts += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+    }
+    const uint32_t base = wave_base(counts, s_wave);  // (at most SG_SIZE of either)
+    int2* moves = a.moves + r * a.moves_stride;
+#pragma unroll
+    for (uint32_t j = 0; j < SG_ROWS; ++j) {
+        const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, mine = below4(i, m);
+        uint32_t hole = from.y + ((base + rank[j]) & 0xFFFFu), move = from.z + ((base + rank[j]) >> 16);
+        for (uint32_t open = mine & ~stay[j]; open; open &= open - 1u) moves[hole++].y = static_cast<int32_t>(i + __ffs(open) - 1);
+        for (uint32_t go = stay[j] & ~mine; go; go &= go - 1u) moves[move++].x = static_cast<int32_t>(i + __ffs(go) - 1);
+        keep4(a, ages, r, i, len, mine & stay[j]);
+    }
+}
+
+// The moves' weights and slots.
+__global__ __launch_bounds__(SG_NT) void sg_finish(EvictArgs a)
+{
+    const uint32_t r = blockIdx.x / a.segments, len = request_len(a, r);
+    const uint32_t n = static_cast<uint32_t>(a.n_moves[r]);
+    const Ages ages(a, r, len);
+    int2* moves = a.moves + r * a.moves_stride;
+    for (uint32_t j = blockIdx.x % a.segments * SG_NT + threadIdx.x; j < n; j += a.segments * SG_NT) {
+        const int2 x = moves[j];
+        moves[j] = move_entry(a, ages, r, static_cast<uint32_t>(x.x), static_cast<uint32_t>(x.y));
     }
 }
 
@@ -435,20 +820,50 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     a.freed = p.d_freed;
     a.freed_cap = p.freed_cap;
     a.counts = p.d_counts;
-    a.keys_stride = (a.room + EV_ROW - 1) / EV_ROW * EV_ROW;
+    auto four = [](const void* p, uint64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 4 == 0; };
+    a.wide = four(p.d_weights, p.weights_stride) && four(p.d_weights_out, p.weights_out_stride) &&
+             (!p.d_positions || four(p.d_positions, p.positions_stride)) &&
+             (!p.d_positions_out || four(p.d_positions_out, p.positions_out_stride));
+    // One workgroup a request while its entries fit the registers.
+    const bool whole = room <= EV_WHOLE;
+    a.segments = whole ? 0 : static_cast<uint32_t>((room + SG_SIZE - 1) / SG_SIZE);
+    const uint64_t segments = static_cast<uint64_t>(a.segments) * p.n_requests;
+    if (segments >> 23) {  // a launch holds fewer than 2^32 threads
+        set_error("cr_paged_evict: too many positions for one call");
+        return CR_ERR_UNSUPPORTED;
+    }
     const bool direct = p.pinned && is_direct(p.pinned);
     const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
     Carver cv;
-    const size_t o_keys = cv.add(static_cast<size_t>(p.n_requests) * a.keys_stride * 4);
-    const size_t o_words = cv.add(p.pinned && !direct ? n_words * 4ull : 0);
+    const size_t o_keys = cv.add(segments * SG_SIZE * 4), o_open = cv.add(segments * SG_SIZE * 8);
+    const size_t o_bins = cv.add(segments * EV_BINS * 2), o_counts = cv.add(segments * 16), o_from = cv.add(segments * 16);
+    const size_t o_picked = cv.add(whole ? 0 : p.n_requests * 32ull);
+    const size_t o_words = cv.add(p.pinned && !direct ? std::max<size_t>(4, n_words * 4ull) : 0);
     Scratch sc;
-    CR_RET(sc.alloc(std::max<size_t>(256, cv.total), s));
+    if (cv.total) CR_RET(sc.alloc(cv.total, s));
     a.keys = sc.at<uint32_t>(o_keys);
+    a.undecided = sc.at<uint2>(o_open);
+    a.bins = sc.at<uint32_t>(o_bins);
+    a.counts_of = sc.at<uint4>(o_counts);
+    a.from = sc.at<uint4>(o_from);
+    a.picked = sc.at<uint4>(o_picked);
     if (p.pinned)
         CR_RET(set_bits(p.pinned, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                         &a.pinned));
     CR_TIMED("ev_pick", s);
-    ev_pick<<<p.n_requests, EV_NT, 0, s>>>(a);
+    const uint32_t n = p.n_requests, parts = static_cast<uint32_t>(segments);
+    if (room <= 4 * EV_NT) {
+        ev_pick<4><<<n, EV_NT, 0, s>>>(a);
+    } else if (room <= 16 * EV_NT) {
+        ev_pick<16><<<n, EV_NT, 0, s>>>(a);
+    } else {
+        sg_keys<<<parts, SG_NT, 0, s>>>(a);
+        sg_digit<<<n, EV_NT, 0, s>>>(a);
+        sg_split<<<parts, SG_NT, 0, s>>>(a);
+        sg_decide<<<n, EV_NT, 0, s>>>(a);
+        sg_place<<<parts, SG_NT, 0, s>>>(a);
+        sg_finish<<<parts, SG_NT, 0, s>>>(a);
+    }
     ev_free<<<p.n_requests, EF_NT, 0, s>>>(a);
     CR_LAUNCH_CHECK();
     return CR_OK;

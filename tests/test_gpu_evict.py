@@ -198,6 +198,24 @@ def test_evict_long(gpu, kv, keep):
     Problem(kv, keep, seed=8, weights="alike", recent=100).check(gpu, in_place=True)
 
 
+@pytest.mark.parametrize("weights", ["spread", "alike", "same", "odd"])
+@pytest.mark.parametrize("what", LENGTHS)
+def test_evict_short_requests_in_long_rows(gpu, what, weights):
+    """Rows with room for more than one workgroup looks at."""
+    _say("evict in long rows", what, weights)
+    Problem(*LENGTHS[what], seed=len(what), weights=weights, wide=1100, pinned=0.1).check(gpu)
+
+
+@pytest.mark.parametrize("weights", ["spread", "alike", "same", "odd"])
+@pytest.mark.parametrize("page", [1, 2, 64])
+def test_evict_long_rows_of_every_kind(gpu, weights, page):
+    _say("evict long rows", weights, page)
+    p = Problem([17000, 16385, 9000, 4096, 4097], [9000, 16384, 0, 4000, 10 ** 6], seed=13, weights=weights, page=page,
+                pinned=0.02, recent=77)
+    p.check(gpu)
+    p.check(gpu, in_place=True, pad=5)
+
+
 def test_evict_very_long(gpu):
     _say("evict very long")
     Problem([70001, 131072], [30000, 120000], seed=9, page=64, recent=500, pinned=0.01).check(gpu)
