@@ -8,6 +8,7 @@
 // [0, m) are filled from [m, L) in order, so that sources and destinations never
 // meet and every token in [0, m) that stays lies where it lay.
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.hpp"
 #include "set_bits.hpp"
@@ -128,21 +129,12 @@ __device__ __forceinline__ void find_digit(F count, uint32_t n, uint32_t* s_scan
     __syncthreads();
 }
 
-// Four neighbouring values of a row from entry i, of which those behind `n` are not
-// looked at.
-template <class T>
-__device__ __forceinline__ void load4(const T* row, uint32_t i, uint32_t n, uint32_t room, bool wide, T (&x)[4])
-{
-    if (wide && i + 4 <= room) {
-        typedef T V __attribute__((ext_vector_type(4)));
-        const V v = *reinterpret_cast<const V*>(row + i);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) x[e] = v[e];
-    } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) x[e] = i + e < n ? row[i + e] : T(0);
-    }
-}
+// Four neighbours each of ROWS parts of a request's row: entries first[j] + e.
+template <uint32_t ROWS>
+struct Entries {
+    float weight[ROWS][4];
+    int32_t position[ROWS][4];
+};
 
 template <class T>
 __device__ __forceinline__ void store4(T* row, uint32_t i, uint32_t on, bool wide, const T (&x)[4])
@@ -157,39 +149,108 @@ __device__ __forceinline__ void store4(T* row, uint32_t i, uint32_t on, bool wid
     }
 }
 
-// The places in the order of entries i .. i + 3 of request r (0 behind its last).
-__device__ __forceinline__ void keys4(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t i, uint32_t len,
-                                      uint32_t (&key)[4])
+// Weights and positions of entries i0 + j * 256 + e < len (len > 0; any values behind them).
+// No load waits for another: rows that can be read four at a time are read up to their end.
+template <uint32_t ROWS>
+__device__ __forceinline__ void load_entries(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t i0, uint32_t len,
+                                             Entries<ROWS>& x)
 {
-    if (i >= len) {
+    const float* weights = a.weights + r * a.weights_stride;
+    if (a.wide) {
+        typedef float VF __attribute__((ext_vector_type(4)));
+        typedef int32_t VI __attribute__((ext_vector_type(4)));
+        VF w[ROWS];
+        VI p[ROWS];
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) key[e] = 0u;
-        return;
-    }
-    float w[4];
-    load4(a.weights + r * a.weights_stride, i, len, a.room, a.wide, w);
-    int32_t p[4] = {0, 0, 0, 0};
-    if (i < ages.kept) load4(ages.row, i, ages.kept, a.room, a.wide, p);
-    uint32_t pinned = 0;
-    if (a.pins) {
-        if (a.page_lg >= 2) {  // four neighbours lie in one page and one word
-            const int32_t slot = slot_at(a, r, i);
-            if (slot >= 0 && static_cast<uint32_t>(slot) < a.pinned.end)
-                pinned = a.pinned.word(static_cast<uint32_t>(slot) >> 5) >> (slot & 31);
-        } else {
+        for (uint32_t j = 0; j < ROWS; ++j) w[j] = *reinterpret_cast<const VF*>(weights + min(i0 + j * 256, a.room - 4));
+        if (ages.kept) {
+#pragma unroll
+            for (uint32_t j = 0; j < ROWS; ++j) p[j] = *reinterpret_cast<const VI*>(ages.row + min(i0 + j * 256, a.room - 4));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < ROWS; ++j)
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
-                const int32_t slot = i + e < len ? slot_at(a, r, i + e) : -1;
-                if (slot >= 0 && static_cast<uint32_t>(slot) < a.pinned.end)
-                    pinned |= ((a.pinned.word(static_cast<uint32_t>(slot) >> 5) >> (slot & 31)) & 1u) << e;
+                x.weight[j][e] = w[j][e];
+                if (ages.kept) x.position[j][e] = p[j][e];
             }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) x.weight[j][e] = weights[min(i0 + j * 256 + e, len - 1)];
+        if (ages.kept) {
+#pragma unroll
+            for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) x.position[j][e] = ages.row[min(i0 + j * 256 + e, ages.kept - 1)];
         }
     }
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        const int64_t at = i + e < ages.kept ? static_cast<int64_t>(p[e]) : ages.first + i + e;
-        key[e] = i + e >= len ? 0u : ages.safe(at) || ((pinned >> e) & 1u) ? EV_SAFE : weight_order(w[e]);
+    for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t i = i0 + j * 256 + e;
+            if (i >= ages.kept) x.position[j][e] = static_cast<int32_t>(ages.first + i);
+        }
+}
+
+// The pinned ones of them, as bits.
+template <uint32_t ROWS>
+__device__ __forceinline__ void load_pinned(const EvictArgs& a, uint32_t r, uint32_t i0, uint32_t len, uint32_t (&on)[ROWS])
+{
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j) on[j] = 0;
+    if (!a.pins || a.pinned.end == 0) return;
+    const int32_t* table = a.table + r * a.table_stride;
+    constexpr uint32_t MOST = ROWS * 4;
+    auto look = [&](auto& word, auto& shift, auto& in, auto n_of, auto entry) {  // side by side
+        constexpr uint32_t N = decltype(n_of)::value;
+        uint32_t slot[N], x[N];
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            const uint32_t i = min(entry(j), len - 1), page = static_cast<uint32_t>(table[i >> a.page_lg]);
+            slot[j] = (page << a.page_lg) + (i & ((1u << a.page_lg) - 1u));
+            in[j] = page < a.n_pages && slot[j] < a.pinned.end;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            word[j] = in[j] ? slot[j] >> 5 : 0u;
+            shift[j] = slot[j] & 31u;
+        }
+        a.pinned.words(word, x);
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) word[j] = in[j] ? x[j] >> shift[j] : 0u;
+    };
+    if (a.page_lg >= 2) {  // four neighbours lie in one page and one word
+        uint32_t word[ROWS], shift[ROWS];
+        bool in[ROWS];
+        look(word, shift, in, std::integral_constant<uint32_t, ROWS>{}, [&](uint32_t j) { return i0 + j * 256; });
+#pragma unroll
+        for (uint32_t j = 0; j < ROWS; ++j) on[j] = word[j] & 15u;
+    } else {
+        uint32_t word[MOST], shift[MOST];
+        bool in[MOST];
+        look(word, shift, in, std::integral_constant<uint32_t, MOST>{},
+             [&](uint32_t j) { return i0 + j / 4 * 256 + j % 4; });
+#pragma unroll
+        for (uint32_t j = 0; j < MOST; ++j) on[j / 4] |= (word[j] & 1u) << (j % 4);
     }
+}
+
+// Their places in the order (0 behind the request's last).
+template <uint32_t ROWS>
+__device__ __forceinline__ void keys_of(const EvictArgs& a, const Ages& ages, uint32_t i0, uint32_t len, const Entries<ROWS>& x,
+                                        const uint32_t (&pinned)[ROWS], uint32_t (&key)[ROWS][4])
+{
+#pragma unroll
+    for (uint32_t j = 0; j < ROWS; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t i = i0 + j * 256 + e;
+            const int64_t at = i < ages.kept ? static_cast<int64_t>(x.position[j][e]) : ages.first + i;
+            key[j][e] = i >= len ? 0u : ages.safe(at) || ((pinned[j] >> e) & 1u) ? EV_SAFE : weight_order(x.weight[j][e]);
+        }
 }
 
 // Bits e of the entries i + e < m of four.
@@ -221,34 +282,51 @@ __device__ __forceinline__ uint32_t ties4(const uint32_t (&key)[4], uint32_t in,
 }
 
 // What lies in the entries `on` of four from i afterwards, where they stay.
-__device__ __forceinline__ void keep4(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t i, uint32_t len, uint32_t on)
+__device__ __forceinline__ void keep4(const EvictArgs& a, uint32_t r, uint32_t i, uint32_t on, const float (&weight)[4],
+                                      const int32_t (&position)[4])
 {
-    if (!on) return;
-    float w[4];
-    load4(a.weights + r * a.weights_stride, i, len, a.room, a.wide, w);
-    store4(a.weights_out + r * a.weights_out_stride, i, on, a.wide, w);
-    if (a.positions_out) {
-        int32_t p[4];
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) p[e] = static_cast<int32_t>(ages.first + i + e);
-        if (i < ages.kept) {
-            int32_t x[4];
-            load4(ages.row, i, ages.kept, a.room, a.wide, x);
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) p[e] = i + e < ages.kept ? x[e] : p[e];
-        }
-        store4(a.positions_out + r * a.positions_out_stride, i, on, a.wide, p);
-    }
+    store4(a.weights_out + r * a.weights_out_stride, i, on, a.wide, weight);
+    if (a.positions_out) store4(a.positions_out + r * a.positions_out_stride, i, on, a.wide, position);
 }
 
-// Entry `from` goes to place `to`.
-__device__ __forceinline__ int2 move_entry(const EvictArgs& a, const Ages& ages, uint32_t r, uint32_t from, uint32_t to)
+// Move j of request r: entry `from` goes to place `to`; of N of them (those that are
+// not there: the same twice), so that no look-up waits for another.
+template <uint32_t N>
+__device__ __forceinline__ void move_entries(const EvictArgs& a, const Ages& ages, uint32_t r, const uint32_t (&from)[N],
+                                             const uint32_t (&to)[N], const uint32_t (&j)[N], const bool (&on)[N])
 {
-    a.weights_out[r * a.weights_out_stride + to] = a.weights[r * a.weights_stride + from];
-    if (a.positions_out)
-        a.positions_out[r * a.positions_out_stride + to] = static_cast<int32_t>(ages.position(from));
-    return make_int2(slot_at(a, r, from), slot_at(a, r, to));
+    float w[N];
+    int32_t p[N], page[2][N];
+    const int32_t* table = a.table + r * a.table_stride;
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) {
+        w[k] = a.weights[r * a.weights_stride + from[k]];
+        page[0][k] = table[from[k] >> a.page_lg];
+        page[1][k] = table[to[k] >> a.page_lg];
+        p[k] = static_cast<int32_t>(ages.first + from[k]);
+    }
+    if (ages.kept) {
+        int32_t x[N];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) x[k] = ages.row[min(from[k], ages.kept - 1)];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) p[k] = from[k] < ages.kept ? x[k] : p[k];
+    }
+    const uint32_t mask = (1u << a.page_lg) - 1u;
+    auto slot = [&](int32_t page, uint32_t i) {
+        return static_cast<uint32_t>(page) < a.n_pages
+                   ? static_cast<int32_t>((static_cast<uint32_t>(page) << a.page_lg) + (i & mask))
+                   : -1;
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) {
+        if (!on[k]) continue;
+        a.weights_out[r * a.weights_out_stride + to[k]] = w[k];
+        if (a.positions_out) a.positions_out[r * a.positions_out_stride + to[k]] = p[k];
+        a.moves[r * a.moves_stride + j[k]] = make_int2(slot(page[0][k], from[k]), slot(page[1][k], to[k]));
+    }
 }
+constexpr uint32_t EV_MOVES = 4;  // a thread's at a time
 
 // How many of the entries are safe, and how many stay in all.
 __device__ __forceinline__ uint32_t staying(uint32_t len, uint32_t keep, uint32_t n_safe)
@@ -256,15 +334,16 @@ __device__ __forceinline__ uint32_t staying(uint32_t len, uint32_t keep, uint32_
     return keep >= len ? len : max(keep, n_safe);
 }
 
-constexpr uint64_t EV_WHOLE = 16 * EV_NT;  // entries of a request that one workgroup takes
+constexpr uint64_t EV_WHOLE = 16384;  // entries of a request that one workgroup takes
 
-// A workgroup a request of at most E * EV_NT entries, whose places in the order stay in
+// A workgroup a request of at most E * NT entries, whose places in the order stay in
 // registers: four neighbours a lane, 256 a wave at a time.
-template <uint32_t E>
-__global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
+template <int NT, uint32_t E>
+__global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
 {
-    constexpr uint32_t ROWS = E / 4, WAVES = EV_NT / 64, HOLES = E * EV_NT / 2;
+    constexpr uint32_t ROWS = E / 4, WAVES = NT / 64, HOLES = E * NT / 2;
     __shared__ uint32_t s_mem[EV_COPIES * EV_BINS > HOLES ? EV_COPIES * EV_BINS : HOLES];  // counts, then holes
+    __shared__ uint32_t s_movers[HOLES];
     __shared__ uint32_t s_scan[WAVES], s_found[2], s_of[2][WAVES];
     const uint32_t r = blockIdx.x, t = threadIdx.x, lane = __lane_id(), wave = t >> 6;
     const uint32_t len = request_len(a, r);
@@ -272,9 +351,23 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
     const uint32_t keep = static_cast<uint32_t>(max(a.keep[r], 0));
     const uint32_t i0 = wave * 64 * E + lane * 4;  // row j: from i0 + j * 256
     uint32_t key[ROWS][4], n_safe = 0;
+    Entries<ROWS> x;
+    if (len) load_entries<ROWS>(a, ages, r, i0, len, x);
+    if (keep >= len) {  // all stay
 #pragma unroll
-    for (uint32_t j = 0; j < ROWS; ++j) keys4(a, ages, r, i0 + j * 256, len, key[j]);
-    for (uint32_t i = t; i < EV_COPIES * EV_BINS; i += EV_NT) s_mem[i] = 0;
+        for (uint32_t j = 0; j < ROWS; ++j) keep4(a, r, i0 + j * 256, below4(i0 + j * 256, len), x.weight[j], x.position[j]);
+        if (t == 0) {
+            a.len[r] = static_cast<int32_t>(len);
+            a.n_moves[r] = 0;
+        }
+        return;
+    }
+    {
+        uint32_t pinned[ROWS];
+        load_pinned<ROWS>(a, r, i0, len, pinned);
+        for (uint32_t i = t; i < EV_COPIES * EV_BINS; i += NT) s_mem[i] = 0;
+        keys_of<ROWS>(a, ages, i0, len, x, pinned, key);
+    }
     __syncthreads();
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j)
@@ -284,16 +377,13 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
             n_safe += key[j][e] == EV_SAFE ? 1u : 0u;
             if (key[j][e] != EV_SAFE) atomicAdd(&s_mem[wave % EV_COPIES * EV_BINS + (key[j][e] >> 21)], 1u);
         }
-    n_safe = block_sum<EV_NT>(n_safe, s_scan);
+    n_safe = block_sum<NT>(n_safe, s_scan);
     const uint32_t m = staying(len, keep, n_safe);
     // Of the others, the m - n_safe largest stay.
     uint32_t last = EV_SAFE, ties = 0;
-    if (m == len) {
-        last = 0;
-        ties = len;
-    } else if (m > n_safe) {
+    if (m > n_safe) {
         uint32_t n = m - n_safe, digit, above;
-        find_digit<EV_NT>(
+        find_digit<NT>(
             [&](uint32_t bin) {
                 uint32_t c = 0;
 #pragma unroll
@@ -306,7 +396,7 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
 #pragma unroll
         for (int shift = 10; shift >= 0; shift -= 10) {
             const uint32_t bits = shift == 10 ? 11 : 10, mask = (1u << bits) - 1u;
-            for (uint32_t i = t; i < EV_BINS; i += EV_NT) s_mem[i] = 0;
+            for (uint32_t i = t; i < EV_BINS; i += NT) s_mem[i] = 0;
             __syncthreads();
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j)
@@ -315,7 +405,7 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
                     if (i0 + j * 256 + e < len && key[j][e] >> (shift + bits) == last >> (shift + bits))
                         atomicAdd(&s_mem[(key[j][e] >> shift) & mask], 1u);
             __syncthreads();
-            find_digit<EV_NT>([&](uint32_t bin) { return s_mem[bin]; }, n, s_scan, s_found, digit, above);
+            find_digit<NT>([&](uint32_t bin) { return s_mem[bin]; }, n, s_scan, s_found, digit, above);
             n -= above;
             last |= digit << shift;
         }
@@ -324,7 +414,7 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
     // Which stay, and how many holes and movers lie before each lane's four: both counts and
     // the ties' fit one word for a wave's 256.
     uint32_t tie0 = 0;
-    if (ties && m < len) {
+    if (ties) {
         uint32_t n = 0;
 #pragma unroll
         for (uint32_t j = 0; j < ROWS; ++j) n += ties4(key[j], below4(i0 + j * 256, len), last);
@@ -338,7 +428,7 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
     for (uint32_t j = 0; j < ROWS; ++j) {
         const uint32_t i = i0 + j * 256, in = below4(i, len), mine = below4(i, m);
         uint32_t tie = tie0;
-        if (ties && m < len) {
+        if (ties) {
             const uint32_t n = ties4(key[j], in, last), upto = wave_incl_scan(n);
             tie = tie0 + upto - n;
             tie0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
@@ -366,18 +456,27 @@ __global__ __launch_bounds__(EV_NT) void ev_pick(EvictArgs a)
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) {
         const uint32_t i = i0 + j * 256, mine = below4(i, m);
-        uint32_t at = hole0 + (rank[j] & 0xFFFFu);
-        for (uint32_t open = mine & ~stay[j]; open; open &= open - 1u) s_mem[at++] = i + __ffs(open) - 1;
-        keep4(a, ages, r, i, len, mine & stay[j]);
+        const uint32_t open = mine & ~stay[j], go = stay[j] & ~mine;
+        uint32_t hole = hole0 + (rank[j] & 0xFFFFu), mover = move0 + (rank[j] >> 16);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if ((open >> e) & 1u) s_mem[hole++] = i + e;
+            if ((go >> e) & 1u) s_movers[mover++] = i + e;
+        }
+        keep4(a, r, i, mine & stay[j], x.weight[j], x.position[j]);
     }
     __syncthreads();
-    int2* moves = a.moves + r * a.moves_stride;
+    for (uint32_t j0 = t; j0 < total; j0 += EV_MOVES * NT) {
+        uint32_t from[EV_MOVES], to[EV_MOVES], at[EV_MOVES];
+        bool on[EV_MOVES];
 #pragma unroll
-    for (uint32_t j = 0; j < ROWS; ++j) {
-        const uint32_t i = i0 + j * 256;
-        uint32_t at = move0 + (rank[j] >> 16);
-        for (uint32_t go = stay[j] & ~below4(i, m); go; go &= go - 1u, ++at)
-            moves[at] = move_entry(a, ages, r, i + __ffs(go) - 1, s_mem[at]);
+        for (uint32_t i = 0; i < EV_MOVES; ++i) {
+            at[i] = min(j0 + i * NT, total - 1);
+            on[i] = j0 + i * NT < total;
+            from[i] = s_movers[at[i]];
+            to[i] = s_mem[at[i]];
+        }
+        move_entries<EV_MOVES>(a, ages, r, from, to, at, on);
     }
     if (t == 0) {
         a.len[r] = static_cast<int32_t>(m);
@@ -403,10 +502,12 @@ __global__ __launch_bounds__(SG_NT) void sg_keys(EvictArgs a)
     const uint32_t lane = __lane_id(), wave = t >> 6, len = request_len(a, r);
     if (seg * SG_SIZE >= len) return;
     const Ages ages(a, r, len);
-    uint32_t key[SG_ROWS][4], n_safe = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < SG_ROWS; ++j)
-        keys4(a, ages, r, seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, len, key[j]);
+    uint32_t key[SG_ROWS][4], pinned[SG_ROWS], n_safe = 0;
+    const uint32_t i0 = seg * SG_SIZE + wave * SG_ROWS * 256 + lane * 4;
+    Entries<SG_ROWS> x;
+    load_pinned<SG_ROWS>(a, r, i0, len, pinned);
+    load_entries<SG_ROWS>(a, ages, r, i0, len, x);
+    keys_of<SG_ROWS>(a, ages, i0, len, x, pinned, key);
     for (uint32_t i = t; i < EV_BINS; i += SG_NT) s_bins[0][i] = s_bins[1][i] = 0;
     __syncthreads();
     uint32_t* keys = a.keys + static_cast<uint64_t>(blockIdx.x) * SG_SIZE;
@@ -444,10 +545,16 @@ __global__ __launch_bounds__(EV_NT) void sg_digit(EvictArgs a)
         static_assert(EV_BINS == 2 * EV_NT, "a word of two counts per thread");
         const uint32_t word = (EV_BINS - 1 - t * 2) / 2;
         uint32_t lo = 0, hi = 0;
-        for (uint32_t i = 0; i < segments; ++i) {
-            const uint32_t x = a.bins[(seg0 + i) * (EV_BINS / 2) + word];
-            lo += x & 0xFFFFu;
-            hi += x >> 16;
+        constexpr uint32_t AHEAD = 8;
+        for (uint32_t i = 0; i < segments; i += AHEAD) {
+            uint32_t x[AHEAD];
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) x[k] = a.bins[(seg0 + min(i + k, segments - 1)) * (EV_BINS / 2) + word];
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                lo += i + k < segments ? x[k] & 0xFFFFu : 0u;
+                hi += i + k < segments ? x[k] >> 16 : 0u;
+            }
         }
         find_digit<EV_NT>([&](uint32_t bin) { return bin & 1u ? hi : lo; }, m - n_safe, s_scan, s_found, digit, above);
     }
@@ -625,7 +732,9 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
     if (seg * SG_SIZE >= len) return;
     const Ages ages(a, r, len);
     uint32_t key[SG_ROWS][4];
+    Entries<SG_ROWS> x;
     load_keys(a, key);
+    load_entries<SG_ROWS>(a, ages, r, seg * SG_SIZE + wave * SG_ROWS * 256 + lane * 4, len, x);
     const uint32_t m = a.picked[2 * r].x;
     const uint4 picked = a.picked[2 * r + 1], from = a.from[blockIdx.x];
     const uint32_t last = picked.x, ties = picked.y;
@@ -659,27 +768,19 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
     for (uint32_t j = 0; j < SG_ROWS; ++j) {
         const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, mine = below4(i, m);
         uint32_t hole = from.y + ((base + rank[j]) & 0xFFFFu), move = from.z + ((base + rank[j]) >> 16);
-        for (uint32_t open = mine & ~stay[j]; open; open &= open - 1u) moves[hole++].y = static_cast<int32_t>(i + __ffs(open) - 1);
-        for (uint32_t go = stay[j] & ~mine; go; go &= go - 1u) moves[move++].x = static_cast<int32_t>(i + __ffs(go) - 1);
-        keep4(a, ages, r, i, len, mine & stay[j]);
-    }
-}
-
-// The moves' weights and slots.
-__global__ __launch_bounds__(SG_NT) void sg_finish(EvictArgs a)
-{
-    const uint32_t r = blockIdx.x / a.segments, len = request_len(a, r);
-    const uint32_t n = static_cast<uint32_t>(a.n_moves[r]);
-    const Ages ages(a, r, len);
-    int2* moves = a.moves + r * a.moves_stride;
-    for (uint32_t j = blockIdx.x % a.segments * SG_NT + threadIdx.x; j < n; j += a.segments * SG_NT) {
-        const int2 x = moves[j];
-        moves[j] = move_entry(a, ages, r, static_cast<uint32_t>(x.x), static_cast<uint32_t>(x.y));
+        const uint32_t open = mine & ~stay[j], go = stay[j] & ~mine;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if ((open >> e) & 1u) moves[hole++].y = static_cast<int32_t>(i + e);
+            if ((go >> e) & 1u) moves[move++].x = static_cast<int32_t>(i + e);
+        }
+        keep4(a, r, i, mine & stay[j], x.weight[j], x.position[j]);
     }
 }
 
 // The pages that get free, requests in order: a workgroup a request, which counts
-// those of the requests before it.
+// those of the requests before it.  Of long rows, the moves' weights and slots too,
+// which a workgroup a segment shares.
 constexpr int EF_NT = 256;
 
 __device__ __forceinline__ uint32_t pages_freed(const EvictArgs& a, uint32_t r, uint32_t& first)
@@ -689,10 +790,28 @@ __device__ __forceinline__ uint32_t pages_freed(const EvictArgs& a, uint32_t r, 
     return static_cast<uint32_t>((request_len(a, r) + page - 1) >> a.page_lg) - first;
 }
 
-__global__ __launch_bounds__(EF_NT) void ev_free(EvictArgs a)
+__global__ __launch_bounds__(EF_NT) void ev_finish(EvictArgs a, uint32_t per)
 {
     __shared__ uint32_t s_sum[EF_NT / 64];
-    const uint32_t r = blockIdx.x, t = threadIdx.x;
+    const uint32_t r = blockIdx.x / per, part = blockIdx.x % per, t = threadIdx.x;
+    if (a.segments) {
+        const Ages ages(a, r, request_len(a, r));
+        const uint32_t n = static_cast<uint32_t>(a.n_moves[r]);
+        for (uint32_t j0 = part * EF_NT + t; j0 < n; j0 += EV_MOVES * per * EF_NT) {
+            uint32_t from[EV_MOVES], to[EV_MOVES], at[EV_MOVES];
+            bool on[EV_MOVES];
+#pragma unroll
+            for (uint32_t i = 0; i < EV_MOVES; ++i) {
+                on[i] = j0 + i * per * EF_NT < n;
+                at[i] = on[i] ? j0 + i * per * EF_NT : j0;
+                const int2 x = a.moves[r * a.moves_stride + at[i]];
+                from[i] = static_cast<uint32_t>(x.x);
+                to[i] = static_cast<uint32_t>(x.y);
+            }
+            move_entries<EV_MOVES>(a, ages, r, from, to, at, on);
+        }
+    }
+    if (part) return;
     const bool last = r + 1 == a.n_requests;
     uint32_t before = 0, moves = 0, first;
     for (uint32_t i = t; i < r; i += EF_NT) before += pages_freed(a, i, first);
@@ -723,35 +842,52 @@ struct MoveArgs {
 
 constexpr int MV_NT = 256;
 
-// Bound by memory.  A thread moves one piece of the keys and of the values at a time.
+// Bound by memory: a thread asks for MV_AHEAD pieces of the keys and of the values at
+// a time, past the caches.
+constexpr uint32_t MV_AHEAD = 2;
+
 template <class U>
 __global__ __launch_bounds__(MV_NT) void ev_move(MoveArgs a)
 {
     const uint32_t r = blockIdx.x / a.per, row = a.heads * a.units;
     const uint32_t n = static_cast<uint32_t>(min(max(a.n_moves[r], 0), static_cast<int32_t>(a.cap)));
     const int2* moves = a.moves + r * a.moves_stride;
-    const uint64_t pieces = static_cast<uint64_t>(n) * row;
-    for (uint64_t i = (blockIdx.x % a.per) * static_cast<uint64_t>(MV_NT) + threadIdx.x; i < pieces;
-         i += static_cast<uint64_t>(a.per) * MV_NT) {
-        const uint32_t j = static_cast<uint32_t>(i / row), in = static_cast<uint32_t>(i % row);
-        const uint32_t head = in / a.units, unit = in % a.units;
-        const int2 move = moves[j];
-        if (move.x < 0 || move.y < 0 || static_cast<uint32_t>(move.x) >= a.n_slots ||
-            static_cast<uint32_t>(move.y) >= a.n_slots)
-            continue;
-        const uint32_t mask = (1u << a.page_lg) - 1u;
-        U x[2];
+    const uint32_t step = a.per * MV_NT, i = blockIdx.x % a.per * MV_NT + threadIdx.x, mask = (1u << a.page_lg) - 1u;
+    uint64_t j = i / row;  // the thread's move, and its piece of it
+    uint32_t in = i % row;
+    while (j < n) {
+        U x[MV_AHEAD][2];
+        char* to[MV_AHEAD][2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-            x[c] = __builtin_nontemporal_load(reinterpret_cast<const U*>(
-                a.base[c] + (static_cast<uint32_t>(move.x) >> a.page_lg) * a.page[c] +
-                (static_cast<uint32_t>(move.x) & mask) * a.slot[c] + head * a.head[c] + unit * sizeof(U)));
+        for (uint32_t k = 0; k < MV_AHEAD; ++k) {
+            to[k][0] = to[k][1] = nullptr;
+            if (j < n) {
+                const uint32_t head = in / a.units, unit = in % a.units;
+                const int2 move = moves[j];
+                const uint32_t from = static_cast<uint32_t>(move.x), into = static_cast<uint32_t>(move.y);
+                if (move.x >= 0 && move.y >= 0 && from < a.n_slots && into < a.n_slots) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-            __builtin_nontemporal_store(
-                x[c], reinterpret_cast<U*>(a.base[c] + (static_cast<uint32_t>(move.y) >> a.page_lg) * a.page[c] +
-                                           (static_cast<uint32_t>(move.y) & mask) * a.slot[c] + head * a.head[c] +
-                                           unit * sizeof(U)));
+                    for (int c = 0; c < 2; ++c) {
+                        const uint64_t off = head * a.head[c] + unit * sizeof(U);
+                        x[k][c] = __builtin_nontemporal_load(reinterpret_cast<const U*>(
+                            a.base[c] + (from >> a.page_lg) * a.page[c] + (from & mask) * a.slot[c] + off));
+                        to[k][c] = a.base[c] + (into >> a.page_lg) * a.page[c] + (into & mask) * a.slot[c] + off;
+                    }
+                }
+            }
+            j += step / row;
+            in += step % row;
+            if (in >= row) {
+                in -= row;
+                ++j;
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < MV_AHEAD; ++k) {
+            if (!to[k][0]) continue;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) __builtin_nontemporal_store(x[k][c], reinterpret_cast<U*>(to[k][c]));
+        }
     }
 }
 
@@ -821,7 +957,7 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     a.freed_cap = p.freed_cap;
     a.counts = p.d_counts;
     auto four = [](const void* p, uint64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 4 == 0; };
-    a.wide = four(p.d_weights, p.weights_stride) && four(p.d_weights_out, p.weights_out_stride) &&
+    a.wide = room >= 4 && room % 4 == 0 && four(p.d_weights, p.weights_stride) && four(p.d_weights_out, p.weights_out_stride) &&
              (!p.d_positions || four(p.d_positions, p.positions_stride)) &&
              (!p.d_positions_out || four(p.d_positions_out, p.positions_out_stride));
     // One workgroup a request while its entries fit the registers.
@@ -852,19 +988,19 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
                         &a.pinned));
     CR_TIMED("ev_pick", s);
     const uint32_t n = p.n_requests, parts = static_cast<uint32_t>(segments);
-    if (room <= 4 * EV_NT) {
-        ev_pick<4><<<n, EV_NT, 0, s>>>(a);
-    } else if (room <= 16 * EV_NT) {
-        ev_pick<16><<<n, EV_NT, 0, s>>>(a);
+    if (room <= 4096) {
+        ev_pick<1024, 4><<<n, 1024, 0, s>>>(a);
+    } else if (whole) {
+        ev_pick<512, 32><<<n, 512, 0, s>>>(a);
     } else {
         sg_keys<<<parts, SG_NT, 0, s>>>(a);
         sg_digit<<<n, EV_NT, 0, s>>>(a);
         sg_split<<<parts, SG_NT, 0, s>>>(a);
         sg_decide<<<n, EV_NT, 0, s>>>(a);
         sg_place<<<parts, SG_NT, 0, s>>>(a);
-        sg_finish<<<parts, SG_NT, 0, s>>>(a);
     }
-    ev_free<<<p.n_requests, EF_NT, 0, s>>>(a);
+    const uint32_t per = whole ? 1 : a.segments;
+    ev_finish<<<n * per, EF_NT, 0, s>>>(a, per);
     CR_LAUNCH_CHECK();
     return CR_OK;
 }
@@ -905,9 +1041,9 @@ extern "C" int cr_paged_move(const int32_t* d_moves, uint32_t moves_cap, uint64_
         set_error("cr_paged_move: too many elements for one call");
         return CR_ERR_UNSUPPORTED;
     }
-    // About eight workgroups a CU, shared evenly by the requests.
+    // About 32 workgroups a CU, shared evenly by the requests, of which some have no moves.
     const uint64_t most = (moves_cap * row + MV_NT - 1) / MV_NT;
-    a.per = static_cast<uint32_t>(std::min<uint64_t>(most, std::max(1u, 8 * num_cus() / n_requests)));
+    a.per = static_cast<uint32_t>(std::min<uint64_t>(most, std::max(1u, 32 * num_cus() / n_requests)));
     const uint32_t grid = a.per * n_requests;
     hipStream_t s = as_stream(stream);
     CR_TIMED("ev_move", s);
