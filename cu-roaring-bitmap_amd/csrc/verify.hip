@@ -10,14 +10,16 @@
 //
 // Sums and exponentials are in 64 bits: a random number falls between two running
 // sums that differ by 1e-5 and less, and which side it falls on is the answer.
-// (gfx950 multiplies and adds 64 bits at the rate of 32.)
+// (gfx950 multiplies and adds 64 bits at the rate of 32.)  Shares below 2^-1000 of a
+// row's largest are none.
 //
 //   1. dv_sums: every row once, a wave per piece of DV_PIECE tokens: largest score, and
 //      the sum of e^((x - largest) / T).
-//   2. dv_rest: which drafts are accepted, from the pieces' sums; then the sums of
-//      max(p - q, 0) of the row where they end, again by pieces.  Without a drafting
-//      model's scores q is 1 for the drafted token, and the pieces of p do.
-//   3. dv_pick: the piece in which the running sum passes the mark, and the token in it.
+//   2. dv_norms: each row's largest score and sum, and whether its draft is accepted.
+//   3. dv_rest: the sums of max(p - q, 0), by pieces, of the row where the accepted ones
+//      end.  Without a drafting model's scores q is 1 for the drafted token, and the
+//      pieces of p do.
+//   4. dv_pick: the piece in which the running sum passes the mark, and the token in it.
 #include <algorithm>
 
 #include "internal.hpp"
@@ -34,6 +36,16 @@ constexpr uint32_t DV_UNIT = 8;                  // neighbouring tokens of a lan
 constexpr uint32_t DV_STEPS = 4;                 // times
 constexpr uint32_t DV_PIECE = 64 * DV_UNIT * DV_STEPS;
 
+struct Norm {  // of a row: p(v) = e^((x_v - top) / T) * part
+    double part;
+    float top;
+};
+
+struct RowState {
+    Norm p, q;
+    uint32_t accepted;  // whether the draft that follows the row is
+};
+
 struct VerifyArgs {
     const void* x;
     const void* draft;  // or nullptr
@@ -42,7 +54,8 @@ struct VerifyArgs {
     const int32_t* tokens;
     const int32_t* starts;
     const float* uniform;
-    double scale;        // log2(e) / temperature
+    double scale;        // 64 log2(e) / temperature
+    float reach;         // scores so far below the largest have no share
     const uint32_t* flat;  // [rows of bits_stride words, or one for all (0)], or nullptr
     uint64_t bits_stride;
     SetBits allowed;
@@ -54,98 +67,203 @@ struct VerifyArgs {
     // [2][n_rows][pieces]: the rows' pieces and the drafts'
     float* top;
     double* mass;
+    RowState* state;       // [n_rows]
     double* rest;          // [n_requests][pieces]
-    struct Decision* decided;  // [n_requests]
 };
 
-// 2^t for t <= 0: the power of two apart, and the series of e^y to y^11 for |y| <=
-// log(2) / 2, which leaves 7e-15 of it.  Far below 2^-1022, and for -inf, 0.
-__device__ __forceinline__ double exp2_64(double t)
+// 2^(i / 64)
+__device__ const double DV_POWERS[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
+
+__device__ __forceinline__ void load_powers(double* s_pow)
 {
-    t = fmax(t, -1100.0);  // (-inf, whose fraction would be NaN; NaN is taken for it)
-    const double n = rint(t), y = (t - n) * 0.693147180559945309417;
-    double e = 2.505210838544171877505e-8;
-    e = fma(e, y, 2.755731922398589065255e-7);
-    e = fma(e, y, 2.755731922398589065255e-6);
-    e = fma(e, y, 2.480158730158730158730e-5);
-    e = fma(e, y, 1.984126984126984126984e-4);
-    e = fma(e, y, 1.388888888888888888889e-3);
-    e = fma(e, y, 8.333333333333333333333e-3);
-    e = fma(e, y, 4.166666666666666666667e-2);
-    e = fma(e, y, 1.666666666666666666667e-1);
-    e = fma(e, y, 0.5);
-    e = fma(e, y, 1.0);
-    e = fma(e, y, 1.0);
-    return ldexp(e, static_cast<int>(n));
+    if (threadIdx.x < 64) s_pow[threadIdx.x] = DV_POWERS[threadIdx.x];
+    __syncthreads();
 }
 
-// e^((x - top) / T); of an infinite largest score, those that reach it share the mass.
-__device__ __forceinline__ double part_of(float x, float top, double scale)
-{
-    return x == top ? (top == -__builtin_inff() ? 0.0 : 1.0)
-                    : exp2_64((static_cast<double>(x) - static_cast<double>(top)) * scale);
-}
-
-__device__ __forceinline__ double wave_sum_f64(double v)
-{
+// e^((x - top) / T) of a row whose largest score is `top`: 2^(u / 64) with u rounded to a
+// whole number n, which is added to an exponent and looked up, and the rest |f| <= 1/2 by
+// the series of e^y to y^4, y = f log(2) / 64, which leaves 4e-14 of it.  Below 2^-1000 of
+// the largest, and for NaN and -inf, nothing; scores of +inf share the mass.
+struct Shares {
+    double scale, from;
+    float top, least;
+    __device__ __forceinline__ Shares(const VerifyArgs& a, float largest)
+    {
+        scale = a.scale;
+        top = largest;
+        from = static_cast<double>(largest);
+        least = fmaxf(largest - a.reach, -3.402823466e38f);
+    }
+    // Of a finite largest score, without a branch.
+    __device__ __forceinline__ double finite(float x, const double* s_pow) const
+    {
+        constexpr double ROUND = 6755399441055744.0;  // 1.5 * 2^52
+        const bool there = x >= least;
+        // (the difference first, which is exact: at low temperatures its factors are far above it)
+        const double u = (static_cast<double>(there ? x : top) - from) * scale, r = u + ROUND, f = u - (r - ROUND);
+        const int32_t n = static_cast<int32_t>(__double_as_longlong(r));
+        const uint64_t power = static_cast<uint64_t>(__double_as_longlong(s_pow[n & 63]));
+        const uint32_t hi = static_cast<uint32_t>(power >> 32) + (static_cast<uint32_t>(n >> 6) << 20);
+        const double p = __longlong_as_double(
+            static_cast<long long>(static_cast<uint64_t>(there ? hi : 0u) << 32 | (there ? static_cast<uint32_t>(power) : 0u)));
+        double q = fma(f, 0x1.3b2ab6fba4e77p-31, 0x1.c6b08d704a0c0p-23);
+        q = fma(f, q, 0x1.ebfbdff82c58fp-15);
+        q = fma(f, q, 0x1.62e42fefa39efp-7);
+        return fma(p * f, q, p);
+    }
+    __device__ __forceinline__ double operator()(float x, const double* s_pow) const
+    {
+        return top == __builtin_inff() ? (x == top ? 1.0 : 0.0) : finite(x, s_pow);
+    }
+    // Many at once: they are worked out side by side.
+    template <uint32_t U>
+    __device__ __forceinline__ void of(const float (&x)[U][DV_UNIT], const double* s_pow, double (&share)[U][DV_UNIT]) const
+    {
+        if (top == __builtin_inff()) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < DV_UNIT; ++e) share[u][e] = x[u][e] == top ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < DV_UNIT; ++e) share[u][e] = finite(x[u][e], s_pow);
+        }
+    }
+};
+
+// Another lane's value within the rows of 16 lanes, then across them; 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint32_t lo = static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b)), CTRL, ROWS, 0xF, false));
+    const uint32_t hi = static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b >> 32)), CTRL, ROWS, 0xF, false));
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
 }
 
+// Inclusive scan over a wave.
 __device__ __forceinline__ double wave_incl_scan_f64(double v)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(v, o, 64);
-        if (static_cast<int>(__lane_id()) >= o) v += x;
-    }
+    v += dpp_f64<0x111, 0xF>(v);
+    v += dpp_f64<0x112, 0xF>(v);
+    v += dpp_f64<0x114, 0xF>(v);
+    v += dpp_f64<0x118, 0xF>(v);
+    v += dpp_f64<0x142, 0xA>(v);
+    v += dpp_f64<0x143, 0xC>(v);
     return v;
+}
+
+__device__ __forceinline__ double lane_f64(double v, int lane)
+{
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(b)), lane));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(b >> 32)), lane));
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) { return lane_f64(wave_incl_scan_f64(v), 63); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_dpp(float v)
+{
+    const int b = static_cast<int>(__float_as_uint(v));
+    return fmaxf(v, __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(b, b, CTRL, ROWS, 0xF, false))));
 }
 
 __device__ __forceinline__ float wave_max(float v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = max_dpp<0x111, 0xF>(v);
+    v = max_dpp<0x112, 0xF>(v);
+    v = max_dpp<0x114, 0xF>(v);
+    v = max_dpp<0x118, 0xF>(v);
+    v = max_dpp<0x142, 0xA>(v);
+    v = max_dpp<0x143, 0xC>(v);
+    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), 63)));
 }
 
-// Tokens [first, first + DV_UNIT) of a row: -inf for those that are not there, may not
-// be used or are NaN.
-template <class E>
-__device__ __forceinline__ void load_scores(const typename E::Bits* row, uint32_t first, uint32_t vocab, uint32_t on,
-                                            float (&x)[DV_UNIT])
+// A lane's tokens of a piece: DV_UNIT neighbours from first + u * 64 * DV_UNIT on, for U values
+// of u; -inf for those that are not there, may not be used after row `row` or are NaN.  No
+// load waits for another.
+template <class E, uint32_t U>
+__device__ __forceinline__ void load_tokens(const VerifyArgs& a, const typename E::Bits* p, uint32_t row, uint32_t first,
+                                            float (&x)[U][DV_UNIT])
 {
     typedef typename E::Bits Bits;
     // rows may begin anywhere
     typedef Bits Wide __attribute__((ext_vector_type(DV_UNIT), aligned(sizeof(Bits))));
-    if (first + DV_UNIT <= vocab) {
-        const Wide w = __builtin_nontemporal_load(reinterpret_cast<const Wide*>(row + first));
+    constexpr uint32_t STEP = 64 * DV_UNIT;
+    uint32_t on[U];
 #pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) x[e] = E::up(w[e]);
+    for (uint32_t u = 0; u < U; ++u) on[u] = 0xFFFFFFFFu;
+    if (a.masked) {
+        const uint32_t last = (a.vocab - 1) / 32u;
+        uint32_t w[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) w[u] = min((first + u * STEP) / 32u, last);
+        if (a.flat) {
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) on[u] = a.flat[row * a.bits_stride + w[u]];
+        } else if (a.allowed.end) {
+            a.allowed.words(w, on);
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) on[u] = 0u;
+        }
+    }
+    if (__builtin_amdgcn_readfirstlane(first) + U * STEP <= a.vocab) {  // (the first lane's are the first)
+        Wide w[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) w[u] = __builtin_nontemporal_load(reinterpret_cast<const Wide*>(p + first + u * STEP));
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) x[u][e] = E::up(w[u][e]);
     } else {
 #pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) x[e] = first + e < vocab ? E::up(row[first + e]) : 0.0f;
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) {
+                const uint32_t at = first + u * STEP + e;
+                const float v = E::up(p[min(at, a.vocab - 1)]);
+                x[u][e] = at < a.vocab ? v : -__builtin_inff();
+            }
     }
 #pragma unroll
-    for (uint32_t e = 0; e < DV_UNIT; ++e) x[e] = (on >> e) & 1u && x[e] == x[e] ? x[e] : -__builtin_inff();
-}
-
-// Which of tokens [first, first + DV_UNIT) are there and may be used after row `row`.
-__device__ __forceinline__ uint32_t allowed_unit(const VerifyArgs& a, uint64_t row, uint32_t first)
-{
-    if (first >= a.vocab) return 0u;
-    uint32_t on = first + DV_UNIT <= a.vocab ? 0xFFu : (1u << (a.vocab - first)) - 1u;
-    if (a.masked) {
-        const uint32_t word = a.flat ? a.flat[row * a.bits_stride + first / 32u] : a.allowed.word(first / 32u);
-        on &= word >> (first % 32u);
-    }
-    return on;
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t e = 0; e < DV_UNIT; ++e) {
+            const bool may = !a.masked || (on[u] >> ((first + e) % 32u)) & 1u;
+            x[u][e] = may && x[u][e] == x[u][e] ? x[u][e] : -__builtin_inff();
+        }
 }
 
 __device__ __forceinline__ bool is_allowed(const VerifyArgs& a, uint64_t row, uint32_t token)
 {
-    return (allowed_unit(a, row, token / DV_UNIT * DV_UNIT) >> (token % DV_UNIT)) & 1u;
+    if (!a.masked) return true;
+    const uint32_t w = token / 32u;
+    const uint32_t word = a.flat ? a.flat[row * a.bits_stride + w] : a.allowed.end ? a.allowed.word(w) : 0u;
+    return (word >> (token % 32u)) & 1u;
 }
 
 struct RequestRows {
@@ -161,35 +279,56 @@ __device__ __forceinline__ RequestRows rows_of(const VerifyArgs& a, uint32_t r)
     return {static_cast<uint32_t>(r0), rows ? rows - 1 : 0u, rows == 0};
 }
 
+// Whether a request ends with this row, after which nothing is drafted: a wave looks at 64
+// starts at a time.
+__device__ __forceinline__ bool is_last(const VerifyArgs& a, uint32_t row)
+{
+    const int32_t next = static_cast<int32_t>(row) + 1;
+    uint32_t lo = 0;
+    for (uint32_t len = a.n_requests + 1; len > 1;) {  // the last start at or before the next row is among these
+        const uint32_t step = (len + 63) / 64, i = lo + __lane_id() * step;
+        const unsigned long long m = __ballot(__lane_id() * step < len && i <= a.n_requests && a.starts[min(i, a.n_requests)] <= next);
+        lo += (max(static_cast<uint32_t>(__popcll(m)), 1u) - 1) * step;
+        len = step;
+    }
+    return a.starts[min(lo, a.n_requests)] == next;
+}
+
 // Every row's pieces; the drafting model's rows behind the model's.
 template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
 {
+    __shared__ double s_pow[64];
     const uint32_t lane = __lane_id(), wave = blockIdx.x * DV_WAVES + (threadIdx.x >> 6);
-    const uint32_t at = wave / a.pieces, piece = wave % a.pieces;
+    load_powers(s_pow);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(wave / a.pieces), piece = __builtin_amdgcn_readfirstlane(wave % a.pieces);
     if (at >= (a.draft ? 2 : 1) * a.n_rows) return;
     const bool drafted = at >= a.n_rows;
     const uint32_t row = drafted ? at - a.n_rows : at;
+    if (drafted && is_last(a, row)) return;
     const auto* p = static_cast<const typename E::Bits*>(drafted ? a.draft : a.x) +
                     row * (drafted ? a.draft_row : a.x_row);
     float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
-    uint32_t on[DV_STEPS];
+    load_tokens<E, DV_STEPS>(a, p, row, piece * DV_PIECE + lane * DV_UNIT, x);
 #pragma unroll
     for (uint32_t u = 0; u < DV_STEPS; ++u)
-        on[u] = allowed_unit(a, row, piece * DV_PIECE + (u * 64 + lane) * DV_UNIT);
-#pragma unroll
-    for (uint32_t u = 0; u < DV_STEPS; ++u) {
-        load_scores<E>(p, piece * DV_PIECE + (u * 64 + lane) * DV_UNIT, a.vocab, on[u], x[u]);
 #pragma unroll
         for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
-    }
     top = wave_max(top);
     double mass = 0.0;
     if (top > -__builtin_inff()) {
+        const Shares share(a, top);
+        if (top == __builtin_inff()) {
 #pragma unroll
-        for (uint32_t u = 0; u < DV_STEPS; ++u)
+            for (uint32_t u = 0; u < DV_STEPS; ++u)
 #pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) mass += part_of(x[u][e], top, a.scale);
+                for (uint32_t e = 0; e < DV_UNIT; ++e) mass += x[u][e] == top ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < DV_STEPS; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < DV_UNIT; ++e) mass += share.finite(x[u][e], s_pow);
+        }
     }
     mass = wave_sum_f64(mass);
     if (lane == 0) {
@@ -198,13 +337,8 @@ __global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
     }
 }
 
-struct Norm {  // of a row: p(v) = e^((x_v - top) / T) * part
-    float top;
-    double part;
-};
-
-// A wave's work: the pieces joined in a fixed order.
-__device__ __forceinline__ Norm norm_of(const VerifyArgs& a, uint32_t at)
+// A wave's work: a row's pieces joined in a fixed order.
+__device__ __forceinline__ Norm norm_of(const VerifyArgs& a, uint32_t at, const double* s_pow)
 {
     const float* top = a.top + static_cast<uint64_t>(at) * a.pieces;
     const double* mass = a.mass + static_cast<uint64_t>(at) * a.pieces;
@@ -212,91 +346,105 @@ __device__ __forceinline__ Norm norm_of(const VerifyArgs& a, uint32_t at)
     for (uint32_t i = __lane_id(); i < a.pieces; i += 64) m = fmaxf(m, top[i]);
     m = wave_max(m);
     double sum = 0.0;
-    for (uint32_t i = __lane_id(); i < a.pieces; i += 64)
-        if (mass[i] > 0.0) sum += mass[i] * part_of(top[i], m, a.scale);
+    if (m > -__builtin_inff()) {
+        const Shares share(a, m);
+        for (uint32_t i = __lane_id(); i < a.pieces; i += 64) sum += mass[i] * share(top[i], s_pow);
+    }
     sum = wave_sum_f64(sum);
-    return {m, sum > 0.0 ? 1.0 / sum : 0.0};
+    return {sum > 0.0 ? 1.0 / sum : 0.0, m};
+}
+
+// The share of one token.
+template <class E>
+__device__ __forceinline__ double share_of(const VerifyArgs& a, const void* x, uint64_t row_stride, uint32_t row,
+                                           uint32_t token, Norm n, const double* s_pow)
+{
+    const float v = E::up(static_cast<const typename E::Bits*>(x)[row * row_stride + token]);
+    return v == v && n.part > 0.0 ? Shares(a, n.top)(v, s_pow) * n.part : 0.0;
+}
+
+// A wave a row: what its shares are divided by, and whether the draft behind it is accepted.
+template <class E>
+__global__ __launch_bounds__(64) void dv_norms(VerifyArgs a)
+{
+    __shared__ double s_pow[64];
+    const uint32_t row = blockIdx.x;
+    load_powers(s_pow);
+    RowState s{};
+    const bool last = row + 1 >= a.n_rows || is_last(a, row);
+    const int32_t token = last ? -1 : a.tokens[row + 1];
+    const bool there = token >= 0 && static_cast<uint32_t>(token) < a.vocab && is_allowed(a, row, static_cast<uint32_t>(token));
+    s.p = norm_of(a, row, s_pow);
+    if (!last) {
+        double p = 0.0, q = 1.0;
+        if (a.draft) s.q = norm_of(a, a.n_rows + row, s_pow);
+        if (there) {
+            p = share_of<E>(a, a.x, a.x_row, row, static_cast<uint32_t>(token), s.p, s_pow);
+            if (a.draft) q = share_of<E>(a, a.draft, a.draft_row, row, static_cast<uint32_t>(token), s.q, s_pow);
+            s.accepted = static_cast<double>(a.uniform[row]) * q < p ? 1u : 0u;
+        }
+    }
+    if (threadIdx.x == 0) a.state[row] = s;
 }
 
 struct Decision {
     uint32_t row, accepted;
-    uint32_t rejected;  // whether the draft there was: its token
+    bool rejected;  // the draft that there was
     int32_t token;
     Norm p, q;
 };
 
-// p and q of one token.
-template <class E>
-__device__ __forceinline__ double share_of(const VerifyArgs& a, const void* x, uint64_t row_stride, uint32_t row,
-                                           uint32_t token, Norm n)
+// Where request r's accepted drafts end; a wave's work.
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& rows)
 {
-    const float v = E::up(static_cast<const typename E::Bits*>(x)[row * row_stride + token]);
-    return v == v && n.part > 0.0 ? part_of(v, n.top, a.scale) * n.part : 0.0;
-}
-
-// How many drafts of request r are accepted.  A workgroup's work, a wave a draft at a time.
-template <class E>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& rows, Decision* s_waves)
-{
-    const uint32_t wave = threadIdx.x >> 6;
-    Decision d{};
-    for (uint32_t j0 = 0;; j0 += DV_WAVES) {
-        const uint32_t j = min(j0 + wave, rows.drafts), row = rows.first + j;
-        d.row = row;
-        d.accepted = j;
-        d.rejected = 0;
-        d.token = -1;
-        d.p = norm_of(a, row);
-        d.q = {0.0f, 0.0};
-        if (j < rows.drafts) {
-            d.token = a.tokens[row + 1];
-            double p = 0.0, q = 1.0;
-            if (a.draft) d.q = norm_of(a, a.n_rows + row);
-            const bool there = d.token >= 0 && static_cast<uint32_t>(d.token) < a.vocab &&
-                               is_allowed(a, row, static_cast<uint32_t>(d.token));
-            if (there) {
-                p = share_of<E>(a, a.x, a.x_row, row, static_cast<uint32_t>(d.token), d.p);
-                if (a.draft) q = share_of<E>(a, a.draft, a.draft_row, row, static_cast<uint32_t>(d.token), d.q);
-            }
-            d.rejected = there && static_cast<double>(a.uniform[row]) * q < p ? 0u : 1u;
+    Decision d;
+    d.accepted = rows.drafts;
+    for (uint32_t j0 = 0; j0 < rows.drafts; j0 += 64) {
+        const uint32_t j = j0 + __lane_id();
+        const unsigned long long no = __ballot(j < rows.drafts && !a.state[rows.first + min(j, rows.drafts - 1)].accepted);
+        if (no) {
+            d.accepted = j0 + static_cast<uint32_t>(__ffsll(no)) - 1;
+            break;
         }
-        if (__lane_id() == 0) s_waves[wave] = d;
-        __syncthreads();
-        // the first that ends it
-        uint32_t end = DV_WAVES;
-        for (uint32_t w = 0; w < DV_WAVES; ++w)
-            if (end == DV_WAVES && (s_waves[w].rejected || s_waves[w].accepted == rows.drafts)) end = w;
-        if (end < DV_WAVES) d = s_waves[end];
-        __syncthreads();
-        if (end < DV_WAVES) return d;
     }
+    d.row = rows.first + d.accepted;
+    d.rejected = d.accepted < rows.drafts;
+    const RowState s = a.state[d.row];
+    d.p = s.p;
+    d.q = s.q;
+    d.token = d.rejected ? a.tokens[d.row + 1] : -1;
+    return d;
 }
 
-// max(p - q, 0), or p behind the last draft, of a lane's tokens from `first`.
-template <class E>
-__device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, uint32_t first, bool plain,
-                                        double (&rest)[DV_UNIT])
+// max(p - q, 0), or p behind the last draft (or where `plain`), of a lane's tokens from `first`.
+template <class E, uint32_t U>
+__device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, uint32_t first, bool plain, const double* s_pow,
+                                        double (&rest)[U][DV_UNIT])
 {
     // each product rounded by itself, so that equal shares leave nothing
 #pragma clang fp contract(off)
-    const uint32_t on = allowed_unit(a, d.row, first);
-    float x[DV_UNIT], y[DV_UNIT];
-    if (first < a.vocab) {
-        load_scores<E>(static_cast<const typename E::Bits*>(a.x) + d.row * a.x_row, first, a.vocab, on, x);
-        if (a.draft && d.rejected && !plain)
-            load_scores<E>(static_cast<const typename E::Bits*>(a.draft) + d.row * a.draft_row, first, a.vocab, on, y);
-    }
+    float x[U][DV_UNIT], y[U][DV_UNIT];
+    const bool both = a.draft && d.rejected && !plain && d.q.part > 0.0;
+    load_tokens<E, U>(a, static_cast<const typename E::Bits*>(a.x) + d.row * a.x_row, d.row, first, x);
+    if (both) load_tokens<E, U>(a, static_cast<const typename E::Bits*>(a.draft) + d.row * a.draft_row, d.row, first, y);
+    Shares(a, d.p.top).of(x, s_pow, rest);  // (no share where the score is -inf)
+    const double p_part = d.p.part, q_part = d.q.part;
+    if (both) {
+        double q[U][DV_UNIT];
+        Shares(a, d.q.top).of(y, s_pow, q);
 #pragma unroll
-    for (uint32_t e = 0; e < DV_UNIT; ++e) {
-        rest[e] = 0.0;
-        if (first >= a.vocab || !((on >> e) & 1u) || d.p.part == 0.0) continue;
-        rest[e] = part_of(x[e], d.p.top, a.scale) * d.p.part;
-        if (!d.rejected || plain) continue;
-        if (a.draft) {
-            if (d.q.part > 0.0) rest[e] = fmax(rest[e] - part_of(y[e], d.q.top, a.scale) * d.q.part, 0.0);
-        } else if (static_cast<int32_t>(first + e) == d.token) {
-            rest[e] = 0.0;
-        }
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) rest[u][e] = fmax(rest[u][e] * p_part - q[u][e] * q_part, 0.0);
+    } else {
+        const bool drop = !a.draft && d.rejected && !plain;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) {
+                const bool is = drop && static_cast<int32_t>(first + u * 64 * DV_UNIT + e) == d.token;
+                rest[u][e] = is ? 0.0 : rest[u][e] * p_part;
+            }
     }
 }
 
@@ -304,40 +452,33 @@ __device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, 
 template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_rest(VerifyArgs a, uint32_t groups)
 {
-    __shared__ Decision s_waves[DV_WAVES];
-    const uint32_t r = blockIdx.x / groups, part = blockIdx.x % groups, lane = __lane_id();
+    __shared__ double s_pow[64];
+    const uint32_t r = blockIdx.x / groups, lane = __lane_id();
+    const uint32_t piece = __builtin_amdgcn_readfirstlane(blockIdx.x % groups * DV_WAVES + (threadIdx.x >> 6));
     const RequestRows rows = rows_of(a, r);
     if (rows.none) return;
-    const Decision d = decide<E>(a, rows, s_waves);
-    if (part == 0 && threadIdx.x == 0) a.decided[r] = d;
-    const uint32_t piece = part * DV_WAVES + (threadIdx.x >> 6);
+    load_powers(s_pow);
     if (piece >= a.pieces) return;
+    const Decision d = decide(a, rows);
     double sum = 0.0;
+    double rest[DV_STEPS][DV_UNIT];
+    rest_of<E, DV_STEPS>(a, d, piece * DV_PIECE + lane * DV_UNIT, false, s_pow, rest);
 #pragma unroll
-    for (uint32_t u = 0; u < DV_STEPS; ++u) {
-        double rest[DV_UNIT];
-        rest_of<E>(a, d, piece * DV_PIECE + (u * 64 + lane) * DV_UNIT, false, rest);
+    for (uint32_t u = 0; u < DV_STEPS; ++u)
 #pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += rest[e];
-    }
+        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += rest[u][e];
     sum = wave_sum_f64(sum);
     if (lane == 0) a.rest[static_cast<uint64_t>(r) * a.pieces + piece] = sum;
 }
 
-// The piece's own sum of p.
-__device__ __forceinline__ double piece_of_p(const VerifyArgs& a, const Decision& d, uint32_t piece)
-{
-    const uint64_t at = static_cast<uint64_t>(d.row) * a.pieces + piece;
-    const double mass = a.mass[at];
-    return mass > 0.0 ? mass * part_of(a.top[at], d.p.top, a.scale) * d.p.part : 0.0;
-}
-
-// A workgroup a request; its first wave finds the token.
+// A workgroup a request.  Its waves all find the piece; each then looks at a part of it.
 template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
 {
-    __shared__ Decision s_waves[DV_WAVES];
-    const uint32_t r = blockIdx.x, lane = __lane_id();
+    static_assert(DV_WAVES == DV_STEPS, "a wave a step of a piece");
+    __shared__ double s_pow[64], s_sum[DV_WAVES];
+    __shared__ int32_t s_hit[DV_WAVES], s_any[DV_WAVES];
+    const uint32_t r = blockIdx.x, lane = __lane_id(), wave = threadIdx.x >> 6;
     const RequestRows rows = rows_of(a, r);
     int32_t* out = a.out + r * a.out_stride;
     if (rows.none) {
@@ -345,91 +486,91 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
         for (uint32_t j = threadIdx.x; j < a.most; j += DV_NT) out[j] = -1;
         return;
     }
-    Decision d;
-    if (a.draft)
-        d = a.decided[r];
-    else
-        d = decide<E>(a, rows, s_waves);
+    load_powers(s_pow);
+    const Decision d = decide(a, rows);
     for (uint32_t j = threadIdx.x; j < a.most; j += DV_NT)
         if (j != d.accepted) out[j] = j < d.accepted ? a.tokens[rows.first + j + 1] : -1;
-    if (threadIdx.x >= 64) return;
-    if (lane == 0) a.accepted[r] = static_cast<int32_t>(d.accepted);
+    if (threadIdx.x == 0) a.accepted[r] = static_cast<int32_t>(d.accepted);
     // the pieces' sums: of what is left of p, or of p where nothing is
-    const double* rest = a.draft ? a.rest + static_cast<uint64_t>(r) * a.pieces : nullptr;
-    const uint32_t gone = !a.draft && d.rejected && d.token >= 0 && static_cast<uint32_t>(d.token) < a.vocab &&
-                                  is_allowed(a, d.row, static_cast<uint32_t>(d.token))
-                              ? static_cast<uint32_t>(d.token)
-                              : 0xFFFFFFFFu;
-    const double gone_p = gone != 0xFFFFFFFFu ? share_of<E>(a, a.x, a.x_row, d.row, gone, d.p) : 0.0;
-    bool plain = false;
+    const uint64_t row0 = static_cast<uint64_t>(d.row) * a.pieces;
+    const Shares share(a, d.p.top);
+    const bool looked_up = !a.draft && d.rejected && d.token >= 0 && static_cast<uint32_t>(d.token) < a.vocab &&
+                           is_allowed(a, d.row, static_cast<uint32_t>(d.token));
+    const uint32_t gone = looked_up ? static_cast<uint32_t>(d.token) / DV_PIECE : 0xFFFFFFFFu;
+    const double gone_p =
+        looked_up ? share_of<E>(a, a.x, a.x_row, d.row, static_cast<uint32_t>(d.token), d.p, s_pow) : 0.0;
+    bool plain = false, empty = false;  // p itself; the draft's piece holds nothing else
     auto piece_sum = [&](uint32_t i) {
-        if (i >= a.pieces) return 0.0;
-        if (plain || !rest) {
-            const double p = piece_of_p(a, d, i);
-            return !plain && gone / DV_PIECE == i ? fmax(p - gone_p, 0.0) : p;
-        }
-        return rest[i];
+        if (i >= a.pieces || !(d.p.part > 0.0)) return 0.0;
+        if (a.draft && d.rejected && !plain) return a.rest[static_cast<uint64_t>(r) * a.pieces + i];
+        const float top = a.top[row0 + i];
+        const double p = top > -__builtin_inff() ? a.mass[row0 + i] * share(top, s_pow) * d.p.part : 0.0;
+        return plain || i != gone ? p : empty ? 0.0 : fmax(p - gone_p, 0.0);
     };
-    double whole = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-        whole = 0.0;
+    int32_t token = -1;
+    for (;;) {
+        double whole = 0.0;
         for (uint32_t i = lane; i < a.pieces; i += 64) whole += piece_sum(i);
         whole = wave_sum_f64(whole);
-        if (whole > 0.0) break;
-        plain = true;
-    }
-    int32_t token = -1;
-    if (whole > 0.0) {
+        if (!(whole > 0.0)) {
+            if (plain) break;
+            plain = true;
+            continue;
+        }
         const double mark = static_cast<double>(a.uniform[rows.first + rows.drafts]) * whole;
         // the first piece whose running sum passes the mark, or the last one that holds anything
         double base = 0.0, before = 0.0;
-        uint32_t found = 0xFFFFFFFFu, last = 0;
-        double last_before = 0.0;
-        for (uint32_t i0 = 0; i0 < a.pieces && found == 0xFFFFFFFFu; i0 += 64) {
+        uint32_t found = 0;
+        for (uint32_t i0 = 0; i0 < a.pieces; i0 += 64) {
             const double mine = piece_sum(i0 + lane), upto = wave_incl_scan_f64(mine);
             const unsigned long long pass = __ballot(mine > 0.0 && base + upto > mark), any = __ballot(mine > 0.0);
-            if (pass) {
-                const int l = __ffsll(static_cast<unsigned long long>(pass)) - 1;
+            if (pass || any) {
+                const int l = pass ? __ffsll(pass) - 1 : 63 - __clzll(static_cast<long long>(any));
                 found = i0 + static_cast<uint32_t>(l);
-                before = base + __shfl(upto, l, 64) - __shfl(mine, l, 64);
-            } else if (any) {
-                const int l = 63 - __clzll(static_cast<long long>(any));
-                last = i0 + static_cast<uint32_t>(l);
-                last_before = base + __shfl(upto, l, 64) - __shfl(mine, l, 64);
+                before = base + lane_f64(upto, __builtin_amdgcn_readfirstlane(l)) - lane_f64(mine, __builtin_amdgcn_readfirstlane(l));
             }
-            base += __shfl(upto, 63, 64);
-        }
-        if (found == 0xFFFFFFFFu) {
-            found = last;
-            before = last_before;
+            if (pass) break;
+            base += lane_f64(upto, 63);
         }
         // the first token of it that does, or its last one that can be drawn
-        int32_t behind = -1;
-        for (uint32_t u = 0; u < DV_STEPS && token < 0; ++u) {
-            const uint32_t first = found * DV_PIECE + (u * 64 + lane) * DV_UNIT;
-            double x[DV_UNIT], sum = 0.0;
-            rest_of<E>(a, d, first, plain, x);
+        const uint32_t first = found * DV_PIECE + (wave * 64 + lane) * DV_UNIT;
+        double x[1][DV_UNIT], sum = 0.0;
+        rest_of<E, 1>(a, d, first, plain, s_pow, x);
 #pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) sum += x[e];
-            const double upto = wave_incl_scan_f64(sum);
-            double run = before + upto - sum;
-            int32_t hit = -1, any = -1;
+        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += x[0][e];
+        const double upto = wave_incl_scan_f64(sum);
+        if (lane == 63) s_sum[wave] = upto;
+        __syncthreads();
+        double run = before + (upto - sum);
+        for (uint32_t w = 0; w < wave; ++w) run += s_sum[w];
+        int32_t hit = -1, any = -1;
 #pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) {
-                run += x[e];
-                if (x[e] > 0.0) {
-                    any = static_cast<int32_t>(first + e);
-                    if (hit < 0 && run > mark) hit = any;
-                }
+        for (uint32_t e = 0; e < DV_UNIT; ++e) {
+            run += x[0][e];
+            if (x[0][e] > 0.0) {
+                any = static_cast<int32_t>(first + e);
+                if (hit < 0 && run > mark) hit = any;
             }
-            const unsigned long long hits = __ballot(hit >= 0), anys = __ballot(any >= 0);
-            if (hits) token = __shfl(hit, __ffsll(hits) - 1, 64);
-            if (anys) behind = __shfl(any, 63 - __clzll(static_cast<long long>(anys)), 64);
-            before += __shfl(upto, 63, 64);
+        }
+        const unsigned long long hits = __ballot(hit >= 0), anys = __ballot(any >= 0);
+        hit = hits ? __shfl(hit, __ffsll(hits) - 1, 64) : -1;
+        any = anys ? __shfl(any, 63 - __clzll(static_cast<long long>(anys)), 64) : -1;
+        if (lane == 0) {
+            s_hit[wave] = hit;
+            s_any[wave] = any;
+        }
+        __syncthreads();
+        int32_t behind = -1;
+        for (uint32_t w = 0; w < DV_WAVES; ++w) {
+            if (token < 0) token = s_hit[w];
+            behind = s_any[w] >= 0 ? s_any[w] : behind;
         }
         if (token < 0) token = behind;
+        if (token >= 0 || empty || plain) break;
+        empty = true;  // rounding had left something where the draft was all there is
+        __syncthreads();
     }
-    if (lane == 0 && d.accepted < a.most) out[d.accepted] = token;
+    if (threadIdx.x == 0 && d.accepted < a.most) out[d.accepted] = token;
 }
 
 template <class E>
@@ -439,6 +580,10 @@ int launch_verify(const VerifyArgs& a, hipStream_t s)
     if (waves) {
         CR_TIMED("dv_sums", s);
         dv_sums<E><<<static_cast<unsigned>((waves + DV_WAVES - 1) / DV_WAVES), DV_NT, 0, s>>>(a);
+    }
+    if (a.n_rows) {
+        CR_TIMED("dv_norms", s);
+        dv_norms<E><<<a.n_rows, 64, 0, s>>>(a);
     }
     if (a.draft) {
         CR_TIMED("dv_rest", s);
@@ -493,7 +638,8 @@ extern "C" int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t str
     a.tokens = p.d_tokens;
     a.starts = p.d_starts;
     a.uniform = p.d_uniform;
-    a.scale = 1.44269504088896340736 / static_cast<double>(p.temperature);
+    a.scale = 64.0 * 1.44269504088896340736 / static_cast<double>(p.temperature);
+    a.reach = static_cast<float>(std::min(3.0e38, 693.0 * static_cast<double>(p.temperature)));
     a.accepted = p.d_accepted;
     a.out = p.d_out;
     a.most = p.out_cols;
@@ -503,14 +649,14 @@ extern "C" int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t str
     Carver cv;
     const size_t o_mass = cv.add(pieces * 8), o_top = cv.add(pieces * 4);
     const size_t o_rest = cv.add(a.draft ? static_cast<size_t>(p.n_requests) * a.pieces * 8 : 0);
-    const size_t o_decided = cv.add(a.draft ? p.n_requests * sizeof(Decision) : 0);
+    const size_t o_state = cv.add(p.n_rows * sizeof(RowState));
     const size_t o_words = cv.add(p.allowed && !direct ? n_words * 4ull : 0);
     Scratch sc;
     CR_RET(sc.alloc(cv.total, s));
     a.mass = sc.at<double>(o_mass);
     a.top = sc.at<float>(o_top);
     a.rest = sc.at<double>(o_rest);
-    a.decided = sc.at<Decision>(o_decided);
+    a.state = sc.at<RowState>(o_state);
     a.masked = p.allowed || p.d_allowed_bits;
     a.flat = p.d_allowed_bits;
     a.bits_stride = p.bits_stride;
