@@ -51,11 +51,12 @@ struct VerifyArgs {
     const void* draft;  // or nullptr
     uint64_t x_row, draft_row;
     uint32_t n_rows, n_requests, vocab, pieces;
+    uint32_t per;        // pieces that a wave of dv_sums takes
     const int32_t* tokens;
     const int32_t* starts;
     const float* uniform;
-    double scale;        // 64 log2(e) / temperature
-    float reach;         // scores so far below the largest have no share
+    double scale;        // 256 log2(e) / temperature
+    double reach;        // scores so far below the largest have no share
     const uint32_t* flat;  // [rows of bits_stride words, or one for all (0)], or nullptr
     uint64_t bits_stride;
     SetBits allowed;
@@ -71,82 +72,114 @@ struct VerifyArgs {
     double* rest;          // [n_requests][pieces]
 };
 
-// 2^(i / 64)
-__device__ const double DV_POWERS[64] = {
-    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
-    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
-    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
-    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
-    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
-    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
-    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
-    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
-    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
-    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
-    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
-    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
-    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
-    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
-};
-
-__device__ __forceinline__ void load_powers(double* s_pow)
+// 2^(i / 256) for i = threadIdx.x: the series of e^y to y^11, y = (i / 256 - 1/2) log(2), which
+// leaves 7e-15 of it, times 2^(1/2).
+__device__ __forceinline__ double power_of(uint32_t i)
 {
-    if (threadIdx.x < 64) s_pow[threadIdx.x] = DV_POWERS[threadIdx.x];
+    const double y = (static_cast<double>(static_cast<int32_t>(i) - 128) / 256.0) * 0.693147180559945309417;
+    double e = 2.505210838544171877505e-8;
+    e = fma(e, y, 2.755731922398589065255e-7);
+    e = fma(e, y, 2.755731922398589065255e-6);
+    e = fma(e, y, 2.480158730158730158730e-5);
+    e = fma(e, y, 1.984126984126984126984e-4);
+    e = fma(e, y, 1.388888888888888888889e-3);
+    e = fma(e, y, 8.333333333333333333333e-3);
+    e = fma(e, y, 4.166666666666666666667e-2);
+    e = fma(e, y, 1.666666666666666666667e-1);
+    e = fma(e, y, 0.5);
+    e = fma(e, y, 1.0);
+    e = fma(e, y, 1.0);
+    return e * 1.41421356237309504880;
+}
+
+constexpr uint32_t DV_POWERS = 256;
+
+template <int NT>
+__device__ __forceinline__ void make_powers(double* s_pow)
+{
+#pragma unroll
+    for (uint32_t i = 0; i < DV_POWERS; i += NT) s_pow[i + threadIdx.x] = power_of(i + threadIdx.x);
     __syncthreads();
 }
 
-// e^((x - top) / T) of a row whose largest score is `top`: 2^(u / 64) with u rounded to a
+// e^((x - top) / T) of a row whose largest score is `top`: 2^(u / 256) with u rounded to a
 // whole number n, which is added to an exponent and looked up, and the rest |f| <= 1/2 by
-// the series of e^y to y^4, y = f log(2) / 64, which leaves 4e-14 of it.  Below 2^-1000 of
-// the largest, and for NaN and -inf, nothing; scores of +inf share the mass.
+// the series of e^y to y^3, y = f log(2) / 256, which leaves 1.4e-13 of it.  Scores of +inf
+// share the mass.
 struct Shares {
-    double scale, from;
-    float top, least;
+    double scale, from, least;
+    float top;
     __device__ __forceinline__ Shares(const VerifyArgs& a, float largest)
     {
         scale = a.scale;
         top = largest;
         from = static_cast<double>(largest);
-        least = fmaxf(largest - a.reach, -3.402823466e38f);
+        least = -a.reach;
     }
-    // Of a finite largest score, without a branch.
-    __device__ __forceinline__ double finite(float x, const double* s_pow) const
+    // How far below a finite largest score x is, which is exact: at low temperatures its factors
+    // are far above it.
+    __device__ __forceinline__ double below(float x) const { return static_cast<double>(x) - from; }
+    // The power and what it is multiplied by, of d from `least` to 0.
+    __device__ __forceinline__ void parts(double d, const double* s_pow, double& power, double& more) const
     {
         constexpr double ROUND = 6755399441055744.0;  // 1.5 * 2^52
-        const bool there = x >= least;
-        // (the difference first, which is exact: at low temperatures its factors are far above it)
-        const double u = (static_cast<double>(there ? x : top) - from) * scale, r = u + ROUND, f = u - (r - ROUND);
-        const int32_t n = static_cast<int32_t>(__double_as_longlong(r));
-        const uint64_t power = static_cast<uint64_t>(__double_as_longlong(s_pow[n & 63]));
-        const uint32_t hi = static_cast<uint32_t>(power >> 32) + (static_cast<uint32_t>(n >> 6) << 20);
-        const double p = __longlong_as_double(
-            static_cast<long long>(static_cast<uint64_t>(there ? hi : 0u) << 32 | (there ? static_cast<uint32_t>(power) : 0u)));
-        double q = fma(f, 0x1.3b2ab6fba4e77p-31, 0x1.c6b08d704a0c0p-23);
-        q = fma(f, q, 0x1.ebfbdff82c58fp-15);
-        q = fma(f, q, 0x1.62e42fefa39efp-7);
-        return fma(p * f, q, p);
+        const double r = fma(d, scale, ROUND), f = fma(d, scale, ROUND - r);
+        const uint32_t n = static_cast<uint32_t>(__double_as_longlong(r));
+        const uint64_t b = static_cast<uint64_t>(__double_as_longlong(s_pow[n % DV_POWERS]));
+        const uint32_t hi = static_cast<uint32_t>(b >> 32) + (n / DV_POWERS << 20);  // (modulo 2^12: n may be negative)
+        power = __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(b)));
+        more = fma(f, fma(f, fma(f, 0x1.c6b08d704a0c0p-29, 0x1.ebfbdff82c58fp-19), 0x1.62e42fefa39efp-9), 1.0);
+    }
+    // Adds a share; those of NaN, -inf and scores below 2^-1000 of the largest as 2^-1000 of
+    // it, which no sum notices.
+    __device__ __forceinline__ void add(float x, const double* s_pow, double& sum) const
+    {
+        double power, more;
+        parts(fmax(below(x), least), s_pow, power, more);
+        sum = fma(power, more, sum);
+    }
+    // The share itself: of those none.
+    __device__ __forceinline__ double finite(float x, const double* s_pow) const
+    {
+        double power, more;
+        const double d = below(x);
+        parts(fmax(d, least), s_pow, power, more);
+        return d >= least ? power * more : 0.0;
     }
     __device__ __forceinline__ double operator()(float x, const double* s_pow) const
     {
         return top == __builtin_inff() ? (x == top ? 1.0 : 0.0) : finite(x, s_pow);
     }
-    // Many at once: they are worked out side by side.
-    template <uint32_t U>
-    __device__ __forceinline__ void of(const float (&x)[U][DV_UNIT], const double* s_pow, double (&share)[U][DV_UNIT]) const
+    // A unit of them, worked out side by side.
+    __device__ __forceinline__ void of(const float (&x)[DV_UNIT], const double* s_pow, double (&share)[DV_UNIT]) const
     {
+        if (top == __builtin_inff()) {
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) share[e] = x[e] == top ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) share[e] = finite(x[e], s_pow);
+        }
+    }
+    template <uint32_t U>
+    __device__ __forceinline__ double sum(const float (&x)[U][DV_UNIT], const double* s_pow) const
+    {
+        double mass = 0.0, more = 0.0;  // (two chains)
         if (top == __builtin_inff()) {
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
-                for (uint32_t e = 0; e < DV_UNIT; ++e) share[u][e] = x[u][e] == top ? 1.0 : 0.0;
+                for (uint32_t e = 0; e < DV_UNIT; ++e) mass += x[u][e] == top ? 1.0 : 0.0;
         } else {
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
-                for (uint32_t e = 0; e < DV_UNIT; ++e) share[u][e] = finite(x[u][e], s_pow);
+                for (uint32_t e = 0; e < DV_UNIT; e += 2) {
+                    add(x[u][e], s_pow, mass);
+                    add(x[u][e + 1], s_pow, more);
+                }
         }
+        return mass + more;
     }
 };
 
@@ -202,61 +235,83 @@ __device__ __forceinline__ float wave_max(float v)
     return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), 63)));
 }
 
+// The allowed tokens' bits where a piece lies, which is within one container: word w of them is
+// (words[w] & keep) ^ flip, and tokens from `end` on may not be used.
+struct Mask {
+    const uint32_t* words;  // nullptr: every token may be used
+    uint32_t keep, flip, end;
+    __device__ __forceinline__ Mask(const VerifyArgs& a, uint32_t row, uint32_t first)
+    {
+        words = nullptr;
+        keep = 0xFFFFFFFFu;
+        flip = 0u;
+        end = a.vocab;
+        if (!a.masked) return;
+        if (a.flat) {
+            words = a.flat + row * a.bits_stride;
+        } else if (a.allowed.flat) {
+            words = a.allowed.flat;
+        } else {
+            const uint32_t key = __builtin_amdgcn_readfirstlane(first) / 65536u;
+            uint32_t c = a.allowed.key_index[min(key, a.allowed.max_key)];
+            if (key > a.allowed.max_key) c = 0xFFFFu;
+            keep = c != 0xFFFFu ? 0xFFFFFFFFu : 0u;
+            flip = a.allowed.flip;
+            end = min(end, a.allowed.end);
+            words = reinterpret_cast<const uint32_t*>(a.allowed.bitmaps) + a.allowed.offsets[c != 0xFFFFu ? c : 0u] / 4u -
+                    static_cast<int64_t>(key) * 2048;
+        }
+    }
+};
+
 // A lane's tokens of a piece: DV_UNIT neighbours from first + u * 64 * DV_UNIT on, for U values
-// of u; -inf for those that are not there, may not be used after row `row` or are NaN.  No
-// load waits for another.
+// of u, as they lie, and which of them are there and may be used.  No load waits for
+// another, and none is waited for here.
 template <class E, uint32_t U>
-__device__ __forceinline__ void load_tokens(const VerifyArgs& a, const typename E::Bits* p, uint32_t row, uint32_t first,
-                                            float (&x)[U][DV_UNIT])
-{
+struct Tokens {
     typedef typename E::Bits Bits;
     // rows may begin anywhere
     typedef Bits Wide __attribute__((ext_vector_type(DV_UNIT), aligned(sizeof(Bits))));
-    constexpr uint32_t STEP = 64 * DV_UNIT;
+    static constexpr uint32_t STEP = 64 * DV_UNIT;
+    Wide raw[U];
     uint32_t on[U];
+    bool all;  // every one is, in the whole wave
+
+    __device__ __forceinline__ void load(const VerifyArgs& a, const Bits* p, const Mask& mask, uint32_t first)
+    {
+        const bool whole = __builtin_amdgcn_readfirstlane(first) + U * STEP <= a.vocab;  // (the first lane's are the first)
+        all = whole && !mask.words;
+        if (mask.words) {
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) on[u] = 0xFFFFFFFFu;
-    if (a.masked) {
-        const uint32_t last = (a.vocab - 1) / 32u;
-        uint32_t w[U];
+            for (uint32_t u = 0; u < U; ++u) on[u] = mask.words[min((first + u * STEP) / 32u, (a.vocab - 1) / 32u)];
+        }
+        if (whole) {
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) w[u] = min((first + u * STEP) / 32u, last);
-        if (a.flat) {
-#pragma unroll
-            for (uint32_t u = 0; u < U; ++u) on[u] = a.flat[row * a.bits_stride + w[u]];
-        } else if (a.allowed.end) {
-            a.allowed.words(w, on);
+            for (uint32_t u = 0; u < U; ++u)
+                raw[u] = __builtin_nontemporal_load(reinterpret_cast<const Wide*>(p + first + u * STEP));
         } else {
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u) on[u] = 0u;
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < DV_UNIT; ++e) raw[u][e] = p[min(first + u * STEP + e, a.vocab - 1)];
         }
     }
-    if (__builtin_amdgcn_readfirstlane(first) + U * STEP <= a.vocab) {  // (the first lane's are the first)
-        Wide w[U];
+    // The scores of unit u: -inf for those that are not there or may not be used.
+    __device__ __forceinline__ void scores(const Mask& mask, uint32_t first, uint32_t u, float (&x)[DV_UNIT]) const
+    {
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) w[u] = __builtin_nontemporal_load(reinterpret_cast<const Wide*>(p + first + u * STEP));
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) x[u][e] = E::up(w[u][e]);
-    } else {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) {
-                const uint32_t at = first + u * STEP + e;
-                const float v = E::up(p[min(at, a.vocab - 1)]);
-                x[u][e] = at < a.vocab ? v : -__builtin_inff();
-            }
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u)
+        for (uint32_t e = 0; e < DV_UNIT; ++e) x[e] = E::up(raw[u][e]);
+        if (all) return;
+        const uint32_t at = first + u * STEP, left = at < mask.end ? mask.end - at : 0u;
+        const uint32_t bits = mask.words ? (on[u] & mask.keep) ^ mask.flip : 0xFFFFFFFFu;
+        const uint32_t may = (bits >> (first % 32u)) & (left >= DV_UNIT ? 0xFFu : (1u << left) - 1u);
 #pragma unroll
         for (uint32_t e = 0; e < DV_UNIT; ++e) {
-            const bool may = !a.masked || (on[u] >> ((first + e) % 32u)) & 1u;
-            x[u][e] = may && x[u][e] == x[u][e] ? x[u][e] : -__builtin_inff();
+            const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(may << (31u - e)) >> 31);
+            x[e] = __uint_as_float((__float_as_uint(x[e]) & keep) | (0xFF800000u & ~keep));
         }
-}
+    }
+};
 
 __device__ __forceinline__ bool is_allowed(const VerifyArgs& a, uint64_t row, uint32_t token)
 {
@@ -294,46 +349,43 @@ __device__ __forceinline__ bool is_last(const VerifyArgs& a, uint32_t row)
     return a.starts[min(lo, a.n_requests)] == next;
 }
 
-// Every row's pieces; the drafting model's rows behind the model's.
+// Every row's pieces, a.per of them a wave; the drafting model's rows behind the model's.
 template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
 {
-    __shared__ double s_pow[64];
-    const uint32_t lane = __lane_id(), wave = blockIdx.x * DV_WAVES + (threadIdx.x >> 6);
-    load_powers(s_pow);
-    const uint32_t at = __builtin_amdgcn_readfirstlane(wave / a.pieces), piece = __builtin_amdgcn_readfirstlane(wave % a.pieces);
-    if (at >= (a.draft ? 2 : 1) * a.n_rows) return;
-    const bool drafted = at >= a.n_rows;
+    __shared__ double s_pow[DV_POWERS];
+    const uint32_t lane = __lane_id(), groups = (a.pieces + a.per - 1) / a.per;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * DV_WAVES + (threadIdx.x >> 6));
+    const uint32_t at = wave / groups, piece0 = wave % groups * a.per, n = min(a.per, a.pieces - piece0);
+    const bool there = at < (a.draft ? 2 : 1) * a.n_rows, drafted = at >= a.n_rows;
     const uint32_t row = drafted ? at - a.n_rows : at;
-    if (drafted && is_last(a, row)) return;
     const auto* p = static_cast<const typename E::Bits*>(drafted ? a.draft : a.x) +
                     row * (drafted ? a.draft_row : a.x_row);
-    float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
-    load_tokens<E, DV_STEPS>(a, p, row, piece * DV_PIECE + lane * DV_UNIT, x);
+    Tokens<E, DV_STEPS> next;
+    Mask mask(a, there ? row : 0u, piece0 * DV_PIECE);
+    if (there) next.load(a, p, mask, piece0 * DV_PIECE + lane * DV_UNIT);
+    make_powers<DV_NT>(s_pow);
+    if (!there || (drafted && is_last(a, row))) return;
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint32_t piece = piece0 + i;
+        float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
 #pragma unroll
-    for (uint32_t u = 0; u < DV_STEPS; ++u)
-#pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
-    top = wave_max(top);
-    double mass = 0.0;
-    if (top > -__builtin_inff()) {
-        const Shares share(a, top);
-        if (top == __builtin_inff()) {
-#pragma unroll
-            for (uint32_t u = 0; u < DV_STEPS; ++u)
-#pragma unroll
-                for (uint32_t e = 0; e < DV_UNIT; ++e) mass += x[u][e] == top ? 1.0 : 0.0;
-        } else {
-#pragma unroll
-            for (uint32_t u = 0; u < DV_STEPS; ++u)
-#pragma unroll
-                for (uint32_t e = 0; e < DV_UNIT; ++e) mass += share.finite(x[u][e], s_pow);
+        for (uint32_t u = 0; u < DV_STEPS; ++u) next.scores(mask, piece * DV_PIECE + lane * DV_UNIT, u, x[u]);
+        if (i + 1 < n) {
+            if ((piece + 1) * DV_PIECE % 65536u == 0) mask = Mask(a, row, (piece + 1) * DV_PIECE);
+            next.load(a, p, mask, (piece + 1) * DV_PIECE + lane * DV_UNIT);
         }
-    }
-    mass = wave_sum_f64(mass);
-    if (lane == 0) {
-        a.top[wave] = top;
-        a.mass[wave] = mass;
+#pragma unroll
+        for (uint32_t u = 0; u < DV_STEPS; ++u)
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
+        top = wave_max(top);
+        double mass = 0.0;
+        if (top > -__builtin_inff()) mass = wave_sum_f64(Shares(a, top).sum(x, s_pow));
+        if (lane == 0) {
+            a.top[static_cast<uint64_t>(at) * a.pieces + piece] = top;
+            a.mass[static_cast<uint64_t>(at) * a.pieces + piece] = mass;
+        }
     }
 }
 
@@ -367,9 +419,9 @@ __device__ __forceinline__ double share_of(const VerifyArgs& a, const void* x, u
 template <class E>
 __global__ __launch_bounds__(64) void dv_norms(VerifyArgs a)
 {
-    __shared__ double s_pow[64];
+    __shared__ double s_pow[DV_POWERS];
     const uint32_t row = blockIdx.x;
-    load_powers(s_pow);
+    make_powers<64>(s_pow);
     RowState s{};
     const bool last = row + 1 >= a.n_rows || is_last(a, row);
     const int32_t token = last ? -1 : a.tokens[row + 1];
@@ -416,57 +468,62 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
     return d;
 }
 
-// max(p - q, 0), or p behind the last draft (or where `plain`), of a lane's tokens from `first`.
-template <class E, uint32_t U>
+// max(p - q, 0), or p behind the last draft (or where `plain`), of a lane's tokens from
+// `first` on: U units, f(u, those of unit u).
+template <class E, uint32_t U, class F>
 __device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, uint32_t first, bool plain, const double* s_pow,
-                                        double (&rest)[U][DV_UNIT])
+                                        F f)
 {
     // each product rounded by itself, so that equal shares leave nothing
 #pragma clang fp contract(off)
-    float x[U][DV_UNIT], y[U][DV_UNIT];
     const bool both = a.draft && d.rejected && !plain && d.q.part > 0.0;
-    load_tokens<E, U>(a, static_cast<const typename E::Bits*>(a.x) + d.row * a.x_row, d.row, first, x);
-    if (both) load_tokens<E, U>(a, static_cast<const typename E::Bits*>(a.draft) + d.row * a.draft_row, d.row, first, y);
-    Shares(a, d.p.top).of(x, s_pow, rest);  // (no share where the score is -inf)
+    const bool drop = !a.draft && d.rejected && !plain;
+    const Mask mask(a, d.row, first);
+    Tokens<E, U> of_model, of_draft;
+    of_model.load(a, static_cast<const typename E::Bits*>(a.x) + d.row * a.x_row, mask, first);
+    if (both) of_draft.load(a, static_cast<const typename E::Bits*>(a.draft) + d.row * a.draft_row, mask, first);
     const double p_part = d.p.part, q_part = d.q.part;
-    if (both) {
-        double q[U][DV_UNIT];
-        Shares(a, d.q.top).of(y, s_pow, q);
+    const Shares p(a, d.p.top), q(a, d.q.top);
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u)
+    for (uint32_t u = 0; u < U; ++u) {
+        float x[DV_UNIT];
+        double rest[DV_UNIT];
+        of_model.scores(mask, first, u, x);
+        p.of(x, s_pow, rest);  // (no share where the score is -inf)
+        if (both) {
+            double y[DV_UNIT];
+            of_draft.scores(mask, first, u, x);
+            q.of(x, s_pow, y);
 #pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) rest[u][e] = fmax(rest[u][e] * p_part - q[u][e] * q_part, 0.0);
-    } else {
-        const bool drop = !a.draft && d.rejected && !plain;
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u)
+            for (uint32_t e = 0; e < DV_UNIT; ++e) rest[e] = fmax(rest[e] * p_part - y[e] * q_part, 0.0);
+        } else {
 #pragma unroll
             for (uint32_t e = 0; e < DV_UNIT; ++e) {
                 const bool is = drop && static_cast<int32_t>(first + u * 64 * DV_UNIT + e) == d.token;
-                rest[u][e] = is ? 0.0 : rest[u][e] * p_part;
+                rest[e] = is ? 0.0 : rest[e] * p_part;
             }
+        }
+        f(u, rest);
     }
 }
 
 // The pieces' sums of what the next token is drawn from, a wave a piece.
 template <class E>
-__global__ __launch_bounds__(DV_NT) void dv_rest(VerifyArgs a, uint32_t groups)
+__global__ __launch_bounds__(DV_NT) __attribute__((amdgpu_waves_per_eu(4))) void dv_rest(VerifyArgs a, uint32_t groups)
 {
-    __shared__ double s_pow[64];
+    __shared__ double s_pow[DV_POWERS];
     const uint32_t r = blockIdx.x / groups, lane = __lane_id();
     const uint32_t piece = __builtin_amdgcn_readfirstlane(blockIdx.x % groups * DV_WAVES + (threadIdx.x >> 6));
     const RequestRows rows = rows_of(a, r);
     if (rows.none) return;
-    load_powers(s_pow);
+    make_powers<DV_NT>(s_pow);
     if (piece >= a.pieces) return;
     const Decision d = decide(a, rows);
     double sum = 0.0;
-    double rest[DV_STEPS][DV_UNIT];
-    rest_of<E, DV_STEPS>(a, d, piece * DV_PIECE + lane * DV_UNIT, false, s_pow, rest);
+    rest_of<E, DV_STEPS>(a, d, piece * DV_PIECE + lane * DV_UNIT, false, s_pow, [&](uint32_t, const double (&rest)[DV_UNIT]) {
 #pragma unroll
-    for (uint32_t u = 0; u < DV_STEPS; ++u)
-#pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += rest[u][e];
+        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += rest[e];
+    });
     sum = wave_sum_f64(sum);
     if (lane == 0) a.rest[static_cast<uint64_t>(r) * a.pieces + piece] = sum;
 }
@@ -476,7 +533,7 @@ template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
 {
     static_assert(DV_WAVES == DV_STEPS, "a wave a step of a piece");
-    __shared__ double s_pow[64], s_sum[DV_WAVES];
+    __shared__ double s_pow[DV_POWERS], s_sum[DV_WAVES];
     __shared__ int32_t s_hit[DV_WAVES], s_any[DV_WAVES];
     const uint32_t r = blockIdx.x, lane = __lane_id(), wave = threadIdx.x >> 6;
     const RequestRows rows = rows_of(a, r);
@@ -486,7 +543,7 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
         for (uint32_t j = threadIdx.x; j < a.most; j += DV_NT) out[j] = -1;
         return;
     }
-    load_powers(s_pow);
+    make_powers<DV_NT>(s_pow);
     const Decision d = decide(a, rows);
     for (uint32_t j = threadIdx.x; j < a.most; j += DV_NT)
         if (j != d.accepted) out[j] = j < d.accepted ? a.tokens[rows.first + j + 1] : -1;
@@ -534,10 +591,14 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
         }
         // the first token of it that does, or its last one that can be drawn
         const uint32_t first = found * DV_PIECE + (wave * 64 + lane) * DV_UNIT;
-        double x[1][DV_UNIT], sum = 0.0;
-        rest_of<E, 1>(a, d, first, plain, s_pow, x);
+        double x[DV_UNIT], sum = 0.0;
+        rest_of<E, 1>(a, d, first, plain, s_pow, [&](uint32_t, const double (&rest)[DV_UNIT]) {
 #pragma unroll
-        for (uint32_t e = 0; e < DV_UNIT; ++e) sum += x[0][e];
+            for (uint32_t e = 0; e < DV_UNIT; ++e) {
+                x[e] = rest[e];
+                sum += rest[e];
+            }
+        });
         const double upto = wave_incl_scan_f64(sum);
         if (lane == 63) s_sum[wave] = upto;
         __syncthreads();
@@ -546,8 +607,8 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
         int32_t hit = -1, any = -1;
 #pragma unroll
         for (uint32_t e = 0; e < DV_UNIT; ++e) {
-            run += x[0][e];
-            if (x[0][e] > 0.0) {
+            run += x[e];
+            if (x[e] > 0.0) {
                 any = static_cast<int32_t>(first + e);
                 if (hit < 0 && run > mark) hit = any;
             }
@@ -576,7 +637,7 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
 template <class E>
 int launch_verify(const VerifyArgs& a, hipStream_t s)
 {
-    const uint64_t waves = static_cast<uint64_t>(a.draft ? 2 : 1) * a.n_rows * a.pieces;
+    const uint64_t waves = static_cast<uint64_t>(a.draft ? 2 : 1) * a.n_rows * ((a.pieces + a.per - 1) / a.per);
     if (waves) {
         CR_TIMED("dv_sums", s);
         dv_sums<E><<<static_cast<unsigned>((waves + DV_WAVES - 1) / DV_WAVES), DV_NT, 0, s>>>(a);
@@ -627,6 +688,10 @@ extern "C" int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t str
         set_error("cr_draft_verify: too many scores for one call");
         return CR_ERR_UNSUPPORTED;
     }
+    // A wave takes as many pieces as let all waves be there at once, up to 8 (the next one's
+    // scores arrive meanwhile).
+    const uint64_t all = static_cast<uint64_t>(p.d_draft ? 2 : 1) * p.n_rows * a.pieces, places = 16ull * num_cus();
+    a.per = static_cast<uint32_t>(std::min<uint64_t>(8, std::max<uint64_t>(1, (all + places - 1) / places)));
     hipStream_t s = as_stream(stream);
     a.x = p.d_scores;
     a.draft = p.n_rows ? p.d_draft : nullptr;
@@ -638,8 +703,8 @@ extern "C" int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t str
     a.tokens = p.d_tokens;
     a.starts = p.d_starts;
     a.uniform = p.d_uniform;
-    a.scale = 64.0 * 1.44269504088896340736 / static_cast<double>(p.temperature);
-    a.reach = static_cast<float>(std::min(3.0e38, 693.0 * static_cast<double>(p.temperature)));
+    a.scale = 256.0 * 1.44269504088896340736 / static_cast<double>(p.temperature);
+    a.reach = 693.0 * static_cast<double>(p.temperature);  // 2^-1000
     a.accepted = p.d_accepted;
     a.out = p.d_out;
     a.most = p.out_cols;
