@@ -51,7 +51,6 @@ struct VerifyArgs {
     const void* draft;  // or nullptr
     uint64_t x_row, draft_row;
     uint32_t n_rows, n_requests, vocab, pieces;
-    uint32_t per;        // pieces that a wave of dv_sums takes
     const int32_t* tokens;
     const int32_t* starts;
     const float* uniform;
@@ -349,43 +348,36 @@ __device__ __forceinline__ bool is_last(const VerifyArgs& a, uint32_t row)
     return a.starts[min(lo, a.n_requests)] == next;
 }
 
-// Every row's pieces, a.per of them a wave; the drafting model's rows behind the model's.
+// Every row's pieces, a wave each; the drafting model's rows behind the model's.
 template <class E>
 __global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
 {
     __shared__ double s_pow[DV_POWERS];
-    const uint32_t lane = __lane_id(), groups = (a.pieces + a.per - 1) / a.per;
+    const uint32_t lane = __lane_id();
     const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * DV_WAVES + (threadIdx.x >> 6));
-    const uint32_t at = wave / groups, piece0 = wave % groups * a.per, n = min(a.per, a.pieces - piece0);
+    const uint32_t at = wave / a.pieces, first = wave % a.pieces * DV_PIECE + lane * DV_UNIT;
     const bool there = at < (a.draft ? 2 : 1) * a.n_rows, drafted = at >= a.n_rows;
     const uint32_t row = drafted ? at - a.n_rows : at;
     const auto* p = static_cast<const typename E::Bits*>(drafted ? a.draft : a.x) +
                     row * (drafted ? a.draft_row : a.x_row);
-    Tokens<E, DV_STEPS> next;
-    Mask mask(a, there ? row : 0u, piece0 * DV_PIECE);
-    if (there) next.load(a, p, mask, piece0 * DV_PIECE + lane * DV_UNIT);
+    Tokens<E, DV_STEPS> tokens;
+    const Mask mask(a, there ? row : 0u, first);
+    if (there) tokens.load(a, p, mask, first);
     make_powers<DV_NT>(s_pow);
     if (!there || (drafted && is_last(a, row))) return;
-    for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t piece = piece0 + i;
-        float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
+    float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
 #pragma unroll
-        for (uint32_t u = 0; u < DV_STEPS; ++u) next.scores(mask, piece * DV_PIECE + lane * DV_UNIT, u, x[u]);
-        if (i + 1 < n) {
-            if ((piece + 1) * DV_PIECE % 65536u == 0) mask = Mask(a, row, (piece + 1) * DV_PIECE);
-            next.load(a, p, mask, (piece + 1) * DV_PIECE + lane * DV_UNIT);
-        }
+    for (uint32_t u = 0; u < DV_STEPS; ++u) {
+        tokens.scores(mask, first, u, x[u]);
 #pragma unroll
-        for (uint32_t u = 0; u < DV_STEPS; ++u)
-#pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
-        top = wave_max(top);
-        double mass = 0.0;
-        if (top > -__builtin_inff()) mass = wave_sum_f64(Shares(a, top).sum(x, s_pow));
-        if (lane == 0) {
-            a.top[static_cast<uint64_t>(at) * a.pieces + piece] = top;
-            a.mass[static_cast<uint64_t>(at) * a.pieces + piece] = mass;
-        }
+        for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
+    }
+    top = wave_max(top);
+    double mass = 0.0;
+    if (top > -__builtin_inff()) mass = wave_sum_f64(Shares(a, top).sum(x, s_pow));
+    if (lane == 0) {
+        a.top[wave] = top;
+        a.mass[wave] = mass;
     }
 }
 
@@ -637,7 +629,7 @@ __global__ __launch_bounds__(DV_NT) void dv_pick(VerifyArgs a)
 template <class E>
 int launch_verify(const VerifyArgs& a, hipStream_t s)
 {
-    const uint64_t waves = static_cast<uint64_t>(a.draft ? 2 : 1) * a.n_rows * ((a.pieces + a.per - 1) / a.per);
+    const uint64_t waves = static_cast<uint64_t>(a.draft ? 2 : 1) * a.n_rows * a.pieces;
     if (waves) {
         CR_TIMED("dv_sums", s);
         dv_sums<E><<<static_cast<unsigned>((waves + DV_WAVES - 1) / DV_WAVES), DV_NT, 0, s>>>(a);
@@ -688,10 +680,6 @@ extern "C" int cr_draft_verify(const cr_draft_verify_args* args, cr_stream_t str
         set_error("cr_draft_verify: too many scores for one call");
         return CR_ERR_UNSUPPORTED;
     }
-    // A wave takes as many pieces as let all waves be there at once, up to 8 (the next one's
-    // scores arrive meanwhile).
-    const uint64_t all = static_cast<uint64_t>(p.d_draft ? 2 : 1) * p.n_rows * a.pieces, places = 16ull * num_cus();
-    a.per = static_cast<uint32_t>(std::min<uint64_t>(8, std::max<uint64_t>(1, (all + places - 1) / places)));
     hipStream_t s = as_stream(stream);
     a.x = p.d_scores;
     a.draft = p.n_rows ? p.d_draft : nullptr;
