@@ -18,7 +18,7 @@ namespace {
 
 constexpr int RO_NT = 256;
 constexpr uint32_t RO_PAIRS = 2048;  // cosines and sines that a workgroup keeps
-constexpr uint32_t RO_AHEAD = 2;     // pieces that a thread asks for at a time
+constexpr uint32_t RO_AHEAD = 2;     // tokens whose pieces a thread asks for at a time
 
 struct Plane {  // rows of one of the tensors; strides in elements
     const void* src;
@@ -36,9 +36,8 @@ struct RotaryArgs {
     const int64_t* slots;
     uint64_t n_slots;
     uint32_t page_lg;
-    uint32_t tokens;     // of a workgroup
-    uint32_t splits;     // workgroups that share them
-    uint32_t per_row, per_token;  // pieces' pairs
+    uint32_t per_row, per_token;   // pairs of pieces
+    uint32_t tokens, rounds, side;  // tokens of a workgroup; workgroups that share them; tokens side by side
 };
 
 // Cosine and sine of position * freq, in 64 bits until whole turns are taken
@@ -64,130 +63,114 @@ __device__ __forceinline__ float2 cos_sin(int32_t position, double freq, float m
     return make_float2((n == 1 || n == 2 ? -cn : cn) * m, (n >= 2 ? -sn : sn) * m);
 }
 
-// Bound by memory: a thread asks for the two pieces that turn together (or two
-// neighbours), and the next two, before the workgroup's cosines are there.
+// Bound by memory.  A thread looks after one pair of pieces that turn together (or of any
+// two of a row), of all tokens of its workgroup (or of every side-th, where a token has few
+// pieces): it works out where they lie once, and asks for those of RO_AHEAD tokens at a
+// time, the first ones before the workgroup's cosines are there.
 template <class E, uint32_t N, bool NEXT>
 __global__ __launch_bounds__(RO_NT) void ro_turn(RotaryArgs a)
 {
     typedef typename E::Bits Bits;
     typedef Piece<E, N> P;
     __shared__ float2 s_turn[RO_PAIRS];
-    const uint32_t t = threadIdx.x, token0 = blockIdx.x / a.splits * a.tokens, part = blockIdx.x % a.splits;
-    const uint32_t tokens = min(a.tokens, a.n_tokens - token0), items = tokens * a.per_token;
-    const uint32_t turned = NEXT ? a.half * 2 : a.half;  // dimensions whose pieces come in turned pairs
-    struct Item {
-        P x, y;
-        Bits* to;         // nullptr: nowhere
-        uint32_t at, two;  // the pieces' first dimensions
-        uint32_t token;
-        bool both, turn;
-    };
-    auto load = [&](uint32_t i) {
-        Item it;
-        const uint32_t local = i / a.per_token, in = i % a.per_token, row = in / a.per_row, c = in % a.per_row * N;
-        const uint32_t token = token0 + local;
-        it.token = local;
-        it.at = c;
-        it.two = c + a.half;
-        if (NEXT) {
-            it.at = 2 * c;
-            it.two = 2 * c + N;
-        } else if (c >= turned) {
-            it.at = 2 * a.half + 2 * (c - a.half);
-            it.two = it.at + N;
+    const uint32_t t = threadIdx.x, token0 = blockIdx.x / a.rounds * a.tokens;
+    const uint32_t end = min(token0 + a.tokens, a.n_tokens), turned = NEXT ? a.half * 2 : a.half;
+    const uint32_t first = token0 + (a.side > 1 ? t / a.per_token : 0u);
+    const uint32_t item = a.side > 1 ? t % a.per_token : blockIdx.x % a.rounds * blockDim.x + t;
+    const bool there = a.side > 1 ? t < a.side * a.per_token : item < a.per_token;
+    const uint32_t row = item / a.per_row, c = item % a.per_row * N;
+    // The pieces' first dimensions.  Neighbouring threads' pieces lie side by side.
+    uint32_t at = c, two = c + (NEXT ? a.per_row * N : a.half);
+    if (NEXT && N == 1) {
+        at = 2 * c;
+        two = at + 1;
+    } else if (!NEXT && c >= turned) {
+        at = a.half + c;
+        two = at + a.per_row * N - a.half;
+    }
+    const bool both = two < a.dim, query = row < a.heads, key = !query && row < a.heads + a.kv_heads;
+    const bool turn = (query || key) && at < turned;
+    const uint32_t head = query ? row : key ? row - a.heads : row - a.heads - a.kv_heads;
+    const Plane& plane = query ? a.q : key ? a.k : a.v;
+    const Bits* from = static_cast<const Bits*>(plane.src) + head * plane.src_head;
+    Bits* to = static_cast<Bits*>(plane.dst) + head * (query ? plane.dst_head : key ? a.k_head : a.v_head);
+    const uint64_t page_stride = key ? a.k_page : a.v_page, slot_stride = key ? a.k_slot : a.v_slot;
+    P x[RO_AHEAD], y[RO_AHEAD];
+    int64_t slot[RO_AHEAD];
+    auto load = [&](uint32_t token) {
+#pragma unroll
+        for (uint32_t j = 0; j < RO_AHEAD; ++j) {
+            const uint32_t i = token + j * a.side;
+            if (i >= end) continue;
+            slot[j] = query ? 0 : a.slots[i];
+            x[j] = P::load(from + i * plane.src_token + at);
+            y[j] = P::load(from + i * plane.src_token + (both ? two : at));
         }
-        it.both = it.two < a.dim;
-        const bool query = row < a.heads, key = !query && row < a.heads + a.kv_heads;
-        const uint32_t head = query ? row : key ? row - a.heads : row - a.heads - a.kv_heads;
-        const Plane& p = query ? a.q : key ? a.k : a.v;
-        it.turn = query || key;
-        const Bits* from = static_cast<const Bits*>(p.src) + token * p.src_token + head * p.src_head;
-        Bits* to;
-        if (query) {
-            to = static_cast<Bits*>(p.dst) + token * p.dst_token + head * p.dst_head;
-        } else {
-            const int64_t slot = a.slots[token];
-            const uint64_t page = static_cast<uint64_t>(slot) >> a.page_lg, off = slot & ((1u << a.page_lg) - 1u);
-            to = static_cast<Bits*>(p.dst) + (key ? page * a.k_page + off * a.k_slot + head * a.k_head
-                                                  : page * a.v_page + off * a.v_slot + head * a.v_head);
-            if (slot < 0 || static_cast<uint64_t>(slot) >= a.n_slots) to = nullptr;
-        }
-        it.to = to;
-        it.x = P::load(from + it.at);
-        it.y = P::load(from + (it.both ? it.two : it.at));
-        return it;
     };
-    auto finish = [&](Item it) {
-        const float2* turn = s_turn + it.token * a.half;
-        if (it.turn) {
-            if (NEXT) {
-                if constexpr (N == 1) {
-                    if (it.at < turned) {
-                        const float2 w = turn[it.at / 2];
-                        const float x = it.x.get(0), y = it.y.get(0);
-                        it.x.set(0, __builtin_fmaf(x, w.x, -(y * w.y)));
-                        it.y.set(0, __builtin_fmaf(y, w.x, x * w.y));
+    auto pair = [](float2 w, float u, float v) {
+        return make_float2(__builtin_fmaf(u, w.x, -(v * w.y)), __builtin_fmaf(v, w.x, u * w.y));
+    };
+    auto finish = [&](uint32_t token) {
+#pragma unroll
+        for (uint32_t j = 0; j < RO_AHEAD; ++j) {
+            const uint32_t i = token + j * a.side;
+            if (i >= end) continue;
+            const float2* w = s_turn + (i - token0) * a.half;
+            if (turn) {
+                if constexpr (NEXT && N > 1) {
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e += 2) {
+                        if (at + e < turned) {
+                            const float2 z = pair(w[(at + e) / 2], x[j].get(e), x[j].get(e + 1));
+                            x[j].set(e, z.x);
+                            x[j].set(e + 1, z.y);
+                        }
+                        if (two + e < turned) {
+                            const float2 z = pair(w[(two + e) / 2], y[j].get(e), y[j].get(e + 1));
+                            y[j].set(e, z.x);
+                            y[j].set(e + 1, z.y);
+                        }
                     }
                 } else {
 #pragma unroll
-                    for (uint32_t e = 0; e < N; e += 2) {
-                        if (it.at + e < turned) {
-                            const float2 w = turn[(it.at + e) / 2];
-                            const float x = it.x.get(e), y = it.x.get(e + 1);
-                            it.x.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
-                            it.x.set(e + 1, __builtin_fmaf(y, w.x, x * w.y));
-                        }
-                        if (it.two + e < turned) {
-                            const float2 w = turn[(it.two + e) / 2];
-                            const float x = it.y.get(e), y = it.y.get(e + 1);
-                            it.y.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
-                            it.y.set(e + 1, __builtin_fmaf(y, w.x, x * w.y));
-                        }
+                    for (uint32_t e = 0; e < N; ++e) {
+                        const float2 z = pair(w[NEXT ? at / 2 : at + e], x[j].get(e), y[j].get(e));
+                        x[j].set(e, z.x);
+                        y[j].set(e, z.y);
                     }
                 }
-            } else if (it.at < turned) {
-#pragma unroll
-                for (uint32_t e = 0; e < N; ++e) {
-                    const float2 w = turn[it.at + e];
-                    const float x = it.x.get(e), y = it.y.get(e);
-                    it.x.set(e, __builtin_fmaf(x, w.x, -(y * w.y)));
-                    it.y.set(e, __builtin_fmaf(y, w.x, x * w.y));
-                }
             }
-        }
-        if (it.to) {
-            it.x.store(it.to + it.at);
-            if (it.both) it.y.store(it.to + it.two);
+            Bits* out = to;
+            if (query) {
+                out += i * plane.dst_token;
+            } else {
+                if (slot[j] < 0 || static_cast<uint64_t>(slot[j]) >= a.n_slots) continue;
+                out += (static_cast<uint64_t>(slot[j]) >> a.page_lg) * page_stride +
+                       (slot[j] & ((1u << a.page_lg) - 1u)) * slot_stride;
+            }
+            x[j].store(out + at);
+            if (both) y[j].store(out + two);
         }
     };
-    const uint32_t step = RO_NT * a.splits;
-    uint32_t i = part * RO_NT + t;
-    Item it[RO_AHEAD];
-#pragma unroll
-    for (uint32_t j = 0; j < RO_AHEAD; ++j)
-        if (i + j * step < items) it[j] = load(i + j * step);
+    if (there) load(first);
     const float m = __uint_as_float(a.magnitude_bits);
-    for (uint32_t k = t; k < tokens * a.half; k += RO_NT)
+    for (uint32_t k = t; k < (end - token0) * a.half; k += blockDim.x)
         s_turn[k] = cos_sin(a.positions[token0 + k / a.half], a.freqs[k % a.half], m);
     __syncthreads();
-    while (i < items) {
-#pragma unroll
-        for (uint32_t j = 0; j < RO_AHEAD; ++j)
-            if (i + j * step < items) finish(it[j]);
-        i += RO_AHEAD * step;
-#pragma unroll
-        for (uint32_t j = 0; j < RO_AHEAD; ++j)
-            if (i + j * step < items) it[j] = load(i + j * step);
+    if (!there) return;
+    for (uint32_t i = first; i < end; i += RO_AHEAD * a.side) {
+        finish(i);
+        load(i + RO_AHEAD * a.side);
     }
 }
 
 template <class E, uint32_t N>
-void launch_rotary(const RotaryArgs& a, bool next, uint32_t grid, hipStream_t s)
+void launch_rotary(const RotaryArgs& a, bool next, uint32_t grid, uint32_t threads, hipStream_t s)
 {
     if (next)
-        ro_turn<E, N, true><<<grid, RO_NT, 0, s>>>(a);
+        ro_turn<E, N, true><<<grid, threads, 0, s>>>(a);
     else
-        ro_turn<E, N, false><<<grid, RO_NT, 0, s>>>(a);
+        ro_turn<E, N, false><<<grid, threads, 0, s>>>(a);
 }
 
 }  // namespace
@@ -262,16 +245,16 @@ extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_
     }
     if (per_token == 0) return CR_OK;
     a.per_token = static_cast<uint32_t>(per_token);
-    // A workgroup's cosines serve all heads of its tokens.  Enough tokens for two
-    // rounds of pieces where there are many; where there are few, several workgroups
-    // share a token.
-    const uint32_t fit = a.half ? RO_PAIRS / a.half : 64;
-    const uint32_t want = std::max<uint32_t>(1, (RO_AHEAD * RO_NT + a.per_token - 1) / a.per_token);
-    a.tokens = std::min({want, fit, std::max<uint32_t>(1, p.n_tokens / num_cus())});
-    const uint32_t groups = (p.n_tokens + a.tokens - 1) / a.tokens;
-    const uint32_t rounds = (a.tokens * a.per_token + RO_NT - 1) / RO_NT;
-    a.splits = std::max<uint32_t>(1, std::min(rounds, num_cus() / groups));
-    const uint64_t grid = static_cast<uint64_t>(groups) * a.splits;
+    // A workgroup's threads share a token's pieces, in several workgroups where there are more,
+    // or take several tokens side by side.  Its cosines serve all of its tokens: as many as
+    // still leave workgroups for the whole card.
+    a.side = std::max(1u, static_cast<uint32_t>(RO_NT) / a.per_token);
+    a.rounds = a.side > 1 ? 1u : (a.per_token + RO_NT - 1) / RO_NT;
+    const uint32_t threads = a.side > 1 ? RO_NT : ((a.per_token + a.rounds - 1) / a.rounds + 63) / 64 * 64;
+    const uint32_t fit = a.half ? RO_PAIRS / a.half : 1u << 16;
+    const uint64_t share = static_cast<uint64_t>(p.n_tokens) * a.rounds / (8ull * num_cus());
+    a.tokens = static_cast<uint32_t>(std::min<uint64_t>(fit, std::max<uint64_t>(a.side, std::min<uint64_t>(2ull * RO_AHEAD * a.side, share))));
+    const uint64_t grid = static_cast<uint64_t>((p.n_tokens + a.tokens - 1) / a.tokens) * a.rounds;
     if (grid >> 23) {  // a launch holds fewer than 2^32 threads
         set_error("cr_paged_rotary: too many tokens for one call");
         return CR_ERR_UNSUPPORTED;
@@ -282,25 +265,25 @@ extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_
     const bool next = p.interleaved != 0;
     if (cache->dtype == CR_F32) {
         if (n == 4)
-            launch_rotary<F32, 4>(a, next, g, s);
+            launch_rotary<F32, 4>(a, next, g, threads, s);
         else if (n == 2)
-            launch_rotary<F32, 2>(a, next, g, s);
+            launch_rotary<F32, 2>(a, next, g, threads, s);
         else
-            launch_rotary<F32, 1>(a, next, g, s);
+            launch_rotary<F32, 1>(a, next, g, threads, s);
     } else if (cache->dtype == CR_F16) {
         if (n == 8)
-            launch_rotary<F16, 8>(a, next, g, s);
+            launch_rotary<F16, 8>(a, next, g, threads, s);
         else if (n == 4)
-            launch_rotary<F16, 4>(a, next, g, s);
+            launch_rotary<F16, 4>(a, next, g, threads, s);
         else
-            launch_rotary<F16, 1>(a, next, g, s);
+            launch_rotary<F16, 1>(a, next, g, threads, s);
     } else {
         if (n == 8)
-            launch_rotary<BF16, 8>(a, next, g, s);
+            launch_rotary<BF16, 8>(a, next, g, threads, s);
         else if (n == 4)
-            launch_rotary<BF16, 4>(a, next, g, s);
+            launch_rotary<BF16, 4>(a, next, g, threads, s);
         else
-            launch_rotary<BF16, 1>(a, next, g, s);
+            launch_rotary<BF16, 1>(a, next, g, threads, s);
     }
     CR_LAUNCH_CHECK();
     return CR_OK;
