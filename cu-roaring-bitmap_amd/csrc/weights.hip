@@ -151,8 +151,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                     const uint32_t d = s * 32 + g * 8;
                     key[i][s] = v8s{};
                     if (from[i] != 0xFFFFFFFFu && d < a.dim)
-                        key[i][s] = __builtin_nontemporal_load(
-                            reinterpret_cast<const v8s*>(a.k + at[i] + h * a.k_head + d));
+                        key[i][s] = *reinterpret_cast<const v8s*>(a.k + at[i] + h * a.k_head + d);
                 }
             for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
                 v8s q[STEPS];
