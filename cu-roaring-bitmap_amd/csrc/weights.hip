@@ -96,63 +96,107 @@ __device__ __forceinline__ Counted counted_of(const WeightArgs& a, uint32_t r)
             static_cast<uint32_t>(min(room, static_cast<uint64_t>(len))), static_cast<int64_t>(a.kv_len[r]) - (t1 - t0)};
 }
 
+// 16 bytes a lane from memory to LDS, lane after lane from `to`, which is the same for the wave.
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
+{
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// How rows lie in LDS: turned by pieces of 16 bytes so that the rows of a fragment share no
+// banks.
+template <uint32_t DIM>
+struct Lines {
+    static constexpr uint32_t CHUNKS = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;  // 16-byte pieces of a row
+    static constexpr uint32_t STRIDE = CHUNKS * 8;                             // its elements
+    static constexpr uint32_t TURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
+};
+
 // Up to this many rows that share a key head in a request, wt_rows.
 constexpr uint32_t WT_FEW = 32;
 
+// ---- few rows: bound by reading the keys -------------------------------------------------
+// A workgroup per span of a request's positions.  Its waves share the key heads, and
+// where there are fewer heads than waves the span; a wave takes the keys of its
+// positions, one head after another, through LDS of its own, to which they go whole
+// lines at a time and without passing through registers, and which hands them out as the
+// columns of 16x16x32 products whose rows are the queries.
 constexpr int WR_NT = 256;
 constexpr uint32_t WR_WAVES = WR_NT / 64;
-constexpr uint32_t WR_TILES = 4;  // of 16 positions, a wave's
+constexpr uint32_t WR_BYTES = 16384;  // of a wave's LDS
 
-// A workgroup per span of a request's positions.  Its waves share the key heads, and
-// where there are fewer heads than waves the span; a wave keeps the keys of its
-// positions in registers, one head after another, as the columns of 16x16x32 products
-// whose rows are the queries.
+// Positions of a wave.
+constexpr uint32_t row_tiles(uint32_t chunks) { return WR_BYTES / (chunks * 16) / 16 > 4 ? 4 : WR_BYTES / (chunks * 16) / 16; }
+constexpr uint32_t row_cols(uint32_t dim) { return row_tiles(dim <= 64 ? 8 : dim <= 128 ? 16 : 32) * 16; }
+
 template <class E, uint32_t DIM>
 __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 {
-    constexpr uint32_t STEPS = DIM / 32;
-    __shared__ float s_sum[WR_WAVES][WR_TILES * 16];
-    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c16 = lane & 15u, g = lane >> 4;
+    using L = Lines<DIM>;
+    constexpr uint32_t STEPS = DIM / 32, TILES = row_tiles(L::CHUNKS), COLS = TILES * 16;
+    constexpr uint32_t PER = 64 / L::CHUNKS, LOADS = COLS / PER;  // rows that an instruction covers, instructions
+    __shared__ alignas(16) uint16_t s_key[WR_WAVES][COLS * L::STRIDE];
+    __shared__ uint64_t s_at[WR_WAVES][COLS];
+    __shared__ uint32_t s_from[WR_WAVES][COLS];
+    __shared__ float s_sum[WR_WAVES][COLS];
+    const uint32_t lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15u, g = lane >> 4;
     const uint32_t r = blockIdx.x / a.spans, tile_waves = WR_WAVES / a.head_waves;
     const uint32_t head_wave = wave % a.head_waves, tile_wave = wave / a.head_waves;
     const Counted t = counted_of(a, r);
-    const uint32_t group = a.heads / a.kv_heads, rows = t.tokens * group, step = tile_waves * WR_TILES * 16;
+    const uint32_t group = a.heads / a.kv_heads, rows = t.tokens * group, step = tile_waves * COLS;
+    uint16_t* sk = s_key[wave];
+    if (a.dim < DIM) {  // pieces behind the head dimension: zeros, as the queries that they meet
+#pragma unroll
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t row = x * PER + lane / L::CHUNKS, pos = lane % L::CHUNKS;
+            if ((pos ^ (row & L::TURN)) * 8 >= a.dim) *reinterpret_cast<v8s*>(sk + row * L::STRIDE + pos * 8) = v8s{};
+        }
+    }
     // (more than once where the caller's most positions are fewer than there are)
     for (uint32_t first = blockIdx.x % a.spans * step; first < t.keys; first += a.spans * step) {
-        const uint32_t p0 = first + tile_wave * WR_TILES * 16;
-        uint64_t at[WR_TILES];
-        uint32_t from[WR_TILES];  // the first row that sees the lane's position
-        float sum[WR_TILES], part[WR_TILES];  // long sums in two steps, which lose less
-#pragma unroll
-        for (uint32_t i = 0; i < WR_TILES; ++i) {
-            const uint32_t p = p0 + i * 16 + c16;
-            sum[i] = part[i] = 0.0f;
-            at[i] = 0;
-            from[i] = 0xFFFFFFFFu;
+        // Lane l looks after position l of the wave's: where its keys lie, and the first row that
+        // sees it.
+        const uint32_t p0 = first + tile_wave * COLS;
+        if (lane < COLS) {
+            const uint32_t p = p0 + lane;
+            uint64_t at = 0;
+            uint32_t from = 0xFFFFFFFFu;
             if (p < t.keys) {
                 const uint32_t page = static_cast<uint32_t>(a.table[r * a.table_stride + (p >> a.page_lg)]);
                 const uint32_t off = p & ((1u << a.page_lg) - 1u), slot = (page << a.page_lg) + off;
                 bool see = page < a.n_pages;
-                if (see && a.gated)
-                    see = slot < a.visible.end && ((a.visible.word(slot >> 5) >> (slot & 31u)) & 1u);
+                if (see && a.gated) see = slot < a.visible.end && ((a.visible.word(slot >> 5) >> (slot & 31u)) & 1u);
                 const int64_t token = a.causal ? max(static_cast<int64_t>(0), static_cast<int64_t>(p) - t.older) : 0;
                 if (see && token < t.tokens) {
-                    at[i] = page * a.k_page + off * a.k_slot;
-                    from[i] = static_cast<uint32_t>(token) * group;
+                    at = page * a.k_page + off * a.k_slot;
+                    from = static_cast<uint32_t>(token) * group;
                 }
             }
+            s_at[wave][lane] = at;
+            s_from[wave][lane] = from;
         }
-        for (uint32_t h = head_wave; h < a.kv_heads; h += a.head_waves) {
-            v8s key[WR_TILES][STEPS];
+        wave_lds_fence();
+        uint64_t at[LOADS];
+        uint32_t on = 0, from[TILES];
+        float sum[TILES], part[TILES];  // long sums in two steps, which lose less
 #pragma unroll
-            for (uint32_t i = 0; i < WR_TILES; ++i)
+        for (uint32_t x = 0; x < LOADS; ++x) {
+            const uint32_t row = x * PER + lane / L::CHUNKS, d = (lane % L::CHUNKS ^ (row & L::TURN)) * 8;
+            at[x] = s_at[wave][row] + d;
+            on |= (s_from[wave][row] != 0xFFFFFFFFu && d < a.dim ? 1u : 0u) << x;
+        }
+        bool any = false;
 #pragma unroll
-                for (uint32_t s = 0; s < STEPS; ++s) {
-                    const uint32_t d = s * 32 + g * 8;
-                    key[i][s] = v8s{};
-                    if (from[i] != 0xFFFFFFFFu && d < a.dim)
-                        key[i][s] = *reinterpret_cast<const v8s*>(a.k + at[i] + h * a.k_head + d);
-                }
+        for (uint32_t i = 0; i < TILES; ++i) {
+            from[i] = s_from[wave][i * 16 + c16];
+            any = any || __ballot(from[i] != 0xFFFFFFFFu) != 0;
+            sum[i] = part[i] = 0.0f;
+        }
+        for (uint32_t h = head_wave; any && h < a.kv_heads; h += a.head_waves) {
+            const uint16_t* kp = a.k + h * a.k_head;
+#pragma unroll
+            for (uint32_t x = 0; x < LOADS; ++x)
+                if ((on >> x) & 1u) load_to_lds(kp + at[x], sk + x * PER * L::STRIDE);
             for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
                 v8s q[STEPS];
                 const uint32_t mine = min(row0 + c16, rows - 1);
@@ -170,38 +214,45 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                     const float z = a.lse[static_cast<uint64_t>(t.token0 + row / group) * a.heads + h * group + row % group];
                     lse2[e] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
                 }
+                // the wave's own keys are in LDS
+                if (row0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-                for (uint32_t i = 0; i < WR_TILES; ++i) {
+                for (uint32_t i = 0; i < TILES; ++i) {
                     f32x4 x = {0, 0, 0, 0};
+                    const uint32_t row = i * 16 + c16;
 #pragma unroll
-                    for (uint32_t s = 0; s < STEPS; ++s) x = E::mfma16(q[s], key[i][s], x);
+                    for (uint32_t s = 0; s < STEPS; ++s) {
+                        const v8s key = *reinterpret_cast<const v8s*>(sk + row * L::STRIDE + ((s * 4 + g) ^ (row & L::TURN)) * 8);
+                        x = E::mfma16(q[s], key, x);
+                    }
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        const uint32_t row = row0 + g * 4 + e;
+                        const uint32_t at_row = row0 + g * 4 + e;
                         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse2[e]));
-                        part[i] += row >= from[i] && row < rows ? w : 0.0f;
+                        part[i] += at_row >= from[i] && at_row < rows ? w : 0.0f;
                     }
                 }
                 if (row0 % 1024 == 1008 || row0 + 16 >= rows) {
 #pragma unroll
-                    for (uint32_t i = 0; i < WR_TILES; ++i) {
+                    for (uint32_t i = 0; i < TILES; ++i) {
                         sum[i] += part[i];
                         part[i] = 0.0f;
                     }
                 }
             }
+            wave_lds_fence();  // its keys are read before the next head's arrive
         }
 #pragma unroll
-        for (uint32_t i = 0; i < WR_TILES; ++i) {
+        for (uint32_t i = 0; i < TILES; ++i) {
             sum[i] += __shfl_xor(sum[i], 16, 64);
             sum[i] += __shfl_xor(sum[i], 32, 64);
             if (g == 0) s_sum[wave][i * 16 + c16] = sum[i];
         }
         __syncthreads();
         // the heads' sums joined in a fixed order
-        const uint32_t in = threadIdx.x % (WR_TILES * 16), of = threadIdx.x / (WR_TILES * 16);
-        const uint32_t p = first + of * WR_TILES * 16 + in;
-        if (of < tile_waves && p < t.keys) {
+        for (uint32_t i = threadIdx.x; i < step; i += WR_NT) {
+            const uint32_t p = first + i, of = i / COLS, in = i % COLS;
+            if (p >= t.keys) break;
             float all = 0.0f;
             for (uint32_t w = 0; w < a.head_waves; ++w) all += s_sum[of * a.head_waves + w][in];
             const float past =
@@ -218,17 +269,12 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 // products; the queries pass by through LDS, 64 rows at a time, where the next ones
 // arrive meanwhile without passing through registers.  A lane sums what its two
 // columns get; the parts' sums are joined by another kernel, heads and parts in order.
-// Rows of LDS are turned by pieces of 16 bytes so that the 32 rows of a fragment
-// share no banks.
 constexpr int WT_NT = 256;
 constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
 
 template <uint32_t DIM>
-struct Stage {
-    static constexpr uint32_t CHUNKS = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;  // 16-byte pieces of a row in LDS
-    static constexpr uint32_t STRIDE = CHUNKS * 8;                             // its elements
-    static constexpr uint32_t TURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
-    static constexpr uint32_t PER = WT_NT / CHUNKS, LOADS = WT_ROWS / PER;  // rows that the workgroup loads at once
+struct Stage : Lines<DIM> {
+    static constexpr uint32_t PER = WT_NT / Lines<DIM>::CHUNKS, LOADS = WT_ROWS / PER;  // rows that the workgroup loads at once
 };
 
 // Blocks of 32 positions whose keys a wave holds; positions of a workgroup's tile.
@@ -256,12 +302,6 @@ __device__ __forceinline__ void rows_of_part(const WeightArgs& a, const Counted&
     const uint64_t sees = static_cast<uint64_t>(first_row(a, t, p, group)) / 32 * 32;
     end = static_cast<uint32_t>(min(static_cast<uint64_t>(rows), from + size));
     first = static_cast<uint32_t>(min(static_cast<uint64_t>(end), max(from, sees)));
-}
-
-__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
-{
-    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void*)from,
-                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
 template <class E, uint32_t DIM>
@@ -589,7 +629,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         o_sums = cv.add(parts * p.n_requests * a.kv_heads * room * 4);
     } else {
         a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
-        const uint32_t span = WR_WAVES / a.head_waves * WR_TILES * 16;
+        const uint32_t span = WR_WAVES / a.head_waves * row_cols(a.dim);
         a.spans = static_cast<uint32_t>((most + span - 1) / span);
         grid = static_cast<uint64_t>(a.spans) * a.n_requests;
         if (grid >> 23) {
