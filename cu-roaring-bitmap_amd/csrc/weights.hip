@@ -97,10 +97,13 @@ __device__ __forceinline__ Counted counted_of(const WeightArgs& a, uint32_t r)
 }
 
 // 16 bytes a lane from memory to LDS, lane after lane from `to`, which is the same for the wave.
+// ONCE: data that no other workgroup reads.
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to)
 {
+    constexpr int NONTEMPORAL = 2;
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void*)from,
-                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, ONCE ? NONTEMPORAL : 0);
 }
 
 // How rows lie in LDS: turned by pieces of 16 bytes so that the rows of a fragment share no
@@ -123,7 +126,7 @@ constexpr uint32_t WT_FEW = 32;
 // columns of 16x16x32 products whose rows are the queries.
 constexpr int WR_NT = 256;
 constexpr uint32_t WR_WAVES = WR_NT / 64;
-constexpr uint32_t WR_BYTES = 16384;  // of a wave's LDS
+constexpr uint32_t WR_BYTES = 8192;  // of a wave's LDS
 
 // Positions of a wave.
 constexpr uint32_t row_tiles(uint32_t chunks) { return WR_BYTES / (chunks * 16) / 16 > 4 ? 4 : WR_BYTES / (chunks * 16) / 16; }
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
             const uint16_t* kp = a.k + h * a.k_head;
 #pragma unroll
             for (uint32_t x = 0; x < LOADS; ++x)
-                if ((on >> x) & 1u) load_to_lds(kp + at[x], sk + x * PER * L::STRIDE);
+                if ((on >> x) & 1u) load_to_lds<true>(kp + at[x], sk + x * PER * L::STRIDE);
             for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
                 v8s q[STEPS];
                 const uint32_t mine = min(row0 + c16, rows - 1);
@@ -356,7 +359,7 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 #pragma unroll
             for (uint32_t x = 0; x < S::LOADS; ++x) {
                 const uint32_t lr = x * S::PER + lrow, d = (lpos ^ (lr & S::TURN)) * 8;
-                if (d < a.dim) load_to_lds(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
+                if (d < a.dim) load_to_lds<false>(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
             }
         };
         __syncthreads();  // the tile before is done with LDS
