@@ -73,7 +73,9 @@ struct WeightArgs {
     uint64_t out_stride;
     float scale2;  // scale * log2(e)
     bool causal, continued;
-    uint32_t head_waves, spans;  // few rows: waves that share the heads; workgroups of a request
+    // Few rows: waves that share the heads, workgroups of a request, and how often a wave's LDS
+    // is filled with positions that it looks up at once.
+    uint32_t head_waves, spans, halves;
     // Many rows: parts of a request's rows, of part_rows or more each; tiles of positions
     // that the launch has for a request; and their sums [n_requests][parts][key heads][room].
     uint32_t parts, part_rows, tiles, room;
@@ -139,14 +141,14 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
     constexpr uint32_t STEPS = DIM / 32, TILES = row_tiles(L::CHUNKS), COLS = TILES * 16;
     constexpr uint32_t PER = 64 / L::CHUNKS, LOADS = COLS / PER;  // rows that an instruction covers, instructions
     __shared__ alignas(16) uint16_t s_key[WR_WAVES][COLS * L::STRIDE];
-    __shared__ uint64_t s_at[WR_WAVES][COLS];
-    __shared__ uint32_t s_from[WR_WAVES][COLS];
-    __shared__ float s_sum[WR_WAVES][COLS];
+    __shared__ uint64_t s_at[WR_WAVES][64];
+    __shared__ uint32_t s_from[WR_WAVES][64];
+    __shared__ float s_sum[WR_WAVES][64];
     const uint32_t lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15u, g = lane >> 4;
     const uint32_t r = blockIdx.x / a.spans, tile_waves = WR_WAVES / a.head_waves;
     const uint32_t head_wave = wave % a.head_waves, tile_wave = wave / a.head_waves;
     const Counted t = counted_of(a, r);
-    const uint32_t group = a.heads / a.kv_heads, rows = t.tokens * group, step = tile_waves * COLS;
+    const uint32_t group = a.heads / a.kv_heads, rows = t.tokens * group, per_wave = a.halves * COLS, step = tile_waves * per_wave;
     uint16_t* sk = s_key[wave];
     if (a.dim < DIM) {  // pieces behind the head dimension: zeros, as the queries that they meet
 #pragma unroll
@@ -159,8 +161,8 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
     for (uint32_t first = blockIdx.x % a.spans * step; first < t.keys; first += a.spans * step) {
         // Lane l looks after position l of the wave's: where its keys lie, and the first row that
         // sees it.
-        const uint32_t p0 = first + tile_wave * COLS;
-        if (lane < COLS) {
+        const uint32_t p0 = first + tile_wave * per_wave;
+        if (lane < per_wave) {
             const uint32_t p = p0 + lane;
             uint64_t at = 0;
             uint32_t from = 0xFFFFFFFFu;
@@ -179,82 +181,84 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
             s_from[wave][lane] = from;
         }
         wave_lds_fence();
-        uint64_t at[LOADS];
-        uint32_t on = 0, from[TILES];
-        float sum[TILES], part[TILES];  // long sums in two steps, which lose less
+        for (uint32_t half = 0; half < a.halves; ++half) {
+            uint64_t at[LOADS];
+            uint32_t on = 0, from[TILES];
+            float sum[TILES], part[TILES];  // long sums in two steps, which lose less
 #pragma unroll
-        for (uint32_t x = 0; x < LOADS; ++x) {
-            const uint32_t row = x * PER + lane / L::CHUNKS, d = (lane % L::CHUNKS ^ (row & L::TURN)) * 8;
-            at[x] = s_at[wave][row] + d;
-            on |= (s_from[wave][row] != 0xFFFFFFFFu && d < a.dim ? 1u : 0u) << x;
-        }
-        bool any = false;
+            for (uint32_t x = 0; x < LOADS; ++x) {
+                const uint32_t row = x * PER + lane / L::CHUNKS, d = (lane % L::CHUNKS ^ (row & L::TURN)) * 8;
+                at[x] = s_at[wave][half * COLS + row] + d;
+                on |= (s_from[wave][half * COLS + row] != 0xFFFFFFFFu && d < a.dim ? 1u : 0u) << x;
+            }
+            bool any = false;
 #pragma unroll
-        for (uint32_t i = 0; i < TILES; ++i) {
-            from[i] = s_from[wave][i * 16 + c16];
-            any = any || __ballot(from[i] != 0xFFFFFFFFu) != 0;
-            sum[i] = part[i] = 0.0f;
-        }
-        for (uint32_t h = head_wave; any && h < a.kv_heads; h += a.head_waves) {
-            const uint16_t* kp = a.k + h * a.k_head;
+            for (uint32_t i = 0; i < TILES; ++i) {
+                from[i] = s_from[wave][half * COLS + i * 16 + c16];
+                any = any || __ballot(from[i] != 0xFFFFFFFFu) != 0;
+                sum[i] = part[i] = 0.0f;
+            }
+            for (uint32_t h = head_wave; any && h < a.kv_heads; h += a.head_waves) {
+                const uint16_t* kp = a.k + h * a.k_head;
 #pragma unroll
-            for (uint32_t x = 0; x < LOADS; ++x)
-                if ((on >> x) & 1u) load_to_lds<true>(kp + at[x], sk + x * PER * L::STRIDE);
-            for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
-                v8s q[STEPS];
-                const uint32_t mine = min(row0 + c16, rows - 1);
-                const uint16_t* qp =
-                    a.q + (t.token0 + mine / group) * a.q_token + (h * group + mine % group) * a.q_head;
-#pragma unroll
-                for (uint32_t s = 0; s < STEPS; ++s) {
-                    const uint32_t d = s * 32 + g * 8;
-                    q[s] = d < a.dim ? *reinterpret_cast<const v8s*>(qp + d) : v8s{};
-                }
-                float lse2[4];
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    const uint32_t row = min(row0 + g * 4 + e, rows - 1);
-                    const float z = a.lse[static_cast<uint64_t>(t.token0 + row / group) * a.heads + h * group + row % group];
-                    lse2[e] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
-                }
-                // the wave's own keys are in LDS
-                if (row0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-                for (uint32_t i = 0; i < TILES; ++i) {
-                    f32x4 x = {0, 0, 0, 0};
-                    const uint32_t row = i * 16 + c16;
+                for (uint32_t x = 0; x < LOADS; ++x)
+                    if ((on >> x) & 1u) load_to_lds<true>(kp + at[x], sk + x * PER * L::STRIDE);
+                for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
+                    v8s q[STEPS];
+                    const uint32_t mine = min(row0 + c16, rows - 1);
+                    const uint16_t* qp =
+                        a.q + (t.token0 + mine / group) * a.q_token + (h * group + mine % group) * a.q_head;
 #pragma unroll
                     for (uint32_t s = 0; s < STEPS; ++s) {
-                        const v8s key = *reinterpret_cast<const v8s*>(sk + row * L::STRIDE + ((s * 4 + g) ^ (row & L::TURN)) * 8);
-                        x = E::mfma16(q[s], key, x);
+                        const uint32_t d = s * 32 + g * 8;
+                        q[s] = d < a.dim ? *reinterpret_cast<const v8s*>(qp + d) : v8s{};
                     }
+                    float lse2[4];
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        const uint32_t at_row = row0 + g * 4 + e;
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse2[e]));
-                        part[i] += at_row >= from[i] && at_row < rows ? w : 0.0f;
+                        const uint32_t row = min(row0 + g * 4 + e, rows - 1);
+                        const float z = a.lse[static_cast<uint64_t>(t.token0 + row / group) * a.heads + h * group + row % group];
+                        lse2[e] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
                     }
-                }
-                if (row0 % 1024 == 1008 || row0 + 16 >= rows) {
+                    // the wave's own keys are in LDS
+                    if (row0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
                     for (uint32_t i = 0; i < TILES; ++i) {
-                        sum[i] += part[i];
-                        part[i] = 0.0f;
+                        f32x4 x = {0, 0, 0, 0};
+                        const uint32_t row = i * 16 + c16;
+#pragma unroll
+                        for (uint32_t s = 0; s < STEPS; ++s) {
+                            const v8s key = *reinterpret_cast<const v8s*>(sk + row * L::STRIDE + ((s * 4 + g) ^ (row & L::TURN)) * 8);
+                            x = E::mfma16(q[s], key, x);
+                        }
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const uint32_t at_row = row0 + g * 4 + e;
+                            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse2[e]));
+                            part[i] += at_row >= from[i] && at_row < rows ? w : 0.0f;
+                        }
+                    }
+                    if (row0 % 1024 == 1008 || row0 + 16 >= rows) {
+#pragma unroll
+                        for (uint32_t i = 0; i < TILES; ++i) {
+                            sum[i] += part[i];
+                            part[i] = 0.0f;
+                        }
                     }
                 }
+                wave_lds_fence();  // its keys are read before the next head's arrive
             }
-            wave_lds_fence();  // its keys are read before the next head's arrive
-        }
 #pragma unroll
-        for (uint32_t i = 0; i < TILES; ++i) {
-            sum[i] += __shfl_xor(sum[i], 16, 64);
-            sum[i] += __shfl_xor(sum[i], 32, 64);
-            if (g == 0) s_sum[wave][i * 16 + c16] = sum[i];
+            for (uint32_t i = 0; i < TILES; ++i) {
+                sum[i] += __shfl_xor(sum[i], 16, 64);
+                sum[i] += __shfl_xor(sum[i], 32, 64);
+                if (g == 0) s_sum[wave][half * COLS + i * 16 + c16] = sum[i];
+            }
         }
         __syncthreads();
         // the heads' sums joined in a fixed order
         for (uint32_t i = threadIdx.x; i < step; i += WR_NT) {
-            const uint32_t p = first + i, of = i / COLS, in = i % COLS;
+            const uint32_t p = first + i, of = i / per_wave, in = i % per_wave;
             if (p >= t.keys) break;
             float all = 0.0f;
             for (uint32_t w = 0; w < a.head_waves; ++w) all += s_sum[of * a.head_waves + w][in];
@@ -632,7 +636,13 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         o_sums = cv.add(parts * p.n_requests * a.kv_heads * room * 4);
     } else {
         a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
-        const uint32_t span = WR_WAVES / a.head_waves * row_cols(a.dim);
+        // A wave looks up 64 positions at once and fills its LDS with them two or four times where there
+        // is work for many rounds of the card, which saves look-ups (64 requests of 16384 positions, 8
+        // heads of 128: 174 -> 167 us), and fills it once where the last round counts (32 requests of
+        // 4096: 27 us, not 32).
+        const uint32_t fill = WR_WAVES / a.head_waves * row_cols(a.dim);
+        a.halves = row_cols(a.dim) <= 32 && most * p.n_requests > 16ull * num_cus() * fill ? 64 / row_cols(a.dim) : 1;
+        const uint32_t span = a.halves * fill;
         a.spans = static_cast<uint32_t>((most + span - 1) / span);
         grid = static_cast<uint64_t>(a.spans) * a.n_requests;
         if (grid >> 23) {
