@@ -334,6 +334,25 @@ __device__ __forceinline__ uint32_t staying(uint32_t len, uint32_t keep, uint32_
     return keep >= len ? len : max(keep, n_safe);
 }
 
+// The pages of a request's first m entries, and how many it holds behind them.
+__device__ __forceinline__ uint32_t pages_freed(const EvictArgs& a, uint32_t len, uint32_t m, uint32_t& first)
+{
+    const uint64_t page = 1ull << a.page_lg;
+    first = static_cast<uint32_t>((m + page - 1) >> a.page_lg);
+    return static_cast<uint32_t>((len + page - 1) >> a.page_lg) - first;
+}
+
+// Their list, behind `before` pages of other requests.
+template <int NT>
+__device__ __forceinline__ uint32_t list_freed(const EvictArgs& a, uint32_t r, uint32_t len, uint32_t m, uint32_t before)
+{
+    uint32_t first;
+    const uint32_t n = pages_freed(a, len, m, first);
+    for (uint32_t i = threadIdx.x; i < n; i += NT)
+        if (before + i < a.freed_cap) a.freed[before + i] = a.table[r * a.table_stride + first + i];
+    return n;
+}
+
 constexpr uint64_t EV_WHOLE = 16384;  // entries of a request that one workgroup takes
 
 // A workgroup a request of at most E * NT entries, whose places in the order stay in
@@ -359,6 +378,7 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
         if (t == 0) {
             a.len[r] = static_cast<int32_t>(len);
             a.n_moves[r] = 0;
+            if (a.n_requests == 1) a.counts[0] = a.counts[1] = 0;
         }
         return;
     }
@@ -478,9 +498,15 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
         }
         move_entries<EV_MOVES>(a, ages, r, from, to, at, on);
     }
+    uint32_t freed = 0;
+    if (a.n_requests == 1) freed = list_freed<NT>(a, r, len, m, 0);
     if (t == 0) {
         a.len[r] = static_cast<int32_t>(m);
         a.n_moves[r] = static_cast<int32_t>(total);
+        if (a.n_requests == 1) {
+            a.counts[0] = static_cast<int32_t>(freed);
+            a.counts[1] = static_cast<int32_t>(total);
+        }
     }
 }
 
@@ -779,16 +805,9 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
 }
 
 // The pages that get free, requests in order: a workgroup a request, which counts
-// those of the requests before it.  Of long rows, the moves' weights and slots too,
+// those of the requests before it (one request in one workgroup does without).  Of long rows, the moves' weights and slots too,
 // which a workgroup a segment shares.
 constexpr int EF_NT = 256;
-
-__device__ __forceinline__ uint32_t pages_freed(const EvictArgs& a, uint32_t r, uint32_t& first)
-{
-    const uint64_t page = 1ull << a.page_lg;
-    first = static_cast<uint32_t>((static_cast<uint64_t>(a.len[r]) + page - 1) >> a.page_lg);
-    return static_cast<uint32_t>((request_len(a, r) + page - 1) >> a.page_lg) - first;
-}
 
 __global__ __launch_bounds__(EF_NT) void ev_finish(EvictArgs a, uint32_t per)
 {
@@ -814,14 +833,13 @@ __global__ __launch_bounds__(EF_NT) void ev_finish(EvictArgs a, uint32_t per)
     if (part) return;
     const bool last = r + 1 == a.n_requests;
     uint32_t before = 0, moves = 0, first;
-    for (uint32_t i = t; i < r; i += EF_NT) before += pages_freed(a, i, first);
+    for (uint32_t i = t; i < r; i += EF_NT)
+        before += pages_freed(a, request_len(a, i), static_cast<uint32_t>(a.len[i]), first);
     if (last)
         for (uint32_t i = t; i < a.n_requests; i += EF_NT) moves += static_cast<uint32_t>(a.n_moves[i]);
     before = block_sum<EF_NT>(before, s_sum);
     if (last) moves = block_sum<EF_NT>(moves, s_sum);
-    const uint32_t n = pages_freed(a, r, first);
-    for (uint32_t i = t; i < n; i += EF_NT)
-        if (before + i < a.freed_cap) a.freed[before + i] = a.table[r * a.table_stride + first + i];
+    const uint32_t n = list_freed<EF_NT>(a, r, request_len(a, r), static_cast<uint32_t>(a.len[r]), before);
     if (last && t == 0) {
         a.counts[0] = static_cast<int32_t>(before + n);
         a.counts[1] = static_cast<int32_t>(moves);
@@ -988,7 +1006,9 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
                         &a.pinned));
     CR_TIMED("ev_pick", s);
     const uint32_t n = p.n_requests, parts = static_cast<uint32_t>(segments);
-    if (room <= 4096) {
+    if (room <= 1024) {
+        ev_pick<256, 4><<<n, 256, 0, s>>>(a);
+    } else if (room <= 4096) {
         ev_pick<1024, 4><<<n, 1024, 0, s>>>(a);
     } else if (whole) {
         ev_pick<512, 32><<<n, 512, 0, s>>>(a);
@@ -1000,7 +1020,7 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
         sg_place<<<parts, SG_NT, 0, s>>>(a);
     }
     const uint32_t per = whole ? 1 : a.segments;
-    ev_finish<<<n * per, EF_NT, 0, s>>>(a, per);
+    if (!whole || n > 1) ev_finish<<<n * per, EF_NT, 0, s>>>(a, per);
     CR_LAUNCH_CHECK();
     return CR_OK;
 }
