@@ -160,7 +160,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
     // (more than once where the caller's most positions are fewer than there are)
     for (uint32_t first = blockIdx.x % a.spans * step; first < t.keys; first += a.spans * step) {
         // Lane l looks after position l of the wave's: where its keys lie, and the first row that
-        // sees it.
+        // sees it, of rows numbered from 1.
         const uint32_t p0 = first + tile_wave * per_wave;
         if (lane < per_wave) {
             const uint32_t p = p0 + lane;
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                 const int64_t token = a.causal ? max(static_cast<int64_t>(0), static_cast<int64_t>(p) - t.older) : 0;
                 if (see && token < t.tokens) {
                     at = page * a.k_page + off * a.k_slot;
-                    from = static_cast<uint32_t>(token) * group;
+                    from = static_cast<uint32_t>(token) * group + 1;
                 }
             }
             s_at[wave][lane] = at;
@@ -214,11 +214,13 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                         q[s] = d < a.dim ? *reinterpret_cast<const v8s*>(qp + d) : v8s{};
                     }
                     float lse2[4];
+                    uint32_t number[4];  // 0: counts for nothing
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        const uint32_t row = min(row0 + g * 4 + e, rows - 1);
+                        const uint32_t at_row = row0 + g * 4 + e, row = min(at_row, rows - 1);
                         const float z = a.lse[static_cast<uint64_t>(t.token0 + row / group) * a.heads + h * group + row % group];
-                        lse2[e] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
+                        lse2[e] = z * LOG2E;
+                        number[e] = at_row < rows && z != -__builtin_inff() ? at_row + 1 : 0u;
                     }
                     // the wave's own keys are in LDS
                     if (row0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -233,9 +235,8 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                         }
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e) {
-                            const uint32_t at_row = row0 + g * 4 + e;
                             const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse2[e]));
-                            part[i] += at_row >= from[i] && at_row < rows ? w : 0.0f;
+                            part[i] += number[e] >= from[i] ? w : 0.0f;
                         }
                     }
                     if (row0 % 1024 == 1008 || row0 + 16 >= rows) {
@@ -277,6 +278,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 // arrive meanwhile without passing through registers.  A lane sums what its two
 // columns get; the parts' sums are joined by another kernel, heads and parts in order.
 constexpr int WT_NT = 256;
+__device__ __attribute__((aligned(16))) uint16_t wt_zeros[WT_DIM_MAX];
 constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
 
 template <uint32_t DIM>
@@ -356,14 +358,18 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             const uint64_t token = t.token0 + row / group;
             const uint32_t head = kh * group + row % group;
             const float z = a.lse[token * a.heads + head];
-            s_at[i % 4][lane] = token * a.q_token + head * a.q_head;
-            s_lse[i % 4][lane] = z == -__builtin_inff() ? __builtin_inff() : z * LOG2E;
+            const bool none = z == -__builtin_inff();  // counts for nothing, whatever it holds
+            const uint16_t* at = none ? wt_zeros : a.q + token * a.q_token + head * a.q_head;
+            s_at[i % 4][lane] = reinterpret_cast<uint64_t>(at);
+            s_lse[i % 4][lane] = none ? __builtin_inff() : z * LOG2E;
         };
         auto load = [&](uint32_t i, uint16_t* sq) {
 #pragma unroll
             for (uint32_t x = 0; x < S::LOADS; ++x) {
                 const uint32_t lr = x * S::PER + lrow, d = (lpos ^ (lr & S::TURN)) * 8;
-                if (d < a.dim) load_to_lds<false>(a.q + s_at[i % 4][lr] + d, sq + (x * S::PER + wave_row) * S::STRIDE);
+                if (d < a.dim)
+                    load_to_lds<false>(reinterpret_cast<const uint16_t*>(s_at[i % 4][lr]) + d,
+                                       sq + (x * S::PER + wave_row) * S::STRIDE);
             }
         };
         __syncthreads();  // the tile before is done with LDS
@@ -571,9 +577,9 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
                   "supported (type %u, %u dimensions)", WT_DIM_MAX, cache->dtype, cache->head_dim);
         return CR_ERR_UNSUPPORTED;
     }
-    if (n_slots >> 31 || room >> 31 || p.n_tokens >> 31 || p.n_heads > 65535 || p.n_requests >> 24 ||
+    if (n_slots >> 31 || room >> 31 || p.n_tokens >> 31 || p.n_heads > 65535 || p.n_requests >> 22 ||
         (static_cast<uint64_t>(p.n_tokens) * p.n_heads) >> 31) {
-        set_error("cr_paged_weights: supported up to 2^31 - 1 slots, positions and rows, 65535 heads and 2^24 - 1 "
+        set_error("cr_paged_weights: supported up to 2^31 - 1 slots, positions and rows, 65535 heads and 2^22 - 1 "
                   "requests");
         return CR_ERR_UNSUPPORTED;
     }
@@ -669,7 +675,8 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     }
     if (many) {
         CR_TIMED("wt_join", s);
-        const uint32_t per_request = static_cast<uint32_t>(std::min<uint64_t>((most + 63) / 64, std::max<uint64_t>(1, (1u << 22) / p.n_requests)));
+        // (fewer than 2^32 threads)
+        const uint32_t per_request = static_cast<uint32_t>(std::min<uint64_t>((most + 63) / 64, ((1u << 22) - 1) / p.n_requests));
         wt_join<<<per_request * p.n_requests, WJ_NT, 0, s>>>(a, per_request, cols);
     }
     CR_LAUNCH_CHECK();

@@ -500,9 +500,9 @@ int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_cache* cach
  * row t sees entries [0, older + t].  (A prompt's last tokens are counted alone with
  * d_starts moved up to them; after a verification, the accepted ones with d_new and
  * a shorter d_kv_len.)  lse [n_tokens][n_heads] is what the attention of these rows
- * left, with the same scale; a row whose lse is -inf counts for nothing.  `visible`, a
- * bitmap over the slots, or NULL: others got nothing, nor did entries whose page is
- * outside the cache.  d_past may be d_out, or NULL: nothing before.  Sums are in
+ * left, with the same scale; a row whose lse is -inf counts for nothing, whatever its q
+ * holds.  `visible`, a bitmap over the slots, or NULL: others got nothing, nor did
+ * entries whose page is outside the cache.  d_past may be d_out, or NULL: nothing before.  Sums are in
  * fp32, in an order that depends on the arguments alone.  Entries behind d_kv_len[r]
  * are left as they were.  Types and alignment are those of cr_paged_attention;
  * cache->v is not looked at. */
@@ -542,7 +542,7 @@ int cr_paged_weights(const cr_paged_weights_args* args, const cr_paged_cache* ca
  * order, into the places in [0, m) that get free: d_moves[r][0, d_n_moves[r]) are
  * pairs (from slot, to slot) for cr_paged_move, never the same slot twice, and
  * d_weights_out[r][0, m) and d_positions_out[r][0, m) (NULL: not wanted) what then
- * lies there; those two may be the inputs themselves.  A row of d_moves holds half as
+ * lies there; those two may be the inputs themselves, the lengths may not.  A row of d_moves holds half as
  * many pairs as a row of the table has positions.  d_freed[0, freed_cap) receives the
  * pages that no entry of their request is in any more, requests in order, and
  * d_counts[0, 2) their number and that of all moves.  The table stays as it is:
@@ -616,7 +616,8 @@ int cr_beam_reorder(const void* d_src, const int32_t* d_parents, uint32_t batch,
  * that was not, or from p of the last row (from p, where nothing else is left): the
  * lowest token at which the running sum exceeds d_uniform[last row] times the whole;
  * then -1 up to out_cols.  d_accepted[r] counts the accepted ones.  A score that is
- * NaN or -inf has probability 0, scores of +inf share it evenly; after a row without a
+ * NaN or -inf, or below the row's largest by more than 693 temperatures, has
+ * probability 0, scores of +inf share it evenly; after a row without a
  * candidate no draft is accepted and the token is -1, as for a request without rows.
  * `allowed` and d_allowed_bits are those of cr_beam_select, a set of bits for each
  * row of d_scores.  Probabilities and their sums are in fp64. */

@@ -231,6 +231,20 @@ def test_rows_that_count_for_nothing(gpu):
     p.check(gpu)
 
 
+@pytest.mark.parametrize("what", ["decode ragged", "a few tokens", "chunk", "prompt", "dims 192", "dims 256"])
+def test_rows_that_count_for_nothing_may_hold_anything(gpu, what):
+    """Padding: queries that are NaN or infinite, with a log-sum of -inf."""
+    _say("weights of rows that hold anything", what)
+    p = Problem("bfloat16", *SHAPES[what], seed=20)
+    gone = [(t, h) for t in range(0, p.q.shape[0], 3) for h in range(t % 2, p.heads, 2)]
+    for t, h in gone:
+        p.lse[t, h] = float("-inf")
+    want = p.run(gpu)
+    for i, (t, h) in enumerate(gone):
+        p.q[t, h] = float("nan") if i % 2 else float("inf")
+    assert np.array_equal(p.run(gpu), want)
+
+
 def test_weights_add_up_to_the_rows(gpu):
     """A row's weights sum to one: the attention's own log-sum goes in, and out comes the number of rows."""
     import torch

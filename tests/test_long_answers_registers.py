@@ -18,7 +18,7 @@ def test_no_kernel_spills(tmp_path):
         for kernel in notes.split("- .agpr_count:")[1:]:
             value = lambda key: re.search(rf"\.{key}:\s*(\S+)", kernel).group(1)  # noqa: E731
             name = value("symbol")
-            if re.search(r"\d(ro|wt|ev|dv)_[a-z]+", name):
+            if re.search(r"\d(ro|wt|ev|sg|dv)_[a-z]+", name):
                 seen[name] = int(value("private_segment_fixed_size")), int(value("vgpr_spill_count"))
     assert any("wt_tiles" in k for k in seen) and any("dv_sums" in k for k in seen), sorted(seen)
     assert set(seen.values()) == {(0, 0)}, {k: v for k, v in seen.items() if v != (0, 0)}
