@@ -805,8 +805,8 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
 }
 
 // The pages that get free, requests in order: a workgroup a request, which counts
-// those of the requests before it (one request in one workgroup does without).  Of long rows, the moves' weights and slots too,
-// which a workgroup a segment shares.
+// those of the requests before it (one request in one workgroup does without).  Of
+// long rows, the moves' weights and slots too, which a workgroup a segment shares.
 constexpr int EF_NT = 256;
 
 __global__ __launch_bounds__(EF_NT) void ev_finish(EvictArgs a, uint32_t per)
@@ -941,6 +941,15 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     if (n_slots >> 31 || room >> 30 || p.n_requests >> 20 || p.sinks >> 31 || p.recent >> 31) {
         set_error("cr_paged_evict: supported up to 2^31 - 1 slots, 2^30 - 1 positions and 2^20 - 1 requests");
         return CR_ERR_UNSUPPORTED;
+    }
+    // What is written is read again behind it: not over the lengths that are asked.
+    auto meets = [&](const int32_t* x) {
+        auto over = [&](const int32_t* y) { return x && y && x < y + p.n_requests && y < x + p.n_requests; };
+        return over(p.d_len) || over(p.d_n_moves);
+    };
+    if (meets(p.d_kv_len) || meets(p.d_keep) || meets(p.d_kept) || meets(p.d_seen)) {
+        set_error("cr_paged_evict: invalid argument (the lengths that are written lie over those that are read)");
+        return CR_ERR_INVALID;
     }
     hipStream_t s = as_stream(stream);
     if (p.n_requests == 0) return fill_u32(reinterpret_cast<uint32_t*>(p.d_counts), 0, 2, s);

@@ -53,7 +53,7 @@ WEIGHTS = dict(q=P, q_token_stride=256, q_head_stride=64, lse=P, n_tokens=3, n_h
     ({}, dict(dtype=cr.F32), UNSUPPORTED), ({}, dict(head_dim=264), UNSUPPORTED), ({}, dict(head_dim=60), UNSUPPORTED),
     (dict(q=P + 8), {}, UNSUPPORTED), (dict(q_head_stride=68), {}, UNSUPPORTED), ({}, dict(k_slot_stride=132), UNSUPPORTED),
     ({}, dict(n_pages=1 << 28), UNSUPPORTED), (dict(n_tokens=1 << 31), {}, UNSUPPORTED),
-    (dict(n_requests=1 << 24), {}, UNSUPPORTED), (dict(n_tokens=1 << 30), {}, UNSUPPORTED),
+    (dict(n_requests=1 << 24), {}, UNSUPPORTED), (dict(n_requests=1 << 22), {}, UNSUPPORTED), (dict(n_tokens=1 << 30), {}, UNSUPPORTED),
     (dict(table_cols=1 << 24, table_stride=1 << 24, out_stride=1 << 28, n_requests=256), {}, UNSUPPORTED),
     (dict(n_requests=0, q=None), {}, OK), (dict(table_cols=0, d_table=None, d_out=None), dict(v=None), OK)])
 def test_weights(args, cache, code):
@@ -63,8 +63,8 @@ def test_weights(args, cache, code):
 
 EVICT = dict(d_weights=P, weights_stride=64, d_positions=P, positions_stride=64, d_kept=P, d_seen=P, d_kv_len=P, d_keep=P,
              d_table=P, table_cols=4, table_stride=4, page_size=16, n_pages=8, n_requests=2, sinks=1, recent=2,
-             d_weights_out=P, weights_out_stride=64, d_positions_out=P, positions_out_stride=64, d_len=P, d_moves=P,
-             moves_cap=32, moves_stride=32, d_n_moves=P, d_freed=P, freed_cap=8, d_counts=P)
+             d_weights_out=P, weights_out_stride=64, d_positions_out=P, positions_out_stride=64, d_len=P + 256, d_moves=P,
+             moves_cap=32, moves_stride=32, d_n_moves=P + 512, d_freed=P, freed_cap=8, d_counts=P)
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -75,7 +75,9 @@ EVICT = dict(d_weights=P, weights_stride=64, d_positions=P, positions_stride=64,
     (dict(positions_out_stride=63), INVALID), (dict(d_len=None), INVALID), (dict(d_moves=None), INVALID),
     (dict(moves_cap=31), INVALID), (dict(moves_stride=31), INVALID), (dict(d_n_moves=None), INVALID),
     (dict(d_freed=None), INVALID), (dict(d_counts=None), INVALID), (dict(n_pages=1 << 28), UNSUPPORTED),
-    (dict(n_requests=1 << 20), UNSUPPORTED), (dict(sinks=1 << 31), UNSUPPORTED), (dict(recent=1 << 31), UNSUPPORTED)])
+    (dict(n_requests=1 << 20), UNSUPPORTED), (dict(sinks=1 << 31), UNSUPPORTED), (dict(recent=1 << 31), UNSUPPORTED),
+    (dict(d_len=P), INVALID), (dict(d_len=P + 4), INVALID), (dict(d_kept=P + 252), INVALID), (dict(d_n_moves=P - 4), INVALID),
+    (dict(d_seen=P + 516), INVALID)])
 def test_evict(bad, code):
     assert cr.load().cr_paged_evict(C.byref(_filled(cr.PagedEvictArgs, EVICT, bad)), None) == code
     assert b"cr_paged_evict" in cr._lib.cr_last_error()
