@@ -142,6 +142,25 @@ def test_verify(gpu, rows, vocab, dtype, draft):
         Problem(rows, vocab, dtype, seed=seed, draft=draft).check(gpu)
 
 
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("noise", [0.5, 0.01])
+@pytest.mark.parametrize("rows", [[9] * 4, [10] * 4, [40], [33] + [1] * 9, [1, 25, 1, 0, 3, 2], [64, 65, 66], [14, 0, 14, 0, 14]])
+def test_verify_many_rows(gpu, rows, noise, draft):
+    """Requests whose rows are decided by a launch of their own, and long ones among short ones, which are not."""
+    _say("verify many rows", rows[:4], noise, draft)
+    for vocab in (37, 4099):
+        Problem(rows, vocab, "bfloat16", seed=len(rows), noise=noise, draft=draft).check(gpu)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("rows,vocab", [([3, 2], 131072), ([3, 2], 140001), ([12], 140001), ([2], 300007)])
+def test_verify_long_rows(gpu, rows, vocab, draft):
+    """More pieces of a row than a wave has lanes."""
+    _say("verify long rows", rows, vocab, draft)
+    Problem(rows, vocab, "float16", seed=21, draft=draft).check(gpu)
+    Problem(rows, vocab, "float16", seed=22, draft=draft, density=0.3, kind="bitmap").check(gpu)
+
+
 @pytest.mark.parametrize("kind", ["bitmap", "arrays", "flat", "rows"])
 @pytest.mark.parametrize("density", [0.0, 0.01, 0.3, 1.0])
 def test_verify_allowed(gpu, kind, density):
