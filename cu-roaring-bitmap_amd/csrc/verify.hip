@@ -328,6 +328,43 @@ struct Tokens {
     }
 };
 
+// Of a piece's tokens, where few may be used, those alone, by their numbers in LDS, in order: one
+// unit a lane.  Exponentials are what a piece costs, and scores that nobody asks for need not be
+// read: 64 requests of 4 drafts over 100003 bf16 tokens take 38 us with a fifth of them allowed and
+// 27 with a thousandth, 48 to 52 either way where all are read.  Asking first costs where many are
+// allowed after all, 55 us and not 52 with 45%, of which a list would make 64.
+constexpr uint32_t DV_FEW = 64 * DV_UNIT;
+
+struct Few {
+    uint32_t total;
+    bool is;  // few enough to be listed
+
+    __device__ __forceinline__ Few(const VerifyArgs& a, const Mask& mask, uint32_t piece, uint16_t* s)
+    {
+        static_assert(DV_PIECE == 64 * 32, "a word a lane");
+        const uint32_t lane = __lane_id(), first = piece * DV_PIECE + lane * 32u;
+        const uint32_t left = first < mask.end ? mask.end - first : 0u;
+        uint32_t bits = (mask.words[min(first, a.vocab - 1) / 32u] & mask.keep) ^ mask.flip;
+        bits &= left >= 32u ? 0xFFFFFFFFu : (1u << left) - 1u;
+        const uint32_t n = __popc(bits), upto = wave_incl_scan(n);
+        total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+        is = total <= DV_FEW;
+        if (!is) return;
+        for (uint32_t to = upto - n; bits; bits &= bits - 1) s[to++] = static_cast<uint16_t>(lane * 32u + __builtin_ctz(bits));
+        wave_lds_fence();
+    }
+    // Their scores, DV_UNIT a lane, -inf behind the last; p: the piece's.
+    template <class E>
+    __device__ __forceinline__ void get(const typename E::Bits* p, const uint16_t* s, float (&x)[DV_UNIT]) const
+    {
+#pragma unroll
+        for (uint32_t e = 0; e < DV_UNIT; ++e) {
+            const uint32_t i = e * 64 + __lane_id();
+            x[e] = i < total ? E::up(p[s[i]]) : -__builtin_inff();
+        }
+    }
+};
+
 __device__ __forceinline__ bool is_allowed(const VerifyArgs& a, uint64_t row, uint32_t token)
 {
     if (!a.masked) return true;
@@ -365,23 +402,46 @@ __device__ __forceinline__ bool is_last(const VerifyArgs& a, uint32_t row)
 }
 
 // Every row's pieces, a wave each; the drafting model's rows behind the model's.
-template <class E>
-__global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
+template <class E, bool MASKED>
+__global__ __launch_bounds__(DV_NT) __attribute__((amdgpu_waves_per_eu(6))) void dv_sums(VerifyArgs a)
 {
     __shared__ double s_pow[DV_POWERS];
-    const uint32_t lane = __lane_id();
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * DV_WAVES + (threadIdx.x >> 6));
+    __shared__ uint16_t s_few[DV_WAVES][MASKED ? DV_FEW : 1];
+    const uint32_t lane = __lane_id(), in_group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wave = blockIdx.x * DV_WAVES + in_group;
     const uint32_t at = wave / a.pieces, first = wave % a.pieces * DV_PIECE + lane * DV_UNIT;
     const bool there = at < (a.draft ? 2 : 1) * a.n_rows, drafted = at >= a.n_rows;
     const uint32_t row = drafted ? at - a.n_rows : at;
     const auto* p = static_cast<const typename E::Bits*>(drafted ? a.draft : a.x) +
                     row * (drafted ? a.draft_row : a.x_row);
-    Tokens<E, DV_STEPS> tokens;
     const Mask mask(a, there ? row : 0u, first);
-    if (there) tokens.load(a, p, mask, first);
-    make_powers<DV_NT>(s_pow);
-    if (!there || (drafted && is_last(a, row))) return;
-    float x[DV_STEPS][DV_UNIT], top = -__builtin_inff();
+    float top = -__builtin_inff();
+    double mass = 0.0;
+    Tokens<E, DV_STEPS> tokens;
+    if constexpr (MASKED) {
+        make_powers<DV_NT>(s_pow);
+        if (!there || (drafted && is_last(a, row))) return;
+        const Few few(a, mask, wave % a.pieces, s_few[in_group]);
+        if (few.is) {
+            float x[1][DV_UNIT];
+            few.get<E>(p + wave % a.pieces * DV_PIECE, s_few[in_group], x[0]);
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[0][e]);
+            top = wave_max(top);
+            if (top > -__builtin_inff()) mass = wave_sum_f64(Shares(a, top).sum(x, s_pow));
+            if (lane == 0) {
+                a.top[wave] = top;
+                a.mass[wave] = mass;
+            }
+            return;
+        }
+        tokens.load(a, p, mask, first);
+    } else {
+        if (there) tokens.load(a, p, mask, first);
+        make_powers<DV_NT>(s_pow);
+        if (!there || (drafted && is_last(a, row))) return;
+    }
+    float x[DV_STEPS][DV_UNIT];
 #pragma unroll
     for (uint32_t u = 0; u < DV_STEPS; ++u) {
         tokens.scores(mask, first, u, x[u]);
@@ -389,7 +449,6 @@ __global__ __launch_bounds__(DV_NT) void dv_sums(VerifyArgs a)
         for (uint32_t e = 0; e < DV_UNIT; ++e) top = fmaxf(top, x[u][e]);
     }
     top = wave_max(top);
-    double mass = 0.0;
     if (top > -__builtin_inff()) mass = wave_sum_f64(Shares(a, top).sum(x, s_pow));
     if (lane == 0) {
         a.top[wave] = top;
@@ -522,14 +581,20 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
     return d;
 }
 
+// max(p - q, 0) of shares and what they are multiplied by, each product rounded by itself, so that
+// equal shares leave nothing.
+__device__ __forceinline__ double left_of(double p, double p_part, double q, double q_part)
+{
+#pragma clang fp contract(off)
+    return fmax(p * p_part - q * q_part, 0.0);
+}
+
 // max(p - q, 0), or p behind the last draft (or where `plain`), of a lane's tokens from
 // `first` on: U units, f(u, those of unit u).
 template <class E, uint32_t U, class F>
 __device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, uint32_t first, bool plain, const double* s_pow,
                                         F f)
 {
-    // each product rounded by itself, so that equal shares leave nothing
-#pragma clang fp contract(off)
     const bool both = a.draft && d.rejected && !plain && d.q.part > 0.0;
     const bool drop = !a.draft && d.rejected && !plain;
     const Mask mask(a, d.row, first);
@@ -549,7 +614,7 @@ __device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, 
             of_draft.scores(mask, first, u, x);
             q.of(x, s_pow, y);
 #pragma unroll
-            for (uint32_t e = 0; e < DV_UNIT; ++e) rest[e] = fmax(rest[e] * p_part - y[e] * q_part, 0.0);
+            for (uint32_t e = 0; e < DV_UNIT; ++e) rest[e] = left_of(rest[e], p_part, y[e], q_part);
         } else {
 #pragma unroll
             for (uint32_t e = 0; e < DV_UNIT; ++e) {
@@ -562,9 +627,10 @@ __device__ __forceinline__ void rest_of(const VerifyArgs& a, const Decision& d, 
 }
 
 // The pieces' sums of what the next token is drawn from, a wave a piece.
-template <class E>
+template <class E, bool MASKED>
 __global__ __launch_bounds__(DV_NT) __attribute__((amdgpu_waves_per_eu(4))) void dv_rest(VerifyArgs a, uint32_t groups)
 {
+    __shared__ uint16_t s_few[DV_WAVES][MASKED ? DV_FEW : 1];
     __shared__ double s_pow[DV_POWERS];
     __shared__ RowState s_state[DV_WAVES];
     const uint32_t r = blockIdx.x / groups, lane = __lane_id();
@@ -575,8 +641,34 @@ __global__ __launch_bounds__(DV_NT) __attribute__((amdgpu_waves_per_eu(4))) void
     const Decision d = decide<E>(a, rows, s_pow, s_state);
     if (piece == 0 && lane == 0) a.decided[r] = d;
     if (piece >= a.pieces) return;
+    const uint32_t first = piece * DV_PIECE + lane * DV_UNIT;
     double sum = 0.0;
-    rest_of<E, DV_STEPS>(a, d, piece * DV_PIECE + lane * DV_UNIT, false, s_pow, [&](uint32_t, const double (&rest)[DV_UNIT]) {
+    if constexpr (MASKED) {
+        const Mask mask(a, d.row, first);
+        const uint16_t* listed = s_few[threadIdx.x >> 6];
+        const Few few(a, mask, piece, s_few[threadIdx.x >> 6]);
+        if (few.is) {
+            const bool both = d.rejected && d.q.part > 0.0;
+            const uint64_t from = static_cast<uint64_t>(piece) * DV_PIECE;
+            const auto* px = static_cast<const typename E::Bits*>(a.x) + d.row * a.x_row + from;
+            const auto* py = static_cast<const typename E::Bits*>(a.draft) + d.row * a.draft_row + from;
+            const Shares p(a, d.p.top), q(a, d.q.top);
+            float x[DV_UNIT];
+            double rest[DV_UNIT], y[DV_UNIT] = {};
+            few.get<E>(px, listed, x);
+            p.of(x, s_pow, rest);
+            if (both) {
+                few.get<E>(py, listed, x);
+                q.of(x, s_pow, y);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < DV_UNIT; ++e) sum += left_of(rest[e], d.p.part, y[e], d.q.part);
+            sum = wave_sum_f64(sum);
+            if (lane == 0) a.rest[static_cast<uint64_t>(r) * a.pieces + piece] = sum;
+            return;
+        }
+    }
+    rest_of<E, DV_STEPS>(a, d, first, false, s_pow, [&](uint32_t, const double (&rest)[DV_UNIT]) {
 #pragma unroll
         for (uint32_t e = 0; e < DV_UNIT; ++e) sum += rest[e];
     });
@@ -697,7 +789,11 @@ int launch_verify(const VerifyArgs& a, hipStream_t s)
     const uint64_t waves = static_cast<uint64_t>(a.draft ? 2 : 1) * a.n_rows * a.pieces;
     if (waves) {
         CR_TIMED("dv_sums", s);
-        dv_sums<E><<<static_cast<unsigned>((waves + DV_WAVES - 1) / DV_WAVES), DV_NT, 0, s>>>(a);
+        const unsigned grid = static_cast<unsigned>((waves + DV_WAVES - 1) / DV_WAVES);
+        if (a.masked)
+            dv_sums<E, true><<<grid, DV_NT, 0, s>>>(a);
+        else
+            dv_sums<E, false><<<grid, DV_NT, 0, s>>>(a);
     }
     if (a.n_rows && !a.folded) {
         CR_TIMED("dv_norms", s);
@@ -706,7 +802,10 @@ int launch_verify(const VerifyArgs& a, hipStream_t s)
     if (a.draft) {
         CR_TIMED("dv_rest", s);
         const uint32_t groups = (a.pieces + DV_WAVES - 1) / DV_WAVES;
-        dv_rest<E><<<a.n_requests * groups, DV_NT, 0, s>>>(a, groups);
+        if (a.masked)
+            dv_rest<E, true><<<a.n_requests * groups, DV_NT, 0, s>>>(a, groups);
+        else
+            dv_rest<E, false><<<a.n_requests * groups, DV_NT, 0, s>>>(a, groups);
     }
     CR_TIMED("dv_pick", s);
     dv_pick<E><<<a.n_requests, DV_NT, 0, s>>>(a);

@@ -177,6 +177,24 @@ def test_verify_temperatures(gpu, temperature):
         Problem([4, 3, 5] * 4, 3001, "float32", seed=6, temperature=temperature, draft=draft).check(gpu)
 
 
+@pytest.mark.parametrize("kind", ["bitmap", "arrays", "flat", "rows"])
+@pytest.mark.parametrize("count", [0, 1, 511, 512, 513, 2047, 2048])
+def test_allowed_tokens_of_a_piece(gpu, kind, count):
+    """So many of every 2048 tokens, in one run or scattered."""
+    _say("verify allowed of 2048", kind, count)
+    for draft in (True, False):
+        for scattered in (True, False):
+            p = Problem([4, 1, 6], 7000, "bfloat16", seed=23, density=0.5, kind=kind, draft=draft)
+            for rows in (p.allowed if kind == "rows" else p.allowed[:1]):
+                rows[:] = False
+                for first in range(0, 7000, 2048):
+                    n = min(2048, 7000 - first)
+                    rows[first + (p.rng.permutation(n)[:count] if scattered else np.arange(n)[max(0, n - count):])] = True
+            if kind != "rows":
+                p.allowed[:] = p.allowed[:1]
+            p.check(gpu)
+
+
 def test_verify_strides(gpu):
     """Rows that lie apart and begin anywhere."""
     _say("verify strides")
