@@ -21,6 +21,7 @@ constexpr int EV_NT = 1024;
 constexpr uint32_t EV_SAFE = 0xFFFFFFFFu;  // above the order of every weight
 constexpr uint32_t EV_BINS = 2048;         // of a digit of 11 bits
 constexpr uint32_t EV_COPIES = 4;          // of the first digit's counts
+constexpr uint32_t EV_ALL = 0xFFFFFFFFu;   // ties: all that equal the last stay
 constexpr uint32_t EV_NO_DIGIT = 2046;     // a first digit above those of all weights and below that of EV_SAFE
 
 struct EvictArgs {
@@ -100,11 +101,11 @@ struct Ages {  // of a request's entries
 };
 
 // Finds the digit in which the n-th largest of the counted values lies (n >= 1, at
-// most their number).  count(bin): how many have it.  Every thread gets the digit and
-// how many values have a higher one.
+// most their number).  count(bin): how many have it.  Every thread gets the digit, how
+// many values have a higher one, and how many have it.
 template <int NT, class F>
 __device__ __forceinline__ void find_digit(F count, uint32_t n, uint32_t* s_scan, uint32_t* s_found, uint32_t& digit,
-                                           uint32_t& above)
+                                           uint32_t& above, uint32_t& here)
 {
     constexpr uint32_t PER = EV_BINS / NT;
     const uint32_t t = threadIdx.x;
@@ -120,12 +121,14 @@ __device__ __forceinline__ void find_digit(F count, uint32_t n, uint32_t* s_scan
         if (before < n && n <= before + c[j]) {
             s_found[0] = EV_BINS - 1 - (t * PER + j);
             s_found[1] = before;
+            s_found[2] = c[j];
         }
         before += c[j];
     }
     __syncthreads();
     digit = s_found[0];
     above = s_found[1];
+    here = s_found[2];
     __syncthreads();
 }
 
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
     constexpr uint32_t ROWS = E / 4, WAVES = NT / 64, HOLES = E * NT / 2;
     __shared__ uint32_t s_mem[EV_COPIES * EV_BINS > HOLES ? EV_COPIES * EV_BINS : HOLES];  // counts, then holes
     __shared__ uint32_t s_movers[HOLES];
-    __shared__ uint32_t s_scan[WAVES], s_found[2], s_of[2][WAVES];
+    __shared__ uint32_t s_scan[WAVES], s_found[3], s_of[2][WAVES];
     const uint32_t r = blockIdx.x, t = threadIdx.x, lane = __lane_id(), wave = t >> 6;
     const uint32_t len = request_len(a, r);
     const Ages ages(a, r, len);
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
     // Of the others, the m - n_safe largest stay.
     uint32_t last = EV_SAFE, ties = 0;
     if (m > n_safe) {
-        uint32_t n = m - n_safe, digit, above;
+        uint32_t n = m - n_safe, digit, above, here;
         find_digit<NT>(
             [&](uint32_t bin) {
                 uint32_t c = 0;
@@ -410,7 +413,7 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
                 for (uint32_t k = 0; k < EV_COPIES; ++k) c += s_mem[k * EV_BINS + bin];
                 return c;
             },
-            n, s_scan, s_found, digit, above);
+            n, s_scan, s_found, digit, above, here);
         n -= above;
         last = digit << 21;
 #pragma unroll
@@ -425,16 +428,17 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
                     if (i0 + j * 256 + e < len && key[j][e] >> (shift + bits) == last >> (shift + bits))
                         atomicAdd(&s_mem[(key[j][e] >> shift) & mask], 1u);
             __syncthreads();
-            find_digit<NT>([&](uint32_t bin) { return s_mem[bin]; }, n, s_scan, s_found, digit, above);
+            find_digit<NT>([&](uint32_t bin) { return s_mem[bin]; }, n, s_scan, s_found, digit, above, here);
             n -= above;
             last |= digit << shift;
         }
-        ties = n;
+        ties = n < here ? n : EV_ALL;
     }
     // Which stay, and how many holes and movers lie before each lane's four: both counts and
     // the ties' fit one word for a wave's 256.
     uint32_t tie0 = 0;
-    if (ties) {
+    const bool ranked = ties != 0 && ties != EV_ALL;
+    if (ranked) {
         uint32_t n = 0;
 #pragma unroll
         for (uint32_t j = 0; j < ROWS; ++j) n += ties4(key[j], below4(i0 + j * 256, len), last);
@@ -448,7 +452,7 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
     for (uint32_t j = 0; j < ROWS; ++j) {
         const uint32_t i = i0 + j * 256, in = below4(i, len), mine = below4(i, m);
         uint32_t tie = tie0;
-        if (ties) {
+        if (ranked) {
             const uint32_t n = ties4(key[j], in, last), upto = wave_incl_scan(n);
             tie = tie0 + upto - n;
             tie0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
@@ -558,7 +562,7 @@ __global__ __launch_bounds__(SG_NT) void sg_keys(EvictArgs a)
 // picked[2 r]: m, the digit, how many stay of those that have it, the request's segments.
 __global__ __launch_bounds__(EV_NT) void sg_digit(EvictArgs a)
 {
-    __shared__ uint32_t s_scan[EV_NT / 64], s_found[2];
+    __shared__ uint32_t s_scan[EV_NT / 64], s_found[3];
     const uint32_t r = blockIdx.x, t = threadIdx.x, len = request_len(a, r);
     const uint32_t keep = static_cast<uint32_t>(max(a.keep[r], 0)), segments = (len + SG_SIZE - 1) / SG_SIZE;
     const uint64_t seg0 = static_cast<uint64_t>(r) * a.segments;
@@ -566,12 +570,12 @@ __global__ __launch_bounds__(EV_NT) void sg_digit(EvictArgs a)
     for (uint32_t i = t; i < segments; i += EV_NT) n_safe += a.counts_of[seg0 + i].w;
     n_safe = block_sum<EV_NT>(n_safe, s_scan);
     const uint32_t m = staying(len, keep, n_safe);
-    uint32_t digit = EV_NO_DIGIT, above = 0;
+    uint32_t digit = EV_NO_DIGIT, above = 0, here;
     if (m > n_safe) {
         static_assert(EV_BINS == 2 * EV_NT, "a word of two counts per thread");
         const uint32_t word = (EV_BINS - 1 - t * 2) / 2;
         uint32_t lo = 0, hi = 0;
-        constexpr uint32_t AHEAD = 8;
+        constexpr uint32_t AHEAD = 32;
         for (uint32_t i = 0; i < segments; i += AHEAD) {
             uint32_t x[AHEAD];
 #pragma unroll
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(EV_NT) void sg_digit(EvictArgs a)
                 hi += i + k < segments ? x[k] >> 16 : 0u;
             }
         }
-        find_digit<EV_NT>([&](uint32_t bin) { return bin & 1u ? hi : lo; }, m - n_safe, s_scan, s_found, digit, above);
+        find_digit<EV_NT>([&](uint32_t bin) { return bin & 1u ? hi : lo; }, m - n_safe, s_scan, s_found, digit, above, here);
     }
     if (t == 0) a.picked[2 * r] = make_uint4(m, digit, m > n_safe ? m - n_safe - above : 0u, segments);
 }
@@ -662,7 +666,7 @@ __global__ __launch_bounds__(SG_NT) void sg_split(EvictArgs a)
 __global__ __launch_bounds__(EV_NT) void sg_decide(EvictArgs a)
 {
     constexpr uint32_t WAVES = EV_NT / 64;
-    __shared__ uint32_t s_bins[EV_BINS], s_scan[WAVES], s_found[2];
+    __shared__ uint32_t s_bins[EV_BINS], s_scan[WAVES], s_found[3];
     const uint32_t r = blockIdx.x, t = threadIdx.x, lane = __lane_id(), wave = t >> 6;
     const uint4 picked = a.picked[2 * r];
     const uint32_t m = picked.x, segments = picked.w;
@@ -682,7 +686,7 @@ __global__ __launch_bounds__(EV_NT) void sg_decide(EvictArgs a)
 #pragma unroll
         for (int shift = 10; shift >= 0; shift -= 10) {
             const uint32_t bits = shift == 10 ? 11 : 10, mask = (1u << bits) - 1u;
-            uint32_t digit, above;
+            uint32_t digit, above, here;
             for (uint32_t i = t; i < EV_BINS; i += EV_NT) s_bins[i] = 0;
             __syncthreads();
             for (uint32_t seg = wave; seg < segments; seg += WAVES)
@@ -690,57 +694,61 @@ __global__ __launch_bounds__(EV_NT) void sg_decide(EvictArgs a)
                     if (in && key >> (shift + bits) == last >> (shift + bits)) atomicAdd(&s_bins[(key >> shift) & mask], 1u);
                 });
             __syncthreads();
-            find_digit<EV_NT>([&](uint32_t bin) { return s_bins[bin]; }, n, s_scan, s_found, digit, above);
+            find_digit<EV_NT>([&](uint32_t bin) { return s_bins[bin]; }, n, s_scan, s_found, digit, above, here);
             n -= above;
             last |= digit << shift;
+            ties = n < here ? n : EV_ALL;
         }
-        ties = n;
     }
-    // ties of each segment, then those before it
-    uint32_t base = 0, holes0 = 0, movers0 = 0;
-    for (uint32_t s0 = 0; s0 < segments; s0 += WAVES) {
-        const uint32_t seg = s0 + wave;
-        uint32_t mine = 0;
-        if (seg < segments)
-            each(seg, [&](bool in, uint32_t key, uint32_t) {
-                mine += static_cast<uint32_t>(__popcll(__ballot(in && key == last && ties)));
-            });
+    const bool ranked = ties != 0 && ties != EV_ALL;
+    // A wave takes neighbouring segments, at most as many as it has lanes; lane k keeps what is
+    // counted of the k-th of them.
+    uint32_t ties0 = 0, holes0 = 0, movers0 = 0;
+    auto before_wave = [&](uint32_t mine, uint32_t* s_wave, uint32_t& all) {  // of the waves before; adds all to `all`
+        if (lane == 63) s_wave[wave] = mine;
         __syncthreads();
-        if (lane == 0) s_scan[wave] = mine;
-        __syncthreads();
-        uint32_t tie = base;
+        uint32_t before = all;
         for (uint32_t w = 0; w < WAVES; ++w) {
-            tie += w < wave ? s_scan[w] : 0u;
-            base += s_scan[w];
+            before += w < wave ? s_wave[w] : 0u;
+            all += s_wave[w];
         }
-        uint32_t holes = 0, movers = 0, run = tie;
-        if (seg < segments) {
-            const uint4 c = a.counts_of[seg0 + seg];
-            holes = c.y;
-            movers = c.z;
-            each(seg, [&](bool in, uint32_t key, uint32_t i) {
+        return before;
+    };
+    for (uint32_t s0 = 0; s0 < segments; s0 += WAVES * 64) {
+        const uint32_t per = (min(segments - s0, WAVES * 64) + WAVES - 1) / WAVES, first = s0 + wave * per;
+        const uint32_t n_mine = first < segments ? min(per, segments - first) : 0u;
+        __syncthreads();
+        uint32_t tie = 0;
+        if (ranked) {
+            for (uint32_t k = 0; k < n_mine; ++k) {
+                uint32_t same = 0;
+                each(first + k, [&](bool in, uint32_t key, uint32_t) {
+                    same += static_cast<uint32_t>(__popcll(__ballot(in && key == last)));
+                });
+                tie = lane == k ? same : tie;
+            }
+            const uint32_t upto = wave_incl_scan(tie);
+            tie = before_wave(upto, s_scan, ties0) + upto - tie;
+        }
+        uint32_t holes = 0, movers = 0;
+        for (uint32_t k = 0; k < n_mine; ++k) {
+            const uint4 c = a.counts_of[seg0 + first + k];
+            uint32_t h = c.y, g = c.z, run = static_cast<uint32_t>(__shfl(static_cast<int>(tie), static_cast<int>(k), 64));
+            each(first + k, [&](bool in, uint32_t key, uint32_t i) {
                 const unsigned long long same = __ballot(in && key == last && ties);
                 const uint32_t rank = run + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
-                const bool stay = key > last || (key == last && ties && rank < ties);
+                const bool stay = key > last || (key == last && rank < ties);
                 run += static_cast<uint32_t>(__popcll(same));
-                holes += static_cast<uint32_t>(__popcll(__ballot(in && !stay && i < m)));
-                movers += static_cast<uint32_t>(__popcll(__ballot(in && stay && i >= m)));
+                h += static_cast<uint32_t>(__popcll(__ballot(in && !stay && i < m)));
+                g += static_cast<uint32_t>(__popcll(__ballot(in && stay && i >= m)));
             });
+            holes = lane == k ? h : holes;
+            movers = lane == k ? g : movers;
         }
-        __syncthreads();
-        if (lane == 0) {
-            s_bins[wave] = holes;
-            s_bins[WAVES + wave] = movers;
-        }
-        __syncthreads();
-        uint32_t hole = holes0, move = movers0;
-        for (uint32_t w = 0; w < WAVES; ++w) {
-            hole += w < wave ? s_bins[w] : 0u;
-            move += w < wave ? s_bins[WAVES + w] : 0u;
-            holes0 += s_bins[w];
-            movers0 += s_bins[WAVES + w];
-        }
-        if (lane == 0 && seg < segments) a.from[seg0 + seg] = make_uint4(tie, hole, move, 0);
+        const uint32_t upto_holes = wave_incl_scan(holes), upto_movers = wave_incl_scan(movers);
+        const uint32_t hole = before_wave(upto_holes, s_bins, holes0) + upto_holes - holes;
+        const uint32_t move = before_wave(upto_movers, s_bins + WAVES, movers0) + upto_movers - movers;
+        if (lane < n_mine) a.from[seg0 + first + lane] = make_uint4(tie, hole, move, 0);
     }
     if (t == 0) {
         a.picked[2 * r + 1] = make_uint4(last, ties, holes0, 0);
@@ -765,7 +773,8 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
     const uint4 picked = a.picked[2 * r + 1], from = a.from[blockIdx.x];
     const uint32_t last = picked.x, ties = picked.y;
     uint32_t tie0 = from.x;
-    if (ties) {
+    const bool ranked = ties != 0 && ties != EV_ALL;
+    if (ranked) {
         uint32_t n = 0;
 #pragma unroll
         for (uint32_t j = 0; j < SG_ROWS; ++j)
@@ -777,7 +786,7 @@ __global__ __launch_bounds__(SG_NT) void sg_place(EvictArgs a)
     for (uint32_t j = 0; j < SG_ROWS; ++j) {
         const uint32_t i = seg * SG_SIZE + (wave * SG_ROWS + j) * 256 + lane * 4, in = below4(i, len), mine = below4(i, m);
         uint32_t tie = tie0;
-        if (ties) {
+        if (ranked) {
             const uint32_t n = ties4(key[j], in, last), upto = wave_incl_scan(n);
             tie += upto - n;
             tie0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));

@@ -221,6 +221,40 @@ def test_evict_very_long(gpu):
     Problem([70001, 131072], [30000, 120000], seed=9, page=64, recent=500, pinned=0.01).check(gpu)
 
 
+@pytest.mark.parametrize("kinds,keep", [(100, 1500000), (100, 40), (2, 2150000), (1 << 30, 3000000)])
+def test_evict_millions(gpu, kinds, keep):
+    """A row of more segments than a workgroup's waves have lanes, with ties across them."""
+    import torch
+    _say("evict millions", kinds, keep)
+    rng = np.random.default_rng(kinds % 97)
+    n, page, sinks, recent = 4300003, 64, 3, 1000
+    cols = -(-n // page)
+    table = rng.permutation(cols).astype(np.int32)
+    w = rng.integers(0, kinds, cols * page).astype(np.float32)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    one = lambda x: torch.tensor([x], **i32)  # noqa: E731
+    w_out, length, n_moves, counts = torch.zeros(1, cols * page, device="cuda"), one(-9), one(-9), torch.zeros(2, **i32)
+    moves, freed = torch.full((1, cols * page // 2, 2), -9, **i32), torch.full((cols,), -9, **i32)
+    gpu.paged_evict(cuda(w)[None], one(n), one(keep), cuda(table)[None], page, w_out, length, moves, n_moves, freed, counts,
+                    sinks=sinks, recent=recent)
+    place = np.arange(n)
+    safe = (place < sinks) | (place >= n - recent)
+    keep = max(keep, int(safe.sum()))
+    stay = np.zeros(n, bool)
+    stay[np.lexsort((place, -w[:n], ~safe))[:keep]] = True
+    holes, movers = np.nonzero(~stay[:keep])[0], keep + np.nonzero(stay[keep:])[0]
+    slot = lambda i: table[i // page] * page + i % page  # noqa: E731
+    lies = np.arange(keep)
+    lies[holes] = movers
+    assert int(length[0]) == keep and int(n_moves[0]) == len(holes)
+    assert np.array_equal(moves[0, :len(holes)].cpu().numpy(), np.stack([slot(movers), slot(holes)], 1))
+    assert np.array_equal(w_out[0, :keep].cpu().numpy(), w[lies])
+    first = -(-keep // page)
+    assert counts.tolist() == [cols - first, len(holes)]
+    assert np.array_equal(freed[:cols - first].cpu().numpy(), table[first:])
+
+
 def test_a_page_outside_the_cache(gpu):
     """Its entries can not be pinned; a move from or to it is listed as -1 and left out."""
     _say("evict with pages outside the cache")
