@@ -356,10 +356,15 @@ __device__ __forceinline__ uint32_t list_freed(const EvictArgs& a, uint32_t r, u
     return n;
 }
 
-constexpr uint64_t EV_WHOLE = 16384;  // entries of a request that one workgroup takes
+// Entries of a request that one workgroup takes: what its registers hold, which is read once
+// and not written down in between (64 requests of 16384, moves included: 187 us, by the launches
+// for longer rows 198).
+constexpr uint64_t EV_WHOLE = 16384;
 
 // A workgroup a request of at most E * NT entries, whose places in the order stay in
-// registers: four neighbours a lane, 256 a wave at a time.
+// registers: four neighbours a lane, 256 a wave at a time.  The last that stays is found by
+// its digits, of 11, 11 and 10 bits, counted in LDS; what bounds it is the chain of those
+// counts and scans, not the bytes (1003 entries: 7.5 us).
 template <int NT, uint32_t E>
 __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
 {
@@ -518,7 +523,10 @@ __global__ __launch_bounds__(NT) void ev_pick(EvictArgs a)
 // The same in launches that leave one another their counts: keys and first digits
 // (sg_keys), the digit in which the last that stays lies (sg_digit), those that have it
 // (sg_split), which of them stay and where each segment's holes and movers begin
-// (sg_decide), and what lies where (sg_place); ev_finish then moves the weights.
+// (sg_decide), and what lies where (sg_place); ev_finish then moves the weights.  Four
+// requests of 131072 entries: 7.9, 5.2, 4.3, 8.3, 6.4 and 5.4 us, most of each the launch
+// and the chain of loads behind it (a workgroup a request, which read its row for every digit:
+// 480 in all).
 constexpr int SG_NT = 256;
 constexpr uint32_t SG_WAVES = SG_NT / 64;
 constexpr uint32_t SG_ROWS = 4;                             // of 256 entries, a wave's
@@ -870,7 +878,8 @@ struct MoveArgs {
 constexpr int MV_NT = 256;
 
 // Bound by memory: a thread asks for MV_AHEAD pieces of the keys and of the values at
-// a time, past the caches.
+// a time, past the caches.  64 requests, 8 heads of 128 in bf16, 90000 tokens: 155 us,
+// 4.7 TB/s read and written, where a copy of 1 GiB reaches 5.1.
 constexpr uint32_t MV_AHEAD = 2;
 
 template <class U>

@@ -63,10 +63,12 @@ __device__ __forceinline__ float2 cos_sin(int32_t position, double freq, float m
     return make_float2((n == 1 || n == 2 ? -cn : cn) * m, (n >= 2 ? -sn : sn) * m);
 }
 
-// Bound by memory.  A thread looks after one pair of pieces that turn together (or of any
-// two of a row), of all tokens of its workgroup (or of every side-th, where a token has few
-// pieces): it works out where they lie once, and asks for those of RO_AHEAD tokens at a
-// time, the first ones before the workgroup's cosines are there.
+// Bound by memory: every row once in, once out.  A thread looks after one pair of pieces that
+// turn together (or of any two of a row), of all tokens of its workgroup (or of every side-th,
+// where a token has few pieces): it works out where they lie once, and asks for those of
+// RO_AHEAD tokens at a time, the first ones before the workgroup's cosines are there.
+// 30011 tokens of 32 + 2 x 8 heads of 128 in f16: 127 us, 5.8 TB/s (192 where a thread took
+// the pieces that came next, wherever they lay); 64 tokens in bf16: 3.5 to 4 us.
 template <class E, uint32_t N, bool NEXT>
 __global__ __launch_bounds__(RO_NT) void ro_turn(RotaryArgs a)
 {
@@ -247,7 +249,8 @@ extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_
     a.per_token = static_cast<uint32_t>(per_token);
     // A workgroup's threads share a token's pieces, in several workgroups where there are more,
     // or take several tokens side by side.  Its cosines serve all of its tokens: as many as
-    // still leave workgroups for the whole card.
+    // still leave workgroups for the whole card, and no more than two rounds of loads (30011
+    // tokens: 127 us, with four 143, with sixteen 155).
     a.side = std::max(1u, static_cast<uint32_t>(RO_NT) / a.per_token);
     a.rounds = a.side > 1 ? 1u : (a.per_token + RO_NT - 1) / RO_NT;
     const uint32_t threads = a.side > 1 ? RO_NT : ((a.per_token + a.rounds - 1) / a.rounds + 63) / 64 * 64;

@@ -117,15 +117,24 @@ struct Lines {
     static constexpr uint32_t TURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
 };
 
-// Up to this many rows that share a key head in a request, wt_rows.
-constexpr uint32_t WT_FEW = 32;
+// Up to this many rows that share a key head in a request, wt_rows, whose products read their
+// keys from LDS again for every 16 rows; wt_tiles keeps them in registers, but takes its time
+// for few rows too.  us of either, 32 requests of 4096 positions and one of 16384, 8 key heads:
+//   64 dimensions, 64 rows: 47 and 60, 13 and 12     128 rows: 71 and 66, 18 and 14
+//   128, 48 rows: 75 and 86, 14 and 15               64 rows: 88 and 86, 17 and 15
+//   256, 24 rows: 145 and 145, 24 and 21             16 rows: 114 and 145, 19 and 21
+constexpr uint32_t few_rows(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 48 : 24; }
 
 // ---- few rows: bound by reading the keys -------------------------------------------------
 // A workgroup per span of a request's positions.  Its waves share the key heads, and
 // where there are fewer heads than waves the span; a wave takes the keys of its
 // positions, one head after another, through LDS of its own, to which they go whole
 // lines at a time and without passing through registers, and which hands them out as the
-// columns of 16x16x32 products whose rows are the queries.
+// columns of 16x16x32 products whose rows are the queries.  A product's 16 rows are not all
+// used where fewer share a key head, which costs nothing: reading is what takes the time.
+// 64 requests of up to 16384 positions, 8 key heads of 128 in bf16, groups of 4: 166 us,
+// 6.5 TB/s (keys through registers and the caches 211, as they came 243; 16 KB of LDS a wave
+// in place of 8, 174); one of 1003 positions: 6 us.
 constexpr int WR_NT = 256;
 constexpr uint32_t WR_WAVES = WR_NT / 64;
 constexpr uint32_t WR_BYTES = 8192;  // of a wave's LDS
@@ -277,6 +286,9 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 // products; the queries pass by through LDS, 64 rows at a time, where the next ones
 // arrive meanwhile without passing through registers.  A lane sums what its two
 // columns get; the parts' sums are joined by another kernel, heads and parts in order.
+// Bound by the matrix units and the exponential of each product beside them: a prompt of
+// 16384 tokens, 8 key heads of 128, groups of 4, takes 1.13 ms, 970 TFLOP/s (1.18 with two
+// waves a SIMD, 1.27 with every row tested for what it sees).
 constexpr int WT_NT = 256;
 __device__ __attribute__((aligned(16))) uint16_t wt_zeros[WT_DIM_MAX];
 constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
@@ -478,7 +490,7 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 }
 
 // The parts' sums joined: 64 positions a workgroup, whose waves share the heads and
-// parts.
+// parts.  6 us for 8 requests of 8192 positions, of which the launch is about half.
 constexpr int WJ_NT = 1024;
 
 __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t cols)
@@ -619,7 +631,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     // Rows of a request that share a key head, as far as the caller says.
     const uint32_t group = a.heads / a.kv_heads;
     const uint64_t typical = p.max_new ? p.max_new : (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests;
-    const bool many = typical * group > WT_FEW;
+    const bool many = typical * group > few_rows(a.dim);
     const uint32_t cols = tile_cols(a.dim);
     a.room = static_cast<uint32_t>(room);
     uint64_t grid;
@@ -627,8 +639,10 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     size_t o_sums = 0;
     if (many) {
         a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
-        // Parts of the rows: as many workgroups as fill the card a few times, and no longer
-        // sums than 2048 rows.
+        // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than
+        // 2048 rows, and no parts of fewer than 256 where it can be helped, which end in more sums
+        // to be joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44;
+        // a prompt of 500 18, not 15).
         const uint64_t rows = (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests * group;
         const uint64_t even = rows * p.n_requests * a.tiles * a.kv_heads / (8ull * num_cus());
         a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;

@@ -209,6 +209,14 @@ def test_hints_do_not_change_the_answer(gpu, what, hints):
     Problem("bfloat16", *SHAPES[what], seed=7).check(gpu, **hints)
 
 
+@pytest.mark.parametrize("max_new", [1, 5000])
+@pytest.mark.parametrize("what", SHAPES)
+def test_either_way_of_splitting(gpu, what, max_new):
+    """Every shape by the kernel for few rows and by the one for many."""
+    _say("weights either way", what, max_new)
+    Problem("float16", *SHAPES[what], seed=21, density=0.7, extra=1).check(gpu, max_new=max_new)
+
+
 @pytest.mark.parametrize("new,kv", [([1], [20011]), ([1, 1], [5000, 12345]), ([17], [9000]), ([33, 2], [6000, 40])])
 def test_weights_long_contexts(gpu, new, kv):
     _say("weights long", new, kv)
