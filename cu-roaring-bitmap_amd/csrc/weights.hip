@@ -500,6 +500,8 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, group = a.heads / a.kv_heads;
     const uint32_t r = blockIdx.x / per_request;
     const Counted t = counted_of(a, r);
+    const uint32_t rows = t.tokens * group, size = part_size(a, rows);
+    const uint32_t held = min(a.parts, (rows + size - 1) / size);  // parts behind have no rows, and left no sums
     for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
         const uint32_t p = p0 + lane, n = a.parts * a.kv_heads;
         float sum = 0.0f;
@@ -510,7 +512,7 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
         }
         if (p < t.keys)
 #pragma unroll 4
-            for (uint32_t i = skip * a.kv_heads + wave; i < n; i += WAVES)
+            for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES)
                 sum += a.sums[(static_cast<uint64_t>(r) * n + i) * a.room + p];
         s_sum[wave][lane] = sum;
         __syncthreads();

@@ -229,6 +229,21 @@ def test_a_prompt_of_many_rows(gpu):
     Problem("bfloat16", [700], [900], 8, 2, 64, 16, seed=18).check(gpu)
 
 
+@pytest.mark.parametrize("what", [([700, 5, 90], [900, 300, 400], 8, 2, 64, 16), ([3, 400, 0, 100], [800, 400, 20, 100], 8, 2, 128, 16),
+                                  ([600, 80], [600, 2000], 4, 1, 256, 16)])
+def test_uneven_requests_after_others(gpu, what):
+    """Requests with fewer parts of rows than the longest, in a workspace that another call has left its sums in."""
+    _say("weights of uneven requests", what[0])
+    for density in (None, 0.5):
+        p = Problem("bfloat16", *what, seed=22, density=density)
+        lse = p.lse
+        for more in (40.0, float("nan")):
+            p.lse = lse - more
+            p.run(gpu)
+            p.lse = lse
+            p.check(gpu)
+
+
 def test_rows_that_count_for_nothing(gpu):
     """Rows whose log-sum is -inf, as those that saw nothing leave it."""
     _say("weights of rows that saw nothing")

@@ -35,7 +35,8 @@ ROTARY = dict(q=P, q_token_stride=256, q_head_stride=64, q_out=P, out_token_stri
     (dict(rotated=63), {}, INVALID), (dict(rotated=66), {}, INVALID), ({}, dict(page_size=12), INVALID),
     ({}, dict(page_size=0), INVALID), ({}, dict(dtype=3), INVALID), ({}, dict(k=None), INVALID), ({}, dict(v=None), INVALID),
     ({}, dict(head_dim=0), INVALID), (dict(rotated=8192), dict(head_dim=8192), UNSUPPORTED),
-    (dict(n_heads=1 << 24), {}, UNSUPPORTED), (dict(n_tokens=1 << 31), {}, UNSUPPORTED), (dict(n_tokens=0, k=None), {}, OK)])
+    (dict(n_heads=1 << 24), {}, UNSUPPORTED), (dict(n_tokens=1 << 31), {}, UNSUPPORTED), (dict(n_tokens=0, k=None), {}, OK),
+    (dict(out_head_stride=0), {}, INVALID), (dict(out_head_stride=63), {}, INVALID), (dict(out_token_stride=0), {}, INVALID)])
 def test_rotary(args, cache, code):
     assert cr.load().cr_paged_rotary(C.byref(_filled(cr.PagedRotaryArgs, ROTARY, args)), C.byref(_cache(**cache)), None) == code
 
