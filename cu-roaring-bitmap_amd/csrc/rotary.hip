@@ -197,13 +197,13 @@ extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_
                   cache->page_size);
         return CR_ERR_INVALID;
     }
-    if ((p.n_heads > 1 && p.out_head_stride < dim) || (p.n_heads && p.n_tokens > 1 && p.out_token_stride < dim)) {
-        set_error("cr_paged_rotary: invalid argument (rows of the turned queries lie over one another)");
-        return CR_ERR_INVALID;
-    }
     if (p.rotated / 2 > RO_PAIRS) {
         set_error("cr_paged_rotary: up to %u dimensions are turned (%u)", 2 * RO_PAIRS, p.rotated);
         return CR_ERR_UNSUPPORTED;
+    }
+    if ((p.n_heads > 1 && p.out_head_stride < dim) || (p.n_heads && p.n_tokens > 1 && p.out_token_stride < dim)) {
+        set_error("cr_paged_rotary: invalid argument (rows of the turned queries lie over one another)");
+        return CR_ERR_INVALID;
     }
     const uint32_t es = cache->dtype == CR_F32 ? 4 : 2;
     RotaryArgs a{};
