@@ -81,7 +81,15 @@ struct WeightArgs {
     // that the launch has for a request; and their sums [n_requests][parts][key heads][room].
     uint32_t parts, part_rows, tiles, room;
     float* sums;
+    // Requests of both kinds: the parts of those with many rows, (request, part of it) [max_listed],
+    // each request's first of them (or NONE), how many there are, and the requests that have some.
+    uint32_t few, max_listed;
+    uint2* listed;
+    uint32_t* first_of;
+    uint32_t* counts;  // parts, requests
+    uint32_t* many;    // [max_listed]
 };
+constexpr uint32_t NONE = 0xFFFFFFFFu;
 
 struct Counted {  // a request's rows and positions
     uint32_t token0, tokens, keys;
@@ -157,6 +165,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
     const uint32_t lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15u, g = lane >> 4;
     const uint32_t r = blockIdx.x / a.spans, tile_waves = WR_WAVES / a.head_waves;
     const uint32_t head_wave = wave % a.head_waves, tile_wave = wave / a.head_waves;
+    if (a.listed && a.first_of[r] != NONE) return;  // wt_tiles takes the request
     const Counted t = counted_of(a, r);
     const uint32_t group = a.heads / a.kv_heads, rows = t.tokens * group, per_wave = a.halves * COLS, step = tile_waves * per_wave;
     uint16_t* sk = s_key[wave];
@@ -344,7 +353,9 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     __shared__ uint32_t s_col[LISTED ? COLS : 1], s_seen[WT_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
     const uint32_t kh = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads / a.tiles;
-    const uint32_t r = part / a.parts, group = a.heads / a.kv_heads;
+    if (a.listed && part >= a.counts[0]) return;
+    const uint2 of = a.listed ? a.listed[part] : make_uint2(part / a.parts, part % a.parts);
+    const uint32_t r = of.x, group = a.heads / a.kv_heads;
     const Counted t = counted_of(a, r);
     const uint32_t rows = t.tokens * group;
     const uint32_t lrow = threadIdx.x / S::CHUNKS, lpos = threadIdx.x % S::CHUNKS;
@@ -362,7 +373,7 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     // (more than once where the caller's most positions are fewer than there are)
     for (uint32_t first = blockIdx.x / a.kv_heads % a.tiles * COLS; first < t.keys; first += a.tiles * COLS) {
         uint32_t row0, row1;
-        rows_of_part(a, t, first, group, part % a.parts, row0, row1);
+        rows_of_part(a, t, first, group, of.y, row0, row1);
         if (row0 >= row1) continue;
         // Whether one of the rows sees position p, and where its keys lie.
         auto look_up = [&](uint32_t p, uint32_t page, uint64_t& at) __attribute__((always_inline)) {
@@ -561,33 +572,76 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
     constexpr uint32_t WAVES = WJ_NT / 64;
     __shared__ float s_sum[WAVES][64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, group = a.heads / a.kv_heads;
-    const uint32_t r = blockIdx.x / per_request;
-    const Counted t = counted_of(a, r);
-    const uint32_t rows = t.tokens * group, size = part_size(a, rows);
-    const uint32_t held = min(a.parts, (rows + size - 1) / size);  // parts behind have no rows, and left no sums
-    for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
-        const uint32_t p = p0 + lane, n = a.parts * a.kv_heads;
-        float sum = 0.0f;
-        uint32_t skip = 0;  // parts that see nothing of the position's tile: the first ones
-        for (uint32_t first, end; skip < a.parts; ++skip) {
-            rows_of_part(a, t, p0 / cols * cols, group, skip, first, end);
-            if (first < end) break;
-        }
-        if (p < t.keys)
+    const uint32_t n_requests = a.listed ? a.counts[1] : a.n_requests;
+    for (uint32_t k = blockIdx.x / per_request; k < n_requests; k += gridDim.x / per_request) {
+        const uint32_t r = a.listed ? a.many[k] : k;
+        const uint64_t part0 = a.listed ? a.first_of[r] : static_cast<uint64_t>(r) * a.parts;
+        const Counted t = counted_of(a, r);
+        const uint32_t rows = t.tokens * group, size = part_size(a, rows);
+        const uint32_t held = min(a.parts, (rows + size - 1) / size);  // parts behind have no rows, and left no sums
+        for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
+            const uint32_t p = p0 + lane;
+            float sum = 0.0f;
+            uint32_t skip = 0;  // parts that see nothing of the position's tile: the first ones
+            for (uint32_t first, end; skip < held; ++skip) {
+                rows_of_part(a, t, p0 / cols * cols, group, skip, first, end);
+                if (first < end) break;
+            }
+            if (p < t.keys)
 #pragma unroll 4
-            for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES)
-                sum += a.sums[(static_cast<uint64_t>(r) * n + i) * a.room + p];
-        s_sum[wave][lane] = sum;
-        __syncthreads();
-        if (wave == 0 && p < t.keys) {
-            float all = 0.0f;
+                for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES)
+                    sum += a.sums[(part0 * a.kv_heads + i) * a.room + p];
+            s_sum[wave][lane] = sum;
+            __syncthreads();
+            if (wave == 0 && p < t.keys) {
+                float all = 0.0f;
 #pragma unroll
-            for (uint32_t w = 0; w < WAVES; ++w) all += s_sum[w][lane];
-            const float past =
-                a.past && (a.continued || static_cast<int64_t>(p) < t.older) ? a.past[r * a.past_stride + p] * a.decay : 0.0f;
-            a.out[r * a.out_stride + p] = past + all;
+                for (uint32_t w = 0; w < WAVES; ++w) all += s_sum[w][lane];
+                const float past =
+                    a.past && (a.continued || static_cast<int64_t>(p) < t.older) ? a.past[r * a.past_stride + p] * a.decay : 0.0f;
+                a.out[r * a.out_stride + p] = past + all;
+            }
+            __syncthreads();
         }
-        __syncthreads();
+    }
+}
+
+// Lists the parts of the requests with many rows, a workgroup's work.  What the list has no room for,
+// where requests count the same rows, stays with wt_rows.  255 single tokens and 2048 of one
+// prompt, 4096 positions each, take 408 us in all, by wt_rows alone 2190, by wt_tiles alone 674.
+constexpr int WS_NT = 1024;
+
+__global__ __launch_bounds__(WS_NT) void wt_split(WeightArgs a)
+{
+    __shared__ uint32_t s_scan[WS_NT / 64], s_end;
+    const uint32_t group = a.heads / a.kv_heads;
+    uint32_t parts = 0, requests = 0;
+    if (threadIdx.x == 0) s_end = 0;
+    __syncthreads();
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += WS_NT) {
+        const uint32_t r = r0 + threadIdx.x;
+        uint32_t n = 0, total, here;
+        if (r < a.n_requests) {
+            const uint32_t rows = counted_of(a, r).tokens * group;
+            n = rows > a.few ? (rows + a.part_rows - 1) / a.part_rows : 0u;
+            n = n <= a.max_listed ? n : 0u;
+        }
+        const uint32_t first = parts + block_excl_scan<WS_NT>(n, s_scan, total);
+        const bool fits = n && first + n <= a.max_listed;
+        const uint32_t k = requests + block_excl_scan<WS_NT>(fits ? 1u : 0u, s_scan, here);
+        if (r < a.n_requests) a.first_of[r] = fits ? first : NONE;
+        if (fits) {
+            a.many[k] = r;
+            for (uint32_t i = 0; i < n; ++i) a.listed[first + i] = make_uint2(r, i);
+        }
+        if (fits) atomicMax(&s_end, first + n);  // (behind one that does not fit none does)
+        parts = min(parts + total, a.max_listed + 1);
+        requests += here;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.counts[0] = s_end;
+        a.counts[1] = requests;
     }
 }
 
@@ -702,23 +756,43 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     if (most == 0) return CR_OK;
     // Rows of a request that share a key head, as far as the caller says.
     const uint32_t group = a.heads / a.kv_heads;
-    const uint64_t typical = p.max_new ? p.max_new : (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests;
-    const bool many = typical * group > few_rows(a.dim);
+    const uint64_t total = static_cast<uint64_t>(p.n_tokens) * group, mean = (total + p.n_requests - 1) / p.n_requests;
+    a.few = few_rows(a.dim);
     const uint32_t cols = tile_cols(a.dim);
     a.room = static_cast<uint32_t>(room);
-    uint64_t grid;
+    a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
+    const uint64_t longest = static_cast<uint64_t>(p.max_new) * group;
+    const bool uneven = p.n_requests > 1 && !p.d_new;
+    const bool many = (uneven || !p.max_new ? mean : longest) > a.few;
+    // Where requests have few rows on average, but one of them may have many (a prompt among single
+    // tokens), each kernel takes its own kind, which a launch before lists.  One new token a request on
+    // average is taken for single tokens.
+    bool mixed = uneven && !many && total > 2 * a.few && (p.max_new ? longest > 2 * a.few : p.n_tokens > p.n_requests);
+    // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than 2048
+    // rows, and no parts of fewer than 256 where it can be helped, which end in more sums to be
+    // joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44; a prompt
+    // of 500 18, not 15).
+    const uint64_t even = total * a.tiles * a.kv_heads / (8ull * num_cus());
+    a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
+    uint64_t grid = 0, rows_grid = 0;
     Carver cv;
-    size_t o_sums = 0;
+    size_t o_sums = 0, o_listed = 0, o_first = 0, o_many = 0;
+    if (mixed) {
+        const uint64_t listed = total / a.part_rows + total / (a.few + 1) + 1;
+        grid = listed * a.tiles * a.kv_heads;
+        if (listed >> 20 || grid >> 23) {
+            mixed = false;  // too large a launch: wt_rows answers them all
+        } else {
+            a.max_listed = static_cast<uint32_t>(listed);
+            a.parts = 1u << 30;  // (as many as the rows need)
+            o_sums = cv.add(listed * a.kv_heads * room * 4);
+            o_listed = cv.add(listed * 8);
+            o_many = cv.add(listed * 4 + 16);
+            o_first = cv.add(p.n_requests * 4ull);
+        }
+    }
     if (many) {
-        a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
-        // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than
-        // 2048 rows, and no parts of fewer than 256 where it can be helped, which end in more sums
-        // to be joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44;
-        // a prompt of 500 18, not 15).
-        const uint64_t rows = (static_cast<uint64_t>(p.n_tokens) + p.n_requests - 1) / p.n_requests * group;
-        const uint64_t even = rows * p.n_requests * a.tiles * a.kv_heads / (8ull * num_cus());
-        a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
-        const uint64_t parts = std::max<uint64_t>(1, (rows + a.part_rows - 1) / a.part_rows);
+        const uint64_t parts = std::max<uint64_t>(1, (mean + a.part_rows - 1) / a.part_rows);
         grid = parts * p.n_requests * a.tiles * a.kv_heads;
         if (grid >> 23) {  // a launch holds fewer than 2^32 threads
             set_error("cr_paged_weights: too many rows and positions for one call");
@@ -736,8 +810,8 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         a.halves = row_cols(a.dim) <= 32 && most * p.n_requests > 16ull * num_cus() * fill ? 64 / row_cols(a.dim) : 1;
         const uint32_t span = a.halves * fill;
         a.spans = static_cast<uint32_t>((most + span - 1) / span);
-        grid = static_cast<uint64_t>(a.spans) * a.n_requests;
-        if (grid >> 23) {
+        rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
+        if (rows_grid >> 23) {
             set_error("cr_paged_weights: too many positions for one call");
             return CR_ERR_UNSUPPORTED;
         }
@@ -751,19 +825,37 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     if (p.visible)
         CR_RET(set_bits(p.visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                         &a.visible));
-    if (many) a.sums = sc.at<float>(o_sums);
-    {
-        CR_TIMED(many ? "wt_tiles" : "wt_rows", s);
-        if (cache->dtype == CR_F16)
-            launch_weights<Half>(a, static_cast<uint32_t>(grid), s);
-        else
-            launch_weights<BHalf>(a, static_cast<uint32_t>(grid), s);
+    if (mixed) {
+        a.listed = sc.at<uint2>(o_listed);
+        a.counts = sc.at<uint32_t>(o_many);
+        a.many = a.counts + 4;
+        a.first_of = sc.at<uint32_t>(o_first);
+        CR_TIMED("wt_split", s);
+        wt_split<<<1, WS_NT, 0, s>>>(a);
     }
-    if (many) {
+    auto launch = [&](uint64_t workgroups) {
+        if (cache->dtype == CR_F16)
+            launch_weights<Half>(a, static_cast<uint32_t>(workgroups), s);
+        else
+            launch_weights<BHalf>(a, static_cast<uint32_t>(workgroups), s);
+    };
+    if (!many) {
+        CR_TIMED("wt_rows", s);
+        launch(rows_grid);
+    }
+    if (many || mixed) {
+        a.sums = sc.at<float>(o_sums);
+        {
+            CR_TIMED("wt_tiles", s);
+            launch(grid);
+        }
         CR_TIMED("wt_join", s);
-        // (fewer than 2^32 threads)
-        const uint32_t per_request = static_cast<uint32_t>(std::min<uint64_t>((most + 63) / 64, ((1u << 22) - 1) / p.n_requests));
-        wt_join<<<per_request * p.n_requests, WJ_NT, 0, s>>>(a, per_request, cols);
+        // (fewer than 2^32 threads; of listed requests, which may be few or none, a few rounds of the card)
+        const uint32_t requests = mixed ? std::min(a.max_listed, a.n_requests) : a.n_requests;
+        const uint32_t wanted = static_cast<uint32_t>((most + 63) / 64);
+        const uint32_t per_request = std::min(wanted, ((1u << 22) - 1) / (mixed ? 1u : requests));
+        const uint32_t side = mixed ? std::max(1u, std::min(requests, 8u * num_cus() / per_request)) : requests;
+        wt_join<<<per_request * side, WJ_NT, 0, s>>>(a, per_request, cols);
     }
     CR_LAUNCH_CHECK();
     return CR_OK;

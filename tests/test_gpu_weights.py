@@ -244,6 +244,31 @@ def test_uneven_requests_after_others(gpu, what):
             p.check(gpu)
 
 
+@pytest.mark.parametrize("density", [None, 0.4])
+@pytest.mark.parametrize("hint", ["none", "longest", "short"])
+@pytest.mark.parametrize("what", [([300] + [1] * 20, [600] + [90] * 20, 8, 2, 64, 16), ([1] * 9 + [80, 1, 40, 0], [130] * 13, 8, 2, 128, 16),
+                                  ([1] * 1030 + [120, 1], [20] * 1030 + [150, 40], 2, 1, 64, 16), ([1, 1, 60, 1, 1], [700] * 5, 4, 1, 256, 16),
+                                  ([2] * 6 + [200] * 2, [300] * 8, 3, 1, 80, 16)])
+def test_long_requests_among_short_ones(gpu, what, hint, density):
+    _say("weights of long and short", what[0][:3], len(what[0]), hint, density)
+    p = Problem("bfloat16", *what, seed=24, density=density, extra=1)
+    p.check(gpu, max_new={"none": 0, "longest": max(what[0]), "short": 60}[hint])
+
+
+def test_many_long_requests_of_the_same_rows(gpu):
+    """More rows in all than there are: what a list has no room for is answered all the same."""
+    import torch
+    _say("weights of shared rows, uneven")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n = 60
+    p = Problem("bfloat16", [90] + [0] * (n - 1), [200] * n, 4, 1, 64, 16, seed=25)
+    starts = [0, 90] * (n // 2) + [0]  # every second request counts all rows, the ones between none
+    got = p.run(gpu, starts=torch.tensor(starts, **i32), max_new=90)
+    p.new = [max(0, b - a) for a, b in zip(starts, starts[1:])]
+    p.q, p.lse = torch.cat([p.q[:90]] * (n // 2)), torch.cat([p.lse[:90]] * (n // 2))
+    p.check(gpu, out=got)
+
+
 def test_rows_that_count_for_nothing(gpu):
     """Rows whose log-sum is -inf, as those that saw nothing leave it."""
     _say("weights of rows that saw nothing")
