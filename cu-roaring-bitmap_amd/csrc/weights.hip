@@ -564,18 +564,19 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 }
 
 // The parts' sums joined: 64 positions a workgroup, whose waves share the heads and
-// parts.  6 us for 8 requests of 8192 positions, of which the launch is about half.
+// parts.  LISTED: of the listed requests, `side` at a time.  6 us for 8 requests of 8192 positions, of which the launch is about half.
 constexpr int WJ_NT = 1024;
 
-__global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t cols)
+template <bool LISTED>
+__global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t side, uint32_t cols)
 {
     constexpr uint32_t WAVES = WJ_NT / 64;
     __shared__ float s_sum[WAVES][64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, group = a.heads / a.kv_heads;
-    const uint32_t n_requests = a.listed ? a.counts[1] : a.n_requests;
-    for (uint32_t k = blockIdx.x / per_request; k < n_requests; k += gridDim.x / per_request) {
-        const uint32_t r = a.listed ? a.many[k] : k;
-        const uint64_t part0 = a.listed ? a.first_of[r] : static_cast<uint64_t>(r) * a.parts;
+    const uint32_t n_requests = LISTED ? a.counts[1] : a.n_requests;
+    for (uint32_t k = blockIdx.x / per_request; k < n_requests; k = LISTED ? k + side : n_requests) {
+        const uint32_t r = LISTED ? a.many[k] : k;
+        const uint64_t part0 = LISTED ? a.first_of[r] : static_cast<uint64_t>(r) * a.parts;
         const Counted t = counted_of(a, r);
         const uint32_t rows = t.tokens * group, size = part_size(a, rows);
         const uint32_t held = min(a.parts, (rows + size - 1) / size);  // parts behind have no rows, and left no sums
@@ -855,7 +856,10 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         const uint32_t wanted = static_cast<uint32_t>((most + 63) / 64);
         const uint32_t per_request = std::min(wanted, ((1u << 22) - 1) / (mixed ? 1u : requests));
         const uint32_t side = mixed ? std::max(1u, std::min(requests, 8u * num_cus() / per_request)) : requests;
-        wt_join<<<per_request * side, WJ_NT, 0, s>>>(a, per_request, cols);
+        if (mixed)
+            wt_join<true><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+        else
+            wt_join<false><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
     }
     CR_LAUNCH_CHECK();
     return CR_OK;
