@@ -255,6 +255,38 @@ def test_long_requests_among_short_ones(gpu, what, hint, density):
     p.check(gpu, max_new={"none": 0, "longest": max(what[0]), "short": 60}[hint])
 
 
+def test_a_captured_call_goes_by_the_lengths_it_finds(gpu):
+    """Replays after another request has become the long one."""
+    import torch
+    _say("weights captured, other lengths")
+    news = [[120] + [1] * 12, [1] * 12 + [120], [1, 60, 1, 1, 61] + [1] * 8, [7] * 8 + [15, 14, 16, 16, 15], [0] * 12 + [132]]
+    p = Problem("bfloat16", news[0], [150] * 13, 8, 2, 64, 16, seed=26)
+    q, lse, out = p.q, p.lse, torch.zeros(13, p.cols * 16, device="cuda")
+    call = lambda s: gpu.paged_weights(q, p.kc, p.table, p.starts, p.kv_len, lse, out, max_new=132, max_kv=150, stream=s)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(side)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call(side)
+    for new in news + news[:2]:
+        starts = torch.tensor(np.concatenate([[0], np.cumsum(new)]).astype(np.int32)).cuda()
+        with torch.cuda.stream(side):
+            p.starts.copy_(starts)
+            call(side)
+            want = out.clone()
+            out.zero_()
+            graph.replay()
+        side.synchronize()
+        assert torch.equal(out, want) and bool(want.abs().sum() > 0), new
+        p.new, p.q, p.lse = new, q, lse
+        got = np.full((13, p.cols * 16 + 5), 7.0)
+        got[:, :150] = out.cpu().numpy()[:, :150]
+        p.check(gpu, past=False, out=got)
+
+
 def test_many_long_requests_of_the_same_rows(gpu):
     """More rows in all than there are: what a list has no room for is answered all the same."""
     import torch
