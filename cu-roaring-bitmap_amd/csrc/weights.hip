@@ -337,8 +337,8 @@ __device__ __forceinline__ void rows_of_part(const WeightArgs& a, const Counted&
 
 // LISTED: where a bitmap leaves positions out, the seen ones of a tile are put side by side first, so
 // that nothing is worked out for the others (8 requests of 100 tokens and 8192 positions, 96
-// dimensions: 60% of them seen 38 -> 36 us, 30% 36 -> 30; a prompt of 8192 with 30% 280 -> 193; all
-// seen 36.4 -> 37).  Where a wave has one block anyway, above 192 dimensions, it would gain little and
+// dimensions: with 60% of them seen 2 us less of 38, with 30% 6 of 36; a prompt of 8192 with 30%
+// 193 us, not 280).  Where a wave has one block anyway, above 192 dimensions, it would gain little and
 // the lists cost 7% with 60% seen.
 template <class E, uint32_t DIM, bool LISTED>
 __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 128 ? 3 : 2))) void wt_tiles(WeightArgs a)
@@ -564,8 +564,11 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 }
 
 // The parts' sums joined: 64 positions a workgroup, whose waves share the heads and
-// parts.  LISTED: of the listed requests, `side` at a time.  6 us for 8 requests of 8192 positions, of which the launch is about half.
-constexpr int WJ_NT = 1024;
+// parts.  LISTED: of the listed requests, `side` at a time.  Four waves, of which many
+// fit a CU: 8 requests of 100 tokens and 8192 positions take 34.5 us in all, with sixteen
+// 37.7; a prompt of 2048, whose positions have 64 sums each, 47.6, with eight 45.1, with
+// two 53.3.
+constexpr int WJ_NT = 256;
 
 template <bool LISTED>
 __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t side, uint32_t cols)
