@@ -216,6 +216,15 @@ def test_evict_long_rows_of_every_kind(gpu, weights, page):
     p.check(gpu, in_place=True, pad=5)
 
 
+@pytest.mark.parametrize("weights", ["spread", "alike"])
+@pytest.mark.parametrize("room", [1008, 1024, 1040, 2048, 2064, 4096, 4112, 8192])
+def test_evict_rooms(gpu, room, weights):
+    """As many positions as the kernels of each size hold, and one page more."""
+    _say("evict room", room, weights)
+    Problem([room], [room // 3], seed=room, weights=weights, pinned=0.05).check(gpu)
+    Problem([room - 5, 3, room, 40], [room // 2, 1, room - 1, 100], seed=room + 1, weights=weights).check(gpu, in_place=True)
+
+
 def test_evict_very_long(gpu):
     _say("evict very long")
     Problem([70001, 131072], [30000, 120000], seed=9, page=64, recent=500, pinned=0.01).check(gpu)
