@@ -778,11 +778,18 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     // of 500 18, not 15).
     const uint64_t even = total * a.tiles * a.kv_heads / (8ull * num_cus());
     a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
+    // A table may have room for far more positions than its requests hold, and a list for more parts than
+    // there are.  Where the caller does not say how many positions there are, workgroups come back for
+    // more of them instead of being launched for none (1024 requests of 500 positions in tables of 65536,
+    // a prompt of 2048 among them: 320 us, not 1130; with max_kv 193).
+    const uint64_t places = (p.max_kv ? 256ull : 64ull) * num_cus();
+    auto at_most = [](uint64_t n, uint64_t most) { return std::max<uint64_t>(1, std::min(n, most)); };
     uint64_t grid = 0, rows_grid = 0;
     Carver cv;
     size_t o_sums = 0, o_listed = 0, o_first = 0, o_many = 0;
     if (mixed) {
         const uint64_t listed = total / a.part_rows + total / (a.few + 1) + 1;
+        a.tiles = static_cast<uint32_t>(at_most(a.tiles, places / (listed * a.kv_heads)));
         grid = listed * a.tiles * a.kv_heads;
         if (listed >> 20 || grid >> 23) {
             mixed = false;  // too large a launch: wt_rows answers them all
@@ -797,6 +804,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     }
     if (many) {
         const uint64_t parts = std::max<uint64_t>(1, (mean + a.part_rows - 1) / a.part_rows);
+        if (!p.max_kv) a.tiles = static_cast<uint32_t>(at_most(a.tiles, places / (parts * p.n_requests * a.kv_heads)));
         grid = parts * p.n_requests * a.tiles * a.kv_heads;
         if (grid >> 23) {  // a launch holds fewer than 2^32 threads
             set_error("cr_paged_weights: too many rows and positions for one call");
@@ -814,6 +822,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         a.halves = row_cols(a.dim) <= 32 && most * p.n_requests > 16ull * num_cus() * fill ? 64 / row_cols(a.dim) : 1;
         const uint32_t span = a.halves * fill;
         a.spans = static_cast<uint32_t>((most + span - 1) / span);
+        if (!p.max_kv) a.spans = static_cast<uint32_t>(at_most(a.spans, places / p.n_requests));
         rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
         if (rows_grid >> 23) {
             set_error("cr_paged_weights: too many positions for one call");
@@ -856,7 +865,8 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         CR_TIMED("wt_join", s);
         // (fewer than 2^32 threads; of listed requests, which may be few or none, a few rounds of the card)
         const uint32_t requests = mixed ? std::min(a.max_listed, a.n_requests) : a.n_requests;
-        const uint32_t wanted = static_cast<uint32_t>((most + 63) / 64);
+        uint32_t wanted = static_cast<uint32_t>((most + 63) / 64);
+        if (!p.max_kv) wanted = static_cast<uint32_t>(at_most(wanted, places / requests));
         const uint32_t per_request = std::min(wanted, ((1u << 22) - 1) / (mixed ? 1u : requests));
         const uint32_t side = mixed ? std::max(1u, std::min(requests, 8u * num_cus() / per_request)) : requests;
         if (mixed)
