@@ -822,12 +822,13 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         a.halves = row_cols(a.dim) <= 32 && most * p.n_requests > 16ull * num_cus() * fill ? 64 / row_cols(a.dim) : 1;
         const uint32_t span = a.halves * fill;
         a.spans = static_cast<uint32_t>((most + span - 1) / span);
-        if (!p.max_kv) a.spans = static_cast<uint32_t>(at_most(a.spans, places / p.n_requests));
         rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
         if (rows_grid >> 23) {
             set_error("cr_paged_weights: too many positions for one call");
             return CR_ERR_UNSUPPORTED;
         }
+        if (!p.max_kv) a.spans = static_cast<uint32_t>(at_most(a.spans, places / p.n_requests));
+        rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
     }
     hipStream_t s = as_stream(stream);
     const bool direct = p.visible && is_direct(p.visible);
