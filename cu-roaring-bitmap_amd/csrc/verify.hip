@@ -370,7 +370,8 @@ __device__ __forceinline__ bool is_allowed(const VerifyArgs& a, uint64_t row, ui
 {
     if (!a.masked) return true;
     const uint32_t w = token / 32u;
-    const uint32_t word = a.flat ? a.flat[row * a.bits_stride + w] : a.allowed.end ? a.allowed.word(w) : 0u;
+    if (!a.flat && token >= a.allowed.end) return false;  // (a complement's words say nothing behind its universe)
+    const uint32_t word = a.flat ? a.flat[row * a.bits_stride + w] : a.allowed.word(w);
     return (word >> (token % 32u)) & 1u;
 }
 
