@@ -1014,7 +1014,11 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
         return CR_ERR_UNSUPPORTED;
     }
     const bool direct = p.pinned && is_direct(p.pinned);
-    const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
+    // What the set can hold: slots behind are not pinned, and take no room where its bits are written out.
+    uint64_t pin_end = n_slots;
+    if (p.pinned && p.pinned->universe_size)
+        pin_end = std::min<uint64_t>(n_slots, (static_cast<uint64_t>(p.pinned->universe_size) + 65535) / 65536 * 65536);
+    const uint32_t n_words = static_cast<uint32_t>((pin_end + 31) / 32);
     Carver cv;
     const size_t o_keys = cv.add(segments * SG_SIZE * 4), o_open = cv.add(segments * SG_SIZE * 8);
     const size_t o_bins = cv.add(segments * EV_BINS * 2), o_counts = cv.add(segments * 16), o_from = cv.add(segments * 16);
@@ -1029,7 +1033,7 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     a.from = sc.at<uint4>(o_from);
     a.picked = sc.at<uint4>(o_picked);
     if (p.pinned)
-        CR_RET(set_bits(p.pinned, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
+        CR_RET(set_bits(p.pinned, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(pin_end), stream,
                         &a.pinned));
     CR_TIMED("ev_pick", s);
     const uint32_t n = p.n_requests, parts = static_cast<uint32_t>(segments);

@@ -898,7 +898,7 @@ def paged_evict(d_weights, d_kv_len, d_keep, d_table, page_size: int, d_weights_
     d_kept[r] entries, as the last call left them; the others are the newest in order.  Written: d_weights_out and
     d_positions_out (the inputs themselves, if need be), d_len int32 [R], d_moves int32 [R, at least half of
     cols * page_size, 2], d_n_moves int32 [R], d_freed int32 [any], d_counts int32 [2]: pages freed and moves in all.
-    n_pages: the cache's (default: those that pinned's universe reaches into, or any).  stream: None is the null
+    n_pages: the cache's (default: any).  Slots behind pinned's universe are not pinned.  stream: None is the null
     stream."""
     n, on = d_kv_len.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
@@ -912,7 +912,7 @@ def paged_evict(d_weights, d_kv_len, d_keep, d_table, page_size: int, d_weights_
         raise CrError(CR_ERR_INVALID, f"paged_evict: moves [{n}, at least {room // 2}, 2] are taken")
     cap = d_moves.shape[1]
     if n_pages is None:
-        n_pages = ((1 << 31) - 1) // page_size if pinned is None else -(-pinned.universe_size // page_size)
+        n_pages = ((1 << 31) - 1) // page_size
     if not (0 <= sinks < 1 << 32 and 0 <= recent < 1 << 32):
         raise CrError(CR_ERR_INVALID, f"paged_evict: sinks {sinks}, recent {recent}")
     a = _EVICT.pack(weights, weights_stride, positions, positions_stride,

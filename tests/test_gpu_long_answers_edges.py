@@ -3,6 +3,7 @@ asked about."""
 import numpy as np
 import pytest
 
+import test_gpu_evict
 import test_gpu_verify
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,35 @@ def test_drafts_behind_the_universe(gpu, universe, vocab, rows, draft):
         p.tokens[i] = d
         p.x[i - 1, d] = 30.0
     p.check(gpu)
+
+
+@pytest.mark.parametrize("kind", ["bitmap", "arrays"])
+@pytest.mark.parametrize("positions", [True, False])
+def test_pinned_slots_of_the_first_pages_alone(gpu, kind, positions):
+    """A bitmap of pinned slots that knows only the first pages says nothing of the others: their tokens move."""
+    import torch
+    _say("evict, few pinned pages", kind, positions)
+    page, n_pages, kv, keep = 16, 40, 600, 250
+    rng = np.random.default_rng(32)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    table = rng.permutation(n_pages).astype(np.int32)[None, :38]
+    w = rng.random((1, 38 * page)).astype(np.float32)
+    at = rng.permutation(38 * page).astype(np.int32)[None]
+    pinned = np.zeros(n_pages * page, bool)
+    pinned[:5 * page] = rng.random(5 * page) < (0.8 if kind == "bitmap" else 0.3)
+    g = gpu.upload_from_ids(np.nonzero(pinned)[0].astype(np.uint32), 5 * page,
+                            gpu.PROMOTE_ALL if kind == "bitmap" else gpu.PROMOTE_KEEP_DEFAULT)
+    one = lambda x: torch.tensor([x], **i32)  # noqa: E731
+    out, p_out, length, n_moves = torch.zeros(1, 38 * page, device="cuda"), torch.zeros(1, 38 * page, **i32), one(-9), one(-9)
+    moves, freed, counts = torch.full((1, 19 * page, 2), -9, **i32), torch.full((38,), -9, **i32), torch.zeros(2, **i32)
+    gpu.paged_evict(cuda(w), one(kv), one(keep), cuda(table), page, out, length, moves, n_moves, freed, counts,
+                    d_positions=cuda(at) if positions else None, d_kept=one(kv) if positions else None,
+                    d_seen=one(kv) if positions else None, d_positions_out=p_out, sinks=2, recent=4, pinned=g)
+    torch.cuda.synchronize()
+    gpu.free(g)
+    m, lies, pos, want, cols = test_gpu_evict.evict_oracle(w[0], at[0], kv if positions else 0, kv, kv, keep, table[0], page,
+                                                           n_pages, 2, 4, pinned)
+    assert int(length[0]) == m and int(n_moves[0]) == len(want) > 0
+    assert moves[0, :len(want)].tolist() == [list(x) for x in want]
+    assert np.array_equal(out[0, :m].cpu().numpy(), w[0][lies]) and p_out[0, :m].tolist() == [pos[i] for i in lies]
