@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "internal.hpp"
+#include "elements.hpp"
 #include "set_bits.hpp"
 
 namespace crimpl {
@@ -24,7 +25,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-struct Half {
+struct Half : F16 {
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0,
@@ -36,7 +37,7 @@ struct Half {
                                                       0);
     }
 };
-struct BHalf {
+struct BHalf : BF16 {
     static __device__ __forceinline__ f32x4 mfma16(v8s x, v8s y, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0,
@@ -570,7 +571,29 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
 // two 53.3.
 constexpr int WJ_NT = 256;
 
-template <bool LISTED>
+// What rows [first, end) of key head kh give seen position p, row by row: those whose log-sum is
+// -inf nothing, whatever the position's key holds.
+template <class E>
+__device__ float sum_of_rows(const WeightArgs& a, const Counted& t, uint32_t r, uint32_t p, uint32_t kh, uint32_t first, uint32_t end)
+{
+    const uint32_t group = a.heads / a.kv_heads, page = static_cast<uint32_t>(a.table[r * a.table_stride + (p >> a.page_lg)]);
+    const uint16_t* key = a.k + page * a.k_page + (p & ((1u << a.page_lg) - 1u)) * a.k_slot + kh * a.k_head;
+    float sum = 0.0f;
+    if (page >= a.n_pages) return sum;
+    for (int64_t row = max(static_cast<int64_t>(first), first_row(a, t, p, group)); row < end && sum == sum; ++row) {
+        const uint64_t token = t.token0 + static_cast<uint32_t>(row) / group;
+        const uint32_t head = kh * group + static_cast<uint32_t>(row) % group;
+        const float z = a.lse[token * a.heads + head];
+        if (z == -__builtin_inff()) continue;
+        const uint16_t* q = a.q + token * a.q_token + head * a.q_head;
+        float x = 0.0f;
+        for (uint32_t d = 0; d < a.dim; ++d) x = __builtin_fmaf(E::up(q[d]), E::up(key[d]), x);
+        sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale2, -(z * LOG2E)));
+    }
+    return sum;
+}
+
+template <class E, bool LISTED>
 __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_request, uint32_t side, uint32_t cols)
 {
     constexpr uint32_t WAVES = WJ_NT / 64;
@@ -595,6 +618,20 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
 #pragma unroll 4
                 for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES)
                     sum += a.sums[(part0 * a.kv_heads + i) * a.room + p];
+            // Not a number: the key holds something that wt_tiles has multiplied rows which count for nothing
+            // with too.  (A test a product there would cost registers that three waves a SIMD do not have.)
+            if (sum != sum) {
+                sum = 0.0f;
+                for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES) {
+                    float more = a.sums[(part0 * a.kv_heads + i) * a.room + p];
+                    if (more != more) {
+                        uint32_t first, end;
+                        rows_of_part(a, t, p0 / cols * cols, group, i / a.kv_heads, first, end);
+                        more = sum_of_rows<E>(a, t, r, p, i % a.kv_heads, first, end);
+                    }
+                    sum += more;
+                }
+            }
             s_sum[wave][lane] = sum;
             __syncthreads();
             if (wave == 0 && p < t.keys) {
@@ -870,10 +907,17 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         if (!p.max_kv) wanted = static_cast<uint32_t>(at_most(wanted, places / requests));
         const uint32_t per_request = std::min(wanted, ((1u << 22) - 1) / (mixed ? 1u : requests));
         const uint32_t side = mixed ? std::max(1u, std::min(requests, 8u * num_cus() / per_request)) : requests;
-        if (mixed)
-            wt_join<true><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+        auto join = [&](auto type) {
+            using E = decltype(type);
+            if (mixed)
+                wt_join<E, true><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+            else
+                wt_join<E, false><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+        };
+        if (cache->dtype == CR_F16)
+            join(Half{});
         else
-            wt_join<false><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+            join(BHalf{});
     }
     CR_LAUNCH_CHECK();
     return CR_OK;

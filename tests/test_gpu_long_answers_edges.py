@@ -1,10 +1,11 @@
 """The operators for long and speculative answers where their arguments meet: sets that are narrower than what they are
-asked about."""
+asked about, and rows that count for nothing beside keys that hold anything."""
 import numpy as np
 import pytest
 
 import test_gpu_evict
 import test_gpu_verify
+import test_gpu_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,36 @@ def test_pinned_slots_of_the_first_pages_alone(gpu, kind, positions):
     assert int(length[0]) == m and int(n_moves[0]) == len(want) > 0
     assert moves[0, :len(want)].tolist() == [list(x) for x in want]
     assert np.array_equal(out[0, :m].cpu().numpy(), w[0][lies]) and p_out[0, :m].tolist() == [pos[i] for i in lies]
+
+
+@pytest.mark.parametrize("density", [None, 0.8])
+@pytest.mark.parametrize("max_new", [1, 5000])
+@pytest.mark.parametrize("what", ["a few tokens", "chunk", "prompt group 3", "dims 192", "dims 256"])
+def test_rows_that_count_for_nothing_beside_any_keys(gpu, what, max_new, density):
+    """Positions that only rows with a log-sum of -inf see, whose keys are NaN or infinite, got nothing."""
+    _say("weights, any keys", what, max_new, density)
+    p = test_gpu_weights.Problem("bfloat16", *test_gpu_weights.SHAPES[what], seed=33, density=density)
+    at = 0
+    for r, (n, kv) in enumerate(zip(p.new, p.kv)):
+        gone = min(n, 3)
+        for i in range(gone):
+            p.lse[at + n - 1 - i] = float("-inf")
+            position = kv - 1 - i
+            p.kc[p.table[r, position // p.page].long(), position % p.page] = float("nan") if i % 2 else float("inf")
+        at += n
+    out = p.run(gpu, max_new=max_new)
+    for r, kv in enumerate(p.kv):
+        assert np.isfinite(out[r, :kv]).all(), (r, np.nonzero(~np.isfinite(out[r, :kv]))[0])
+    p.check(gpu, out=out)
+
+
+@pytest.mark.parametrize("density", [None, 0.4])
+@pytest.mark.parametrize("max_new", [1, 5000])
+@pytest.mark.parametrize("what", test_gpu_weights.SHAPES)
+def test_weights_are_finite(gpu, what, max_new, density):
+    """Keys that nobody sees are NaN in all of these: a comparison of differences alone would let theirs pass."""
+    _say("weights finite", what, max_new, density)
+    p = test_gpu_weights.Problem("bfloat16", *test_gpu_weights.SHAPES[what], seed=36, density=density)
+    out = p.run(gpu, max_new=max_new)
+    assert all(np.isfinite(out[r, :max(0, kv)]).all() for r, kv in enumerate(p.kv))
+    p.check(gpu, out=out)
