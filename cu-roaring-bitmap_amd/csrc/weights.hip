@@ -11,6 +11,7 @@
 #include "internal.hpp"
 #include "elements.hpp"
 #include "set_bits.hpp"
+#include "weights_work.hpp"
 
 namespace crimpl {
 
@@ -127,14 +128,6 @@ struct Lines {
     static constexpr uint32_t TURN = CHUNKS < 16 ? CHUNKS - 1 : 15;
 };
 
-// Up to this many rows that share a key head in a request, wt_rows, whose products read their
-// keys from LDS again for every 16 rows; wt_tiles keeps them in registers, but takes its time
-// for few rows too.  us of either, 32 requests of 4096 positions and one of 16384, 8 key heads:
-//   64 dimensions, 64 rows: 47 and 60, 13 and 12     128 rows: 71 and 66, 18 and 14
-//   128, 48 rows: 75 and 86, 14 and 15               64 rows: 88 and 86, 17 and 15
-//   256, 24 rows: 145 and 145, 24 and 21             16 rows: 114 and 145, 19 and 21
-constexpr uint32_t few_rows(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 48 : 24; }
-
 // ---- few rows: bound by reading the keys -------------------------------------------------
 // A workgroup per span of a request's positions.  Its waves share the key heads, and
 // where there are fewer heads than waves the span; a wave takes the keys of its
@@ -145,14 +138,6 @@ constexpr uint32_t few_rows(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ?
 // 64 requests of up to 16384 positions, 8 key heads of 128 in bf16, groups of 4: 166 us,
 // 6.5 TB/s (keys through registers and the caches 211, as they came 243; 16 KB of LDS a wave
 // in place of 8, 174); one of 1003 positions: 6 us.
-constexpr int WR_NT = 256;
-constexpr uint32_t WR_WAVES = WR_NT / 64;
-constexpr uint32_t WR_BYTES = 8192;  // of a wave's LDS
-
-// Positions of a wave.
-constexpr uint32_t row_tiles(uint32_t chunks) { return WR_BYTES / (chunks * 16) / 16 > 4 ? 4 : WR_BYTES / (chunks * 16) / 16; }
-constexpr uint32_t row_cols(uint32_t dim) { return row_tiles(dim <= 64 ? 8 : dim <= 128 ? 16 : 32) * 16; }
-
 template <class E, uint32_t DIM>
 __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 {
@@ -300,7 +285,6 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
 // Bound by the matrix units and the exponential of each product beside them: a prompt of
 // 16384 tokens, 8 key heads of 128, groups of 4, takes 1.13 ms, 970 TFLOP/s (1.18 with two
 // waves a SIMD, 1.27 with every row tested for what it sees).
-constexpr int WT_NT = 256;
 __device__ __attribute__((aligned(16))) uint16_t wt_zeros[WT_DIM_MAX];
 constexpr uint32_t WT_ROWS = 64;   // rows that arrive at a time
 
@@ -308,10 +292,6 @@ template <uint32_t DIM>
 struct Stage : Lines<DIM> {
     static constexpr uint32_t PER = WT_NT / Lines<DIM>::CHUNKS, LOADS = WT_ROWS / PER;  // rows that the workgroup loads at once
 };
-
-// Blocks of 32 positions whose keys a wave holds; positions of a workgroup's tile.
-constexpr uint32_t tile_blocks(uint32_t dim) { return dim <= 192 ? 2 : 1; }
-constexpr uint32_t tile_cols(uint32_t dim) { return tile_blocks(dim) * 32 * (WT_NT / 64); }
 
 // The first row that sees a position, at or behind all that its tokens are.
 __device__ __forceinline__ int64_t first_row(const WeightArgs& a, const Counted& t, uint32_t p, uint32_t group)
@@ -793,80 +773,26 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     a.scale2 = static_cast<float>(static_cast<double>(p.scale) * 1.44269504088896340736);
     a.causal = p.causal != 0;
     a.continued = p.continued != 0;
-    const uint64_t most = p.max_kv ? std::min<uint64_t>(room, p.max_kv) : room;
-    if (most == 0) return CR_OK;
-    // Rows of a request that share a key head, as far as the caller says.
-    const uint32_t group = a.heads / a.kv_heads;
-    const uint64_t total = static_cast<uint64_t>(p.n_tokens) * group, mean = (total + p.n_requests - 1) / p.n_requests;
-    a.few = few_rows(a.dim);
-    const uint32_t cols = tile_cols(a.dim);
     a.room = static_cast<uint32_t>(room);
-    a.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
-    const uint64_t longest = static_cast<uint64_t>(p.max_new) * group;
-    const bool uneven = p.n_requests > 1 && !p.d_new;
-    const bool many = (uneven || !p.max_new ? mean : longest) > a.few;
-    // Where requests have few rows on average, but one of them may have many (a prompt among single
-    // tokens), each kernel takes its own kind, which a launch before lists.  One new token a request on
-    // average is taken for single tokens.
-    bool mixed = uneven && !many && total > 2 * a.few && (p.max_new ? longest > 2 * a.few : p.n_tokens > p.n_requests);
-    // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than 2048
-    // rows, and no parts of fewer than 256 where it can be helped, which end in more sums to be
-    // joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44; a prompt
-    // of 500 18, not 15).
-    const uint64_t even = total * a.tiles * a.kv_heads / (8ull * num_cus());
-    a.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
-    // A table may have room for far more positions than its requests hold, and a list for more parts than
-    // there are.  Where the caller does not say how many positions there are, workgroups come back for
-    // more of them instead of being launched for none (1024 requests of 500 positions in tables of 65536,
-    // a prompt of 2048 among them: 320 us, not 1130; with max_kv 193).
-    const uint64_t places = (p.max_kv ? 256ull : 64ull) * num_cus();
-    auto at_most = [](uint64_t n, uint64_t most) { return std::max<uint64_t>(1, std::min(n, most)); };
-    uint64_t grid = 0, rows_grid = 0;
+    if (room == 0) return CR_OK;
+    WeightsWork w;
+    const WeightsShape shape{p.n_tokens, p.n_heads, cache->n_heads, cache->head_dim, p.n_requests, room, p.max_new, p.max_kv,
+                             p.d_new != nullptr, static_cast<uint32_t>(num_cus())};
+    if (const char* wrong = weights_work(shape, w)) {
+        set_error("cr_paged_weights: %s", wrong);
+        return CR_ERR_UNSUPPORTED;
+    }
+    a.few = w.few;
+    a.head_waves = w.head_waves;
+    a.halves = w.halves;
+    a.spans = w.spans;
+    a.part_rows = w.part_rows;
+    a.parts = w.parts;
+    a.tiles = w.tiles;
+    a.max_listed = w.max_listed;
     Carver cv;
-    size_t o_sums = 0, o_listed = 0, o_first = 0, o_many = 0;
-    if (mixed) {
-        const uint64_t listed = total / a.part_rows + total / (a.few + 1) + 1;
-        a.tiles = static_cast<uint32_t>(at_most(a.tiles, places / (listed * a.kv_heads)));
-        grid = listed * a.tiles * a.kv_heads;
-        if (listed >> 20 || grid >> 23) {
-            mixed = false;  // too large a launch: wt_rows answers them all
-        } else {
-            a.max_listed = static_cast<uint32_t>(listed);
-            a.parts = 1u << 30;  // (as many as the rows need)
-            o_sums = cv.add(listed * a.kv_heads * room * 4);
-            o_listed = cv.add(listed * 8);
-            o_many = cv.add(listed * 4 + 16);
-            o_first = cv.add(p.n_requests * 4ull);
-        }
-    }
-    if (many) {
-        const uint64_t parts = std::max<uint64_t>(1, (mean + a.part_rows - 1) / a.part_rows);
-        if (!p.max_kv) a.tiles = static_cast<uint32_t>(at_most(a.tiles, places / (parts * p.n_requests * a.kv_heads)));
-        grid = parts * p.n_requests * a.tiles * a.kv_heads;
-        if (grid >> 23) {  // a launch holds fewer than 2^32 threads
-            set_error("cr_paged_weights: too many rows and positions for one call");
-            return CR_ERR_UNSUPPORTED;
-        }
-        a.parts = static_cast<uint32_t>(parts);
-        o_sums = cv.add(parts * p.n_requests * a.kv_heads * room * 4);
-    } else {
-        a.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
-        // A wave looks up 64 positions at once and fills its LDS with them two or four times where there
-        // is work for many rounds of the card, which saves look-ups (64 requests of 16384 positions, 8
-        // heads of 128: 174 -> 167 us), and fills it once where the last round counts (32 requests of
-        // 4096: 27 us, not 32).
-        const uint32_t fill = WR_WAVES / a.head_waves * row_cols(a.dim);
-        a.halves = row_cols(a.dim) <= 32 && most * p.n_requests > 16ull * num_cus() * fill ? 64 / row_cols(a.dim) : 1;
-        const uint32_t span = a.halves * fill;
-        a.spans = static_cast<uint32_t>((most + span - 1) / span);
-        rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
-        if (rows_grid >> 23) {
-            set_error("cr_paged_weights: too many positions for one call");
-            return CR_ERR_UNSUPPORTED;
-        }
-        if (!p.max_kv) a.spans = static_cast<uint32_t>(at_most(a.spans, places / p.n_requests));
-        rows_grid = static_cast<uint64_t>(a.spans) * a.n_requests;
-    }
+    const size_t o_sums = cv.add(w.sums * 4), o_listed = cv.add(w.max_listed * 8ull);
+    const size_t o_many = cv.add(w.mixed ? w.max_listed * 4ull + 16 : 0), o_first = cv.add(w.mixed ? p.n_requests * 4ull : 0);
     hipStream_t s = as_stream(stream);
     const bool direct = p.visible && is_direct(p.visible);
     const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
@@ -876,7 +802,7 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     if (p.visible)
         CR_RET(set_bits(p.visible, direct, sc.at<uint32_t>(o_words), n_words, static_cast<uint32_t>(n_slots), stream,
                         &a.visible));
-    if (mixed) {
+    if (w.mixed) {
         a.listed = sc.at<uint2>(o_listed);
         a.counts = sc.at<uint32_t>(o_many);
         a.many = a.counts + 4;
@@ -884,35 +810,30 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         CR_TIMED("wt_split", s);
         wt_split<<<1, WS_NT, 0, s>>>(a);
     }
-    auto launch = [&](uint64_t workgroups) {
+    auto launch = [&](uint32_t workgroups) {
         if (cache->dtype == CR_F16)
-            launch_weights<Half>(a, static_cast<uint32_t>(workgroups), s);
+            launch_weights<Half>(a, workgroups, s);
         else
-            launch_weights<BHalf>(a, static_cast<uint32_t>(workgroups), s);
+            launch_weights<BHalf>(a, workgroups, s);
     };
-    if (!many) {
+    if (!w.many) {
         CR_TIMED("wt_rows", s);
-        launch(rows_grid);
+        launch(w.rows_grid);
     }
-    if (many || mixed) {
+    if (w.many || w.mixed) {
         a.sums = sc.at<float>(o_sums);
         {
             CR_TIMED("wt_tiles", s);
-            launch(grid);
+            launch(w.tiles_grid);
         }
         CR_TIMED("wt_join", s);
-        // (fewer than 2^32 threads; of listed requests, which may be few or none, a few rounds of the card)
-        const uint32_t requests = mixed ? std::min(a.max_listed, a.n_requests) : a.n_requests;
-        uint32_t wanted = static_cast<uint32_t>((most + 63) / 64);
-        if (!p.max_kv) wanted = static_cast<uint32_t>(at_most(wanted, places / requests));
-        const uint32_t per_request = std::min(wanted, ((1u << 22) - 1) / (mixed ? 1u : requests));
-        const uint32_t side = mixed ? std::max(1u, std::min(requests, 8u * num_cus() / per_request)) : requests;
         auto join = [&](auto type) {
             using E = decltype(type);
-            if (mixed)
-                wt_join<E, true><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+            const uint32_t grid = w.join_per_request * w.join_side, cols = tile_cols(a.dim);
+            if (w.mixed)
+                wt_join<E, true><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, w.join_side, cols);
             else
-                wt_join<E, false><<<per_request * side, WJ_NT, 0, s>>>(a, per_request, side, cols);
+                wt_join<E, false><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, w.join_side, cols);
         };
         if (cache->dtype == CR_F16)
             join(Half{});
