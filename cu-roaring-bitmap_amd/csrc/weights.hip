@@ -737,9 +737,9 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         return CR_ERR_UNSUPPORTED;
     }
     if (n_slots >> 31 || room >> 31 || p.n_tokens >> 31 || p.n_heads > 65535 || p.n_requests >> 22 ||
-        (static_cast<uint64_t>(p.n_tokens) * p.n_heads) >> 31) {
-        set_error("cr_paged_weights: supported up to 2^31 - 1 slots, positions and rows, 65535 heads and 2^22 - 1 "
-                  "requests");
+        (static_cast<uint64_t>(p.n_tokens) * p.n_heads) >> 31 || (room * p.n_requests) >> 36) {
+        set_error("cr_paged_weights: supported up to 2^31 - 1 slots, positions and rows, 65535 heads, 2^22 - 1 requests and "
+                  "2^36 - 1 weights");
         return CR_ERR_UNSUPPORTED;
     }
     WeightArgs a{};
@@ -775,13 +775,8 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     a.continued = p.continued != 0;
     a.room = static_cast<uint32_t>(room);
     if (room == 0) return CR_OK;
-    WeightsWork w;
-    const WeightsShape shape{p.n_tokens, p.n_heads, cache->n_heads, cache->head_dim, p.n_requests, room, p.max_new, p.max_kv,
-                             p.d_new != nullptr, static_cast<uint32_t>(num_cus())};
-    if (const char* wrong = weights_work(shape, w)) {
-        set_error("cr_paged_weights: %s", wrong);
-        return CR_ERR_UNSUPPORTED;
-    }
+    const WeightsWork w = weights_work({p.n_tokens, p.n_heads, cache->n_heads, cache->head_dim, p.n_requests, room, p.max_new,
+                                        p.max_kv, p.d_new != nullptr, num_cus()});
     a.few = w.few;
     a.head_waves = w.head_waves;
     a.halves = w.halves;
@@ -810,35 +805,47 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         CR_TIMED("wt_split", s);
         wt_split<<<1, WS_NT, 0, s>>>(a);
     }
-    auto launch = [&](uint32_t workgroups) {
+    auto launch = [&](const WeightArgs& a, uint32_t workgroups) {
         if (cache->dtype == CR_F16)
             launch_weights<Half>(a, workgroups, s);
         else
             launch_weights<BHalf>(a, workgroups, s);
     };
+    auto join = [&](const WeightArgs& a, uint32_t side, auto type) {
+        using E = decltype(type);
+        const uint32_t grid = w.join_per_request * side, cols = tile_cols(a.dim);
+        if (w.mixed)
+            wt_join<E, true><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, side, cols);
+        else
+            wt_join<E, false><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, side, cols);
+    };
     if (!w.many) {
         CR_TIMED("wt_rows", s);
-        launch(w.rows_grid);
+        launch(a, w.rows_grid);
     }
-    if (w.many || w.mixed) {
-        a.sums = sc.at<float>(o_sums);
+    if (w.many || w.mixed) a.sums = sc.at<float>(o_sums);
+    for (uint32_t r = 0; w.mixed ? r == 0 : w.many && r < p.n_requests; r += w.mixed ? 1 : w.batch) {
+        WeightArgs b = a;  // of requests from r on
+        uint32_t side = w.join_side, grid = w.tiles_grid;
+        if (w.many) {
+            b.starts += r;
+            if (b.fresh) b.fresh += r;
+            b.kv_len += r;
+            b.table += r * b.table_stride;
+            if (b.past) b.past += r * b.past_stride;
+            b.out += r * b.out_stride;
+            b.n_requests = side = std::min(w.batch, p.n_requests - r);
+            grid = grid / w.batch * side;
+        }
         {
             CR_TIMED("wt_tiles", s);
-            launch(w.tiles_grid);
+            launch(b, grid);
         }
         CR_TIMED("wt_join", s);
-        auto join = [&](auto type) {
-            using E = decltype(type);
-            const uint32_t grid = w.join_per_request * w.join_side, cols = tile_cols(a.dim);
-            if (w.mixed)
-                wt_join<E, true><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, w.join_side, cols);
-            else
-                wt_join<E, false><<<grid, WJ_NT, 0, s>>>(a, w.join_per_request, w.join_side, cols);
-        };
         if (cache->dtype == CR_F16)
-            join(Half{});
+            join(b, side, Half{});
         else
-            join(BHalf{});
+            join(b, side, BHalf{});
     }
     CR_LAUNCH_CHECK();
     return CR_OK;

@@ -47,15 +47,19 @@ struct WeightsWork {
     // wt_tiles: parts of a request's rows, of part_rows or more each; tiles of positions that the
     // launch has for a request; and the parts that the list has room for.
     uint32_t part_rows, parts, tiles, max_listed, tiles_grid;
-    uint64_t sums;  // floats that it leaves for wt_join
+    uint32_t batch;  // requests of a launch, one after another: all of them, unless a launch cannot hold them
+    uint64_t sums;   // floats that it leaves for wt_join
     // wt_join: workgroups of a request, and requests at a time.
     uint32_t join_per_request, join_side;
 };
 
-// What is wrong with a call, or nullptr.  A launch holds fewer than 2^32 threads.
-inline const char* weights_work(const WeightsShape& a, WeightsWork& w)
+// A launch holds fewer than 2^32 threads.  Workgroups come back for more positions where it does not
+// hold one for all of them, so that the caller's hints never decide whether it is answered.
+constexpr uint64_t WT_LAUNCH = (1u << 23) - 1;
+
+inline WeightsWork weights_work(const WeightsShape& a)
 {
-    w = WeightsWork{};
+    WeightsWork w{};
     const uint64_t most = a.max_kv ? std::min<uint64_t>(a.room, a.max_kv) : a.room;
     // Rows of a request that share a key head, as far as the caller says.
     const uint32_t group = a.heads / a.kv_heads;
@@ -97,12 +101,13 @@ inline const char* weights_work(const WeightsShape& a, WeightsWork& w)
     }
     if (w.many) {
         const uint64_t parts = std::max<uint64_t>(1, (mean + w.part_rows - 1) / w.part_rows);
+        w.parts = static_cast<uint32_t>(std::min(parts, WT_LAUNCH / a.kv_heads));
+        const uint64_t each = static_cast<uint64_t>(w.parts) * a.kv_heads;  // workgroups of a request and a tile
+        w.batch = static_cast<uint32_t>(std::min<uint64_t>(a.n_requests, WT_LAUNCH / each));
         if (!a.max_kv) w.tiles = static_cast<uint32_t>(at_most(w.tiles, places / (parts * a.n_requests * a.kv_heads)));
-        const uint64_t grid = parts * a.n_requests * w.tiles * a.kv_heads;
-        if (grid >> 23) return "too many rows and positions for one call";
-        w.tiles_grid = static_cast<uint32_t>(grid);
-        w.parts = static_cast<uint32_t>(parts);
-        w.sums = parts * a.n_requests * a.kv_heads * a.room;
+        w.tiles = static_cast<uint32_t>(at_most(w.tiles, WT_LAUNCH / (each * w.batch)));
+        w.tiles_grid = static_cast<uint32_t>(each * w.batch * w.tiles);
+        w.sums = each * w.batch * a.room;
     } else {
         w.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
         // A wave looks up 64 positions at once and fills its LDS with them two or four times where there
@@ -113,20 +118,20 @@ inline const char* weights_work(const WeightsShape& a, WeightsWork& w)
         w.halves = row_cols(a.dim) <= 32 && most * a.n_requests > 16ull * a.cus * fill ? 64 / row_cols(a.dim) : 1;
         const uint32_t span = w.halves * fill;
         uint64_t spans = (most + span - 1) / span;
-        if ((spans * a.n_requests) >> 23) return "too many positions for one call";
         if (!a.max_kv) spans = at_most(spans, places / a.n_requests);
+        spans = at_most(spans, WT_LAUNCH / a.n_requests);
         w.spans = static_cast<uint32_t>(spans);
         w.rows_grid = static_cast<uint32_t>(spans * a.n_requests);
     }
     if (w.many || w.mixed) {
         // (fewer than 2^32 threads; of listed requests, which may be few or none, a few rounds of the card)
-        const uint32_t requests = w.mixed ? std::min(w.max_listed, a.n_requests) : a.n_requests;
+        const uint32_t requests = w.mixed ? std::min(w.max_listed, a.n_requests) : w.batch;
         uint64_t wanted = (most + 63) / 64;
         if (!a.max_kv) wanted = at_most(wanted, places / requests);
         w.join_per_request = static_cast<uint32_t>(std::min<uint64_t>(wanted, ((1u << 22) - 1) / (w.mixed ? 1u : requests)));
         w.join_side = w.mixed ? std::max(1u, std::min(requests, 8u * a.cus / w.join_per_request)) : requests;
     }
-    return nullptr;
+    return w;
 }
 
 }  // namespace

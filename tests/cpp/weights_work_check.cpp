@@ -1,5 +1,5 @@
 // How cr_paged_weights splits its work (csrc/weights_work.hpp), run on the CPU for shapes of every size.
-//   - every launch has work and fewer than 2^32 threads;
+//   - every launch has work and fewer than 2^32 threads, whatever the caller says of its lengths;
 //   - the requests with many rows fit the list that is made of them.
 // Prints how often each way was taken, and "weights_work_check: OK".
 #include <cstdio>
@@ -35,15 +35,10 @@ static std::string text(const WeightsShape& a)
 
 constexpr uint64_t LAUNCH = 1ull << 23;  // workgroups of 512 threads or fewer
 
-static bool check(const WeightsShape& a, std::mt19937_64& rng)
+static void check(const WeightsShape& a, std::mt19937_64& rng)
 {
-    WeightsWork w;
-    const char* wrong = weights_work(a, w);
+    const WeightsWork w = weights_work(a);
     const std::string what = text(a);
-    if (wrong) {
-        ++g_ways[std::string("refused: ") + wrong];
-        return false;
-    }
     const uint32_t group = a.heads / a.kv_heads;
     EXPECT(!(w.many && w.mixed), "%s", what.c_str());
     if (!w.many) {
@@ -57,8 +52,9 @@ static bool check(const WeightsShape& a, std::mt19937_64& rng)
         EXPECT(w.join_per_request && w.join_side && static_cast<uint64_t>(w.join_per_request) * w.join_side < LAUNCH * 2, "%s", what.c_str());
     }
     if (w.many) {
-        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.parts) * a.n_requests * w.tiles * a.kv_heads, "%s", what.c_str());
-        EXPECT(w.sums == static_cast<uint64_t>(w.parts) * a.n_requests * a.kv_heads * a.room, "%s", what.c_str());
+        EXPECT(w.batch && w.batch <= a.n_requests, "%s", what.c_str());
+        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.parts) * w.batch * w.tiles * a.kv_heads, "%s", what.c_str());
+        EXPECT(w.sums == static_cast<uint64_t>(w.parts) * w.batch * a.kv_heads * a.room, "%s", what.c_str());
     }
     if (w.mixed) {
         EXPECT(w.tiles_grid == static_cast<uint64_t>(w.max_listed) * w.tiles * a.kv_heads, "%s", what.c_str());
@@ -78,7 +74,6 @@ static bool check(const WeightsShape& a, std::mt19937_64& rng)
         }
     }
     ++g_ways[w.many ? "many rows" : w.mixed ? "mixed" : "few rows"];
-    return true;
 }
 
 int main()
@@ -89,10 +84,16 @@ int main()
         return static_cast<uint64_t>(static_cast<double>(lo) * __builtin_pow(static_cast<double>(hi) / static_cast<double>(lo), x));
     };
     const uint32_t dims[] = {64, 96, 128, 192, 256};
+    // answered with hints as without
+    check({524288, 32, 8, 128, 1, 524288, 0, 0, false, 256}, rng);
+    check({524288, 32, 8, 128, 1, 524288, 524288, 524288, false, 256}, rng);
+    check({512 * 2048, 32, 8, 128, 512, 131072, 2048, 131072, false, 256}, rng);
+    check({4096, 32, 8, 128, 4096, 131072, 1, 0, false, 256}, rng);
+    check({4096, 32, 8, 128, 4096, 131072, 1, 131072, false, 256}, rng);
     for (int i = 0; i < 200000; ++i) {
         WeightsShape a{};
-        a.kv_heads = 1u << rng() % 7;
-        a.heads = a.kv_heads * static_cast<uint32_t>(1 + rng() % 8);
+        a.kv_heads = i % 7 ? 1u << rng() % 7 : static_cast<uint32_t>(spread(1, 65535));
+        a.heads = a.kv_heads * static_cast<uint32_t>(1 + rng() % std::min<uint32_t>(8, 65535 / a.kv_heads));
         a.dim = dims[rng() % 5];
         a.n_requests = static_cast<uint32_t>(spread(1, i % 3 ? 3000 : (1 << 22) - 1));
         a.room = spread(1, i % 5 ? 1 << 20 : (1u << 31) - 1);

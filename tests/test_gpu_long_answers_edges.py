@@ -115,3 +115,50 @@ def test_weights_are_finite(gpu, what, max_new, density):
     out = p.run(gpu, max_new=max_new)
     assert all(np.isfinite(out[r, :max(0, kv)]).all() for r, kv in enumerate(p.kv))
     p.check(gpu, out=out)
+
+
+def _requests(gpu, n, cols, heads, kv_heads, hints, tokens=1, seed=37):
+    """Weights of n short requests in rows of `cols` pages of 16, by calls of the given numbers of requests."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    i32, dim, pages = dict(dtype=torch.int32, device="cuda"), 8, 512
+    table = torch.full((n, cols), -1, **i32)
+    table[:, :2] = torch.randint(0, pages, (n, 2), device="cuda", generator=g).to(torch.int32)
+    kc = torch.randn(pages, 16, kv_heads, dim, device="cuda", generator=g).half()
+    q = torch.empty(n * tokens, heads, dim, device="cuda", dtype=torch.float16).normal_(generator=g)
+    lse = torch.full((n * tokens, heads), 3.0, device="cuda")
+    kv_len = torch.randint(1, 33, (n,), device="cuda", generator=g).to(torch.int32)
+    starts = torch.arange(0, n * tokens + 1, tokens, **i32)
+
+    def weights(each):
+        out = torch.full((n, cols * 16), 7.0, device="cuda")
+        for r in range(0, n, each):
+            s = slice(r, r + each)
+            gpu.paged_weights(q[r * tokens:(r + each) * tokens], kc, table[s], starts[r:r + each + 1] - starts[r], kv_len[s],
+                              lse[r * tokens:(r + each) * tokens], out[s], **hints)
+        torch.cuda.synchronize()
+        return out, kv_len
+
+    return weights
+
+
+def test_more_requests_than_a_launch_holds(gpu):
+    """131072 requests of 65 rows to each of 64 key heads: 2^23 workgroups."""
+    import torch
+    _say("weights, more than a launch")
+    weights = _requests(gpu, 1 << 17, 2, 64 * 65, 64, dict(max_new=1))
+    got, kv_len = weights(1 << 17)
+    want, _ = weights(1 << 15)
+    seen = torch.arange(32, device="cuda")[None] < kv_len[:, None]
+    assert torch.equal(got, want) and bool((got[seen] > 0).all()) and bool((got[~seen] == 7.0).all())
+
+
+@pytest.mark.parametrize("hints", [{}, dict(max_kv=1 << 17, max_new=1), dict(max_kv=32)])
+def test_many_requests_in_wide_tables(gpu, hints):
+    """4096 single tokens whose tables have room for 131072 positions each: refused with no launch of that size to make."""
+    import torch
+    _say("weights in wide tables", hints)
+    got, kv_len = _requests(gpu, 4096, 8192, 16, 8, hints)(4096)
+    want, _ = _requests(gpu, 4096, 2, 16, 8, {})(4096)
+    assert torch.equal(got[:, :32], want) and bool((got[:, 32:] == 7.0).all())
+    assert bool((want[:, 0] > 0).all())
