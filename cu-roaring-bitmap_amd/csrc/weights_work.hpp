@@ -63,7 +63,9 @@ inline WeightsWork weights_work(const WeightsShape& a)
     const uint64_t most = a.max_kv ? std::min<uint64_t>(a.room, a.max_kv) : a.room;
     // Rows of a request that share a key head, as far as the caller says.
     const uint32_t group = a.heads / a.kv_heads;
-    const uint64_t total = static_cast<uint64_t>(a.n_tokens) * group, mean = (total + a.n_requests - 1) / a.n_requests;
+    // (q may hold more tokens than are counted: a prompt's last ones, with starts moved up to them)
+    const uint64_t counted = a.max_new ? std::min<uint64_t>(a.n_tokens, static_cast<uint64_t>(a.max_new) * a.n_requests) : a.n_tokens;
+    const uint64_t total = counted * group, mean = (total + a.n_requests - 1) / a.n_requests;
     w.few = few_rows(a.dim);
     const uint32_t cols = tile_cols(a.dim);
     w.tiles = static_cast<uint32_t>((most + cols - 1) / cols);
@@ -73,7 +75,7 @@ inline WeightsWork weights_work(const WeightsShape& a)
     // Where requests have few rows on average, but one of them may have many (a prompt among single
     // tokens), each kernel takes its own kind, which a launch before lists.  One new token a request on
     // average is taken for single tokens.
-    w.mixed = uneven && !w.many && total > 2 * w.few && (a.max_new ? longest > 2 * w.few : a.n_tokens > a.n_requests);
+    w.mixed = uneven && !w.many && total > 2 * w.few && (a.max_new ? longest > 2 * w.few : counted > a.n_requests);
     // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than 2048
     // rows, and no parts of fewer than 256 where it can be helped, which end in more sums to be
     // joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44; a prompt

@@ -90,6 +90,17 @@ int main()
     check({512 * 2048, 32, 8, 128, 512, 131072, 2048, 131072, false, 256}, rng);
     check({4096, 32, 8, 128, 4096, 131072, 1, 0, false, 256}, rng);
     check({4096, 32, 8, 128, 4096, 131072, 1, 131072, false, 256}, rng);
+    // a prompt's last tokens, or some of each request's, in a q that holds all: one part of rows
+    for (bool some : {false, true}) {
+        const WeightsShape last{131072, 32, 8, 128, 1, 131072, 64, 0, some, 256};
+        const WeightsShape each{131072, 32, 8, 128, 8, 32768, 100, 32768, some, 256};
+        check(last, rng);
+        check(each, rng);
+        EXPECT(weights_work(last).sums <= last.kv_heads * last.room, "%s: %llu", text(last).c_str(),
+               static_cast<unsigned long long>(weights_work(last).sums));
+        EXPECT(weights_work(each).sums <= 8 * 2 * each.kv_heads * each.room, "%s: %llu", text(each).c_str(),
+               static_cast<unsigned long long>(weights_work(each).sums));
+    }
     for (int i = 0; i < 200000; ++i) {
         WeightsShape a{};
         a.kv_heads = i % 7 ? 1u << rng() % 7 : static_cast<uint32_t>(spread(1, 65535));

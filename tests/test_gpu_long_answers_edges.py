@@ -162,3 +162,19 @@ def test_many_requests_in_wide_tables(gpu, hints):
     want, _ = _requests(gpu, 4096, 2, 16, 8, {})(4096)
     assert torch.equal(got[:, :32], want) and bool((got[:, 32:] == 7.0).all())
     assert bool((want[:, 0] > 0).all())
+
+
+@pytest.mark.parametrize("max_new", [0, 40, 20])
+@pytest.mark.parametrize("some", [False, True])
+def test_the_last_tokens_of_a_prompt(gpu, some, max_new):
+    """Starts moved up to the tokens that count, in a q that holds all of them; a hint that is too small changes nothing."""
+    import torch
+    _say("weights of a prompt's last tokens", some, max_new)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    p = test_gpu_weights.Problem("bfloat16", [700], [900], 8, 2, 128, 16, seed=38)
+    if some:
+        got = p.run(gpu, starts=torch.tensor([660], **i32), d_new=torch.tensor([40], **i32), max_new=max_new)
+    else:
+        got = p.run(gpu, starts=torch.tensor([660, 700], **i32), max_new=max_new)
+    p.new, p.q, p.lse = [40], p.q[660:].contiguous(), p.lse[660:].contiguous()
+    p.check(gpu, out=got)
