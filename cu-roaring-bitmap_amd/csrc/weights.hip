@@ -80,8 +80,9 @@ struct WeightArgs {
     // is filled with positions that it looks up at once.
     uint32_t head_waves, spans, halves;
     // Many rows: parts of a request's rows, of part_rows or more each; tiles of positions
-    // that the launch has for a request; and their sums [n_requests][parts][key heads][room].
-    uint32_t parts, part_rows, tiles, room;
+    // that the launch has for a request; and the sums of the `side` parts from part `first` on
+    // (of the list: from entry `first` on) that the launch takes, [n_requests][side][key heads][room].
+    uint32_t parts, part_rows, tiles, room, first, side;
     float* sums;
     // Requests of both kinds: the parts of those with many rows, (request, part of it) [max_listed],
     // each request's first of them (or NONE), how many there are, and the requests that have some.
@@ -334,8 +335,8 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
     __shared__ uint32_t s_col[LISTED ? COLS : 1], s_seen[WT_NT / 64];
     const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6, c32 = lane & 31u, h = lane >> 5;
     const uint32_t kh = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads / a.tiles;
-    if (a.listed && part >= a.counts[0]) return;
-    const uint2 of = a.listed ? a.listed[part] : make_uint2(part / a.parts, part % a.parts);
+    if (a.listed && a.first + part >= a.counts[0]) return;
+    const uint2 of = a.listed ? a.listed[a.first + part] : make_uint2(part / a.side, a.first + part % a.side);
     const uint32_t r = of.x, group = a.heads / a.kv_heads;
     const Counted t = counted_of(a, r);
     const uint32_t rows = t.tokens * group;
@@ -582,31 +583,42 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
     const uint32_t n_requests = LISTED ? a.counts[1] : a.n_requests;
     for (uint32_t k = blockIdx.x / per_request; k < n_requests; k = LISTED ? k + side : n_requests) {
         const uint32_t r = LISTED ? a.many[k] : k;
-        const uint64_t part0 = LISTED ? a.first_of[r] : static_cast<uint64_t>(r) * a.parts;
         const Counted t = counted_of(a, r);
         const uint32_t rows = t.tokens * group, size = part_size(a, rows);
-        const uint32_t held = min(a.parts, (rows + size - 1) / size);  // parts behind have no rows, and left no sums
+        // The request's parts that this launch has sums of, which lie from part `at` on.
+        uint32_t lo = a.first, hi = min((rows + size - 1) / size, a.first + a.side);  // (those behind have no rows)
+        uint64_t at = static_cast<uint64_t>(r) * a.side;
+        bool begins = a.first == 0;  // the launch has the first of them
+        if (LISTED) {
+            const uint32_t part0 = a.first_of[r];
+            begins = part0 >= a.first;
+            lo = begins ? 0u : a.first - part0;
+            hi = part0 >= a.first + a.side ? 0u : min((rows + size - 1) / size, a.first + a.side - part0);
+            if (lo >= hi) continue;
+            at = begins ? part0 - a.first : 0u;
+        }
+        hi = max(lo, hi);
         for (uint32_t p0 = blockIdx.x % per_request * 64; p0 < t.keys; p0 += per_request * 64) {
             const uint32_t p = p0 + lane;
             float sum = 0.0f;
-            uint32_t skip = 0;  // parts that see nothing of the position's tile: the first ones
-            for (uint32_t first, end; skip < held; ++skip) {
+            uint32_t skip = lo;  // parts that see nothing of the position's tile: the first ones
+            for (uint32_t first, end; skip < hi; ++skip) {
                 rows_of_part(a, t, p0 / cols * cols, group, skip, first, end);
                 if (first < end) break;
             }
             if (p < t.keys)
 #pragma unroll 4
-                for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES)
-                    sum += a.sums[(part0 * a.kv_heads + i) * a.room + p];
+                for (uint32_t i = (skip - lo) * a.kv_heads + wave; i < (hi - lo) * a.kv_heads; i += WAVES)
+                    sum += a.sums[(at * a.kv_heads + i) * a.room + p];
             // Not a number: the key holds something that wt_tiles has multiplied rows which count for nothing
             // with too.  (A test a product there would cost registers that three waves a SIMD do not have.)
             if (sum != sum) {
                 sum = 0.0f;
-                for (uint32_t i = skip * a.kv_heads + wave; i < held * a.kv_heads; i += WAVES) {
-                    float more = a.sums[(part0 * a.kv_heads + i) * a.room + p];
+                for (uint32_t i = (skip - lo) * a.kv_heads + wave; i < (hi - lo) * a.kv_heads; i += WAVES) {
+                    float more = a.sums[(at * a.kv_heads + i) * a.room + p];
                     if (more != more) {
                         uint32_t first, end;
-                        rows_of_part(a, t, p0 / cols * cols, group, i / a.kv_heads, first, end);
+                        rows_of_part(a, t, p0 / cols * cols, group, lo + i / a.kv_heads, first, end);
                         more = sum_of_rows<E>(a, t, r, p, i % a.kv_heads, first, end);
                     }
                     sum += more;
@@ -619,7 +631,8 @@ __global__ __launch_bounds__(WJ_NT) void wt_join(WeightArgs a, uint32_t per_requ
 #pragma unroll
                 for (uint32_t w = 0; w < WAVES; ++w) all += s_sum[w][lane];
                 const float past =
-                    a.past && (a.continued || static_cast<int64_t>(p) < t.older) ? a.past[r * a.past_stride + p] * a.decay : 0.0f;
+                    !begins ? a.out[r * a.out_stride + p]
+                    : a.past && (a.continued || static_cast<int64_t>(p) < t.older) ? a.past[r * a.past_stride + p] * a.decay : 0.0f;
                 a.out[r * a.out_stride + p] = past + all;
             }
             __syncthreads();
@@ -782,12 +795,13 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
     a.halves = w.halves;
     a.spans = w.spans;
     a.part_rows = w.part_rows;
-    a.parts = w.parts;
+    a.parts = w.mixed ? 1u << 30 : w.parts;  // (of listed requests as many as the rows need)
+    a.side = w.side;
     a.tiles = w.tiles;
-    a.max_listed = w.max_listed;
+    a.max_listed = w.parts;
     Carver cv;
-    const size_t o_sums = cv.add(w.sums * 4), o_listed = cv.add(w.max_listed * 8ull);
-    const size_t o_many = cv.add(w.mixed ? w.max_listed * 4ull + 16 : 0), o_first = cv.add(w.mixed ? p.n_requests * 4ull : 0);
+    const size_t o_sums = cv.add(w.sums * 4), o_listed = cv.add(w.mixed ? w.parts * 8ull : 0);
+    const size_t o_many = cv.add(w.mixed ? w.parts * 4ull + 16 : 0), o_first = cv.add(w.mixed ? p.n_requests * 4ull : 0);
     hipStream_t s = as_stream(stream);
     const bool direct = p.visible && is_direct(p.visible);
     const uint32_t n_words = static_cast<uint32_t>((n_slots + 31) / 32);
@@ -823,10 +837,10 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         CR_TIMED("wt_rows", s);
         launch(a, w.rows_grid);
     }
-    if (w.many || w.mixed) a.sums = sc.at<float>(o_sums);
-    for (uint32_t r = 0; w.mixed ? r == 0 : w.many && r < p.n_requests; r += w.mixed ? 1 : w.batch) {
+    if (w.side) a.sums = sc.at<float>(o_sums);
+    for (uint32_t r = 0; w.side && r < p.n_requests; r += w.mixed ? p.n_requests : w.batch) {
         WeightArgs b = a;  // of requests from r on
-        uint32_t side = w.join_side, grid = w.tiles_grid;
+        uint32_t at_once = w.join_side, grid = w.tiles_grid;
         if (w.many) {
             b.starts += r;
             if (b.fresh) b.fresh += r;
@@ -834,18 +848,20 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
             b.table += r * b.table_stride;
             if (b.past) b.past += r * b.past_stride;
             b.out += r * b.out_stride;
-            b.n_requests = side = std::min(w.batch, p.n_requests - r);
-            grid = grid / w.batch * side;
+            b.n_requests = at_once = std::min(w.batch, p.n_requests - r);
+            grid = grid / w.batch * at_once;
         }
-        {
-            CR_TIMED("wt_tiles", s);
-            launch(b, grid);
+        for (b.first = 0; b.first < w.parts; b.first += w.side) {
+            {
+                CR_TIMED("wt_tiles", s);
+                launch(b, grid);
+            }
+            CR_TIMED("wt_join", s);
+            if (cache->dtype == CR_F16)
+                join(b, at_once, Half{});
+            else
+                join(b, at_once, BHalf{});
         }
-        CR_TIMED("wt_join", s);
-        if (cache->dtype == CR_F16)
-            join(b, side, Half{});
-        else
-            join(b, side, BHalf{});
     }
     CR_LAUNCH_CHECK();
     return CR_OK;

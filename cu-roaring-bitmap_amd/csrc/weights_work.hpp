@@ -44,11 +44,11 @@ struct WeightsWork {
     // wt_rows: waves that share the heads, how often a wave's LDS is filled with positions that it
     // looks up at once, and workgroups of a request.
     uint32_t head_waves, halves, spans, rows_grid;
-    // wt_tiles: parts of a request's rows, of part_rows or more each; tiles of positions that the
-    // launch has for a request; and the parts that the list has room for.
-    uint32_t part_rows, parts, tiles, max_listed, tiles_grid;
-    uint32_t batch;  // requests of a launch, one after another: all of them, unless a launch cannot hold them
-    uint64_t sums;   // floats that it leaves for wt_join
+    // wt_tiles: parts of a request's rows, of part_rows or more each (or, of listed requests, how many
+    // parts there may be in all), and tiles of positions that a launch has for a request.  A launch
+    // takes `batch` requests and `side` of their parts, or `side` of the list.
+    uint32_t part_rows, parts, side, batch, tiles, tiles_grid;
+    uint64_t sums;  // floats that a launch leaves for wt_join
     // wt_join: workgroups of a request, and requests at a time.
     uint32_t join_per_request, join_side;
 };
@@ -56,6 +56,10 @@ struct WeightsWork {
 // A launch holds fewer than 2^32 threads.  Workgroups come back for more positions where it does not
 // hold one for all of them, so that the caller's hints never decide whether it is answered.
 constexpr uint64_t WT_LAUNCH = (1u << 23) - 1;
+// The sums of a launch of wt_tiles take at most 512 MB: every part of rows leaves one for each key head and
+// each position that a table has room for.  More parts go launch after launch; where one takes more, wt_rows
+// takes them all.  (8 key heads, tables of 131072 positions: 128 parts.)
+constexpr uint64_t WT_SUMS = 1u << 27;
 
 inline WeightsWork weights_work(const WeightsShape& a)
 {
@@ -88,28 +92,35 @@ inline WeightsWork weights_work(const WeightsShape& a)
     // a prompt of 2048 among them: 320 us, not 1130; with max_kv 193).
     const uint64_t places = (a.max_kv ? 256ull : 64ull) * a.cus;
     auto at_most = [](uint64_t n, uint64_t most) { return std::max<uint64_t>(1, std::min(n, most)); };
+    const uint64_t per = a.kv_heads * a.room, most_side = std::min(per ? WT_SUMS / per : WT_SUMS, WT_LAUNCH / a.kv_heads);
+    w.many = w.many && most_side;
+    w.mixed = w.mixed && most_side;
     if (w.mixed) {
-        const uint64_t listed = total / w.part_rows + total / (w.few + 1) + 1;
-        const uint64_t tiles = at_most(w.tiles, places / (listed * a.kv_heads)), grid = listed * tiles * a.kv_heads;
-        if (listed >> 20 || grid >> 23) {
-            w.mixed = false;  // too large a launch: wt_rows answers them all
+        // A request counts as one of many rows from more rows on, where the list would have room for little
+        // but requests of one part.
+        const uint64_t full = total / w.part_rows + 1;
+        if (full + std::min<uint64_t>(total / (w.few + 1), a.n_requests) > most_side)
+            w.few = std::max(w.few, static_cast<uint32_t>(total / std::max(most_side, full)));
+        const uint64_t listed = full + std::min<uint64_t>(total / (w.few + 1), a.n_requests);
+        if (listed >> 20) {
+            w.mixed = false;  // too long a list: wt_rows answers them all
         } else {
-            w.tiles = static_cast<uint32_t>(tiles);
-            w.tiles_grid = static_cast<uint32_t>(grid);
-            w.max_listed = static_cast<uint32_t>(listed);
-            w.parts = 1u << 30;  // (as many as the rows need)
-            w.sums = listed * a.kv_heads * a.room;
+            w.parts = static_cast<uint32_t>(listed);
+            w.side = static_cast<uint32_t>(std::min(listed, most_side));
+            w.tiles = static_cast<uint32_t>(at_most(w.tiles, places / (static_cast<uint64_t>(w.side) * a.kv_heads)));
+            w.tiles_grid = w.side * w.tiles * a.kv_heads;
+            w.sums = w.side * per;
         }
     }
     if (w.many) {
-        const uint64_t parts = std::max<uint64_t>(1, (mean + w.part_rows - 1) / w.part_rows);
-        w.parts = static_cast<uint32_t>(std::min(parts, WT_LAUNCH / a.kv_heads));
-        const uint64_t each = static_cast<uint64_t>(w.parts) * a.kv_heads;  // workgroups of a request and a tile
-        w.batch = static_cast<uint32_t>(std::min<uint64_t>(a.n_requests, WT_LAUNCH / each));
-        if (!a.max_kv) w.tiles = static_cast<uint32_t>(at_most(w.tiles, places / (parts * a.n_requests * a.kv_heads)));
+        w.parts = static_cast<uint32_t>(std::max<uint64_t>(1, (mean + w.part_rows - 1) / w.part_rows));
+        w.side = static_cast<uint32_t>(std::min<uint64_t>(w.parts, most_side));
+        const uint64_t each = static_cast<uint64_t>(w.side) * a.kv_heads;  // workgroups of a request and a tile
+        w.batch = static_cast<uint32_t>(std::min<uint64_t>(a.n_requests, most_side / w.side));
+        if (!a.max_kv) w.tiles = static_cast<uint32_t>(at_most(w.tiles, places / (each * w.batch)));
         w.tiles = static_cast<uint32_t>(at_most(w.tiles, WT_LAUNCH / (each * w.batch)));
         w.tiles_grid = static_cast<uint32_t>(each * w.batch * w.tiles);
-        w.sums = each * w.batch * a.room;
+        w.sums = w.side * w.batch * per;
     } else {
         w.head_waves = a.kv_heads >= 3 ? 4 : a.kv_heads;
         // A wave looks up 64 positions at once and fills its LDS with them two or four times where there
@@ -127,7 +138,7 @@ inline WeightsWork weights_work(const WeightsShape& a)
     }
     if (w.many || w.mixed) {
         // (fewer than 2^32 threads; of listed requests, which may be few or none, a few rounds of the card)
-        const uint32_t requests = w.mixed ? std::min(w.max_listed, a.n_requests) : w.batch;
+        const uint32_t requests = w.mixed ? std::min(w.parts, a.n_requests) : w.batch;
         uint64_t wanted = (most + 63) / 64;
         if (!a.max_kv) wanted = at_most(wanted, places / requests);
         w.join_per_request = static_cast<uint32_t>(std::min<uint64_t>(wanted, ((1u << 22) - 1) / (w.mixed ? 1u : requests)));

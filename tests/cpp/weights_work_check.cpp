@@ -1,6 +1,7 @@
 // How cr_paged_weights splits its work (csrc/weights_work.hpp), run on the CPU for shapes of every size.
 //   - every launch has work and fewer than 2^32 threads, whatever the caller says of its lengths;
-//   - the requests with many rows fit the list that is made of them.
+//   - the requests with many rows fit the list that is made of them;
+//   - the sums that a launch leaves take at most 512 MB.
 // Prints how often each way was taken, and "weights_work_check: OK".
 #include <cstdio>
 #include <cstdlib>
@@ -51,14 +52,16 @@ static void check(const WeightsShape& a, std::mt19937_64& rng)
         EXPECT(w.part_rows >= 64 && w.part_rows % 64 == 0, "%s: %u", what.c_str(), w.part_rows);
         EXPECT(w.join_per_request && w.join_side && static_cast<uint64_t>(w.join_per_request) * w.join_side < LAUNCH * 2, "%s", what.c_str());
     }
+    EXPECT(w.sums <= WT_SUMS, "%s: %llu", what.c_str(), static_cast<unsigned long long>(w.sums));
+    if (w.many || w.mixed) EXPECT(w.side && w.side <= w.parts, "%s", what.c_str());
     if (w.many) {
         EXPECT(w.batch && w.batch <= a.n_requests, "%s", what.c_str());
-        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.parts) * w.batch * w.tiles * a.kv_heads, "%s", what.c_str());
-        EXPECT(w.sums == static_cast<uint64_t>(w.parts) * w.batch * a.kv_heads * a.room, "%s", what.c_str());
+        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.side) * w.batch * w.tiles * a.kv_heads, "%s", what.c_str());
+        EXPECT(w.sums == static_cast<uint64_t>(w.side) * w.batch * a.kv_heads * a.room, "%s", what.c_str());
     }
     if (w.mixed) {
-        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.max_listed) * w.tiles * a.kv_heads, "%s", what.c_str());
-        EXPECT(w.sums == static_cast<uint64_t>(w.max_listed) * a.kv_heads * a.room, "%s", what.c_str());
+        EXPECT(w.tiles_grid == static_cast<uint64_t>(w.side) * w.tiles * a.kv_heads, "%s", what.c_str());
+        EXPECT(w.sums == static_cast<uint64_t>(w.side) * a.kv_heads * a.room, "%s", what.c_str());
         // the parts of requests that share the tokens in any way, of which none has more than the caller says
         for (int way = 0; way < 4; ++way) {
             uint64_t left = a.n_tokens, parts = 0;
@@ -70,10 +73,13 @@ static void check(const WeightsShape& a, std::mt19937_64& rng)
                 const uint64_t rows = n * group;
                 if (rows > w.few) parts += (rows + w.part_rows - 1) / w.part_rows;
             }
-            EXPECT(parts <= w.max_listed, "%s: %llu parts, %u listed", what.c_str(), static_cast<unsigned long long>(parts), w.max_listed);
+            EXPECT(parts <= w.parts, "%s: %llu parts, %u listed", what.c_str(), static_cast<unsigned long long>(parts), w.parts);
         }
     }
     ++g_ways[w.many ? "many rows" : w.mixed ? "mixed" : "few rows"];
+    if (w.many && w.batch < a.n_requests) ++g_ways["many rows, some requests at a time"];
+    if (w.many && w.side < w.parts) ++g_ways["many rows, some parts at a time"];
+    if (w.mixed && w.side < w.parts) ++g_ways["mixed, some parts at a time"];
 }
 
 int main()
@@ -101,6 +107,10 @@ int main()
         EXPECT(weights_work(each).sums <= 8 * 2 * each.kv_heads * each.room, "%s: %llu", text(each).c_str(),
                static_cast<unsigned long long>(weights_work(each).sums));
     }
+    // long prompts, alone and among single tokens in wide tables
+    check({131072, 32, 8, 128, 1, 131072, 131072, 131072, false, 256}, rng);
+    check({1 << 21, 32, 8, 128, 1, 1 << 21, 0, 0, false, 256}, rng);
+    check({4096 + 1023, 64, 8, 128, 1024, 131072, 4096, 0, false, 256}, rng);
     for (int i = 0; i < 200000; ++i) {
         WeightsShape a{};
         a.kv_heads = i % 7 ? 1u << rng() % 7 : static_cast<uint32_t>(spread(1, 65535));
@@ -116,7 +126,8 @@ int main()
         check(a, rng);
     }
     for (const auto& [way, times] : g_ways) printf("%s: %d\n", way.c_str(), times);
-    for (const char* way : {"many rows", "mixed", "few rows"}) EXPECT(g_ways.count(way), "\"%s\" was not taken", way);
+    for (const char* way : {"many rows", "mixed", "few rows", "many rows, some requests at a time", "many rows, some parts at a time",
+                            "mixed, some parts at a time"}) EXPECT(g_ways.count(way), "\"%s\" was not taken", way);
     if (g_errors) {
         printf("weights_work_check: %d errors\n", g_errors);
         return 1;

@@ -178,3 +178,45 @@ def test_the_last_tokens_of_a_prompt(gpu, some, max_new):
         got = p.run(gpu, starts=torch.tensor([660, 700], **i32), max_new=max_new)
     p.new, p.q, p.lse = [40], p.q[660:].contiguous(), p.lse[660:].contiguous()
     p.check(gpu, out=got)
+
+
+@pytest.mark.parametrize("what", [
+    # tokens of each request, heads, key heads, room: sums of some requests or some parts of rows at a time
+    ([64] * 300, 32, 8, 65536), ([10000], 32, 8, 1 << 20), ([9000, 100, 0, 12000], 32, 8, 1 << 20),
+    ([1] * 450 + [10000] + [1] * 400 + [70] + [1] * 48, 256, 64, 131072)])
+def test_sums_that_do_not_fit_at_once(gpu, what):
+    """The same requests in tables of just their positions and in wide ones, whose sums go launch after launch.  Either
+    adds the same n terms in an order of its own, n 2^-24 of the sum off at most, and may multiply by the other kernel:
+    a score is (dim + 8) 2^-23 of the size of its terms off, its difference to the log-sum 2^-24 of each, the exponential
+    2^-22."""
+    import torch
+    tokens, heads, kv_heads, room = what
+    _say("weights whose sums do not fit", len(tokens), max(tokens), room)
+    g = torch.Generator(device="cuda").manual_seed(39)
+    i32, dim, n, total = dict(dtype=torch.int32, device="cuda"), 64, len(tokens), sum(tokens)
+    most = max(t + 300 for t in tokens)
+    cols, pages = -(-most // 16), 1024
+    near = torch.randint(0, pages, (n, cols), device="cuda", generator=g).to(torch.int32)
+    wide = torch.full((n, room // 16), -1, **i32)
+    wide[:, :cols] = near
+    kc = torch.randn(pages, 16, kv_heads, dim, device="cuda", generator=g).half()
+    q = torch.empty(total, heads, dim, device="cuda", dtype=torch.float16).normal_(generator=g)
+    lse = torch.rand(total, heads, device="cuda", generator=g) + 8
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(tokens)]).astype(np.int32)).cuda()
+    kv_len = torch.tensor([t + 7 * r % 300 for r, t in enumerate(tokens)], **i32)
+    outs = []
+    for table in (near, wide):
+        out = torch.full((n, table.shape[1] * 16), 7.0, device="cuda")
+        out[:, :cols * 16] = 0.25
+        gpu.paged_weights(q, kc, table, starts, kv_len, lse, out, d_past=out, decay=0.5)
+        outs.append(out[:, :cols * 16])
+        assert bool((out[:, cols * 16:] == 7.0).all())
+    torch.cuda.synchronize()
+    rows = torch.tensor(tokens, device="cuda")[:, None] * (heads // kv_heads) * kv_heads
+    seen = torch.arange(cols * 16, device="cuda")[None] < kv_len[:, None]
+    near, wide = outs
+    assert bool((near[seen] > 0).all()) and bool((near[~seen] == 0.25).all()) and bool((wide[~seen] == 0.25).all())
+    size = dim ** -0.5 * float(q.float().norm(dim=-1).max()) * float(kc.float().norm(dim=-1).max())  # of a score's terms
+    off = (dim + 8) * 2.0 ** -23 * size + 2.0 ** -24 * (3 * size + 2 * 9) + 2.0 ** -22
+    terms = (rows / 16 + 64).expand_as(near)  # (a lane adds sixteen rows in pairs, so that no chain is longer)
+    assert bool(((near - wide).abs() <= 2 * (off + terms * 2.0 ** -24) * near).all()), ((near - wide).abs() / near).max()
