@@ -525,13 +525,18 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
         };
         if (!LISTED) __syncthreads();  // (the rows' places are noted)
         if (!none) load(0, s_q0);
-        for (uint32_t i = 0; !none && i < n_stages; i += 2) {
+        // Each wave waits for its own loads to LDS before all meet.
+        auto arrived = [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
             __syncthreads();
+        };
+        for (uint32_t i = 0; !none && i < n_stages; i += 2) {
+            arrived();
             if (i + 1 < n_stages) load(i + 1, s_q1);
             if (wave == 2 && i + 2 < n_stages) note(i + 2);
             multiply(i, s_q0);
             if (i + 1 >= n_stages) break;
-            __syncthreads();
+            arrived();
             if (i + 2 < n_stages) load(i + 2, s_q0);
             if (wave == 3 && i + 3 < n_stages) note(i + 3);
             multiply(i + 1, s_q1);
