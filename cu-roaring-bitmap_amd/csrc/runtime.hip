@@ -311,18 +311,49 @@ static uint32_t g_fail_skip = 0, g_fail_count = 0;
 
 // A call that is captured into a graph keeps its workspace for good: the graph names
 // its address and may be replayed at any time, beside whatever runs then.  Such
-// blocks are allocated past the pool, which a capture would record, never handed out
-// again, and marked by this in place of a device.
+// blocks are allocated past the pool, which a capture would record, and marked by this
+// in place of a device.  What one call of a capture has freed, a later one on the same
+// stream of that capture is handed again, since the graph keeps their order; no other
+// capture is, nor any call outside.
 constexpr int CAPTURED = -1;
+struct CapturedBlock {
+    void* p;
+    size_t bytes;
+    hipStream_t stream;
+    unsigned long long capture;
+};
+static std::unordered_map<void*, CapturedBlock> g_captured;  // handed out
+static std::vector<CapturedBlock> g_captured_free;           // of captures that may be over: oldest first
+constexpr size_t CAPTURED_MAX_BLOCKS = 256;
 
-static bool is_capturing(hipStream_t s)
+// The number of the capture that the stream is in, which no other has: 0 outside.
+static unsigned long long capture_of(hipStream_t s)
 {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    return s && hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusActive;
+    unsigned long long id = 0;
+    return s && hipStreamGetCaptureInfo(s, &st, &id) == hipSuccess && st == hipStreamCaptureStatusActive ? id : 0;
 }
 
-static int captured_alloc(void** p, size_t bytes)
+static int captured_alloc(void** p, size_t bytes, hipStream_t s, unsigned long long capture)
 {
+    {
+        std::lock_guard<std::mutex> lock(g_cache_mu);
+        size_t best = g_captured_free.size();
+        for (size_t i = 0; i < g_captured_free.size(); ++i) {
+            const CapturedBlock& b = g_captured_free[i];
+            if (b.capture == capture && b.stream == s && b.bytes >= bytes &&
+                (best == g_captured_free.size() || b.bytes < g_captured_free[best].bytes))
+                best = i;
+        }
+        if (best != g_captured_free.size()) {
+            const CapturedBlock b = g_captured_free[best];
+            g_captured_free.erase(g_captured_free.begin() + static_cast<std::ptrdiff_t>(best));
+            g_live[b.p] = {b.bytes, CAPTURED};
+            g_captured[b.p] = b;
+            *p = b.p;
+            return CR_OK;
+        }
+    }
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     CR_HIP_RET(hipThreadExchangeStreamCaptureMode(&mode));
     const hipError_t e = hipMalloc(p, bytes);
@@ -334,6 +365,7 @@ static int captured_alloc(void** p, size_t bytes)
     }
     std::lock_guard<std::mutex> lock(g_cache_mu);
     g_live[*p] = {bytes, CAPTURED};
+    g_captured[*p] = {*p, bytes, s, capture};
     return CR_OK;
 }
 
@@ -344,7 +376,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
     if (bytes == 0) bytes = 256;
     int dev = 0;
     CR_HIP_RET(hipGetDevice(&dev));
-    const bool capturing = is_capturing(s);
+    const unsigned long long capture = capture_of(s);
     {
         std::lock_guard<std::mutex> lock(g_cache_mu);
         if (g_fail_count) {
@@ -357,7 +389,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
             }
         }
         size_t best = g_cache.size();
-        for (size_t i = 0; !capturing && i < g_cache.size(); ++i) {
+        for (size_t i = 0; !capture && i < g_cache.size(); ++i) {
             const CachedBlock& b = g_cache[i];
             if (b.dev == dev && b.stream == s && b.bytes >= bytes && b.bytes <= 2 * bytes &&
                 (best == g_cache.size() || b.bytes < g_cache[best].bytes))
@@ -372,7 +404,7 @@ int dev_alloc(void** p, size_t bytes, hipStream_t s)
             return CR_OK;
         }
     }
-    if (capturing) return captured_alloc(p, bytes);
+    if (capture) return captured_alloc(p, bytes, s, capture);
     hipMemPool_t pool = library_pool();
     hipError_t e = pool ? hipMallocFromPoolAsync(p, bytes, pool, s) : hipMallocAsync(p, bytes, s);
     if (e != hipSuccess) {
@@ -398,7 +430,13 @@ int dev_free(void* p, hipStream_t s)
             return CR_OK;
         }
         if (it->second.second == CAPTURED) {
+            const CapturedBlock b = g_captured[p];
             g_live.erase(it);
+            g_captured.erase(p);
+            if (s == b.stream && capture_of(s) == b.capture) {
+                if (g_captured_free.size() == CAPTURED_MAX_BLOCKS) g_captured_free.erase(g_captured_free.begin());
+                g_captured_free.push_back(b);
+            }
             return CR_OK;
         }
         g_cache.push_back({p, it->second.first, it->second.second, s});

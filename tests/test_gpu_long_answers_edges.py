@@ -220,3 +220,90 @@ def test_sums_that_do_not_fit_at_once(gpu, what):
     off = (dim + 8) * 2.0 ** -23 * size + 2.0 ** -24 * (3 * size + 2 * 9) + 2.0 ** -22
     terms = (rows / 16 + 64).expand_as(near)  # (a lane adds sixteen rows in pairs, so that no chain is longer)
     assert bool(((near - wide).abs() <= 2 * (off + terms * 2.0 ** -24) * near).all()), ((near - wide).abs() / near).max()
+
+
+def _layers(n, seed=35):
+    """The weights of n layers, whose rows are many: (call(i, out, stream), the calls' own results)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    requests, tokens, heads, kv_heads, dim, page, cols = 16, 64, 32, 8, 64, 16, 4096
+    i32 = dict(dtype=torch.int32, device="cuda")
+    half = lambda *s: torch.randn(*s, device="cuda", generator=g).half()  # noqa: E731
+    table = torch.arange(requests * 4, **i32).view(requests, 4).repeat(1, cols // 4)
+    kc = half(requests * 4, page, kv_heads, dim)
+    q = [half(requests * tokens, heads, dim) for _ in range(n)]
+    starts, kv_len = torch.arange(0, requests * tokens + 1, tokens, **i32), torch.full((requests,), tokens, **i32)
+    lse = torch.full((requests * tokens, heads), 4.0, device="cuda")
+
+    def call(gpu, i, out, stream):
+        gpu.paged_weights(q[i], kc, table, starts, kv_len, lse, out, max_new=tokens, stream=stream)
+
+    return call, lambda: torch.zeros(requests, cols * page, device="cuda")
+
+
+def test_captured_layers_share_their_workspace(gpu):
+    """The calls of one capture on one stream follow one another: their workspaces, 32 MB each, are one block.  Replays
+    give what eager calls give."""
+    import torch
+    _say("captured layers")
+    n = 24
+    call, room = _layers(n)
+    outs = [room() for _ in range(n)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(n):
+            call(gpu, i, outs[i], side)
+    side.synchronize()
+    wants = [t.clone() for t in outs]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    with torch.cuda.graph(graph, stream=side):
+        for i in range(n):
+            call(gpu, i, outs[i], side)
+    torch.cuda.synchronize()
+    taken = free - torch.cuda.mem_get_info()[0]
+    assert taken < 4 * 32 << 20, taken
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            for t in outs:
+                t.zero_()
+            graph.replay()
+            call(gpu, 0, room(), side)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+
+
+def test_captured_streams_do_not_share(gpu):
+    """Calls on two streams of one capture run side by side, each in a workspace of its own, as do two graphs."""
+    import torch
+    _say("captured streams")
+    call, room = _layers(4)
+    outs = [room() for _ in range(4)]
+    for i in range(4):
+        call(gpu, i, outs[i], None)
+    torch.cuda.synchronize()
+    wants = [t.clone() for t in outs]
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs = []
+    for first in (0, 2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=one):
+            two.wait_stream(one)
+            call(gpu, first, outs[first], one)
+            with torch.cuda.stream(two):
+                call(gpu, first + 1, outs[first + 1], two)
+            one.wait_stream(two)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, wants))
