@@ -10,6 +10,7 @@
 
 #include "internal.hpp"
 #include "elements.hpp"
+#include "rows.hpp"
 #include "set_bits.hpp"
 
 namespace crimpl {
@@ -250,6 +251,14 @@ extern "C" int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_
         return CR_ERR_UNSUPPORTED;
     }
     if (per_token == 0) return CR_OK;
+    const uint64_t row = static_cast<uint64_t>(dim) * es;
+    const Rows out(p.q_out, p.n_tokens, p.out_token_stride * es, p.n_heads, p.out_head_stride * es, row);
+    const Rows in(p.q, p.n_tokens, p.q_token_stride * es, p.n_heads, p.q_head_stride * es, row);
+    if (rows_overlap(out) || rows_overwrite(out, in)) {
+        set_error("cr_paged_rotary: invalid argument (rows of the turned queries lie over one another, or over other rows of "
+                  "those that are read)");
+        return CR_ERR_INVALID;
+    }
     a.per_token = static_cast<uint32_t>(per_token);
     // A workgroup's threads share a token's pieces, in several workgroups where there are more,
     // or take several tokens side by side.  Its cosines serve all of its tokens: as many as

@@ -472,7 +472,8 @@ int cr_paged_attention(const cr_paged_attention_args* args, const cr_paged_cache
  * 2 i + 1 where `interleaved`) is turned by d_positions[token] * d_freqs[i] and
  * multiplied by `magnitude`; the rest of the row, and the values, stay as they are.
  * Angles are worked out in 64 bits, products in fp32 and rounded once.  q_out may be
- * q, if its rows do not lie over one another.  n_heads 0: keys and values alone.  A token whose slot is outside the cache (-1)
+ * q itself, with the same strides; otherwise its rows lie beside those of q, and never over
+ * one another.  n_heads 0: keys and values alone.  A token whose slot is outside the cache (-1)
  * gets its queries turned. */
 typedef struct cr_paged_rotary_args {
     const void* q; /* [n_tokens][n_heads][cache->head_dim] */

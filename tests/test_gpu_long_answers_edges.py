@@ -307,3 +307,30 @@ def test_captured_streams_do_not_share(gpu):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+
+
+@pytest.mark.parametrize("layout", ["beside", "behind", "between tokens", "heads first", "one token"])
+def test_turned_queries_between_others(gpu, layout):
+    """Queries and turned ones in one tensor, whose rows do not meet."""
+    import torch
+    _say("rotary within one tensor", layout)
+    g = torch.Generator(device="cuda").manual_seed(40)
+    tokens, heads, kv_heads, dim = 1 if layout == "one token" else 21, 6, 2, 64
+    shape = {"beside": (tokens, heads, 2, dim), "behind": (2, tokens, heads, dim), "between tokens": (tokens, 2, heads, dim),
+             "heads first": (2, heads, tokens, dim), "one token": (tokens, heads, 2, dim)}[layout]
+    both = torch.randn(*shape, device="cuda", generator=g).half()
+    axis = shape.index(2)
+    q, out = both.select(axis, 0), both.select(axis, 1)
+    if layout == "heads first":
+        q, out = q.transpose(0, 1), out.transpose(0, 1)
+    if layout == "one token":  # whose stride may be any number
+        out = out.as_strided(out.shape, (7, out.stride(1), 1))
+    k = torch.randn(tokens, kv_heads, dim, device="cuda", generator=g).half()
+    caches = [torch.zeros(4, 16, kv_heads, dim, device="cuda").half() for _ in range(2)]
+    at = torch.arange(tokens, device="cuda") + 5
+    freqs, _ = gpu.rotary_frequencies(dim)
+    want, before = torch.empty(tokens, heads, dim, device="cuda").half(), q.clone()
+    for to in (want, out):
+        gpu.paged_rotary(k, k, at.to(torch.int32), freqs, at, *caches, d_q=q, d_q_out=to)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(q, before)
