@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "internal.hpp"
+#include "rows.hpp"
 #include "set_bits.hpp"
 
 namespace crimpl {
@@ -967,6 +968,12 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     };
     if (meets(p.d_kv_len) || meets(p.d_keep) || meets(p.d_kept) || meets(p.d_seen)) {
         set_error("cr_paged_evict: invalid argument (the lengths that are written lie over those that are read)");
+        return CR_ERR_INVALID;
+    }
+    auto rows = [&](const void* x, uint64_t stride) { return Rows(x, x ? p.n_requests : 0, stride * 4, 1, 0, room * 4); };
+    if (rows_overwrite(rows(p.d_weights_out, p.weights_out_stride), rows(p.d_weights, p.weights_stride)) ||
+        rows_overwrite(rows(p.d_positions_out, p.positions_out_stride), rows(p.d_positions, p.positions_stride))) {
+        set_error("cr_paged_evict: invalid argument (the rows that are written lie over others of those that are read)");
         return CR_ERR_INVALID;
     }
     hipStream_t s = as_stream(stream);

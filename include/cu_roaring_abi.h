@@ -543,7 +543,7 @@ int cr_paged_weights(const cr_paged_weights_args* args, const cr_paged_cache* ca
  * order, into the places in [0, m) that get free: d_moves[r][0, d_n_moves[r]) are
  * pairs (from slot, to slot) for cr_paged_move, never the same slot twice, and
  * d_weights_out[r][0, m) and d_positions_out[r][0, m) (NULL: not wanted) what then
- * lies there; those two may be the inputs themselves, the lengths may not.  A row of d_moves holds half as
+ * lies there; those two may be the inputs themselves, with the same strides, the lengths may not.  A row of d_moves holds half as
  * many pairs as a row of the table has positions.  d_freed[0, freed_cap) receives the
  * pages that no entry of their request is in any more, requests in order, and
  * d_counts[0, 2) their number and that of all moves.  The table stays as it is:

@@ -334,3 +334,35 @@ def test_turned_queries_between_others(gpu, layout):
         gpu.paged_rotary(k, k, at.to(torch.int32), freqs, at, *caches, d_q=q, d_q_out=to)
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(q, before)
+
+
+@pytest.mark.parametrize("apart", ["beside", "behind"])
+@pytest.mark.parametrize("kv", [300, 20000])
+def test_evicted_rows_between_others(gpu, kv, apart):
+    """Rows that are read and written in one tensor, beside one another."""
+    import torch
+    _say("evict within one tensor", kv, apart)
+    rng = np.random.default_rng(41)
+    n, page, keep = 3, 16, kv // 3
+    room = -(-kv // page) * page
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    shape = (n, 2, room) if apart == "beside" else (2, n, room)
+    w, at = torch.zeros(shape, device="cuda"), torch.zeros(shape, **i32)
+    split = (lambda t, i: t[:, i]) if apart == "beside" else (lambda t, i: t[i])
+    weights, places = rng.random((n, room)).astype(np.float32), np.stack([rng.permutation(room) for _ in range(n)]).astype(np.int32)
+    split(w, 0).copy_(cuda(weights))
+    split(at, 0).copy_(cuda(places))
+    table = torch.arange(n * room // page, **i32).view(n, -1)
+    full = lambda x: torch.full((n,), x, **i32)  # noqa: E731
+    length, n_moves, counts = full(-9), full(-9), torch.zeros(2, **i32)
+    moves, freed = torch.zeros(n, room // 2, 2, **i32), torch.zeros(table.numel(), **i32)
+    gpu.paged_evict(split(w, 0), full(kv), full(keep), table, page, split(w, 1), length, moves, n_moves, freed, counts,
+                    d_positions=split(at, 0), d_kept=full(kv), d_seen=full(kv), d_positions_out=split(at, 1), sinks=2, recent=9)
+    torch.cuda.synchronize()
+    assert np.array_equal(split(w, 0).cpu().numpy(), weights) and np.array_equal(split(at, 0).cpu().numpy(), places)
+    for r in range(n):
+        m, lies, pos, _, _ = test_gpu_evict.evict_oracle(weights[r], places[r], kv, kv, kv, keep, table[r].cpu().numpy(), page,
+                                                         table.numel(), 2, 9, np.zeros(n * room, bool))
+        assert int(length[r]) == m and np.array_equal(split(w, 1)[r, :m].cpu().numpy(), weights[r][lies])
+        assert split(at, 1)[r, :m].tolist() == [pos[i] for i in lies]

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import curoaring as cr
-from test_long_answers_abi import INVALID, P, ROTARY, _cache, _filled
+from test_long_answers_abi import EVICT, INVALID, P, ROTARY, _cache, _filled
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -30,3 +30,13 @@ def test_turned_queries_over_others(args):
     a = _filled(cr.PagedRotaryArgs, ROTARY, args)
     assert cr.load().cr_paged_rotary(C.byref(a), C.byref(_cache()), None) == INVALID
     assert b"lie over one another" in cr._lib.cr_last_error()
+
+
+@pytest.mark.parametrize("args", [
+    dict(weights_out_stride=68), dict(weights_stride=128), dict(d_weights_out=P + 16), dict(d_weights_out=P + 256),
+    dict(d_weights=P + 252), dict(positions_out_stride=128), dict(d_positions_out=P + 4), dict(d_positions=P + 256),
+    dict(weights_stride=128, weights_out_stride=128, d_weights_out=P + 252)])
+def test_evicted_rows_over_others(args):
+    a = _filled(cr.PagedEvictArgs, EVICT, args)
+    assert cr.load().cr_paged_evict(C.byref(a), None) == INVALID
+    assert b"lie over others" in cr._lib.cr_last_error()
