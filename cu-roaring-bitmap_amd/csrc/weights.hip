@@ -10,6 +10,7 @@
 
 #include "internal.hpp"
 #include "elements.hpp"
+#include "rows.hpp"
 #include "set_bits.hpp"
 #include "weights_work.hpp"
 
@@ -759,6 +760,11 @@ extern "C" int cr_paged_weights(const cr_paged_weights_args* args, const cr_page
         set_error("cr_paged_weights: supported up to 2^31 - 1 slots, positions and rows, 65535 heads, 2^22 - 1 requests and "
                   "2^36 - 1 weights");
         return CR_ERR_UNSUPPORTED;
+    }
+    auto rows = [&](const void* x, uint64_t stride) { return Rows(x, x ? p.n_requests : 0, stride * 4, 1, 0, room * 4); };
+    if (rows_overwrite(rows(p.d_out, p.out_stride), rows(p.d_past, p.past_stride))) {
+        set_error("cr_paged_weights: invalid argument (the weights that are written lie over others of those that are read)");
+        return CR_ERR_INVALID;
     }
     WeightArgs a{};
     a.q = static_cast<const uint16_t*>(p.q);

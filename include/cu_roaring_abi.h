@@ -503,7 +503,7 @@ int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_cache* cach
  * a shorter d_kv_len.)  lse [n_tokens][n_heads] is what the attention of these rows
  * left, with the same scale; a row whose lse is -inf counts for nothing, whatever its q
  * holds.  `visible`, a bitmap over the slots, or NULL: others got nothing, nor did
- * entries whose page is outside the cache.  d_past may be d_out, or NULL: nothing before.  Sums are in
+ * entries whose page is outside the cache.  d_past may be d_out, with the same stride, or NULL: nothing before.  Sums are in
  * fp32, in an order that depends on the arguments alone.  Entries behind d_kv_len[r]
  * are left as they were.  Types and alignment are those of cr_paged_attention;
  * cache->v is not looked at. */

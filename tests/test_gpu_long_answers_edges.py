@@ -366,3 +366,18 @@ def test_evicted_rows_between_others(gpu, kv, apart):
                                                          table.numel(), 2, 9, np.zeros(n * room, bool))
         assert int(length[r]) == m and np.array_equal(split(w, 1)[r, :m].cpu().numpy(), weights[r][lies])
         assert split(at, 1)[r, :m].tolist() == [pos[i] for i in lies]
+
+
+@pytest.mark.parametrize("what", ["decode ragged", "chunk"])
+def test_weights_between_others(gpu, what):
+    """What was there and what is written in one tensor, row beside row."""
+    import torch
+    _say("weights within one tensor", what)
+    p = test_gpu_weights.Problem("bfloat16", *test_gpu_weights.SHAPES[what], seed=42)
+    room = p.cols * p.page
+    both = torch.full((len(p.kv), 2, room), 7.0, device="cuda")
+    both[:, 0] = p.past[:, :room]
+    gpu.paged_weights(p.q, p.kc, p.table, p.starts, p.kv_len, p.lse, both[:, 1], d_past=both[:, 0], decay=0.75, scale=p.scale)
+    torch.cuda.synchronize()
+    assert torch.equal(both[:, 0], p.past[:, :room])
+    p.check(gpu, out=both[:, 1].cpu().numpy().astype(np.float64))

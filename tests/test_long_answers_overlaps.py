@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import curoaring as cr
-from test_long_answers_abi import EVICT, INVALID, P, ROTARY, _cache, _filled
+from test_long_answers_abi import EVICT, INVALID, P, ROTARY, WEIGHTS, _cache, _filled
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -39,4 +39,13 @@ def test_turned_queries_over_others(args):
 def test_evicted_rows_over_others(args):
     a = _filled(cr.PagedEvictArgs, EVICT, args)
     assert cr.load().cr_paged_evict(C.byref(a), None) == INVALID
+    assert b"lie over others" in cr._lib.cr_last_error()
+
+
+@pytest.mark.parametrize("args", [dict(d_past=P, past_stride=68), dict(d_past=P, past_stride=64, out_stride=128),
+                                  dict(d_past=P + 16, past_stride=64), dict(d_past=P + 256, past_stride=64),
+                                  dict(d_past=P + 252, past_stride=128, out_stride=128)])
+def test_weights_over_others(args):
+    a = _filled(cr.PagedWeightsArgs, WEIGHTS, args)
+    assert cr.load().cr_paged_weights(C.byref(a), C.byref(_cache()), None) == INVALID
     assert b"lie over others" in cr._lib.cr_last_error()
