@@ -855,8 +855,8 @@ def paged_weights(d_q, d_k_cache, d_table, d_starts, d_kv_len, d_lse, d_out, d_p
     heads into d_out float32 [R, at least cols * page_size].
 
     d_lse: float32 [T, heads], what paged_attention left for the same rows and scale.  d_past (d_out itself, if need
-    be): what the tokens older than these rows had, times decay; continued: what all had, as between the layers of a
-    step whose weights are summed.  Rows of request r: [starts[r], starts[r + 1]), or
+    be): what the tokens older than these rows had, times decay; continued: what all had, times decay, as between the
+    layers of a step whose weights are summed (decay 1 behind the first).  Rows of request r: [starts[r], starts[r + 1]), or
     new[r] of them from starts[r] where d_new int32 [R] is given (d_starts then has R or R + 1 entries): the last of its
     kv_len[r] positions.  visible: a bitmap of slots.  max_new and max_kv: the most rows and positions of a request if
     known; they choose how the work is split.  stream: None is the null stream."""

@@ -525,7 +525,9 @@ typedef struct cr_paged_weights_args {
     uint64_t out_stride;
     float scale, decay;
     uint32_t causal;
-    uint32_t continued; /* d_past counts for all entries: a step's layers behind the first */
+    /* d_past, times decay, counts for all entries: a step's layers behind the first, for which
+     * decay is 1 where their weights are to be summed. */
+    uint32_t continued;
     /* The most rows and positions of a request, where the caller knows them (0: not
      * known).  They choose how the work is split, never the answer. */
     uint32_t max_new, max_kv;

@@ -381,3 +381,43 @@ def test_weights_between_others(gpu, what):
     torch.cuda.synchronize()
     assert torch.equal(both[:, 0], p.past[:, :room])
     p.check(gpu, out=both[:, 1].cpu().numpy().astype(np.float64))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("decay", [0.75, 1.0, 0.0])
+@pytest.mark.parametrize("max_new", [1, 5000])
+@pytest.mark.parametrize("what", ["decode ragged", "chunk", "prompt group 3", "more tokens than positions", "dims 256"])
+def test_weights_summed_over_layers(gpu, what, max_new, decay, in_place):
+    """continued: what was there counts for every entry, the newest among them, times decay; in place as beside it.  The
+    product and the sum are rounded once each at most: 2^-23 of either."""
+    _say("weights continued", what, max_new, decay, in_place)
+    p = test_gpu_weights.Problem("bfloat16", *test_gpu_weights.SHAPES[what], seed=34)
+    alone = p.run(gpu, past=False, max_new=max_new)
+    p.check(gpu, past=False, out=alone)
+    got = p.run(gpu, decay=decay, max_new=max_new, continued=True, in_place=in_place)
+    before = p.past.cpu().numpy().astype(np.float64)
+    for r, kv in enumerate(p.kv):
+        want = alone[r, :kv] + decay * before[r, :kv]
+        assert np.all(np.abs(got[r, :kv] - want) <= 2.0 ** -23 * (want + decay * before[r, :kv])), r
+        rest = before[r, kv:] if in_place else np.full(got.shape[1], 7.0)[kv:before.shape[1]]
+        assert np.array_equal(got[r, kv:before.shape[1]], rest)
+
+
+def test_a_step_of_layers_decays_once(gpu):
+    """Three layers as a step sums them: what older tokens had counts for decay of it, what each layer adds for all."""
+    import torch
+    _say("weights of a step's layers")
+    layers = [test_gpu_weights.Problem("bfloat16", *test_gpu_weights.SHAPES["chunk"], seed=s) for s in (43, 44, 45)]
+    decay, room = 0.5, layers[0].cols * 16
+    out = layers[0].past.clone()
+    for i, p in enumerate(layers):
+        gpu.paged_weights(p.q, p.kc, p.table, p.starts, p.kv_len, p.lse, out, d_past=out, decay=decay if i == 0 else 1.0,
+                          continued=i > 0, scale=p.scale)
+    torch.cuda.synchronize()
+    alone = [p.run(gpu, past=False) for p in layers]
+    before, got = layers[0].past.cpu().numpy().astype(np.float64), out.cpu().numpy().astype(np.float64)
+    for r, (n, kv) in enumerate(zip(layers[0].new, layers[0].kv)):
+        want = sum(a[r, :kv] for a in alone)
+        want[:kv - n] += decay * before[r, :kv - n]
+        assert np.all(np.abs(got[r, :kv] - want) <= 4 * 2.0 ** -24 * want)  # three sums and a product, rounded once each
+        assert np.array_equal(got[r, kv:room], before[r, kv:room])
