@@ -800,10 +800,12 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: Optional[st
 
     scaling, for contexts `factor` times as long: "linear" divides every frequency by it; "base" raises the base, so
     that the slowest pair is divided by it and the fastest stays; "parts" leaves the pairs that turn more than `fast`
-    times over the `original` positions, divides those that turn fewer than `slow` times, passes over evenly between
-    them, and lengthens the rows by a tenth of the factor's logarithm.  Worked out in 64 bits."""
+    times over the `original` positions, divides those that turn fewer than `slow` times, passes over evenly in their
+    turns between them, and lengthens the rows by a tenth of the factor's logarithm.  Worked out in 64 bits.  A model
+    that was trained with other frequencies (passing over evenly in the pairs' numbers, say) brings its own table."""
     import torch
-    if rotated < 0 or rotated % 2 or base <= 0 or factor <= 0 or scaling not in (None, "linear", "base", "parts"):
+    if rotated < 0 or rotated % 2 or base <= 0 or factor <= 0 or scaling not in (None, "linear", "base", "parts") or (
+            scaling == "parts" and not (fast > slow and original > 0)):
         raise CrError(CR_ERR_INVALID, f"rotary_frequencies: {rotated} dimensions, base {base}, scaling {scaling!r} by "
                                       f"{factor}")
     if scaling == "base" and rotated > 2:
