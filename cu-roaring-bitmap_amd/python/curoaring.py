@@ -904,6 +904,8 @@ def paged_evict(d_weights, d_kv_len, d_keep, d_table, page_size: int, d_weights_
     stream."""
     n, on = d_kv_len.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
+    if not (0 < page_size < 1 << 32 and (n_pages is None or 0 <= n_pages < 1 << 32)):
+        raise CrError(CR_ERR_INVALID, f"paged_evict: page size {page_size}, {n_pages} pages")
     room = cols * page_size
     weights, weights_stride = _matrix(d_weights, "weights", "float32", n, room, on)
     w_out, w_out_stride = _matrix(d_weights_out, "weights_out", "float32", n, room, on)
