@@ -84,6 +84,7 @@ def test_pinned_slots_of_the_first_pages_alone(gpu, kind, positions):
     assert np.array_equal(out[0, :m].cpu().numpy(), w[0][lies]) and p_out[0, :m].tolist() == [pos[i] for i in lies]
 
 
+@pytest.mark.filterwarnings("ignore:invalid value encountered")
 @pytest.mark.parametrize("density", [None, 0.8])
 @pytest.mark.parametrize("max_new", [1, 5000])
 @pytest.mark.parametrize("what", ["a few tokens", "chunk", "prompt group 3", "dims 192", "dims 256"])
