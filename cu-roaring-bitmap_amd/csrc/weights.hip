@@ -226,7 +226,7 @@ __global__ __launch_bounds__(WR_NT) void wt_rows(WeightArgs a)
                     for (uint32_t e = 0; e < 4; ++e) {
                         const uint32_t at_row = row0 + g * 4 + e, row = min(at_row, rows - 1);
                         const float z = a.lse[static_cast<uint64_t>(t.token0 + row / group) * a.heads + h * group + row % group];
-                        lse2[e] = z * LOG2E;
+                        lse2[e] = z * LOG2E;  // (rounded: 1.3e-6 of a weight at a log-sum of 32, less below it)
                         number[e] = at_row < rows && z != -__builtin_inff() ? at_row + 1 : 0u;
                     }
                     // the wave's own keys are in LDS
@@ -396,6 +396,8 @@ __global__ __launch_bounds__(WT_NT) __attribute__((amdgpu_waves_per_eu(DIM <= 12
             const bool none = z == -__builtin_inff();  // counts for nothing, whatever it holds
             const uint16_t* at = none ? wt_zeros : a.q + token * a.q_token + head * a.q_head;
             s_at[i % 4][lane] = reinterpret_cast<uint64_t>(at);
+            // (rounded: 1.3e-6 of a weight at a log-sum of 32, less below it; what the product loses, given back,
+            // would be an operation more for each exponential)
             s_lse[i % 4][lane] = none ? __builtin_inff() : z * LOG2E;
         };
         auto load = [&](uint32_t i, uint16_t* sq) __attribute__((always_inline)) {

@@ -506,7 +506,8 @@ int cr_paged_rotary(const cr_paged_rotary_args* args, const cr_paged_cache* cach
  * entries whose page is outside the cache.  d_past may be d_out, with the same stride, or NULL: nothing before.  Sums are in
  * fp32, in an order that depends on the arguments alone.  Entries behind d_kv_len[r]
  * are left as they were.  Types and alignment are those of cr_paged_attention;
- * cache->v is not looked at. */
+ * cache->v is not looked at.  Workspace: at most 512 MB of sums, lists of 12 B a part of rows
+ * and 4 B a request, and a bit a slot for a `visible` of other than bitmap containers. */
 typedef struct cr_paged_weights_args {
     const void* q; /* [n_tokens][n_heads][head_dim] */
     uint64_t q_token_stride, q_head_stride;
@@ -547,7 +548,8 @@ int cr_paged_weights(const cr_paged_weights_args* args, const cr_paged_cache* ca
  * d_weights_out[r][0, m) and d_positions_out[r][0, m) (NULL: not wanted) what then
  * lies there; those two may be the inputs themselves, with the same strides, the lengths may not.  A row of d_moves holds half as
  * many pairs as a row of the table has positions.  d_freed[0, freed_cap) receives the
- * pages that no entry of their request is in any more, requests in order, and
+ * pages that no entry of their request is in any more, requests in order and as their rows have them (one outside the
+ * cache too), and
  * d_counts[0, 2) their number and that of all moves.  The table stays as it is:
  * cr_paged_plan, with d_len for d_cached, writes over what is behind.  Pages that
  * several requests share have to be pinned, first in their rows and no more than
