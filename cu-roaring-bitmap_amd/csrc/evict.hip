@@ -1024,7 +1024,7 @@ extern "C" int cr_paged_evict(const cr_paged_evict_args* args, cr_stream_t strea
     // What the set can hold: slots behind are not pinned, and take no room where its bits are written out.
     uint64_t pin_end = n_slots;
     if (p.pinned && p.pinned->universe_size)
-        pin_end = std::min<uint64_t>(n_slots, (static_cast<uint64_t>(p.pinned->universe_size) + 65535) / 65536 * 65536);
+        pin_end = std::min(n_slots, (std::max<uint64_t>((p.pinned->universe_size - 1u) >> 16, p.pinned->max_key) + 1) << 16);
     const uint32_t n_words = static_cast<uint32_t>((pin_end + 31) / 32);
     Carver cv;
     const size_t o_keys = cv.add(segments * SG_SIZE * 4), o_open = cv.add(segments * SG_SIZE * 8);

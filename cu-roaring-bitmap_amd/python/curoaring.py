@@ -900,8 +900,7 @@ def paged_evict(d_weights, d_kv_len, d_keep, d_table, page_size: int, d_weights_
     d_kept[r] entries, as the last call left them; the others are the newest in order.  Written: d_weights_out and
     d_positions_out (the inputs themselves, if need be), d_len int32 [R], d_moves int32 [R, at least half of
     cols * page_size, 2], d_n_moves int32 [R], d_freed int32 [any], d_counts int32 [2]: pages freed and moves in all.
-    n_pages: the cache's (default: any).  Slots behind pinned's universe are not pinned.  stream: None is the null
-    stream."""
+    n_pages: the cache's (default: any, whatever pinned's universe).  stream: None is the null stream."""
     n, on = d_kv_len.numel(), _device()
     table, cols, stride = _table(d_table, n, on)
     if not (0 < page_size < 1 << 32 and (n_pages is None or 0 <= n_pages < 1 << 32)):

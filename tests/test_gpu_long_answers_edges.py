@@ -422,3 +422,42 @@ def test_a_step_of_layers_decays_once(gpu):
         want[:kv - n] += decay * before[r, :kv - n]
         assert np.all(np.abs(got[r, :kv] - want) <= 4 * 2.0 ** -24 * want)  # three sums and a product, rounded once each
         assert np.array_equal(got[r, kv:room], before[r, kv:room])
+
+
+@pytest.mark.parametrize("kind", ["bitmap", "array"])
+def test_pinned_slots_behind_the_universe_that_is_named(gpu, kind):
+    """Containers uploaded with a universe that ends before their last key: what they hold counts all the same."""
+    import torch
+    _say("evict, containers behind the universe", kind)
+    page, n_pages, kv, keep = 16, 9000, 480, 200
+    rng = np.random.default_rng(46)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    table = (4096 + rng.permutation(4000)[:30]).astype(np.int32)[None]  # slots of the second container
+    pinned = np.zeros(n_pages * page, bool)
+    slots = (table[0, ::3, None].astype(np.int64) * page + np.arange(0, page, 2)).reshape(-1)
+    pinned[slots] = True
+    low = np.sort(slots - 65536).astype(np.uint16)
+    if kind == "bitmap":
+        words = np.zeros(65536, np.uint8)
+        words[low] = 1
+        first, second = np.zeros(1024, np.uint64), np.packbits(words, bitorder="little").view(np.uint64)
+        first[0] = 1
+        containers = [(0, gpu.TC_BITSET, 1, first), (1, gpu.TC_BITSET, len(low), second)]
+    else:
+        containers = [(0, gpu.TC_ARRAY, 1, np.zeros(1, np.uint16)), (1, gpu.TC_ARRAY, len(low), low)]
+    g = gpu.upload_containers(containers, universe=1000, threshold=gpu.PROMOTE_KEEP_DEFAULT)
+    assert g.n_bitmap_containers == (2 if kind == "bitmap" else 0)
+    pinned[0] = True
+    w = rng.random((1, 480)).astype(np.float32)
+    one = lambda x: torch.tensor([x], **i32)  # noqa: E731
+    out, length, n_moves = torch.zeros(1, 480, device="cuda"), one(-9), one(-9)
+    moves, freed, counts = torch.full((1, 240, 2), -9, **i32), torch.full((30,), -9, **i32), torch.zeros(2, **i32)
+    gpu.paged_evict(cuda(w), one(kv), one(keep), cuda(table), page, out, length, moves, n_moves, freed, counts, sinks=2,
+                    recent=4, pinned=g, n_pages=n_pages)
+    torch.cuda.synchronize()
+    gpu.free(g)
+    m, lies, _, want, _ = test_gpu_evict.evict_oracle(w[0], w[0], 0, kv, kv, keep, table[0], page, n_pages, 2, 4, pinned)
+    assert int(length[0]) == m and int(n_moves[0]) == len(want) > 0
+    assert moves[0, :len(want)].tolist() == [list(x) for x in want]
+    assert np.array_equal(out[0, :m].cpu().numpy(), w[0][lies])
