@@ -81,9 +81,9 @@ inline WeightsWork weights_work(const WeightsShape& a)
     // average is taken for single tokens.
     w.mixed = uneven && !w.many && total > 2 * w.few && (a.max_new ? longest > 2 * w.few : counted > a.n_requests);
     // Parts of the rows: as many workgroups as fill the card a few times, no longer sums than 2048
-    // rows, and no parts of fewer than 256 where it can be helped, which end in more sums to be
-    // joined (32 requests of 100 tokens, group 3: 39 us, with parts of 64 or 128 rows 44; a prompt
-    // of 500 18, not 15).
+    // rows (in requests of the mean: a launch has as many parts of each), and no parts of fewer than
+    // 256 where it can be helped, which end in more sums to be joined (32 requests of 100 tokens,
+    // group 3: 39 us, with parts of 64 or 128 rows 44; a prompt of 500 18, not 15).
     const uint64_t even = total * w.tiles * a.kv_heads / (8ull * a.cus);
     w.part_rows = static_cast<uint32_t>(std::min<uint64_t>(2048, std::max<uint64_t>(256, even))) / 64 * 64;
     // A table may have room for far more positions than its requests hold, and a list for more parts than
